@@ -51,7 +51,7 @@ extern "C" {
 #define PU_DTYPE_BF16 0
 #define PU_DTYPE_F16 1
 #define PU_DTYPE_F32 2
-#define PU_DTYPE_FP8_E4M3 3   /* KV caches of pu_decode_gqa only */
+#define PU_DTYPE_FP8_E4M3 3   /* KV caches with grouped heads (pu_decode_gqa, pu_decode_paged_gqa) */
 
 /* Number of floats in one packed split-KV partial record: m, l, o[D]. */
 #define PU_PARTIAL_FLOATS(D) ((D) + 2)
@@ -320,6 +320,142 @@ PU_API int pu_decode_paged(const void* q, int q_dtype,
                            void* workspace, size_t workspace_bytes,
                            int64_t B, int64_t H, int64_t D,
                            float sm_scale, void* stream);
+
+/*
+ * Decode step over a paged cache with grouped K/V heads and optional fp8
+ * pools: pu_decode_gqa's step on the dense cache the pages describe.
+ * No counterpart in the reference (kernels/decoding.py:86-115).
+ *   q [B,H,1,D] f16/bf16; pools [num_pages][H_kv][page_size][D] with
+ *   H % H_kv == 0; kv_dtype PU_DTYPE_F16, PU_DTYPE_BF16 or
+ *   PU_DTYPE_FP8_E4M3, whose stored values times k_scale / v_scale are the
+ *   keys / values; D 64 or 128.  o bf16 [B,H,1,D]; lse fp32 [B,H] or NULL.
+ *   A sequence of length 0 gives o = 0 and lse = -inf.
+ * The work is shared evenly over the SMs whatever the lengths are.
+ *   workspace: pu_decode_paged_gqa_workspace_size() bytes, zeroed before its
+ *   first use (left zeroed, as for pu_decode).
+ */
+PU_API size_t pu_decode_paged_gqa_workspace_size(int64_t B, int64_t H, int64_t H_kv,
+                                                 int64_t max_pages_per_seq, int64_t page_size,
+                                                 int64_t D);
+
+PU_API int pu_decode_paged_gqa(const void* q, int q_dtype,
+                               const void* k_pool, const void* v_pool, int kv_dtype,
+                               const int32_t* page_table, int64_t max_pages_per_seq,
+                               int64_t num_pages, int64_t page_size,
+                               const int32_t* kv_lens, void* o, float* lse,
+                               void* workspace, size_t workspace_bytes,
+                               int64_t B, int64_t H, int64_t H_kv, int64_t D,
+                               float sm_scale, float k_scale, float v_scale, void* stream);
+
+/*
+ * Plan a batch's next tokens on the device: page table rows, slots and
+ * positions from lengths alone.  No counterpart in the reference.
+ *   page_table [B][max_pages_per_seq], kv_lens [B]: the state before;
+ *   new_lens int32 [B]: tokens each sequence gets now (negative: 0);
+ *   release: [B] bytes or NULL; where nonzero the sequence's pages go back
+ *     first and it starts empty.
+ *   free_ring int32 [num_pages], cursor int64 [2] = {head, tail}: the free
+ *     pages are free_ring[i % num_pages], head <= i < tail.  Pages are taken
+ *     at the head, in sequence order, and returned at the tail; those returned
+ *     in a call are handed out from the next call on.
+ * Results:
+ *   page_table_out, kv_lens_out, cursor_out: the state after.  Either all
+ *     three are the inputs themselves (advanced in place) or none is; a
+ *     separate table is written whole, -1 past each sequence's pages, while in
+ *     place only entries that change are written.
+ *   slots, positions, seq_ids int32 [num_tokens]: for row t of the packed
+ *     batch (the new tokens of sequence 0, then 1, ...) its place
+ *     page * page_size + row in a pool, its position and its sequence; -1, 0, -1
+ *     for rows behind the last token.
+ *   cu_new int32 [B+1]: first row of each sequence.
+ * A sequence whose tokens exceed its table row or the num_tokens rows, or for
+ * which the free pages do not last, is refused: it keeps its pages and length
+ * and its rows get slot -1.  pu_device_status then reports
+ * PU_ERR_INVALID_ARGUMENT, detail 307 (does not fit; also a kept page outside
+ * the pool), or PU_ERR_WORKSPACE, detail 308 (no free pages); a cursor that
+ * describes no ring of this size is PU_ERR_INVALID_ARGUMENT, detail 308.
+ * B <= 8192.
+ */
+PU_API int pu_page_plan(const int32_t* page_table, int32_t* page_table_out,
+                        int64_t max_pages_per_seq, const int32_t* kv_lens, int32_t* kv_lens_out,
+                        const int32_t* new_lens, const uint8_t* release,
+                        int32_t* free_ring, int64_t num_pages,
+                        const int64_t* cursor, int64_t* cursor_out, int64_t page_size,
+                        int32_t* slots, int32_t* positions, int32_t* seq_ids, int32_t* cu_new,
+                        int64_t B, int64_t num_tokens, void* stream);
+
+/*
+ * Norms of queries and keys for each head with the position rotation in the
+ * same pass.  No counterpart in the reference (its attention takes q, k, v as
+ * they are, src/pallas_flash/ops/interface.py:20-27).  For a row x of D values
+ * (one head of one token):
+ *   n = x / sqrt(mean(x^2) + eps) * weight      (no weight: n = x)
+ *   (a, b) -> (a cos t - b sin t, b cos t + a sin t),  t = position * inv_freq[p]
+ * for the pairs p < rotary_dim/2 of n: (p, p + rotary_dim/2), or with
+ * `interleaved` (2p, 2p+1); values behind rotary_dim are normed only.
+ * Computed in fp32 and rounded once; angles are exact to fp32 at any position.
+ *
+ * The description's fields are all 8 bytes wide.  Strides are in elements;
+ * the last dimension is dense.  Rows start on 16-byte boundaries.
+ *   dtype: PU_DTYPE_BF16, F16 or F32 of q, k, v and the outputs.
+ *   D: a multiple of 16 up to 128; rotary_dim: a multiple of 16 up to D.
+ *   inv_freq: [rotary_dim/2] fp64 (freq_is_f64 != 0) or fp32.
+ *   positions: int64 (pos_is_i64 != 0) or int32 with strides {axis, B, N}, or
+ *     NULL: the token's index.  axes 1..4; pairs [0, sections[0]) turn with
+ *     axis 0, the next sections[1] with axis 1, ...; the sections add up to
+ *     rotary_dim/2 (axes = 1: sections[0] = rotary_dim/2).
+ *   weights: [D] of their dtype, or NULL.
+ */
+typedef struct pu_qk_rope_desc {
+  int64_t B, N, H, H_kv, D, dtype;
+  int64_t rotary_dim, interleaved;
+  const void* inv_freq;
+  int64_t freq_is_f64;
+  const void* positions;
+  int64_t pos_is_i64, pos_stride[3];
+  int64_t axes, sections[4];
+  const void* q_weight;
+  int64_t q_weight_dtype;
+  const void* k_weight;
+  int64_t k_weight_dtype;
+  double eps;
+  int64_t q_stride[3], k_stride[3], v_stride[3];     /* {B, H, N} of the inputs */
+  int64_t gq_stride[3], gk_stride[3];                /* of the output gradients */
+  int64_t dq_stride[3], dk_stride[3];                /* of the input gradients */
+} pu_qk_rope_desc;
+
+/* Forward: q_out [B,H,N,D], k_out [B,H_kv,N,D] dense. */
+PU_API int pu_qk_norm_rope_fwd(const pu_qk_rope_desc* desc, const void* q, const void* k,
+                               void* q_out, void* k_out, void* stream);
+
+/* Bytes of workspace the weight gradients need (contents need not be initialised). */
+PU_API size_t pu_qk_norm_rope_bwd_workspace_size(int64_t D);
+
+/*
+ * Backward: dq, dk (either may be NULL) from the inputs and the output
+ * gradients gq, gk; dq_weight, dk_weight (NULL: not wanted) in the weights'
+ * dtypes.  No atomics: the same bits every time.  The workspace may be NULL
+ * without weight gradients.
+ */
+PU_API int pu_qk_norm_rope_bwd(const pu_qk_rope_desc* desc, const void* q, const void* k,
+                               const void* gq, const void* gk, void* dq, void* dk,
+                               void* dq_weight, void* dk_weight,
+                               void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Serving form for N packed tokens (B = 1; q [N,H,D], k and v [N,H_kv,D] by
+ * their strides): q_out dense [N,H,D]; the normed and rotated key and the
+ * value of token t go to row slots[t] % page_size of page slots[t] / page_size
+ * of the pools [num_pages][H_kv][page_size][D] (pool_dtype PU_DTYPE_F16, BF16
+ * or FP8_E4M3, divided by k_scale / v_scale and, e4m3, saturated).  A negative
+ * slot writes nothing (a padding row); one past the pool is reported
+ * (pu_device_status, PU_ERR_INVALID_ARGUMENT, detail 306) and writes nothing.
+ * No slot may occur twice.
+ */
+PU_API int pu_qk_norm_rope_append(const pu_qk_rope_desc* desc, const void* q, const void* k,
+                                  const void* v, void* q_out, const int32_t* slots,
+                                  void* k_pool, void* v_pool, int pool_dtype, int64_t num_pages,
+                                  int64_t page_size, float k_scale, float v_scale, void* stream);
 
 /*
  * Append one token per sequence to a paged cache: writes k_new/v_new

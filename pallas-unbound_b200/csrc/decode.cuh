@@ -635,11 +635,11 @@ int launch_kv(const Params& prm, int kv_dtype, dim3 grid, cudaStream_t st) {
     e = launch_pdl(split_kv_kernel<QT, __nv_bfloat16, DD, kFinal, kPaged, kPush>, grid, dim3(kThreads), 0, st, prm);
   } else {
     // fp8 caches are read by the single-GPU final-output step
-    if constexpr (kFinal && !kPaged && !kPush) {
+    if constexpr (kFinal && !kPush) {
       e = launch_pdl(split_kv_kernel<QT, __nv_fp8_e4m3, DD, kFinal, kPaged, kPush>, grid, dim3(kThreads), 0, st,
                      prm);
     } else {
-      return set_error(PU_ERR_UNSUPPORTED, "fp8 caches: single-GPU dense decode only");
+      return set_error(PU_ERR_UNSUPPORTED, "fp8 caches: single-GPU decode only");
     }
   }
   return check_cuda(e, "split-KV decode launch");

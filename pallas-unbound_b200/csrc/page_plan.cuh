@@ -1,0 +1,293 @@
+// page_plan.cuh — page table rows, slots and positions of a batch's next
+// tokens, from lengths alone, in one launch with no host in between.
+//
+// No counterpart in the reference (dense padded caches,
+// src/pallas_flash/kernels/decoding.py:86-103).  Per sequence b with held
+// length L_b (0 if it is released first), N_b new tokens and page size S:
+//   have_b = ceil(L_b / S), need_b = ceil((L_b + N_b) / S) - have_b
+//   its new pages are ring[head + sum_{b' < b} need_b' + i], i < need_b
+//   token i of the packed batch belongs to the b with start_b <= i < start_b
+//   + N_b (start = exclusive sum of N), has position L_b + i - start_b and
+//   slot page * S + row
+// Free pages wait in a ring: they are taken at its head and returned at its
+// tail, so the places read and the places written by one call never meet
+// (free + returned pages never exceed the ring), and pages of a sequence
+// that is released in this call are handed out from the next call on.
+//
+// Every CTA scans all B sequences itself (three block-wide sums in 64 bits;
+// a second kernel would cost more than the repeated reads of a few KB from
+// L2) and then takes its share of table rows and tokens.  Where the state is
+// advanced in place, the CTAs form one cluster of 8 and meet at its barrier
+// between the last read of the lengths and the first write; with separate
+// outputs nothing is shared and the grid grows with the work.
+#pragma once
+
+#include "paged.cuh"
+
+namespace pu {
+namespace plan {
+
+constexpr int kThreads = 1024;
+constexpr int kMaxB = 8192;
+constexpr int kCluster = 8;
+
+struct Params {
+  const int32_t* table;      // [B][max_pages]
+  int32_t* table_out;
+  const int32_t* lens;       // [B]
+  int32_t* lens_out;
+  const int32_t* add;        // [B] new tokens
+  const uint8_t* release;    // [B] or nullptr
+  int32_t* ring;             // [num_pages] free page numbers
+  const long long* cursor;   // head, tail (counts that only grow)
+  long long* cursor_out;
+  int32_t* slots;            // [T]
+  int32_t* positions;        // [T]
+  int32_t* seq_ids;          // [T]
+  int32_t* cu;               // [B + 1]
+  int B, max_pages, num_pages, page_shift;
+  long long T;
+};
+
+// Exclusive block-wide sum of one value per thread; *total = the sum of all.
+__device__ __forceinline__ long long block_scan(long long v, long long* s_warp, long long* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long x = v;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, x, off);
+    if (lane >= off) x += y;
+  }
+  __syncthreads();                       // the previous scan's sums have been read
+  if (lane == 31) s_warp[warp] = x;
+  __syncthreads();
+  if (warp == 0) {
+    long long w = s_warp[lane];
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, w, off);
+      if (lane >= off) w += y;
+    }
+    s_warp[lane] = w;
+  }
+  __syncthreads();
+  *total = s_warp[31];
+  return x - v + (warp > 0 ? s_warp[warp - 1] : 0);
+}
+
+template <bool kInPlace>
+__global__ void __launch_bounds__(kThreads) page_plan_kernel(const Params p) {
+  extern __shared__ int s_dyn[];
+  int* s_start = s_dyn;                  // [B + 1] first token (at most T)
+  int* s_base = s_start + p.B + 1;       // [B] tokens held before
+  int* s_last = s_base + p.B;            // [B] pages held after
+  int* s_new = s_last + p.B;             // [B] ring place of the first new page, from the head
+  int* s_freed = s_new + p.B;            // [B] ring place of the first returned page, from the tail; -1: none
+  __shared__ long long s_warp[32];
+  const int tid = threadIdx.x;
+  grid_dep_wait();
+  grid_dep_launch_dependents();
+
+  const int page = 1 << p.page_shift;
+  const long long cap = (long long)p.max_pages << p.page_shift;
+  const long long head = p.cursor[0], tail = p.cursor[1];
+  long long avail = tail - head;
+  const bool ring_ok = head >= 0 && avail >= 0 && avail <= p.num_pages;
+  if (!ring_ok) avail = 0;
+  const int head0 = ring_ok ? (int)(head % p.num_pages) : 0, tail0 = ring_ok ? (int)(tail % p.num_pages) : 0;
+
+  // this thread's sequences
+  const int per = (p.B + kThreads - 1) / kThreads, b0 = min(tid * per, p.B), b1 = min(b0 + per, p.B);
+  long long tokens = 0, freed = 0;
+  for (int b = b0; b < b1; ++b) {
+    const long long held = min((long long)max(p.lens[b], 0), cap);
+    const bool gone = p.release != nullptr && p.release[b] != 0;
+    s_base[b] = gone ? 0 : (int)held;
+    s_freed[b] = gone ? (int)((held + page - 1) >> p.page_shift) : 0;
+    tokens += max(p.add[b], 0);
+    freed += s_freed[b];
+  }
+  long long total_tokens, total_freed, total_need, total_used;
+  long long start = block_scan(tokens, s_warp, &total_tokens);
+  long long back = block_scan(freed, s_warp, &total_freed);
+  // what fits the table and the rows of the batch asks for pages
+  long long need = 0, at = start;
+  for (int b = b0; b < b1; ++b) {
+    const long long n = max(p.add[b], 0), base = s_base[b];
+    const int have = (int)((base + page - 1) >> p.page_shift);
+    const bool fits = base + n <= cap && at + n <= p.T;
+    if (!fits) record_device_error(PU_ERR_INVALID_ARGUMENT, kSitePagePlan);
+    s_start[b] = (int)min(at, p.T);
+    s_last[b] = fits ? (int)((base + n + page - 1) >> p.page_shift) : -1;
+    need += fits ? s_last[b] - have : 0;
+    at += n;
+  }
+  long long upto = block_scan(need, s_warp, &total_need);
+  // pages go to the sequences in order while they last
+  long long used = 0;
+  for (int b = b0; b < b1; ++b) {
+    const int have = (s_base[b] + page - 1) >> p.page_shift;
+    const int want = s_last[b] < 0 ? 0 : s_last[b] - have;
+    const bool served = s_last[b] >= 0 && (want == 0 || upto + want <= avail);
+    if (s_last[b] >= 0 && !served) record_device_error(PU_ERR_WORKSPACE, kSiteFreePages);
+    s_new[b] = served ? (int)min(upto, avail) : -1;        // -1: refused, the sequence stays as it is
+    if (!served) s_last[b] = have;
+    else used += want;
+    upto += want;
+  }
+  block_scan(used, s_warp, &total_used);
+  const bool give = ring_ok && avail + total_freed <= p.num_pages;
+  if (tid == 0 && blockIdx.x == 0 && (!ring_ok || !give)) record_device_error(PU_ERR_INVALID_ARGUMENT, kSiteFreePages);
+  for (int b = b0; b < b1; ++b) {
+    const int f = s_freed[b];
+    s_freed[b] = f > 0 && give ? (int)back : -1;
+    back += f;
+  }
+  if (tid == 0) s_start[p.B] = (int)min(total_tokens, p.T);
+  __syncthreads();
+
+  // rows: pages kept, pages taken, then none
+  const int warps = (int)gridDim.x * (kThreads / 32), wid = (int)blockIdx.x * (kThreads / 32) + (tid >> 5), lane = tid & 31;
+  auto taken = [&](int i) { int r = head0 + i; return p.ring[r >= p.num_pages ? r - p.num_pages : r]; };
+  // lengths held before (the pages a released row returns), read ahead of the barrier
+  constexpr int kSeg = 512;              // entries a warp takes at once
+  const int segs = (p.max_pages + kSeg - 1) / kSeg;
+  if constexpr (kInPlace) {
+    // only the released rows still need their old lengths: put them where the
+    // rows' owners find them before the lengths change
+    for (int b = tid; b < p.B; b += kThreads)
+      if (p.release != nullptr && p.release[b] != 0) {
+        const long long held = min((long long)max(p.lens[b], 0), cap);
+        s_base[b] = -(int)held - 1;      // base is 0 for a released sequence
+      }
+    __syncthreads();
+    cluster_sync();
+  }
+  auto base_of = [&](int b) { return kInPlace && s_base[b] < 0 ? 0 : s_base[b]; };
+  auto old_of = [&](int b) -> int {      // pages the row returns
+    if (p.release == nullptr || p.release[b] == 0) return 0;
+    const long long held = kInPlace ? -(long long)(s_base[b] + 1) : min((long long)max(p.lens[b], 0), cap);
+    return (int)((held + page - 1) >> p.page_shift);
+  };
+  for (long long u = wid; u < (long long)p.B * segs; u += warps) {
+    const int b = (int)(u / segs), lo = (int)(u % segs) * kSeg, hi = min(lo + kSeg, p.max_pages);
+    const int have = (base_of(b) + page - 1) >> p.page_shift, last = s_last[b], old = old_of(b), to = s_freed[b];
+    const int32_t* in = p.table + (size_t)b * p.max_pages;
+    int32_t* out = p.table_out + (size_t)b * p.max_pages;
+    // in place, the kept entries stay and those past both page counts are not touched
+    const int from = kInPlace ? max(lo, have) : lo, end = kInPlace ? min(hi, max(last, old)) : hi;
+    for (int j = from + lane; j < end; j += 32) {
+      if (j < old && to >= 0) {
+        int r = tail0 + to + j;
+        p.ring[r >= p.num_pages ? r - p.num_pages : r] = in[j];
+      }
+      out[j] = j < have ? in[j] : j < last ? taken(s_new[b] + j - have) : -1;
+    }
+  }
+  if (blockIdx.x == 0) {
+    for (int b = tid; b <= p.B; b += kThreads) {
+      p.cu[b] = s_start[b];
+      if (b < p.B) p.lens_out[b] = base_of(b) + (s_new[b] >= 0 ? max(p.add[b], 0) : 0);
+    }
+    if (tid == 0) {
+      p.cursor_out[0] = head + total_used;
+      p.cursor_out[1] = tail + (give ? total_freed : 0);
+    }
+  }
+  // tokens
+  const long long threads = (long long)gridDim.x * kThreads;
+  for (long long t = (long long)blockIdx.x * kThreads + tid; t < p.T; t += threads) {
+    int seq = -1, pos = 0, slot = -1;
+    if (t < s_start[p.B]) {
+      int a = 0, z = p.B;                // last b with start_b <= t
+      while (z - a > 1) {
+        const int m = (a + z) >> 1;
+        if (s_start[m] <= t) a = m;
+        else z = m;
+      }
+      const int base = base_of(a), have = (base + page - 1) >> p.page_shift;
+      seq = a;
+      pos = (int)min((long long)base + (t - s_start[a]), 2147483647ll);
+      if (s_new[a] >= 0) {
+        const int e = pos >> p.page_shift;
+        const int pg = e < have ? p.table[(size_t)a * p.max_pages + e] : taken(s_new[a] + e - have);
+        if ((unsigned)pg < (unsigned)p.num_pages) slot = (pg << p.page_shift) | (pos & (page - 1));
+        else record_device_error(PU_ERR_INVALID_ARGUMENT, kSitePagePlan);
+      }
+    }
+    p.slots[t] = slot;
+    p.positions[t] = pos;
+    p.seq_ids[t] = seq;
+  }
+}
+
+}  // namespace plan
+}  // namespace pu
+
+extern "C" int pu_page_plan(const int32_t* page_table, int32_t* page_table_out, int64_t max_pages_per_seq,
+                            const int32_t* kv_lens, int32_t* kv_lens_out, const int32_t* new_lens,
+                            const uint8_t* release, int32_t* free_ring, int64_t num_pages, const int64_t* cursor,
+                            int64_t* cursor_out, int64_t page_size, int32_t* slots, int32_t* positions,
+                            int32_t* seq_ids, int32_t* cu_new, int64_t B, int64_t num_tokens, void* stream) {
+  using namespace pu::plan;
+  if (!page_table || !page_table_out || !kv_lens || !kv_lens_out || !new_lens || !free_ring || !cursor || !cursor_out ||
+      !cu_new || (num_tokens > 0 && (!slots || !positions || !seq_ids)))
+    return pu::set_error(PU_ERR_INVALID_ARGUMENT, "page plan: null pointer");
+  if (B <= 0 || B > kMaxB) return pu::set_error(PU_ERR_UNSUPPORTED, "page plan: %lld sequences (1 to %d)", (long long)B, kMaxB);
+  if (num_tokens < 0 || num_tokens > 2147483647ll)
+    return pu::set_error(PU_ERR_UNSUPPORTED, "page plan: %lld tokens", (long long)num_tokens);
+  int shift = 0;
+  int rc = pu::paged::check_pool(num_pages, page_size, &shift);
+  if (rc) return rc;
+  if (max_pages_per_seq <= 0 || max_pages_per_seq > (1ll << 30) / page_size)
+    return pu::set_error(PU_ERR_UNSUPPORTED, "page plan: %lld pages per sequence", (long long)max_pages_per_seq);
+  Params p{};
+  p.table = page_table;
+  p.table_out = page_table_out;
+  p.lens = kv_lens;
+  p.lens_out = kv_lens_out;
+  p.add = new_lens;
+  p.release = release;
+  p.ring = free_ring;
+  p.cursor = reinterpret_cast<const long long*>(cursor);
+  p.cursor_out = reinterpret_cast<long long*>(cursor_out);
+  p.slots = slots;
+  p.positions = positions;
+  p.seq_ids = seq_ids;
+  p.cu = cu_new;
+  p.B = (int)B;
+  p.max_pages = (int)max_pages_per_seq;
+  p.num_pages = (int)num_pages;
+  p.page_shift = shift;
+  p.T = num_tokens;
+  const bool table_in = page_table == page_table_out, lens_in = kv_lens == kv_lens_out, cur_in = cursor == cursor_out;
+  if (table_in != lens_in || lens_in != cur_in)
+    return pu::set_error(PU_ERR_INVALID_ARGUMENT, "page plan: table, lengths and cursor are advanced in place together or not at all");
+  const int smem = (int)(5 * B + 1) * (int)sizeof(int);
+  const void* f = table_in ? reinterpret_cast<const void*>(page_plan_kernel<true>)
+                           : reinterpret_cast<const void*>(page_plan_kernel<false>);
+  rc = pu::set_max_dynamic_smem(f, (5 * kMaxB + 1) * (int)sizeof(int), "page plan shared memory");
+  if (rc) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (!table_in) {
+    // 4096 entries or tokens a CTA: below that its scan is most of its time
+    const long long work = B * max_pages_per_seq + num_tokens;
+    const long long grid = std::max<long long>(1, std::min<long long>((work + 4095) / 4096, pu::sm_count()));
+    return pu::check_cuda(pu::decode::launch_pdl(page_plan_kernel<false>, dim3((unsigned)grid), dim3(kThreads), smem, st, p),
+                          "page plan launch");
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(kCluster);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = kCluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return pu::check_cuda(cudaLaunchKernelEx(&cfg, page_plan_kernel<true>, p), "page plan launch");
+}

@@ -64,6 +64,16 @@ __global__ void __launch_bounds__(256) append_kernel(const T* __restrict__ k_new
   if (threadIdx.x == 0) lens[b] = pos + 1;
 }
 
+// Page count and size of a pool; *shift = log2(page size).
+inline int check_pool(long long num_pages, long long page_size, int* shift) {
+  if (num_pages <= 0) return set_error(PU_ERR_INVALID_ARGUMENT, "page counts must be positive");
+  const int s = log2_exact(page_size);
+  if (s < 4 || s > 12) return set_error(PU_ERR_UNSUPPORTED, "page size %lld (power of two in [16, 4096])", page_size);
+  if (num_pages > (1ll << 31) / page_size) return set_error(PU_ERR_UNSUPPORTED, "page pool too large");
+  *shift = s;
+  return PU_OK;
+}
+
 inline int check_pages(const int32_t* table, long long max_pages, long long num_pages, long long page_size,
                        int* shift) {
   if (!table) return set_error(PU_ERR_INVALID_ARGUMENT, "null page table");

@@ -1,0 +1,909 @@
+// paged_tc.cuh — attention of one new token over a paged cache with grouped
+// heads, on the tensor core: 16-bit caches of q's type with G = H / H_kv >= 2
+// (D = 64 or 128), e4m3 caches with any G (D = 128).
+//
+// No counterpart in the reference (dense caches, one K/V head per query head:
+// src/pallas_flash/kernels/decoding.py:86-115).  The products are those of
+// the dense grouped kernel, with the rows of a 128-token tile as the MMA's M
+// and up to 16 query heads as its N:
+//   S [128 rows x 16 heads] = K_tile Q^T,   O^T [D x 16 heads] += V_tile^T P^T
+// about 64 D flops per row of 4 D bytes: far below the ridge, so the kernel
+// is bound by reading the pages once.
+//
+// Work.  The tiles of all (sequence, K/V head, slice of 16 query heads) are
+// numbered in one line and cut into as many equal parts as there are CTAs
+// (one per SM), so a ragged batch keeps every SM equally busy whatever the
+// lengths, which the host does not know; a grid cut by the table's capacity
+// leaves most SMs idle when sequences are shorter than the table.  A part
+// may begin and end inside a sequence: such an end is written as a record
+// (m, l, o) and the last CTA of the sequence joins its records; a CTA has at
+// most two of them, so the workspace is a few MB whatever the batch.  No CTA
+// waits for another.
+//
+// Roles (352 threads):
+//   warps 0-7   two softmax groups; group t & 1 takes tile t, each with its
+//               own running maximum, sums and accumulator (row r of the tile
+//               = TMEM lane r = thread r; at the end of a segment both add
+//               up).  One group alone left the tensor core and the loads
+//               waiting on e4m3 tiles, whose softmax takes longer than their
+//               bytes.
+//   warp 8      page table lookups and TMA loads, lane i page box i
+//   warp 9      tcgen05 issue, S and P V products as each becomes ready
+//   warp 10     queries of the next segments into shared memory (e4m3: scaled
+//               by a power of two and split into parts)
+// K/V tiles run through one ring across segments, so a new sequence's first
+// pages are on their way while the previous one ends.
+//
+// e4m3: K and V tiles are operands as stored; q and P are split into e4m3
+// parts stacked along N: q into two parts if bf16 (8 significant bits are
+// two e4m3 parts exactly) and three if f16 (11 bits), P into three.
+//
+// Pages.  Only pages that hold tokens of the sequence are read.  An entry
+// outside the pool is not followed: it is reported (detail 302) and its
+// tokens are left out.  Rows past the length and rows not loaded are masked,
+// and their V rows are zeroed in shared memory, so stale values never count.
+#pragma once
+
+#include "gqa_tc.cuh"
+
+namespace pu {
+namespace decode {
+namespace ptc {
+
+using tc::to16;
+
+constexpr int BT = 128;                    // cache rows per tile (MMA M)
+constexpr int NP = 16;                     // query heads per slice (MMA N per part)
+constexpr int kGroups = 2;                 // softmax groups of 128 threads
+constexpr int kSoftmax = kGroups * 128;
+constexpr int kLoadWarp = 8, kMmaWarp = 9, kQueryWarp = 10;
+constexpr int kCtaThreads = 352;
+constexpr int kQSlots = 4;
+constexpr int kHead = 4;                   // floats before o in a record: m, l, and two that keep o 16-byte aligned
+
+template <typename T, typename KVT, int D>
+struct Cfg {
+  static constexpr bool kF8 = sizeof(KVT) == 1;
+  static constexpr int kQParts = !kF8 ? 1 : std::is_same<T, __nv_bfloat16>::value ? 2 : 3;
+  static constexpr int kPParts = kF8 ? 3 : 1;
+  // P = 2^(s - m) with m = the running maximum - kShift; m moves (and the
+  // accumulator is rescaled) once a score passes the maximum by kRescale, so
+  // P <= 2^(kShift + kRescale), near the top of its type: a long tail of
+  // small weights then stays above the type's smallest step (f16 2^-24, three
+  // e4m3 parts 2^-19; bf16 has fp32's range and needs no shift).
+  static constexpr float kRescale = kF8 ? 2.f : 8.f;
+  static constexpr float kShift = kF8 ? 6.f : std::is_same<T, __nv_bfloat16>::value ? 0.f : 7.f;
+  static constexpr int kRowBytes = D * (int)sizeof(KVT);
+  static constexpr int kBlocks = kRowBytes / 128;          // 128-byte swizzle blocks of a tile
+  static_assert(kRowBytes % 128 == 0, "rows are whole swizzle blocks");
+  static constexpr int kTile = BT * kRowBytes;
+  static constexpr int NS = kTile == 32768 ? 3 : kF8 ? 5 : 6;   // ring stages: 160 to 192 KB in flight
+  static constexpr int kQBlock = NP * 128;                 // one swizzle block of one part of q or P
+  static constexpr int kQBytes = (kF8 ? kQParts : kBlocks) * kQBlock;
+  static constexpr int kPBytes = (kF8 ? kPParts : 2) * kQBlock;   // 16 heads x 128 rows
+  static constexpr int kOffKV = 0;                         // stage: V, then K
+  static constexpr int kOffQ = NS * 2 * kTile;
+  static constexpr int kOffP = kOffQ + kQSlots * kQBytes;
+  static constexpr int kOffBar = kOffP + kGroups * kPBytes;
+  // full[NS], empty[NS], qfull[4], qfree[4], sfull[4], pfull[2], pvdone[2], ofree, drain
+  static constexpr int kBars = 2 * NS + 2 * kQSlots + 4 + 2 * kGroups + 2;
+  static constexpr int kOffMisc = kOffBar + kBars * 8;     // tmem base, abort flag, last-CTA flag
+  static constexpr int kOffBad = kOffMisc + 16;            // [NS] boxes of the stage that were not loaded
+  static constexpr int kOffMax = kOffBad + 32;             // [2 groups][4 warps][NP] tile maxima
+  static constexpr int kOffM = kOffMax + kGroups * 4 * NP * 4;   // [2 parities][2 groups][NP]
+  static constexpr int kOffL = kOffM + 2 * kGroups * NP * 4;     // [2 parities][2 groups][4 warps][NP]
+  static constexpr int kOffQinv = kOffL + 2 * kGroups * 4 * NP * 4;   // [4 slots][NP]
+  static constexpr int kSmem = kOffQinv + kQSlots * NP * 4;
+  static constexpr int kSCols = kQParts * NP, kOCols = kPParts * NP;
+  static constexpr int kColO = 4 * kSCols;                 // four S buffers, then an accumulator per group
+  static constexpr int kCols = kColO + kGroups * kOCols;
+  static constexpr uint32_t kTmemCols = kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
+  static_assert(kSmem <= 232448, "shared memory of one CTA");
+};
+
+struct Params {
+  const void* q;               // [B, H, D]
+  const int32_t* table;        // [B][max_pages]
+  const int32_t* lens;         // [B]
+  __nv_bfloat16* o;            // [B, H, D]
+  float* lse;                  // [B, H] or nullptr
+  int* count;                  // [CTAs] zero between calls
+  float* rec;                  // [CTAs][2][NP][D + kHead]
+  int B, H, H_kv, group, slices;
+  int max_pages, num_pages, page_shift;
+  int box;                     // rows of one TMA box: min(page size, 128)
+  float scale_log2, o_scale;
+};
+
+// x as N e4m3 parts, x ~ sum_i part_i / kPartScale^i: each part is the e4m3
+// rounding of what the ones before left, times kPartScale when `scaled` (a
+// remainder of a value up to 256 is at most 8, so 32 keeps it below 256).
+constexpr float kPartScale = 32.f;
+
+template <bool scaled, int N>
+__device__ __forceinline__ void split_e4m3(float a, float b, uint16_t (&part)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const __nv_fp8x2_storage_t h2 = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+    part[i] = (uint16_t)h2;
+    if (i + 1 < N) {
+      const float2 hf = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(h2, __NV_E4M3)));
+      a = (a - hf.x) * (scaled ? kPartScale : 1.f);
+      b = (b - hf.y) * (scaled ? kPartScale : 1.f);
+    }
+  }
+}
+
+// The tiles of this CTA in order.  An item is (sequence b, inner index r =
+// K/V head * slices + slice); a segment is the CTA's run of one item's tiles.
+struct Walk {
+  const Params* p;
+  int b, r, t, tiles, inner, left, seg, loc;
+  __device__ __forceinline__ int len_of(int i) const {
+    const int n = p->lens[i], cap = p->max_pages << p->page_shift;
+    return n < 0 ? 0 : n > cap ? cap : n;
+  }
+  __device__ __forceinline__ int tiles_of(int i) const { return (len_of(i) + BT - 1) / BT; }
+  // is the current tile the last of its segment?
+  __device__ __forceinline__ bool last() const { return left == 1 || t + 1 == tiles; }
+  // to the next tile, or over all n tiles of the segment
+  __device__ __forceinline__ void next(int n = 1) {
+    left -= n;
+    t += n;
+    loc += n;
+    if (left == 0 || t < tiles) return;
+    t = loc = 0;
+    ++seg;
+    if (++r < inner) return;
+    r = 0;
+    do tiles = tiles_of(++b);
+    while (tiles == 0);
+  }
+};
+
+// Sum of the warp's 16 values per lane over its 32 lanes: lanes 2 h and 2 h + 1
+// return head h's sum (each step halves the values a lane still holds).
+__device__ __forceinline__ float sum16(const float (&v)[NP], int lane) {
+  float a[8], b[4], c[2], d;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float keep = lane & 16 ? v[i + 8] : v[i], give = lane & 16 ? v[i] : v[i + 8];
+    a[i] = keep + __shfl_xor_sync(0xffffffffu, give, 16);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float keep = lane & 8 ? a[i + 4] : a[i], give = lane & 8 ? a[i] : a[i + 4];
+    b[i] = keep + __shfl_xor_sync(0xffffffffu, give, 8);
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float keep = lane & 4 ? b[i + 2] : b[i], give = lane & 4 ? b[i] : b[i + 2];
+    c[i] = keep + __shfl_xor_sync(0xffffffffu, give, 4);
+  }
+  d = (lane & 2 ? c[1] : c[0]) + __shfl_xor_sync(0xffffffffu, lane & 2 ? c[0] : c[1], 2);
+  return d + __shfl_xor_sync(0xffffffffu, d, 1);
+}
+
+template <typename T, typename KVT, int D>
+__global__ void __launch_bounds__(kCtaThreads, 1)
+    paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                    const __grid_constant__ Params p) {
+  using C = Cfg<T, KVT, D>;
+  constexpr int NS = C::NS, kQParts = C::kQParts, kPParts = C::kPParts, kTile = C::kTile;
+  constexpr bool kF8 = C::kF8;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (smem_u32(smem) & 1023u) {
+    if (tid == 0) record_device_error(PU_ERR_UNSUPPORTED, kSiteDecodeTc);
+    return;
+  }
+  uint8_t* sKV = smem + C::kOffKV;
+  uint8_t* sQ = smem + C::kOffQ;
+  uint8_t* sP = smem + C::kOffP;
+  uint64_t* bFull = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
+  uint64_t* bEmpty = bFull + NS;
+  uint64_t* bQfull = bEmpty + NS;        // [4] queries of segment s in slot s & 3
+  uint64_t* bQfree = bQfull + kQSlots;   // [4] its products (and scales, e4m3) have been read
+  uint64_t* bSf = bQfree + kQSlots;      // [4] S of tile t in buffer t & 3
+  uint64_t* bPf = bSf + 4;               // [2] P of the group's tile written (128 arrivals)
+  uint64_t* bPv = bPf + kGroups;         // [2] the group's P V product done
+  uint64_t* bOfree = bPv + kGroups;      // both accumulators of a segment read (256 arrivals)
+  uint64_t* bDrain = bOfree + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kOffMisc + 4);
+  int* s_last = reinterpret_cast<int*>(smem + C::kOffMisc + 8);
+  volatile uint32_t* s_bad = reinterpret_cast<volatile uint32_t*>(smem + C::kOffBad);
+  float* s_max = reinterpret_cast<float*>(smem + C::kOffMax);
+  float* s_m = reinterpret_cast<float*>(smem + C::kOffM);
+  float* s_l = reinterpret_cast<float*>(smem + C::kOffL);
+  float* s_qinv = reinterpret_cast<float*>(smem + C::kOffQinv);
+
+  if (tid == 0) {
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(bFull + s, 1);
+      mbar_init(bEmpty + s, 1);
+    }
+    for (int s = 0; s < kQSlots; ++s) {
+      mbar_init(bQfull + s, 32);
+      mbar_init(bQfree + s, kF8 ? 1 + kGroups : 1);
+      mbar_init(bSf + s, 1);
+    }
+    for (int g = 0; g < kGroups; ++g) {
+      mbar_init(bPf + g, 128);
+      mbar_init(bPv + g, 1);
+    }
+    mbar_init(bOfree, kSoftmax);
+    mbar_init(bDrain, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(tmem_slot, C::kTmemCols);
+    tmem_relinquish();
+  }
+  if (warp == kLoadWarp && lane == 0) {
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
+  grid_dep_wait();
+  grid_dep_launch_dependents();
+
+  // Where this CTA's tiles begin: every warp finds it for itself (two passes
+  // over the lengths, which stay in L1).
+  Walk w0;
+  w0.p = &p;
+  w0.inner = p.H_kv * p.slices;
+  long long all = 0;
+  for (int i = lane; i < p.B; i += 32) all += w0.tiles_of(i);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) all += __shfl_xor_sync(0xffffffffu, all, off);
+  all *= w0.inner;
+  // no part is empty, so every CTA between an item's first and last has a record
+  const long long ctas = min((long long)gridDim.x, all);
+  const bool busy = blockIdx.x < ctas;
+  const long long first = busy ? blockIdx.x * all / ctas : 0;
+  w0.left = busy ? (int)((blockIdx.x + 1ll) * all / ctas - first) : 0;
+  w0.b = w0.r = w0.t = w0.tiles = w0.seg = w0.loc = 0;
+  long long item0 = 0;                   // number of the current sequence's first tile
+  if (w0.left > 0) {
+    long long before = 0;
+    for (int i0 = 0;; i0 += 32) {
+      const int n = i0 + lane < p.B ? w0.tiles_of(i0 + lane) : 0;
+      long long x = n;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, x, off);
+        if (lane >= off) x += y;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, (before + x) * w0.inner > first);
+      if (hit) {
+        const int src = __ffs(hit) - 1;
+        w0.b = i0 + src;
+        w0.tiles = __shfl_sync(0xffffffffu, n, src);
+        item0 = (before + __shfl_sync(0xffffffffu, x, src) - w0.tiles) * w0.inner;
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, x, 31);
+    }
+    w0.r = (int)((first - item0) / w0.tiles);
+    w0.t = (int)((first - item0) % w0.tiles);
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == kLoadWarp) {
+    // ---------------- pages -> ring ----------------
+    const int boxes = BT / p.box, per_page = 1 << p.page_shift;
+    int n = 0;
+    for (Walk w = w0; w.left > 0; w.next(), ++n) {
+      const int s = n % NS, len = w.len_of(w.b);
+      const int row = w.t * BT + lane * p.box;
+      const bool mine = lane < boxes && row < len;
+      int pg = 0;
+      if (mine) pg = p.table[(size_t)w.b * p.max_pages + (row >> p.page_shift)];
+      const bool good = mine && (unsigned)pg < (unsigned)p.num_pages;
+      if (mine && !good) record_device_error(PU_ERR_INVALID_ARGUMENT, kSiteDecodePage);
+      const unsigned loaded = __ballot_sync(0xffffffffu, good);
+      if (n >= NS && !mbar_wait(bEmpty + s, (n / NS - 1) & 1, abort_flag, kSiteDecodeTc)) break;
+      __syncwarp();
+      uint8_t* dV = sKV + s * 2 * kTile + lane * p.box * 128;
+      uint8_t* dK = dV + kTile;
+      if (lane == 0) {
+        s_bad[s] = ~loaded;
+        mbar_arrive_expect_tx(bFull + s, (uint32_t)__popc(loaded) * 2 * p.box * C::kRowBytes);
+      }
+      __syncwarp();
+      if (good) {
+        const int outer = pg * p.H_kv + w.r / p.slices, in = row & (per_page - 1);
+        constexpr int cols = kF8 ? 128 : 64;
+#pragma unroll
+        for (int cb = 0; cb < C::kBlocks; ++cb) tma_load_3d(dK + cb * BT * 128, &tmK, bFull + s, cb * cols, in, outer);
+#pragma unroll
+        for (int cb = 0; cb < C::kBlocks; ++cb) tma_load_3d(dV + cb * BT * 128, &tmV, bFull + s, cb * cols, in, outer);
+      }
+      __syncwarp();
+    }
+    // copies still in flight land before the CTA may exit (after an abort the
+    // ring may stop anywhere: the last NS issued tiles are the ones in flight)
+    volatile int no_abort = 0;
+    for (int i = max(0, n - NS); i < n; ++i) mbar_wait(bFull + i % NS, (i / NS) & 1, &no_abort, kSiteDecodeTc);
+  } else if (warp == kQueryWarp) {
+    // ---------------- queries -> shared memory ----------------
+    int done = -1;                         // last segment staged
+    for (Walk w = w0; w.left > 0; w.next()) {
+      if (w.seg == done) continue;
+      done = w.seg;
+      const int slot = w.seg & (kQSlots - 1);
+      if (w.seg >= kQSlots && !mbar_wait(bQfree + slot, (w.seg / kQSlots - 1) & 1, abort_flag, kSiteDecodeTc)) break;
+      __syncwarp();
+      const int slice = w.r % p.slices, heads = min(NP, p.group - slice * NP);
+      const T* q = static_cast<const T*>(p.q) + ((size_t)w.b * p.H + (w.r / p.slices) * p.group + slice * NP) * D;
+      uint8_t* dst = sQ + slot * C::kQBytes;
+      constexpr int kVecs = D / 8;         // 16-byte vectors of a row
+      uint4 v[NP * kVecs / 32];
+#pragma unroll
+      for (int i = 0; i < NP * kVecs / 32; ++i) {
+        const int h = (i * 32 + lane) / kVecs, c = (i * 32 + lane) % kVecs;
+        v[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (h < heads) v[i] = *reinterpret_cast<const uint4*>(q + (size_t)h * D + c * 8);
+      }
+#pragma unroll
+      for (int i = 0; i < NP * kVecs / 32; ++i) {
+        const int h = (i * 32 + lane) / kVecs, c = (i * 32 + lane) % kVecs;
+        if constexpr (!kF8) {
+          *reinterpret_cast<uint4*>(dst + (c >> 3) * C::kQBlock + h * 128 + (((c & 7) ^ (h & 7)) << 4)) = v[i];
+        } else {
+          // scaled by a power of two so that the head's largest |q| lies in
+          // [128, 256), then split; 16 lanes hold a head
+          float x[8];
+          unpack8<T>(v[i], x);
+          float mx = 0.f;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) mx = fmaxf(mx, fabsf(x[k]));
+#pragma unroll
+          for (int off = 8; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+          const int e = (mx > 0.f && isfinite(mx)) ? ((__float_as_int(mx) >> 23) & 0xff) - 127 : 7;
+          const int sh = max(-100, min(100, 7 - e));
+          const float up = __int_as_float((127 + sh) << 23), down = __int_as_float((127 - sh) << 23);
+          uint32_t wd[kQParts][2];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            uint16_t pr[kQParts];
+            split_e4m3<false>(x[2 * k] * up, x[2 * k + 1] * up, pr);
+#pragma unroll
+            for (int j = 0; j < kQParts; ++j)
+              wd[j][k >> 1] = (k & 1) ? (wd[j][k >> 1] | ((uint32_t)pr[j] << 16)) : (uint32_t)pr[j];
+          }
+          const int at = h * 128 + (((c >> 1) ^ (h & 7)) << 4) + (c & 1) * 8;
+#pragma unroll
+          for (int j = 0; j < kQParts; ++j)
+            *reinterpret_cast<uint2*>(dst + j * C::kQBlock + at) = make_uint2(wd[j][0], wd[j][1]);
+          // a head that is not finite makes its scores NaN, as it would in 16 bits
+          if (c == 0) s_qinv[slot * NP + h] = isfinite(mx) ? down : mx - mx;
+        }
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(bQfull + slot);
+    }
+  } else if (warp == kMmaWarp) {
+    // ---------------- tcgen05 issuer ----------------
+    if (lane == 0) {
+      constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+      constexpr uint32_t idS = kF8 ? make_idesc_e4m3(BT, C::kSCols, 0, 0) : make_idesc_16(BT, NP, 0, 0, kBf16);
+      constexpr uint32_t idO = kF8 ? make_idesc_e4m3(128, C::kOCols, 1, 0) : make_idesc_16(128, NP, 1, 0, kBf16);
+      const uint64_t dQ0 = make_sdesc_sw128(smem_u32(sQ), 16, 1024);
+      const uint64_t dP0 = make_sdesc_sw128(smem_u32(sP), 16, 1024);
+      // D = 64: M is still 128, with the K tile's 64 columns behind V's as
+      // the other half; its rows of the accumulator are never read
+      const uint64_t dV0 = make_sdesc_sw128(smem_u32(sKV), D == 64 ? kTile : BT * 128, 1024);
+      const uint64_t dK0 = make_sdesc_sw128(smem_u32(sKV + kTile), 16, 1024);
+      Walk ws = w0, wp = w0;
+      int js = 0, jp = 0;                  // next S product, next P V product
+      uint64_t t_last = global_timer_ns();
+      while (wp.left > 0) {
+        bool progressed = false;
+        // S of tile js overwrites the buffer of tile js - 4, read once that
+        // tile's P was written, so once its P V product was issued
+        if (ws.left > 0 && js < jp + 4 && mbar_try_wait(smem_u32(bFull + js % NS), (js / NS) & 1) &&
+            (ws.loc > 0 || mbar_try_wait(smem_u32(bQfull + (ws.seg & 3)), (ws.seg >> 2) & 1))) {
+          tc_fence_after();
+          const uint64_t dk = sdesc_add(dK0, (js % NS) * 2 * kTile), dq = sdesc_add(dQ0, (ws.seg & 3) * C::kQBytes);
+          const uint32_t col = tmem + (js & 3) * C::kSCols;
+          if constexpr (kF8) {
+#pragma unroll
+            for (int kk = 0; kk < D / 32; ++kk) mma_ss_f8(col, sdesc_add(dk, kk * 32), sdesc_add(dq, kk * 32), idS, kk > 0);
+          } else {
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk)
+              mma_ss(col, sdesc_add(dk, (kk >> 2) * (BT * 128) + (kk & 3) * 32),
+                     sdesc_add(dq, (kk >> 2) * C::kQBlock + (kk & 3) * 32), idS, kk > 0);
+          }
+          mma_commit(bSf + (js & 3));
+          if (ws.last()) mma_commit(bQfree + (ws.seg & 3));
+          ws.next();
+          ++js;
+          progressed = true;
+        }
+        if (jp < js && mbar_try_wait(smem_u32(bPf + (jp & 1)), (jp >> 1) & 1) &&
+            (wp.loc > 0 || wp.seg == 0 || mbar_try_wait(smem_u32(bOfree), (wp.seg - 1) & 1))) {
+          tc_fence_after();
+          const uint64_t dv = sdesc_add(dV0, (jp % NS) * 2 * kTile), dp = sdesc_add(dP0, (jp & 1) * C::kPBytes);
+          const uint32_t col = tmem + C::kColO + (jp & 1) * C::kOCols;
+          const bool more = wp.loc >= kGroups;   // the group's accumulator already holds tiles of this segment
+          if constexpr (kF8) {
+#pragma unroll
+            for (int kk = 0; kk < BT / 32; ++kk)
+              mma_ss_f8(col, sdesc_add(dv, kk * 32 * 128), sdesc_add(dp, kk * 32), idO, more || kk > 0);
+          } else {
+#pragma unroll
+            for (int kk = 0; kk < BT / 16; ++kk)
+              mma_ss(col, sdesc_add(dv, kk * 16 * 128), sdesc_add(dp, (kk >> 2) * C::kQBlock + (kk & 3) * 32), idO,
+                     more || kk > 0);
+          }
+          mma_commit(bPv + (jp & 1));
+          mma_commit(bEmpty + jp % NS);
+          wp.next();
+          ++jp;
+          progressed = true;
+        }
+        if (progressed) {
+          t_last = global_timer_ns();
+        } else {
+          if (*abort_flag) break;
+          if (global_timer_ns() - t_last > kWaitTimeoutNs) {
+            *abort_flag = 1;
+            record_device_error(PU_ERR_DEVICE_TIMEOUT, kSiteDecodeTc);
+            break;
+          }
+        }
+      }
+      // every issued product completes before TMEM and shared memory go away
+      mma_commit(bDrain);
+      volatile int no_abort = 0;
+      mbar_wait(bDrain, 0, &no_abort, kSiteDecodeTc);
+    }
+  } else {
+    // ---------------- softmax groups ----------------
+    const int grp = warp >> 2, row = tid & 127, w4 = warp & 3;
+    const uint32_t lane_base = static_cast<uint32_t>(w4 * 32) << 16;
+    float* gmax = s_max + grp * 4 * NP;
+    uint8_t* myP = sP + grp * C::kPBytes;
+    const int box_shift = 31 - __clz(p.box);
+    int t = 0, mine = 0;                   // tiles of the CTA so far, of this group
+    Walk w = w0;
+    while (w.left > 0) {
+      // ---- one segment ----
+      const int seg = w.seg, b = w.b, r = w.r, t0 = w.t, tiles = w.tiles;
+      const int n = min(w.left, tiles - t0), len = w.len_of(b);
+      const int slice = r % p.slices, G = min(NP, p.group - slice * NP);
+      float qf = p.scale_log2, qs[NP];     // e4m3: a factor per head undoes the query's scale
+      if constexpr (kF8) {
+        const int slot = seg & 3;
+        mbar_wait(bQfull + slot, (seg >> 2) & 1, abort_flag, kSiteDecodeTc);
+#pragma unroll
+        for (int h = 0; h < NP; ++h) qs[h] = s_qinv[slot * NP + h] * p.scale_log2;
+        bar_sync_named(1 + grp, 128);
+        if (row == 0) mbar_arrive(bQfree + slot);
+      }
+      float m[NP], l[NP];
+#pragma unroll
+      for (int h = 0; h < NP; ++h) {
+        m[h] = -INFINITY;
+        l[h] = 0.f;
+      }
+      for (int i = 0; i < n; ++i, ++t) {
+        if ((t & 1) != grp) continue;
+        const int stage = t % NS, buf = t & 3;
+        mbar_wait(bSf + buf, (t >> 2) & 1, abort_flag, kSiteDecodeTc);
+        mbar_wait(bFull + stage, (t / NS) & 1, abort_flag, kSiteDecodeTc);
+        __syncwarp();
+        tc_fence_after();
+        const bool valid = (t0 + i) * BT + row < len && !((s_bad[stage] >> (row >> box_shift)) & 1u);
+        float s[NP];
+        {
+          uint32_t raw[kQParts][NP];
+#pragma unroll
+          for (int k = 0; k < kQParts; ++k) tmem_ld16(tmem + lane_base + buf * C::kSCols + k * NP, raw[k]);
+          tmem_wait_ld();
+#pragma unroll
+          for (int k = 0; k < kQParts; ++k) reg_fence(raw[k]);
+#pragma unroll
+          for (int h = 0; h < NP; ++h) {
+            float x = __uint_as_float(raw[0][h]);
+            if constexpr (kQParts > 1) x += __uint_as_float(raw[1][h]);
+            if constexpr (kQParts > 2) x += __uint_as_float(raw[2][h]);
+            s[h] = valid ? x * (kF8 ? qs[h] : qf) : -INFINITY;
+          }
+        }
+        bool up = false;
+#pragma unroll
+        for (int h = 0; h < NP; ++h)
+          if (h < G) up |= s[h] > m[h] + (C::kShift + C::kRescale);
+        if (bar_any_named(1 + grp, 128, up)) {
+          // the tile's maximum of each head over its 128 rows
+#pragma unroll
+          for (int h = 0; h < NP; ++h) {
+            if (h >= G) break;
+            float v = s[h];
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
+            if (lane == 0) gmax[w4 * NP + h] = v;
+          }
+          bar_sync_named(1 + grp, 128);
+          float alpha[NP];
+#pragma unroll
+          for (int h = 0; h < NP; ++h) {
+            alpha[h] = 1.f;
+            if (h >= G) continue;
+            const float tm = fmaxf(fmaxf(gmax[h], gmax[NP + h]), fmaxf(gmax[2 * NP + h], gmax[3 * NP + h]));
+            if (tm > m[h] + (C::kShift + C::kRescale)) {   // the same decision in every thread of the group
+              alpha[h] = m[h] == -INFINITY ? 0.f : ex2(m[h] - (tm - C::kShift));
+              m[h] = tm - C::kShift;
+            }
+            l[h] *= alpha[h];
+          }
+          if (i >= kGroups) {              // the accumulator holds earlier tiles of this segment
+            mbar_wait(bPv + grp, (mine - 1) & 1, abort_flag, kSiteDecodeTc);
+            __syncwarp();
+            tc_fence_after();
+#pragma unroll
+            for (int k = 0; k < kPParts; ++k) {
+              uint32_t ov[NP];
+              const uint32_t at = tmem + lane_base + C::kColO + grp * C::kOCols + k * NP;
+              tmem_ld16(at, ov);
+              tmem_wait_ld();
+              reg_fence(ov);
+#pragma unroll
+              for (int h = 0; h < NP; ++h) ov[h] = __float_as_uint(__uint_as_float(ov[h]) * alpha[h]);
+              tmem_st16(at, ov);
+            }
+            tmem_wait_st();
+          }
+        }
+        if (!valid) {
+          // rows past the length or not loaded: zero V, so that P = 0 times them is 0
+          uint8_t* vrow = sKV + stage * 2 * kTile + row * 128;
+#pragma unroll
+          for (int cb = 0; cb < C::kBlocks; ++cb)
+#pragma unroll
+            for (int c = 0; c < 8; ++c) reinterpret_cast<uint4*>(vrow + cb * BT * 128)[c] = make_uint4(0u, 0u, 0u, 0u);
+        }
+        // the group's previous P V product has read its P
+        if (mine > 0) mbar_wait(bPv + grp, (mine - 1) & 1, abort_flag, kSiteDecodeTc);
+        if constexpr (kF8) {
+          uint8_t* pb = myP + (row & 15);
+          const int chunk = row >> 4;
+#pragma unroll
+          for (int h = 0; h < NP; h += 2) {
+            if (h >= G) break;
+            const float p0 = s[h] == -INFINITY ? 0.f : ex2(s[h] - m[h]);
+            const float p1 = h + 1 >= G || s[h + 1] == -INFINITY ? 0.f : ex2(s[h + 1] - m[h + 1]);
+            l[h] += p0;
+            l[h + 1] += p1;
+            uint16_t pr[kPParts];
+            split_e4m3<true>(p0, p1, pr);
+            const int o0 = h * 128 + ((chunk ^ (h & 7)) << 4), o1 = (h + 1) * 128 + ((chunk ^ ((h + 1) & 7)) << 4);
+#pragma unroll
+            for (int k = 0; k < kPParts; ++k) {
+              pb[k * C::kQBlock + o0] = (uint8_t)(pr[k] & 0xff);
+              pb[k * C::kQBlock + o1] = (uint8_t)(pr[k] >> 8);
+            }
+          }
+        } else {
+          // row `row` of P: block row / 64, 16-byte chunk (row / 8) & 7
+          uint8_t* pb = myP + (row >> 6) * C::kQBlock + (row & 7) * 2;
+          const int chunk = (row >> 3) & 7;
+#pragma unroll
+          for (int h = 0; h < NP; ++h) {
+            if (h >= G) break;
+            const float pr = s[h] == -INFINITY ? 0.f : ex2(s[h] - m[h]);
+            l[h] += pr;
+            *reinterpret_cast<uint16_t*>(pb + h * 128 + ((chunk ^ (h & 7)) << 4)) = to16<T>(pr);
+          }
+        }
+        fence_proxy_async_smem();
+        tc_fence_before();
+        mbar_arrive(bPf + grp);
+        ++mine;
+        __syncwarp();
+      }
+
+      // ---- the segment's sums, both groups together ----
+      const int par = seg & 1;
+      float* pm = s_m + par * kGroups * NP;
+      float* pl = s_l + par * kGroups * 4 * NP;
+      const float ls = sum16(l, lane);
+      if ((lane & 1) == 0) pl[(grp * 4 + w4) * NP + (lane >> 1)] = ls;
+      if (row == 0) {
+#pragma unroll
+        for (int h = 0; h < NP; ++h) pm[grp * NP + h] = m[h];
+      }
+      // which groups have an accumulator for this segment: group g iff one of
+      // the tiles t - n .. t - 1 has parity g
+      const bool have0 = n > 1 || ((t - n) & 1) == 0, have1 = n > 1 || ((t - n) & 1) == 1;
+      if (mine > 0) mbar_wait(bPv + grp, (mine - 1) & 1, abort_flag, kSiteDecodeTc);
+      tc_fence_before();
+      bar_sync_named(3, kSoftmax);         // the other group's products are done too
+      tc_fence_after();
+      // group g finishes heads 8 g .. 8 g + 7; thread `row` holds column row of o
+      constexpr int kHalf = NP / 2;
+      const int h0 = grp * kHalf;
+      float oa[kHalf];
+#pragma unroll
+      for (int h = 0; h < kHalf; ++h) oa[h] = 0.f;
+      float M[kHalf], L[kHalf];
+#pragma unroll
+      for (int h = 0; h < kHalf; ++h) {
+        const float m0 = pm[h0 + h], m1 = pm[NP + h0 + h];
+        M[h] = fmaxf(m0, m1);
+        L[h] = 0.f;
+      }
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+        if (!(g ? have1 : have0)) continue;
+        float a[kHalf];
+#pragma unroll
+        for (int h = 0; h < kHalf; ++h) {
+          const float mg = pm[g * NP + h0 + h];
+          a[h] = mg == -INFINITY ? 0.f : ex2(mg - M[h]);
+          const float* x = pl + g * 4 * NP + h0 + h;
+          L[h] = fmaf(a[h], (x[0] + x[NP]) + (x[2 * NP] + x[3 * NP]), L[h]);
+        }
+        float wk = 1.f;
+#pragma unroll
+        for (int k = 0; k < kPParts; ++k, wk *= 1.f / kPartScale) {
+          uint32_t ov[kHalf];
+          tmem_ld8(tmem + lane_base + C::kColO + g * C::kOCols + k * NP + h0, ov);
+          tmem_wait_ld();
+          reg_fence(ov);
+#pragma unroll
+          for (int h = 0; h < kHalf; ++h) oa[h] = fmaf(__uint_as_float(ov[h]) * wk, a[h], oa[h]);
+        }
+      }
+      tc_fence_before();
+      mbar_arrive(bOfree);
+
+      // ---- result or record ----
+      // number of the item's first tile, and the CTAs that hold its tiles
+      const long long i0 = item0 + (long long)r * tiles, i1 = i0 + tiles;
+      const long long c0 = ((i0 + 1) * ctas - 1) / all, c1 = (i1 * ctas - 1) / all;
+      const size_t bh0 = (size_t)b * p.H + (size_t)(r / p.slices) * p.group + slice * NP;
+      if (c0 == c1) {
+#pragma unroll
+        for (int h = 0; h < kHalf; ++h) {
+          if (h0 + h >= G) break;
+          const float inv = L[h] == 0.f ? 0.f : p.o_scale / L[h];
+          if (row < D) p.o[(bh0 + h0 + h) * D + row] = __float2bfloat16_rn(oa[h] * inv);
+          if (row == 0 && p.lse != nullptr) p.lse[bh0 + h0 + h] = L[h] == 0.f ? -INFINITY : (M[h] + lg2(L[h])) * kLn2;
+        }
+      } else {
+        // this CTA's record: 0 where the item is the first of its part, else 1
+        const int which = seg == 0 ? 0 : 1;
+        float* rec = p.rec + ((size_t)blockIdx.x * 2 + which) * NP * (D + kHead);
+#pragma unroll
+        for (int h = 0; h < kHalf; ++h) {
+          if (h0 + h >= G) break;
+          float* x = rec + (h0 + h) * (D + kHead);
+          if (row < D) __stcg(x + kHead + row, oa[h] * p.o_scale);
+          if (row == 0) __stcg(reinterpret_cast<float2*>(x), make_float2(M[h], L[h]));
+        }
+        bar_sync_named(3, kSoftmax);
+        if (tid == 0) {
+          // the barrier orders every thread's record before this fence
+          __threadfence();
+          *s_last = atomicAdd(p.count + c0, 1) == (int)(c1 - c0);
+        }
+        bar_sync_named(3, kSoftmax);
+        if (*s_last) {
+          __threadfence();
+          // the last CTA of the item joins its records: a warp per head, lane
+          // i the i-th record's weight and columns 4 i .. 4 i + 3
+          const int nrec = (int)(c1 - c0) + 1;
+          // the first CTA's record is its second unless the item begins its part
+          const int w_first = c0 * all / ctas < i0 ? 1 : 0;
+          for (int h = warp; h < G; h += kSoftmax / 32) {
+            float Mx = -INFINITY, Ls = 0.f, o4[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int base = 0; base < nrec; base += 32) {
+              const int k = base + lane;
+              float2 ml = make_float2(-INFINITY, 0.f);
+              if (k < nrec)
+                ml = __ldcg(reinterpret_cast<const float2*>(
+                    p.rec + (((size_t)(c0 + k) * 2 + (k == 0 ? w_first : 0)) * NP + h) * (D + kHead)));
+              float bm = fmaxf(ml.x, Mx);
+#pragma unroll
+              for (int off = 16; off > 0; off >>= 1) bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, off));
+              const float keep = Mx == -INFINITY ? 0.f : ex2(Mx - bm);
+              const float wt = ml.x == -INFINITY ? 0.f : ex2(ml.x - bm);
+              float lw = wt * ml.y;
+#pragma unroll
+              for (int off = 16; off > 0; off >>= 1) lw += __shfl_xor_sync(0xffffffffu, lw, off);
+              Ls = fmaf(Ls, keep, lw);
+              Mx = bm;
+#pragma unroll
+              for (int c = 0; c < 4; ++c) o4[c] *= keep;
+              const int many = min(32, nrec - base);
+              constexpr int kAhead = 8;
+              for (int k0 = 0; k0 < many; k0 += kAhead) {
+                float4 x[kAhead];
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) {
+                  x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                  const int kk = base + k0 + u;
+                  if (k0 + u < many && lane * 4 < D)
+                    x[u] = __ldcg(reinterpret_cast<const float4*>(
+                        p.rec + (((size_t)(c0 + kk) * 2 + (kk == 0 ? w_first : 0)) * NP + h) * (D + kHead) + kHead) + lane);
+                }
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) {
+                  const float wu = __shfl_sync(0xffffffffu, wt, (k0 + u) & 31);
+                  if (k0 + u < many) {
+                    o4[0] = fmaf(wu, x[u].x, o4[0]);
+                    o4[1] = fmaf(wu, x[u].y, o4[1]);
+                    o4[2] = fmaf(wu, x[u].z, o4[2]);
+                    o4[3] = fmaf(wu, x[u].w, o4[3]);
+                  }
+                }
+              }
+            }
+            const float inv = Ls == 0.f ? 0.f : 1.f / Ls;
+            if (lane * 4 < D) {
+              uint2 out;
+              out.x = pack_bf16x2(o4[0] * inv, o4[1] * inv);
+              out.y = pack_bf16x2(o4[2] * inv, o4[3] * inv);
+              reinterpret_cast<uint2*>(p.o + (bh0 + h) * D)[lane] = out;
+            }
+            if (lane == 0 && p.lse != nullptr) p.lse[bh0 + h] = Ls == 0.f ? -INFINITY : (Mx + lg2(Ls)) * kLn2;
+          }
+          if (tid == 0) p.count[c0] = 0;     // left zeroed for the next call
+        }
+      }
+      // on to the next segment; a new sequence begins behind this one's items
+      w.next(n);
+      if (w.left > 0 && w.b != b) item0 += (long long)w.inner * tiles;
+    }
+    // sequences that hold nothing
+    for (int b = blockIdx.x; b < p.B; b += (int)gridDim.x) {
+      if (w0.len_of(b) > 0) continue;
+      for (int i = tid; i < p.H * D / 2; i += kSoftmax)
+        reinterpret_cast<uint32_t*>(p.o + (size_t)b * p.H * D)[i] = 0u;
+      if (p.lse != nullptr)
+        for (int i = tid; i < p.H; i += kSoftmax) p.lse[(size_t)b * p.H + i] = -INFINITY;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::kTmemCols);
+  }
+}
+
+inline bool eligible(long long H, long long H_kv, long long D, int q_dtype, int kv_dtype) {
+  if (q_dtype != PU_DTYPE_F16 && q_dtype != PU_DTYPE_BF16) return false;
+  if (kv_dtype == PU_DTYPE_FP8_E4M3) return D == 128;
+  return (D == 64 || D == 128) && q_dtype == kv_dtype && H / H_kv >= 2;
+}
+
+inline size_t workspace_bytes(long long D) {
+  return kCountBytes + round_up((size_t)sm_count() * 2 * NP * (D + kHead) * sizeof(float), 256);
+}
+
+template <typename T, typename KVT, int D>
+int launch_as(const CUtensorMap& tk, const CUtensorMap& tv, const Params& prm, cudaStream_t st) {
+  constexpr int smem = Cfg<T, KVT, D>::kSmem;
+  const int rc = set_max_dynamic_smem(reinterpret_cast<const void*>(paged_tc_kernel<T, KVT, D>), smem,
+                                      "paged grouped-head decode shared memory");
+  if (rc) return rc;
+  return check_cuda(launch_pdl(paged_tc_kernel<T, KVT, D>, dim3((unsigned)sm_count()), dim3(kCtaThreads), smem, st, tk, tv, prm),
+                    "paged grouped-head decode launch");
+}
+
+inline int launch(const Params& prm, const void* k, const void* v, int q_dtype, int kv_dtype, int D, cudaStream_t st) {
+  const bool f8 = kv_dtype == PU_DTYPE_FP8_E4M3;
+  const uint64_t rows = 1ull << prm.page_shift, outer = (uint64_t)prm.num_pages * prm.H_kv;
+  CUtensorMap tk, tv;
+  int rc = f8 ? make_tmap_u8_3d(&tk, k, D, rows, outer, 128, prm.box, true)
+              : make_tmap_bf16_3d(&tk, k, D, rows, outer, 64, prm.box, true);
+  if (!rc)
+    rc = f8 ? make_tmap_u8_3d(&tv, v, D, rows, outer, 128, prm.box, true)
+            : make_tmap_bf16_3d(&tv, v, D, rows, outer, 64, prm.box, true);
+  if (rc) return rc;
+  const bool h = q_dtype == PU_DTYPE_F16;
+  if (f8)
+    return h ? launch_as<__half, __nv_fp8_e4m3, 128>(tk, tv, prm, st)
+             : launch_as<__nv_bfloat16, __nv_fp8_e4m3, 128>(tk, tv, prm, st);
+  if (D == 128)
+    return h ? launch_as<__half, __half, 128>(tk, tv, prm, st) : launch_as<__nv_bfloat16, __nv_bfloat16, 128>(tk, tv, prm, st);
+  return h ? launch_as<__half, __half, 64>(tk, tv, prm, st) : launch_as<__nv_bfloat16, __nv_bfloat16, 64>(tk, tv, prm, st);
+}
+
+}  // namespace ptc
+}  // namespace decode
+}  // namespace pu
+
+extern "C" {
+
+size_t pu_decode_paged_gqa_workspace_size(int64_t B, int64_t H, int64_t H_kv, int64_t max_pages_per_seq,
+                                          int64_t page_size, int64_t D) {
+  using namespace pu::decode;
+  if (B <= 0 || H <= 0 || H_kv <= 0 || H % H_kv || max_pages_per_seq <= 0 || page_size <= 0 || D <= 0) return 0;
+  return std::max(ptc::workspace_bytes(D), pu_decode_paged_workspace_size(B, H, max_pages_per_seq, page_size, D));
+}
+
+int pu_decode_paged_gqa(const void* q, int q_dtype, const void* k_pool, const void* v_pool, int kv_dtype,
+                        const int32_t* page_table, int64_t max_pages_per_seq, int64_t num_pages, int64_t page_size,
+                        const int32_t* kv_lens, void* o, float* lse, void* workspace, size_t workspace_bytes, int64_t B,
+                        int64_t H, int64_t H_kv, int64_t D, float sm_scale, float k_scale, float v_scale, void* stream) {
+  using namespace pu::decode;
+  int shift = 0;
+  int rc = pu::paged::check_pages(page_table, max_pages_per_seq, num_pages, page_size, &shift);
+  if (rc) return rc;
+  const long long n_cap = max_pages_per_seq * page_size;
+  rc = check_args(q, q_dtype, k_pool, v_pool, kv_dtype, B, H, n_cap, D, true);
+  if (rc) return rc;
+  if (!o || !kv_lens) return pu::set_error(PU_ERR_INVALID_ARGUMENT, "null output or lengths");
+  if (H_kv <= 0 || H % H_kv != 0)
+    return pu::set_error(PU_ERR_INVALID_ARGUMENT, "H = %lld is not a multiple of H_kv = %lld", (long long)H, (long long)H_kv);
+  if (num_pages > 2147483647ll / H_kv) return pu::set_error(PU_ERR_UNSUPPORTED, "page pool too large");
+  if (!(k_scale > 0.f) || !(v_scale > 0.f) || !isfinite(k_scale) || !isfinite(v_scale))
+    return pu::set_error(PU_ERR_INVALID_ARGUMENT, "k_scale and v_scale must be positive and finite");
+  const bool tensor = ptc::eligible(H, H_kv, D, q_dtype, kv_dtype);
+  const Plan pl = make_plan(B * H, n_cap, D, pu::sm_count(), true, page_size);
+  const size_t need = tensor ? ptc::workspace_bytes(D) : pl.total_bytes;
+  if (!workspace || workspace_bytes < need)
+    return pu::set_error(PU_ERR_WORKSPACE, "paged decode workspace needs %zu bytes, got %zu", need, workspace_bytes);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const float scale_log2 = sm_scale * k_scale * kLog2e;
+  if (tensor) {
+    ptc::Params prm{};
+    prm.q = q;
+    prm.table = page_table;
+    prm.lens = kv_lens;
+    prm.o = static_cast<__nv_bfloat16*>(o);
+    prm.lse = lse;
+    prm.count = static_cast<int*>(workspace);
+    prm.rec = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCountBytes);
+    prm.B = (int)B;
+    prm.H = (int)H;
+    prm.H_kv = (int)H_kv;
+    prm.group = (int)(H / H_kv);
+    prm.slices = (prm.group + ptc::NP - 1) / ptc::NP;
+    prm.max_pages = (int)max_pages_per_seq;
+    prm.num_pages = (int)num_pages;
+    prm.page_shift = shift;
+    prm.box = (int)std::min<long long>(page_size, ptc::BT);
+    prm.scale_log2 = scale_log2;
+    prm.o_scale = v_scale;
+    return ptc::launch(prm, k_pool, v_pool, q_dtype, kv_dtype, (int)D, st);
+  }
+  // q and cache of different 16-bit types, one query head per K/V head, and
+  // e4m3 caches with D = 64: the query-head kernel reading K/V head h / G
+  Params prm{};
+  prm.q = q;
+  prm.k = k_pool;
+  prm.v = v_pool;
+  prm.lens = kv_lens;
+  prm.kv_offset = 0;
+  prm.n_local = (int)n_cap;
+  prm.H = (int)H;
+  prm.group = (int)(H / H_kv);
+  prm.o_scale = v_scale;
+  prm.splits = pl.splits;
+  prm.chunk = pl.chunk;
+  prm.scale_log2 = scale_log2;
+  prm.ws_rec = reinterpret_cast<float*>(static_cast<char*>(workspace) + pl.rec_off);
+  prm.ws_count = static_cast<int*>(workspace);
+  prm.o = static_cast<__nv_bfloat16*>(o);
+  prm.lse = lse;
+  prm.page_table = page_table;
+  prm.max_pages = (int)max_pages_per_seq;
+  prm.num_pages = (int)num_pages;
+  prm.page_shift = shift;
+  return launch<true, true>(prm, q_dtype, kv_dtype, (int)D, (int)(B * H), st);
+}
+
+}  // extern "C"

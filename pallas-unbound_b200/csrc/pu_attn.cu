@@ -5,6 +5,9 @@
 #include "decode.cuh"
 #include "paged.cuh"
 #include "gqa_tc.cuh"
+#include "paged_tc.cuh"
+#include "page_plan.cuh"
+#include "rope.cuh"
 #include "peer.cuh"
 #include "outproj.cuh"
 #include "attn_fwd.cuh"

@@ -41,6 +41,9 @@ enum WaitSite : int {
   kSiteAppendPage = 303,
   kSiteDecodePeer = 304,
   kSiteDecodeTc = 305,
+  kSiteAppendSlot = 306,
+  kSitePagePlan = 307,
+  kSiteFreePages = 308,
   kSiteOutProj = 401,
   kSiteSelfTest = 901,
 };

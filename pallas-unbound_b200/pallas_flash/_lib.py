@@ -11,6 +11,8 @@ import os
 import threading
 from pathlib import Path
 
+import torch
+
 PU_OK = 0
 PU_ERR_INVALID_ARGUMENT = 1
 PU_ERR_UNSUPPORTED = 2
@@ -91,6 +93,18 @@ SIGNATURES = {
     "pu_comm_init": (_int, [_c_void_p, _i64, _i64, ctypes.POINTER(_c_void_p)]),
     "pu_allgather_partials": (_int, [_c_void_p, _c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p]),
     "pu_comm_destroy": (_int, [_c_void_p]),
+    "pu_decode_paged_gqa_workspace_size": (_size_t, [_i64, _i64, _i64, _i64, _i64, _i64]),
+    "pu_decode_paged_gqa": (_int, [_c_void_p, _int, _c_void_p, _c_void_p, _int, _c_void_p, _i64,
+                                   _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _size_t,
+                                   _i64, _i64, _i64, _i64, _float, _float, _float, _c_void_p]),
+    "pu_page_plan": (_int, [_c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
+                            _c_void_p, _i64, _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p,
+                            _c_void_p, _c_void_p, _i64, _i64, _c_void_p]),
+    # the description (pu_qk_rope_desc) is passed as packed bytes
+    "pu_qk_norm_rope_fwd": (_int, [_c_void_p] * 6),
+    "pu_qk_norm_rope_bwd_workspace_size": (_size_t, [_i64]),
+    "pu_qk_norm_rope_bwd": (_int, [_c_void_p] * 10 + [_size_t, _c_void_p]),
+    "pu_qk_norm_rope_append": (_int, [_c_void_p] * 8 + [_int, _i64, _i64, _float, _float, _c_void_p]),
     "pu_kv_append": (_int, [_c_void_p, _c_void_p, _int, _c_void_p, _c_void_p, _c_void_p, _i64,
                             _i64, _i64, _c_void_p, _i64, _i64, _i64, _c_void_p]),
 }
@@ -136,6 +150,27 @@ def check(code: int, where: str) -> None:
     if code != PU_OK:
         msg = lib().pu_last_error()
         raise PuError(code, where, msg.decode() if msg else "")
+
+
+class on_device:
+    """Makes `device` current where it is not and gives the handle of its
+    current stream: `with on_device(t.device) as stream`."""
+
+    __slots__ = ("device", "before")
+
+    def __init__(self, device: torch.device):
+        self.device = device
+
+    def __enter__(self) -> int:
+        now = torch.cuda.current_device()
+        self.before = None if now == self.device.index else now
+        if self.before is not None:
+            torch.cuda.set_device(self.device)
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    def __exit__(self, *exc) -> None:
+        if self.before is not None:
+            torch.cuda.set_device(self.before)
 
 
 def device_status() -> tuple[int, int]:

@@ -36,7 +36,8 @@ Keyword-only additions:
   k_scale, v_scale  per-tensor scales of an fp8 (torch.float8_e4m3fn) cache:
               keys / values are the stored values times the scale
   page_table  int32 [B, max_pages_per_seq]: the caches are then page pools
-              [num_pages, H, page_size, D] (see kernels/paged.py) and
+              [num_pages, H_kv, page_size, D] (see kernels/paged.py; H_kv
+              divides H, fp16, bf16 or fp8 with k_scale / v_scale) and
               kv_lens is required; single GPU only.
 """
 from __future__ import annotations
@@ -61,11 +62,19 @@ class DecodeWorkspace:
     (device, stream).  The kernels leave it zeroed after each call, so one
     workspace must not be shared by decode calls that overlap on the GPU."""
 
+    _COUNTERS = 256 * 1024     # the part that must start zeroed
     _cache: dict = {}
     _lock = threading.Lock()
 
     @classmethod
     def get(cls, device: torch.device, nbytes: int) -> torch.Tensor:
+        if torch.cuda.is_current_stream_capturing():
+            # a captured call owns its scratch: two graphs captured on one
+            # stream may run at the same time, and a larger call may replace
+            # the cached buffer while a graph still points at it
+            buf = torch.empty(max(nbytes, cls._COUNTERS), dtype=torch.uint8, device=device)
+            buf[:cls._COUNTERS].zero_()
+            return buf
         stream = torch.cuda.current_stream(device).cuda_stream
         key = (device.index, stream)
         with cls._lock:
@@ -130,7 +139,7 @@ def pallas_flash_decoding(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
         if group is not None or kv_lens is None:
             raise ValueError("a paged cache needs kv_lens and runs on one GPU (group=None)")
         return paged_decode(q, k_cache, v_cache, page_table, kv_lens, sm_scale=sm_scale,
-                            return_lse=return_lse)
+                            return_lse=return_lse, k_scale=k_scale, v_scale=v_scale)
     if q.dim() != 4 or q.shape[2] != 1:
         raise ValueError("q must be [B, H, 1, D]")
     if k_cache.shape != v_cache.shape or k_cache.shape[0] != q.shape[0] \

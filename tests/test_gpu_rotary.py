@@ -1,0 +1,394 @@
+"""Norm and rotation of queries and keys (pu_qk_norm_rope_fwd, _bwd) against
+the formula in 64 bits.
+
+Tolerances, element by element.  A result is rounded once to its type (half a
+step: eps/2 of the value) after fp32 work: the sum of D squares is a chain of
+at most 16 + 3 roundings of positive terms (halved by the root), the root 2
+ulp, and about 14 more for the products, the sine and cosine (2 ulp) and the
+angle (2^-25 of half a turn): under 32 roundings of 2^-24 of the pair's
+magnitude |a| + |b|.  The gradient adds a dot product (19 roundings of the sum
+of magnitudes) and four products: 48 roundings of its terms' magnitudes.  A
+weight gradient sums rows one after the other: rows/8 + 64 roundings of the
+sum of magnitudes cover the longest chain of these shapes.
+"""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from helpers import assert_close_grad, assert_close_o, to_np
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def rot(built_lib):
+    if not torch.cuda.is_available():
+        pytest.fail("CUDA device required for -m gpu tests")
+    from pallas_flash import _lib
+    from pallas_flash.ops import rotary
+    _lib.device_status()
+    return rotary
+
+
+def _gen(shape, seed, dtype=torch.float32, scale=1.0):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return (torch.randn(shape, device="cuda", generator=g) * scale).to(dtype)
+
+
+def _turns(f, pos, sections, B, N):
+    """cos, sin fp64 [B, 1, N, R/2]."""
+    f = f.double()
+    if pos is None:
+        pos = torch.arange(N, device="cuda")
+    if sections is None:
+        t = pos.double().expand(B, N).unsqueeze(-1) * f
+    else:
+        parts, at = [], 0
+        for a, n in enumerate(sections):
+            parts.append(pos[a].double().expand(B, N).unsqueeze(-1) * f[at:at + n])
+            at += n
+        t = torch.cat(parts, -1)
+    return t.cos().unsqueeze(1), t.sin().unsqueeze(1)
+
+
+def _pairs(n, R, inter):
+    return (n[..., 0:R:2], n[..., 1:R:2]) if inter else (n[..., :R // 2], n[..., R // 2:R])
+
+
+def _join(a, b, rest, inter):
+    y = torch.stack((a, b), -1).flatten(-2) if inter else torch.cat((a, b), -1)
+    return torch.cat((y, rest), -1)
+
+
+def _oracle(x, w, cos, sin, inter, eps):
+    """(result, magnitude |a| + |b| of each value's pair) in 64 bits."""
+    x = x.double()
+    R = 2 * cos.shape[-1]
+    n = x if w is None else x / (x.square().mean(-1, keepdim=True) + eps).sqrt() * w.double()
+    a, b = _pairs(n, R, inter)
+    y = _join(a * cos - b * sin, b * cos + a * sin, n[..., R:], inter)
+    m = a.abs() + b.abs()
+    return y, _join(m, m, n[..., R:].abs(), inter)
+
+
+def _oracle_back(x, w, g, cos, sin, inter, eps):
+    """(dx, magnitude of its terms, dw, magnitude of its terms) in 64 bits."""
+    x, g = x.double(), g.double()
+    R, D = 2 * cos.shape[-1], x.shape[-1]
+    a, b = _pairs(g, R, inter)
+    h = _join(a * cos + b * sin, b * cos - a * sin, g[..., R:], inter)
+    m = _join(a.abs() + b.abs(), a.abs() + b.abs(), g[..., R:].abs(), inter)
+    if w is None:
+        return h, m, None, None
+    w = w.double()
+    r = 1 / (x.square().mean(-1, keepdim=True) + eps).sqrt()
+    dx = r * (h * w - x * r * r * (h * w * x).mean(-1, keepdim=True))
+    dxm = r * (m * w.abs() + x.abs() * r * r * (m * w.abs() * x.abs()).mean(-1, keepdim=True))
+    return dx, dxm, (h * x * r).sum((0, 1, 2)), (m * x.abs() * r).sum((0, 1, 2))
+
+
+def _close(got, want, mag, steps, what):
+    half = torch.finfo(got.dtype).eps / 2
+    # a result below the type's smallest normal value is off by up to half its smallest step
+    tiny = torch.finfo(got.dtype).tiny * torch.finfo(got.dtype).eps
+    tol = half * want.abs() + steps * U * mag + tiny
+    err = (got.double() - want).abs()
+    bad = err > tol
+    assert not bad.any(), f"{what}: {int(bad.sum())} off, worst {float((err / tol).max()):.2f} of the tolerance"
+
+
+CASES = [
+    # B, N, H, H_kv, D, R, dtype, weights, interleaved, sections
+    (2, 33, 4, 2, 128, 128, torch.bfloat16, torch.float32, False, None),
+    (1, 1, 1, 1, 64, 64, torch.float16, torch.float16, False, None),
+    (3, 17, 5, 3, 96, 32, torch.float32, torch.float32, True, None),
+    (2, 129, 7, 1, 80, 80, torch.bfloat16, torch.bfloat16, True, None),
+    (1, 1000, 32, 8, 128, 64, torch.float16, torch.bfloat16, False, None),
+    (2, 50, 16, 2, 64, 64, torch.bfloat16, torch.float32, False, (8, 12, 12)),
+    (2, 31, 3, 2, 128, 96, torch.float32, torch.float32, True, (16, 0, 20, 12)),
+    (1, 5, 9, 9, 16, 16, torch.float32, torch.float32, False, (8,)),
+    (2, 40, 4, 4, 112, 48, torch.bfloat16, None, False, None),
+    (4, 700, 40, 8, 128, 128, torch.bfloat16, torch.float32, False, None),
+]
+
+
+def _inputs(case, seed=0):
+    B, N, H, H_kv, D, R, dt, wdt, inter, sections = case
+    # heads beside each other in one projection, as a model has them
+    x = _gen((B, N, (H + H_kv) * D), 1 + seed, dt, 2.0)
+    q = x[..., :H * D].view(B, N, H, D).transpose(1, 2)
+    k = x[..., H * D:].view(B, N, H_kv, D).transpose(1, 2)
+    wq, wk = (None, None) if wdt is None else ((1 + 0.2 * _gen((D,), s)).to(wdt) for s in (2, 3))
+    f = torch.pow(torch.tensor(1e4, dtype=torch.float64), -torch.arange(0, R, 2, dtype=torch.float64) / R).cuda()
+    if sections is None:
+        pos = torch.randint(0, 1 << 20, (B, N), device="cuda", dtype=torch.int32)
+    else:
+        pos = torch.randint(0, 5000, (len(sections), B, N), device="cuda", dtype=torch.int64)
+    return q, k, wq, wk, f, pos, sections, inter
+
+
+@pytest.mark.parametrize("case", CASES, ids=[str(i) for i in range(len(CASES))])
+def test_forward_and_backward(rot, case):
+    B, N, H, H_kv, D, R, dt, wdt, inter, sections = case
+    eps = 1e-5
+    q, k, wq, wk, f, pos, sections, inter = _inputs(case)
+    cos, sin = _turns(f, pos, sections, B, N)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k) + (() if wq is None else (wq, wk))]
+    lq, lk = leaves[:2]
+    lwq, lwk = leaves[2:] if wq is not None else (None, None)
+    yq, yk = rot.qk_norm_rope(lq, lk, f, pos, q_weight=lwq, k_weight=lwk, eps=eps, sections=sections, interleaved=inter)
+    assert yq.shape == q.shape and yk.shape == k.shape and yq.dtype == dt
+    assert yq.is_contiguous() and yk.is_contiguous()
+    gq, gk = _gen(q.shape, 11, dt), _gen(k.shape, 12, dt)
+    grads = torch.autograd.grad((yq, yk), leaves, (gq, gk))
+    for i, (x, w, g, y) in enumerate(((q, wq, gq, yq), (k, wk, gk, yk))):
+        want, mag = _oracle(x, w, cos, sin, inter, eps)
+        _close(y.detach(), want, mag, 32, f"output {i}")
+        dx, dxm, dw, dwm = _oracle_back(x, w, g, cos, sin, inter, eps)
+        assert grads[i].dtype == dt and grads[i].shape == x.shape
+        _close(grads[i], dx, dxm, 48, f"gradient {i}")
+        if w is not None:
+            assert grads[2 + i].dtype == w.dtype
+            rows = B * N * (H, H_kv)[i]
+            _close(grads[2 + i], dw, dwm, rows / 8 + 64, f"weight gradient {i}")
+    # the gradient of a projection's view keeps its heads beside each other
+    assert N == 1 or H == 1 or grads[0].stride(1) == D
+
+
+@pytest.mark.parametrize("inter", [False, True])
+def test_gradient_against_differences(rot, inter):
+    """Central differences of the kernel's own fp32 forward along a random
+    direction.  Tolerance: the roundings of the two sums (32 of 2^-24 of the
+    terms' magnitudes, over the step) and what the step itself leaves, twice
+    its value in 64 bits."""
+    B, N, H, H_kv, D, R = 1, 6, 2, 1, 64, 32
+    case = (B, N, H, H_kv, D, R, torch.float32, torch.float32, inter, None)
+    q, k, wq, wk, f, pos, _, _ = _inputs(case)
+    gq, gk = _gen(q.shape, 21), _gen(k.shape, 22)
+    leaves = [t.detach().clone().requires_grad_(True) for t in (q, k, wq, wk)]
+    y = rot.qk_norm_rope(leaves[0], leaves[1], f, pos, q_weight=leaves[2], k_weight=leaves[3], interleaved=inter)
+    grads = torch.autograd.grad(y, leaves, (gq, gk))
+    cos, sin = _turns(f, pos, None, B, N)
+    h = 2.0 ** -6
+
+    def in64(q, k, wq, wk):
+        return sum((_oracle(x, w, cos, sin, inter, 1e-6)[0] * g.double()).sum() for x, w, g in ((q, wq, gq), (k, wk, gk)))
+
+    for which in range(4):
+        d = _gen(leaves[which].shape, 30 + which)
+        at = lambda s: [t.detach() + s * d if i == which else t.detach() for i, t in enumerate(leaves)]   # noqa: E731
+        total, mags = [], 0.0
+        for s in (h, -h):
+            a = at(s)
+            yq, yk = rot.qk_norm_rope_forward(a[0], a[1], f, pos, q_weight=a[2], k_weight=a[3], interleaved=inter)
+            total.append((yq.double() * gq.double()).sum() + (yk.double() * gk.double()).sum())
+            for x, w, g in ((a[0], a[2], gq), (a[1], a[3], gk)):
+                mags += float((_oracle(x, w, cos, sin, inter, 1e-6)[1] * g.double().abs()).sum())
+        got = float((total[0] - total[1]) / (2 * h))
+        want = float((grads[which].double() * d.double()).sum())
+        d64 = d.double()
+        at64 = lambda s: [t.detach().double() + s * d64 if i == which else t.detach().double() for i, t in enumerate(leaves)]   # noqa: E731
+        step = float((in64(*at64(h)) - in64(*at64(-h))) / (2 * h))
+        tiny = h / 64
+        exact = float((in64(*at64(tiny)) - in64(*at64(-tiny))) / (2 * tiny))
+        assert abs(got - want) <= 32 * U * mags / (2 * h) + 2 * abs(step - exact) + 1e-5 * abs(want)
+
+
+def test_far_positions(rot):
+    """Angles stay exact to fp32 up to 2^31 - 1 (a position times a frequency in
+    fp32 would be off by whole turns) and for negative positions."""
+    D = 64
+    pos = torch.tensor([0, 1, 131071, (1 << 24) + 1, (1 << 31) - 1, -1, -12345678], dtype=torch.int64, device="cuda")
+    N = pos.numel()
+    q, k = _gen((1, 2, N, D), 1), _gen((1, 1, N, D), 2)
+    f = rot.rotary_frequencies(D, theta=1e4)
+    y, _ = rot.qk_norm_rope(q, k, f, pos)
+    # 64-bit angles carry 2^-53 of up to 2^31 turns: 2^-22 of a turn, about 2^-19 rad at the far end
+    cos, sin = _turns(f, pos, None, 1, N)
+    want, mag = _oracle(q, None, cos, sin, False, 0.0)
+    tol = 32 * U * mag + (pos.abs().double() * 2.0 ** -51).view(1, 1, N, 1) * mag
+    assert ((y.double() - want).abs() <= tol).all()
+    y32, _ = rot.qk_norm_rope(q[:, :, 2:4].contiguous(), k[:, :, 2:4].contiguous(), f, pos[2:4].int())
+    assert torch.equal(y32, y[:, :, 2:4])
+    # frequencies held in fp32 are taken as those values
+    y_f32, _ = rot.qk_norm_rope(q[:, :, :3].contiguous(), k[:, :, :3].contiguous(), f.float(), pos[:3])
+    cos, sin = _turns(f.float(), pos[:3], None, 1, 3)
+    want, mag = _oracle(q[:, :, :3], None, cos, sin, False, 0.0)
+    _close(y_f32, want, mag, 32, "fp32 frequencies")
+
+
+def test_strides_alignment_and_defaults(rot):
+    """Views that the kernel reads in place, and ones that go through a copy;
+    positions that are left out, shared by sequences or strided."""
+    B, N, H, D = 2, 9, 3, 64
+    f = rot.rotary_frequencies(D)
+    w = 1 + 0.1 * _gen((D,), 5)
+    base = _gen((B, H, N, D), 1, torch.bfloat16)
+    k = _gen((B, 1, N, D), 2, torch.bfloat16)
+    want = rot.qk_norm_rope(base, k, f, q_weight=w, k_weight=w)
+    odd = torch.empty(base.numel() + 1, dtype=torch.bfloat16, device="cuda")[1:].view(B, H, N, D).copy_(base)
+    assert odd.data_ptr() % 16
+    wide = torch.zeros((B, H, N, D + 4), dtype=torch.bfloat16, device="cuda")
+    wide[..., :D] = base
+    turned = base.transpose(2, 3).contiguous().transpose(2, 3)
+    every = torch.empty((B, N, 2 * H, D), dtype=torch.bfloat16, device="cuda").transpose(1, 2)[:, ::2]
+    every.copy_(base)
+    for q in (odd, wide[..., :D], turned, every):
+        got = rot.qk_norm_rope(q, k, f, q_weight=w, k_weight=w)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        leaf = q.detach().requires_grad_(True)
+        y, _ = rot.qk_norm_rope(leaf, k, f, q_weight=w, k_weight=w)
+        g = _gen((B, H, N, D), 8, torch.bfloat16)
+        (dq,) = torch.autograd.grad(y, leaf, g)
+        ref = base.detach().requires_grad_(True)
+        yr, _ = rot.qk_norm_rope(ref, k, f, q_weight=w, k_weight=w)
+        (dr,) = torch.autograd.grad(yr, ref, g)
+        assert torch.equal(dq, dr)
+    pos = torch.arange(N, device="cuda", dtype=torch.int32)
+    for p in (pos, pos.long(), pos.expand(B, N), torch.arange(2 * N, device="cuda", dtype=torch.int32)[::2] // 2):
+        got = rot.qk_norm_rope(base, k, f, p, q_weight=w, k_weight=w)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_broadcast_inputs_and_gradients(rot):
+    """A key head expanded over the batch, and a gradient that is one value
+    expanded over the output: sums of the rows' gradients."""
+    B, N, H, D = 3, 20, 2, 64
+    f, w = rot.rotary_frequencies(D), (1 + 0.1 * _gen((D,), 5)).requires_grad_(True)
+    q = _gen((B, H, N, D), 1)
+    k1 = _gen((1, 1, N, D), 2).requires_grad_(True)
+    yq, yk = rot.qk_norm_rope(q, k1.expand(B, 1, N, D), f, q_weight=w, k_weight=w)
+    dk, dw = torch.autograd.grad(yk.sum(), (k1, w))
+    cos, sin = _turns(f, None, None, B, N)
+    ones = torch.ones((B, 1, N, D), device="cuda")
+    dx, dxm, dwr, dwm = _oracle_back(k1.detach().expand(B, 1, N, D), w.detach(), ones, cos, sin, False, 1e-6)
+    _close(dk, dx.sum(0, keepdim=True), dxm.sum(0, keepdim=True), 60, "shared key")
+    _close(dw, dwr, dwm, 100, "shared weight")     # the unused query output adds nothing
+    assert torch.equal(dw, torch.autograd.grad(rot.qk_norm_rope(q, k1.expand(B, 1, N, D), f, q_weight=w, k_weight=w)[1].sum(), w)[0])
+
+
+def test_partial_requirements(rot):
+    """Only what asks for a gradient gets one; a second derivative is refused."""
+    q, k = _gen((1, 2, 4, 32), 1), _gen((1, 1, 4, 32), 2)
+    f = rot.rotary_frequencies(32)
+    w = _gen((32,), 3).requires_grad_(True)
+    yq, yk = rot.qk_norm_rope(q, k, f, q_weight=w, k_weight=None)
+    assert yq.requires_grad
+    (dw,) = torch.autograd.grad(yq.square().sum(), w)
+    assert dw.shape == (32,) and torch.isfinite(dw).all()
+    qa = q.clone().requires_grad_(True)
+    y, _ = rot.qk_norm_rope(qa, k, f)
+    (d,) = torch.autograd.grad(y.square().sum(), qa, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(d.sum(), qa)
+    with torch.no_grad():
+        assert not rot.qk_norm_rope(qa, k, f)[0].requires_grad
+
+
+def test_values_out_of_range_stay_in_their_rows(rot):
+    """NaN or infinity in one row reaches that row alone; without a norm, values
+    behind the rotation are copied as they are; an all-zero row gives zeros and
+    finite gradients."""
+    N, D, R = 6, 64, 32
+    f = rot.rotary_frequencies(R)
+    w = 1 + 0.1 * _gen((D,), 4)
+    q, k = _gen((1, 2, N, D), 1), _gen((1, 1, N, D), 2)
+    clean, _ = rot.qk_norm_rope(q, k, f, q_weight=w)
+    bad = q.clone()
+    bad[0, 1, 2, 5] = math.nan
+    bad[0, 0, 4, 40] = math.inf
+    bad[0, 0, 5] = 0
+    leaf = bad.clone().requires_grad_(True)
+    y, _ = rot.qk_norm_rope(leaf, k, f, q_weight=w)
+    hit = torch.zeros((1, 2, N), dtype=torch.bool, device="cuda")
+    hit[0, 1, 2] = hit[0, 0, 4] = hit[0, 0, 5] = True
+    assert torch.equal(y[~hit], clean[~hit])
+    assert y[0, 1, 2].isnan().all() and (y[0, 0, 5] == 0).all()
+    (d,) = torch.autograd.grad(y, leaf, torch.ones_like(y))
+    rest = torch.ones_like(hit)
+    rest[0, 1, 2] = rest[0, 0, 4] = False
+    assert torch.isfinite(d[rest]).all()
+    plain, _ = rot.qk_norm_rope(bad, k, f)
+    assert plain[0, 0, 4, 40] == math.inf and torch.isfinite(plain[0, 0, 4, :R]).all()
+    assert torch.equal(plain[0, 0, 4, R:], bad[0, 0, 4, R:])
+
+
+def test_reproducible_and_captured(rot):
+    """The same bits every time; captured into a graph with its backward and
+    replayed on new inputs, also while another stream runs the same call."""
+    case = (2, 300, 8, 2, 128, 128, torch.bfloat16, torch.float32, False, None)
+    q, k, wq, wk, f, pos, _, _ = _inputs(case)
+    gq, gk = _gen(q.shape, 11, q.dtype), _gen(k.shape, 12, k.dtype)
+    kw = dict(q_weight=wq, k_weight=wk)
+    first = rot.qk_norm_rope_forward(q, k, f, pos, **kw) + rot.qk_norm_rope_backward(gq, gk, q, k, f, pos, **kw)
+    for _ in range(3):
+        again = rot.qk_norm_rope_forward(q, k, f, pos, **kw) + rot.qk_norm_rope_backward(gq, gk, q, k, f, pos, **kw)
+        assert all(torch.equal(a, b) for a, b in zip(first, again))
+    sq, sk = q.clone(), k.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = rot.qk_norm_rope_forward(sq, sk, f, pos, **kw) + rot.qk_norm_rope_backward(gq, gk, sq, sk, f, pos, **kw)
+    other = _inputs(case, seed=50)
+    sq.copy_(other[0])
+    sk.copy_(other[1])
+    graph.replay()
+    with torch.cuda.stream(side):
+        at_once = rot.qk_norm_rope_backward(gq, gk, q, k, f, pos, **kw)
+    torch.cuda.synchronize()
+    want = rot.qk_norm_rope_forward(other[0], other[1], f, pos, **kw) + \
+        rot.qk_norm_rope_backward(gq, gk, other[0], other[1], f, pos, **kw)
+    assert all(torch.equal(a, b) for a, b in zip(out, want))
+    assert all(torch.equal(a, b) for a, b in zip(at_once, first[2:]))
+
+
+def test_empty(rot):
+    f = rot.rotary_frequencies(64)
+    w = torch.ones(64, device="cuda").requires_grad_(True)
+    q = torch.empty((2, 3, 0, 64), device="cuda", requires_grad=True)
+    k = torch.empty((2, 1, 0, 64), device="cuda")
+    yq, yk = rot.qk_norm_rope(q, k, f, q_weight=w, k_weight=w)
+    assert yq.shape == q.shape and yk.shape == k.shape
+    dq, dw = torch.autograd.grad(yq.sum(), (q, w))
+    assert dq.shape == q.shape and (dw == 0).all()
+
+
+def test_training_chain(rot):
+    """Projection -> norm and rotation -> causal attention -> gradients, against
+    the same chain in 64 bits (the attention's own bar for outputs and
+    gradients: bf16 products inside)."""
+    from pallas_flash.ops.interface import pallas_flash_attention
+    B, N, H, D = 2, 160, 3, 128
+    x = _gen((B, N, 3 * H * D), 1, torch.bfloat16)
+    wq, wk = ((1 + 0.1 * _gen((D,), s)) for s in (2, 3))
+    f = rot.rotary_frequencies(D)
+    do = _gen((B, H, N, D), 4, torch.bfloat16)
+
+    def split(t):
+        return [p.view(B, N, H, D).transpose(1, 2) for p in t.split(H * D, -1)]
+
+    leaf = x.clone().requires_grad_(True)
+    ws = [w.clone().requires_grad_(True) for w in (wq, wk)]
+    q, k, v = split(leaf)
+    q, k = rot.qk_norm_rope(q, k, f, q_weight=ws[0], k_weight=ws[1])
+    o = pallas_flash_attention(q, k, v, causal=True)
+    got = torch.autograd.grad(o, [leaf] + ws, do)
+
+    leaf64 = x.double().requires_grad_(True)
+    ws64 = [w.double().requires_grad_(True) for w in (wq, wk)]
+    q, k, v = split(leaf64)
+    cos, sin = _turns(f, None, None, B, N)
+    q, k = (_oracle(t, w, cos, sin, False, 1e-6)[0] for t, w in ((q, ws64[0]), (k, ws64[1])))
+    s = (q @ k.transpose(2, 3)) / math.sqrt(D)
+    s = s.masked_fill(torch.ones(N, N, dtype=torch.bool, device="cuda").triu(1), -math.inf)
+    o64 = s.softmax(-1) @ v
+    want = torch.autograd.grad(o64, [leaf64] + ws64, do.double())
+    assert_close_o(to_np(o), to_np(o64), what="chain")
+    for n, a, b in zip(("x", "wq", "wk"), got, want):
+        assert_close_grad(to_np(a), to_np(b), what=n)

@@ -1,0 +1,181 @@
+"""Argument errors of the norm + rotation, page planning and grouped paged
+decode entry points, without a GPU: the host checks come before any CUDA call
+(pointers here are never followed)."""
+from __future__ import annotations
+
+import ctypes
+import re
+from pathlib import Path
+
+import pytest
+import torch
+
+P = 1 << 12      # 16-byte aligned, never followed
+ROOT = Path(__file__).resolve().parent.parent
+
+
+@pytest.fixture(scope="module")
+def lib(built_lib):
+    from pallas_flash import _lib
+    return _lib, _lib.lib()
+
+
+def desc(**kw):
+    """A valid description of 2 x 5 tokens, with changes."""
+    from pallas_flash.ops import rotary
+    f = dict(B=2, N=5, H=4, H_kv=2, D=64, dtype=0, R=64, inter=0, freq=P, f64=1, pos=P, pos64=0, pos_st=(0, 5, 1), axes=1,
+             sizes=(32, 0, 0, 0), wq=P, wqd=2, wk=P, wkd=2, eps=1e-6, strides=(1280, 320, 64) * 7)
+    f.update(kw)
+    return rotary._DESC.pack(f["B"], f["N"], f["H"], f["H_kv"], f["D"], f["dtype"], f["R"], f["inter"], f["freq"], f["f64"], f["pos"],
+                             f["pos64"], *f["pos_st"], f["axes"], *f["sizes"], f["wq"], f["wqd"], f["wk"], f["wkd"], f["eps"],
+                             *f["strides"])
+
+
+def test_description_matches_the_header():
+    """The packed description has the header's fields in its order, 8 bytes each."""
+    from pallas_flash.ops import rotary
+    text = (ROOT / "include" / "pu_attn.h").read_text()
+    body = re.search(r"typedef struct pu_qk_rope_desc \{(.*?)\} pu_qk_rope_desc;", text, re.S).group(1)
+    body = re.sub(r"/\*.*?\*/", "", body, flags=re.S)
+    kinds = ""
+    for line in body.split(";"):
+        m = re.match(r"\s*(int64_t|double|const void\s*\*)\s*(.*)", line.strip(), re.S)
+        if not m:
+            continue
+        for name in m.group(2).split(","):
+            n = re.search(r"\[(\d+)\]", name)
+            kinds += ("d" if m.group(1) == "double" else "q") * (int(n.group(1)) if n else 1)
+    assert kinds == "q" * 24 + "d" + "q" * 21
+    assert rotary._DESC.size == 8 * len(kinds)
+
+
+BAD = [
+    dict(B=0), dict(N=-1), dict(H=0), dict(H_kv=0), dict(D=0), dict(D=24), dict(D=144), dict(R=0), dict(R=80), dict(R=24),
+    dict(dtype=3), dict(freq=0), dict(wqd=3), dict(wkd=9), dict(eps=-1.0), dict(eps=float("nan")), dict(axes=0), dict(axes=5),
+    dict(axes=2, sizes=(16, 16, 0, 0), pos=0), dict(sizes=(31, 0, 0, 0)), dict(axes=2, sizes=(40, -8, 0, 0)),
+    dict(B=1 << 20, N=1 << 20), dict(strides=(1280, 324, 64) * 7), dict(strides=(1280, 320, 60) * 7),
+]
+
+
+@pytest.mark.parametrize("change", BAD, ids=[str(i) for i in range(len(BAD))])
+def test_descriptions_are_checked(lib, change):
+    _lib, so = lib
+    d = desc(**change)
+    refused = (_lib.PU_ERR_INVALID_ARGUMENT, _lib.PU_ERR_UNSUPPORTED)
+    assert so.pu_qk_norm_rope_fwd(d, P, P, P, P, None) in refused
+    assert so.pu_last_error()
+    assert so.pu_qk_norm_rope_bwd(d, P, P, P, P, P, P, P, P, P, 1 << 20, None) in refused
+    one = dict(change) if "B" in change else dict(change, B=1)
+    assert so.pu_qk_norm_rope_append(desc(**one), P, P, P, P, P, P, P, 0, 8, 16, 1.0, 1.0, None) in refused
+
+
+def test_pointers_and_pools_are_checked(lib):
+    _lib, so = lib
+    inv, uns, ws = _lib.PU_ERR_INVALID_ARGUMENT, _lib.PU_ERR_UNSUPPORTED, _lib.PU_ERR_WORKSPACE
+    d, d1 = desc(), desc(B=1)
+    assert so.pu_qk_norm_rope_fwd(None, P, P, P, P, None) == inv
+    for i in range(4):
+        a = [P] * 4
+        a[i] = None
+        assert so.pu_qk_norm_rope_fwd(d, *a, None) == inv
+        a[i] = P + 8
+        assert so.pu_qk_norm_rope_fwd(d, *a, None) == inv
+    assert so.pu_qk_norm_rope_bwd(d, P, P, P, P, None, None, None, None, None, 0, None) == inv
+    assert so.pu_qk_norm_rope_bwd(d, P, P, None, P, P, P, None, None, None, 0, None) == inv
+    assert so.pu_qk_norm_rope_bwd(d, P, P, P, P, None, P, P, None, P, 1 << 20, None) == inv      # a weight's gradient without its rows
+    assert so.pu_qk_norm_rope_bwd(desc(wq=0), P, P, P, P, P, P, P, None, P, 1 << 20, None) == inv
+    assert so.pu_qk_norm_rope_bwd(d, P, P, P, P, P, P, P, P, P, 16, None) == ws
+    assert so.pu_qk_norm_rope_bwd(d, P, P, P, P, P, P, P, P, None, 1 << 20, None) == ws
+    assert so.pu_qk_norm_rope_bwd_workspace_size(0) == 0 and so.pu_qk_norm_rope_bwd_workspace_size(128) > 0
+    good = [P, P, P, P, P, P, P, 0, 8, 16, 1.0, 1.0, None]
+    assert so.pu_qk_norm_rope_append(d, *good) == inv                  # B must be 1
+    for at, bad, code in ((0, None, inv), (4, None, inv), (6, None, inv), (2, P + 2, inv), (5, P + 8, inv), (7, 2, uns), (8, 0, inv),
+                          (9, 24, uns), (9, 8, uns), (9, 8192, uns), (8, 1 << 28, uns), (10, 0.0, inv), (11, float("inf"), inv)):
+        a = list(good)
+        a[at] = bad
+        assert so.pu_qk_norm_rope_append(d1, *a) == code, (at, bad)
+
+
+def test_page_plan_arguments(lib):
+    _lib, so = lib
+    inv, uns = _lib.PU_ERR_INVALID_ARGUMENT, _lib.PU_ERR_UNSUPPORTED
+    Q = P + 4096
+    #       table, out, width, lens, out, new, release, ring, pages, cursor, out, page, slots, pos, seq, cu, B, T, stream
+    good = [P, Q, 4, P, Q, P, None, P, 8, P, Q, 16, P, P, P, P, 2, 3, None]
+    for at in (0, 1, 3, 4, 5, 7, 9, 10, 12, 13, 14, 15):
+        a = list(good)
+        a[at] = None
+        assert so.pu_page_plan(*a) == inv, at
+    for at, bad, code in ((2, 0, uns), (2, 1 << 30, uns), (8, 0, inv), (11, 24, uns), (11, 8, uns), (16, 0, uns), (16, 8193, uns),
+                          (17, -1, uns), (1, P, inv), (4, P, inv), (10, P, inv)):
+        a = list(good)
+        a[at] = bad
+        assert so.pu_page_plan(*a) == code, (at, bad)
+
+
+def test_grouped_paged_decode_arguments(lib):
+    _lib, so = lib
+    inv, uns, ws = _lib.PU_ERR_INVALID_ARGUMENT, _lib.PU_ERR_UNSUPPORTED, _lib.PU_ERR_WORKSPACE
+    #       q, qdt, k, v, kvdt, table, width, pages, page, lens, o, lse, ws, bytes, B, H, H_kv, D, scale, ks, vs, stream
+    good = [P, 0, P, P, 0, P, 4, 8, 16, P, P, None, P, 1 << 24, 2, 8, 2, 128, 0.1, 1.0, 1.0, None]
+    for at, bad, code in ((0, None, inv), (2, None, inv), (5, None, inv), (9, None, inv), (10, None, inv), (12, None, ws), (13, 4096, ws),
+                          (1, 2, uns), (1, 3, uns), (4, 2, uns), (6, 0, inv), (7, 0, inv), (8, 24, uns), (14, 0, inv), (15, 7, inv),
+                          (16, 0, inv), (16, 3, inv), (17, 96, uns), (0, P + 8, inv), (3, P + 8, inv), (19, 0.0, inv),
+                          (20, float("nan"), inv), (14, 40000, uns)):
+        a = list(good)
+        a[at] = bad
+        assert so.pu_decode_paged_gqa(*a) == code, (at, bad)
+    assert so.pu_decode_paged_gqa_workspace_size(2, 8, 3, 4, 16, 128) == 0
+    assert so.pu_decode_paged_gqa_workspace_size(2, 8, 2, 4, 16, 128) > 0
+
+
+def test_python_checks_come_first():
+    """Host tensors and mismatched shapes are refused before the library is asked."""
+    from pallas_flash.kernels.paged import DevicePagedKVCache, paged_decode, plan_append, qk_norm_rope_append
+    from pallas_flash.ops.rotary import qk_norm_rope, rotary_frequencies
+    z = torch.zeros
+    f = z(32, dtype=torch.float64)
+    with pytest.raises(ValueError, match="CUDA"):
+        qk_norm_rope(z(1, 2, 3, 64), z(1, 1, 3, 64), f)
+    with pytest.raises(ValueError, match="does not match"):
+        qk_norm_rope(z(1, 2, 3, 64), z(1, 1, 4, 64), f)
+    with pytest.raises(ValueError, match="B, H, N, D"):
+        qk_norm_rope(z(2, 3, 64), z(1, 3, 64), f)
+    with pytest.raises(ValueError, match="multiple of 16"):
+        rotary_frequencies(40, device="cpu")
+    i32 = lambda *s: z(*s, dtype=torch.int32)     # noqa: E731
+    cursor = z(2, dtype=torch.int64)
+    for bad in (dict(kv_lens=i32(3)), dict(new_lens=z(2)), dict(cursor=i32(2)), dict(page_table=z(2, 4)), dict(free_ring=z(8)),
+                dict(release=z(2)), dict()):
+        a = dict(page_table=i32(2, 4), kv_lens=i32(2), new_lens=i32(2), free_ring=i32(8), cursor=cursor)
+        rel = bad.pop("release", None)
+        a.update(bad)
+        with pytest.raises(ValueError):
+            plan_append(*a.values(), page_size=16, num_tokens=2, release=rel)
+    with pytest.raises(ValueError):
+        paged_decode(z(2, 4, 1, 64).half(), z(8, 2, 16, 64).half(), z(8, 2, 16, 64).half(), i32(2, 4), i32(2))
+    with pytest.raises(ValueError, match="T, H, D"):
+        qk_norm_rope_append(z(3, 4, 64), z(3, 2, 64), z(2, 2, 64), f, i32(3), i32(3), z(8, 2, 16, 64), z(8, 2, 16, 64))
+    with pytest.raises(ValueError, match="page_size"):
+        DevicePagedKVCache(1, 1, 64, num_pages=4, page_size=24, max_seq_len=64, device="cpu")
+
+
+def test_sections_and_positions_are_checked():
+    from pallas_flash.ops.rotary import _check_angles
+    dev = torch.device("cpu")
+    f = torch.zeros(32, dtype=torch.float64)
+    pos = lambda *s: torch.zeros(*s, dtype=torch.int32)     # noqa: E731
+    ok = _check_angles(f, pos(2, 5), None, 64, (2, 5), dev)
+    assert ok[1:] == (64, (0, 5, 1), 1, (32, 0, 0, 0))
+    assert _check_angles(f, pos(5), None, 64, (2, 5), dev)[2] == (0, 0, 1)
+    assert _check_angles(f, pos(3, 2, 5), (8, 12, 12), 64, (2, 5), dev)[2:] == ((10, 5, 1), 3, (8, 12, 12, 0))
+    assert _check_angles(f, pos(3, 5), (8, 12, 12), 64, (2, 5), dev)[2] == (5, 0, 1)
+    assert _check_angles(f, pos(3, 5), (8, 12, 12), 64, (5,), dev)[2] == (5, 1)
+    assert _check_angles(f, None, None, 64, (2, 5), dev)[2] == (0, 0, 0)
+    for args in ((f, pos(2, 6), None, 64), (f, pos(5, 2), None, 64), (f, pos(2, 5), (8, 12, 12), 64), (f, None, (16, 16), 64),
+                 (f, pos(3, 2, 5), (8, 12, 13), 64), (f, pos(3, 2, 5), (8, 12, 20, -8, 0), 64), (f, torch.zeros(2, 5), None, 64),
+                 (f, pos(2, 5), None, 32), (torch.zeros(12, dtype=torch.float64), pos(2, 5), None, 64), (f.half(), pos(2, 5), None, 64),
+                 (f, pos(1, 2, 5), (), 64)):
+        with pytest.raises(ValueError):
+            _check_angles(*args, (2, 5), dev)
+    assert ctypes.sizeof(ctypes.c_void_p) == 8
