@@ -296,14 +296,31 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
 
   if (warp == kLoadWarp) {
     // ---------------- pages -> ring ----------------
+    // The table is read kAhead tiles before its use (lane i: box i's entry),
+    // or each tile would wait for its entries before its loads could leave.
+    constexpr int kAhead = 4;
     const int boxes = BT / p.box, per_page = 1 << p.page_shift;
+    Walk wl = w0;                          // the tile whose entries are read next
+    int ahead[kAhead];
+    auto look_up = [&]() -> int {
+      int pg = 0;
+      if (wl.left > 0) {
+        const int row = wl.t * BT + lane * p.box;
+        if (lane < boxes && row < wl.len_of(wl.b)) pg = p.table[(size_t)wl.b * p.max_pages + (row >> p.page_shift)];
+        wl.next();
+      }
+      return pg;
+    };
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) ahead[i] = look_up();
     int n = 0;
     for (Walk w = w0; w.left > 0; w.next(), ++n) {
       const int s = n % NS, len = w.len_of(w.b);
-      const int row = w.t * BT + lane * p.box;
+      const int row = w.t * BT + lane * p.box, pg = ahead[0];
+#pragma unroll
+      for (int i = 0; i + 1 < kAhead; ++i) ahead[i] = ahead[i + 1];
+      ahead[kAhead - 1] = look_up();
       const bool mine = lane < boxes && row < len;
-      int pg = 0;
-      if (mine) pg = p.table[(size_t)w.b * p.max_pages + (row >> p.page_shift)];
       const bool good = mine && (unsigned)pg < (unsigned)p.num_pages;
       if (mine && !good) record_device_error(PU_ERR_INVALID_ARGUMENT, kSiteDecodePage);
       const unsigned loaded = __ballot_sync(0xffffffffu, good);
@@ -407,8 +424,8 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
         bool progressed = false;
         // S of tile js overwrites the buffer of tile js - 4, read once that
         // tile's P was written, so once its P V product was issued
-        if (ws.left > 0 && js < jp + 4 && mbar_try_wait(smem_u32(bFull + js % NS), (js / NS) & 1) &&
-            (ws.loc > 0 || mbar_try_wait(smem_u32(bQfull + (ws.seg & 3)), (ws.seg >> 2) & 1))) {
+        if (ws.left > 0 && js < jp + 4 && mbar_test_wait(bFull + js % NS, (js / NS) & 1) &&
+            (ws.loc > 0 || mbar_test_wait(bQfull + (ws.seg & 3), (ws.seg >> 2) & 1))) {
           tc_fence_after();
           const uint64_t dk = sdesc_add(dK0, (js % NS) * 2 * kTile), dq = sdesc_add(dQ0, (ws.seg & 3) * C::kQBytes);
           const uint32_t col = tmem + (js & 3) * C::kSCols;
@@ -427,8 +444,8 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
           ++js;
           progressed = true;
         }
-        if (jp < js && mbar_try_wait(smem_u32(bPf + (jp & 1)), (jp >> 1) & 1) &&
-            (wp.loc > 0 || wp.seg == 0 || mbar_try_wait(smem_u32(bOfree), (wp.seg - 1) & 1))) {
+        if (jp < js && mbar_test_wait(bPf + (jp & 1), (jp >> 1) & 1) &&
+            (wp.loc > 0 || wp.seg == 0 || mbar_test_wait(bOfree, (wp.seg - 1) & 1))) {
           tc_fence_after();
           const uint64_t dv = sdesc_add(dV0, (jp % NS) * 2 * kTile), dp = sdesc_add(dP0, (jp & 1) * C::kPBytes);
           const uint32_t col = tmem + C::kColO + (jp & 1) * C::kOCols;

@@ -41,6 +41,8 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kMaxDim = 128;
 constexpr int kMaxPairs = kMaxDim / 2;
 constexpr int kMaxAxes = 4;
+constexpr int kFwdCtasPerSm = 2;     // resident CTAs the grids ask for
+constexpr int kCtasPerSm = 2;
 
 // Rows of one tensor: element (b, h, n, d) at b sB + h sH + n sN + d.
 struct Rows {
@@ -76,7 +78,7 @@ struct Params {
   long long N;            // tokens per sequence
   long long T;            // tokens in all
   int D, R;
-  float eps;
+  float eps, inv_d;
   int chunk;              // forward: passes per warp
   int chunks;             // warps per token (backward: of either kind)
   // append
@@ -86,13 +88,24 @@ struct Params {
   long long num_slots;
 };
 
-// 8 elements: 16 bytes (16-bit types) or 32 (fp32).
+// 8 elements: 16 bytes (16-bit types) or 32 (fp32), as four packed fp32 pairs.
 template <typename T>
 struct Vec8 {
   uint4 w;
   __device__ __forceinline__ void load(const T* p) { w = decode::ld_stream(reinterpret_cast<const uint4*>(p)); }
   __device__ __forceinline__ void zero() { w = make_uint4(0u, 0u, 0u, 0u); }
-  __device__ __forceinline__ void get(float (&f)[8]) const { decode::unpack8<T>(w, f); }
+  __device__ __forceinline__ void get(uint64_t (&f)[4]) const {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same<T, __half>::value) {
+        const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+        f[i] = f2_pack(x.x, x.y);
+      } else {
+        f[i] = f2_pack(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xFFFF0000u));
+      }
+    }
+  }
 };
 template <>
 struct Vec8<float> {
@@ -102,13 +115,11 @@ struct Vec8<float> {
     w[1] = decode::ld_stream(reinterpret_cast<const uint4*>(p) + 1);
   }
   __device__ __forceinline__ void zero() { w[0] = w[1] = make_uint4(0u, 0u, 0u, 0u); }
-  __device__ __forceinline__ void get(float (&f)[8]) const {
+  __device__ __forceinline__ void get(uint64_t (&f)[4]) const {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      f[4 * i] = __uint_as_float(w[i].x);
-      f[4 * i + 1] = __uint_as_float(w[i].y);
-      f[4 * i + 2] = __uint_as_float(w[i].z);
-      f[4 * i + 3] = __uint_as_float(w[i].w);
+      f[2 * i] = f2_pack(__uint_as_float(w[i].x), __uint_as_float(w[i].y));
+      f[2 * i + 1] = f2_pack(__uint_as_float(w[i].z), __uint_as_float(w[i].w));
     }
   }
 };
@@ -119,35 +130,45 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
 }
 
 template <typename T>
-__device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
-  uint4 w;
-  if constexpr (std::is_same<T, __half>::value)
-    w = make_uint4(pack_f16x2(f[0], f[1]), pack_f16x2(f[2], f[3]), pack_f16x2(f[4], f[5]), pack_f16x2(f[6], f[7]));
-  else
-    w = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
-  *reinterpret_cast<uint4*>(p) = w;
-}
-template <>
-__device__ __forceinline__ void store8<float>(float* p, const float (&f)[8]) {
-  reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
-  reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+__device__ __forceinline__ void store8(T* p, const uint64_t (&f)[4]) {
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f2_unpack(f[i], x[2 * i], x[2 * i + 1]);
+  if constexpr (sizeof(T) == 4) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+  } else if constexpr (std::is_same<T, __half>::value) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(pack_f16x2(x[0], x[1]), pack_f16x2(x[2], x[3]), pack_f16x2(x[4], x[5]),
+                                              pack_f16x2(x[6], x[7]));
+  } else {
+    *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]),
+                                              pack_bf16x2(x[6], x[7]));
+  }
 }
 
-// 8 values into a pool row of pool_dtype (saturating e4m3, or 16-bit).
-__device__ __forceinline__ void store8_pool(void* pool, size_t at, int dtype, const float (&f)[8]) {
+// 8 values / unit into a pool row of pool_dtype (saturating e4m3, or 16-bit).
+__device__ __forceinline__ void store8_pool(void* pool, size_t at, int dtype, float unit, uint64_t (&f)[4]) {
+  if (unit != 1.f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float a, b;
+      f2_unpack(f[i], a, b);
+      f[i] = f2_pack(a / unit, b / unit);
+    }
+  }
   if (dtype == PU_DTYPE_BF16) {
     store8(static_cast<__nv_bfloat16*>(pool) + at, f);
   } else if (dtype == PU_DTYPE_F16) {
     store8(static_cast<__half*>(pool) + at, f);
   } else {
-    uint32_t w[2];
+    uint32_t h[4];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(f[4 * i], f[4 * i + 1]), __NV_SATFINITE, __NV_E4M3);
-      const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(f[4 * i + 2], f[4 * i + 3]), __NV_SATFINITE, __NV_E4M3);
-      w[i] = lo | (hi << 16);
+    for (int i = 0; i < 4; ++i) {
+      float2 x;
+      f2_unpack(f[i], x.x, x.y);
+      h[i] = __nv_cvt_float2_to_fp8x2(x, __NV_SATFINITE, __NV_E4M3);
     }
-    *reinterpret_cast<uint2*>(static_cast<uint8_t*>(pool) + at) = make_uint2(w[0], w[1]);
+    *reinterpret_cast<uint2*>(static_cast<uint8_t*>(pool) + at) = make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
   }
 }
 
@@ -157,13 +178,33 @@ __device__ __forceinline__ float load_weight(const void* w, int dtype, int i) {
   return __bfloat162float(static_cast<const __nv_bfloat16*>(w)[i]);
 }
 
-// cos and sin of every pair of one token into the warp's shared row.
-__device__ __forceinline__ void make_angles(const Angles& a, int pairs, long long b, long long n, int lane, float2* out) {
-  for (int p = lane; p < pairs; p += 32) {
-    const double f = a.freq64 ? static_cast<const double*>(a.freq)[p] : (double)static_cast<const float*>(a.freq)[p];
+// What a CTA keeps in shared memory: the weights as fp32 (1 without a norm)
+// and every pair's 64-bit turn per position; per warp, cos and sin of a token.
+struct Shared {
+  float w[2][kMaxDim];
+  unsigned long long step[kMaxPairs];
+  float cs[kWarps][2][kMaxPairs];
+};
+
+__device__ __forceinline__ void fill_shared(const Params& p, Shared& sh) {
+  for (int i = threadIdx.x; i < 2 * p.D; i += kThreads) {
+    const int k = i >= p.D, d = i - k * p.D;
+    sh.w[k][d] = p.side[k].w != nullptr ? load_weight(p.side[k].w, p.side[k].w_dtype, d) : 1.f;
+  }
+  for (int i = threadIdx.x; i < p.R / 2; i += kThreads) {
+    const double f = p.ang.freq64 ? static_cast<const double*>(p.ang.freq)[i] : (double)static_cast<const float*>(p.ang.freq)[i];
     double turns = f * 0.15915494309189533577;               // per position: 1 / 2 pi
     turns -= floor(turns);
-    const unsigned long long step = (unsigned long long)(turns * 18446744073709551616.0);   // * 2^64, below it
+    sh.step[i] = (unsigned long long)(turns * 18446744073709551616.0);   // * 2^64, below it
+  }
+  __syncthreads();
+}
+
+// cos and sin of every pair of one token into the warp's shared rows.
+__device__ __forceinline__ void make_angles(const Angles& a, const Shared& sh, int pairs, long long b, long long n, int lane,
+                                            float* cs, float* sn) {
+  __syncwarp();                          // the previous token's have been read
+  for (int p = lane; p < pairs; p += 32) {
     long long pos = n;
     if (a.pos != nullptr) {
       int axis = 0;
@@ -172,11 +213,10 @@ __device__ __forceinline__ void make_angles(const Angles& a, int pairs, long lon
       const long long at = axis * a.pA + b * a.pB + n * a.pN;
       pos = a.pos64 ? static_cast<const long long*>(a.pos)[at] : (long long)static_cast<const int32_t*>(a.pos)[at];
     }
-    const int turn = (int)((step * (unsigned long long)pos) >> 32);     // signed: half turns of 2^31
-    float s, c;
-    sincospif((float)turn * 4.6566128730773926e-10f, &s, &c);           // 2^-31
-    out[p] = make_float2(c, s);
+    const int turn = (int)((sh.step[p] * (unsigned long long)pos) >> 32);   // signed: half turns of 2^31
+    sincospif((float)turn * 4.6566128730773926e-10f, sn + p, cs + p);       // 2^-31
   }
+  __syncwarp();
 }
 
 // What a lane of a row group holds: its two vectors' places in the row.
@@ -195,28 +235,6 @@ __device__ __forceinline__ Place make_place(int sub, int D, int R) {
   return pl;
 }
 
-// Rotates the lane's 8 pairs by (c, s); with s negated, back.
-template <bool kInter>
-__device__ __forceinline__ void rotate(float (&a)[8], float (&b)[8], const float (&c)[8], const float (&s)[8]) {
-  if constexpr (kInter) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float x0 = a[2 * i], x1 = a[2 * i + 1], y0 = b[2 * i], y1 = b[2 * i + 1];
-      a[2 * i] = fmaf(x0, c[i], -x1 * s[i]);
-      a[2 * i + 1] = fmaf(x1, c[i], x0 * s[i]);
-      b[2 * i] = fmaf(y0, c[4 + i], -y1 * s[4 + i]);
-      b[2 * i + 1] = fmaf(y1, c[4 + i], y0 * s[4 + i]);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float x = a[i], y = b[i];
-      a[i] = fmaf(x, c[i], -y * s[i]);
-      b[i] = fmaf(y, c[i], x * s[i]);
-    }
-  }
-}
-
 template <int kLanes>
 __device__ __forceinline__ float group_sum(float v) {
 #pragma unroll
@@ -224,123 +242,169 @@ __device__ __forceinline__ float group_sum(float v) {
   return v;
 }
 
-// The lane's cos and sin (pairs 8 sub ..) from the warp's shared row.
-__device__ __forceinline__ void take_angles(const float2* row, const Place& pl, int sub, float (&c)[8], float (&s)[8]) {
+__device__ __forceinline__ uint64_t f2_swap(uint64_t v) {
+  float a, b;
+  f2_unpack(v, a, b);
+  return f2_pack(b, a);
+}
+
+// Row coefficients: with a, b the lane's two vectors (four pairs of values
+// each), the rotated norm is, up to 1 / rms,
+//   a' = a k0 + x k1,  b' = b k2 + y k3,  (x, y) = (b, a), or interleaved the
+//   vectors' own values with neighbours swapped
+// so the weight, the rotation and its signs cost one product and one fma per
+// two values.
+struct Coef {
+  uint64_t k0[4], k1[4], k2[4], k3[4];
+};
+
+// wa, wb: the weights of the lane's two vectors; kBack: the transposed
+// rotation with no weight.
+template <bool kInter, bool kBack>
+__device__ __forceinline__ void make_coef(const float* cs, const float* sn, const float* wa, const float* wb, const Place& pl,
+                                          int sub, Coef& k) {
+  float c[8], s[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float2 v = pl.rot ? row[sub * 8 + i] : make_float2(1.f, 0.f);
-    c[i] = v.x;
-    s[i] = v.y;
+    c[i] = pl.rot ? cs[sub * 8 + i] : 1.f;
+    s[i] = pl.rot ? sn[sub * 8 + i] : 0.f;
+    if (kBack) s[i] = -s[i];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float a0 = kBack || !pl.in ? 1.f : wa[pl.o0 + 2 * i], a1 = kBack || !pl.in ? 1.f : wa[pl.o0 + 2 * i + 1];
+    const float b0 = kBack || !pl.in ? 1.f : wb[pl.o1 + 2 * i], b1 = kBack || !pl.in ? 1.f : wb[pl.o1 + 2 * i + 1];
+    if constexpr (kInter) {
+      k.k0[i] = f2_pack(a0 * c[i], a1 * c[i]);
+      k.k1[i] = f2_pack(-a1 * s[i], a0 * s[i]);
+      k.k2[i] = f2_pack(b0 * c[4 + i], b1 * c[4 + i]);
+      k.k3[i] = f2_pack(-b1 * s[4 + i], b0 * s[4 + i]);
+    } else {
+      k.k0[i] = f2_pack(a0 * c[2 * i], a1 * c[2 * i + 1]);
+      k.k1[i] = f2_pack(-b0 * s[2 * i], -b1 * s[2 * i + 1]);
+      k.k2[i] = f2_pack(b0 * c[2 * i], b1 * c[2 * i + 1]);
+      k.k3[i] = f2_pack(a0 * s[2 * i], a1 * s[2 * i + 1]);
+    }
   }
 }
 
-__device__ __forceinline__ void take_weight(const Side& sd, const Place& pl, float (&wa)[8], float (&wb)[8]) {
+// a, b -> a', b'.  Lanes behind R take no cross term (theirs would be 0 times
+// a value that need not be finite).
+template <bool kInter>
+__device__ __forceinline__ void apply_coef(const Coef& k, bool partial, bool rot, uint64_t (&a)[4], uint64_t (&b)[4]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const bool use = sd.w != nullptr && pl.in;
-    wa[i] = use ? load_weight(sd.w, sd.w_dtype, pl.o0 + i) : 1.f;
-    wb[i] = use ? load_weight(sd.w, sd.w_dtype, pl.o1 + i) : 1.f;
+  for (int i = 0; i < 4; ++i) {
+    uint64_t x = kInter ? f2_swap(a[i]) : b[i], y = kInter ? f2_swap(b[i]) : a[i];
+    if (partial && !rot) x = y = 0ull;
+    a[i] = f2_fma(x, k.k1[i], f2_mul(a[i], k.k0[i]));
+    b[i] = f2_fma(y, k.k3[i], f2_mul(b[i], k.k2[i]));
   }
+}
+
+__device__ __forceinline__ float f2_sum(uint64_t v) {
+  float a, b;
+  f2_unpack(v, a, b);
+  return a + b;
 }
 
 // A pass is 32 / kLanes rows (heads) of one token; queries' passes come
-// first, then keys', then values'.  Each warp takes `chunk` consecutive passes
-// of one token, kBatch of them loaded before the first is used.
+// first, then keys', then values'.  A warp walks units of `chunk` consecutive
+// passes of one token, kBatch of them loaded before the first is used (and the
+// first ones before the token's angles are made).
 template <typename T, int kLanes, bool kInter, bool kAppend>
-__global__ void __launch_bounds__(kThreads) fwd_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kThreads, kFwdCtasPerSm) fwd_kernel(const __grid_constant__ Params p) {
   constexpr int kRows = 32 / kLanes;
   constexpr int kBatch = sizeof(T) == 4 ? 2 : 4;
-  __shared__ float2 s_ang[kWarps][kMaxPairs];
+  __shared__ Shared sh;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int sub = lane % kLanes, row = lane / kLanes;
-  const long long unit = (long long)blockIdx.x * kWarps + warp;
-  const long long t = unit / p.chunks;
   grid_dep_wait();
   grid_dep_launch_dependents();
-  if (t >= p.T) return;
-  const long long b = t / p.N, n = t - b * p.N;
+  fill_shared(p, sh);
   const Place pl = make_place<kInter>(sub, p.D, p.R);
-  make_angles(p.ang, p.R / 2, b, n, lane, s_ang[warp]);
-  __syncwarp();
-  float c[8], s[8];
-  take_angles(s_ang[warp], pl, sub, c, s);
-
-  size_t pool_row = 0;      // append: page and row of this token
-  bool put = true;
-  if constexpr (kAppend) {
-    const long long slot = p.slots[t];
-    put = slot >= 0 && slot < p.num_slots;
-    if (slot >= p.num_slots && lane == 0) record_device_error(PU_ERR_INVALID_ARGUMENT, kSiteAppendSlot);
-    pool_row = put ? (size_t)slot : 0;
-  }
-  const int first = (int)(unit - t * p.chunks) * p.chunk, last = first + p.chunk;
-  int begin = 0;
+  const bool partial = p.R < p.D;
+  const int end0 = (p.side[0].heads + kRows - 1) / kRows, end1 = end0 + (p.side[1].heads + kRows - 1) / kRows;
+  const int end2 = kAppend ? end1 + (p.side[2].heads + kRows - 1) / kRows : end1;
+  const long long units = p.T * p.chunks, stride = (long long)gridDim.x * kWarps;
+  for (long long unit = (long long)blockIdx.x * kWarps + warp; unit < units; unit += stride) {
+    const long long t = unit / p.chunks;
+    const long long b = t / p.N, n = t - b * p.N;
+    const int first = (int)(unit - t * p.chunks) * p.chunk, last = min(first + p.chunk, end2);
+    size_t pool_row = 0;    // append: page and row of this token
+    bool put = true;
+    if constexpr (kAppend) {
+      const long long slot = p.slots[t];
+      put = slot >= 0 && slot < p.num_slots;
+      if (slot >= p.num_slots && lane == 0) record_device_error(PU_ERR_INVALID_ARGUMENT, kSiteAppendSlot);
+      pool_row = put ? (size_t)slot : 0;
+    }
+    Coef k;
+    int kind_of_k = -1;
+    for (int pass = first; pass < last; pass += kBatch) {
+      Vec8<T> va[kBatch], vb[kBatch];
 #pragma unroll
-  for (int kind = 0; kind < (kAppend ? 3 : 2); ++kind) {
-    const Side& sd = p.side[kind];
-    const int end = begin + (sd.heads + kRows - 1) / kRows;
-    const int lo = max(first, begin), hi = min(last, end);
-    if (lo < hi) {
-      const T* x0 = static_cast<const T*>(sd.x.p) + b * sd.x.sB + n * sd.x.sN;
-      float wa[8], wb[8];
-      if (kind < 2) take_weight(sd, pl, wa, wb);
-      for (int pass = lo; pass < hi; pass += kBatch) {
-        Vec8<T> va[kBatch], vb[kBatch];
+      for (int u = 0; u < kBatch; ++u) {
+        const int ps = pass + u, kind = ps < end0 ? 0 : ps < end1 ? 1 : 2;
+        const Side& sd = p.side[kind];
+        const int h = (ps - (kind == 0 ? 0 : kind == 1 ? end0 : end1)) * kRows + row;
+        va[u].zero();
+        vb[u].zero();
+        if (ps < last && h < sd.heads && pl.in) {
+          const T* x = static_cast<const T*>(sd.x.p) + b * sd.x.sB + n * sd.x.sN + h * sd.x.sH;
+          va[u].load(x + pl.o0);
+          vb[u].load(x + pl.o1);
+        }
+      }
+      if (pass == first) make_angles(p.ang, sh, p.R / 2, b, n, lane, sh.cs[warp][0], sh.cs[warp][1]);
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
-          const int h = (pass + u - begin) * kRows + row;
-          va[u].zero();
-          vb[u].zero();
-          if (pass + u < hi && h < sd.heads && pl.in) {
-            const T* x = x0 + h * sd.x.sH;
-            va[u].load(x + pl.o0);
-            vb[u].load(x + pl.o1);
+      for (int u = 0; u < kBatch; ++u) {
+        const int ps = pass + u, kind = ps < end0 ? 0 : ps < end1 ? 1 : 2;
+        if (ps >= last) break;
+        const Side& sd = p.side[kind];
+        const int h = (ps - (kind == 0 ? 0 : kind == 1 ? end0 : end1)) * kRows + row;
+        const bool live = h < sd.heads && pl.in;
+        uint64_t a[4], bb[4];
+        va[u].get(a);
+        vb[u].get(bb);
+        if (!kAppend || kind < 2) {
+          if (kind != kind_of_k) {
+            make_coef<kInter, false>(sh.cs[warp][0], sh.cs[warp][1], sh.w[kind], sh.w[kind], pl, sub, k);
+            kind_of_k = kind;
+          }
+          float r = 1.f;
+          if (sd.w != nullptr) {
+            uint64_t s0 = 0ull, s1 = 0ull;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              s0 = f2_fma(a[i], a[i], s0);
+              s1 = f2_fma(bb[i], bb[i], s1);
+            }
+            r = rsqrtf(group_sum<kLanes>(f2_sum(f2_add(s0, s1))) * p.inv_d + p.eps);
+          }
+          apply_coef<kInter>(k, partial, pl.rot, a, bb);
+          if (sd.w != nullptr) {
+            const uint64_t rr = f2_pack(r, r);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              a[i] = f2_mul(a[i], rr);
+              bb[i] = f2_mul(bb[i], rr);
+            }
           }
         }
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
-          const int h = (pass + u - begin) * kRows + row;
-          if (pass + u >= hi) break;
-          float a[8], bb[8];
-          va[u].get(a);
-          vb[u].get(bb);
-          if (kind < 2) {
-            if (sd.w != nullptr) {
-              float ss = 0.f;
-#pragma unroll
-              for (int i = 0; i < 8; ++i) ss = fmaf(a[i], a[i], fmaf(bb[i], bb[i], ss));
-              const float r = rsqrtf(group_sum<kLanes>(ss) / (float)p.D + p.eps);
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                a[i] *= r * wa[i];
-                bb[i] *= r * wb[i];
-              }
-            }
-            if (pl.rot) rotate<kInter>(a, bb, c, s);
-          }
-          if (h >= sd.heads || !pl.in) continue;
-          if (kAppend && kind > 0) {
-            if (!put) continue;
-            if (sd.unit != 1.f) {
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                a[i] = a[i] / sd.unit;
-                bb[i] = bb[i] / sd.unit;
-              }
-            }
-            const size_t mask = ((size_t)1 << p.page_shift) - 1;
-            const size_t at = ((((pool_row >> p.page_shift) * sd.heads + h) << p.page_shift) + (pool_row & mask)) * p.D;
-            store8_pool(sd.y.p, at + pl.o0, p.pool_dtype, a);
-            store8_pool(sd.y.p, at + pl.o1, p.pool_dtype, bb);
-          } else {
-            T* y = static_cast<T*>(sd.y.p) + b * sd.y.sB + h * sd.y.sH + n * sd.y.sN;
-            store8(y + pl.o0, a);
-            store8(y + pl.o1, bb);
-          }
+        if (!live) continue;
+        if (kAppend && kind > 0) {
+          if (!put) continue;
+          const size_t mask = ((size_t)1 << p.page_shift) - 1;
+          const size_t at = ((((pool_row >> p.page_shift) * sd.heads + h) << p.page_shift) + (pool_row & mask)) * p.D;
+          store8_pool(sd.y.p, at + pl.o0, p.pool_dtype, sd.unit, a);
+          store8_pool(sd.y.p, at + pl.o1, p.pool_dtype, sd.unit, bb);
+        } else {
+          T* y = static_cast<T*>(sd.y.p) + b * sd.y.sB + h * sd.y.sH + n * sd.y.sN;
+          store8(y + pl.o0, a);
+          store8(y + pl.o1, bb);
         }
       }
     }
-    begin = end;
   }
 }
 
@@ -349,10 +413,10 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(const __grid_constant__ P
 // its rows in registers; each CTA writes one partial row, summed in a fixed
 // order by dw_kernel (no atomics: the same bits every time).
 template <typename T, int kLanes, bool kInter>
-__global__ void __launch_bounds__(kThreads) bwd_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) bwd_kernel(const __grid_constant__ Params p) {
   constexpr int kRows = 32 / kLanes;
   constexpr int kBatch = sizeof(T) == 4 ? 1 : 2;
-  __shared__ float2 s_ang[kWarps][kMaxPairs];
+  __shared__ Shared sh;
   __shared__ float s_dw[kWarps][kMaxDim];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int sub = lane % kLanes, row = lane / kLanes;
@@ -362,29 +426,23 @@ __global__ void __launch_bounds__(kThreads) bwd_kernel(const __grid_constant__ P
   const Place pl = make_place<kInter>(sub, p.D, p.R);
   grid_dep_wait();
   grid_dep_launch_dependents();
-  const bool norm = sd.w != nullptr;
-  float wa[8], wb[8], da[8], db[8];
-  take_weight(sd, pl, wa, wb);
+  fill_shared(p, sh);
+  const bool norm = sd.w != nullptr, partial = p.R < p.D;
+  const float* w = sh.w[kind];
+  uint64_t da[4], db[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) da[i] = db[i] = 0.f;
+  for (int i = 0; i < 4; ++i) da[i] = db[i] = 0ull;
   const int passes = (sd.heads + kRows - 1) / kRows;
   const int chunk = (passes + p.chunks - 1) / p.chunks;
-  const float inv_d = 1.f / (float)p.D;
   const long long units = p.T * p.chunks, stride = (long long)sd.ctas * kWarps;
   for (long long unit = (long long)cta * kWarps + warp; unit < units; unit += stride) {
     const long long t = unit / p.chunks;
     const long long b = t / p.N, n = t - b * p.N;
     const int lo = (int)(unit - t * p.chunks) * chunk, hi = min(lo + chunk, passes);
-    __syncwarp();
-    make_angles(p.ang, p.R / 2, b, n, lane, s_ang[warp]);
-    __syncwarp();
-    float c[8], s[8];
-    take_angles(s_ang[warp], pl, sub, c, s);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) s[i] = -s[i];
     const T* x0 = static_cast<const T*>(sd.x.p) + b * sd.x.sB + n * sd.x.sN;
     const T* g0 = static_cast<const T*>(sd.g.p) + b * sd.g.sB + n * sd.g.sN;
     T* y0 = static_cast<T*>(sd.y.p) + b * sd.y.sB + n * sd.y.sN;
+    Coef k;
     for (int pass = lo; pass < hi; pass += kBatch) {
       Vec8<T> xa[kBatch], xb[kBatch], ga[kBatch], gb[kBatch];
 #pragma unroll
@@ -405,34 +463,43 @@ __global__ void __launch_bounds__(kThreads) bwd_kernel(const __grid_constant__ P
           }
         }
       }
+      if (pass == lo) {
+        make_angles(p.ang, sh, p.R / 2, b, n, lane, sh.cs[warp][0], sh.cs[warp][1]);
+        make_coef<kInter, true>(sh.cs[warp][0], sh.cs[warp][1], nullptr, nullptr, pl, sub, k);
+      }
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
         const int h = (pass + u) * kRows + row;
         if (pass + u >= hi) break;
-        float ha[8], hb[8];
+        uint64_t ha[4], hb[4];
         ga[u].get(ha);
         gb[u].get(hb);
-        if (pl.rot) rotate<kInter>(ha, hb, c, s);
+        apply_coef<kInter>(k, partial, pl.rot, ha, hb);
         if (norm) {
-          float x[8], y[8];
+          uint64_t x[4], y[4], s0 = 0ull, s1 = 0ull, t0 = 0ull, t1 = 0ull, va[4], vb[4];
           xa[u].get(x);
           xb[u].get(y);
-          float ss = 0.f, dot = 0.f;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            ss = fmaf(x[i], x[i], fmaf(y[i], y[i], ss));
-            dot = fmaf(ha[i] * wa[i], x[i], fmaf(hb[i] * wb[i], y[i], dot));
+          for (int i = 0; i < 4; ++i) {
+            // in-range lanes' weights; the others' rows are zeros
+            va[i] = f2_mul(ha[i], *reinterpret_cast<const uint64_t*>(w + (pl.in ? pl.o0 : 0) + 2 * i));
+            vb[i] = f2_mul(hb[i], *reinterpret_cast<const uint64_t*>(w + (pl.in ? pl.o1 : 8) + 2 * i));
+            s0 = f2_fma(x[i], x[i], s0);
+            s1 = f2_fma(y[i], y[i], s1);
+            t0 = f2_fma(va[i], x[i], t0);
+            t1 = f2_fma(vb[i], y[i], t1);
           }
-          ss = group_sum<kLanes>(ss);
-          dot = group_sum<kLanes>(dot);
-          const float r = rsqrtf(ss * inv_d + p.eps);
-          const float k = dot * inv_d * r * r * r;        // dx = r (h w) - x k
+          const float ss = group_sum<kLanes>(f2_sum(f2_add(s0, s1)));
+          const float dot = group_sum<kLanes>(f2_sum(f2_add(t0, t1)));
+          const float r = rsqrtf(ss * p.inv_d + p.eps);
+          const float q = -dot * p.inv_d * r * r * r;        // dx = r (h w) + x q
+          const uint64_t rr = f2_pack(r, r), qq = f2_pack(q, q);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            da[i] = fmaf(ha[i] * r, x[i], da[i]);
-            db[i] = fmaf(hb[i] * r, y[i], db[i]);
-            ha[i] = fmaf(ha[i] * wa[i], r, -x[i] * k);
-            hb[i] = fmaf(hb[i] * wb[i], r, -y[i] * k);
+          for (int i = 0; i < 4; ++i) {
+            da[i] = f2_fma(ha[i], f2_mul(x[i], rr), da[i]);
+            db[i] = f2_fma(hb[i], f2_mul(y[i], rr), db[i]);
+            ha[i] = f2_fma(va[i], rr, f2_mul(x[i], qq));
+            hb[i] = f2_fma(vb[i], rr, f2_mul(y[i], qq));
           }
         }
         if (h >= sd.heads || !pl.in) continue;
@@ -445,25 +512,27 @@ __global__ void __launch_bounds__(kThreads) bwd_kernel(const __grid_constant__ P
   if (sd.dw_part == nullptr) return;
   // rows of the warp, then the warps
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < 4; ++i) {
+    float v[4];
+    f2_unpack(da[i], v[0], v[1]);
+    f2_unpack(db[i], v[2], v[3]);
 #pragma unroll
-    for (int off = kLanes; off < 32; off <<= 1) {
-      da[i] += __shfl_xor_sync(0xffffffffu, da[i], off);
-      db[i] += __shfl_xor_sync(0xffffffffu, db[i], off);
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int off = kLanes; off < 32; off <<= 1) v[j] += __shfl_xor_sync(0xffffffffu, v[j], off);
     }
-  }
-  if (row == 0 && pl.in) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      s_dw[warp][pl.o0 + i] = da[i];
-      s_dw[warp][pl.o1 + i] = db[i];
+    if (row == 0 && pl.in) {
+      s_dw[warp][pl.o0 + 2 * i] = v[0];
+      s_dw[warp][pl.o0 + 2 * i + 1] = v[1];
+      s_dw[warp][pl.o1 + 2 * i] = v[2];
+      s_dw[warp][pl.o1 + 2 * i + 1] = v[3];
     }
   }
   __syncthreads();
   if ((int)threadIdx.x < p.D) {
     float v = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) v += s_dw[w][threadIdx.x];
+    for (int i = 0; i < kWarps; ++i) v += s_dw[i][threadIdx.x];
     sd.dw_part[(size_t)cta * p.D + threadIdx.x] = v;
   }
 }
@@ -497,8 +566,6 @@ __global__ void __launch_bounds__(kMaxDim * kDwParts) dw_kernel(const __grid_con
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
-constexpr int kCtasPerSm = 2;        // resident CTAs the backward's grid asks for
-
 inline bool type_ok(int64_t t) { return t == PU_DTYPE_BF16 || t == PU_DTYPE_F16 || t == PU_DTYPE_F32; }
 
 // Every row a kernel reads or writes in 16-byte vectors starts on a 16-byte
@@ -548,6 +615,7 @@ inline int check(const pu_qk_rope_desc* d, const char* who, Params* p) {
   p->D = (int)d->D;
   p->R = (int)d->rotary_dim;
   p->eps = (float)d->eps;
+  p->inv_d = 1.f / (float)d->D;
   p->side[0].heads = (int)d->H;
   p->side[1].heads = p->side[2].heads = (int)d->H_kv;
   p->side[0].w = d->q_weight;
@@ -572,8 +640,7 @@ int launch_fwd(Params& p, bool inter, cudaStream_t st) {
   const long long want = (long long)sm_count() * 32;
   p.chunk = (int)std::max<long long>(1, std::min<long long>(passes, p.T * passes / want));
   p.chunks = (passes + p.chunk - 1) / p.chunk;
-  const long long grid = (p.T * p.chunks + kWarps - 1) / kWarps;
-  if (grid > 2147483647ll) return set_error(PU_ERR_UNSUPPORTED, "too many rows for one launch");
+  const long long grid = std::min<long long>((p.T * p.chunks + kWarps - 1) / kWarps, (long long)sm_count() * kFwdCtasPerSm);
   const bool wide = lanes_of(p.D) == 8;
   auto* k = wide ? (inter ? fwd_kernel<T, 8, true, kAppend> : fwd_kernel<T, 8, false, kAppend>)
                  : (inter ? fwd_kernel<T, 4, true, kAppend> : fwd_kernel<T, 4, false, kAppend>);

@@ -152,21 +152,29 @@ def check(code: int, where: str) -> None:
         raise PuError(code, where, msg.decode() if msg else "")
 
 
+# handle of a device's current stream (the public call builds a Stream object
+# first, which costs more than a small kernel's launch)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 class on_device:
     """Makes `device` current where it is not and gives the handle of its
     current stream: `with on_device(t.device) as stream`."""
 
-    __slots__ = ("device", "before")
+    __slots__ = ("index", "before")
 
     def __init__(self, device: torch.device):
-        self.device = device
+        self.index = device.index
 
     def __enter__(self) -> int:
         now = torch.cuda.current_device()
-        self.before = None if now == self.device.index else now
-        if self.before is not None:
-            torch.cuda.set_device(self.device)
-        return torch.cuda.current_stream(self.device).cuda_stream
+        if now == self.index:
+            self.before = None
+        else:
+            self.before = now
+            torch.cuda.set_device(self.index)
+        return _raw_stream(self.index)
 
     def __exit__(self, *exc) -> None:
         if self.before is not None:

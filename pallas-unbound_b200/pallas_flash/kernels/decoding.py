@@ -75,8 +75,10 @@ class DecodeWorkspace:
             buf = torch.empty(max(nbytes, cls._COUNTERS), dtype=torch.uint8, device=device)
             buf[:cls._COUNTERS].zero_()
             return buf
-        stream = torch.cuda.current_stream(device).cuda_stream
-        key = (device.index, stream)
+        key = (device.index, _lib._raw_stream(device.index))
+        buf = cls._cache.get(key)
+        if buf is not None and buf.numel() >= nbytes:
+            return buf
         with cls._lock:
             buf = cls._cache.get(key)
             if buf is None or buf.numel() < nbytes:

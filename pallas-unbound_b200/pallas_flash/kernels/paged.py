@@ -26,6 +26,7 @@ into a CUDA graph and replayed.
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import NamedTuple, Optional, Sequence
 
@@ -50,9 +51,16 @@ def _check_pool(k_pool: torch.Tensor, v_pool: torch.Tensor, page_table: torch.Te
         raise ValueError("page_table must be int32 [B, max_pages_per_seq]")
     if kv_lens.dtype != torch.int32 or kv_lens.numel() != page_table.shape[0]:
         raise ValueError("kv_lens must be int32 [B]")
-    for t in (k_pool, v_pool, page_table, kv_lens):
-        if not t.is_cuda or not t.is_contiguous() or t.device != k_pool.device:
-            raise ValueError("pools, page table and lengths must be contiguous CUDA tensors on one device")
+    dev = k_pool.device
+    if not (k_pool.is_cuda and v_pool.device == dev and page_table.device == dev and kv_lens.device == dev
+            and k_pool.is_contiguous() and v_pool.is_contiguous() and page_table.is_contiguous()
+            and kv_lens.is_contiguous()):
+        raise ValueError("pools, page table and lengths must be contiguous CUDA tensors on one device")
+
+
+@functools.lru_cache(maxsize=256)
+def _gqa_bytes(device: int, B: int, H: int, H_kv: int, max_pages: int, page_size: int, D: int) -> int:
+    return int(_lib.lib().pu_decode_paged_gqa_workspace_size(B, H, H_kv, max_pages, page_size, D))
 
 
 def paged_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
@@ -90,8 +98,7 @@ def paged_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
                                            lse.data_ptr(), ws.data_ptr(), ws.numel(), B, H, D,
                                            float(sm_scale), stream), "pu_decode_paged")
         else:
-            need = int(lib.pu_decode_paged_gqa_workspace_size(B, H, H_kv, max_pages, page_size, D))
-            ws = DecodeWorkspace.get(q.device, need)
+            ws = DecodeWorkspace.get(q.device, _gqa_bytes(q.device.index, B, H, H_kv, max_pages, page_size, D))
             _lib.check(lib.pu_decode_paged_gqa(q.data_ptr(), _DT[q.dtype], k_pool.data_ptr(),
                                                v_pool.data_ptr(), _DT_KV[k_pool.dtype],
                                                page_table.data_ptr(), max_pages, P, page_size,
@@ -154,17 +161,19 @@ def plan_append(page_table: torch.Tensor, kv_lens: torch.Tensor, new_lens: torch
         raise ValueError("page_table must be int32 [B, max_pages_per_seq]")
     B, max_pages = page_table.shape
     dev = page_table.device
-    for name, t, dt, shape in (("kv_lens", kv_lens, torch.int32, (B,)), ("new_lens", new_lens, torch.int32, (B,)),
-                               ("cursor", cursor, torch.int64, (2,))):
-        if t.dtype != dt or t.shape != shape:
-            raise ValueError(f"{name} must be {dt} {list(shape)}")
+    if kv_lens.dtype != torch.int32 or new_lens.dtype != torch.int32 or kv_lens.shape != (B,) or new_lens.shape != (B,):
+        raise ValueError(f"kv_lens and new_lens must be int32 [{B}]")
+    if cursor.dtype != torch.int64 or cursor.shape != (2,):
+        raise ValueError("cursor must be int64 [2]")
     if free_ring.dim() != 1 or free_ring.dtype != torch.int32:
         raise ValueError("free_ring must be int32 [num_pages]")
-    if release is not None and (release.dtype not in (torch.bool, torch.uint8) or release.shape != (B,)):
-        raise ValueError("release must be bool [B]")
-    for t in (page_table, kv_lens, new_lens, free_ring, cursor) + (() if release is None else (release,)):
-        if not t.is_cuda or not t.is_contiguous() or t.device != dev:
-            raise ValueError("the plan's tensors must be contiguous CUDA tensors on one device")
+    if not (page_table.is_cuda and kv_lens.device == dev and new_lens.device == dev and free_ring.device == dev
+            and cursor.device == dev and page_table.is_contiguous() and kv_lens.is_contiguous()
+            and new_lens.is_contiguous() and free_ring.is_contiguous() and cursor.is_contiguous()):
+        raise ValueError("the plan's tensors must be contiguous CUDA tensors on one device")
+    if release is not None and (release.dtype not in (torch.bool, torch.uint8) or release.shape != (B,)
+                                or release.device != dev or not release.is_contiguous()):
+        raise ValueError(f"release must be a contiguous bool [{B}] on {dev}")
     if inplace and new_lens.data_ptr() == kv_lens.data_ptr():
         raise ValueError("new_lens must not be kv_lens when they are advanced in place")
     T = int(num_tokens)
@@ -212,13 +221,14 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, inv_f
         raise TypeError("q, k and v must share one dtype: bf16, fp16 or fp32")
     if slots.dtype != torch.int32 or slots.shape != (T,) or not slots.is_contiguous():
         raise ValueError("slots must be a contiguous int32 [T]")
-    if not q.is_cuda or any(t.device != dev for t in (k, v, slots, k_pool, v_pool)):
+    if not (q.is_cuda and k.device == dev and v.device == dev and slots.device == dev and k_pool.device == dev
+            and v_pool.device == dev):
         raise ValueError("q, k, v, slots and pools must be CUDA tensors on one device")
     if not k_pool.is_contiguous() or not v_pool.is_contiguous():
         raise ValueError("pools must be contiguous")
     if D % 16 or not 16 <= D <= 128 or H == 0 or H_kv == 0:
         raise ValueError(f"{H} and {H_kv} heads of size {D} (at least one head, a multiple of 16 up to 128)")
-    if any(t.requires_grad for t in (q, k, v)) and torch.is_grad_enabled():
+    if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
         raise ValueError("qk_norm_rope_append writes a cache and has no gradient")
     wq, wk = _check_weight(q_weight, D, dev, "q_weight"), _check_weight(k_weight, D, dev, "k_weight")
     if positions is None:

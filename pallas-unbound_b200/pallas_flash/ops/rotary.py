@@ -48,13 +48,19 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, device=None) -> 
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
-    """`t`, or a dense copy where a kernel cannot read its rows in 16-byte vectors."""
-    unit = 16 // t.element_size()
-    st = t.stride()
-    ok = st[-1] == 1 and t.data_ptr() % 16 == 0
-    for i in range(t.dim() - 1):
-        ok = ok and (st[i] % unit == 0 or t.shape[i] <= 1)
-    return t if ok else t.clone(memory_format=torch.contiguous_format)
+    """`t`, or a dense copy where a kernel cannot read its rows in 16-byte vectors
+    (rows are a multiple of 16 elements)."""
+    if t.data_ptr() % 16 == 0:
+        if t.is_contiguous():
+            return t
+        unit, st, shape = 16 // t.element_size(), t.stride(), t.shape
+        ok = st[-1] == 1
+        for i in range(len(st) - 1):
+            if st[i] % unit and shape[i] > 1:
+                ok = False
+        if ok:
+            return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _check_weight(w, D: int, device, name: str):
