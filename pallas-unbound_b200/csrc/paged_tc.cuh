@@ -20,17 +20,26 @@
 // most two of them, so the workspace is a few MB whatever the batch.  No CTA
 // waits for another.
 //
-// Roles (352 threads):
+// Roles (512 threads, registers shared out with setmaxnreg):
 //   warps 0-7   two softmax groups; group t & 1 takes tile t, each with its
 //               own running maximum, sums and accumulator (row r of the tile
-//               = TMEM lane r = thread r; at the end of a segment both add
-//               up).  One group alone left the tensor core and the loads
-//               waiting on e4m3 tiles, whose softmax takes longer than their
-//               bytes.
-//   warp 8      page table lookups and TMA loads, lane i page box i
-//   warp 9      tcgen05 issue, S and P V products as each becomes ready
+//               = TMEM lane r = thread r).  One group alone left the tensor
+//               core and the loads waiting on e4m3 tiles, whose softmax takes
+//               longer than their bytes.
+//   warp 8      page table lookups and TMA loads
+//   warp 9      tcgen05 issue of the S products; also owns the TMEM
 //   warp 10     queries of the next segments into shared memory (e4m3: scaled
 //               by a power of two and split into parts)
+//   warp 11     tcgen05 issue of the P V products
+//   warps 12-15 the end of each segment: both groups' accumulators and sums
+//               into the output or a record, and the joins.  The accumulators
+//               are double buffered over segments, so the softmax groups go on
+//               with the next sequence at once (done by them, the end took
+//               longer than two tiles: 2048 sequences of 128 tokens 107 us).
+// One thread issues, elected with elect.sync inside a warp-uniform branch:
+// that tells the compiler that a single thread runs there.  Behind
+// `lane == 0` it wraps each tensor or TMA instruction in a loop over the active
+// lanes, and a product of 40 clocks took 154 to issue.
 // K/V tiles run through one ring across segments, so a new sequence's first
 // pages are on their way while the previous one ends.
 //
@@ -56,8 +65,11 @@ constexpr int BT = 128;                    // cache rows per tile (MMA M)
 constexpr int NP = 16;                     // query heads per slice (MMA N per part)
 constexpr int kGroups = 2;                 // softmax groups of 128 threads
 constexpr int kSoftmax = kGroups * 128;
-constexpr int kLoadWarp = 8, kMmaWarp = 9, kQueryWarp = 10;
-constexpr int kCtaThreads = 352;
+constexpr int kLoadWarp = 8, kScoreWarp = 9, kQueryWarp = 10, kValueWarp = 11;
+constexpr int kEndWarps = 12;               // first of four
+constexpr int kCtaThreads = 512;
+// registers a thread: softmax 256 x 160, roles 128 x 72, ends 128 x 120 = the launch's 512 x 128
+constexpr int kSoftmaxRegs = 160, kRoleRegs = 72, kEndRegs = 120;
 constexpr int kQSlots = 4;
 constexpr int kHead = 4;                   // floats before o in a record: m, l, and two that keep o 16-byte aligned
 
@@ -85,20 +97,22 @@ struct Cfg {
   static constexpr int kOffQ = NS * 2 * kTile;
   static constexpr int kOffP = kOffQ + kQSlots * kQBytes;
   static constexpr int kOffBar = kOffP + kGroups * kPBytes;
-  // full[NS], empty[NS], qfull[4], qfree[4], sfull[4], pfull[2], pvdone[2], ofree, drain
-  static constexpr int kBars = 2 * NS + 2 * kQSlots + 4 + 2 * kGroups + 2;
-  static constexpr int kOffMisc = kOffBar + kBars * 8;     // tmem base, abort flag, last-CTA flag
+  // full[NS], empty[NS], qfull[4], qfree[4], sfull[4], sfree[4], pfull[2], pvdone[2], sums[2], odone[2], ofree[2], drain[2]
+  static constexpr int kBars = 2 * NS + 2 * kQSlots + 8 + 2 * kGroups + 8;
+  static constexpr int kOffMisc = (kOffBar + kBars * 8 + 15) / 16 * 16;   // tmem base, abort flag, last-CTA flag
   static constexpr int kOffBad = kOffMisc + 16;            // [NS] boxes of the stage that were not loaded
-  static constexpr int kOffMax = kOffBad + 32;             // [2 groups][4 warps][NP] tile maxima
-  static constexpr int kOffM = kOffMax + kGroups * 4 * NP * 4;   // [2 parities][2 groups][NP]
+  static constexpr int kOffMax = kOffBad + 32;             // [2 groups][2][4 warps][NP] tile maxima
+  static constexpr int kOffM = kOffMax + kGroups * 2 * 4 * NP * 4;   // [2 parities][2 groups][NP]
   static constexpr int kOffL = kOffM + 2 * kGroups * NP * 4;     // [2 parities][2 groups][4 warps][NP]
-  static constexpr int kOffQinv = kOffL + 2 * kGroups * 4 * NP * 4;   // [4 slots][NP]
+  static constexpr int kOffFac = kOffL + 2 * kGroups * 4 * NP * 4;    // [4 warps][2 groups][NP]
+  static constexpr int kOffQinv = kOffFac + 4 * 2 * NP * 4;           // [4 slots][NP]
   static constexpr int kSmem = kOffQinv + kQSlots * NP * 4;
   static constexpr int kSCols = kQParts * NP, kOCols = kPParts * NP;
-  static constexpr int kColO = 4 * kSCols;                 // four S buffers, then an accumulator per group
-  static constexpr int kCols = kColO + kGroups * kOCols;
+  static constexpr int kColO = 4 * kSCols;                 // four S buffers, then two accumulators per group
+  static constexpr int kCols = kColO + 2 * kGroups * kOCols;
   static constexpr uint32_t kTmemCols = kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
   static_assert(kSmem <= 232448, "shared memory of one CTA");
+  static_assert(kOffBar % 8 == 0 && kOffMax % 16 == 0, "barriers, and maxima that are read as float4");
 };
 
 struct Params {
@@ -138,7 +152,7 @@ __device__ __forceinline__ void split_e4m3(float a, float b, uint16_t (&part)[N]
 // K/V head * slices + slice); a segment is the CTA's run of one item's tiles.
 struct Walk {
   const Params* p;
-  int b, r, t, tiles, inner, left, seg, loc;
+  int b, r, t, tiles, len, inner, left, seg, loc;
   __device__ __forceinline__ int len_of(int i) const {
     const int n = p->lens[i], cap = p->max_pages << p->page_shift;
     return n < 0 ? 0 : n > cap ? cap : n;
@@ -156,32 +170,37 @@ struct Walk {
     ++seg;
     if (++r < inner) return;
     r = 0;
-    do tiles = tiles_of(++b);
-    while (tiles == 0);
+    do len = len_of(++b);
+    while (len == 0);
+    tiles = (len + BT - 1) / BT;
   }
 };
 
-// Sum of the warp's 16 values per lane over its 32 lanes: lanes 2 h and 2 h + 1
-// return head h's sum (each step halves the values a lane still holds).
-__device__ __forceinline__ float sum16(const float (&v)[NP], int lane) {
+// Sum or maximum of the warp's 16 values per lane over its 32 lanes: lanes 2 h
+// and 2 h + 1 return head h's (each step halves the values a lane still holds).
+template <bool kMax>
+__device__ __forceinline__ float join(float a, float b) { return kMax ? fmaxf(a, b) : a + b; }
+
+template <bool kMax>
+__device__ __forceinline__ float reduce16(const float (&v)[NP], int lane) {
   float a[8], b[4], c[2], d;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float keep = lane & 16 ? v[i + 8] : v[i], give = lane & 16 ? v[i] : v[i + 8];
-    a[i] = keep + __shfl_xor_sync(0xffffffffu, give, 16);
+    a[i] = join<kMax>(keep, __shfl_xor_sync(0xffffffffu, give, 16));
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float keep = lane & 8 ? a[i + 4] : a[i], give = lane & 8 ? a[i] : a[i + 4];
-    b[i] = keep + __shfl_xor_sync(0xffffffffu, give, 8);
+    b[i] = join<kMax>(keep, __shfl_xor_sync(0xffffffffu, give, 8));
   }
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const float keep = lane & 4 ? b[i + 2] : b[i], give = lane & 4 ? b[i] : b[i + 2];
-    c[i] = keep + __shfl_xor_sync(0xffffffffu, give, 4);
+    c[i] = join<kMax>(keep, __shfl_xor_sync(0xffffffffu, give, 4));
   }
-  d = (lane & 2 ? c[1] : c[0]) + __shfl_xor_sync(0xffffffffu, lane & 2 ? c[0] : c[1], 2);
-  return d + __shfl_xor_sync(0xffffffffu, d, 1);
+  d = join<kMax>(lane & 2 ? c[1] : c[0], __shfl_xor_sync(0xffffffffu, lane & 2 ? c[0] : c[1], 2));
+  return join<kMax>(d, __shfl_xor_sync(0xffffffffu, d, 1));
 }
 
 template <typename T, typename KVT, int D>
@@ -205,10 +224,13 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
   uint64_t* bQfull = bEmpty + NS;        // [4] queries of segment s in slot s & 3
   uint64_t* bQfree = bQfull + kQSlots;   // [4] its products (and scales, e4m3) have been read
   uint64_t* bSf = bQfree + kQSlots;      // [4] S of tile t in buffer t & 3
-  uint64_t* bPf = bSf + 4;               // [2] P of the group's tile written (128 arrivals)
+  uint64_t* bSfree = bSf + 4;            // [4] read into registers (an arrival per warp)
+  uint64_t* bPf = bSfree + 4;            // [2] P of the group's tile written (128 arrivals)
   uint64_t* bPv = bPf + kGroups;         // [2] the group's P V product done
-  uint64_t* bOfree = bPv + kGroups;      // both accumulators of a segment read (256 arrivals)
-  uint64_t* bDrain = bOfree + 1;
+  uint64_t* bSums = bPv + kGroups;       // [2] maxima and sums of segment s in buffer s & 1 (an arrival per warp)
+  uint64_t* bOdone = bSums + 2;          // [2] its products done
+  uint64_t* bOfree = bOdone + 2;         // [2] its accumulators and sums read (128 arrivals)
+  uint64_t* bDrain = bOfree + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kOffMisc + 4);
   int* s_last = reinterpret_cast<int*>(smem + C::kOffMisc + 8);
@@ -216,6 +238,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
   float* s_max = reinterpret_cast<float*>(smem + C::kOffMax);
   float* s_m = reinterpret_cast<float*>(smem + C::kOffM);
   float* s_l = reinterpret_cast<float*>(smem + C::kOffL);
+  float* s_fac = reinterpret_cast<float*>(smem + C::kOffFac);
   float* s_qinv = reinterpret_cast<float*>(smem + C::kOffQinv);
 
   if (tid == 0) {
@@ -227,17 +250,23 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
       mbar_init(bQfull + s, 32);
       mbar_init(bQfree + s, kF8 ? 1 + kGroups : 1);
       mbar_init(bSf + s, 1);
+      mbar_init(bSfree + s, 4);
     }
     for (int g = 0; g < kGroups; ++g) {
       mbar_init(bPf + g, 128);
       mbar_init(bPv + g, 1);
     }
-    mbar_init(bOfree, kSoftmax);
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(bSums + g, kSoftmax / 32);
+      mbar_init(bOdone + g, 1);
+      mbar_init(bOfree + g, 128);
+    }
     mbar_init(bDrain, 1);
+    mbar_init(bDrain + 1, 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == kMmaWarp) {
+  if (warp == kScoreWarp) {
     tmem_alloc(tmem_slot, C::kTmemCols);
     tmem_relinquish();
   }
@@ -263,12 +292,12 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
   const bool busy = blockIdx.x < ctas;
   const long long first = busy ? blockIdx.x * all / ctas : 0;
   w0.left = busy ? (int)((blockIdx.x + 1ll) * all / ctas - first) : 0;
-  w0.b = w0.r = w0.t = w0.tiles = w0.seg = w0.loc = 0;
+  w0.b = w0.r = w0.t = w0.tiles = w0.len = w0.seg = w0.loc = 0;
   long long item0 = 0;                   // number of the current sequence's first tile
   if (w0.left > 0) {
     long long before = 0;
     for (int i0 = 0;; i0 += 32) {
-      const int n = i0 + lane < p.B ? w0.tiles_of(i0 + lane) : 0;
+      const int len = i0 + lane < p.B ? w0.len_of(i0 + lane) : 0, n = (len + BT - 1) / BT;
       long long x = n;
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
@@ -280,6 +309,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
         const int src = __ffs(hit) - 1;
         w0.b = i0 + src;
         w0.tiles = __shfl_sync(0xffffffffu, n, src);
+        w0.len = __shfl_sync(0xffffffffu, len, src);
         item0 = (before + __shfl_sync(0xffffffffu, x, src) - w0.tiles) * w0.inner;
         break;
       }
@@ -294,57 +324,70 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
+  if (warp >= kSoftmax / 32 && warp < kEndWarps) {
+  reg_dealloc<kRoleRegs>();
   if (warp == kLoadWarp) {
     // ---------------- pages -> ring ----------------
-    // The table is read kAhead tiles before its use (lane i: box i's entry),
-    // or each tile would wait for its entries before its loads could leave.
-    constexpr int kAhead = 4;
-    const int boxes = BT / p.box, per_page = 1 << p.page_shift;
-    Walk wl = w0;                          // the tile whose entries are read next
-    int ahead[kAhead];
+    // The table is read for up to 8 tiles of a segment at a time (lane j * boxes
+    // + i: box i of the j-th), two such batches ahead, or each tile's loads
+    // would wait for its entries first.
+    const int box_shift = 31 - __clz(p.box), boxes = BT >> box_shift, batch = min(32 / boxes, 8);
+    const int lane_tile = lane / boxes, lane_row = (lane & (boxes - 1)) << box_shift, per_page = 1 << p.page_shift;
+    Walk wl = w0;                          // the first tile of the next batch
     auto look_up = [&]() -> int {
-      int pg = 0;
-      if (wl.left > 0) {
-        const int row = wl.t * BT + lane * p.box;
-        if (lane < boxes && row < wl.len_of(wl.b)) pg = p.table[(size_t)wl.b * p.max_pages + (row >> p.page_shift)];
-        wl.next();
-      }
+      const int cnt = min(min(wl.left, wl.tiles - wl.t), batch);
+      const int row = (wl.t + lane_tile) * BT + lane_row;
+      const int32_t* at = p.table + (size_t)wl.b * p.max_pages + (row >> p.page_shift);
+      int pg = -1;
+      asm volatile("{\n .reg .pred q;\n setp.ne.b32 q, %2, 0;\n @q ld.global.b32 %0, [%1];\n}"
+                   : "+r"(pg) : "l"(at), "r"((int)(lane_tile < cnt && row < wl.len)));
+      if (cnt > 0) wl.next(cnt);
       return pg;
     };
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) ahead[i] = look_up();
-    int n = 0;
-    for (Walk w = w0; w.left > 0; w.next(), ++n) {
-      const int s = n % NS, len = w.len_of(w.b);
-      const int row = w.t * BT + lane * p.box, pg = ahead[0];
-#pragma unroll
-      for (int i = 0; i + 1 < kAhead; ++i) ahead[i] = ahead[i + 1];
-      ahead[kAhead - 1] = look_up();
-      const bool mine = lane < boxes && row < len;
+    int entries = 0, next1 = look_up(), next2 = look_up();
+    int n = 0, j = 0, cnt = 0, s = 0, turn = 0, seg = -1, head = 0;   // stage s for the turn-th time
+    for (Walk w = w0; w.left > 0; w.next(), ++n, ++j) {
+      if (j == cnt) {
+        j = 0;
+        cnt = min(min(w.left, w.tiles - w.t), batch);
+        entries = next1;
+        next1 = next2;
+        next2 = look_up();
+      }
+      if (w.seg != seg) {
+        seg = w.seg;
+        head = w.r / p.slices;
+      }
+      const int pg = __shfl_sync(0xffffffffu, entries, (j * boxes + lane) & 31), row0 = w.t * BT;
+      const bool mine = lane < boxes && row0 + lane_row < w.len;
       const bool good = mine && (unsigned)pg < (unsigned)p.num_pages;
       if (mine && !good) record_device_error(PU_ERR_INVALID_ARGUMENT, kSiteDecodePage);
       const unsigned loaded = __ballot_sync(0xffffffffu, good);
-      if (n >= NS && !mbar_wait(bEmpty + s, (n / NS - 1) & 1, abort_flag, kSiteDecodeTc)) break;
+      const int outer = pg * p.H_kv + head, in = p.box < BT ? 0 : row0 & (per_page - 1);
+      if (turn > 0 && !mbar_wait(bEmpty + s, (turn - 1) & 1, abort_flag, kSiteDecodeTc)) break;
       __syncwarp();
-      uint8_t* dV = sKV + s * 2 * kTile + lane * p.box * 128;
-      uint8_t* dK = dV + kTile;
-      if (lane == 0) {
+      if (elect_one_sync()) {
         s_bad[s] = ~loaded;
         mbar_arrive_expect_tx(bFull + s, (uint32_t)__popc(loaded) * 2 * p.box * C::kRowBytes);
       }
-      __syncwarp();
-      if (good) {
-        const int outer = pg * p.H_kv + w.r / p.slices, in = row & (per_page - 1);
-        constexpr int cols = kF8 ? 128 : 64;
+      uint8_t* dV = sKV + s * 2 * kTile;
+      for (int i = 0; i < boxes; ++i, dV += p.box * 128) {
+        const int at = __shfl_sync(0xffffffffu, outer, i);
+        if (!((loaded >> i) & 1u)) continue;
+        if (elect_one_sync()) {
+          constexpr int cols = kF8 ? 128 : 64;
 #pragma unroll
-        for (int cb = 0; cb < C::kBlocks; ++cb) tma_load_3d(dK + cb * BT * 128, &tmK, bFull + s, cb * cols, in, outer);
+          for (int cb = 0; cb < C::kBlocks; ++cb) tma_load_3d(dV + kTile + cb * BT * 128, &tmK, bFull + s, cb * cols, in, at);
 #pragma unroll
-        for (int cb = 0; cb < C::kBlocks; ++cb) tma_load_3d(dV + cb * BT * 128, &tmV, bFull + s, cb * cols, in, outer);
+          for (int cb = 0; cb < C::kBlocks; ++cb) tma_load_3d(dV + cb * BT * 128, &tmV, bFull + s, cb * cols, in, at);
+        }
       }
-      __syncwarp();
+      if (++s == NS) {
+        s = 0;
+        ++turn;
+      }
     }
-    // copies still in flight land before the CTA may exit (after an abort the
-    // ring may stop anywhere: the last NS issued tiles are the ones in flight)
+    // copies still in flight land before the CTA may exit
     volatile int no_abort = 0;
     for (int i = max(0, n - NS); i < n; ++i) mbar_wait(bFull + i % NS, (i / NS) & 1, &no_abort, kSiteDecodeTc);
   } else if (warp == kQueryWarp) {
@@ -405,97 +448,89 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
       fence_proxy_async_smem();
       mbar_arrive(bQfull + slot);
     }
-  } else if (warp == kMmaWarp) {
-    // ---------------- tcgen05 issuer ----------------
-    if (lane == 0) {
+  } else if (warp == kScoreWarp) {
+    // ---------------- tcgen05: S products ----------------
+    if (elect_one_sync()) {
       constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
       constexpr uint32_t idS = kF8 ? make_idesc_e4m3(BT, C::kSCols, 0, 0) : make_idesc_16(BT, NP, 0, 0, kBf16);
-      constexpr uint32_t idO = kF8 ? make_idesc_e4m3(128, C::kOCols, 1, 0) : make_idesc_16(128, NP, 1, 0, kBf16);
       const uint64_t dQ0 = make_sdesc_sw128(smem_u32(sQ), 16, 1024);
-      const uint64_t dP0 = make_sdesc_sw128(smem_u32(sP), 16, 1024);
-      // D = 64: M is still 128, with the K tile's 64 columns behind V's as
-      // the other half; its rows of the accumulator are never read
-      const uint64_t dV0 = make_sdesc_sw128(smem_u32(sKV), D == 64 ? kTile : BT * 128, 1024);
       const uint64_t dK0 = make_sdesc_sw128(smem_u32(sKV + kTile), 16, 1024);
-      Walk ws = w0, wp = w0;
-      int js = 0, jp = 0;                  // next S product, next P V product
-      uint64_t t_last = global_timer_ns();
-      while (wp.left > 0) {
-        bool progressed = false;
-        // S of tile js overwrites the buffer of tile js - 4, read once that
-        // tile's P was written, so once its P V product was issued
-        if (ws.left > 0 && js < jp + 4 && mbar_test_wait(bFull + js % NS, (js / NS) & 1) &&
-            (ws.loc > 0 || mbar_test_wait(bQfull + (ws.seg & 3), (ws.seg >> 2) & 1))) {
-          tc_fence_after();
-          const uint64_t dk = sdesc_add(dK0, (js % NS) * 2 * kTile), dq = sdesc_add(dQ0, (ws.seg & 3) * C::kQBytes);
-          const uint32_t col = tmem + (js & 3) * C::kSCols;
-          if constexpr (kF8) {
+      int t = 0;
+      for (Walk w = w0; w.left > 0; w.next(), ++t) {
+        const int slot = w.seg & (kQSlots - 1), buf = t & 3;
+        if (w.loc == 0 && !mbar_wait(bQfull + slot, (w.seg / kQSlots) & 1, abort_flag, kSiteDecodeTc)) break;
+        if (t >= 4 && !mbar_wait(bSfree + buf, ((t >> 2) - 1) & 1, abort_flag, kSiteDecodeTc)) break;
+        if (!mbar_wait(bFull + t % NS, (t / NS) & 1, abort_flag, kSiteDecodeTc)) break;
+        tc_fence_after();
+        const uint64_t dk = sdesc_add(dK0, (t % NS) * 2 * kTile), dq = sdesc_add(dQ0, slot * C::kQBytes);
+        const uint32_t col = tmem + buf * C::kSCols;
+        if constexpr (kF8) {
 #pragma unroll
-            for (int kk = 0; kk < D / 32; ++kk) mma_ss_f8(col, sdesc_add(dk, kk * 32), sdesc_add(dq, kk * 32), idS, kk > 0);
-          } else {
-#pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk)
-              mma_ss(col, sdesc_add(dk, (kk >> 2) * (BT * 128) + (kk & 3) * 32),
-                     sdesc_add(dq, (kk >> 2) * C::kQBlock + (kk & 3) * 32), idS, kk > 0);
-          }
-          mma_commit(bSf + (js & 3));
-          if (ws.last()) mma_commit(bQfree + (ws.seg & 3));
-          ws.next();
-          ++js;
-          progressed = true;
-        }
-        if (jp < js && mbar_test_wait(bPf + (jp & 1), (jp >> 1) & 1) &&
-            (wp.loc > 0 || wp.seg == 0 || mbar_test_wait(bOfree, (wp.seg - 1) & 1))) {
-          tc_fence_after();
-          const uint64_t dv = sdesc_add(dV0, (jp % NS) * 2 * kTile), dp = sdesc_add(dP0, (jp & 1) * C::kPBytes);
-          const uint32_t col = tmem + C::kColO + (jp & 1) * C::kOCols;
-          const bool more = wp.loc >= kGroups;   // the group's accumulator already holds tiles of this segment
-          if constexpr (kF8) {
-#pragma unroll
-            for (int kk = 0; kk < BT / 32; ++kk)
-              mma_ss_f8(col, sdesc_add(dv, kk * 32 * 128), sdesc_add(dp, kk * 32), idO, more || kk > 0);
-          } else {
-#pragma unroll
-            for (int kk = 0; kk < BT / 16; ++kk)
-              mma_ss(col, sdesc_add(dv, kk * 16 * 128), sdesc_add(dp, (kk >> 2) * C::kQBlock + (kk & 3) * 32), idO,
-                     more || kk > 0);
-          }
-          mma_commit(bPv + (jp & 1));
-          mma_commit(bEmpty + jp % NS);
-          wp.next();
-          ++jp;
-          progressed = true;
-        }
-        if (progressed) {
-          t_last = global_timer_ns();
+          for (int kk = 0; kk < D / 32; ++kk) mma_ss_f8(col, sdesc_add(dk, kk * 32), sdesc_add(dq, kk * 32), idS, kk > 0);
         } else {
-          if (*abort_flag) break;
-          if (global_timer_ns() - t_last > kWaitTimeoutNs) {
-            *abort_flag = 1;
-            record_device_error(PU_ERR_DEVICE_TIMEOUT, kSiteDecodeTc);
-            break;
-          }
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk)
+            mma_ss(col, sdesc_add(dk, (kk >> 2) * (BT * 128) + (kk & 3) * 32),
+                   sdesc_add(dq, (kk >> 2) * C::kQBlock + (kk & 3) * 32), idS, kk > 0);
         }
+        mma_commit(bSf + buf);
+        if (w.last()) mma_commit(bQfree + slot);
       }
       // every issued product completes before TMEM and shared memory go away
       mma_commit(bDrain);
       volatile int no_abort = 0;
       mbar_wait(bDrain, 0, &no_abort, kSiteDecodeTc);
     }
-  } else {
+  } else if (warp == kValueWarp) {
+    // ---------------- tcgen05: P V products ----------------
+    if (elect_one_sync()) {
+      constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+      constexpr uint32_t idO = kF8 ? make_idesc_e4m3(128, C::kOCols, 1, 0) : make_idesc_16(128, NP, 1, 0, kBf16);
+      const uint64_t dP0 = make_sdesc_sw128(smem_u32(sP), 16, 1024);
+      // D = 64: M is still 128, with the K tile's 64 columns behind V's as
+      // the other half; its rows of the accumulator are never read
+      const uint64_t dV0 = make_sdesc_sw128(smem_u32(sKV), D == 64 ? kTile : BT * 128, 1024);
+      int t = 0;
+      for (Walk w = w0; w.left > 0; w.next(), ++t) {
+        const int grp = t & 1;
+        const int par = w.seg & 1;
+        if (w.loc == 0 && w.seg > 1 && !mbar_wait(bOfree + par, ((w.seg >> 1) - 1) & 1, abort_flag, kSiteDecodeTc)) break;
+        if (!mbar_wait(bPf + grp, (t >> 1) & 1, abort_flag, kSiteDecodeTc)) break;
+        tc_fence_after();
+        const uint64_t dv = sdesc_add(dV0, (t % NS) * 2 * kTile), dp = sdesc_add(dP0, grp * C::kPBytes);
+        const uint32_t col = tmem + C::kColO + (par * kGroups + grp) * C::kOCols;
+        const bool more = w.loc >= kGroups;    // the group's accumulator already holds tiles of this segment
+        if constexpr (kF8) {
+#pragma unroll
+          for (int kk = 0; kk < BT / 32; ++kk)
+            mma_ss_f8(col, sdesc_add(dv, kk * 32 * 128), sdesc_add(dp, kk * 32), idO, more || kk > 0);
+        } else {
+#pragma unroll
+          for (int kk = 0; kk < BT / 16; ++kk)
+            mma_ss(col, sdesc_add(dv, kk * 16 * 128), sdesc_add(dp, (kk >> 2) * C::kQBlock + (kk & 3) * 32), idO, more || kk > 0);
+        }
+        mma_commit(bPv + grp);
+        mma_commit(bEmpty + t % NS);
+        if (w.last()) mma_commit(bOdone + par);
+      }
+      mma_commit(bDrain + 1);
+      volatile int no_abort = 0;
+      mbar_wait(bDrain + 1, 0, &no_abort, kSiteDecodeTc);
+    }
+  }
+  } else if (warp < kSoftmax / 32) {
+    reg_alloc<kSoftmaxRegs>();
     // ---------------- softmax groups ----------------
     const int grp = warp >> 2, row = tid & 127, w4 = warp & 3;
     const uint32_t lane_base = static_cast<uint32_t>(w4 * 32) << 16;
-    float* gmax = s_max + grp * 4 * NP;
     uint8_t* myP = sP + grp * C::kPBytes;
     const int box_shift = 31 - __clz(p.box);
     int t = 0, mine = 0;                   // tiles of the CTA so far, of this group
     Walk w = w0;
     while (w.left > 0) {
       // ---- one segment ----
-      const int seg = w.seg, b = w.b, r = w.r, t0 = w.t, tiles = w.tiles;
-      const int n = min(w.left, tiles - t0), len = w.len_of(b);
-      const int slice = r % p.slices, G = min(NP, p.group - slice * NP);
+      const int seg = w.seg, par = seg & 1, t0 = w.t, n = min(w.left, w.tiles - t0), len = w.len;
+      const int slice = p.slices == 1 ? 0 : w.r % p.slices, G = min(NP, p.group - slice * NP);
       float qf = p.scale_log2, qs[NP];     // e4m3: a factor per head undoes the query's scale
       if constexpr (kF8) {
         const int slot = seg & 3;
@@ -527,6 +562,9 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
           tmem_wait_ld();
 #pragma unroll
           for (int k = 0; k < kQParts; ++k) reg_fence(raw[k]);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bSfree + buf);
 #pragma unroll
           for (int h = 0; h < NP; ++h) {
             float x = __uint_as_float(raw[0][h]);
@@ -535,41 +573,55 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
             s[h] = valid ? x * (kF8 ? qs[h] : qf) : -INFINITY;
           }
         }
+        // Heads are taken four at a time: a branch for each would put their
+        // chains of instructions one behind the other.
+        const bool fresh = i < kGroups;    // the group's first tile of the segment
         bool up = false;
+        if (!fresh) {
 #pragma unroll
-        for (int h = 0; h < NP; ++h)
-          if (h < G) up |= s[h] > m[h] + (C::kShift + C::kRescale);
-        if (bar_any_named(1 + grp, 128, up)) {
-          // the tile's maximum of each head over its 128 rows
-#pragma unroll
-          for (int h = 0; h < NP; ++h) {
-            if (h >= G) break;
-            float v = s[h];
-#pragma unroll
-            for (int off = 16; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
-            if (lane == 0) gmax[w4 * NP + h] = v;
-          }
+          for (int h = 0; h < NP; ++h) up |= h < G && s[h] > m[h] + (C::kShift + C::kRescale);
+        }
+        if (fresh || bar_any_named(1 + grp, 128, up)) {
+          // the tile's maximum of each head over its 128 rows (the buffer
+          // alternates: a slow thread may still read the previous one)
+          float* gmax = s_max + (grp * 2 + (mine & 1)) * 4 * NP;
+          const float wm = reduce16<true>(s, lane);
+          if ((lane & 1) == 0) gmax[w4 * NP + (lane >> 1)] = wm;
           bar_sync_named(1 + grp, 128);
           float alpha[NP];
 #pragma unroll
-          for (int h = 0; h < NP; ++h) {
-            alpha[h] = 1.f;
-            if (h >= G) continue;
-            const float tm = fmaxf(fmaxf(gmax[h], gmax[NP + h]), fmaxf(gmax[2 * NP + h], gmax[3 * NP + h]));
-            if (tm > m[h] + (C::kShift + C::kRescale)) {   // the same decision in every thread of the group
-              alpha[h] = m[h] == -INFINITY ? 0.f : ex2(m[h] - (tm - C::kShift));
-              m[h] = tm - C::kShift;
+          for (int h0 = 0; h0 < NP; h0 += 4) {
+            if (h0 >= G) break;
+            float4 x[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[k] = *reinterpret_cast<const float4*>(gmax + k * NP + h0);
+            const float tm[4] = {fmaxf(fmaxf(x[0].x, x[1].x), fmaxf(x[2].x, x[3].x)), fmaxf(fmaxf(x[0].y, x[1].y), fmaxf(x[2].y, x[3].y)),
+                                 fmaxf(fmaxf(x[0].z, x[1].z), fmaxf(x[2].z, x[3].z)), fmaxf(fmaxf(x[0].w, x[1].w), fmaxf(x[2].w, x[3].w))};
+#pragma unroll
+            for (int h = h0; h < h0 + 4; ++h) {
+              // the same decision in every thread of the group
+              const float mx = tm[h - h0], to = mx - C::kShift;
+              if (fresh) {
+                m[h] = to;
+              } else {
+                const bool move = mx > m[h] + (C::kShift + C::kRescale);
+                alpha[h] = !move ? 1.f : m[h] == -INFINITY ? 0.f : ex2(m[h] - to);
+                m[h] = move ? to : m[h];
+                l[h] *= alpha[h];
+              }
             }
-            l[h] *= alpha[h];
           }
-          if (i >= kGroups) {              // the accumulator holds earlier tiles of this segment
+          if (!fresh) {                    // the accumulator holds earlier tiles of this segment
+#pragma unroll
+            for (int h = 0; h < NP; ++h)
+              if (h >= (G + 3) / 4 * 4) alpha[h] = 1.f;
             mbar_wait(bPv + grp, (mine - 1) & 1, abort_flag, kSiteDecodeTc);
             __syncwarp();
             tc_fence_after();
 #pragma unroll
             for (int k = 0; k < kPParts; ++k) {
               uint32_t ov[NP];
-              const uint32_t at = tmem + lane_base + C::kColO + grp * C::kOCols + k * NP;
+              const uint32_t at = tmem + lane_base + C::kColO + (par * kGroups + grp) * C::kOCols + k * NP;
               tmem_ld16(at, ov);
               tmem_wait_ld();
               reg_fence(ov);
@@ -590,35 +642,36 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
         }
         // the group's previous P V product has read its P
         if (mine > 0) mbar_wait(bPv + grp, (mine - 1) & 1, abort_flag, kSiteDecodeTc);
-        if constexpr (kF8) {
-          uint8_t* pb = myP + (row & 15);
-          const int chunk = row >> 4;
+        float pr[NP];
 #pragma unroll
-          for (int h = 0; h < NP; h += 2) {
-            if (h >= G) break;
-            const float p0 = s[h] == -INFINITY ? 0.f : ex2(s[h] - m[h]);
-            const float p1 = h + 1 >= G || s[h + 1] == -INFINITY ? 0.f : ex2(s[h + 1] - m[h + 1]);
-            l[h] += p0;
-            l[h + 1] += p1;
-            uint16_t pr[kPParts];
-            split_e4m3<true>(p0, p1, pr);
-            const int o0 = h * 128 + ((chunk ^ (h & 7)) << 4), o1 = (h + 1) * 128 + ((chunk ^ ((h + 1) & 7)) << 4);
+        for (int h0 = 0; h0 < NP; h0 += 4) {
+          if (h0 >= G) break;
 #pragma unroll
-            for (int k = 0; k < kPParts; ++k) {
-              pb[k * C::kQBlock + o0] = (uint8_t)(pr[k] & 0xff);
-              pb[k * C::kQBlock + o1] = (uint8_t)(pr[k] >> 8);
-            }
+          for (int h = h0; h < h0 + 4; ++h) {
+            pr[h] = s[h] == -INFINITY ? 0.f : ex2(s[h] - m[h]);
+            l[h] += pr[h];
           }
-        } else {
-          // row `row` of P: block row / 64, 16-byte chunk (row / 8) & 7
-          uint8_t* pb = myP + (row >> 6) * C::kQBlock + (row & 7) * 2;
-          const int chunk = (row >> 3) & 7;
+          if constexpr (kF8) {
+            // byte `row` of P's rows h, of each part
+            uint8_t* pb = myP + (row & 15);
+            const int chunk = row >> 4;
 #pragma unroll
-          for (int h = 0; h < NP; ++h) {
-            if (h >= G) break;
-            const float pr = s[h] == -INFINITY ? 0.f : ex2(s[h] - m[h]);
-            l[h] += pr;
-            *reinterpret_cast<uint16_t*>(pb + h * 128 + ((chunk ^ (h & 7)) << 4)) = to16<T>(pr);
+            for (int h = h0; h < h0 + 4; h += 2) {
+              uint16_t part[kPParts];
+              split_e4m3<true>(pr[h], pr[h + 1], part);
+              const int o0 = h * 128 + ((chunk ^ (h & 7)) << 4), o1 = (h + 1) * 128 + ((chunk ^ ((h + 1) & 7)) << 4);
+#pragma unroll
+              for (int k = 0; k < kPParts; ++k) {
+                pb[k * C::kQBlock + o0] = (uint8_t)(part[k] & 0xff);
+                pb[k * C::kQBlock + o1] = (uint8_t)(part[k] >> 8);
+              }
+            }
+          } else {
+            // column `row` of P: block row / 64, 16-byte chunk (row / 8) & 7
+            uint8_t* pb = myP + (row >> 6) * C::kQBlock + (row & 7) * 2;
+            const int chunk = (row >> 3) & 7;
+#pragma unroll
+            for (int h = h0; h < h0 + 4; ++h) *reinterpret_cast<uint16_t*>(pb + h * 128 + ((chunk ^ (h & 7)) << 4)) = to16<T>(pr[h]);
           }
         }
         fence_proxy_async_smem();
@@ -628,92 +681,106 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
         __syncwarp();
       }
 
-      // ---- the segment's sums, both groups together ----
-      const int par = seg & 1;
-      float* pm = s_m + par * kGroups * NP;
-      float* pl = s_l + par * kGroups * 4 * NP;
-      const float ls = sum16(l, lane);
-      if ((lane & 1) == 0) pl[(grp * 4 + w4) * NP + (lane >> 1)] = ls;
+      // ---- the group's maxima and sums of the segment ----
+      if (seg > 1) mbar_wait(bOfree + par, ((seg >> 1) - 1) & 1, abort_flag, kSiteDecodeTc);
+      const float ls = reduce16<false>(l, lane);
+      if ((lane & 1) == 0) s_l[((par * kGroups + grp) * 4 + w4) * NP + (lane >> 1)] = ls;
       if (row == 0) {
 #pragma unroll
-        for (int h = 0; h < NP; ++h) pm[grp * NP + h] = m[h];
+        for (int h = 0; h < NP; ++h) s_m[(par * kGroups + grp) * NP + h] = m[h];
       }
-      // which groups have an accumulator for this segment: group g iff one of
-      // the tiles t - n .. t - 1 has parity g
-      const bool have0 = n > 1 || ((t - n) & 1) == 0, have1 = n > 1 || ((t - n) & 1) == 1;
-      if (mine > 0) mbar_wait(bPv + grp, (mine - 1) & 1, abort_flag, kSiteDecodeTc);
-      tc_fence_before();
-      bar_sync_named(3, kSoftmax);         // the other group's products are done too
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bSums + par);
+      w.next(n);
+    }
+  } else {
+    reg_dealloc<kEndRegs>();
+    // ---------------- ends of segments ----------------
+    const int row = tid & 127, w4 = warp & 3;
+    const uint32_t lane_base = static_cast<uint32_t>(w4 * 32) << 16;
+    int t = 0;                             // the segment's first tile
+    for (Walk w = w0; w.left > 0;) {
+      const int seg = w.seg, par = seg & 1, b = w.b, r = w.r, tiles = w.tiles, n = min(w.left, tiles - w.t);
+      const int slice = p.slices == 1 ? 0 : r % p.slices, G = min(NP, p.group - slice * NP);
+      const float* pm = s_m + par * kGroups * NP;
+      const float* pl = s_l + par * kGroups * 4 * NP;
+      mbar_wait(bSums + par, (seg >> 1) & 1, abort_flag, kSiteDecodeTc);
+      mbar_wait(bOdone + par, (seg >> 1) & 1, abort_flag, kSiteDecodeTc);
+      __syncwarp();
       tc_fence_after();
-      // group g finishes heads 8 g .. 8 g + 7; thread `row` holds column row of o
-      constexpr int kHalf = NP / 2;
-      const int h0 = grp * kHalf;
-      float oa[kHalf];
+      // Lane h of every warp: maximum and sum of head h over both groups and
+      // the factors of their accumulators, passed on through shared memory
+      // (each thread working out 16 heads' took longer than two tiles).
+      const bool whole = n == tiles;       // every tile of the item is this CTA's
+      const int hl = lane & (NP - 1);
+      const float m0 = pm[hl], m1 = pm[NP + hl], M = fmaxf(m0, m1);
+      const float a0 = m0 == -INFINITY ? 0.f : ex2(m0 - M), a1 = m1 == -INFINITY ? 0.f : ex2(m1 - M);
+      const float* x0 = pl + hl;
+      const float* x1 = pl + 4 * NP + hl;
+      const float L = fmaf(a0, (x0[0] + x0[NP]) + (x0[2 * NP] + x0[3 * NP]), a1 * ((x1[0] + x1[NP]) + (x1[2 * NP] + x1[3 * NP])));
+      const float f = !whole ? p.o_scale : L == 0.f ? 0.f : __fdividef(p.o_scale, L);
+      float* fac = s_fac + w4 * 2 * NP;
+      fac[lane] = (lane < NP ? a0 : a1) * f;
+      __syncwarp();
+      float oa[NP];                        // thread `row`: column row of o
 #pragma unroll
-      for (int h = 0; h < kHalf; ++h) oa[h] = 0.f;
-      float M[kHalf], L[kHalf];
-#pragma unroll
-      for (int h = 0; h < kHalf; ++h) {
-        const float m0 = pm[h0 + h], m1 = pm[NP + h0 + h];
-        M[h] = fmaxf(m0, m1);
-        L[h] = 0.f;
-      }
+      for (int h = 0; h < NP; ++h) oa[h] = 0.f;
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) {
-        if (!(g ? have1 : have0)) continue;
-        float a[kHalf];
-#pragma unroll
-        for (int h = 0; h < kHalf; ++h) {
-          const float mg = pm[g * NP + h0 + h];
-          a[h] = mg == -INFINITY ? 0.f : ex2(mg - M[h]);
-          const float* x = pl + g * 4 * NP + h0 + h;
-          L[h] = fmaf(a[h], (x[0] + x[NP]) + (x[2 * NP] + x[3 * NP]), L[h]);
-        }
+        // a group has an accumulator iff it took a tile
+        if (!(n > 1 || (t & 1) == g)) continue;
         float wk = 1.f;
 #pragma unroll
         for (int k = 0; k < kPParts; ++k, wk *= 1.f / kPartScale) {
-          uint32_t ov[kHalf];
-          tmem_ld8(tmem + lane_base + C::kColO + g * C::kOCols + k * NP + h0, ov);
+          uint32_t ov[NP];
+          tmem_ld16(tmem + lane_base + C::kColO + (par * kGroups + g) * C::kOCols + k * NP, ov);
           tmem_wait_ld();
           reg_fence(ov);
 #pragma unroll
-          for (int h = 0; h < kHalf; ++h) oa[h] = fmaf(__uint_as_float(ov[h]) * wk, a[h], oa[h]);
+          for (int h = 0; h < NP; h += 4) {
+            const float4 y = *reinterpret_cast<const float4*>(fac + g * NP + h);
+            oa[h] = fmaf(__uint_as_float(ov[h]) * wk, y.x, oa[h]);
+            oa[h + 1] = fmaf(__uint_as_float(ov[h + 1]) * wk, y.y, oa[h + 1]);
+            oa[h + 2] = fmaf(__uint_as_float(ov[h + 2]) * wk, y.z, oa[h + 2]);
+            oa[h + 3] = fmaf(__uint_as_float(ov[h + 3]) * wk, y.w, oa[h + 3]);
+          }
         }
       }
       tc_fence_before();
-      mbar_arrive(bOfree);
+      __syncwarp();                        // the factors have been read
+      mbar_arrive(bOfree + par);
 
       // ---- result or record ----
-      // number of the item's first tile, and the CTAs that hold its tiles
-      const long long i0 = item0 + (long long)r * tiles, i1 = i0 + tiles;
-      const long long c0 = ((i0 + 1) * ctas - 1) / all, c1 = (i1 * ctas - 1) / all;
-      const size_t bh0 = (size_t)b * p.H + (size_t)(r / p.slices) * p.group + slice * NP;
-      if (c0 == c1) {
+      const size_t bh0 = (size_t)b * p.H + (size_t)(p.slices == 1 ? r : r / p.slices) * p.group + slice * NP;
+      if (whole) {
+        __nv_bfloat16* o = p.o + bh0 * D + row;
 #pragma unroll
-        for (int h = 0; h < kHalf; ++h) {
-          if (h0 + h >= G) break;
-          const float inv = L[h] == 0.f ? 0.f : p.o_scale / L[h];
-          if (row < D) p.o[(bh0 + h0 + h) * D + row] = __float2bfloat16_rn(oa[h] * inv);
-          if (row == 0 && p.lse != nullptr) p.lse[bh0 + h0 + h] = L[h] == 0.f ? -INFINITY : (M[h] + lg2(L[h])) * kLn2;
+        for (int h0 = 0; h0 < NP; h0 += 4) {
+          if (h0 >= G) break;
+#pragma unroll
+          for (int h = h0; h < h0 + 4; ++h)
+            if (row < D && h < G) o[h * D] = __float2bfloat16_rn(oa[h]);
         }
+        if (p.lse != nullptr && row < G) p.lse[bh0 + row] = L == 0.f ? -INFINITY : (M + lg2(L)) * kLn2;
       } else {
+        // number of the item's first tile, and the CTAs that hold its tiles
+        const long long i0 = item0 + (long long)r * tiles, i1 = i0 + tiles;
+        const long long c0 = ((i0 + 1) * ctas - 1) / all, c1 = (i1 * ctas - 1) / all;
         // this CTA's record: 0 where the item is the first of its part, else 1
         const int which = seg == 0 ? 0 : 1;
         float* rec = p.rec + ((size_t)blockIdx.x * 2 + which) * NP * (D + kHead);
 #pragma unroll
-        for (int h = 0; h < kHalf; ++h) {
-          if (h0 + h >= G) break;
-          float* x = rec + (h0 + h) * (D + kHead);
-          if (row < D) __stcg(x + kHead + row, oa[h] * p.o_scale);
-          if (row == 0) __stcg(reinterpret_cast<float2*>(x), make_float2(M[h], L[h]));
+        for (int h = 0; h < NP; ++h) {
+          if (row < D && h < G) __stcg(rec + h * (D + kHead) + kHead + row, oa[h]);
         }
-        bar_sync_named(3, kSoftmax);
-        if (tid == 0) {
+        if (row < G) __stcg(reinterpret_cast<float2*>(rec + row * (D + kHead)), make_float2(M, L));
+        bar_sync_named(3, 128);
+        if (row == 0) {
           // the barrier orders every thread's record before this fence
           __threadfence();
           *s_last = atomicAdd(p.count + c0, 1) == (int)(c1 - c0);
         }
-        bar_sync_named(3, kSoftmax);
+        bar_sync_named(3, 128);
         if (*s_last) {
           __threadfence();
           // the last CTA of the item joins its records: a warp per head, lane
@@ -721,7 +788,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
           const int nrec = (int)(c1 - c0) + 1;
           // the first CTA's record is its second unless the item begins its part
           const int w_first = c0 * all / ctas < i0 ? 1 : 0;
-          for (int h = warp; h < G; h += kSoftmax / 32) {
+          for (int h = w4; h < G; h += 4) {
             float Mx = -INFINITY, Ls = 0.f, o4[4] = {0.f, 0.f, 0.f, 0.f};
             for (int base = 0; base < nrec; base += 32) {
               const int k = base + lane;
@@ -774,26 +841,27 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
             }
             if (lane == 0 && p.lse != nullptr) p.lse[bh0 + h] = Ls == 0.f ? -INFINITY : (Mx + lg2(Ls)) * kLn2;
           }
-          if (tid == 0) p.count[c0] = 0;     // left zeroed for the next call
+          if (row == 0) p.count[c0] = 0;     // left zeroed for the next call
         }
       }
       // on to the next segment; a new sequence begins behind this one's items
+      t += n;
       w.next(n);
       if (w.left > 0 && w.b != b) item0 += (long long)w.inner * tiles;
     }
     // sequences that hold nothing
     for (int b = blockIdx.x; b < p.B; b += (int)gridDim.x) {
       if (w0.len_of(b) > 0) continue;
-      for (int i = tid; i < p.H * D / 2; i += kSoftmax)
+      for (int i = row; i < p.H * D / 2; i += 128)
         reinterpret_cast<uint32_t*>(p.o + (size_t)b * p.H * D)[i] = 0u;
       if (p.lse != nullptr)
-        for (int i = tid; i < p.H; i += kSoftmax) p.lse[(size_t)b * p.H + i] = -INFINITY;
+        for (int i = row; i < p.H; i += 128) p.lse[(size_t)b * p.H + i] = -INFINITY;
     }
   }
 
   tc_fence_before();
   __syncthreads();
-  if (warp == kMmaWarp) {
+  if (warp == kScoreWarp) {
     tc_fence_after();
     tmem_dealloc(tmem, C::kTmemCols);
   }

@@ -134,6 +134,20 @@ __device__ __forceinline__ void grid_dep_launch_dependents() {
 }
 
 // ---------------------------------------------------------------------------
+// Registers of a warpgroup (four warps, all of which execute the same one):
+// raise or lower every thread's count to N (a multiple of 8).  The shares of
+// all warpgroups together stay within what the launch allocated.
+// ---------------------------------------------------------------------------
+template <int N>
+__device__ __forceinline__ void reg_alloc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void reg_dealloc() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+// ---------------------------------------------------------------------------
 // mbarrier
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
@@ -162,20 +176,6 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar_addr, uint32_t parity
       "selp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(ok)
       : "r"(bar_addr), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-
-// The same question without the wait that try_wait may take: for a thread that
-// polls several barriers in turn.
-__device__ __forceinline__ bool mbar_test_wait(const uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
       : "memory");
   return ok != 0;
 }
