@@ -289,9 +289,12 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
   all *= w0.inner;
   // no part is empty, so every CTA between an item's first and last has a record
   const long long ctas = min((long long)gridDim.x, all);
+  // CTA c: tiles [c q + min(c, rem), ...), q or q + 1 of them
+  const long long q = ctas > 0 ? all / ctas : 0, rem = all - q * ctas;
+  auto part = [&](long long c) { return c * q + min(c, rem); };
   const bool busy = blockIdx.x < ctas;
-  const long long first = busy ? blockIdx.x * all / ctas : 0;
-  w0.left = busy ? (int)((blockIdx.x + 1ll) * all / ctas - first) : 0;
+  const long long first = busy ? part(blockIdx.x) : 0;
+  w0.left = busy ? (int)(part(blockIdx.x + 1) - first) : 0;
   w0.b = w0.r = w0.t = w0.tiles = w0.len = w0.seg = w0.loc = 0;
   long long item0 = 0;                   // number of the current sequence's first tile
   if (w0.left > 0) {
@@ -366,22 +369,30 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
       const int outer = pg * p.H_kv + head, in = p.box < BT ? 0 : row0 & (per_page - 1);
       if (turn > 0 && !mbar_wait(bEmpty + s, (turn - 1) & 1, abort_flag, kSiteDecodeTc)) break;
       __syncwarp();
+      // box i's coordinates to the issuing thread (all of them ahead of it: a
+      // shuffle and a branch for each box put the boxes one behind the other)
+      int at[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) at[i] = __shfl_sync(0xffffffffu, outer, i);
       if (elect_one_sync()) {
         s_bad[s] = ~loaded;
         mbar_arrive_expect_tx(bFull + s, (uint32_t)__popc(loaded) * 2 * p.box * C::kRowBytes);
-      }
-      uint8_t* dV = sKV + s * 2 * kTile;
-      for (int i = 0; i < boxes; ++i, dV += p.box * 128) {
-        const int at = __shfl_sync(0xffffffffu, outer, i);
-        if (!((loaded >> i) & 1u)) continue;
-        if (elect_one_sync()) {
-          constexpr int cols = kF8 ? 128 : 64;
+        uint8_t* dV = sKV + s * 2 * kTile;
+        const int step = p.box * 128;
+        constexpr int cols = kF8 ? 128 : 64;
 #pragma unroll
-          for (int cb = 0; cb < C::kBlocks; ++cb) tma_load_3d(dV + kTile + cb * BT * 128, &tmK, bFull + s, cb * cols, in, at);
+        for (int i = 0; i < 8; ++i) {
+          if ((loaded >> i) & 1u) {
 #pragma unroll
-          for (int cb = 0; cb < C::kBlocks; ++cb) tma_load_3d(dV + cb * BT * 128, &tmV, bFull + s, cb * cols, in, at);
+            for (int cb = 0; cb < C::kBlocks; ++cb)
+              tma_load_3d(dV + kTile + cb * BT * 128 + i * step, &tmK, bFull + s, cb * cols, in, at[i]);
+#pragma unroll
+            for (int cb = 0; cb < C::kBlocks; ++cb)
+              tma_load_3d(dV + cb * BT * 128 + i * step, &tmV, bFull + s, cb * cols, in, at[i]);
+          }
         }
       }
+      __syncwarp();
       if (++s == NS) {
         s = 0;
         ++turn;
@@ -573,8 +584,6 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
             s[h] = valid ? x * (kF8 ? qs[h] : qf) : -INFINITY;
           }
         }
-        // Heads are taken four at a time: a branch for each would put their
-        // chains of instructions one behind the other.
         const bool fresh = i < kGroups;    // the group's first tile of the segment
         bool up = false;
         if (!fresh) {
@@ -642,6 +651,8 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
         }
         // the group's previous P V product has read its P
         if (mine > 0) mbar_wait(bPv + grp, (mine - 1) & 1, abort_flag, kSiteDecodeTc);
+        // Heads are taken four at a time: a branch for each would put their
+        // chains of instructions one behind the other.
         float pr[NP];
 #pragma unroll
         for (int h0 = 0; h0 < NP; h0 += 4) {
@@ -765,7 +776,14 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
       } else {
         // number of the item's first tile, and the CTAs that hold its tiles
         const long long i0 = item0 + (long long)r * tiles, i1 = i0 + tiles;
-        const long long c0 = ((i0 + 1) * ctas - 1) / all, c1 = (i1 * ctas - 1) / all;
+        auto holder = [&](long long x) {   // an estimate in fp64 (x is exact there), then its neighbour if it is off
+          long long c = x < rem * (q + 1) ? (long long)((double)x / (double)(q + 1)) : (long long)((double)(x - rem) / (double)q);
+          if (part(c) > x) --c;
+          else if (part(c + 1) <= x) ++c;
+          return c;
+        };
+        const long long c0 = i0 >= first ? (long long)blockIdx.x : holder(i0);
+        const long long c1 = i1 <= first + w0.left ? (long long)blockIdx.x : holder(i1 - 1);
         // this CTA's record: 0 where the item is the first of its part, else 1
         const int which = seg == 0 ? 0 : 1;
         float* rec = p.rec + ((size_t)blockIdx.x * 2 + which) * NP * (D + kHead);
@@ -776,26 +794,37 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
         if (row < G) __stcg(reinterpret_cast<float2*>(rec + row * (D + kHead)), make_float2(M, L));
         bar_sync_named(3, 128);
         if (row == 0) {
-          // the barrier orders every thread's record before this fence
-          __threadfence();
-          *s_last = atomicAdd(p.count + c0, 1) == (int)(c1 - c0);
+          // the barrier orders every thread's record before this release, and
+          // what the others released before the loads below
+          int before;
+          asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(p.count + c0) : "memory");
+          *s_last = before == (int)(c1 - c0);
         }
         bar_sync_named(3, 128);
         if (*s_last) {
-          __threadfence();
           // the last CTA of the item joins its records: a warp per head, lane
-          // i the i-th record's weight and columns 4 i .. 4 i + 3
+          // i the i-th record's weight and columns 4 i .. 4 i + 3; weights and
+          // columns are asked for together (one L2 round trip per 8 records)
           const int nrec = (int)(c1 - c0) + 1;
           // the first CTA's record is its second unless the item begins its part
-          const int w_first = c0 * all / ctas < i0 ? 1 : 0;
+          const int w_first = part(c0) < i0 ? 1 : 0;
           for (int h = w4; h < G; h += 4) {
+            const float* recs = p.rec + ((size_t)c0 * 2 * NP + h) * (D + kHead);
+            constexpr size_t kStep = (size_t)2 * NP * (D + kHead), kSecond = (size_t)NP * (D + kHead);
             float Mx = -INFINITY, Ls = 0.f, o4[4] = {0.f, 0.f, 0.f, 0.f};
-            for (int base = 0; base < nrec; base += 32) {
-              const int k = base + lane;
+            constexpr int kAhead = 8;
+            for (int base = 0; base < nrec; base += kAhead) {
+              const int many = min(kAhead, nrec - base);
               float2 ml = make_float2(-INFINITY, 0.f);
-              if (k < nrec)
-                ml = __ldcg(reinterpret_cast<const float2*>(
-                    p.rec + (((size_t)(c0 + k) * 2 + (k == 0 ? w_first : 0)) * NP + h) * (D + kHead)));
+              if (lane < many)
+                ml = __ldcg(reinterpret_cast<const float2*>(recs + (base + lane) * kStep + (base + lane == 0 ? w_first : 0) * kSecond));
+              float4 x[kAhead];
+#pragma unroll
+              for (int u = 0; u < kAhead; ++u) {
+                x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (u < many && lane * 4 < D)
+                  x[u] = __ldcg(reinterpret_cast<const float4*>(recs + (base + u) * kStep + (base + u == 0 ? w_first : 0) * kSecond + kHead) + lane);
+              }
               float bm = fmaxf(ml.x, Mx);
 #pragma unroll
               for (int off = 16; off > 0; off >>= 1) bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, off));
@@ -808,28 +837,13 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
               Mx = bm;
 #pragma unroll
               for (int c = 0; c < 4; ++c) o4[c] *= keep;
-              const int many = min(32, nrec - base);
-              constexpr int kAhead = 8;
-              for (int k0 = 0; k0 < many; k0 += kAhead) {
-                float4 x[kAhead];
 #pragma unroll
-                for (int u = 0; u < kAhead; ++u) {
-                  x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-                  const int kk = base + k0 + u;
-                  if (k0 + u < many && lane * 4 < D)
-                    x[u] = __ldcg(reinterpret_cast<const float4*>(
-                        p.rec + (((size_t)(c0 + kk) * 2 + (kk == 0 ? w_first : 0)) * NP + h) * (D + kHead) + kHead) + lane);
-                }
-#pragma unroll
-                for (int u = 0; u < kAhead; ++u) {
-                  const float wu = __shfl_sync(0xffffffffu, wt, (k0 + u) & 31);
-                  if (k0 + u < many) {
-                    o4[0] = fmaf(wu, x[u].x, o4[0]);
-                    o4[1] = fmaf(wu, x[u].y, o4[1]);
-                    o4[2] = fmaf(wu, x[u].z, o4[2]);
-                    o4[3] = fmaf(wu, x[u].w, o4[3]);
-                  }
-                }
+              for (int u = 0; u < kAhead; ++u) {
+                const float wu = __shfl_sync(0xffffffffu, wt, u);   // 0 behind the last record
+                o4[0] = fmaf(wu, x[u].x, o4[0]);
+                o4[1] = fmaf(wu, x[u].y, o4[1]);
+                o4[2] = fmaf(wu, x[u].z, o4[2]);
+                o4[3] = fmaf(wu, x[u].w, o4[3]);
               }
             }
             const float inv = Ls == 0.f ? 0.f : 1.f / Ls;
