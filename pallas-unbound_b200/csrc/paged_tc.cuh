@@ -414,16 +414,19 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
       const T* q = static_cast<const T*>(p.q) + ((size_t)w.b * p.H + (w.r / p.slices) * p.group + slice * NP) * D;
       uint8_t* dst = sQ + slot * C::kQBytes;
       constexpr int kVecs = D / 8;         // 16-byte vectors of a row
-      uint4 v[NP * kVecs / 32];
+      constexpr int kHold = NP * kVecs / 64;   // vectors a lane holds, in two rounds
+#pragma unroll 1
+      for (int i0 = 0; i0 < 2 * kHold; i0 += kHold) {
+      uint4 v[kHold];
 #pragma unroll
-      for (int i = 0; i < NP * kVecs / 32; ++i) {
-        const int h = (i * 32 + lane) / kVecs, c = (i * 32 + lane) % kVecs;
+      for (int i = 0; i < kHold; ++i) {
+        const int h = ((i0 + i) * 32 + lane) / kVecs, c = ((i0 + i) * 32 + lane) % kVecs;
         v[i] = make_uint4(0u, 0u, 0u, 0u);
         if (h < heads) v[i] = *reinterpret_cast<const uint4*>(q + (size_t)h * D + c * 8);
       }
 #pragma unroll
-      for (int i = 0; i < NP * kVecs / 32; ++i) {
-        const int h = (i * 32 + lane) / kVecs, c = (i * 32 + lane) % kVecs;
+      for (int i = 0; i < kHold; ++i) {
+        const int h = ((i0 + i) * 32 + lane) / kVecs, c = ((i0 + i) * 32 + lane) % kVecs;
         if constexpr (!kF8) {
           *reinterpret_cast<uint4*>(dst + (c >> 3) * C::kQBlock + h * 128 + (((c & 7) ^ (h & 7)) << 4)) = v[i];
         } else {
@@ -455,6 +458,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
           // a head that is not finite makes its scores NaN, as it would in 16 bits
           if (c == 0) s_qinv[slot * NP + h] = isfinite(mx) ? down : mx - mx;
         }
+      }
       }
       fence_proxy_async_smem();
       mbar_arrive(bQfull + slot);

@@ -258,22 +258,31 @@ struct Coef {
   uint64_t k0[4], k1[4], k2[4], k3[4];
 };
 
-// wa, wb: the weights of the lane's two vectors; kBack: the transposed
-// rotation with no weight.
+// w: the kind's weights; kBack: the transposed rotation with no weight.
 template <bool kInter, bool kBack>
-__device__ __forceinline__ void make_coef(const float* cs, const float* sn, const float* wa, const float* wb, const Place& pl,
-                                          int sub, Coef& k) {
-  float c[8], s[8];
+__device__ __forceinline__ void make_coef(const float* cs, const float* sn, const float* w, const Place& pl, int sub, Coef& k) {
+  float c[8], s[8], wa[8], wb[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    c[i] = pl.rot ? cs[sub * 8 + i] : 1.f;
-    s[i] = pl.rot ? sn[sub * 8 + i] : 0.f;
-    if (kBack) s[i] = -s[i];
+  for (int i = 0; i < 8; i += 4) {
+    float4 v = make_float4(1.f, 1.f, 1.f, 1.f), u = make_float4(0.f, 0.f, 0.f, 0.f), x = v, y = v;
+    if (pl.rot) {
+      v = *reinterpret_cast<const float4*>(cs + sub * 8 + i);
+      u = *reinterpret_cast<const float4*>(sn + sub * 8 + i);
+    }
+    if (!kBack && pl.in) {
+      x = *reinterpret_cast<const float4*>(w + pl.o0 + i);
+      y = *reinterpret_cast<const float4*>(w + pl.o1 + i);
+    }
+    c[i] = v.x, c[i + 1] = v.y, c[i + 2] = v.z, c[i + 3] = v.w;
+    s[i] = u.x, s[i + 1] = u.y, s[i + 2] = u.z, s[i + 3] = u.w;
+    wa[i] = x.x, wa[i + 1] = x.y, wa[i + 2] = x.z, wa[i + 3] = x.w;
+    wb[i] = y.x, wb[i + 1] = y.y, wb[i + 2] = y.z, wb[i + 3] = y.w;
   }
 #pragma unroll
+  for (int i = 0; i < 8; ++i) s[i] = kBack ? -s[i] : s[i];
+#pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float a0 = kBack || !pl.in ? 1.f : wa[pl.o0 + 2 * i], a1 = kBack || !pl.in ? 1.f : wa[pl.o0 + 2 * i + 1];
-    const float b0 = kBack || !pl.in ? 1.f : wb[pl.o1 + 2 * i], b1 = kBack || !pl.in ? 1.f : wb[pl.o1 + 2 * i + 1];
+    const float a0 = wa[2 * i], a1 = wa[2 * i + 1], b0 = wb[2 * i], b1 = wb[2 * i + 1];
     if constexpr (kInter) {
       k.k0[i] = f2_pack(a0 * c[i], a1 * c[i]);
       k.k1[i] = f2_pack(-a1 * s[i], a0 * s[i]);
@@ -292,10 +301,17 @@ __device__ __forceinline__ void make_coef(const float* cs, const float* sn, cons
 // a value that need not be finite).
 template <bool kInter>
 __device__ __forceinline__ void apply_coef(const Coef& k, bool partial, bool rot, uint64_t (&a)[4], uint64_t (&b)[4]) {
+  if (partial && !rot) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      a[i] = f2_mul(a[i], k.k0[i]);
+      b[i] = f2_mul(b[i], k.k2[i]);
+    }
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    uint64_t x = kInter ? f2_swap(a[i]) : b[i], y = kInter ? f2_swap(b[i]) : a[i];
-    if (partial && !rot) x = y = 0ull;
+    const uint64_t x = kInter ? f2_swap(a[i]) : b[i], y = kInter ? f2_swap(b[i]) : a[i];
     a[i] = f2_fma(x, k.k1[i], f2_mul(a[i], k.k0[i]));
     b[i] = f2_fma(y, k.k3[i], f2_mul(b[i], k.k2[i]));
   }
@@ -310,12 +326,12 @@ __device__ __forceinline__ float f2_sum(uint64_t v) {
 // A pass is 32 / kLanes rows (heads) of one token; queries' passes come
 // first, then keys', then values'.  A warp walks units of `chunk` consecutive
 // passes of one token, kBatch of them loaded before the first is used (and the
-// first ones before the token's angles are made).
+// unit's first ones before the token's angles are made).
 template <typename T, int kLanes, bool kInter, bool kAppend>
 __global__ void __launch_bounds__(kThreads, kFwdCtasPerSm) fwd_kernel(const __grid_constant__ Params p) {
   constexpr int kRows = 32 / kLanes;
   constexpr int kBatch = sizeof(T) == 4 ? 2 : 4;
-  __shared__ Shared sh;
+  __shared__ __align__(16) Shared sh;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int sub = lane % kLanes, row = lane / kLanes;
   grid_dep_wait();
@@ -323,13 +339,20 @@ __global__ void __launch_bounds__(kThreads, kFwdCtasPerSm) fwd_kernel(const __gr
   fill_shared(p, sh);
   const Place pl = make_place<kInter>(sub, p.D, p.R);
   const bool partial = p.R < p.D;
-  const int end0 = (p.side[0].heads + kRows - 1) / kRows, end1 = end0 + (p.side[1].heads + kRows - 1) / kRows;
-  const int end2 = kAppend ? end1 + (p.side[2].heads + kRows - 1) / kRows : end1;
   const long long units = p.T * p.chunks, stride = (long long)gridDim.x * kWarps;
   for (long long unit = (long long)blockIdx.x * kWarps + warp; unit < units; unit += stride) {
-    const long long t = unit / p.chunks;
-    const long long b = t / p.N, n = t - b * p.N;
-    const int first = (int)(unit - t * p.chunks) * p.chunk, last = min(first + p.chunk, end2);
+    long long t = unit, b = 0, n = unit;
+    int first = 0;
+    if (p.chunks > 1) {
+      t = unit / p.chunks;
+      first = (int)(unit - t * p.chunks) * p.chunk;
+      n = t;
+    }
+    if (!kAppend) {
+      b = t / p.N;
+      n = t - b * p.N;
+    }
+    const int last = first + p.chunk;
     size_t pool_row = 0;    // append: page and row of this token
     bool put = true;
     if constexpr (kAppend) {
@@ -338,72 +361,95 @@ __global__ void __launch_bounds__(kThreads, kFwdCtasPerSm) fwd_kernel(const __gr
       if (slot >= p.num_slots && lane == 0) record_device_error(PU_ERR_INVALID_ARGUMENT, kSiteAppendSlot);
       pool_row = put ? (size_t)slot : 0;
     }
-    Coef k;
-    int kind_of_k = -1;
-    for (int pass = first; pass < last; pass += kBatch) {
-      Vec8<T> va[kBatch], vb[kBatch];
+    bool angles = false;
+    int begin = 0;
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
-        const int ps = pass + u, kind = ps < end0 ? 0 : ps < end1 ? 1 : 2;
-        const Side& sd = p.side[kind];
-        const int h = (ps - (kind == 0 ? 0 : kind == 1 ? end0 : end1)) * kRows + row;
-        va[u].zero();
-        vb[u].zero();
-        if (ps < last && h < sd.heads && pl.in) {
-          const T* x = static_cast<const T*>(sd.x.p) + b * sd.x.sB + n * sd.x.sN + h * sd.x.sH;
-          va[u].load(x + pl.o0);
-          vb[u].load(x + pl.o1);
-        }
-      }
-      if (pass == first) make_angles(p.ang, sh, p.R / 2, b, n, lane, sh.cs[warp][0], sh.cs[warp][1]);
-#pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
-        const int ps = pass + u, kind = ps < end0 ? 0 : ps < end1 ? 1 : 2;
-        if (ps >= last) break;
-        const Side& sd = p.side[kind];
-        const int h = (ps - (kind == 0 ? 0 : kind == 1 ? end0 : end1)) * kRows + row;
-        const bool live = h < sd.heads && pl.in;
-        uint64_t a[4], bb[4];
-        va[u].get(a);
-        vb[u].get(bb);
-        if (!kAppend || kind < 2) {
-          if (kind != kind_of_k) {
-            make_coef<kInter, false>(sh.cs[warp][0], sh.cs[warp][1], sh.w[kind], sh.w[kind], pl, sub, k);
-            kind_of_k = kind;
-          }
-          float r = 1.f;
-          if (sd.w != nullptr) {
-            uint64_t s0 = 0ull, s1 = 0ull;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              s0 = f2_fma(a[i], a[i], s0);
-              s1 = f2_fma(bb[i], bb[i], s1);
-            }
-            r = rsqrtf(group_sum<kLanes>(f2_sum(f2_add(s0, s1))) * p.inv_d + p.eps);
-          }
-          apply_coef<kInter>(k, partial, pl.rot, a, bb);
-          if (sd.w != nullptr) {
-            const uint64_t rr = f2_pack(r, r);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              a[i] = f2_mul(a[i], rr);
-              bb[i] = f2_mul(bb[i], rr);
-            }
-          }
-        }
-        if (!live) continue;
-        if (kAppend && kind > 0) {
-          if (!put) continue;
+    for (int kind = 0; kind < (kAppend ? 3 : 2); ++kind) {
+      const Side& sd = p.side[kind];
+      const int heads = sd.heads, end = begin + (heads + kRows - 1) / kRows;
+      const int lo = max(first, begin), hi = min(last, end);
+      if (lo < hi) {
+        // the lane's rows of the kind: head h, then kRows heads further, ...
+        int h = (lo - begin) * kRows + row;
+        const long long xs = sd.x.sH;
+        const T* x = static_cast<const T*>(sd.x.p) + b * sd.x.sB + n * sd.x.sN + h * xs;
+        const bool norm = kind < 2 && sd.w != nullptr;
+        constexpr bool kPool = kAppend;
+        T* y = nullptr;
+        size_t at = 0, ys = 0;
+        if (kPool && kind > 0) {
           const size_t mask = ((size_t)1 << p.page_shift) - 1;
-          const size_t at = ((((pool_row >> p.page_shift) * sd.heads + h) << p.page_shift) + (pool_row & mask)) * p.D;
-          store8_pool(sd.y.p, at + pl.o0, p.pool_dtype, sd.unit, a);
-          store8_pool(sd.y.p, at + pl.o1, p.pool_dtype, sd.unit, bb);
+          at = ((((pool_row >> p.page_shift) * heads + h) << p.page_shift) + (pool_row & mask)) * p.D;
+          ys = (size_t)p.D << p.page_shift;
         } else {
-          T* y = static_cast<T*>(sd.y.p) + b * sd.y.sB + h * sd.y.sH + n * sd.y.sN;
-          store8(y + pl.o0, a);
-          store8(y + pl.o1, bb);
+          ys = sd.y.sH;
+          y = static_cast<T*>(sd.y.p) + b * sd.y.sB + n * sd.y.sN + h * ys;
+        }
+        Coef k;
+        bool coef = false;
+        for (int pass = lo; pass < hi; pass += kBatch) {
+          Vec8<T> va[kBatch], vb[kBatch];
+#pragma unroll
+          for (int u = 0; u < kBatch; ++u) {
+            va[u].zero();
+            vb[u].zero();
+            if (pass + u < hi && h + u * kRows < heads && pl.in) {
+              va[u].load(x + u * kRows * xs + pl.o0);
+              vb[u].load(x + u * kRows * xs + pl.o1);
+            }
+          }
+          if (kind < 2 && !coef) {
+            coef = true;
+            if (!angles) make_angles(p.ang, sh, p.R / 2, b, n, lane, sh.cs[warp][0], sh.cs[warp][1]);
+            angles = true;
+            make_coef<kInter, false>(sh.cs[warp][0], sh.cs[warp][1], sh.w[kind], pl, sub, k);
+          }
+#pragma unroll
+          for (int u = 0; u < kBatch; ++u) {
+            if (pass + u >= hi) break;
+            uint64_t a[4], bb[4];
+            va[u].get(a);
+            vb[u].get(bb);
+            if (kind < 2) {
+              uint64_t rr = 0ull;
+              if (norm) {
+                uint64_t s0 = 0ull, s1 = 0ull;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  s0 = f2_fma(a[i], a[i], s0);
+                  s1 = f2_fma(bb[i], bb[i], s1);
+                }
+                const float r = rsqrtf(group_sum<kLanes>(f2_sum(f2_add(s0, s1))) * p.inv_d + p.eps);
+                rr = f2_pack(r, r);
+              }
+              apply_coef<kInter>(k, partial, pl.rot, a, bb);
+              if (norm) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  a[i] = f2_mul(a[i], rr);
+                  bb[i] = f2_mul(bb[i], rr);
+                }
+              }
+            }
+            if (h + u * kRows < heads && pl.in) {
+              if (kPool && kind > 0) {
+                if (put) {
+                  store8_pool(sd.y.p, at + u * kRows * ys + pl.o0, p.pool_dtype, sd.unit, a);
+                  store8_pool(sd.y.p, at + u * kRows * ys + pl.o1, p.pool_dtype, sd.unit, bb);
+                }
+              } else {
+                store8(y + u * kRows * ys + pl.o0, a);
+                store8(y + u * kRows * ys + pl.o1, bb);
+              }
+            }
+          }
+          h += kBatch * kRows;
+          x += kBatch * kRows * xs;
+          y += kBatch * kRows * ys;
+          at += kBatch * kRows * ys;
         }
       }
+      begin = end;
     }
   }
 }
@@ -416,7 +462,7 @@ template <typename T, int kLanes, bool kInter>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) bwd_kernel(const __grid_constant__ Params p) {
   constexpr int kRows = 32 / kLanes;
   constexpr int kBatch = sizeof(T) == 4 ? 1 : 2;
-  __shared__ Shared sh;
+  __shared__ __align__(16) Shared sh;
   __shared__ float s_dw[kWarps][kMaxDim];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int sub = lane % kLanes, row = lane / kLanes;
@@ -428,48 +474,52 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) bwd_kernel(const __grid_
   grid_dep_launch_dependents();
   fill_shared(p, sh);
   const bool norm = sd.w != nullptr, partial = p.R < p.D;
-  const float* w = sh.w[kind];
+  const float* wa = sh.w[kind] + (pl.in ? pl.o0 : 0);
+  const float* wb = sh.w[kind] + (pl.in ? pl.o1 : 8);
   uint64_t da[4], db[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) da[i] = db[i] = 0ull;
-  const int passes = (sd.heads + kRows - 1) / kRows;
+  const int heads = sd.heads, passes = (heads + kRows - 1) / kRows;
   const int chunk = (passes + p.chunks - 1) / p.chunks;
   const long long units = p.T * p.chunks, stride = (long long)sd.ctas * kWarps;
+  const long long xs = sd.x.sH * kRows, gs = sd.g.sH * kRows, ys = sd.y.sH * kRows;   // from one pass to the next
   for (long long unit = (long long)cta * kWarps + warp; unit < units; unit += stride) {
-    const long long t = unit / p.chunks;
+    long long t = unit;
+    int lo = 0;
+    if (p.chunks > 1) {
+      t = unit / p.chunks;
+      lo = (int)(unit - t * p.chunks) * chunk;
+    }
     const long long b = t / p.N, n = t - b * p.N;
-    const int lo = (int)(unit - t * p.chunks) * chunk, hi = min(lo + chunk, passes);
-    const T* x0 = static_cast<const T*>(sd.x.p) + b * sd.x.sB + n * sd.x.sN;
-    const T* g0 = static_cast<const T*>(sd.g.p) + b * sd.g.sB + n * sd.g.sN;
-    T* y0 = static_cast<T*>(sd.y.p) + b * sd.y.sB + n * sd.y.sN;
+    const int hi = min(lo + chunk, passes);
+    int h = lo * kRows + row;
+    const T* xp = static_cast<const T*>(sd.x.p) + b * sd.x.sB + n * sd.x.sN + h * sd.x.sH;
+    const T* gp = static_cast<const T*>(sd.g.p) + b * sd.g.sB + n * sd.g.sN + h * sd.g.sH;
+    T* yp = static_cast<T*>(sd.y.p) + b * sd.y.sB + n * sd.y.sN + h * sd.y.sH;
     Coef k;
     for (int pass = lo; pass < hi; pass += kBatch) {
       Vec8<T> xa[kBatch], xb[kBatch], ga[kBatch], gb[kBatch];
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
-        const int h = (pass + u) * kRows + row;
         xa[u].zero();
         xb[u].zero();
         ga[u].zero();
         gb[u].zero();
-        if (pass + u < hi && h < sd.heads && pl.in) {
-          const T* g = g0 + h * sd.g.sH;
-          ga[u].load(g + pl.o0);
-          gb[u].load(g + pl.o1);
+        if (pass + u < hi && h + u * kRows < heads && pl.in) {
+          ga[u].load(gp + u * gs + pl.o0);
+          gb[u].load(gp + u * gs + pl.o1);
           if (norm) {
-            const T* x = x0 + h * sd.x.sH;
-            xa[u].load(x + pl.o0);
-            xb[u].load(x + pl.o1);
+            xa[u].load(xp + u * xs + pl.o0);
+            xb[u].load(xp + u * xs + pl.o1);
           }
         }
       }
       if (pass == lo) {
         make_angles(p.ang, sh, p.R / 2, b, n, lane, sh.cs[warp][0], sh.cs[warp][1]);
-        make_coef<kInter, true>(sh.cs[warp][0], sh.cs[warp][1], nullptr, nullptr, pl, sub, k);
+        make_coef<kInter, true>(sh.cs[warp][0], sh.cs[warp][1], nullptr, pl, sub, k);
       }
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
-        const int h = (pass + u) * kRows + row;
         if (pass + u >= hi) break;
         uint64_t ha[4], hb[4];
         ga[u].get(ha);
@@ -480,10 +530,16 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) bwd_kernel(const __grid_
           xa[u].get(x);
           xb[u].get(y);
 #pragma unroll
+          for (int i = 0; i < 4; i += 2) {
+            // lanes without a place in the row hold zeros
+            const ulonglong2 w0 = *reinterpret_cast<const ulonglong2*>(wa + 2 * i), w1 = *reinterpret_cast<const ulonglong2*>(wb + 2 * i);
+            va[i] = f2_mul(ha[i], w0.x);
+            va[i + 1] = f2_mul(ha[i + 1], w0.y);
+            vb[i] = f2_mul(hb[i], w1.x);
+            vb[i + 1] = f2_mul(hb[i + 1], w1.y);
+          }
+#pragma unroll
           for (int i = 0; i < 4; ++i) {
-            // in-range lanes' weights; the others' rows are zeros
-            va[i] = f2_mul(ha[i], *reinterpret_cast<const uint64_t*>(w + (pl.in ? pl.o0 : 0) + 2 * i));
-            vb[i] = f2_mul(hb[i], *reinterpret_cast<const uint64_t*>(w + (pl.in ? pl.o1 : 8) + 2 * i));
             s0 = f2_fma(x[i], x[i], s0);
             s1 = f2_fma(y[i], y[i], s1);
             t0 = f2_fma(va[i], x[i], t0);
@@ -502,11 +558,15 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) bwd_kernel(const __grid_
             hb[i] = f2_fma(vb[i], rr, f2_mul(y[i], qq));
           }
         }
-        if (h >= sd.heads || !pl.in) continue;
-        T* y = y0 + h * sd.y.sH;
-        store8(y + pl.o0, ha);
-        store8(y + pl.o1, hb);
+        if (h + u * kRows < heads && pl.in) {
+          store8(yp + u * ys + pl.o0, ha);
+          store8(yp + u * ys + pl.o1, hb);
+        }
       }
+      h += kBatch * kRows;
+      xp += kBatch * xs;
+      gp += kBatch * gs;
+      yp += kBatch * ys;
     }
   }
   if (sd.dw_part == nullptr) return;
