@@ -66,8 +66,7 @@ struct Side {
   const void* w;          // [D] norm weight, or nullptr: no norm
   int w_dtype;
   int heads;
-  int ctas;               // backward: CTAs that work on this kind
-  float* dw_part;         // backward: [ctas][D] partial weight gradients, or nullptr
+  float* dw_part;         // backward: [CTAs][D] partial weight gradients, or nullptr
   void* dw;               // backward: [D] weight gradient in w_dtype
   float unit;             // append: the stored value is the value / unit
 };
@@ -79,8 +78,9 @@ struct Params {
   long long T;            // tokens in all
   int D, R;
   float eps, inv_d;
-  int chunk;              // forward: passes per warp
-  int chunks;             // warps per token (backward: of either kind)
+  int chunk;              // passes a warp takes of one token
+  int chunks;             // warps per token
+  int ctas;               // backward: CTAs, each with a partial weight gradient
   // append
   const int32_t* slots;   // [T] page * page_size + row, negative: none
   int pool_dtype;
@@ -92,8 +92,8 @@ struct Params {
 template <typename T>
 struct Vec8 {
   uint4 w;
-  __device__ __forceinline__ void load(const T* p) { w = decode::ld_stream(reinterpret_cast<const uint4*>(p)); }
-  __device__ __forceinline__ void zero() { w = make_uint4(0u, 0u, 0u, 0u); }
+  // zeros where `use` is false (a predicated load, not a branch)
+  __device__ __forceinline__ void load(const T* p, bool use) { w = decode::ld_stream_if(reinterpret_cast<const uint4*>(p), use); }
   __device__ __forceinline__ void get(uint64_t (&f)[4]) const {
     const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -110,11 +110,10 @@ struct Vec8 {
 template <>
 struct Vec8<float> {
   uint4 w[2];
-  __device__ __forceinline__ void load(const float* p) {
-    w[0] = decode::ld_stream(reinterpret_cast<const uint4*>(p));
-    w[1] = decode::ld_stream(reinterpret_cast<const uint4*>(p) + 1);
+  __device__ __forceinline__ void load(const float* p, bool use) {
+    w[0] = decode::ld_stream_if(reinterpret_cast<const uint4*>(p), use);
+    w[1] = decode::ld_stream_if(reinterpret_cast<const uint4*>(p) + 1, use);
   }
-  __device__ __forceinline__ void zero() { w[0] = w[1] = make_uint4(0u, 0u, 0u, 0u); }
   __device__ __forceinline__ void get(uint64_t (&f)[4]) const {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -179,11 +178,11 @@ __device__ __forceinline__ float load_weight(const void* w, int dtype, int i) {
 }
 
 // What a CTA keeps in shared memory: the weights as fp32 (1 without a norm)
-// and every pair's 64-bit turn per position; per warp, cos and sin of a token.
+// and, per warp, cos and sin of a token's pairs.
 struct Shared {
   float w[2][kMaxDim];
-  unsigned long long step[kMaxPairs];
-  float cs[kWarps][2][kMaxPairs];
+  unsigned long long step[kMaxPairs];    // turn per position, as a 64-bit fraction
+  float cs[kWarps][4][kMaxPairs];        // forward: cos, sin; backward: see back_angles
 };
 
 __device__ __forceinline__ void fill_shared(const Params& p, Shared& sh) {
@@ -200,24 +199,68 @@ __device__ __forceinline__ void fill_shared(const Params& p, Shared& sh) {
   __syncthreads();
 }
 
-// cos and sin of every pair of one token into the warp's shared rows.
-__device__ __forceinline__ void make_angles(const Angles& a, const Shared& sh, int pairs, long long b, long long n, int lane,
-                                            float* cs, float* sn) {
-  __syncwarp();                          // the previous token's have been read
-  for (int p = lane; p < pairs; p += 32) {
-    long long pos = n;
-    if (a.pos != nullptr) {
-      int axis = 0;
-#pragma unroll
-      for (int i = 0; i + 1 < kMaxAxes; ++i) axis += p >= a.pair_end[i];
-      const long long at = axis * a.pA + b * a.pB + n * a.pN;
-      pos = a.pos64 ? static_cast<const long long*>(a.pos)[at] : (long long)static_cast<const int32_t*>(a.pos)[at];
-    }
-    const int turn = (int)((sh.step[p] * (unsigned long long)pos) >> 32);   // signed: half turns of 2^31
-    sincospif((float)turn * 4.6566128730773926e-10f, sn + p, cs + p);       // 2^-31
-  }
-  __syncwarp();
+// Sine and cosine of 2 pi turn / 2^32.  The nearest quarter turn comes off in
+// integers; the rest, at most pi / 4, through the Taylor series up to x^9 and
+// x^8 (the terms left out are below 2 10^-9 and 3 10^-8).
+__device__ __forceinline__ void sin_cos(int turn, float& s, float& c) {
+  const int quarter = (int)((unsigned)turn + 0x20000000u) >> 30;
+  const float x = (float)(turn - (int)((unsigned)quarter << 30)) * 1.4629180792671596e-9f;   // 2 pi / 2^32
+  const float z = x * x;
+  float ps = fmaf(z, 1.f / 362880.f, -1.f / 5040.f);
+  ps = fmaf(z, ps, 1.f / 120.f);
+  ps = fmaf(z, ps, -1.f / 6.f);
+  ps = fmaf(x * z, ps, x);
+  float pc = fmaf(z, 1.f / 40320.f, -1.f / 720.f);
+  pc = fmaf(z, pc, 1.f / 24.f);
+  pc = fmaf(z, pc, -0.5f);
+  pc = fmaf(z, pc, 1.f);
+  const float a = quarter & 1 ? pc : ps, b = quarter & 1 ? ps : pc;
+  s = __uint_as_float(__float_as_uint(a) ^ ((unsigned)(quarter & 2) << 30));
+  c = __uint_as_float(__float_as_uint(b) ^ ((unsigned)((quarter + 1) & 2) << 30));
 }
+
+// A lane's share of a token's angles: pairs `lane` and `lane + 32`.
+struct Turner {
+  int axis[2];                  // of the pair; -1: no such pair
+  long long pos[2];             // of the token that comes next
+
+  __device__ __forceinline__ void start(const Params& p, int lane) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int pair = lane + 32 * i;
+      axis[i] = 0;
+      pos[i] = 0;
+#pragma unroll
+      for (int a = 0; a + 1 < kMaxAxes; ++a) axis[i] += pair >= p.ang.pair_end[a];
+      if (pair >= p.R / 2) axis[i] = -1;
+    }
+  }
+  // asks for a token's positions (used by the next turn)
+  __device__ __forceinline__ void fetch(const Angles& a, unsigned b, unsigned n) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (axis[i] < 0) continue;
+      if (a.pos == nullptr) {
+        pos[i] = n;
+      } else {
+        const long long at = axis[i] * a.pA + b * a.pB + n * a.pN;
+        pos[i] = a.pos64 ? static_cast<const long long*>(a.pos)[at] : (long long)static_cast<const int32_t*>(a.pos)[at];
+      }
+    }
+  }
+  // sine and cosine of pair lane + 32 i at its fetched position
+  __device__ __forceinline__ void turn(const Shared& sh, int lane, int i, float& s, float& c) const {
+    sin_cos((int)((sh.step[lane + 32 * i] * (unsigned long long)pos[i]) >> 32), s, c);
+  }
+  // of all pairs, into the warp's shared rows
+  __device__ __forceinline__ void make(const Shared& sh, int lane, float* cs, float* sn) const {
+    __syncwarp();                        // the previous token's have been read
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (axis[i] >= 0) turn(sh, lane, i, sn[lane + 32 * i], cs[lane + 32 * i]);
+    __syncwarp();
+  }
+};
 
 // What a lane of a row group holds: its two vectors' places in the row.
 struct Place {
@@ -258,8 +301,8 @@ struct Coef {
   uint64_t k0[4], k1[4], k2[4], k3[4];
 };
 
-// w: the kind's weights; kBack: the transposed rotation with no weight.
-template <bool kInter, bool kBack>
+// w: the kind's weights
+template <bool kInter>
 __device__ __forceinline__ void make_coef(const float* cs, const float* sn, const float* w, const Place& pl, int sub, Coef& k) {
   float c[8], s[8], wa[8], wb[8];
 #pragma unroll
@@ -269,7 +312,7 @@ __device__ __forceinline__ void make_coef(const float* cs, const float* sn, cons
       v = *reinterpret_cast<const float4*>(cs + sub * 8 + i);
       u = *reinterpret_cast<const float4*>(sn + sub * 8 + i);
     }
-    if (!kBack && pl.in) {
+    if (pl.in) {
       x = *reinterpret_cast<const float4*>(w + pl.o0 + i);
       y = *reinterpret_cast<const float4*>(w + pl.o1 + i);
     }
@@ -278,8 +321,6 @@ __device__ __forceinline__ void make_coef(const float* cs, const float* sn, cons
     wa[i] = x.x, wa[i + 1] = x.y, wa[i + 2] = x.z, wa[i + 3] = x.w;
     wb[i] = y.x, wb[i + 1] = y.y, wb[i + 2] = y.z, wb[i + 3] = y.w;
   }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) s[i] = kBack ? -s[i] : s[i];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float a0 = wa[2 * i], a1 = wa[2 * i + 1], b0 = wb[2 * i], b1 = wb[2 * i + 1];
@@ -317,6 +358,54 @@ __device__ __forceinline__ void apply_coef(const Coef& k, bool partial, bool rot
   }
 }
 
+// The rotation back, straight from shared memory (its coefficients would take
+// the registers that hold rows in flight).  The warp's 256 floats: for halves
+// c, s, -s of each pair; interleaved (c, c) and (s, -s) of each.
+template <bool kInter>
+__device__ __forceinline__ void back_angles(const Turner& t, const Shared& sh, int lane, float* m) {
+  __syncwarp();                          // the previous token's have been read
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (t.axis[i] < 0) continue;
+    const int pair = lane + 32 * i;
+    float s, c;
+    t.turn(sh, lane, i, s, c);
+    if constexpr (kInter) {
+      reinterpret_cast<float2*>(m)[pair] = make_float2(c, c);
+      reinterpret_cast<float2*>(m + 2 * kMaxPairs)[pair] = make_float2(s, -s);
+    } else {
+      m[pair] = c;
+      m[kMaxPairs + pair] = s;
+      m[2 * kMaxPairs + pair] = -s;
+    }
+  }
+  __syncwarp();
+}
+
+template <bool kInter>
+__device__ __forceinline__ void turn_back(const float* m, int sub, uint64_t (&a)[4], uint64_t (&b)[4]) {
+  auto two = [](const float* p) { return *reinterpret_cast<const ulonglong2*>(p); };
+#pragma unroll
+  for (int i = 0; i < 4; i += 2) {
+    if constexpr (kInter) {
+      const float* c = m + sub * 16 + 2 * i;
+      const ulonglong2 ca = two(c), sa = two(c + 2 * kMaxPairs), cb = two(c + 8), sb = two(c + 8 + 2 * kMaxPairs);
+      a[i] = f2_fma(f2_swap(a[i]), sa.x, f2_mul(a[i], ca.x));
+      a[i + 1] = f2_fma(f2_swap(a[i + 1]), sa.y, f2_mul(a[i + 1], ca.y));
+      b[i] = f2_fma(f2_swap(b[i]), sb.x, f2_mul(b[i], cb.x));
+      b[i + 1] = f2_fma(f2_swap(b[i + 1]), sb.y, f2_mul(b[i + 1], cb.y));
+    } else {
+      const float* c = m + sub * 8 + 2 * i;
+      const ulonglong2 cc = two(c), ss = two(c + kMaxPairs), ns = two(c + 2 * kMaxPairs);
+      const uint64_t a0 = a[i], a1 = a[i + 1];
+      a[i] = f2_fma(b[i], ss.x, f2_mul(a0, cc.x));
+      a[i + 1] = f2_fma(b[i + 1], ss.y, f2_mul(a1, cc.y));
+      b[i] = f2_fma(a0, ns.x, f2_mul(b[i], cc.x));
+      b[i + 1] = f2_fma(a1, ns.y, f2_mul(b[i + 1], cc.y));
+    }
+  }
+}
+
 __device__ __forceinline__ float f2_sum(uint64_t v) {
   float a, b;
   f2_unpack(v, a, b);
@@ -339,19 +428,25 @@ __global__ void __launch_bounds__(kThreads, kFwdCtasPerSm) fwd_kernel(const __gr
   fill_shared(p, sh);
   const Place pl = make_place<kInter>(sub, p.D, p.R);
   const bool partial = p.R < p.D;
-  const long long units = p.T * p.chunks, stride = (long long)gridDim.x * kWarps;
-  for (long long unit = (long long)blockIdx.x * kWarps + warp; unit < units; unit += stride) {
-    long long t = unit, b = 0, n = unit;
+  // units: tokens, or with chunks > 1 (few tokens) parts of one
+  const unsigned units = (unsigned)(p.T * p.chunks), stride = gridDim.x * kWarps, N = (unsigned)p.N;
+  Turner turner;
+  turner.start(p, lane);
+  unsigned unit = blockIdx.x * kWarps + warp;
+  auto fetch = [&](unsigned u) {
+    if (u >= units) return;
+    const unsigned t = p.chunks > 1 ? u / (unsigned)p.chunks : u, b = kAppend ? 0u : t / N;
+    turner.fetch(p.ang, b, t - b * N);
+  };
+  fetch(unit);
+  for (; unit < units; unit += stride) {
+    unsigned t = unit;
     int first = 0;
     if (p.chunks > 1) {
-      t = unit / p.chunks;
+      t = unit / (unsigned)p.chunks;
       first = (int)(unit - t * p.chunks) * p.chunk;
-      n = t;
     }
-    if (!kAppend) {
-      b = t / p.N;
-      n = t - b * p.N;
-    }
+    const long long b = kAppend ? 0u : t / N, n = t - (unsigned)b * N;
     const int last = first + p.chunk;
     size_t pool_row = 0;    // append: page and row of this token
     bool put = true;
@@ -391,18 +486,18 @@ __global__ void __launch_bounds__(kThreads, kFwdCtasPerSm) fwd_kernel(const __gr
           Vec8<T> va[kBatch], vb[kBatch];
 #pragma unroll
           for (int u = 0; u < kBatch; ++u) {
-            va[u].zero();
-            vb[u].zero();
-            if (pass + u < hi && h + u * kRows < heads && pl.in) {
-              va[u].load(x + u * kRows * xs + pl.o0);
-              vb[u].load(x + u * kRows * xs + pl.o1);
-            }
+            const bool use = pass + u < hi && h + u * kRows < heads && pl.in;
+            va[u].load(x + u * kRows * xs + pl.o0, use);
+            vb[u].load(x + u * kRows * xs + pl.o1, use);
           }
           if (kind < 2 && !coef) {
             coef = true;
-            if (!angles) make_angles(p.ang, sh, p.R / 2, b, n, lane, sh.cs[warp][0], sh.cs[warp][1]);
+            if (!angles) {
+              turner.make(sh, lane, sh.cs[warp][0], sh.cs[warp][1]);
+              fetch(unit + stride);
+            }
             angles = true;
-            make_coef<kInter, false>(sh.cs[warp][0], sh.cs[warp][1], sh.w[kind], pl, sub, k);
+            make_coef<kInter>(sh.cs[warp][0], sh.cs[warp][1], sh.w[kind], pl, sub, k);
           }
 #pragma unroll
           for (int u = 0; u < kBatch; ++u) {
@@ -451,149 +546,180 @@ __global__ void __launch_bounds__(kThreads, kFwdCtasPerSm) fwd_kernel(const __gr
       }
       begin = end;
     }
+    if (!angles) fetch(unit + stride);   // a unit of values alone
   }
 }
 
-// CTAs [0, side[0].ctas) take the queries, the rest the keys; a warp walks
-// units (token, chunk of passes) of its kind and keeps the weight gradient of
-// its rows in registers; each CTA writes one partial row, summed in a fixed
-// order by dw_kernel (no atomics: the same bits every time).
+// As the forward: a warp walks units of passes, queries' first, then keys'.
+// The weight gradients of a unit's rows go from registers into sums of the
+// lane in shared memory; each CTA writes one partial row of either kind, summed
+// in a fixed order by dw_kernel (no atomics: the same bits every time).
+constexpr int kDwStride = 18;   // floats a lane: 16 sums, and 2 that keep lanes on different banks
 template <typename T, int kLanes, bool kInter>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) bwd_kernel(const __grid_constant__ Params p) {
   constexpr int kRows = 32 / kLanes;
   constexpr int kBatch = sizeof(T) == 4 ? 1 : 2;
   __shared__ __align__(16) Shared sh;
-  __shared__ float s_dw[kWarps][kMaxDim];
+  __shared__ __align__(16) float s_dw[2][kWarps][32][kDwStride];   // sums by lane, queries' and keys'
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int sub = lane % kLanes, row = lane / kLanes;
-  const int kind = (int)blockIdx.x < p.side[0].ctas ? 0 : 1;
-  const int cta = (int)blockIdx.x - (kind ? p.side[0].ctas : 0);
-  const Side& sd = p.side[kind];
   const Place pl = make_place<kInter>(sub, p.D, p.R);
   grid_dep_wait();
   grid_dep_launch_dependents();
   fill_shared(p, sh);
-  const bool norm = sd.w != nullptr, partial = p.R < p.D;
-  const float* wa = sh.w[kind] + (pl.in ? pl.o0 : 0);
-  const float* wb = sh.w[kind] + (pl.in ? pl.o1 : 8);
-  uint64_t da[4], db[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) da[i] = db[i] = 0ull;
-  const int heads = sd.heads, passes = (heads + kRows - 1) / kRows;
-  const int chunk = (passes + p.chunks - 1) / p.chunks;
-  const long long units = p.T * p.chunks, stride = (long long)sd.ctas * kWarps;
-  const long long xs = sd.x.sH * kRows, gs = sd.g.sH * kRows, ys = sd.y.sH * kRows;   // from one pass to the next
-  for (long long unit = (long long)cta * kWarps + warp; unit < units; unit += stride) {
-    long long t = unit;
-    int lo = 0;
+  for (int kind = 0; kind < 2; ++kind)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s_dw[kind][warp][lane][i] = 0.f;
+  const unsigned units = (unsigned)(p.T * p.chunks), stride = gridDim.x * kWarps, N = (unsigned)p.N;
+  Turner turner;
+  turner.start(p, lane);
+  unsigned unit = blockIdx.x * kWarps + warp;
+  auto fetch = [&](unsigned u) {
+    if (u >= units) return;
+    const unsigned t = p.chunks > 1 ? u / (unsigned)p.chunks : u, b = t / N;
+    turner.fetch(p.ang, b, t - b * N);
+  };
+  fetch(unit);
+  for (; unit < units; unit += stride) {
+    unsigned t = unit;
+    int first = 0;
     if (p.chunks > 1) {
-      t = unit / p.chunks;
-      lo = (int)(unit - t * p.chunks) * chunk;
+      t = unit / (unsigned)p.chunks;
+      first = (int)(unit - t * p.chunks) * p.chunk;
     }
-    const long long b = t / p.N, n = t - b * p.N;
-    const int hi = min(lo + chunk, passes);
-    int h = lo * kRows + row;
-    const T* xp = static_cast<const T*>(sd.x.p) + b * sd.x.sB + n * sd.x.sN + h * sd.x.sH;
-    const T* gp = static_cast<const T*>(sd.g.p) + b * sd.g.sB + n * sd.g.sN + h * sd.g.sH;
-    T* yp = static_cast<T*>(sd.y.p) + b * sd.y.sB + n * sd.y.sN + h * sd.y.sH;
-    Coef k;
-    for (int pass = lo; pass < hi; pass += kBatch) {
-      Vec8<T> xa[kBatch], xb[kBatch], ga[kBatch], gb[kBatch];
+    const long long b = t / N, n = t - (unsigned)b * N;
+    const int last = first + p.chunk;
+    bool angles = false;
+    int begin = 0;
+#pragma unroll 1
+    for (int kind = 0; kind < 2; ++kind) {
+      const Side& sd = p.side[kind];
+      const int heads = sd.heads, end = begin + (heads + kRows - 1) / kRows;   // heads: 0 where no gradient is asked for
+      const int lo = max(first, begin), hi = min(last, end);
+      if (lo < hi) {
+        const bool norm = sd.w != nullptr;
+        const float* wa = sh.w[kind] + (pl.in ? pl.o0 : 0);   // lanes without a place hold zeros
+        const float* wb = sh.w[kind] + (pl.in ? pl.o1 : 8);
+        const long long xs = sd.x.sH, gs = sd.g.sH, ys = sd.y.sH;
+        int h = (lo - begin) * kRows + row;
+        const T* xp = static_cast<const T*>(sd.x.p) + b * sd.x.sB + n * sd.x.sN + h * xs;
+        const T* gp = static_cast<const T*>(sd.g.p) + b * sd.g.sB + n * sd.g.sN + h * gs;
+        T* yp = static_cast<T*>(sd.y.p) + b * sd.y.sB + n * sd.y.sN + h * ys;
+        uint64_t da[4], db[4];               // weight gradient of the unit's rows
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
-        xa[u].zero();
-        xb[u].zero();
-        ga[u].zero();
-        gb[u].zero();
-        if (pass + u < hi && h + u * kRows < heads && pl.in) {
-          ga[u].load(gp + u * gs + pl.o0);
-          gb[u].load(gp + u * gs + pl.o1);
-          if (norm) {
-            xa[u].load(xp + u * xs + pl.o0);
-            xb[u].load(xp + u * xs + pl.o1);
+        for (int i = 0; i < 4; ++i) da[i] = db[i] = 0ull;
+        for (int pass = lo; pass < hi; pass += kBatch) {
+          Vec8<T> xa[kBatch], xb[kBatch], ga[kBatch], gb[kBatch];
+#pragma unroll
+          for (int u = 0; u < kBatch; ++u) {
+            const bool use = pass + u < hi && h + u * kRows < heads && pl.in;
+            ga[u].load(gp + u * kRows * gs + pl.o0, use);
+            gb[u].load(gp + u * kRows * gs + pl.o1, use);
+            xa[u].load(xp + u * kRows * xs + pl.o0, use && norm);
+            xb[u].load(xp + u * kRows * xs + pl.o1, use && norm);
           }
+          if (!angles) {
+            back_angles<kInter>(turner, sh, lane, sh.cs[warp][0]);
+            fetch(unit + stride);
+            angles = true;
+          }
+#pragma unroll
+          for (int u = 0; u < kBatch; ++u) {
+            if (pass + u >= hi) break;
+            uint64_t ha[4], hb[4];
+            ga[u].get(ha);
+            gb[u].get(hb);
+            if (pl.rot) turn_back<kInter>(sh.cs[warp][0], sub, ha, hb);   // others: no coefficients of theirs are there
+            if (norm) {
+              uint64_t x[4], y[4], s0 = 0ull, s1 = 0ull, t0 = 0ull, t1 = 0ull, va[4], vb[4];
+              xa[u].get(x);
+              xb[u].get(y);
+#pragma unroll
+              for (int i = 0; i < 4; i += 2) {
+                const ulonglong2 w0 = *reinterpret_cast<const ulonglong2*>(wa + 2 * i), w1 = *reinterpret_cast<const ulonglong2*>(wb + 2 * i);
+                va[i] = f2_mul(ha[i], w0.x);
+                va[i + 1] = f2_mul(ha[i + 1], w0.y);
+                vb[i] = f2_mul(hb[i], w1.x);
+                vb[i + 1] = f2_mul(hb[i + 1], w1.y);
+              }
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                s0 = f2_fma(x[i], x[i], s0);
+                s1 = f2_fma(y[i], y[i], s1);
+                t0 = f2_fma(va[i], x[i], t0);
+                t1 = f2_fma(vb[i], y[i], t1);
+              }
+              const float ss = group_sum<kLanes>(f2_sum(f2_add(s0, s1)));
+              const float dot = group_sum<kLanes>(f2_sum(f2_add(t0, t1)));
+              const float r = rsqrtf(ss * p.inv_d + p.eps);
+              const float q = -dot * p.inv_d * r * r * r;      // dx = r (h w) + x q
+              const uint64_t rr = f2_pack(r, r), qq = f2_pack(q, q);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                da[i] = f2_fma(ha[i], f2_mul(x[i], rr), da[i]);
+                db[i] = f2_fma(hb[i], f2_mul(y[i], rr), db[i]);
+                ha[i] = f2_fma(va[i], rr, f2_mul(x[i], qq));
+                hb[i] = f2_fma(vb[i], rr, f2_mul(y[i], qq));
+              }
+            }
+            if (h + u * kRows < heads && pl.in) {
+              store8(yp + u * kRows * ys + pl.o0, ha);
+              store8(yp + u * kRows * ys + pl.o1, hb);
+            }
+          }
+          h += kBatch * kRows;
+          xp += kBatch * kRows * xs;
+          gp += kBatch * kRows * gs;
+          yp += kBatch * kRows * ys;
         }
-      }
-      if (pass == lo) {
-        make_angles(p.ang, sh, p.R / 2, b, n, lane, sh.cs[warp][0], sh.cs[warp][1]);
-        make_coef<kInter, true>(sh.cs[warp][0], sh.cs[warp][1], nullptr, pl, sub, k);
-      }
-#pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
-        if (pass + u >= hi) break;
-        uint64_t ha[4], hb[4];
-        ga[u].get(ha);
-        gb[u].get(hb);
-        apply_coef<kInter>(k, partial, pl.rot, ha, hb);
-        if (norm) {
-          uint64_t x[4], y[4], s0 = 0ull, s1 = 0ull, t0 = 0ull, t1 = 0ull, va[4], vb[4];
-          xa[u].get(x);
-          xb[u].get(y);
-#pragma unroll
-          for (int i = 0; i < 4; i += 2) {
-            // lanes without a place in the row hold zeros
-            const ulonglong2 w0 = *reinterpret_cast<const ulonglong2*>(wa + 2 * i), w1 = *reinterpret_cast<const ulonglong2*>(wb + 2 * i);
-            va[i] = f2_mul(ha[i], w0.x);
-            va[i + 1] = f2_mul(ha[i + 1], w0.y);
-            vb[i] = f2_mul(hb[i], w1.x);
-            vb[i + 1] = f2_mul(hb[i + 1], w1.y);
-          }
+        if (sd.dw_part != nullptr) {
+          float* mine = s_dw[kind][warp][lane];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            s0 = f2_fma(x[i], x[i], s0);
-            s1 = f2_fma(y[i], y[i], s1);
-            t0 = f2_fma(va[i], x[i], t0);
-            t1 = f2_fma(vb[i], y[i], t1);
+            uint64_t* a = reinterpret_cast<uint64_t*>(mine + 2 * i);
+            uint64_t* c = reinterpret_cast<uint64_t*>(mine + 8 + 2 * i);
+            *a = f2_add(*a, da[i]);
+            *c = f2_add(*c, db[i]);
           }
-          const float ss = group_sum<kLanes>(f2_sum(f2_add(s0, s1)));
-          const float dot = group_sum<kLanes>(f2_sum(f2_add(t0, t1)));
-          const float r = rsqrtf(ss * p.inv_d + p.eps);
-          const float q = -dot * p.inv_d * r * r * r;        // dx = r (h w) + x q
-          const uint64_t rr = f2_pack(r, r), qq = f2_pack(q, q);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            da[i] = f2_fma(ha[i], f2_mul(x[i], rr), da[i]);
-            db[i] = f2_fma(hb[i], f2_mul(y[i], rr), db[i]);
-            ha[i] = f2_fma(va[i], rr, f2_mul(x[i], qq));
-            hb[i] = f2_fma(vb[i], rr, f2_mul(y[i], qq));
-          }
-        }
-        if (h + u * kRows < heads && pl.in) {
-          store8(yp + u * ys + pl.o0, ha);
-          store8(yp + u * ys + pl.o1, hb);
         }
       }
-      h += kBatch * kRows;
-      xp += kBatch * xs;
-      gp += kBatch * gs;
-      yp += kBatch * ys;
+      begin = end;
     }
   }
-  if (sd.dw_part == nullptr) return;
-  // rows of the warp, then the warps
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float v[4];
-    f2_unpack(da[i], v[0], v[1]);
-    f2_unpack(db[i], v[2], v[3]);
+  for (int kind = 0; kind < 2; ++kind) {
+    const Side& sd = p.side[kind];
+    if (sd.dw_part == nullptr) continue;
+    // rows of the warp, then the warps
+    float v[16];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int i = 0; i < 4; ++i) {
+      const float* mine = s_dw[kind][warp][lane];
+      v[2 * i] = mine[2 * i], v[2 * i + 1] = mine[2 * i + 1];
+      v[8 + 2 * i] = mine[8 + 2 * i], v[8 + 2 * i + 1] = mine[8 + 2 * i + 1];
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
 #pragma unroll
       for (int off = kLanes; off < 32; off <<= 1) v[j] += __shfl_xor_sync(0xffffffffu, v[j], off);
     }
+    __syncthreads();                       // the other kind's sums have been read
+    float* sums = sh.cs[warp][0];          // no more angles
     if (row == 0 && pl.in) {
-      s_dw[warp][pl.o0 + 2 * i] = v[0];
-      s_dw[warp][pl.o0 + 2 * i + 1] = v[1];
-      s_dw[warp][pl.o1 + 2 * i] = v[2];
-      s_dw[warp][pl.o1 + 2 * i + 1] = v[3];
-    }
-  }
-  __syncthreads();
-  if ((int)threadIdx.x < p.D) {
-    float v = 0.f;
 #pragma unroll
-    for (int i = 0; i < kWarps; ++i) v += s_dw[i][threadIdx.x];
-    sd.dw_part[(size_t)cta * p.D + threadIdx.x] = v;
+      for (int j = 0; j < 8; ++j) {
+        sums[pl.o0 + j] = v[j];
+        sums[pl.o1 + j] = v[8 + j];
+      }
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < p.D) {
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < kWarps; ++i) sum += (&sh.cs[i][0][0])[threadIdx.x];
+      sd.dw_part[(size_t)blockIdx.x * p.D + threadIdx.x] = sum;
+    }
   }
 }
 
@@ -610,7 +736,7 @@ __global__ void __launch_bounds__(kMaxDim * kDwParts) dw_kernel(const __grid_con
   float v = 0.f;
   if (d < p.D) {
 #pragma unroll 8
-    for (int c = part; c < sd.ctas; c += kDwParts) v += __ldcg(sd.dw_part + (size_t)c * p.D + d);
+    for (int c = part; c < p.ctas; c += kDwParts) v += __ldcg(sd.dw_part + (size_t)c * p.D + d);
   }
   s[part][d] = v;
   __syncthreads();
@@ -691,20 +817,26 @@ inline Rows rows_of(const void* p, const int64_t* st) { return Rows{const_cast<v
 inline int lanes_of(int D) { return D <= 64 ? 4 : 8; }
 inline int passes_of(int heads, int D) { return (heads + 32 / lanes_of(D) - 1) / (32 / lanes_of(D)); }
 
-template <typename T, bool kAppend>
-int launch_fwd(Params& p, bool inter, cudaStream_t st) {
+// Cuts the tokens' passes into units; returns the CTAs.  A warp takes all
+// passes of its token, so that the angles are made once, unless that leaves
+// SMs without work (32 warps on each are wanted; then there are few tokens, and
+// units are far below 2^32).
+inline int share_out(Params& p, int kinds, int ctas_per_sm) {
   int passes = 0;
-  for (int k = 0; k < (kAppend ? 3 : 2); ++k) passes += passes_of(p.side[k].heads, p.D);
-  // A warp takes all passes of its token, so that the angles are made once,
-  // unless that leaves SMs without work (32 warps on each are wanted).
+  for (int k = 0; k < kinds; ++k) passes += p.side[k].heads ? passes_of(p.side[k].heads, p.D) : 0;
   const long long want = (long long)sm_count() * 32;
   p.chunk = (int)std::max<long long>(1, std::min<long long>(passes, p.T * passes / want));
   p.chunks = (passes + p.chunk - 1) / p.chunk;
-  const long long grid = std::min<long long>((p.T * p.chunks + kWarps - 1) / kWarps, (long long)sm_count() * kFwdCtasPerSm);
+  return (int)std::min<long long>((p.T * p.chunks + kWarps - 1) / kWarps, (long long)sm_count() * ctas_per_sm);
+}
+
+template <typename T, bool kAppend>
+int launch_fwd(Params& p, bool inter, cudaStream_t st) {
+  const int grid = share_out(p, kAppend ? 3 : 2, kFwdCtasPerSm);
   const bool wide = lanes_of(p.D) == 8;
   auto* k = wide ? (inter ? fwd_kernel<T, 8, true, kAppend> : fwd_kernel<T, 8, false, kAppend>)
                  : (inter ? fwd_kernel<T, 4, true, kAppend> : fwd_kernel<T, 4, false, kAppend>);
-  return check_cuda(decode::launch_pdl(k, dim3((unsigned)grid), dim3(kThreads), 0, st, p), "norm and rotation launch");
+  return check_cuda(decode::launch_pdl(k, dim3(grid), dim3(kThreads), 0, st, p), "norm and rotation launch");
 }
 
 template <bool kAppend>
@@ -784,7 +916,7 @@ int pu_qk_norm_rope_append(const pu_qk_rope_desc* d, const void* q, const void* 
 
 size_t pu_qk_norm_rope_bwd_workspace_size(int64_t D) {
   if (D <= 0 || D > pu::rope::kMaxDim) return 0;
-  return (size_t)pu::rope::bwd_ctas() * D * sizeof(float);
+  return (size_t)pu::rope::bwd_ctas() * 2 * D * sizeof(float);
 }
 
 int pu_qk_norm_rope_bwd(const pu_qk_rope_desc* d, const void* q, const void* k, const void* gq, const void* gk, void* dq,
@@ -807,19 +939,9 @@ int pu_qk_norm_rope_bwd(const pu_qk_rope_desc* d, const void* q, const void* k, 
   const size_t need = pu_qk_norm_rope_bwd_workspace_size(d->D);
   if ((dq_weight || dk_weight) && (!workspace || workspace_bytes < need || !pu::aligned16(workspace)))
     return pu::set_error(PU_ERR_WORKSPACE, "norm and rotation backward needs %zu bytes of workspace, got %zu", need, workspace_bytes);
-  // warps for the rows of either kind in proportion, each with whole tokens
-  // unless there are fewer tokens than warps
-  const int pq = dq ? passes_of(p.side[0].heads, p.D) : 0, pk = dk ? passes_of(p.side[1].heads, p.D) : 0;
-  const long long most = bwd_ctas();
-  p.chunks = (int)std::max<long long>(1, std::min<long long>(std::max(pq, pk), most * kWarps / p.T));
-  const long long per_kind = (p.T * p.chunks + kWarps - 1) / kWarps;
-  long long nq = pq ? std::max<long long>(1, most * pq / (pq + pk)) : 0;
-  nq = std::min(nq, pk ? most - 1 : most);
-  long long nk = pk ? most - nq : 0;
-  nq = std::min(nq, per_kind);
-  nk = std::min(nk, per_kind);
-  p.side[0].ctas = (int)nq;
-  p.side[1].ctas = (int)nk;
+  if (!dq) p.side[0].heads = 0;
+  if (!dk) p.side[1].heads = 0;
+  p.ctas = share_out(p, 2, kCtasPerSm);
   p.side[0].x = rows_of(q, d->q_stride);
   p.side[1].x = rows_of(k, d->k_stride);
   p.side[0].g = rows_of(gq, d->gq_stride);
@@ -828,12 +950,12 @@ int pu_qk_norm_rope_bwd(const pu_qk_rope_desc* d, const void* q, const void* k, 
   p.side[1].y = rows_of(dk, d->dk_stride);
   float* part = static_cast<float*>(workspace);
   p.side[0].dw_part = dq_weight ? part : nullptr;
-  p.side[1].dw_part = dk_weight ? part + (size_t)nq * d->D : nullptr;
+  p.side[1].dw_part = dk_weight ? part + (size_t)bwd_ctas() * d->D : nullptr;
   p.side[0].dw = dq_weight;
   p.side[1].dw = dk_weight;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool inter = d->interleaved != 0;
-  const int grid = (int)(nq + nk);
+  const int grid = p.ctas;
   rc = d->dtype == PU_DTYPE_F32 ? launch_bwd<float>(p, inter, grid, st)
        : d->dtype == PU_DTYPE_F16 ? launch_bwd<__half>(p, inter, grid, st)
                                   : launch_bwd<__nv_bfloat16>(p, inter, grid, st);
