@@ -11,8 +11,9 @@
 // is bound by reading the pages once.
 //
 // Work.  The tiles of all (sequence, K/V head, slice of 16 query heads) are
-// numbered in one line and cut into as many equal parts as there are CTAs
-// (one per SM), so a ragged batch keeps every SM equally busy whatever the
+// numbered in one line, an item's cost of starting and ending before its
+// tiles, and cut into as many equal parts as there are CTAs (one per SM), so a
+// ragged batch keeps every SM equally busy whatever the
 // lengths, which the host does not know; a grid cut by the table's capacity
 // leaves most SMs idle when sequences are shorter than the table.  A part
 // may begin and end inside a sequence: such an end is written as a record
@@ -88,6 +89,9 @@ struct Cfg {
   static constexpr int kRowBytes = D * (int)sizeof(KVT);
   static constexpr int kBlocks = kRowBytes / 128;          // 128-byte swizzle blocks of a tile
   static_assert(kRowBytes % 128 == 0, "rows are whole swizzle blocks");
+  // what starting and ending a segment costs, in tiles (1.9 us against 0.9 us
+  // a 32 KB tile): parts are cut by tiles plus this for each item
+  static constexpr int kItemCost = BT * kRowBytes == 32768 ? 1 : 2;
   static constexpr int kTile = BT * kRowBytes;
   static constexpr int NS = kTile == 32768 ? 3 : kF8 ? 5 : 6;   // ring stages: 160 to 192 KB in flight
   static constexpr int kQBlock = NP * 128;                 // one swizzle block of one part of q or P
@@ -106,7 +110,8 @@ struct Cfg {
   static constexpr int kOffL = kOffM + 2 * kGroups * NP * 4;     // [2 parities][2 groups][4 warps][NP]
   static constexpr int kOffFac = kOffL + 2 * kGroups * 4 * NP * 4;    // [4 warps][2 groups][NP]
   static constexpr int kOffQinv = kOffFac + 4 * 2 * NP * 4;           // [4 slots][NP]
-  static constexpr int kSmem = kOffQinv + kQSlots * NP * 4;
+  static constexpr int kOffStart = (kOffQinv + kQSlots * NP * 4 + 15) / 16 * 16;
+  static constexpr int kSmem = kOffStart + 96;
   static constexpr int kSCols = kQParts * NP, kOCols = kPParts * NP;
   static constexpr int kColO = 4 * kSCols;                 // four S buffers, then two accumulators per group
   static constexpr int kCols = kColO + 2 * kGroups * kOCols;
@@ -152,7 +157,7 @@ __device__ __forceinline__ void split_e4m3(float a, float b, uint16_t (&part)[N]
 // K/V head * slices + slice); a segment is the CTA's run of one item's tiles.
 struct Walk {
   const Params* p;
-  int b, r, t, tiles, len, inner, left, seg, loc;
+  int b, r, t, tiles, len, inner, left, seg, loc, cost;   // left: the part's units from this tile on
   __device__ __forceinline__ int len_of(int i) const {
     const int n = p->lens[i], cap = p->max_pages << p->page_shift;
     return n < 0 ? 0 : n > cap ? cap : n;
@@ -165,7 +170,9 @@ struct Walk {
     left -= n;
     t += n;
     loc += n;
-    if (left == 0 || t < tiles) return;
+    if (left <= 0 || t < tiles) return;
+    left -= cost;
+    if (left <= 0) return;
     t = loc = 0;
     ++seg;
     if (++r < inner) return;
@@ -175,6 +182,115 @@ struct Walk {
     tiles = (len + BT - 1) / BT;
   }
 };
+
+// A CTA's part of the line of units (an item's cost, then its tiles).
+struct Start {
+  long long ctas, q, rem, first, end;    // parts of q or (the first rem) q + 1 units; this one's
+  long long item0;                       // first unit of sequence b
+  int b, r, t, tiles, len, left, cost;   // the Walk's first tile
+};
+
+template <int kItemCost>
+__device__ __forceinline__ void find_start(const Params& p, int lane, Start* out) {
+  constexpr int kHold = 8;
+  const int inner = p.H_kv * p.slices, cap = p.max_pages << p.page_shift;
+  int len[kHold];
+  // lengths of sequences base + 8 lane + k, in a lane's registers
+  auto load = [&](int base) {
+#pragma unroll
+    for (int k = 0; k < kHold; ++k) {
+      const int i = base + lane * kHold + k;
+      len[k] = i < p.B ? p.lens[i] : 0;
+    }
+#pragma unroll
+    for (int k = 0; k < kHold; ++k) len[k] = max(0, min(len[k], cap));
+  };
+  long long tiles = 0;
+  int items = 0;
+  for (int base = 0; base < p.B; base += 32 * kHold) {
+    load(base);
+#pragma unroll
+    for (int k = 0; k < kHold; ++k) {
+      tiles += (len[k] + BT - 1) / BT;
+      items += len[k] > 0;
+    }
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    tiles += __shfl_xor_sync(0xffffffffu, tiles, off);
+    items += __shfl_xor_sync(0xffffffffu, items, off);
+  }
+  // with no more tiles than CTAs each has one of its own
+  Start s;
+  s.cost = tiles * inner <= (long long)gridDim.x ? 0 : kItemCost;
+  const long long all = (tiles + (long long)items * s.cost) * inner;
+  // no part is empty, so every CTA between an item's first and last has a record
+  s.ctas = min((long long)gridDim.x, all);
+  if (all <= 0xffffffffll) {             // 32-bit division where it does (the 64-bit one takes 1 us)
+    s.q = s.ctas > 0 ? (unsigned)all / (unsigned)s.ctas : 0;
+  } else {
+    s.q = all / s.ctas;
+  }
+  s.rem = all - s.q * s.ctas;
+  const long long c = blockIdx.x;
+  s.first = c < s.ctas ? c * s.q + min(c, s.rem) : 0;
+  s.end = c < s.ctas ? (c + 1) * s.q + min(c + 1, s.rem) : 0;
+  s.left = (int)(s.end - s.first);
+  s.item0 = 0;
+  s.b = s.r = s.t = s.tiles = s.len = 0;
+  if (s.left > 0) {
+    long long before = 0;
+    for (int base = 0;; base += 32 * kHold) {
+      if (p.B > 32 * kHold) load(base);  // otherwise they are still there
+      long long mine = 0;
+#pragma unroll
+      for (int k = 0; k < kHold; ++k) mine += len[k] > 0 ? (len[k] + BT - 1) / BT + s.cost : 0;
+      long long x = mine;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, x, off);
+        if (lane >= off) x += y;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, (before + x) * inner > s.first);
+      if (hit) {
+        // the lane that holds the sequence finds it among its eight
+        const int src = __ffs(hit) - 1;
+        long long at = before + x - mine;
+        bool found = false;
+#pragma unroll
+        for (int k = 0; k < kHold; ++k) {
+          const int n = (len[k] + BT - 1) / BT, units = len[k] > 0 ? n + s.cost : 0;
+          if (!found && (at + units) * inner > s.first) {
+            found = true;
+            s.b = base + lane * kHold + k;
+            s.tiles = n;
+            s.len = len[k];
+            s.item0 = at * inner;
+          }
+          at += units;
+        }
+        if (lane == src) {
+          const long long in = s.first - s.item0;
+          const int per = s.tiles + s.cost;
+          if (in <= 0xffffffffll) {
+            s.r = (int)((unsigned)in / (unsigned)per);
+          } else {
+            s.r = (int)(in / per);
+          }
+          s.t = (int)(in - (long long)s.r * per) - s.cost;
+          if (s.t < 0) {                 // the part begins inside an item's cost
+            s.left += s.t;
+            s.t = 0;
+          }
+          *out = s;
+        }
+        return;
+      }
+      before += __shfl_sync(0xffffffffu, x, 31);
+    }
+  }
+  if (lane == 0) *out = s;
+}
 
 // Sum or maximum of the warp's 16 values per lane over its 32 lanes: lanes 2 h
 // and 2 h + 1 return head h's (each step halves the values a lane still holds).
@@ -238,6 +354,8 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
   float* s_max = reinterpret_cast<float*>(smem + C::kOffMax);
   float* s_m = reinterpret_cast<float*>(smem + C::kOffM);
   float* s_l = reinterpret_cast<float*>(smem + C::kOffL);
+  Start* s_start = reinterpret_cast<Start*>(smem + C::kOffStart);
+  static_assert(sizeof(Start) <= 96, "room for the start");
   float* s_fac = reinterpret_cast<float*>(smem + C::kOffFac);
   float* s_qinv = reinterpret_cast<float*>(smem + C::kOffQinv);
 
@@ -277,55 +395,31 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
   grid_dep_wait();
   grid_dep_launch_dependents();
 
-  // Where this CTA's tiles begin: every warp finds it for itself (two passes
-  // over the lengths, which stay in L1).
-  Walk w0;
-  w0.p = &p;
-  w0.inner = p.H_kv * p.slices;
-  long long all = 0;
-  for (int i = lane; i < p.B; i += 32) all += w0.tiles_of(i);
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) all += __shfl_xor_sync(0xffffffffu, all, off);
-  all *= w0.inner;
-  // no part is empty, so every CTA between an item's first and last has a record
-  const long long ctas = min((long long)gridDim.x, all);
-  // CTA c: tiles [c q + min(c, rem), ...), q or q + 1 of them
-  const long long q = ctas > 0 ? all / ctas : 0, rem = all - q * ctas;
-  auto part = [&](long long c) { return c * q + min(c, rem); };
-  const bool busy = blockIdx.x < ctas;
-  const long long first = busy ? part(blockIdx.x) : 0;
-  w0.left = busy ? (int)(part(blockIdx.x + 1) - first) : 0;
-  w0.b = w0.r = w0.t = w0.tiles = w0.len = w0.seg = w0.loc = 0;
-  long long item0 = 0;                   // number of the current sequence's first tile
-  if (w0.left > 0) {
-    long long before = 0;
-    for (int i0 = 0;; i0 += 32) {
-      const int len = i0 + lane < p.B ? w0.len_of(i0 + lane) : 0, n = (len + BT - 1) / BT;
-      long long x = n;
-#pragma unroll
-      for (int off = 1; off < 32; off <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, x, off);
-        if (lane >= off) x += y;
-      }
-      const unsigned hit = __ballot_sync(0xffffffffu, (before + x) * w0.inner > first);
-      if (hit) {
-        const int src = __ffs(hit) - 1;
-        w0.b = i0 + src;
-        w0.tiles = __shfl_sync(0xffffffffu, n, src);
-        w0.len = __shfl_sync(0xffffffffu, len, src);
-        item0 = (before + __shfl_sync(0xffffffffu, x, src) - w0.tiles) * w0.inner;
-        break;
-      }
-      before += __shfl_sync(0xffffffffu, x, 31);
-    }
-    w0.r = (int)((first - item0) / w0.tiles);
-    w0.t = (int)((first - item0) % w0.tiles);
-  }
+  // Where this CTA's tiles begin.  One warp looks, 256 lengths at a time with
+  // all of a lane's eight loads in flight (32 at a time in every warp took 2 to
+  // 4 us for 256 sequences), and leaves it in shared memory.
+  if (warp == kEndWarps) find_start<C::kItemCost>(p, lane, s_start);
 
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  const Start st = *s_start;
+  // CTA c: units [c q + min(c, rem), ...), q or q + 1 of them
+  const long long ctas = st.ctas, q = st.q, rem = st.rem, first = st.first, end = st.end;
+  auto part = [&](long long c) { return c * q + min(c, rem); };
+  long long item0 = st.item0;
+  Walk w0;
+  w0.p = &p;
+  w0.inner = p.H_kv * p.slices;
+  w0.b = st.b;
+  w0.r = st.r;
+  w0.t = st.t;
+  w0.tiles = st.tiles;
+  w0.len = st.len;
+  w0.left = st.left;
+  w0.cost = st.cost;
+  w0.seg = w0.loc = 0;
 
   if (warp >= kSoftmax / 32 && warp < kEndWarps) {
   reg_dealloc<kRoleRegs>();
@@ -415,7 +509,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
       uint8_t* dst = sQ + slot * C::kQBytes;
       constexpr int kVecs = D / 8;         // 16-byte vectors of a row
       constexpr int kHold = NP * kVecs / 64;   // vectors a lane holds, in two rounds
-#pragma unroll 1
+#pragma unroll
       for (int i0 = 0; i0 < 2 * kHold; i0 += kHold) {
       uint4 v[kHold];
 #pragma unroll
@@ -778,8 +872,8 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
         }
         if (p.lse != nullptr && row < G) p.lse[bh0 + row] = L == 0.f ? -INFINITY : (M + lg2(L)) * kLn2;
       } else {
-        // number of the item's first tile, and the CTAs that hold its tiles
-        const long long i0 = item0 + (long long)r * tiles, i1 = i0 + tiles;
+        // unit of the item's first tile, and the CTAs that hold its tiles
+        const long long i0 = item0 + (long long)r * (tiles + w0.cost) + w0.cost, i1 = i0 + tiles;
         auto holder = [&](long long x) {   // an estimate in fp64 (x is exact there), then its neighbour if it is off
           long long c = x < rem * (q + 1) ? (long long)((double)x / (double)(q + 1)) : (long long)((double)(x - rem) / (double)q);
           if (part(c) > x) --c;
@@ -787,7 +881,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
           return c;
         };
         const long long c0 = i0 >= first ? (long long)blockIdx.x : holder(i0);
-        const long long c1 = i1 <= first + w0.left ? (long long)blockIdx.x : holder(i1 - 1);
+        const long long c1 = i1 <= end ? (long long)blockIdx.x : holder(i1 - 1);
         // this CTA's record: 0 where the item is the first of its part, else 1
         const int which = seg == 0 ? 0 : 1;
         float* rec = p.rec + ((size_t)blockIdx.x * 2 + which) * NP * (D + kHead);
@@ -811,7 +905,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
           // columns are asked for together (one L2 round trip per 8 records)
           const int nrec = (int)(c1 - c0) + 1;
           // the first CTA's record is its second unless the item begins its part
-          const int w_first = part(c0) < i0 ? 1 : 0;
+          const int w_first = part(c0) < i0 - w0.cost ? 1 : 0;
           for (int h = w4; h < G; h += 4) {
             const float* recs = p.rec + ((size_t)c0 * 2 * NP + h) * (D + kHead);
             constexpr size_t kStep = (size_t)2 * NP * (D + kHead), kSecond = (size_t)NP * (D + kHead);
@@ -865,7 +959,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
       // on to the next segment; a new sequence begins behind this one's items
       t += n;
       w.next(n);
-      if (w.left > 0 && w.b != b) item0 += (long long)w.inner * tiles;
+      if (w.left > 0 && w.b != b) item0 += (long long)w.inner * (tiles + w.cost);
     }
     // sequences that hold nothing
     for (int b = blockIdx.x; b < p.B; b += (int)gridDim.x) {
