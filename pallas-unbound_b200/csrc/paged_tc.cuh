@@ -71,7 +71,6 @@ constexpr int kEndWarps = 12;               // first of four
 constexpr int kCtaThreads = 512;
 // registers a thread: softmax 256 x 160, roles 128 x 72, ends 128 x 120 = the launch's 512 x 128
 constexpr int kSoftmaxRegs = 160, kRoleRegs = 72, kEndRegs = 120;
-constexpr int kQSlots = 4;
 constexpr int kHead = 4;                   // floats before o in a record: m, l, and two that keep o 16-byte aligned
 
 template <typename T, typename KVT, int D>
@@ -93,7 +92,8 @@ struct Cfg {
   // a 32 KB tile): parts are cut by tiles plus this for each item
   static constexpr int kItemCost = BT * kRowBytes == 32768 ? 1 : 2;
   static constexpr int kTile = BT * kRowBytes;
-  static constexpr int NS = kTile == 32768 ? 3 : kF8 ? 5 : 6;   // ring stages: 160 to 192 KB in flight
+  static constexpr int NS = kTile == 32768 ? 3 : 6;        // ring stages: 192 KB in flight (e4m3: 57.5 us with 5, see below)
+  static constexpr int kQSlots = kF8 ? 3 : 4;              // segments whose queries are staged ahead
   static constexpr int kQBlock = NP * 128;                 // one swizzle block of one part of q or P
   static constexpr int kQBytes = (kF8 ? kQParts : kBlocks) * kQBlock;
   static constexpr int kPBytes = (kF8 ? kPParts : 2) * kQBlock;   // 16 heads x 128 rows
@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
     paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                     const __grid_constant__ Params p) {
   using C = Cfg<T, KVT, D>;
-  constexpr int NS = C::NS, kQParts = C::kQParts, kPParts = C::kPParts, kTile = C::kTile;
+  constexpr int NS = C::NS, kQSlots = C::kQSlots, kQParts = C::kQParts, kPParts = C::kPParts, kTile = C::kTile;
   constexpr bool kF8 = C::kF8;
   extern __shared__ __align__(1024) uint8_t smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -337,8 +337,8 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
   uint8_t* sP = smem + C::kOffP;
   uint64_t* bFull = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
   uint64_t* bEmpty = bFull + NS;
-  uint64_t* bQfull = bEmpty + NS;        // [4] queries of segment s in slot s & 3
-  uint64_t* bQfree = bQfull + kQSlots;   // [4] its products (and scales, e4m3) have been read
+  uint64_t* bQfull = bEmpty + NS;        // [kQSlots] queries of segment s in slot s % kQSlots
+  uint64_t* bQfree = bQfull + kQSlots;   // [kQSlots] its products (and scales, e4m3) have been read
   uint64_t* bSf = bQfree + kQSlots;      // [4] S of tile t in buffer t & 3
   uint64_t* bSfree = bSf + 4;            // [4] read into registers (an arrival per warp)
   uint64_t* bPf = bSfree + 4;            // [2] P of the group's tile written (128 arrivals)
@@ -367,6 +367,8 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
     for (int s = 0; s < kQSlots; ++s) {
       mbar_init(bQfull + s, 32);
       mbar_init(bQfree + s, kF8 ? 1 + kGroups : 1);
+    }
+    for (int s = 0; s < 4; ++s) {
       mbar_init(bSf + s, 1);
       mbar_init(bSfree + s, 4);
     }
@@ -501,7 +503,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
     for (Walk w = w0; w.left > 0; w.next()) {
       if (w.seg == done) continue;
       done = w.seg;
-      const int slot = w.seg & (kQSlots - 1);
+      const int slot = w.seg % kQSlots;
       if (w.seg >= kQSlots && !mbar_wait(bQfree + slot, (w.seg / kQSlots - 1) & 1, abort_flag, kSiteDecodeTc)) break;
       __syncwarp();
       const int slice = w.r % p.slices, heads = min(NP, p.group - slice * NP);
@@ -566,7 +568,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
       const uint64_t dK0 = make_sdesc_sw128(smem_u32(sKV + kTile), 16, 1024);
       int t = 0;
       for (Walk w = w0; w.left > 0; w.next(), ++t) {
-        const int slot = w.seg & (kQSlots - 1), buf = t & 3;
+        const int slot = w.seg % kQSlots, buf = t & 3;
         if (w.loc == 0 && !mbar_wait(bQfull + slot, (w.seg / kQSlots) & 1, abort_flag, kSiteDecodeTc)) break;
         if (t >= 4 && !mbar_wait(bSfree + buf, ((t >> 2) - 1) & 1, abort_flag, kSiteDecodeTc)) break;
         if (!mbar_wait(bFull + t % NS, (t / NS) & 1, abort_flag, kSiteDecodeTc)) break;
@@ -642,8 +644,8 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
       const int slice = p.slices == 1 ? 0 : w.r % p.slices, G = min(NP, p.group - slice * NP);
       float qf = p.scale_log2, qs[NP];     // e4m3: a factor per head undoes the query's scale
       if constexpr (kF8) {
-        const int slot = seg & 3;
-        mbar_wait(bQfull + slot, (seg >> 2) & 1, abort_flag, kSiteDecodeTc);
+        const int slot = seg % kQSlots;
+        mbar_wait(bQfull + slot, (seg / kQSlots) & 1, abort_flag, kSiteDecodeTc);
 #pragma unroll
         for (int h = 0; h < NP; ++h) qs[h] = s_qinv[slot * NP + h] * p.scale_log2;
         bar_sync_named(1 + grp, 128);
