@@ -57,6 +57,9 @@ _FP8 = getattr(torch, "float8_e4m3fn", None)
 _DT_KV = {**_DT, **({_FP8: _lib.PU_DTYPE_FP8_E4M3} if _FP8 is not None else {})}
 
 
+_paged_decode = None     # kernels.paged.paged_decode, which imports this module
+
+
 class DecodeWorkspace:
     """Zero-initialised device scratch for the split-KV kernels, cached per
     (device, stream).  The kernels leave it zeroed after each call, so one
@@ -137,10 +140,12 @@ def pallas_flash_decoding(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
                           k_scale: float = 1.0, v_scale: float = 1.0):
     """One decode step of attention for a query token per (b, h)."""
     if page_table is not None:
-        from .paged import paged_decode
+        global _paged_decode
+        if _paged_decode is None:
+            from .paged import paged_decode as _paged_decode
         if group is not None or kv_lens is None:
             raise ValueError("a paged cache needs kv_lens and runs on one GPU (group=None)")
-        return paged_decode(q, k_cache, v_cache, page_table, kv_lens, sm_scale=sm_scale,
+        return _paged_decode(q, k_cache, v_cache, page_table, kv_lens, sm_scale=sm_scale,
                             return_lse=return_lse, k_scale=k_scale, v_scale=v_scale)
     if q.dim() != 4 or q.shape[2] != 1:
         raise ValueError("q must be [B, H, 1, D]")

@@ -85,7 +85,7 @@ def paged_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
         sm_scale = 1.0 / math.sqrt(D)
     lib = _lib.lib()
     with _lib.on_device(q.device) as stream:
-        o = torch.empty((B, H, 1, D), dtype=torch.bfloat16, device=q.device)
+        o = torch.empty_like(q, dtype=torch.bfloat16)
         lse = torch.empty((B, H), dtype=torch.float32, device=q.device)
         if B == 0:
             return (o, lse) if return_lse else o
@@ -235,7 +235,7 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, inv_f
         raise ValueError("appended tokens need their positions")
     f, R, pos_st, axes, sizes = _check_angles(inv_freq, positions, sections, D, (T,), dev)
     with _lib.on_device(dev) as stream:
-        q_out = torch.empty((T, H, D), dtype=q.dtype, device=dev)
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
         if T:
             q, k, v = _rows(q), _rows(k), _rows(v)
             by = lambda t: (0, t.stride(1), t.stride(0))     # noqa: E731

@@ -22,6 +22,7 @@ fallback.
 """
 from __future__ import annotations
 
+import functools
 import struct
 from typing import Optional, Sequence
 
@@ -144,10 +145,7 @@ def _description(q, k, inv_freq, positions, q_weight, k_weight, eps, sections, i
     return (B, N, H, k.shape[1], D, q.dtype, R, interleaved, f, positions, pos_st, axes, sizes, wq, wk, float(eps))
 
 
-def qk_norm_rope_forward(q, k, inv_freq, positions=None, *, q_weight=None, k_weight=None, eps: float = 1e-6,
-                         sections: Optional[Sequence[int]] = None, interleaved: bool = False):
-    """`qk_norm_rope` without autograd (pu_qk_norm_rope_fwd on the current stream)."""
-    desc = _description(q, k, inv_freq, positions, q_weight, k_weight, eps, sections, interleaved)
+def _forward(desc, q, k):
     B, N, H, H_kv, D = desc[:5]
     with _lib.on_device(q.device) as stream:
         q_out = torch.empty((B, H, N, D), dtype=q.dtype, device=q.device)
@@ -160,9 +158,54 @@ def qk_norm_rope_forward(q, k, inv_freq, positions=None, *, q_weight=None, k_wei
     return q_out, k_out
 
 
+def qk_norm_rope_forward(q, k, inv_freq, positions=None, *, q_weight=None, k_weight=None, eps: float = 1e-6,
+                         sections: Optional[Sequence[int]] = None, interleaved: bool = False):
+    """`qk_norm_rope` without autograd (pu_qk_norm_rope_fwd on the current stream)."""
+    return _forward(_description(q, k, inv_freq, positions, q_weight, k_weight, eps, sections, interleaved), q, k)
+
+
 def _grad_like(t: torch.Tensor) -> torch.Tensor:
     """A gradient laid out like `t` (a projection's heads stay beside each other)."""
     return torch.empty_like(t) if t.stride(-1) == 1 else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
+@functools.lru_cache(maxsize=64)
+def _bwd_bytes(device: int, D: int) -> int:
+    return int(_lib.lib().pu_qk_norm_rope_bwd_workspace_size(D))
+
+
+def _backward(desc, gq, gk, q, k, want_wq: bool, want_wk: bool):
+    B, N, H, H_kv, D = desc[:5]
+    for g, t in ((gq, q), (gk, k)):
+        if g is not None and (g.shape != t.shape or g.dtype != t.dtype or g.device != t.device):
+            raise ValueError(f"an output gradient must match {tuple(t.shape)} {t.dtype} on {t.device}")
+    if gq is None and gk is None:
+        return None, None, None, None
+    wq, wk = desc[13], desc[14]
+    dq = dk = dwq = dwk = ws = None
+    with _lib.on_device(q.device) as stream:
+        make = torch.empty_like if B * N else torch.zeros_like
+        if gq is not None:
+            dq = _grad_like(q)
+            if want_wq and wq is not None:
+                dwq = make(wq)
+        if gk is not None:
+            dk = _grad_like(k)
+            if want_wk and wk is not None:
+                dwk = make(wk)
+        if B * N:
+            q, k = _rows(q), _rows(k)
+            gq, gk = (None if g is None else _rows(g) for g in (gq, gk))
+            need = 0
+            if dwq is not None or dwk is not None:
+                need = _bwd_bytes(q.device.index, D)
+                ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+            st = lambda t: _NONE if t is None else t.stride()[:3]     # noqa: E731
+            ptr = lambda t: None if t is None else t.data_ptr()       # noqa: E731
+            _lib.check(_lib.lib().pu_qk_norm_rope_bwd(
+                _pack(*desc, st(q), st(k), _NONE, st(gq), st(gk), st(dq), st(dk)), q.data_ptr(), k.data_ptr(),
+                ptr(gq), ptr(gk), ptr(dq), ptr(dk), ptr(dwq), ptr(dwk), ptr(ws), need, stream), "pu_qk_norm_rope_bwd")
+    return dq, dk, dwq, dwk
 
 
 def qk_norm_rope_backward(gq, gk, q, k, inv_freq, positions=None, *, q_weight=None, k_weight=None,
@@ -173,30 +216,7 @@ def qk_norm_rope_backward(gq, gk, q, k, inv_freq, positions=None, *, q_weight=No
     A None output gradient gives None for that side; `weight_grads=False`
     leaves the weights' out.  Calls pu_qk_norm_rope_bwd on the current stream."""
     desc = _description(q, k, inv_freq, positions, q_weight, k_weight, eps, sections, interleaved)
-    B, N, H, H_kv, D = desc[:5]
-    for name, g, t in (("gq", gq, q), ("gk", gk, k)):
-        if g is not None and (g.shape != t.shape or g.dtype != t.dtype or g.device != t.device):
-            raise ValueError(f"{name} must match {tuple(t.shape)} {t.dtype} on {t.device}")
-    if gq is None and gk is None:
-        return None, None, None, None
-    wq, wk = desc[13], desc[14]
-    with _lib.on_device(q.device) as stream:
-        dq, dk = (None if g is None else _grad_like(t) for g, t in ((gq, q), (gk, k)))
-        make = torch.empty_like if B * N else torch.zeros_like
-        dwq = make(wq) if weight_grads and wq is not None and gq is not None else None
-        dwk = make(wk) if weight_grads and wk is not None and gk is not None else None
-        if B * N:
-            lib = _lib.lib()
-            q, k = _rows(q), _rows(k)
-            gq, gk = (None if g is None else _rows(g) for g in (gq, gk))
-            need = int(lib.pu_qk_norm_rope_bwd_workspace_size(D)) if dwq is not None or dwk is not None else 0
-            ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-            st = lambda t: _NONE if t is None else t.stride()[:3]     # noqa: E731
-            ptr = lambda t: None if t is None else t.data_ptr()       # noqa: E731
-            _lib.check(lib.pu_qk_norm_rope_bwd(
-                _pack(*desc, st(q), st(k), _NONE, st(gq), st(gk), st(dq), st(dk)), q.data_ptr(), k.data_ptr(),
-                ptr(gq), ptr(gk), ptr(dq), ptr(dk), ptr(dwq), ptr(dwk), ptr(ws), need, stream), "pu_qk_norm_rope_bwd")
-    return dq, dk, dwq, dwk
+    return _backward(desc, gq, gk, q, k, weight_grads, weight_grads)
 
 
 class _QkNormRope(torch.autograd.Function):
@@ -204,24 +224,23 @@ class _QkNormRope(torch.autograd.Function):
     def forward(ctx, q, k, q_weight, k_weight, inv_freq, positions, eps, sections, interleaved):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(q, k, q_weight, k_weight, inv_freq, positions)
-        ctx.eps, ctx.sections, ctx.interleaved = eps, sections, interleaved
-        return qk_norm_rope_forward(q, k, inv_freq, positions, q_weight=q_weight, k_weight=k_weight, eps=eps,
-                                    sections=sections, interleaved=interleaved)
+        desc = _description(q, k, inv_freq, positions, q_weight, k_weight, eps, sections, interleaved)
+        ctx.plain = desc[:8] + desc[10:13] + desc[15:]     # what holds no tensor
+        return _forward(desc, q, k)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gq, gk):
         q, k, wq, wk, inv_freq, positions = ctx.saved_tensors
-        need = ctx.needs_input_grad
+        need, plain = ctx.needs_input_grad, ctx.plain
         if not (need[0] or need[2]):
             gq = None
         if not (need[1] or need[3]):
             gk = None
-        dq, dk, dwq, dwk = qk_norm_rope_backward(gq, gk, q, k, inv_freq, positions, q_weight=wq, k_weight=wk,
-                                                 eps=ctx.eps, sections=ctx.sections, interleaved=ctx.interleaved,
-                                                 weight_grads=need[2] or need[3])
-        return (dq if need[0] else None, dk if need[1] else None, dwq if need[2] else None,
-                dwk if need[3] else None, None, None, None, None, None)
+        wq, wk = (None if w is None else w.contiguous() for w in (wq, wk))
+        desc = plain[:8] + (inv_freq.contiguous(), positions) + plain[8:11] + (wq, wk) + plain[11:]
+        dq, dk, dwq, dwk = _backward(desc, gq, gk, q, k, need[2], need[3])
+        return (dq if need[0] else None, dk if need[1] else None, dwq, dwk, None, None, None, None, None)
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, inv_freq: torch.Tensor,
