@@ -88,11 +88,13 @@ struct Cfg {
   static constexpr int kRowBytes = D * (int)sizeof(KVT);
   static constexpr int kBlocks = kRowBytes / 128;          // 128-byte swizzle blocks of a tile
   static_assert(kRowBytes % 128 == 0, "rows are whole swizzle blocks");
-  // what starting and ending a segment costs, in tiles (1.9 us against 0.9 us
-  // a 32 KB tile): parts are cut by tiles plus this for each item
+  // What starting and ending a segment costs, in tiles: parts are cut by tiles
+  // plus this for each item (200 e4m3 sequences of up to 4000 tokens, 4 K/V
+  // heads: 115 us with 2, 121 with 1, 128 with 0; 64 KB tiles: 1 and 2 the same).
   static constexpr int kItemCost = BT * kRowBytes == 32768 ? 1 : 2;
   static constexpr int kTile = BT * kRowBytes;
-  static constexpr int NS = kTile == 32768 ? 3 : 6;        // ring stages: 192 KB in flight (e4m3: 57.5 us with 5, see below)
+  // ring stages: 192 KB in flight (16 x 16384 tokens of e4m3, 4 K/V heads: 55.5 us; with 5 stages 57.5)
+  static constexpr int NS = kTile == 32768 ? 3 : 6;
   static constexpr int kQSlots = kF8 ? 3 : 4;              // segments whose queries are staged ahead
   static constexpr int kQBlock = NP * 128;                 // one swizzle block of one part of q or P
   static constexpr int kQBytes = (kF8 ? kQParts : kBlocks) * kQBlock;
@@ -424,211 +426,212 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
   w0.seg = w0.loc = 0;
 
   if (warp >= kSoftmax / 32 && warp < kEndWarps) {
-  reg_dealloc<kRoleRegs>();
-  if (warp == kLoadWarp) {
-    // ---------------- pages -> ring ----------------
-    // The table is read for up to 8 tiles of a segment at a time (lane j * boxes
-    // + i: box i of the j-th), two such batches ahead, or each tile's loads
-    // would wait for its entries first.
-    const int box_shift = 31 - __clz(p.box), boxes = BT >> box_shift, batch = min(32 / boxes, 8);
-    const int lane_tile = lane / boxes, lane_row = (lane & (boxes - 1)) << box_shift, per_page = 1 << p.page_shift;
-    Walk wl = w0;                          // the first tile of the next batch
-    auto look_up = [&]() -> int {
-      const int cnt = min(min(wl.left, wl.tiles - wl.t), batch);
-      const int row = (wl.t + lane_tile) * BT + lane_row;
-      const int32_t* at = p.table + (size_t)wl.b * p.max_pages + (row >> p.page_shift);
-      int pg = -1;
-      asm volatile("{\n .reg .pred q;\n setp.ne.b32 q, %2, 0;\n @q ld.global.b32 %0, [%1];\n}"
-                   : "+r"(pg) : "l"(at), "r"((int)(lane_tile < cnt && row < wl.len)));
-      if (cnt > 0) wl.next(cnt);
-      return pg;
-    };
-    int entries = 0, next1 = look_up(), next2 = look_up();
-    int n = 0, j = 0, cnt = 0, s = 0, turn = 0, seg = -1, head = 0;   // stage s for the turn-th time
-    for (Walk w = w0; w.left > 0; w.next(), ++n, ++j) {
-      if (j == cnt) {
-        j = 0;
-        cnt = min(min(w.left, w.tiles - w.t), batch);
-        entries = next1;
-        next1 = next2;
-        next2 = look_up();
-      }
-      if (w.seg != seg) {
-        seg = w.seg;
-        head = w.r / p.slices;
-      }
-      const int pg = __shfl_sync(0xffffffffu, entries, (j * boxes + lane) & 31), row0 = w.t * BT;
-      const bool mine = lane < boxes && row0 + lane_row < w.len;
-      const bool good = mine && (unsigned)pg < (unsigned)p.num_pages;
-      if (mine && !good) record_device_error(PU_ERR_INVALID_ARGUMENT, kSiteDecodePage);
-      const unsigned loaded = __ballot_sync(0xffffffffu, good);
-      const int outer = pg * p.H_kv + head, in = p.box < BT ? 0 : row0 & (per_page - 1);
-      if (turn > 0 && !mbar_wait(bEmpty + s, (turn - 1) & 1, abort_flag, kSiteDecodeTc)) break;
-      __syncwarp();
-      // box i's coordinates to the issuing thread (all of them ahead of it: a
-      // shuffle and a branch for each box put the boxes one behind the other)
-      int at[8];
+    reg_dealloc<kRoleRegs>();
+    if (warp == kLoadWarp) {
+      // ---------------- pages -> ring ----------------
+      // The table is read for up to 8 tiles of a segment at a time (lane j * boxes
+      // + i: box i of the j-th), two such batches ahead, or each tile's loads
+      // would wait for its entries first.
+      const int box_shift = 31 - __clz(p.box), boxes = BT >> box_shift, batch = min(32 / boxes, 8);
+      const int lane_tile = lane / boxes, lane_row = (lane & (boxes - 1)) << box_shift, per_page = 1 << p.page_shift;
+      Walk wl = w0;                          // the first tile of the next batch
+      auto look_up = [&]() -> int {
+        const int cnt = min(min(wl.left, wl.tiles - wl.t), batch);
+        const int row = (wl.t + lane_tile) * BT + lane_row;
+        const int32_t* at = p.table + (size_t)wl.b * p.max_pages + (row >> p.page_shift);
+        int pg = -1;
+        asm volatile("{\n .reg .pred q;\n setp.ne.b32 q, %2, 0;\n @q ld.global.b32 %0, [%1];\n}"
+                     : "+r"(pg) : "l"(at), "r"((int)(lane_tile < cnt && row < wl.len)));
+        if (cnt > 0) wl.next(cnt);
+        return pg;
+      };
+      int entries = 0, next1 = look_up(), next2 = look_up();
+      int n = 0, j = 0, cnt = 0, s = 0, turn = 0, seg = -1, head = 0;   // stage s for the turn-th time
+      for (Walk w = w0; w.left > 0; w.next(), ++n, ++j) {
+        if (j == cnt) {
+          j = 0;
+          cnt = min(min(w.left, w.tiles - w.t), batch);
+          entries = next1;
+          next1 = next2;
+          next2 = look_up();
+        }
+        if (w.seg != seg) {
+          seg = w.seg;
+          head = w.r / p.slices;
+        }
+        const int pg = __shfl_sync(0xffffffffu, entries, (j * boxes + lane) & 31), row0 = w.t * BT;
+        const bool mine = lane < boxes && row0 + lane_row < w.len;
+        const bool good = mine && (unsigned)pg < (unsigned)p.num_pages;
+        if (mine && !good) record_device_error(PU_ERR_INVALID_ARGUMENT, kSiteDecodePage);
+        const unsigned loaded = __ballot_sync(0xffffffffu, good);
+        const int outer = pg * p.H_kv + head, in = p.box < BT ? 0 : row0 & (per_page - 1);
+        // one answer for the warp: a lane that gave up alone would leave the others at the next vote
+        if (turn > 0 && !__all_sync(0xffffffffu, mbar_wait(bEmpty + s, (turn - 1) & 1, abort_flag, kSiteDecodeTc))) break;
+        // box i's coordinates to the issuing thread (all of them ahead of it: a
+        // shuffle and a branch for each box put the boxes one behind the other)
+        int at[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) at[i] = __shfl_sync(0xffffffffu, outer, i);
+        for (int i = 0; i < 8; ++i) at[i] = __shfl_sync(0xffffffffu, outer, i);
+        if (elect_one_sync()) {
+          s_bad[s] = ~loaded;
+          mbar_arrive_expect_tx(bFull + s, (uint32_t)__popc(loaded) * 2 * p.box * C::kRowBytes);
+          uint8_t* dV = sKV + s * 2 * kTile;
+          const int step = p.box * 128;
+          constexpr int cols = kF8 ? 128 : 64;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if ((loaded >> i) & 1u) {
+#pragma unroll
+              for (int cb = 0; cb < C::kBlocks; ++cb)
+                tma_load_3d(dV + kTile + cb * BT * 128 + i * step, &tmK, bFull + s, cb * cols, in, at[i]);
+#pragma unroll
+              for (int cb = 0; cb < C::kBlocks; ++cb)
+                tma_load_3d(dV + cb * BT * 128 + i * step, &tmV, bFull + s, cb * cols, in, at[i]);
+            }
+          }
+        }
+        __syncwarp();
+        if (++s == NS) {
+          s = 0;
+          ++turn;
+        }
+      }
+      // copies still in flight land before the CTA may exit
+      volatile int no_abort = 0;
+      for (int i = max(0, n - NS); i < n; ++i) mbar_wait(bFull + i % NS, (i / NS) & 1, &no_abort, kSiteDecodeTc);
+    } else if (warp == kQueryWarp) {
+      // ---------------- queries -> shared memory ----------------
+      int done = -1;                         // last segment staged
+      for (Walk w = w0; w.left > 0; w.next()) {
+        if (w.seg == done) continue;
+        done = w.seg;
+        const int slot = w.seg % kQSlots;
+        if (w.seg >= kQSlots &&
+            !__all_sync(0xffffffffu, mbar_wait(bQfree + slot, (w.seg / kQSlots - 1) & 1, abort_flag, kSiteDecodeTc)))
+          break;
+        const int slice = w.r % p.slices, heads = min(NP, p.group - slice * NP);
+        const T* q = static_cast<const T*>(p.q) + ((size_t)w.b * p.H + (w.r / p.slices) * p.group + slice * NP) * D;
+        uint8_t* dst = sQ + slot * C::kQBytes;
+        constexpr int kVecs = D / 8;         // 16-byte vectors of a row
+        constexpr int kHold = NP * kVecs / 64;   // vectors a lane holds, in two rounds
+#pragma unroll
+        for (int i0 = 0; i0 < 2 * kHold; i0 += kHold) {
+          uint4 v[kHold];
+#pragma unroll
+          for (int i = 0; i < kHold; ++i) {
+            const int h = ((i0 + i) * 32 + lane) / kVecs, c = ((i0 + i) * 32 + lane) % kVecs;
+            v[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (h < heads) v[i] = *reinterpret_cast<const uint4*>(q + (size_t)h * D + c * 8);
+          }
+#pragma unroll
+          for (int i = 0; i < kHold; ++i) {
+            const int h = ((i0 + i) * 32 + lane) / kVecs, c = ((i0 + i) * 32 + lane) % kVecs;
+            if constexpr (!kF8) {
+              *reinterpret_cast<uint4*>(dst + (c >> 3) * C::kQBlock + h * 128 + (((c & 7) ^ (h & 7)) << 4)) = v[i];
+            } else {
+              // scaled by a power of two so that the head's largest |q| lies in
+              // [128, 256), then split; 16 lanes hold a head
+              float x[8];
+              unpack8<T>(v[i], x);
+              float mx = 0.f;
+#pragma unroll
+              for (int k = 0; k < 8; ++k) mx = fmaxf(mx, fabsf(x[k]));
+#pragma unroll
+              for (int off = 8; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+              const int e = (mx > 0.f && isfinite(mx)) ? ((__float_as_int(mx) >> 23) & 0xff) - 127 : 7;
+              const int sh = max(-100, min(100, 7 - e));
+              const float up = __int_as_float((127 + sh) << 23), down = __int_as_float((127 - sh) << 23);
+              uint32_t wd[kQParts][2];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                uint16_t pr[kQParts];
+                split_e4m3<false>(x[2 * k] * up, x[2 * k + 1] * up, pr);
+#pragma unroll
+                for (int j = 0; j < kQParts; ++j)
+                  wd[j][k >> 1] = (k & 1) ? (wd[j][k >> 1] | ((uint32_t)pr[j] << 16)) : (uint32_t)pr[j];
+              }
+              const int at = h * 128 + (((c >> 1) ^ (h & 7)) << 4) + (c & 1) * 8;
+#pragma unroll
+              for (int j = 0; j < kQParts; ++j)
+                *reinterpret_cast<uint2*>(dst + j * C::kQBlock + at) = make_uint2(wd[j][0], wd[j][1]);
+              // a head that is not finite makes its scores NaN, as it would in 16 bits
+              if (c == 0) s_qinv[slot * NP + h] = isfinite(mx) ? down : mx - mx;
+            }
+          }
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(bQfull + slot);
+      }
+    } else if (warp == kScoreWarp) {
+      // ---------------- tcgen05: S products ----------------
       if (elect_one_sync()) {
-        s_bad[s] = ~loaded;
-        mbar_arrive_expect_tx(bFull + s, (uint32_t)__popc(loaded) * 2 * p.box * C::kRowBytes);
-        uint8_t* dV = sKV + s * 2 * kTile;
-        const int step = p.box * 128;
-        constexpr int cols = kF8 ? 128 : 64;
+        constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+        constexpr uint32_t idS = kF8 ? make_idesc_e4m3(BT, C::kSCols, 0, 0) : make_idesc_16(BT, NP, 0, 0, kBf16);
+        const uint64_t dQ0 = make_sdesc_sw128(smem_u32(sQ), 16, 1024);
+        const uint64_t dK0 = make_sdesc_sw128(smem_u32(sKV + kTile), 16, 1024);
+        int t = 0;
+        for (Walk w = w0; w.left > 0; w.next(), ++t) {
+          const int slot = w.seg % kQSlots, buf = t & 3;
+          if (w.loc == 0 && !mbar_wait(bQfull + slot, (w.seg / kQSlots) & 1, abort_flag, kSiteDecodeTc)) break;
+          if (t >= 4 && !mbar_wait(bSfree + buf, ((t >> 2) - 1) & 1, abort_flag, kSiteDecodeTc)) break;
+          if (!mbar_wait(bFull + t % NS, (t / NS) & 1, abort_flag, kSiteDecodeTc)) break;
+          tc_fence_after();
+          const uint64_t dk = sdesc_add(dK0, (t % NS) * 2 * kTile), dq = sdesc_add(dQ0, slot * C::kQBytes);
+          const uint32_t col = tmem + buf * C::kSCols;
+          if constexpr (kF8) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if ((loaded >> i) & 1u) {
+            for (int kk = 0; kk < D / 32; ++kk) mma_ss_f8(col, sdesc_add(dk, kk * 32), sdesc_add(dq, kk * 32), idS, kk > 0);
+          } else {
 #pragma unroll
-            for (int cb = 0; cb < C::kBlocks; ++cb)
-              tma_load_3d(dV + kTile + cb * BT * 128 + i * step, &tmK, bFull + s, cb * cols, in, at[i]);
-#pragma unroll
-            for (int cb = 0; cb < C::kBlocks; ++cb)
-              tma_load_3d(dV + cb * BT * 128 + i * step, &tmV, bFull + s, cb * cols, in, at[i]);
+            for (int kk = 0; kk < D / 16; ++kk)
+              mma_ss(col, sdesc_add(dk, (kk >> 2) * (BT * 128) + (kk & 3) * 32),
+                     sdesc_add(dq, (kk >> 2) * C::kQBlock + (kk & 3) * 32), idS, kk > 0);
           }
+          mma_commit(bSf + buf);
+          if (w.last()) mma_commit(bQfree + slot);
         }
+        // every issued product completes before TMEM and shared memory go away
+        mma_commit(bDrain);
+        volatile int no_abort = 0;
+        mbar_wait(bDrain, 0, &no_abort, kSiteDecodeTc);
       }
-      __syncwarp();
-      if (++s == NS) {
-        s = 0;
-        ++turn;
-      }
-    }
-    // copies still in flight land before the CTA may exit
-    volatile int no_abort = 0;
-    for (int i = max(0, n - NS); i < n; ++i) mbar_wait(bFull + i % NS, (i / NS) & 1, &no_abort, kSiteDecodeTc);
-  } else if (warp == kQueryWarp) {
-    // ---------------- queries -> shared memory ----------------
-    int done = -1;                         // last segment staged
-    for (Walk w = w0; w.left > 0; w.next()) {
-      if (w.seg == done) continue;
-      done = w.seg;
-      const int slot = w.seg % kQSlots;
-      if (w.seg >= kQSlots && !mbar_wait(bQfree + slot, (w.seg / kQSlots - 1) & 1, abort_flag, kSiteDecodeTc)) break;
-      __syncwarp();
-      const int slice = w.r % p.slices, heads = min(NP, p.group - slice * NP);
-      const T* q = static_cast<const T*>(p.q) + ((size_t)w.b * p.H + (w.r / p.slices) * p.group + slice * NP) * D;
-      uint8_t* dst = sQ + slot * C::kQBytes;
-      constexpr int kVecs = D / 8;         // 16-byte vectors of a row
-      constexpr int kHold = NP * kVecs / 64;   // vectors a lane holds, in two rounds
+    } else if (warp == kValueWarp) {
+      // ---------------- tcgen05: P V products ----------------
+      if (elect_one_sync()) {
+        constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+        constexpr uint32_t idO = kF8 ? make_idesc_e4m3(128, C::kOCols, 1, 0) : make_idesc_16(128, NP, 1, 0, kBf16);
+        const uint64_t dP0 = make_sdesc_sw128(smem_u32(sP), 16, 1024);
+        // D = 64: M is still 128, with the K tile's 64 columns behind V's as
+        // the other half; its rows of the accumulator are never read
+        const uint64_t dV0 = make_sdesc_sw128(smem_u32(sKV), D == 64 ? kTile : BT * 128, 1024);
+        int t = 0;
+        for (Walk w = w0; w.left > 0; w.next(), ++t) {
+          const int grp = t & 1;
+          const int par = w.seg & 1;
+          if (w.loc == 0 && w.seg > 1 && !mbar_wait(bOfree + par, ((w.seg >> 1) - 1) & 1, abort_flag, kSiteDecodeTc)) break;
+          if (!mbar_wait(bPf + grp, (t >> 1) & 1, abort_flag, kSiteDecodeTc)) break;
+          tc_fence_after();
+          const uint64_t dv = sdesc_add(dV0, (t % NS) * 2 * kTile), dp = sdesc_add(dP0, grp * C::kPBytes);
+          const uint32_t col = tmem + C::kColO + (par * kGroups + grp) * C::kOCols;
+          const bool more = w.loc >= kGroups;    // the group's accumulator already holds tiles of this segment
+          if constexpr (kF8) {
 #pragma unroll
-      for (int i0 = 0; i0 < 2 * kHold; i0 += kHold) {
-      uint4 v[kHold];
+            for (int kk = 0; kk < BT / 32; ++kk)
+              mma_ss_f8(col, sdesc_add(dv, kk * 32 * 128), sdesc_add(dp, kk * 32), idO, more || kk > 0);
+          } else {
 #pragma unroll
-      for (int i = 0; i < kHold; ++i) {
-        const int h = ((i0 + i) * 32 + lane) / kVecs, c = ((i0 + i) * 32 + lane) % kVecs;
-        v[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (h < heads) v[i] = *reinterpret_cast<const uint4*>(q + (size_t)h * D + c * 8);
-      }
-#pragma unroll
-      for (int i = 0; i < kHold; ++i) {
-        const int h = ((i0 + i) * 32 + lane) / kVecs, c = ((i0 + i) * 32 + lane) % kVecs;
-        if constexpr (!kF8) {
-          *reinterpret_cast<uint4*>(dst + (c >> 3) * C::kQBlock + h * 128 + (((c & 7) ^ (h & 7)) << 4)) = v[i];
-        } else {
-          // scaled by a power of two so that the head's largest |q| lies in
-          // [128, 256), then split; 16 lanes hold a head
-          float x[8];
-          unpack8<T>(v[i], x);
-          float mx = 0.f;
-#pragma unroll
-          for (int k = 0; k < 8; ++k) mx = fmaxf(mx, fabsf(x[k]));
-#pragma unroll
-          for (int off = 8; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-          const int e = (mx > 0.f && isfinite(mx)) ? ((__float_as_int(mx) >> 23) & 0xff) - 127 : 7;
-          const int sh = max(-100, min(100, 7 - e));
-          const float up = __int_as_float((127 + sh) << 23), down = __int_as_float((127 - sh) << 23);
-          uint32_t wd[kQParts][2];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            uint16_t pr[kQParts];
-            split_e4m3<false>(x[2 * k] * up, x[2 * k + 1] * up, pr);
-#pragma unroll
-            for (int j = 0; j < kQParts; ++j)
-              wd[j][k >> 1] = (k & 1) ? (wd[j][k >> 1] | ((uint32_t)pr[j] << 16)) : (uint32_t)pr[j];
+            for (int kk = 0; kk < BT / 16; ++kk)
+              mma_ss(col, sdesc_add(dv, kk * 16 * 128), sdesc_add(dp, (kk >> 2) * C::kQBlock + (kk & 3) * 32), idO, more || kk > 0);
           }
-          const int at = h * 128 + (((c >> 1) ^ (h & 7)) << 4) + (c & 1) * 8;
-#pragma unroll
-          for (int j = 0; j < kQParts; ++j)
-            *reinterpret_cast<uint2*>(dst + j * C::kQBlock + at) = make_uint2(wd[j][0], wd[j][1]);
-          // a head that is not finite makes its scores NaN, as it would in 16 bits
-          if (c == 0) s_qinv[slot * NP + h] = isfinite(mx) ? down : mx - mx;
+          mma_commit(bPv + grp);
+          mma_commit(bEmpty + t % NS);
+          if (w.last()) mma_commit(bOdone + par);
         }
+        mma_commit(bDrain + 1);
+        volatile int no_abort = 0;
+        mbar_wait(bDrain + 1, 0, &no_abort, kSiteDecodeTc);
       }
-      }
-      fence_proxy_async_smem();
-      mbar_arrive(bQfull + slot);
     }
-  } else if (warp == kScoreWarp) {
-    // ---------------- tcgen05: S products ----------------
-    if (elect_one_sync()) {
-      constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
-      constexpr uint32_t idS = kF8 ? make_idesc_e4m3(BT, C::kSCols, 0, 0) : make_idesc_16(BT, NP, 0, 0, kBf16);
-      const uint64_t dQ0 = make_sdesc_sw128(smem_u32(sQ), 16, 1024);
-      const uint64_t dK0 = make_sdesc_sw128(smem_u32(sKV + kTile), 16, 1024);
-      int t = 0;
-      for (Walk w = w0; w.left > 0; w.next(), ++t) {
-        const int slot = w.seg % kQSlots, buf = t & 3;
-        if (w.loc == 0 && !mbar_wait(bQfull + slot, (w.seg / kQSlots) & 1, abort_flag, kSiteDecodeTc)) break;
-        if (t >= 4 && !mbar_wait(bSfree + buf, ((t >> 2) - 1) & 1, abort_flag, kSiteDecodeTc)) break;
-        if (!mbar_wait(bFull + t % NS, (t / NS) & 1, abort_flag, kSiteDecodeTc)) break;
-        tc_fence_after();
-        const uint64_t dk = sdesc_add(dK0, (t % NS) * 2 * kTile), dq = sdesc_add(dQ0, slot * C::kQBytes);
-        const uint32_t col = tmem + buf * C::kSCols;
-        if constexpr (kF8) {
-#pragma unroll
-          for (int kk = 0; kk < D / 32; ++kk) mma_ss_f8(col, sdesc_add(dk, kk * 32), sdesc_add(dq, kk * 32), idS, kk > 0);
-        } else {
-#pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk)
-            mma_ss(col, sdesc_add(dk, (kk >> 2) * (BT * 128) + (kk & 3) * 32),
-                   sdesc_add(dq, (kk >> 2) * C::kQBlock + (kk & 3) * 32), idS, kk > 0);
-        }
-        mma_commit(bSf + buf);
-        if (w.last()) mma_commit(bQfree + slot);
-      }
-      // every issued product completes before TMEM and shared memory go away
-      mma_commit(bDrain);
-      volatile int no_abort = 0;
-      mbar_wait(bDrain, 0, &no_abort, kSiteDecodeTc);
-    }
-  } else if (warp == kValueWarp) {
-    // ---------------- tcgen05: P V products ----------------
-    if (elect_one_sync()) {
-      constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
-      constexpr uint32_t idO = kF8 ? make_idesc_e4m3(128, C::kOCols, 1, 0) : make_idesc_16(128, NP, 1, 0, kBf16);
-      const uint64_t dP0 = make_sdesc_sw128(smem_u32(sP), 16, 1024);
-      // D = 64: M is still 128, with the K tile's 64 columns behind V's as
-      // the other half; its rows of the accumulator are never read
-      const uint64_t dV0 = make_sdesc_sw128(smem_u32(sKV), D == 64 ? kTile : BT * 128, 1024);
-      int t = 0;
-      for (Walk w = w0; w.left > 0; w.next(), ++t) {
-        const int grp = t & 1;
-        const int par = w.seg & 1;
-        if (w.loc == 0 && w.seg > 1 && !mbar_wait(bOfree + par, ((w.seg >> 1) - 1) & 1, abort_flag, kSiteDecodeTc)) break;
-        if (!mbar_wait(bPf + grp, (t >> 1) & 1, abort_flag, kSiteDecodeTc)) break;
-        tc_fence_after();
-        const uint64_t dv = sdesc_add(dV0, (t % NS) * 2 * kTile), dp = sdesc_add(dP0, grp * C::kPBytes);
-        const uint32_t col = tmem + C::kColO + (par * kGroups + grp) * C::kOCols;
-        const bool more = w.loc >= kGroups;    // the group's accumulator already holds tiles of this segment
-        if constexpr (kF8) {
-#pragma unroll
-          for (int kk = 0; kk < BT / 32; ++kk)
-            mma_ss_f8(col, sdesc_add(dv, kk * 32 * 128), sdesc_add(dp, kk * 32), idO, more || kk > 0);
-        } else {
-#pragma unroll
-          for (int kk = 0; kk < BT / 16; ++kk)
-            mma_ss(col, sdesc_add(dv, kk * 16 * 128), sdesc_add(dp, (kk >> 2) * C::kQBlock + (kk & 3) * 32), idO, more || kk > 0);
-        }
-        mma_commit(bPv + grp);
-        mma_commit(bEmpty + t % NS);
-        if (w.last()) mma_commit(bOdone + par);
-      }
-      mma_commit(bDrain + 1);
-      volatile int no_abort = 0;
-      mbar_wait(bDrain + 1, 0, &no_abort, kSiteDecodeTc);
-    }
-  }
   } else if (warp < kSoftmax / 32) {
     reg_alloc<kSoftmaxRegs>();
     // ---------------- softmax groups ----------------

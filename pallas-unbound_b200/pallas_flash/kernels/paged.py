@@ -76,7 +76,7 @@ def paged_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     P, H_kv, page_size, D = k_pool.shape
     B, max_pages = page_table.shape
     H = q.shape[1] if q.dim() == 4 else 0
-    if q.shape != (B, H, 1, D) or H == 0 or H % H_kv or q.dtype not in _DT or q.device != k_pool.device:
+    if q.shape != (B, H, 1, D) or H == 0 or H_kv == 0 or H % H_kv or q.dtype not in _DT or q.device != k_pool.device:
         raise ValueError(f"q must be fp16/bf16 CUDA [{B}, multiple of {H_kv}, 1, {D}] on {k_pool.device}")
     q = q.contiguous()
     if q.data_ptr() % 16:

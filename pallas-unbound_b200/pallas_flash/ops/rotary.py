@@ -229,8 +229,13 @@ class _QkNormRope(torch.autograd.Function):
         return _forward(desc, q, k)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, gq, gk):
+        # (the decorator costs more than a small kernel; it only matters where a
+        # graph of the gradients is kept)
+        return _QkNormRope._once(ctx, gq, gk) if torch.is_grad_enabled() else _QkNormRope._grads(ctx, gq, gk)
+
+    @staticmethod
+    def _grads(ctx, gq, gk):
         q, k, wq, wk, inv_freq, positions = ctx.saved_tensors
         need, plain = ctx.needs_input_grad, ctx.plain
         if not (need[0] or need[2]):
@@ -241,6 +246,8 @@ class _QkNormRope(torch.autograd.Function):
         desc = plain[:8] + (inv_freq.contiguous(), positions) + plain[8:11] + (wq, wk) + plain[11:]
         dq, dk, dwq, dwk = _backward(desc, gq, gk, q, k, need[2], need[3])
         return (dq if need[0] else None, dk if need[1] else None, dwq, dwk, None, None, None, None, None)
+
+    _once = staticmethod(once_differentiable(lambda ctx, gq, gk: _QkNormRope._grads(ctx, gq, gk)))
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, inv_freq: torch.Tensor,
