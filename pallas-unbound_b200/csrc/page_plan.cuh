@@ -20,6 +20,11 @@
 // advanced in place, the CTAs form one cluster of 8 and meet at its barrier
 // between the last read of the lengths and the first write; with separate
 // outputs nothing is shared and the grid grows with the work.
+//
+// Bound by latency: one read of the lengths, three scans, the dependent reads
+// of table and ring, one write.  256 sequences with 2048 table entries each
+// (2 MB of table written) and 61 prompts of up to 2500 tokens both take 9 us a
+// call back to back; the call's own host time is 20 us.
 #pragma once
 
 #include "paged.cuh"

@@ -20,12 +20,21 @@
 // turns of the double product it comes from, stays under 2^-23 up to 2^31).
 //
 // A row is spread over D/16 lanes (a group of 4 or 8): each lane holds two
-// 16-byte vectors (8 elements each, for fp32 two loads per vector) which are
-// partners, 8p.. and R/2 + 8p.., so the rotation needs no exchange between
-// lanes and the group reads whole 128-byte lines.  cos and sin are made once
-// per token by the warp, pass through shared memory into registers, and
-// serve all heads of the token that the warp takes.
-// Both kernels are bound by HBM: forward 2, backward 3 passes over the rows.
+// vectors of 8 elements which are partners, 8p.. and R/2 + 8p.., so the rotation
+// needs no exchange between lanes and the group reads whole 128-byte lines.
+// cos and sin are made once per token by the warp, pass through shared memory
+// and serve all heads of the token that the warp takes.  Arithmetic is on
+// packed fp32 pairs; a warp loads several passes' rows before it uses the
+// first, and a token's first rows and the next one's positions before the
+// angles.
+//
+// Both directions read and write each row once: forward 2, backward 3 passes
+// over the rows.  Measured (calls back to back; copy rate 6.4 TB/s): 4 x 4096
+// tokens, 32 + 8 heads of 128, bf16: forward 336 MB in 61 us (5.5 TB/s, 86 %),
+// backward 503 MB in 114 us (4.4 TB/s, 69 %: instructions share the time with
+// the loads; 128 registers and 16 warps an SM measured best, 24 warps with fewer
+// rows in flight 127 us).  17 packed prompts of 15.6 thousand tokens into a
+// cache, 184 MB, 47 us.  64 tokens 4 us.
 #pragma once
 
 #include <cmath>

@@ -16,7 +16,9 @@ len(inv_freq); the values behind R are normed and not rotated.  Everything is
 fp32 inside and rounded once; angles are exact to fp32 at any position.
 
 Differentiable by q, k and the weights (once); the weights' gradients come
-from fixed-order sums, the same bits every time.  Compute runs in
+from fixed-order sums, the same bits every time.  Into a CUDA graph, capture
+`qk_norm_rope_forward` and `qk_norm_rope_backward`: autograd inside a capture
+waits for the streams of eager graphs that hold the same leaves.  Compute runs in
 libpu_attn.so (pu_qk_norm_rope_fwd, pu_qk_norm_rope_bwd); there is no CPU
 fallback.
 """

@@ -324,6 +324,44 @@ def test_two_graphs_at_once(mods):
     assert _lib.device_status() == (0, 0)
 
 
+def test_threads_and_streams(mods):
+    """Decodes of different shapes from several host threads, each on its own
+    stream with its own scratch."""
+    import threading
+    _lib, dec, paged = mods
+    shapes = [(3, 16, 2, 128, 64, [3000, 50, 9000], BF, BF), (20, 8, 2, 64, 16, list(range(0, 400, 20)), HF, HF),
+              (2, 8, 8, 128, 32, [700, 10000], BF, FP8), (1, 32, 4, 128, 64, [20000], HF, HF)]
+    sets = [make(*a[:8], seed=70 + i) for i, a in enumerate(shapes)]
+    want = [paged.paged_decode(*x, return_lse=True) for x in sets]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(40):
+                o, lse = paged.paged_decode(*sets[i], return_lse=True)
+                if not (torch.equal(o, want[i][0]) and torch.equal(lse, want[i][1])):
+                    bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    torch.cuda.synchronize()
+    assert not bad and _lib.device_status() == (0, 0)
+
+
+def test_shared_pages(mods):
+    """Sequences that share their first pages (a common prompt)."""
+    _lib, dec, paged = mods
+    lens, page = [300, 420, 256], 64
+    q, k, v, table, n = make(3, 8, 2, 128, page, lens, BF, BF, 80, width=8)
+    table[1, :4] = table[0, :4]
+    table[2, :4] = table[0, :4]
+    o, lse = paged.paged_decode(q, k, v, table, n, return_lse=True)
+    check(o, lse, q, k, v, table, lens, what="shared")
+    assert _lib.device_status() == (0, 0)
+
+
 # ---------------------------------------------------------------------------
 # norm, rotation and cache write
 # ---------------------------------------------------------------------------

@@ -359,6 +359,52 @@ def test_empty(rot):
     assert dq.shape == q.shape and (dw == 0).all()
 
 
+def test_more_than_2_31_elements(rot):
+    """Rows whose offsets pass 2^31 elements and 2^32 bytes: the last tokens equal
+    the same tokens in a small call, forward and backward."""
+    H, N, D = 20, 900_001, 128
+    f, w = rot.rotary_frequencies(D), 1 + 0.1 * _gen((D,), 5)
+    q = torch.empty((1, H, N, D), dtype=torch.bfloat16, device="cuda")
+    q.random_(-8, 9)
+    k = q[:, :1, :, :]
+    pos = torch.arange(N, device="cuda", dtype=torch.int32)
+    y, yk = rot.qk_norm_rope_forward(q, k, f, pos, q_weight=w, k_weight=w)
+    dq, dk, dw, _ = rot.qk_norm_rope_backward(y, yk, q, k, f, pos, q_weight=w, k_weight=w)
+    for at in (slice(0, 50), slice(N - 50, N)):
+        a, b = (t[:, :, at].contiguous() for t in (q, k))
+        ya, yb = rot.qk_norm_rope_forward(a, b, f, pos[at].contiguous(), q_weight=w, k_weight=w)
+        assert torch.equal(ya, y[:, :, at]) and torch.equal(yb, yk[:, :, at])
+        da, db, _, _ = rot.qk_norm_rope_backward(ya, yb, a, b, f, pos[at].contiguous(), q_weight=w, k_weight=w)
+        assert torch.equal(da, dq[:, :, at]) and torch.equal(db, dk[:, :, at])
+    assert torch.isfinite(dw).all()
+
+
+def test_threads_and_streams(rot):
+    """Calls from several host threads, each on its own stream."""
+    import threading
+    case = (2, 200, 8, 2, 128, 128, torch.bfloat16, torch.float32, False, None)
+    sets = [_inputs(case, seed=60 + i) for i in range(4)]
+    want = [rot.qk_norm_rope_forward(q, k, f, p, q_weight=wq, k_weight=wk) for q, k, wq, wk, f, p, _, _ in sets]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        q, k, wq, wk, f, p, _, _ = sets[i]
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(30):
+                a = [t.detach().requires_grad_(True) for t in (q, k, wq, wk)]
+                y = rot.qk_norm_rope(a[0], a[1], f, p, q_weight=a[2], k_weight=a[3])
+                torch.autograd.grad(y, a, y)
+                if not all(torch.equal(u, v) for u, v in zip(y, want[i])):
+                    bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    torch.cuda.synchronize()
+    assert not bad
+
+
 def test_training_chain(rot):
     """Projection -> norm and rotation -> causal attention -> gradients, against
     the same chain in 64 bits (the attention's own bar for outputs and
