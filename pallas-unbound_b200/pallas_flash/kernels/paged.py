@@ -86,7 +86,7 @@ def paged_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     lib = _lib.lib()
     with _lib.on_device(q.device) as stream:
         o = torch.empty_like(q, dtype=torch.bfloat16)
-        lse = torch.empty((B, H), dtype=torch.float32, device=q.device)
+        lse = torch.empty(B, H, dtype=torch.float32, device=q.device)
         if B == 0:
             return (o, lse) if return_lse else o
         if H == H_kv and k_pool.dtype in _DT and k_scale == 1.0 and v_scale == 1.0:
@@ -147,8 +147,8 @@ def plan_append(page_table: torch.Tensor, kv_lens: torch.Tensor, new_lens: torch
     at least the sum of new_lens, the rest are padding rows.  The free pages
     are free_ring[i % num_pages] for cursor[0] <= i < cursor[1]; pages are
     taken from its head in sequence order.  Where `release` [B] (bool) is set,
-    a sequence's pages go to the ring's tail first and it starts empty; they
-    are handed out from the next call on.
+    a sequence's pages (which no other may share) go to the ring's tail first and
+    it starts empty; they are handed out from the next call on.
 
     A sequence that does not fit its table row or the batch's rows, or for
     which the free pages do not last, is refused: it stays as it is, its rows
@@ -180,8 +180,8 @@ def plan_append(page_table: torch.Tensor, kv_lens: torch.Tensor, new_lens: torch
     if T < 0:
         raise ValueError("num_tokens must not be negative")
     with _lib.on_device(dev) as stream:
-        slots, positions, seq_ids, cu, lens_out = torch.empty(
-            3 * T + 2 * B + 1, dtype=torch.int32, device=dev).split((T, T, T, B + 1, B))
+        slots, positions, seq_ids, cu, lens_out = torch.split_with_sizes(
+            torch.empty(3 * T + 2 * B + 1, dtype=torch.int32, device=dev), (T, T, T, B + 1, B))
         if inplace:
             table_out, lens_out, cursor_out = page_table, kv_lens, cursor
         else:

@@ -150,8 +150,8 @@ def _description(q, k, inv_freq, positions, q_weight, k_weight, eps, sections, i
 def _forward(desc, q, k):
     B, N, H, H_kv, D = desc[:5]
     with _lib.on_device(q.device) as stream:
-        q_out = torch.empty((B, H, N, D), dtype=q.dtype, device=q.device)
-        k_out = torch.empty((B, H_kv, N, D), dtype=q.dtype, device=q.device)
+        q_out = torch.empty(B, H, N, D, dtype=q.dtype, device=q.device)
+        k_out = torch.empty(B, H_kv, N, D, dtype=q.dtype, device=q.device)
         if B * N:
             q, k = _rows(q), _rows(k)
             _lib.check(_lib.lib().pu_qk_norm_rope_fwd(_pack(*desc, q.stride()[:3], k.stride()[:3]), q.data_ptr(),
