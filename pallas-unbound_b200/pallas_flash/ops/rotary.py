@@ -168,7 +168,8 @@ def qk_norm_rope_forward(q, k, inv_freq, positions=None, *, q_weight=None, k_wei
 
 def _grad_like(t: torch.Tensor) -> torch.Tensor:
     """A gradient laid out like `t` (a projection's heads stay beside each other)."""
-    return torch.empty_like(t) if t.stride(-1) == 1 else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    g = torch.empty_like(t)
+    return g if g.stride(-1) == 1 else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 @functools.lru_cache(maxsize=64)

@@ -255,6 +255,27 @@ def test_strides_alignment_and_defaults(rot):
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
+def test_overlapping_windows(rot):
+    """Rows that share elements (windows of one buffer): read as they are or
+    through a copy, and a gradient of its own for every row."""
+    B, H, N, D = 2, 4, 8, 32
+    f = rot.rotary_frequencies(D)
+    w = 1 + 0.1 * _gen((D,), 5)
+    buf = _gen((4096,), 1, torch.bfloat16)
+    k = _gen((B, 1, N, D), 2, torch.bfloat16)
+    gq, gk = _gen((B, H, N, D), 3, torch.bfloat16), _gen((B, 1, N, D), 4, torch.bfloat16)
+    for st in ((1024, 1, 64, 1), (1024, 256, 1, 1), (8, 16, 32, 1), (0, 8, 16, 1)):
+        q = buf.as_strided((B, H, N, D), st)
+        got = rot.qk_norm_rope_backward(gq, gk, q, k, f, q_weight=w, k_weight=w)
+        want = rot.qk_norm_rope_backward(gq, gk, q.contiguous(), k, f, q_weight=w, k_weight=w)
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), st
+        leaf = buf.clone().requires_grad_(True)
+        y, _ = rot.qk_norm_rope(leaf.as_strided((B, H, N, D), st), k, f, q_weight=w, k_weight=w)
+        assert torch.equal(y, rot.qk_norm_rope(q.contiguous(), k, f, q_weight=w, k_weight=w)[0])
+        (grad,) = torch.autograd.grad(y, leaf, gq)
+        assert torch.isfinite(grad).all()
+
+
 def test_broadcast_inputs_and_gradients(rot):
     """A key head expanded over the batch, and a gradient that is one value
     expanded over the output: sums of the rows' gradients."""

@@ -179,3 +179,21 @@ def test_sections_and_positions_are_checked():
         with pytest.raises(ValueError):
             _check_angles(*args, (2, 5), dev)
     assert ctypes.sizeof(ctypes.c_void_p) == 8
+
+
+@pytest.mark.parametrize("shape,stride", [
+    ((2, 4, 8, 32), (1024, 1, 64, 1)), ((2, 4, 8, 32), (1024, 256, 1, 1)), ((2, 4, 8, 32), (0, 256, 32, 1)),
+    ((2, 4, 8, 32), (1024, 32, 128, 1)), ((2, 4, 8, 32), (1024, 1, 4, 32)), ((1, 4, 1, 32), (7, 32, 1, 1)),
+    ((2, 40, 1, 32), (0, 1, 1, 1)), ((2, 4, 64, 16), (0, 0, 1, 1)),
+])
+def test_gradients_have_dense_rows(shape, stride):
+    """Whatever the input's strides (windows that overlap, expanded heads), a
+    gradient has its own element for each and rows on 16-byte boundaries."""
+    from pallas_flash.ops.rotary import _grad_like
+    t = torch.empty(1 << 14, dtype=torch.float16).as_strided(shape, stride)
+    g = _grad_like(t)
+    assert g.shape == t.shape and g.stride(-1) == 1
+    assert all(n == 1 or s % 8 == 0 for n, s in zip(shape[:-1], g.stride()))
+    seen = torch.zeros(g.untyped_storage().nbytes() // 2, dtype=torch.int32)
+    seen.as_strided(g.shape, g.stride()).add_(1)
+    assert int(seen.sum()) == g.numel() and int(seen.max()) == 1
