@@ -80,7 +80,7 @@ inline int check_pages(const int32_t* table, long long max_pages, long long num_
   if (max_pages <= 0 || num_pages <= 0) return set_error(PU_ERR_INVALID_ARGUMENT, "page counts must be positive");
   const int s = log2_exact(page_size);
   if (s < 4 || s > 12) return set_error(PU_ERR_UNSUPPORTED, "page size %lld (power of two in [16, 4096])", page_size);
-  if (num_pages * page_size > (1ll << 31) || max_pages * page_size > (1ll << 30))
+  if (num_pages > (1ll << 31) / page_size || max_pages > (1ll << 30) / page_size)
     return set_error(PU_ERR_UNSUPPORTED, "page pool too large");
   *shift = s;
   return PU_OK;

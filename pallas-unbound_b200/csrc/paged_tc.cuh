@@ -548,7 +548,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
 #pragma unroll
               for (int off = 8; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
               const int e = (mx > 0.f && isfinite(mx)) ? ((__float_as_int(mx) >> 23) & 0xff) - 127 : 7;
-              const int sh = max(-100, min(100, 7 - e));
+              const int sh = min(126, 7 - e);      // -120 at least: 2^sh and 2^-sh are both normal numbers
               const float up = __int_as_float((127 + sh) << 23), down = __int_as_float((127 - sh) << 23);
               uint32_t wd[kQParts][2];
 #pragma unroll
@@ -1057,6 +1057,8 @@ int pu_decode_paged_gqa(const void* q, int q_dtype, const void* k_pool, const vo
   rc = check_args(q, q_dtype, k_pool, v_pool, kv_dtype, B, H, n_cap, D, true);
   if (rc) return rc;
   if (!o || !kv_lens) return pu::set_error(PU_ERR_INVALID_ARGUMENT, "null output or lengths");
+  if (!pu::aligned16(o) || !pu::aligned16(workspace))
+    return pu::set_error(PU_ERR_INVALID_ARGUMENT, "the output and the workspace must be 16-byte aligned");
   if (H_kv <= 0 || H % H_kv != 0)
     return pu::set_error(PU_ERR_INVALID_ARGUMENT, "H = %lld is not a multiple of H_kv = %lld", (long long)H, (long long)H_kv);
   if (num_pages > 2147483647ll / H_kv) return pu::set_error(PU_ERR_UNSUPPORTED, "page pool too large");

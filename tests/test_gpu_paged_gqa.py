@@ -248,6 +248,22 @@ def test_every_e4m3_code(mods):
         check(o, lse, q, k, v, table, [n, 1], None, 0.004, 1.0, f"codes {qdt}")
 
 
+@pytest.mark.parametrize("qdt,power", [(BF, 120), (BF, -120), (HF, 11), (HF, -14)])
+def test_queries_of_any_size(mods, qdt, power):
+    """e4m3 pools: queries near both ends of their type's range, with a k_scale that
+    brings the scores back (a power of two: nothing is rounded by it)."""
+    _lib, dec, paged = mods
+    lens = [1, 129, 700]
+    q, k, v, table, n = make(3, 8, 2, 128, 32, lens, torch.float32, FP8, 11)
+    q = (q.clamp(-4, 4) * 2.0 ** power).to(qdt)
+    assert torch.isfinite(q).all()
+    ks = 2.0 ** -power
+    o, lse = paged.paged_decode(q, k, v, table, n, return_lse=True, k_scale=ks)
+    torch.cuda.synchronize()
+    assert _lib.device_status() == (0, 0)
+    check(o, lse, q, k, v, table, lens, None, ks, 1.0, f"2^{power}")
+
+
 def test_layouts_and_clamps(mods):
     """A strided and an unaligned q, a table wider than needed, lengths behind
     the table and below zero, any scale."""

@@ -181,6 +181,17 @@ def test_sections_and_positions_are_checked():
     assert ctypes.sizeof(ctypes.c_void_p) == 8
 
 
+def test_grouped_paged_decode_alignment_and_page_counts(lib):
+    """An output or workspace off a 16-byte boundary, and page counts whose products pass 64 bits."""
+    _lib, so = lib
+    inv, uns = _lib.PU_ERR_INVALID_ARGUMENT, _lib.PU_ERR_UNSUPPORTED
+    good = [P, 0, P, P, 0, P, 4, 8, 16, P, P, None, P, 1 << 24, 2, 8, 2, 128, 0.1, 1.0, 1.0, None]
+    for at, bad, code in ((10, P + 8, inv), (12, P + 8, inv), (6, (1 << 60) + 1, uns), (7, (1 << 60) + 1, uns), (7, 1 << 28, uns)):
+        a = list(good)
+        a[at] = bad
+        assert so.pu_decode_paged_gqa(*a) == code, (at, bad)
+
+
 @pytest.mark.parametrize("shape,stride", [
     ((2, 4, 8, 32), (1024, 1, 64, 1)), ((2, 4, 8, 32), (1024, 256, 1, 1)), ((2, 4, 8, 32), (0, 256, 32, 1)),
     ((2, 4, 8, 32), (1024, 32, 128, 1)), ((2, 4, 8, 32), (1024, 1, 4, 32)), ((1, 4, 1, 32), (7, 32, 1, 1)),
