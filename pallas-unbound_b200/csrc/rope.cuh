@@ -24,17 +24,17 @@
 // needs no exchange between lanes and the group reads whole 128-byte lines.
 // cos and sin are made once per token by the warp, pass through shared memory
 // and serve all heads of the token that the warp takes.  Arithmetic is on
-// packed fp32 pairs; a warp loads several passes' rows before it uses the
-// first, and a token's first rows and the next one's positions before the
-// angles.
+// packed fp32 pairs; rows reach the warps through a ring in shared memory, asked
+// for two to three passes ahead over the borders of heads and tokens, and the
+// next token's positions before the angles of this one.
 //
 // Both directions read and write each row once: forward 2, backward 3 passes
 // over the rows.  Measured (calls back to back; copy rate 6.4 TB/s): 4 x 4096
-// tokens, 32 + 8 heads of 128, bf16: forward 336 MB in 61 us (5.5 TB/s, 86 %),
-// backward 503 MB in 114 us (4.4 TB/s, 69 %: instructions share the time with
-// the loads; 128 registers and 16 warps an SM measured best, 24 warps with fewer
-// rows in flight 127 us).  17 packed prompts of 15.6 thousand tokens into a
-// cache, 184 MB, 47 us.  64 tokens 4 us.
+// tokens, 32 + 8 heads of 128, bf16: forward 336 MB in 58 us (5.8 TB/s, 91 %),
+// backward 503 MB in 109 us (4.6 TB/s, 72 %: instructions share the time with
+// the copies).  128 registers and 16 warps an SM measured best: 24 warps forward
+// 65 us, 20 warps 64.  17 packed prompts of 15 thousand tokens into a cache,
+// 184 MB, 44 us.  64 tokens 4 us.
 #pragma once
 
 #include <cmath>
@@ -87,8 +87,12 @@ struct Params {
   long long T;            // tokens in all
   int D, R;
   float eps, inv_d;
-  int chunk;              // passes a warp takes of one token
-  int chunks;             // warps per token
+  unsigned whole;         // units below: a token each; the other tokens are cut into parts
+  unsigned units;
+  unsigned step_b, step_n;   // sequences and tokens from a warp's unit to its next
+  int passes;             // of a token
+  int chunk;              // passes of a part
+  int chunks;             // parts of a token
   int ctas;               // backward: CTAs, each with a partial weight gradient
   // append
   const int32_t* slots;   // [T] page * page_size + row, negative: none
@@ -101,8 +105,7 @@ struct Params {
 template <typename T>
 struct Vec8 {
   uint4 w;
-  // zeros where `use` is false (a predicated load, not a branch)
-  __device__ __forceinline__ void load(const T* p, bool use) { w = decode::ld_stream_if(reinterpret_cast<const uint4*>(p), use); }
+  __device__ __forceinline__ void set(int, uint4 x) { w = x; }
   __device__ __forceinline__ void get(uint64_t (&f)[4]) const {
     const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -119,10 +122,7 @@ struct Vec8 {
 template <>
 struct Vec8<float> {
   uint4 w[2];
-  __device__ __forceinline__ void load(const float* p, bool use) {
-    w[0] = decode::ld_stream_if(reinterpret_cast<const uint4*>(p), use);
-    w[1] = decode::ld_stream_if(reinterpret_cast<const uint4*>(p) + 1, use);
-  }
+  __device__ __forceinline__ void set(int c, uint4 x) { w[c] = x; }
   __device__ __forceinline__ void get(uint64_t (&f)[4]) const {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -271,6 +271,38 @@ struct Turner {
   }
 };
 
+// The units of a warp: a token each, or one part of a token's passes.
+struct Unit {
+  unsigned id, b, n;          // the token's sequence and index in it
+  int first, last;            // its passes
+
+  __device__ __forceinline__ void cut(const Params& p) {
+    const unsigned v = id - p.whole, part = v / (unsigned)p.chunks, t = p.whole + part;
+    first = (int)(v - part * p.chunks) * p.chunk;
+    last = first + p.chunk;
+    b = t / (unsigned)p.N;
+    n = t - b * (unsigned)p.N;
+  }
+  __device__ __forceinline__ void start(const Params& p, unsigned warp) {
+    id = warp;
+    first = 0;
+    last = p.passes;
+    b = id / (unsigned)p.N;
+    n = id - b * (unsigned)p.N;
+    if (id >= p.whole) cut(p);
+  }
+  __device__ __forceinline__ void next(const Params& p, unsigned warps) {
+    id += warps;
+    n += p.step_n;                       // whole tokens: no division
+    b += p.step_b;
+    if (n >= (unsigned)p.N) {
+      n -= (unsigned)p.N;
+      ++b;
+    }
+    if (id >= p.whole) cut(p);
+  }
+};
+
 // What a lane of a row group holds: its two vectors' places in the row.
 struct Place {
   int o0, o1;
@@ -305,65 +337,72 @@ __device__ __forceinline__ uint64_t f2_swap(uint64_t v) {
 //   a' = a k0 + x k1,  b' = b k2 + y k3,  (x, y) = (b, a), or interleaved the
 //   vectors' own values with neighbours swapped
 // so the weight, the rotation and its signs cost one product and one fma per
-// two values.
-struct Coef {
-  uint64_t k0[4], k1[4], k2[4], k3[4];
-};
-
-// w: the kind's weights
-template <bool kInter>
-__device__ __forceinline__ void make_coef(const float* cs, const float* sn, const float* w, const Place& pl, int sub, Coef& k) {
-  float c[8], s[8], wa[8], wb[8];
-#pragma unroll
-  for (int i = 0; i < 8; i += 4) {
-    float4 v = make_float4(1.f, 1.f, 1.f, 1.f), u = make_float4(0.f, 0.f, 0.f, 0.f), x = v, y = v;
-    if (pl.rot) {
-      v = *reinterpret_cast<const float4*>(cs + sub * 8 + i);
-      u = *reinterpret_cast<const float4*>(sn + sub * 8 + i);
-    }
-    if (pl.in) {
-      x = *reinterpret_cast<const float4*>(w + pl.o0 + i);
-      y = *reinterpret_cast<const float4*>(w + pl.o1 + i);
-    }
-    c[i] = v.x, c[i + 1] = v.y, c[i + 2] = v.z, c[i + 3] = v.w;
-    s[i] = u.x, s[i + 1] = u.y, s[i + 2] = u.z, s[i + 3] = u.w;
-    wa[i] = x.x, wa[i + 1] = x.y, wa[i + 2] = x.z, wa[i + 3] = x.w;
-    wb[i] = y.x, wb[i + 1] = y.y, wb[i + 2] = y.z, wb[i + 3] = y.w;
+// two values.  They are made once for a token and kind, k_i by the i-th row's lanes, and
+// lie in shared memory as 16-byte pieces [k0 .. k3][2][lane of the row].  (In
+// registers, made by every lane: 17 prompts into a cache 46 us instead of 44.)
+template <bool kInter, int kLanes>
+__device__ __forceinline__ void put_coef(const float* cs, const float* sn, const float* w, const Place& pl, int lane, float4* out) {
+  const int sub = lane % kLanes, which = lane / kLanes;
+  if (which >= 4) return;
+  const bool far = kInter ? which >= 2 : which == 1 || which == 2, sine = which & 1;
+  float4 w0 = make_float4(1.f, 1.f, 1.f, 1.f), w1 = w0;
+  if (pl.in) {
+    const float4* from = reinterpret_cast<const float4*>(w + (far ? pl.o1 : pl.o0));
+    w0 = from[0], w1 = from[1];
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float a0 = wa[2 * i], a1 = wa[2 * i + 1], b0 = wb[2 * i], b1 = wb[2 * i + 1];
+  const float other = sine ? 0.f : 1.f;
+  float4 t0 = make_float4(other, other, other, other), t1 = t0;
+  if (pl.rot) {
+    const float4* from = reinterpret_cast<const float4*>((sine ? sn : cs) + sub * 8);
     if constexpr (kInter) {
-      k.k0[i] = f2_pack(a0 * c[i], a1 * c[i]);
-      k.k1[i] = f2_pack(-a1 * s[i], a0 * s[i]);
-      k.k2[i] = f2_pack(b0 * c[4 + i], b1 * c[4 + i]);
-      k.k3[i] = f2_pack(-b1 * s[4 + i], b0 * s[4 + i]);
+      t0 = from[far];
     } else {
-      k.k0[i] = f2_pack(a0 * c[2 * i], a1 * c[2 * i + 1]);
-      k.k1[i] = f2_pack(-b0 * s[2 * i], -b1 * s[2 * i + 1]);
-      k.k2[i] = f2_pack(b0 * c[2 * i], b1 * c[2 * i + 1]);
-      k.k3[i] = f2_pack(a0 * s[2 * i], a1 * s[2 * i + 1]);
+      t0 = from[0], t1 = from[1];
     }
   }
+  if constexpr (kInter) {
+    if (sine) {
+      w0 = make_float4(-w0.y, w0.x, -w0.w, w0.z);
+      w1 = make_float4(-w1.y, w1.x, -w1.w, w1.z);
+    }
+    t1 = make_float4(t0.z, t0.z, t0.w, t0.w);
+    t0 = make_float4(t0.x, t0.x, t0.y, t0.y);
+  } else if (which == 1) {
+    w0 = make_float4(-w0.x, -w0.y, -w0.z, -w0.w);
+    w1 = make_float4(-w1.x, -w1.y, -w1.z, -w1.w);
+  }
+  out[(2 * which) * kLanes + sub] = make_float4(w0.x * t0.x, w0.y * t0.y, w0.z * t0.z, w0.w * t0.w);
+  out[(2 * which + 1) * kLanes + sub] = make_float4(w1.x * t1.x, w1.y * t1.y, w1.z * t1.z, w1.w * t1.w);
 }
 
-// a, b -> a', b'.  Lanes behind R take no cross term (theirs would be 0 times
+// a, b -> a', b' of kU rows.  Lanes behind R take no cross term (theirs would be 0 times
 // a value that need not be finite).
-template <bool kInter>
-__device__ __forceinline__ void apply_coef(const Coef& k, bool partial, bool rot, uint64_t (&a)[4], uint64_t (&b)[4]) {
-  if (partial && !rot) {
+template <bool kInter, int kLanes, int kU>
+__device__ __forceinline__ void apply_coef(const float4* k, int sub, bool partial, bool rot, uint64_t (&a)[kU][4], uint64_t (&b)[kU][4]) {
+  auto two = [&](int c) { return *reinterpret_cast<const ulonglong2*>(k + c * kLanes + sub); };
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      a[i] = f2_mul(a[i], k.k0[i]);
-      b[i] = f2_mul(b[i], k.k2[i]);
+  for (int half = 0; half < 2; ++half) {
+    const ulonglong2 k0 = two(half), k2 = two(4 + half);
+    if (partial && !rot) {
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        a[u][2 * half] = f2_mul(a[u][2 * half], k0.x);
+        a[u][2 * half + 1] = f2_mul(a[u][2 * half + 1], k0.y);
+        b[u][2 * half] = f2_mul(b[u][2 * half], k2.x);
+        b[u][2 * half + 1] = f2_mul(b[u][2 * half + 1], k2.y);
+      }
+    } else {
+      const ulonglong2 k1 = two(2 + half), k3 = two(6 + half);
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint64_t p = a[u][2 * half + i], q = b[u][2 * half + i];
+          a[u][2 * half + i] = f2_fma(kInter ? f2_swap(p) : q, i ? k1.y : k1.x, f2_mul(p, i ? k0.y : k0.x));
+          b[u][2 * half + i] = f2_fma(kInter ? f2_swap(q) : p, i ? k3.y : k3.x, f2_mul(q, i ? k2.y : k2.x));
+        }
+      }
     }
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint64_t x = kInter ? f2_swap(a[i]) : b[i], y = kInter ? f2_swap(b[i]) : a[i];
-    a[i] = f2_fma(x, k.k1[i], f2_mul(a[i], k.k0[i]));
-    b[i] = f2_fma(y, k.k3[i], f2_mul(b[i], k.k2[i]));
   }
 }
 
@@ -422,45 +461,174 @@ __device__ __forceinline__ float f2_sum(uint64_t v) {
 }
 
 // A pass is 32 / kLanes rows (heads) of one token; queries' passes come
-// first, then keys', then values'.  A warp walks units of `chunk` consecutive
-// passes of one token, kBatch of them loaded before the first is used (and the
-// unit's first ones before the token's angles are made).
+// first, then keys', then values'.  A warp walks units, whole tokens or parts
+// of one; a run is a unit's passes of one kind.
+//
+// Rows come through a ring in shared memory: each lane copies its own
+// vectors of the passes to come (cp.async) into places of its own, kSlots - 2
+// passes ahead, over the borders of runs and tokens.  Nobody else reads them, so a
+// lane waits for its own copies and for no other thread.  (Loads into registers
+// run ahead inside a run only: forward 61 us instead of 58, backward 114 instead of
+// 109, 17 prompts into a cache 48 instead of 44.)
+// kVecs: vectors of 8 a lane copies for a pass, two of the row and, backward, two of its gradient.
+template <typename T, int kLanes, int kKinds, int kVecs>
+struct Feed {
+  static constexpr int kRows = 32 / kLanes;
+  static constexpr int kSlots = sizeof(T) == 4 || kVecs == 4 ? 4 : 5;   // forward, 16-bit: 4 58.9 us, 5 57.8, 6 59.9
+  static constexpr int kChunks = (int)sizeof(T) / 2;        // 16-byte pieces of a vector
+  static constexpr int kSlotBytes = kVecs * kChunks * 512;
+  static constexpr int kBytes = kWarps * kSlots * kSlotBytes;
+  static_assert(kSlots >= 4, "two passes in use, two on their way");
+  Unit unit;
+  unsigned warps;
+  uint32_t base, fill;        // the lane's place in slot 0; byte offset of the slot to fill
+  int gap;                    // bytes between the lane's two vectors
+  int kind, begin;
+  int left, h, heads;         // of the run: passes to ask for; the lane's head, and below which it copies
+  const uint8_t *x, *g;       // the lane's first vector of the next row
+  const uint8_t* safe;        // a row's address for copies that read nothing
+  long long xs, gs;
+  bool norm;
+
+  // to the next run, of this unit or a later one; heads = 0 behind the last
+  __device__ __forceinline__ void run(const Params& p, const Place& pl, int row) {
+    for (; unit.id < p.units; unit.next(p, warps), kind = -1, begin = 0) {
+      while (++kind < kKinds) {
+        const Side& sd = p.side[kind];
+        const int passes = (sd.heads + kRows - 1) / kRows;
+        const int lo = max(unit.first - begin, 0), hi = min(unit.last - begin, passes);
+        begin += passes;
+        if (lo >= hi) continue;
+        left = hi - lo;
+        heads = pl.in ? sd.heads : 0;
+        h = lo * kRows + row;
+        xs = sd.x.sH * (long long)sizeof(T);
+        x = static_cast<const uint8_t*>(sd.x.p) +
+            (unit.b * sd.x.sB + unit.n * sd.x.sN + pl.o0) * (long long)sizeof(T) + h * xs;
+        xs *= kRows;
+        if constexpr (kVecs == 4) {
+          norm = sd.w != nullptr;
+          gs = sd.g.sH * (long long)sizeof(T);
+          g = static_cast<const uint8_t*>(sd.g.p) +
+              (unit.b * sd.g.sB + unit.n * sd.g.sN + pl.o0) * (long long)sizeof(T) + h * gs;
+          gs *= kRows;
+        }
+        return;
+      }
+    }
+    h = heads = 0;                       // (a warp may come here before its first run)
+    left = 1 << 30;
+  }
+  // Asks for one pass; zeros where the lane has no row or no place in it.
+  __device__ __forceinline__ void ask(const Params& p, const Place& pl, int row) {
+    const uint32_t to = base + fill;
+    const bool use = h < heads;
+    auto copy = [&](int v, const uint8_t* from, bool read) {
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + (v * kChunks + c) * 512), "l"(from + c * 16),
+                     "r"(read ? 16 : 0)
+                     : "memory");
+    };
+    const int far = use ? gap : 0;
+    const uint8_t* from = use ? x : safe;
+    copy(0, from, use && (kVecs == 2 || norm));
+    copy(1, from + far, use && (kVecs == 2 || norm));
+    if constexpr (kVecs == 4) {
+      const uint8_t* grad = use ? g : safe;
+      copy(2, grad, use);
+      copy(3, grad + far, use);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    fill = fill + kSlotBytes == kSlots * kSlotBytes ? 0 : fill + kSlotBytes;
+    h += kRows;
+    x += xs;
+    if constexpr (kVecs == 4) g += gs;
+    if (--left == 0) run(p, pl, row);
+  }
+  __device__ __forceinline__ void start(const Params& p, uint8_t* smem, int warp, int lane, const Place& pl) {
+    base = smem_u32(smem) + (uint32_t)(warp * kSlots * kSlotBytes + lane * 16);
+    gap = (pl.o1 - pl.o0) * (int)sizeof(T);
+    warps = gridDim.x * kWarps;
+    fill = 0;
+    kind = -1;
+    begin = 0;
+    x = g = nullptr;
+    xs = gs = 0;
+    safe = static_cast<const uint8_t*>(p.side[p.side[0].heads > 0 ? 0 : 1].x.p);
+    unit.start(p, blockIdx.x * kWarps + warp);
+    run(p, pl, lane / kLanes);
+    for (int i = 0; i + 2 < kSlots; ++i) ask(p, pl, lane / kLanes);
+  }
+  // Waits for the next kU passes (1 or 2) and returns the place of the first.
+  template <int kU>
+  __device__ __forceinline__ void wait() const {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kSlots - 2 - kU) : "memory");
+  }
+  __device__ __forceinline__ void get(int u, int v, uint64_t (&f)[4]) const {
+    const uint32_t off = fill + (2 + u) * kSlotBytes, at = base + (off >= kSlots * kSlotBytes ? off - kSlots * kSlotBytes : off);
+    Vec8<T> x;
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+      uint4 w;
+      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
+                   : "r"(at + (v * kChunks + c) * 512)
+                   : "memory");
+      x.set(c, w);
+    }
+    x.get(f);
+  }
+  // The vectors of the next kU passes.  The slots that are refilled are those of
+  // the two passes before, whose values have been used.
+  template <int kU>
+  __device__ __forceinline__ void take(const Params& p, const Place& pl, int row, uint64_t (&a)[kU][4], uint64_t (&c)[kU][4]) {
+    wait<kU>();
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      get(u, 0, a[u]);
+      get(u, 1, c[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kU; ++u) ask(p, pl, row);
+  }
+};
+
 template <typename T, int kLanes, bool kInter, bool kAppend>
 __global__ void __launch_bounds__(kThreads, kFwdCtasPerSm) fwd_kernel(const __grid_constant__ Params p) {
   constexpr int kRows = 32 / kLanes;
-  constexpr int kBatch = sizeof(T) == 4 ? 2 : 4;
+  extern __shared__ __align__(16) uint8_t smem[];
   __shared__ __align__(16) Shared sh;
+  __shared__ float4 s_coef[kWarps][2][8 * kLanes];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int sub = lane % kLanes, row = lane / kLanes;
   grid_dep_wait();
   grid_dep_launch_dependents();
-  fill_shared(p, sh);
   const Place pl = make_place<kInter>(sub, p.D, p.R);
+  Feed<T, kLanes, kAppend ? 3 : 2, 2> feed;
+  feed.start(p, smem, warp, lane, pl);
+  fill_shared(p, sh);
   const bool partial = p.R < p.D;
-  // units: tokens, or with chunks > 1 (few tokens) parts of one
-  const unsigned units = (unsigned)(p.T * p.chunks), stride = gridDim.x * kWarps, N = (unsigned)p.N;
   Turner turner;
   turner.start(p, lane);
-  unsigned unit = blockIdx.x * kWarps + warp;
-  auto fetch = [&](unsigned u) {
-    if (u >= units) return;
-    const unsigned t = p.chunks > 1 ? u / (unsigned)p.chunks : u, b = kAppend ? 0u : t / N;
-    turner.fetch(p.ang, b, t - b * N);
+  int next_slot = -1;        // append: where the next unit's token goes
+  Unit next;
+  auto fetch = [&] {
+    if (next.id >= p.units) return;
+    turner.fetch(p.ang, next.b, next.n);
+    if (kAppend) next_slot = p.slots[next.n];
   };
-  fetch(unit);
-  for (; unit < units; unit += stride) {
-    unsigned t = unit;
-    int first = 0;
-    if (p.chunks > 1) {
-      t = unit / (unsigned)p.chunks;
-      first = (int)(unit - t * p.chunks) * p.chunk;
-    }
-    const long long b = kAppend ? 0u : t / N, n = t - (unsigned)b * N;
-    const int last = first + p.chunk;
+  next.start(p, blockIdx.x * kWarps + warp);
+  fetch();
+  while (next.id < p.units) {
+    const Unit unit = next;
+    const int first = unit.first, last = unit.last;
+    const long long b = unit.b, n = unit.n;
+    next.next(p, gridDim.x * kWarps);
     size_t pool_row = 0;    // append: page and row of this token
     bool put = true;
     if constexpr (kAppend) {
-      const long long slot = p.slots[t];
+      const long long slot = next_slot;
       put = slot >= 0 && slot < p.num_slots;
       if (slot >= p.num_slots && lane == 0) record_device_error(PU_ERR_INVALID_ARGUMENT, kSiteAppendSlot);
       pool_row = put ? (size_t)slot : 0;
@@ -475,8 +643,6 @@ __global__ void __launch_bounds__(kThreads, kFwdCtasPerSm) fwd_kernel(const __gr
       if (lo < hi) {
         // the lane's rows of the kind: head h, then kRows heads further, ...
         int h = (lo - begin) * kRows + row;
-        const long long xs = sd.x.sH;
-        const T* x = static_cast<const T*>(sd.x.p) + b * sd.x.sB + n * sd.x.sN + h * xs;
         const bool norm = kind < 2 && sd.w != nullptr;
         constexpr bool kPool = kAppend;
         T* y = nullptr;
@@ -489,73 +655,80 @@ __global__ void __launch_bounds__(kThreads, kFwdCtasPerSm) fwd_kernel(const __gr
           ys = sd.y.sH;
           y = static_cast<T*>(sd.y.p) + b * sd.y.sB + n * sd.y.sN + h * ys;
         }
-        Coef k;
-        bool coef = false;
-        for (int pass = lo; pass < hi; pass += kBatch) {
-          Vec8<T> va[kBatch], vb[kBatch];
+        if (kind < 2 && !angles) {
+          turner.make(sh, lane, sh.cs[warp][0], sh.cs[warp][1]);
+          put_coef<kInter, kLanes>(sh.cs[warp][0], sh.cs[warp][1], sh.w[0], pl, lane, s_coef[warp][0]);
+          put_coef<kInter, kLanes>(sh.cs[warp][0], sh.cs[warp][1], sh.w[1], pl, lane, s_coef[warp][1]);
+          __syncwarp();
+          fetch();
+          angles = true;
+        }
+        // kU passes, their chains of sums and shuffles side by side
+        auto passes = [&](auto count) {
+          constexpr int kU = decltype(count)::value;
+          uint64_t a[kU][4], bb[kU][4];
+          feed.take(p, pl, row, a, bb);
+          if (kind < 2) {
+            uint64_t rr[kU];
+            if (norm) {
+              float ss[kU];
 #pragma unroll
-          for (int u = 0; u < kBatch; ++u) {
-            const bool use = pass + u < hi && h + u * kRows < heads && pl.in;
-            va[u].load(x + u * kRows * xs + pl.o0, use);
-            vb[u].load(x + u * kRows * xs + pl.o1, use);
-          }
-          if (kind < 2 && !coef) {
-            coef = true;
-            if (!angles) {
-              turner.make(sh, lane, sh.cs[warp][0], sh.cs[warp][1]);
-              fetch(unit + stride);
-            }
-            angles = true;
-            make_coef<kInter>(sh.cs[warp][0], sh.cs[warp][1], sh.w[kind], pl, sub, k);
-          }
-#pragma unroll
-          for (int u = 0; u < kBatch; ++u) {
-            if (pass + u >= hi) break;
-            uint64_t a[4], bb[4];
-            va[u].get(a);
-            vb[u].get(bb);
-            if (kind < 2) {
-              uint64_t rr = 0ull;
-              if (norm) {
+              for (int u = 0; u < kU; ++u) {
                 uint64_t s0 = 0ull, s1 = 0ull;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                  s0 = f2_fma(a[i], a[i], s0);
-                  s1 = f2_fma(bb[i], bb[i], s1);
+                  s0 = f2_fma(a[u][i], a[u][i], s0);
+                  s1 = f2_fma(bb[u][i], bb[u][i], s1);
                 }
-                const float r = rsqrtf(group_sum<kLanes>(f2_sum(f2_add(s0, s1))) * p.inv_d + p.eps);
-                rr = f2_pack(r, r);
+                ss[u] = f2_sum(f2_add(s0, s1));
               }
-              apply_coef<kInter>(k, partial, pl.rot, a, bb);
-              if (norm) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  a[i] = f2_mul(a[i], rr);
-                  bb[i] = f2_mul(bb[i], rr);
-                }
+              for (int off = kLanes / 2; off > 0; off >>= 1)
+#pragma unroll
+                for (int u = 0; u < kU; ++u) ss[u] += __shfl_xor_sync(0xffffffffu, ss[u], off);
+#pragma unroll
+              for (int u = 0; u < kU; ++u) {
+                const float r = rsqrtf(ss[u] * p.inv_d + p.eps);
+                rr[u] = f2_pack(r, r);
               }
             }
+            apply_coef<kInter, kLanes>(s_coef[warp][kind & 1], sub, partial, pl.rot, a, bb);
+            if (norm) {
+#pragma unroll
+              for (int u = 0; u < kU; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  a[u][i] = f2_mul(a[u][i], rr[u]);
+                  bb[u][i] = f2_mul(bb[u][i], rr[u]);
+                }
+            }
+          }
+#pragma unroll
+          for (int u = 0; u < kU; ++u) {
             if (h + u * kRows < heads && pl.in) {
               if (kPool && kind > 0) {
                 if (put) {
-                  store8_pool(sd.y.p, at + u * kRows * ys + pl.o0, p.pool_dtype, sd.unit, a);
-                  store8_pool(sd.y.p, at + u * kRows * ys + pl.o1, p.pool_dtype, sd.unit, bb);
+                  store8_pool(sd.y.p, at + u * kRows * ys + pl.o0, p.pool_dtype, sd.unit, a[u]);
+                  store8_pool(sd.y.p, at + u * kRows * ys + pl.o1, p.pool_dtype, sd.unit, bb[u]);
                 }
               } else {
-                store8(y + u * kRows * ys + pl.o0, a);
-                store8(y + u * kRows * ys + pl.o1, bb);
+                store8(y + u * kRows * ys + pl.o0, a[u]);
+                store8(y + u * kRows * ys + pl.o1, bb[u]);
               }
             }
           }
-          h += kBatch * kRows;
-          x += kBatch * kRows * xs;
-          y += kBatch * kRows * ys;
-          at += kBatch * kRows * ys;
-        }
+          h += kU * kRows;
+          y += kU * kRows * ys;
+          at += kU * kRows * ys;
+        };
+        int pass = lo;
+#pragma unroll 1
+        for (; pass + 1 < hi; pass += 2) passes(std::integral_constant<int, 2>());
+        if (pass < hi) passes(std::integral_constant<int, 1>());
       }
       begin = end;
     }
-    if (!angles) fetch(unit + stride);   // a unit of values alone
+    if (!angles) fetch();   // a unit of values alone
   }
 }
 
@@ -567,7 +740,7 @@ constexpr int kDwStride = 18;   // floats a lane: 16 sums, and 2 that keep lanes
 template <typename T, int kLanes, bool kInter>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) bwd_kernel(const __grid_constant__ Params p) {
   constexpr int kRows = 32 / kLanes;
-  constexpr int kBatch = sizeof(T) == 4 ? 1 : 2;
+  extern __shared__ __align__(16) uint8_t smem[];
   __shared__ __align__(16) Shared sh;
   __shared__ __align__(16) float s_dw[2][kWarps][32][kDwStride];   // sums by lane, queries' and keys'
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -575,30 +748,26 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) bwd_kernel(const __grid_
   const Place pl = make_place<kInter>(sub, p.D, p.R);
   grid_dep_wait();
   grid_dep_launch_dependents();
+  Feed<T, kLanes, 2, 4> feed;
+  feed.start(p, smem, warp, lane, pl);
   fill_shared(p, sh);
 #pragma unroll
   for (int kind = 0; kind < 2; ++kind)
 #pragma unroll
     for (int i = 0; i < 16; ++i) s_dw[kind][warp][lane][i] = 0.f;
-  const unsigned units = (unsigned)(p.T * p.chunks), stride = gridDim.x * kWarps, N = (unsigned)p.N;
   Turner turner;
   turner.start(p, lane);
-  unsigned unit = blockIdx.x * kWarps + warp;
-  auto fetch = [&](unsigned u) {
-    if (u >= units) return;
-    const unsigned t = p.chunks > 1 ? u / (unsigned)p.chunks : u, b = t / N;
-    turner.fetch(p.ang, b, t - b * N);
+  Unit next;
+  auto fetch = [&] {
+    if (next.id < p.units) turner.fetch(p.ang, next.b, next.n);
   };
-  fetch(unit);
-  for (; unit < units; unit += stride) {
-    unsigned t = unit;
-    int first = 0;
-    if (p.chunks > 1) {
-      t = unit / (unsigned)p.chunks;
-      first = (int)(unit - t * p.chunks) * p.chunk;
-    }
-    const long long b = t / N, n = t - (unsigned)b * N;
-    const int last = first + p.chunk;
+  next.start(p, blockIdx.x * kWarps + warp);
+  fetch();
+  while (next.id < p.units) {
+    const Unit unit = next;
+    const int first = unit.first, last = unit.last;
+    const long long b = unit.b, n = unit.n;
+    next.next(p, gridDim.x * kWarps);
     bool angles = false;
     int begin = 0;
 #pragma unroll 1
@@ -610,77 +779,64 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) bwd_kernel(const __grid_
         const bool norm = sd.w != nullptr;
         const float* wa = sh.w[kind] + (pl.in ? pl.o0 : 0);   // lanes without a place hold zeros
         const float* wb = sh.w[kind] + (pl.in ? pl.o1 : 8);
-        const long long xs = sd.x.sH, gs = sd.g.sH, ys = sd.y.sH;
+        const long long ys = sd.y.sH;
         int h = (lo - begin) * kRows + row;
-        const T* xp = static_cast<const T*>(sd.x.p) + b * sd.x.sB + n * sd.x.sN + h * xs;
-        const T* gp = static_cast<const T*>(sd.g.p) + b * sd.g.sB + n * sd.g.sN + h * gs;
         T* yp = static_cast<T*>(sd.y.p) + b * sd.y.sB + n * sd.y.sN + h * ys;
         uint64_t da[4], db[4];               // weight gradient of the unit's rows
 #pragma unroll
         for (int i = 0; i < 4; ++i) da[i] = db[i] = 0ull;
-        for (int pass = lo; pass < hi; pass += kBatch) {
-          Vec8<T> xa[kBatch], xb[kBatch], ga[kBatch], gb[kBatch];
+        if (!angles) {
+          back_angles<kInter>(turner, sh, lane, sh.cs[warp][0]);
+          fetch();
+          angles = true;
+        }
+#pragma unroll 1
+        for (int pass = lo; pass < hi; ++pass) {
+          const bool use = h < heads && pl.in;
+          uint64_t x[4], y[4], ha[4], hb[4];
+          feed.template wait<1>();
+          feed.get(0, 2, ha);
+          feed.get(0, 3, hb);
+          feed.get(0, 0, x);
+          feed.get(0, 1, y);
+          feed.ask(p, pl, row);
+          if (pl.rot) turn_back<kInter>(sh.cs[warp][0], sub, ha, hb);   // others: no coefficients of theirs are there
+          if (norm) {
+            uint64_t s0 = 0ull, s1 = 0ull, t0 = 0ull, t1 = 0ull, va[4], vb[4];
 #pragma unroll
-          for (int u = 0; u < kBatch; ++u) {
-            const bool use = pass + u < hi && h + u * kRows < heads && pl.in;
-            ga[u].load(gp + u * kRows * gs + pl.o0, use);
-            gb[u].load(gp + u * kRows * gs + pl.o1, use);
-            xa[u].load(xp + u * kRows * xs + pl.o0, use && norm);
-            xb[u].load(xp + u * kRows * xs + pl.o1, use && norm);
-          }
-          if (!angles) {
-            back_angles<kInter>(turner, sh, lane, sh.cs[warp][0]);
-            fetch(unit + stride);
-            angles = true;
-          }
-#pragma unroll
-          for (int u = 0; u < kBatch; ++u) {
-            if (pass + u >= hi) break;
-            uint64_t ha[4], hb[4];
-            ga[u].get(ha);
-            gb[u].get(hb);
-            if (pl.rot) turn_back<kInter>(sh.cs[warp][0], sub, ha, hb);   // others: no coefficients of theirs are there
-            if (norm) {
-              uint64_t x[4], y[4], s0 = 0ull, s1 = 0ull, t0 = 0ull, t1 = 0ull, va[4], vb[4];
-              xa[u].get(x);
-              xb[u].get(y);
-#pragma unroll
-              for (int i = 0; i < 4; i += 2) {
-                const ulonglong2 w0 = *reinterpret_cast<const ulonglong2*>(wa + 2 * i), w1 = *reinterpret_cast<const ulonglong2*>(wb + 2 * i);
-                va[i] = f2_mul(ha[i], w0.x);
-                va[i + 1] = f2_mul(ha[i + 1], w0.y);
-                vb[i] = f2_mul(hb[i], w1.x);
-                vb[i + 1] = f2_mul(hb[i + 1], w1.y);
-              }
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                s0 = f2_fma(x[i], x[i], s0);
-                s1 = f2_fma(y[i], y[i], s1);
-                t0 = f2_fma(va[i], x[i], t0);
-                t1 = f2_fma(vb[i], y[i], t1);
-              }
-              const float ss = group_sum<kLanes>(f2_sum(f2_add(s0, s1)));
-              const float dot = group_sum<kLanes>(f2_sum(f2_add(t0, t1)));
-              const float r = rsqrtf(ss * p.inv_d + p.eps);
-              const float q = -dot * p.inv_d * r * r * r;      // dx = r (h w) + x q
-              const uint64_t rr = f2_pack(r, r), qq = f2_pack(q, q);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                da[i] = f2_fma(ha[i], f2_mul(x[i], rr), da[i]);
-                db[i] = f2_fma(hb[i], f2_mul(y[i], rr), db[i]);
-                ha[i] = f2_fma(va[i], rr, f2_mul(x[i], qq));
-                hb[i] = f2_fma(vb[i], rr, f2_mul(y[i], qq));
-              }
+            for (int i = 0; i < 4; i += 2) {
+              const ulonglong2 w0 = *reinterpret_cast<const ulonglong2*>(wa + 2 * i), w1 = *reinterpret_cast<const ulonglong2*>(wb + 2 * i);
+              va[i] = f2_mul(ha[i], w0.x);
+              va[i + 1] = f2_mul(ha[i + 1], w0.y);
+              vb[i] = f2_mul(hb[i], w1.x);
+              vb[i + 1] = f2_mul(hb[i + 1], w1.y);
             }
-            if (h + u * kRows < heads && pl.in) {
-              store8(yp + u * kRows * ys + pl.o0, ha);
-              store8(yp + u * kRows * ys + pl.o1, hb);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              s0 = f2_fma(x[i], x[i], s0);
+              s1 = f2_fma(y[i], y[i], s1);
+              t0 = f2_fma(va[i], x[i], t0);
+              t1 = f2_fma(vb[i], y[i], t1);
+            }
+            const float ss = group_sum<kLanes>(f2_sum(f2_add(s0, s1)));
+            const float dot = group_sum<kLanes>(f2_sum(f2_add(t0, t1)));
+            const float r = use ? rsqrtf(ss * p.inv_d + p.eps) : 0.f;   // no row: 0 times 0, also where eps is 0
+            const float q = -dot * p.inv_d * r * r * r;      // dx = r (h w) + x q
+            const uint64_t rr = f2_pack(r, r), qq = f2_pack(q, q);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              da[i] = f2_fma(ha[i], f2_mul(x[i], rr), da[i]);
+              db[i] = f2_fma(hb[i], f2_mul(y[i], rr), db[i]);
+              ha[i] = f2_fma(va[i], rr, f2_mul(x[i], qq));
+              hb[i] = f2_fma(vb[i], rr, f2_mul(y[i], qq));
             }
           }
-          h += kBatch * kRows;
-          xp += kBatch * kRows * xs;
-          gp += kBatch * kRows * gs;
-          yp += kBatch * kRows * ys;
+          if (use) {
+            store8(yp + pl.o0, ha);
+            store8(yp + pl.o1, hb);
+          }
+          h += kRows;
+          yp += kRows * ys;
         }
         if (sd.dw_part != nullptr) {
           float* mine = s_dw[kind][warp][lane];
@@ -827,16 +983,22 @@ inline int lanes_of(int D) { return D <= 64 ? 4 : 8; }
 inline int passes_of(int heads, int D) { return (heads + 32 / lanes_of(D) - 1) / (32 / lanes_of(D)); }
 
 // Cuts the tokens' passes into units; returns the CTAs.  A warp takes all
-// passes of its token, so that the angles are made once, unless that leaves
-// SMs without work (32 warps on each are wanted; then there are few tokens, and
-// units are far below 2^32).
+// passes of a token, so that the angles are made once; the tokens left over
+// after the last full round of the warps are cut into parts while that leaves
+// no warp a second one (17 prompts of 15 thousand
+// tokens: 6.3 rounds, the last one then a third of a token long).
 inline int share_out(Params& p, int kinds, int ctas_per_sm) {
-  int passes = 0;
-  for (int k = 0; k < kinds; ++k) passes += p.side[k].heads ? passes_of(p.side[k].heads, p.D) : 0;
-  const long long want = (long long)sm_count() * 32;
-  p.chunk = (int)std::max<long long>(1, std::min<long long>(passes, p.T * passes / want));
-  p.chunks = (passes + p.chunk - 1) / p.chunk;
-  return (int)std::min<long long>((p.T * p.chunks + kWarps - 1) / kWarps, (long long)sm_count() * ctas_per_sm);
+  p.passes = 0;
+  for (int k = 0; k < kinds; ++k) p.passes += p.side[k].heads ? passes_of(p.side[k].heads, p.D) : 0;
+  const long long ctas = (long long)sm_count() * ctas_per_sm, warps = ctas * kWarps, rest = p.T % warps;
+  p.chunks = rest ? (int)std::min<long long>(p.passes, std::max<long long>(1, warps / rest)) : 1;
+  p.chunk = (p.passes + p.chunks - 1) / p.chunks;
+  p.chunks = (p.passes + p.chunk - 1) / p.chunk;
+  p.whole = (unsigned)(p.T - rest);
+  p.units = (unsigned)(p.whole + rest * p.chunks);
+  p.step_b = (unsigned)(warps / p.N);
+  p.step_n = (unsigned)(warps % p.N);
+  return (int)std::min<long long>((p.units + kWarps - 1ll) / kWarps, ctas);
 }
 
 template <typename T, bool kAppend>
@@ -845,7 +1007,10 @@ int launch_fwd(Params& p, bool inter, cudaStream_t st) {
   const bool wide = lanes_of(p.D) == 8;
   auto* k = wide ? (inter ? fwd_kernel<T, 8, true, kAppend> : fwd_kernel<T, 8, false, kAppend>)
                  : (inter ? fwd_kernel<T, 4, true, kAppend> : fwd_kernel<T, 4, false, kAppend>);
-  return check_cuda(decode::launch_pdl(k, dim3(grid), dim3(kThreads), 0, st, p), "norm and rotation launch");
+  const int smem = wide ? Feed<T, 8, 2, 2>::kBytes : Feed<T, 4, 2, 2>::kBytes;
+  const int rc = set_max_dynamic_smem(reinterpret_cast<const void*>(k), smem, "norm and rotation shared memory");
+  if (rc) return rc;
+  return check_cuda(decode::launch_pdl(k, dim3(grid), dim3(kThreads), smem, st, p), "norm and rotation launch");
 }
 
 template <bool kAppend>
@@ -859,7 +1024,10 @@ int launch_bwd(const Params& p, bool inter, int grid, cudaStream_t st) {
   const bool wide = lanes_of(p.D) == 8;
   auto* k = wide ? (inter ? bwd_kernel<T, 8, true> : bwd_kernel<T, 8, false>)
                  : (inter ? bwd_kernel<T, 4, true> : bwd_kernel<T, 4, false>);
-  return check_cuda(decode::launch_pdl(k, dim3((unsigned)grid), dim3(kThreads), 0, st, p), "norm and rotation backward launch");
+  const int smem = wide ? Feed<T, 8, 2, 4>::kBytes : Feed<T, 4, 2, 4>::kBytes;
+  const int rc = set_max_dynamic_smem(reinterpret_cast<const void*>(k), smem, "norm and rotation backward shared memory");
+  if (rc) return rc;
+  return check_cuda(decode::launch_pdl(k, dim3((unsigned)grid), dim3(kThreads), smem, st, p), "norm and rotation backward launch");
 }
 
 inline long long bwd_ctas() { return (long long)sm_count() * kCtasPerSm; }

@@ -276,6 +276,47 @@ def test_overlapping_windows(rot):
         assert torch.isfinite(grad).all()
 
 
+@pytest.mark.parametrize("H,H_kv,D", [(3, 1, 128), (5, 2, 64), (9, 7, 96)])
+def test_no_epsilon(rot, H, H_kv, D):
+    """eps = 0 with head counts that leave lanes without a row, whose 0 / 0 must reach
+    no sum; the gradients of the weights are those of the rows that are there."""
+    B, N = 2, 37
+    f = rot.rotary_frequencies(64 if D == 128 else 32)
+    q, k = _gen((B, H, N, D), 1, torch.bfloat16), _gen((B, H_kv, N, D), 2, torch.bfloat16)
+    w = 1 + 0.2 * _gen((D,), 3)
+    gq, gk = _gen(q.shape, 4, torch.bfloat16), _gen(k.shape, 5, torch.bfloat16)
+    got = rot.qk_norm_rope_backward(gq, gk, q, k, f, q_weight=w, k_weight=w, eps=0.0)
+    cos, sin = _turns(f, None, None, B, N)
+    for i, (x, g) in enumerate(((q, gq), (k, gk))):
+        dx, dxm, dw, dwm = _oracle_back(x, w, g, cos, sin, False, 0.0)
+        _close(got[i], dx, dxm, 48, f"gradient {i}")
+        _close(got[2 + i], dw, dwm, B * N * x.shape[1] / 8 + 64, f"weight gradient {i}")
+
+
+@pytest.mark.parametrize("T", [2367, 2368, 2369, 3551, 3553, 5000])
+def test_token_counts_around_a_round_of_warps(rot, T):
+    """Counts at which the tokens behind the last full round are cut differently,
+    in sequences shorter than a round: the same rows as alone."""
+    B = 7 if T % 7 == 0 else 1
+    H, H_kv, D = 6, 2, 128
+    f = rot.rotary_frequencies(D)
+    w = 1 + 0.2 * _gen((D,), 3)
+    for b in {1, B}:
+        n = T // b
+        q, k = _gen((b, H, n, D), 1, torch.bfloat16), _gen((b, H_kv, n, D), 2, torch.bfloat16)
+        gq, gk = _gen(q.shape, 4, torch.bfloat16), _gen(k.shape, 5, torch.bfloat16)
+        pos = torch.randint(0, 1 << 20, (b, n), device="cuda", dtype=torch.int32)
+        yq, yk = rot.qk_norm_rope_forward(q, k, f, pos, q_weight=w, k_weight=w)
+        dq, dk, dwq, dwk = rot.qk_norm_rope_backward(gq, gk, q, k, f, pos, q_weight=w, k_weight=w)
+        cos, sin = _turns(f, pos, None, b, n)
+        for i, (x, g, y, d, dw) in enumerate(((q, gq, yq, dq, dwq), (k, gk, yk, dk, dwk))):
+            want, mag = _oracle(x, w, cos, sin, False, 1e-6)
+            _close(y, want, mag, 32, f"output {i}")
+            dx, dxm, dwr, dwm = _oracle_back(x, w, g, cos, sin, False, 1e-6)
+            _close(d, dx, dxm, 48, f"gradient {i}")
+            _close(dw, dwr, dwm, T * x.shape[1] / 8 + 64, f"weight gradient {i}")
+
+
 def test_broadcast_inputs_and_gradients(rot):
     """A key head expanded over the batch, and a gradient that is one value
     expanded over the output: sums of the rows' gradients."""
