@@ -222,13 +222,18 @@ def qk_norm_rope_backward(gq, gk, q, k, inv_freq, positions=None, *, q_weight=No
     return _backward(desc, gq, gk, q, k, weight_grads, weight_grads)
 
 
+def _plain(desc):
+    """What a description holds beside tensors and their strides."""
+    return desc[:8] + desc[11:13] + desc[15:]
+
+
 class _QkNormRope(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, inv_freq, positions, eps, sections, interleaved):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(q, k, q_weight, k_weight, inv_freq, positions)
         desc = _description(q, k, inv_freq, positions, q_weight, k_weight, eps, sections, interleaved)
-        ctx.plain = desc[:8] + desc[10:13] + desc[15:]     # what holds no tensor
+        ctx.plain, ctx.sections = _plain(desc), None if sections is None else desc[12][:desc[11]]
         return _forward(desc, q, k)
 
     @staticmethod
@@ -245,8 +250,12 @@ class _QkNormRope(torch.autograd.Function):
             gq = None
         if not (need[1] or need[3]):
             gk = None
-        wq, wk = (None if w is None else w.contiguous() for w in (wq, wk))
-        desc = plain[:8] + (inv_freq.contiguous(), positions) + plain[8:11] + (wq, wk) + plain[11:]
+        # described anew: saved-tensor hooks may give other tensors back (dense
+        # copies of strided views, say), so nothing of the forward's pointers,
+        # strides or types is carried over
+        desc = _description(q, k, inv_freq, positions, wq, wk, plain[-1], ctx.sections, plain[7])
+        if _plain(desc) != plain:
+            raise ValueError("a saved tensor came back with another shape or type")
         dq, dk, dwq, dwk = _backward(desc, gq, gk, q, k, need[2], need[3])
         return (dq if need[0] else None, dk if need[1] else None, dwq, dwk, None, None, None, None, None)
 

@@ -500,3 +500,31 @@ def test_training_chain(rot):
     assert_close_o(to_np(o), to_np(o64), what="chain")
     for n, a, b in zip(("x", "wq", "wk"), got, want):
         assert_close_grad(to_np(a), to_np(b), what=n)
+
+
+def test_saved_tensor_hooks(rot):
+    """Gradients are the same where hooks copy the saved tensors (to the host and
+    back, or to a dense tensor): views of positions, weights and inputs."""
+    for sections in (None, (8, 12, 12)):
+        B, N, H, H_kv, D = 3, 17, 4, 2, 64
+        x = _gen((B, N, (H + H_kv) * D), 1, torch.bfloat16)
+        q = x[..., :H * D].view(B, N, H, D).transpose(1, 2)
+        k = x[..., H * D:].view(B, N, H_kv, D).transpose(1, 2)
+        big = torch.randint(0, 10000, (3, B, 100), device="cuda", dtype=torch.int32)
+        pos = big[:, :, 10:10 + N] if sections else big[1, :, 10:10 + N]
+        f = rot.rotary_frequencies(2 * D).contiguous()[::2]
+        w = (1 + 0.1 * _gen((2 * D,), 3))[::2]
+        gq, gk = _gen((B, H, N, D), 4, torch.bfloat16), _gen((B, H_kv, N, D), 5, torch.bfloat16)
+
+        def grads(hooks):
+            a = [t.detach().requires_grad_(True) for t in (q, k, w, w)]
+            with hooks:
+                y = rot.qk_norm_rope(a[0], a[1], f, pos, q_weight=a[2], k_weight=a[3], sections=sections)
+                return torch.autograd.grad(y, a, (gq, gk))
+
+        import contextlib
+        want = grads(contextlib.nullcontext())
+        clone = lambda t: t.detach().clone(memory_format=torch.contiguous_format)     # noqa: E731
+        for hooks in (torch.autograd.graph.saved_tensors_hooks(clone, lambda t: t), torch.autograd.graph.save_on_cpu()):
+            got = grads(hooks)
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), sections

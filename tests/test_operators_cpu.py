@@ -208,3 +208,105 @@ def test_gradients_have_dense_rows(shape, stride):
     seen = torch.zeros(g.untyped_storage().nbytes() // 2, dtype=torch.int32)
     seen.as_strided(g.shape, g.stride()).add_(1)
     assert int(seen.sum()) == g.numel() and int(seen.max()) == 1
+
+
+class _Library:
+    """Stands in for libpu_attn.so: keeps what its entry points were given."""
+
+    def __init__(self):
+        self.calls = {}
+
+    def __getattr__(self, name):
+        if name.endswith("workspace_size"):
+            return lambda *a: 256
+        return lambda *a: self.calls.__setitem__(name, a) or 0
+
+
+@pytest.fixture
+def host_rotary(monkeypatch):
+    """ops.rotary on host tensors, with the library's calls recorded."""
+    import contextlib
+    from pallas_flash import _lib
+    from pallas_flash.ops import rotary
+    so = _Library()
+    check = rotary._check_qk
+
+    class OnGpu:
+        """A tensor's shape, type and device, as one on a GPU."""
+        is_cuda = True
+
+        def __init__(self, t):
+            self.t = t
+
+        def __getattr__(self, name):
+            return getattr(self.t, name)
+
+        def dim(self):
+            return self.t.dim()
+
+    monkeypatch.setattr(rotary, "_check_qk", lambda q, k: check(OnGpu(q), OnGpu(k)))
+    monkeypatch.setattr(_lib, "lib", lambda: so)
+    monkeypatch.setattr(_lib, "on_device", lambda device: contextlib.nullcontext(0))
+    rotary._bwd_bytes.cache_clear()
+    yield rotary, so
+    rotary._bwd_bytes.cache_clear()
+
+
+def _addressed(pointer, strides, shape, dtype):
+    """(first, last) byte that a [..] view of these strides reads at `pointer`."""
+    last = sum((n - 1) * s for n, s in zip(shape, strides))
+    return pointer, pointer + (last + 1) * dtype.itemsize
+
+
+@pytest.mark.parametrize("sections", [None, (8, 12, 12)])
+@pytest.mark.parametrize("hooked", [False, True])
+def test_backward_addresses_the_saved_tensors(host_rotary, sections, hooked):
+    """What the backward is told to read lies inside the tensors that it was given, also
+    where saved-tensor hooks gave copies with other strides back."""
+    import contextlib
+    rotary, so = host_rotary
+    B, N, H, H_kv, D = 3, 4, 4, 2, 64
+    x = torch.randn(B, N, (H + H_kv) * D, dtype=torch.bfloat16)
+    q = x[..., :H * D].view(B, N, H, D).transpose(1, 2).detach().requires_grad_(True)
+    k = x[..., H * D:].view(B, N, H_kv, D).transpose(1, 2).detach().requires_grad_(True)
+    big = torch.arange(3 * B * 100, dtype=torch.int32).view(3, B, 100)
+    pos = big[:, :, 10:10 + N] if sections else big[0, :, 10:10 + N]
+    freq = torch.arange(64, dtype=torch.float64)[::2]
+    w = torch.ones(2 * D)[::2].requires_grad_(True)
+    held = []
+
+    def give(t):
+        held.append(t.detach().clone(memory_format=torch.contiguous_format))
+        return held[-1]
+
+    hooks = torch.autograd.graph.saved_tensors_hooks(lambda t: t, give) if hooked else contextlib.nullcontext()
+    with hooks:
+        y = rotary.qk_norm_rope(q, k, freq, pos, q_weight=w, k_weight=w, sections=sections)
+        torch.autograd.grad(y, (q, k, w), tuple(torch.ones_like(t) for t in y))
+    desc, pq, pk = so.calls["pu_qk_norm_rope_bwd"][:3]
+    d = rotary._DESC.unpack(desc)
+    known = held if hooked else [t.detach() for t in (q, k, freq, pos, w)]
+    inside = lambda lo, hi: any(t.data_ptr() <= lo and hi <= t.data_ptr() + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+                                * t.element_size() for t in known)     # noqa: E731
+    assert len(d) == 46 and d[10] != 0
+    strides = d[12:15]
+    shape = (3, B, N) if sections else (1, B, N)
+    assert strides == (((4 * B, 4, 1) if hooked else (100 * B, 100, 1)) if sections else ((0, 4, 1) if hooked else (0, 100, 1)))
+    assert inside(*_addressed(d[10], strides, shape, torch.int32))
+    for p, st, heads in ((pq, d[25:28], H), (pk, d[28:31], H_kv)):
+        assert inside(*_addressed(p, tuple(st) + (1,), (B, heads, N, D), torch.bfloat16))
+
+
+def test_hooks_that_give_other_tensors_back_are_refused(host_rotary):
+    """A saved tensor of another type or shape is refused before the library is asked."""
+    rotary, so = host_rotary
+    q, k = (torch.randn(2, h, 5, 64, dtype=torch.bfloat16, requires_grad=True) for h in (4, 2))
+    f, pos = torch.ones(32, dtype=torch.float64), torch.zeros(2, 5, dtype=torch.int32)
+    for which, other in ((torch.int32, lambda t: t.float()), (torch.int32, lambda t: t[:, :3]), (torch.float64, lambda t: t[:8]),
+                         (torch.bfloat16, lambda t: t.float())):
+        so.calls.clear()
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: other(t) if t.dtype == which else t):
+            y = rotary.qk_norm_rope(q, k, f, pos)
+            with pytest.raises((ValueError, TypeError)):
+                torch.autograd.grad(y, (q, k), tuple(torch.ones_like(t) for t in y))
+        assert "pu_qk_norm_rope_bwd" not in so.calls
