@@ -34,7 +34,7 @@ import numpy as np
 import torch
 
 from .. import _lib
-from ..ops.rotary import _DT as _DT_ROPE, _NONE, _check_angles, _check_weight, _pack, _rows
+from ..ops.rotary import _DT as _DT_ROPE, _NONE, _check_angles, _check_weight, _pack, _refuse_tangents, _rows
 from .decoding import _DT, _DT_KV, DecodeWorkspace
 
 __all__ = ["PageAllocator", "PagedKVCache", "DevicePagedKVCache", "AppendPlan", "paged_decode", "kv_append",
@@ -230,6 +230,7 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, inv_f
         raise ValueError(f"{H} and {H_kv} heads of size {D} (at least one head, a multiple of 16 up to 128)")
     if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
         raise ValueError("qk_norm_rope_append writes a cache and has no gradient")
+    _refuse_tangents(q, k, v, inv_freq, q_weight, k_weight)
     wq, wk = _check_weight(q_weight, D, dev, "q_weight"), _check_weight(k_weight, D, dev, "k_weight")
     if positions is None:
         raise ValueError("appended tokens need their positions")

@@ -15,7 +15,7 @@ Pair p is (p, p + R/2), or (2p, 2p + 1) with `interleaved`, where R = 2 *
 len(inv_freq); the values behind R are normed and not rotated.  Everything is
 fp32 inside and rounded once; angles are exact to fp32 at any position.
 
-Differentiable by q, k and the weights (once); the weights' gradients come
+Differentiable by q, k and the weights (once, in reverse mode); the weights' gradients come
 from fixed-order sums, the same bits every time.  Into a CUDA graph, capture
 `qk_norm_rope_forward` and `qk_norm_rope_backward`: autograd inside a capture
 waits for the streams of eager graphs that hold the same leaves.  Compute runs in
@@ -29,6 +29,7 @@ import struct
 from typing import Optional, Sequence
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
@@ -64,6 +65,16 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
         if ok:
             return t
     return t.clone(memory_format=torch.contiguous_format)
+
+
+def _refuse_tangents(*tensors) -> None:
+    """Raises where an input carries a forward-mode tangent: the result would have
+    none, which reads as a derivative of zero."""
+    if getattr(forward_ad, "_current_level", 0) < 0:        # outside every dual level there are none
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("norm and rotation have no forward-mode derivative")
 
 
 def _check_weight(w, D: int, device, name: str):
@@ -140,6 +151,7 @@ def _check_qk(q: torch.Tensor, k: torch.Tensor):
 def _description(q, k, inv_freq, positions, q_weight, k_weight, eps, sections, interleaved):
     """Checked arguments of a pass over [B, H, N, D] tensors, for _pack."""
     _check_qk(q, k)
+    _refuse_tangents(q, k, inv_freq, q_weight, k_weight)
     B, H, N, D = q.shape
     dev = q.device
     wq, wk = _check_weight(q_weight, D, dev, "q_weight"), _check_weight(k_weight, D, dev, "k_weight")
@@ -182,6 +194,7 @@ def _backward(desc, gq, gk, q, k, want_wq: bool, want_wk: bool):
     for g, t in ((gq, q), (gk, k)):
         if g is not None and (g.shape != t.shape or g.dtype != t.dtype or g.device != t.device):
             raise ValueError(f"an output gradient must match {tuple(t.shape)} {t.dtype} on {t.device}")
+    _refuse_tangents(gq, gk)
     if gq is None and gk is None:
         return None, None, None, None
     wq, wk = desc[13], desc[14]

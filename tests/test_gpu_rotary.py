@@ -528,3 +528,21 @@ def test_saved_tensor_hooks(rot):
         for hooks in (torch.autograd.graph.saved_tensors_hooks(clone, lambda t: t), torch.autograd.graph.save_on_cpu()):
             got = grads(hooks)
             assert all(torch.equal(a, b) for a, b in zip(got, want)), sections
+
+
+def test_forward_mode_is_refused(rot):
+    import torch.autograd.forward_ad as fwAD
+    q, k = _gen((1, 2, 4, 32), 1), _gen((1, 1, 4, 32), 2)
+    f = rot.rotary_frequencies(32)
+    with fwAD.dual_level():
+        for a, b in ((fwAD.make_dual(q, q), k), (q, fwAD.make_dual(k, k)), (fwAD.make_dual(q.clone().requires_grad_(True), q), k)):
+            with pytest.raises(NotImplementedError):
+                rot.qk_norm_rope(a, b, f)
+        with pytest.raises(NotImplementedError):
+            rot.qk_norm_rope(q, k, f, q_weight=fwAD.make_dual(q[0, 0, 0].clone(), q[0, 0, 1].clone()))
+        leaf = q.clone().requires_grad_(True)
+        y, _ = rot.qk_norm_rope(leaf, k, f)
+        with pytest.raises(NotImplementedError):
+            torch.autograd.grad(y, leaf, fwAD.make_dual(q, q))
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda x: rot.qk_norm_rope(x, k, f)[0], (q,), (q,))

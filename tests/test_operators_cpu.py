@@ -310,3 +310,35 @@ def test_hooks_that_give_other_tensors_back_are_refused(host_rotary):
             with pytest.raises((ValueError, TypeError)):
                 torch.autograd.grad(y, (q, k), tuple(torch.ones_like(t) for t in y))
         assert "pu_qk_norm_rope_bwd" not in so.calls
+
+
+def test_forward_mode_is_refused(host_rotary):
+    """An input with a tangent is refused: the result would have none, which reads as
+    a derivative of zero."""
+    import torch.autograd.forward_ad as fwAD
+    rotary, so = host_rotary
+    f, w = torch.ones(32, dtype=torch.float64), torch.ones(64)
+    pos = torch.zeros(2, 5, dtype=torch.int32)
+    with fwAD.dual_level():
+        for which in range(5):
+            a = [torch.randn(2, 4, 5, 64), torch.randn(2, 2, 5, 64), f, w, w]
+            a[which] = fwAD.make_dual(a[which], torch.ones_like(a[which]))
+            for call in (rotary.qk_norm_rope, rotary.qk_norm_rope_forward):
+                so.calls.clear()
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    call(a[0], a[1], a[2], pos, q_weight=a[3], k_weight=a[4])
+                assert not so.calls
+        q, k, v = (torch.randn(5, h, 64) for h in (4, 2, 2))
+        from pallas_flash.kernels.paged import _refuse_tangents
+        _refuse_tangents(q, k, v, None)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            _refuse_tangents(q, k, fwAD.make_dual(v, v), None)
+        # a tangent of an output's gradient
+        q = torch.randn(2, 4, 5, 64, requires_grad=True)
+        y, _ = rotary.qk_norm_rope(q, torch.randn(2, 2, 5, 64), f, pos)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.autograd.grad(y, q, fwAD.make_dual(torch.ones_like(y), torch.ones_like(y)))
+        so.calls.clear()
+        # no tangent: served
+        rotary.qk_norm_rope(torch.randn(2, 4, 5, 64), torch.randn(2, 2, 5, 64), f, pos)
+        assert "pu_qk_norm_rope_fwd" in so.calls
