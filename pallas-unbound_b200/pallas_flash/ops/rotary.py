@@ -286,13 +286,16 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, inv_freq: torch.Tensor,
     a projection's [B,N,H,D] transposed: rows that start on 16-byte boundaries
     are read where they are, others through a copy.
 
-      inv_freq   [R/2] fp64 or fp32 radians per position; R/2 a multiple of 8
+      inv_freq   [R/2] fp64 or fp32 radians per position; R/2 a multiple of 8.  There
+                 is no gradient by them: one that requires_grad is refused
       positions  int32 or int64 [N] or [B,N]; default 0..N-1
       q_weight, k_weight   [D] norm weights; None: that side is only rotated
       sections   sizes of 1 to 4 runs of pairs, one for each axis of
                  `positions` [axes,N] or [axes,B,N]: the first run turns with
                  axis 0 (time, say), the next with axis 1 (height), ...
     """
+    if inv_freq.requires_grad and torch.is_grad_enabled():
+        raise ValueError("the frequencies have no gradient: pass inv_freq.detach()")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad
                                     or (q_weight is not None and q_weight.requires_grad)
                                     or (k_weight is not None and k_weight.requires_grad)):

@@ -342,3 +342,17 @@ def test_forward_mode_is_refused(host_rotary):
         # no tangent: served
         rotary.qk_norm_rope(torch.randn(2, 4, 5, 64), torch.randn(2, 2, 5, 64), f, pos)
         assert "pu_qk_norm_rope_fwd" in so.calls
+
+
+def test_frequencies_that_want_a_gradient_are_refused(host_rotary):
+    """There is none by the frequencies: asked for one, the call says so."""
+    rotary, so = host_rotary
+    q, k = torch.randn(2, 4, 5, 64, requires_grad=True), torch.randn(2, 2, 5, 64)
+    f = torch.ones(32, dtype=torch.float64, requires_grad=True)
+    for x in (q, q.detach()):
+        with pytest.raises(ValueError, match="frequencies"):
+            rotary.qk_norm_rope(x, k, f)
+    assert not so.calls
+    rotary.qk_norm_rope(q, k, f.detach())
+    with torch.no_grad():
+        rotary.qk_norm_rope(q, k, f)
