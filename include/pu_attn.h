@@ -360,7 +360,8 @@ PU_API int pu_decode_paged_gqa(const void* q, int q_dtype,
  *     in a call are handed out from the next call on.
  * Results:
  *   page_table_out, kv_lens_out, cursor_out: the state after.  Either all
- *     three are the inputs themselves (advanced in place) or none is; a
+ *     three are the inputs themselves (advanced in place; new_lens may not
+ *     overlap kv_lens then) or none is; a
  *     separate table is written whole, -1 past each sequence's pages, while in
  *     place only entries that change are written.
  *   slots, positions, seq_ids int32 [num_tokens]: for row t of the packed

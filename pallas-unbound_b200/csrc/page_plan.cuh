@@ -268,6 +268,9 @@ extern "C" int pu_page_plan(const int32_t* page_table, int32_t* page_table_out, 
   const bool table_in = page_table == page_table_out, lens_in = kv_lens == kv_lens_out, cur_in = cursor == cursor_out;
   if (table_in != lens_in || lens_in != cur_in)
     return pu::set_error(PU_ERR_INVALID_ARGUMENT, "page plan: table, lengths and cursor are advanced in place together or not at all");
+  // in place the lengths are written while other CTAs still read the counts
+  if (lens_in && new_lens < kv_lens + B && kv_lens < new_lens + B)
+    return pu::set_error(PU_ERR_INVALID_ARGUMENT, "page plan: new_lens overlaps the lengths that are advanced in place");
   const int smem = (int)(5 * B + 1) * (int)sizeof(int);
   const void* f = table_in ? reinterpret_cast<const void*>(page_plan_kernel<true>)
                            : reinterpret_cast<const void*>(page_plan_kernel<false>);

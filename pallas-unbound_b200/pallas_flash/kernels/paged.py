@@ -174,8 +174,8 @@ def plan_append(page_table: torch.Tensor, kv_lens: torch.Tensor, new_lens: torch
     if release is not None and (release.dtype not in (torch.bool, torch.uint8) or release.shape != (B,)
                                 or release.device != dev or not release.is_contiguous()):
         raise ValueError(f"release must be a contiguous bool [{B}] on {dev}")
-    if inplace and new_lens.data_ptr() == kv_lens.data_ptr():
-        raise ValueError("new_lens must not be kv_lens when they are advanced in place")
+    if inplace and abs(new_lens.data_ptr() - kv_lens.data_ptr()) < 4 * B:
+        raise ValueError("new_lens must not overlap kv_lens when they are advanced in place")
     T = int(num_tokens)
     if T < 0:
         raise ValueError("num_tokens must not be negative")

@@ -356,3 +356,12 @@ def test_frequencies_that_want_a_gradient_are_refused(host_rotary):
     rotary.qk_norm_rope(q, k, f.detach())
     with torch.no_grad():
         rotary.qk_norm_rope(q, k, f)
+
+
+def test_page_plan_in_place_counts(lib):
+    """In place, the new counts may not lie where the lengths are written."""
+    _lib, so = lib
+    Q, B = P + 4096, 2
+    a = [P, P, 4, P, P, Q, None, P, 8, P, P, 16, P, P, P, P, B, 3, None]
+    for new in (P, P + 4, P - 4):
+        assert so.pu_page_plan(*a[:5], new, *a[6:]) == _lib.PU_ERR_INVALID_ARGUMENT, new
