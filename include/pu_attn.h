@@ -371,10 +371,15 @@ PU_API int pu_decode_paged_gqa(const void* q, int q_dtype,
  *   cu_new int32 [B+1]: first row of each sequence.
  * A sequence whose tokens exceed its table row or the num_tokens rows, or for
  * which the free pages do not last, is refused: it keeps its pages and length
- * and its rows get slot -1.  pu_device_status then reports
- * PU_ERR_INVALID_ARGUMENT, detail 307 (does not fit; also a kept page outside
- * the pool), or PU_ERR_WORKSPACE, detail 308 (no free pages); a cursor that
- * describes no ring of this size is PU_ERR_INVALID_ARGUMENT, detail 308.
+ * (none, if it was released in the call) and its rows get slot -1.  Free pages
+ * are counted in sequence order, also for a sequence that is refused: later ones
+ * that need a page are refused with it, those that need none are served.
+ * pu_device_status then reports PU_ERR_INVALID_ARGUMENT, detail 307 (does not
+ * fit; also a kept page outside the pool), or PU_ERR_WORKSPACE, detail 308 (no free pages); a cursor that
+ * describes no ring of this size, or more free and released pages than there
+ * are, is PU_ERR_INVALID_ARGUMENT, detail 308: released sequences are refused
+ * then and keep their pages and lengths, unless the ring holds every page
+ * already, theirs among them.
  * B <= 8192.
  */
 PU_API int pu_page_plan(const int32_t* page_table, int32_t* page_table_out,

@@ -12,7 +12,9 @@
 // Free pages wait in a ring: they are taken at its head and returned at its
 // tail, so the places read and the places written by one call never meet
 // (free + returned pages never exceed the ring), and pages of a sequence
-// that is released in this call are handed out from the next call on.
+// that is released in this call are handed out from the next call on.  A
+// release is refused whole where the ring has no room for the pages (they would be
+// in neither table nor ring).
 //
 // Every CTA scans all B sequences itself (three block-wide sums in 64 bits;
 // a second kernel would cost more than the repeated reads of a few KB from
@@ -54,30 +56,34 @@ struct Params {
   long long T;
 };
 
-// Exclusive block-wide sum of one value per thread; *total = the sum of all.
-__device__ __forceinline__ long long block_scan(long long v, long long* s_warp, long long* total) {
+// Exclusive block-wide sums of N values per thread; total[i] = the i-th's sum of all.
+template <int N>
+__device__ __forceinline__ void block_scan(long long (&v)[N], long long (*s_warp)[32], long long (&total)[N]) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long x = v;
-#pragma unroll
-  for (int off = 1; off < 32; off <<= 1) {
-    const long long y = __shfl_up_sync(0xffffffffu, x, off);
-    if (lane >= off) x += y;
-  }
-  __syncthreads();                       // the previous scan's sums have been read
-  if (lane == 31) s_warp[warp] = x;
-  __syncthreads();
-  if (warp == 0) {
-    long long w = s_warp[lane];
+  auto scan = [&](long long x) {
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, w, off);
-      if (lane >= off) w += y;
+      const long long y = __shfl_up_sync(0xffffffffu, x, off);
+      if (lane >= off) x += y;
     }
-    s_warp[lane] = w;
+    return x;
+  };
+  long long x[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] = scan(v[i]);
+  __syncthreads();                       // the previous scan's sums have been read
+  if (lane == 31) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) s_warp[i][warp] = x[i];
   }
   __syncthreads();
-  *total = s_warp[31];
-  return x - v + (warp > 0 ? s_warp[warp - 1] : 0);
+  if (warp < N) s_warp[warp][lane] = scan(s_warp[warp][lane]);
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    total[i] = s_warp[i][31];
+    v[i] = x[i] - v[i] + (warp > 0 ? s_warp[i][warp - 1] : 0);
+  }
 }
 
 template <bool kInPlace>
@@ -88,8 +94,10 @@ __global__ void __launch_bounds__(kThreads) page_plan_kernel(const Params p) {
   int* s_last = s_base + p.B;            // [B] pages held after
   int* s_new = s_last + p.B;             // [B] ring place of the first new page, from the head
   int* s_freed = s_new + p.B;            // [B] ring place of the first returned page, from the tail; -1: none
-  __shared__ long long s_warp[32];
+  __shared__ long long s_warp[2][32];
+  __shared__ int s_used;                 // pages taken
   const int tid = threadIdx.x;
+  if (tid == 0) s_used = 0;
   grid_dep_wait();
   grid_dep_launch_dependents();
 
@@ -103,33 +111,45 @@ __global__ void __launch_bounds__(kThreads) page_plan_kernel(const Params p) {
 
   // this thread's sequences
   const int per = (p.B + kThreads - 1) / kThreads, b0 = min(tid * per, p.B), b1 = min(b0 + per, p.B);
+  auto held_of = [&](int b) { return (int)min((long long)max(p.lens[b], 0), cap); };
+  auto gone = [&](int b) { return p.release != nullptr && p.release[b] != 0; };
   long long tokens = 0, freed = 0;
   for (int b = b0; b < b1; ++b) {
-    const long long held = min((long long)max(p.lens[b], 0), cap);
-    const bool gone = p.release != nullptr && p.release[b] != 0;
-    s_base[b] = gone ? 0 : (int)held;
-    s_freed[b] = gone ? (int)((held + page - 1) >> p.page_shift) : 0;
-    tokens += max(p.add[b], 0);
+    s_base[b] = gone(b) ? 0 : held_of(b);
+    s_freed[b] = gone(b) ? (held_of(b) + page - 1) >> p.page_shift : 0;
     freed += s_freed[b];
+    tokens += max(p.add[b], 0);
   }
-  long long total_tokens, total_freed, total_need, total_used;
-  long long start = block_scan(tokens, s_warp, &total_tokens);
-  long long back = block_scan(freed, s_warp, &total_freed);
+  const int lane = tid & 31;
+  long long sums[2] = {tokens, freed}, totals[2];
+  block_scan(sums, s_warp, totals);
+  const long long start = sums[0], total_tokens = totals[0], total_freed = totals[1];
+  long long back = sums[1];
+  // A release that the ring has no room for is refused with its sequence, which stays
+  // as it is; a ring that holds every page has the row's too, and the row is emptied.
+  const bool give = ring_ok && avail + total_freed <= p.num_pages;
+  const bool keep = !give && !(ring_ok && avail == p.num_pages);
+  if (tid == 0 && blockIdx.x == 0 && !give) record_device_error(PU_ERR_INVALID_ARGUMENT, kSiteFreePages);
   // what fits the table and the rows of the batch asks for pages
-  long long need = 0, at = start;
+  long long need[1] = {0}, total_need[1], at = start;
   for (int b = b0; b < b1; ++b) {
+    const bool stuck = keep && gone(b);
+    if (stuck) s_base[b] = held_of(b);
     const long long n = max(p.add[b], 0), base = s_base[b];
     const int have = (int)((base + page - 1) >> p.page_shift);
-    const bool fits = base + n <= cap && at + n <= p.T;
-    if (!fits) record_device_error(PU_ERR_INVALID_ARGUMENT, kSitePagePlan);
+    const bool fits = !stuck && base + n <= cap && at + n <= p.T;
+    if (!fits && !stuck) record_device_error(PU_ERR_INVALID_ARGUMENT, kSitePagePlan);
     s_start[b] = (int)min(at, p.T);
     s_last[b] = fits ? (int)((base + n + page - 1) >> p.page_shift) : -1;
-    need += fits ? s_last[b] - have : 0;
+    need[0] += fits ? s_last[b] - have : 0;
     at += n;
   }
-  long long upto = block_scan(need, s_warp, &total_need);
-  // pages go to the sequences in order while they last
-  long long used = 0;
+  block_scan(need, s_warp, total_need);
+  long long upto = need[0];
+  // Pages go to the sequences in order while they last: behind the first for which
+  // they do not, only those that need none are served, so what is taken in all is the
+  // furthest place that a served sequence reaches.
+  int used = 0;
   for (int b = b0; b < b1; ++b) {
     const int have = (s_base[b] + page - 1) >> p.page_shift;
     const int want = s_last[b] < 0 ? 0 : s_last[b] - have;
@@ -137,12 +157,11 @@ __global__ void __launch_bounds__(kThreads) page_plan_kernel(const Params p) {
     if (s_last[b] >= 0 && !served) record_device_error(PU_ERR_WORKSPACE, kSiteFreePages);
     s_new[b] = served ? (int)min(upto, avail) : -1;        // -1: refused, the sequence stays as it is
     if (!served) s_last[b] = have;
-    else used += want;
+    else if (want > 0) used = (int)upto + want;
     upto += want;
   }
-  block_scan(used, s_warp, &total_used);
-  const bool give = ring_ok && avail + total_freed <= p.num_pages;
-  if (tid == 0 && blockIdx.x == 0 && (!ring_ok || !give)) record_device_error(PU_ERR_INVALID_ARGUMENT, kSiteFreePages);
+  used = __reduce_max_sync(0xffffffffu, used);
+  if (lane == 0 && used > 0) atomicMax(&s_used, used);
   for (int b = b0; b < b1; ++b) {
     const int f = s_freed[b];
     s_freed[b] = f > 0 && give ? (int)back : -1;
@@ -152,33 +171,30 @@ __global__ void __launch_bounds__(kThreads) page_plan_kernel(const Params p) {
   __syncthreads();
 
   // rows: pages kept, pages taken, then none
-  const int warps = (int)gridDim.x * (kThreads / 32), wid = (int)blockIdx.x * (kThreads / 32) + (tid >> 5), lane = tid & 31;
+  const int warps = (int)gridDim.x * (kThreads / 32), wid = (int)blockIdx.x * (kThreads / 32) + (tid >> 5);
   auto taken = [&](int i) { int r = head0 + i; return p.ring[r >= p.num_pages ? r - p.num_pages : r]; };
-  // lengths held before (the pages a released row returns), read ahead of the barrier
   constexpr int kSeg = 512;              // entries a warp takes at once
   const int segs = (p.max_pages + kSeg - 1) / kSeg;
   if constexpr (kInPlace) {
     // only the released rows still need their old lengths: put them where the
     // rows' owners find them before the lengths change
     for (int b = tid; b < p.B; b += kThreads)
-      if (p.release != nullptr && p.release[b] != 0) {
-        const long long held = min((long long)max(p.lens[b], 0), cap);
-        s_base[b] = -(int)held - 1;      // base is 0 for a released sequence
-      }
+      if (gone(b) && !keep) s_base[b] = -held_of(b) - 1;      // base is 0 for a released sequence
     __syncthreads();
     cluster_sync();
   }
   auto base_of = [&](int b) { return kInPlace && s_base[b] < 0 ? 0 : s_base[b]; };
   auto old_of = [&](int b) -> int {      // pages the row returns
-    if (p.release == nullptr || p.release[b] == 0) return 0;
-    const long long held = kInPlace ? -(long long)(s_base[b] + 1) : min((long long)max(p.lens[b], 0), cap);
-    return (int)((held + page - 1) >> p.page_shift);
+    if (!gone(b) || keep) return 0;
+    const int held = kInPlace ? -(s_base[b] + 1) : held_of(b);
+    return (held + page - 1) >> p.page_shift;
   };
   for (long long u = wid; u < (long long)p.B * segs; u += warps) {
-    const int b = (int)(u / segs), lo = (int)(u % segs) * kSeg, hi = min(lo + kSeg, p.max_pages);
-    const int have = (base_of(b) + page - 1) >> p.page_shift, last = s_last[b], old = old_of(b), to = s_freed[b];
+    const int b = (int)(u / segs), lo = (int)(u % segs) * kSeg;
+    const int have = (base_of(b) + page - 1) >> p.page_shift, last = s_last[b], old = old_of(b);
     const int32_t* in = p.table + (size_t)b * p.max_pages;
     int32_t* out = p.table_out + (size_t)b * p.max_pages;
+    const int to = s_freed[b], hi = min(lo + kSeg, p.max_pages);
     // in place, the kept entries stay and those past both page counts are not touched
     const int from = kInPlace ? max(lo, have) : lo, end = kInPlace ? min(hi, max(last, old)) : hi;
     for (int j = from + lane; j < end; j += 32) {
@@ -195,7 +211,7 @@ __global__ void __launch_bounds__(kThreads) page_plan_kernel(const Params p) {
       if (b < p.B) p.lens_out[b] = base_of(b) + (s_new[b] >= 0 ? max(p.add[b], 0) : 0);
     }
     if (tid == 0) {
-      p.cursor_out[0] = head + total_used;
+      p.cursor_out[0] = head + s_used;
       p.cursor_out[1] = tail + (give ? total_freed : 0);
     }
   }

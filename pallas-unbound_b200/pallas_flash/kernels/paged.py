@@ -151,8 +151,12 @@ def plan_append(page_table: torch.Tensor, kv_lens: torch.Tensor, new_lens: torch
     it starts empty; they are handed out from the next call on.
 
     A sequence that does not fit its table row or the batch's rows, or for
-    which the free pages do not last, is refused: it stays as it is, its rows
-    get slot -1, and device_status() reports it (detail 307 or 308).
+    which the free pages do not last, is refused: it stays as it is (empty, if
+    it was released in the call), its rows get slot -1, and device_status()
+    reports it (detail 307 or 308).  Pages are counted in sequence order, those
+    that a refused sequence asked for as well, so later ones that need a page are
+    refused with it.  Where the ring has no room for what is released, released
+    sequences are refused and keep pages and lengths (detail 308).
 
     With `inplace` the table, lengths and cursor are advanced where they are
     (the same tensors come back); otherwise new ones are returned and only the

@@ -227,3 +227,59 @@ def test_captured_in_place(mods):
     np.testing.assert_array_equal(t[0].cpu().numpy(), want_state[0])
     np.testing.assert_array_equal(t[3].cpu().numpy(), want_state[3])
     assert _lib.device_status() == (0, 0)
+
+
+@pytest.mark.parametrize("inplace", [False, True])
+def test_refused_releases_lose_no_page(mods, inplace):
+    """Where the ring cannot take what is released (a cursor that describes no ring,
+    more free and released pages than there are), sequences keep their pages and
+    lengths, get no new tokens, and the status says so; the others are served."""
+    _lib, paged = mods
+    page, width, B = 16, 6, 4
+    table, lens, ring, cursor = state(B, width, page, [40, 33, 0, 20], 5, 3, head=7)
+    t = lambda a: torch.from_numpy(np.asarray(a).copy()).cuda()   # noqa: E731
+    P = len(ring)
+    release = torch.tensor([True, False, False, True], device="cuda")
+    new = torch.tensor([10, 3, 0, 0], dtype=torch.int32, device="cuda")
+    # free: 5 of 13; with a tail that claims 9, the 5 released pages no longer fit
+    for bad in ([-3, 2], [0, P + 1], [7, 2], [7, 7 + 9]):
+        a = [t(x) for x in (table, lens, ring, np.array(bad, np.int64))]
+        plan = paged.plan_append(a[0], a[1], new, a[2], a[3], page_size=page, num_tokens=14, release=release, inplace=inplace)
+        got = plan.page_table.cpu().numpy()
+        np.testing.assert_array_equal(got, table)                 # sequence 1's tokens fit its last page
+        assert plan.kv_lens.tolist() == [40, 36, 0, 20], bad
+        assert plan.slots[:10].tolist() == [-1] * 10 and (plan.slots[10:13] >= 0).all() and plan.slots[13] == -1
+        assert plan.seq_ids.tolist() == [0] * 10 + [1] * 3 + [-1]
+        assert plan.positions[:13].tolist() == list(range(40, 50)) + [33, 34, 35]
+        assert plan.cursor.tolist() == bad
+        np.testing.assert_array_equal(a[2].cpu().numpy(), ring)
+        assert _lib.device_status() == (_lib.PU_ERR_INVALID_ARGUMENT, 308), bad
+    # a ring that holds every page has those of the row already: the row is emptied
+    a = [t(x) for x in (np.array([[1, 0, -1]], np.int32), np.array([20], np.int32), np.arange(2, dtype=np.int32), np.array([4, 6], np.int64))]
+    plan = paged.plan_append(a[0], a[1], torch.tensor([5], dtype=torch.int32, device="cuda"), a[2], a[3], page_size=page, num_tokens=5,
+                             release=torch.ones(1, dtype=torch.bool, device="cuda"), inplace=inplace)
+    assert plan.kv_lens.tolist() == [5] and plan.page_table.tolist() == [[0, -1, -1]] and plan.cursor.tolist() == [5, 6]
+    assert _lib.device_status() == (_lib.PU_ERR_INVALID_ARGUMENT, 308)
+
+
+def test_refused_after_release(mods):
+    """A sequence that is released and then does not fit is left empty, its pages back."""
+    _lib, paged = mods
+    page, width = 16, 2
+    st = state(2, width, page, [20, 5], 4, 1)
+    for inplace in (False, True):
+        _, want, after = check(paged, st, [40, 2], page, 42, [True, False], inplace)
+        assert want["refused"] == {"fit"} and after[1].tolist() == [0, 7] and (after[0][0] == -1).all()
+        assert after[3][1] - st[3][1] == 2
+        assert _lib.device_status() == (_lib.PU_ERR_INVALID_ARGUMENT, 307)
+
+
+def test_pages_are_counted_in_sequence_order(mods):
+    """A sequence refused for want of pages keeps its claim within the call: later ones that
+    need a page are refused as well, those that need none are served."""
+    _lib, paged = mods
+    page = 16
+    st = state(4, 8, page, [16, 16, 5, 16], 2, 1)
+    _, want, after = check(paged, st, [1, 40, 2, 1], page, 44)
+    assert want["refused"] == {"free"} and after[1].tolist() == [17, 16, 7, 16]
+    assert _lib.device_status() == (_lib.PU_ERR_WORKSPACE, 308)
