@@ -375,7 +375,8 @@ PU_API int pu_decode_paged_gqa(const void* q, int q_dtype,
  * are counted in sequence order, also for a sequence that is refused: later ones
  * that need a page are refused with it, those that need none are served.
  * pu_device_status then reports PU_ERR_INVALID_ARGUMENT, detail 307 (does not
- * fit; also a kept page outside the pool), or PU_ERR_WORKSPACE, detail 308 (no free pages); a cursor that
+ * fit; also a kept or returned entry outside the pool, which never becomes a
+ * free page), or PU_ERR_WORKSPACE, detail 308 (no free pages); a cursor that
  * describes no ring of this size, or more free and released pages than there
  * are, is PU_ERR_INVALID_ARGUMENT, detail 308: released sequences are refused
  * then and keep their pages and lengths, unless the ring holds every page

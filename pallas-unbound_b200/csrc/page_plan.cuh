@@ -14,7 +14,7 @@
 // (free + returned pages never exceed the ring), and pages of a sequence
 // that is released in this call are handed out from the next call on.  A
 // release is refused whole where the ring has no room for the pages (they would be
-// in neither table nor ring).
+// in neither table nor ring), and only entries that name a page go back.
 //
 // Every CTA scans all B sequences itself (three block-wide sums in 64 bits;
 // a second kernel would cost more than the repeated reads of a few KB from
@@ -27,6 +27,7 @@
 // of table and ring, one write.  256 sequences with 2048 table entries each
 // (2 MB of table written) and 61 prompts of up to 2500 tokens both take 9 us a
 // call back to back; the call's own host time is 20 us.
+// Released rows are read ahead of the scans, to count the pages that come back.
 #pragma once
 
 #include "paged.cuh"
@@ -93,7 +94,8 @@ __global__ void __launch_bounds__(kThreads) page_plan_kernel(const Params p) {
   int* s_base = s_start + p.B + 1;       // [B] tokens held before
   int* s_last = s_base + p.B;            // [B] pages held after
   int* s_new = s_last + p.B;             // [B] ring place of the first new page, from the head
-  int* s_freed = s_new + p.B;            // [B] ring place of the first returned page, from the tail; -1: none
+  int* s_freed = s_new + p.B;            // [B] ring place of the first returned page, from the tail; -1: none;
+                                         // -2 - place: the row has entries that are no pages
   __shared__ long long s_warp[2][32];
   __shared__ int s_used;                 // pages taken
   const int tid = threadIdx.x;
@@ -114,13 +116,30 @@ __global__ void __launch_bounds__(kThreads) page_plan_kernel(const Params p) {
   auto held_of = [&](int b) { return (int)min((long long)max(p.lens[b], 0), cap); };
   auto gone = [&](int b) { return p.release != nullptr && p.release[b] != 0; };
   long long tokens = 0, freed = 0;
+  bool any = false;
   for (int b = b0; b < b1; ++b) {
     s_base[b] = gone(b) ? 0 : held_of(b);
     s_freed[b] = gone(b) ? (held_of(b) + page - 1) >> p.page_shift : 0;
-    freed += s_freed[b];
+    any |= s_freed[b] > 0;
     tokens += max(p.add[b], 0);
   }
   const int lane = tid & 31;
+  if (__syncthreads_or(any)) {
+    // how many of a released row's entries name a page (-1 - the count where some do
+    // not): a warp per row
+    for (int b = tid >> 5; b < p.B; b += kThreads / 32) {
+      const int old = s_freed[b];
+      if (old == 0) continue;
+      int good = 0;
+      for (int j = lane; j < old; j += 32) good += (unsigned)p.table[(size_t)b * p.max_pages + j] < (unsigned)p.num_pages;
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) good += __shfl_xor_sync(0xffffffffu, good, off);
+      __syncwarp();                      // every lane has read the row's page count
+      if (lane == 0) s_freed[b] = good == old ? good : -1 - good;
+    }
+    __syncthreads();
+    for (int b = b0; b < b1; ++b) freed += s_freed[b] < 0 ? -1 - s_freed[b] : s_freed[b];
+  }
   long long sums[2] = {tokens, freed}, totals[2];
   block_scan(sums, s_warp, totals);
   const long long start = sums[0], total_tokens = totals[0], total_freed = totals[1];
@@ -163,8 +182,10 @@ __global__ void __launch_bounds__(kThreads) page_plan_kernel(const Params p) {
   used = __reduce_max_sync(0xffffffffu, used);
   if (lane == 0 && used > 0) atomicMax(&s_used, used);
   for (int b = b0; b < b1; ++b) {
-    const int f = s_freed[b];
-    s_freed[b] = f > 0 && give ? (int)back : -1;
+    const bool whole = s_freed[b] >= 0;
+    const int f = whole ? s_freed[b] : -1 - s_freed[b];
+    if (!whole) record_device_error(PU_ERR_INVALID_ARGUMENT, kSitePagePlan);
+    s_freed[b] = f == 0 || !give ? -1 : whole ? (int)back : -2 - (int)back;
     back += f;
   }
   if (tid == 0) s_start[p.B] = (int)min(total_tokens, p.T);
@@ -194,7 +215,23 @@ __global__ void __launch_bounds__(kThreads) page_plan_kernel(const Params p) {
     const int have = (base_of(b) + page - 1) >> p.page_shift, last = s_last[b], old = old_of(b);
     const int32_t* in = p.table + (size_t)b * p.max_pages;
     int32_t* out = p.table_out + (size_t)b * p.max_pages;
-    const int to = s_freed[b], hi = min(lo + kSeg, p.max_pages);
+    int to = s_freed[b], hi = min(lo + kSeg, p.max_pages);
+    if (to <= -2) {
+      // entries that are no pages are left out: one warp takes the row, the others'
+      // segments of it too, and closes the gaps
+      if (lo > 0) continue;
+      hi = p.max_pages;
+      int put = tail0 - 2 - to;
+      for (int j0 = 0; j0 < old; j0 += 32) {
+        const int pg = j0 + lane < old ? in[j0 + lane] : -1;
+        const bool good = (unsigned)pg < (unsigned)p.num_pages;
+        const unsigned all = __ballot_sync(0xffffffffu, good);
+        const int r = put + __popc(all & ((1u << lane) - 1u));
+        if (good) p.ring[r >= p.num_pages ? r - p.num_pages : r] = pg;
+        put += __popc(all);
+      }
+      to = -1;
+    }
     // in place, the kept entries stay and those past both page counts are not touched
     const int from = kInPlace ? max(lo, have) : lo, end = kInPlace ? min(hi, max(last, old)) : hi;
     for (int j = from + lane; j < end; j += 32) {

@@ -156,7 +156,8 @@ def plan_append(page_table: torch.Tensor, kv_lens: torch.Tensor, new_lens: torch
     reports it (detail 307 or 308).  Pages are counted in sequence order, those
     that a refused sequence asked for as well, so later ones that need a page are
     refused with it.  Where the ring has no room for what is released, released
-    sequences are refused and keep pages and lengths (detail 308).
+    sequences are refused and keep pages and lengths (detail 308); entries of a
+    released row that name no page are reported (307) and left out of the ring.
 
     With `inplace` the table, lengths and cursor are advanced where they are
     (the same tensors come back); otherwise new ones are returned and only the

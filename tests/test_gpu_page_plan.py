@@ -262,6 +262,45 @@ def test_refused_releases_lose_no_page(mods, inplace):
     assert _lib.device_status() == (_lib.PU_ERR_INVALID_ARGUMENT, 308)
 
 
+@pytest.mark.parametrize("inplace", [False, True])
+def test_release_returns_pages_of_the_pool_only(mods, inplace):
+    """Entries of a released row that name no page (a length past the pages it holds, a
+    damaged table) are reported and never become free pages; the others come back in
+    order.  Rows over several of a warp's segments, beside sound ones."""
+    _lib, paged = mods
+    page, width, B = 16, 1400, 5
+    r = np.random.RandomState(5)
+    held = np.array([1300 * 16 - 3, 50, 16, 700 * 16, 900], np.int32)
+    table, lens, ring, cursor = state(B, width, page, held, 9, 5, head=3)
+    P = len(ring)
+    for b, at in ((0, [0, 5, 511, 512, 513, 1024, 1299]), (2, [0]), (3, [])):
+        table[b, at] = r.choice([-1, P, P + 7, -(1 << 31), (1 << 31) - 1], len(at))
+    gone = np.array([1, 0, 1, 1, 0], bool)
+    new = np.array([20, 2, 0, 3, 1], np.int32)
+    t = lambda a: torch.from_numpy(np.asarray(a).copy()).cuda()   # noqa: E731
+    a = [t(x) for x in (table, lens, ring, cursor)]
+    plan = paged.plan_append(a[0], a[1], t(new), a[2], a[3], page_size=page, num_tokens=26, release=t(gone), inplace=inplace)
+    assert _lib.device_status() == (_lib.PU_ERR_INVALID_ARGUMENT, 307)
+    back = [int(e) for b in (0, 2, 3) for e in table[b, :-(-int(held[b]) // page)] if 0 <= e < P]
+    head, tail = (int(c) for c in cursor)
+    want_ring = ring.copy()
+    for i, e in enumerate(back):
+        want_ring[(tail + i) % P] = e
+    np.testing.assert_array_equal(a[2].cpu().numpy(), want_ring)
+    free = [int(ring[(head + i) % P]) for i in range(9)]
+    want = table.copy()
+    want[[0, 2, 3]] = -1
+    want[0, :2], want[3, 0] = free[:2], free[2]
+    np.testing.assert_array_equal(plan.page_table.cpu().numpy(), want)
+    assert plan.kv_lens.tolist() == [20, 52, 0, 3, 901]
+    assert plan.cursor.tolist() == [head + 3, tail + len(back)]
+    assert (plan.slots >= 0).all()
+    # every place that is free now names a page of the pool
+    at = (int(plan.cursor[0]) + np.arange(int(plan.cursor[1] - plan.cursor[0]))) % P
+    got = a[2].cpu().numpy()[at]
+    assert ((got >= 0) & (got < P)).all()
+
+
 def test_refused_after_release(mods):
     """A sequence that is released and then does not fit is left empty, its pages back."""
     _lib, paged = mods
