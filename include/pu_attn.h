@@ -400,7 +400,8 @@ PU_API int pu_page_plan(const int32_t* page_table, int32_t* page_table_out,
  *   (a, b) -> (a cos t - b sin t, b cos t + a sin t),  t = position * inv_freq[p]
  * for the pairs p < rotary_dim/2 of n: (p, p + rotary_dim/2), or with
  * `interleaved` (2p, 2p+1); values behind rotary_dim are normed only.
- * Computed in fp32 and rounded once; angles are exact to fp32 at any position.
+ * Computed in fp32 and rounded once.  An angle is a 64-bit fraction of a turn: off
+ * by |position| 2^-54 of a turn, and sines of small angles keep fp32's precision.
  *
  * The description's fields are all 8 bytes wide.  Strides are in elements;
  * the last dimension is dense.  Rows start on 16-byte boundaries.

@@ -14,10 +14,9 @@
 // are normed and not rotated.
 //
 // Everything is computed in fp32 from one read of each row and rounded once.
-// The angle is exact to the last fp32 bit at any position: f_p / 2 pi is
-// held as a 64-bit fixed-point fraction of a turn, so position * f_p modulo
-// one turn is one wrapping integer product (its error, position * 2^-54
-// turns of the double product it comes from, stays under 2^-23 up to 2^31).
+// f_p / 2 pi is held as a 64-bit fixed-point fraction of a turn, so position * f_p
+// modulo one turn is one wrapping integer product; its error is position * 2^-54
+// turns, that of the double product it comes from (under 2^-23 up to 2^31).
 //
 // A row is spread over D/16 lanes (a group of 4 or 8): each lane holds two
 // vectors of 8 elements which are partners, 8p.. and R/2 + 8p.., so the rotation
@@ -208,12 +207,14 @@ __device__ __forceinline__ void fill_shared(const Params& p, Shared& sh) {
   __syncthreads();
 }
 
-// Sine and cosine of 2 pi turn / 2^32.  The nearest quarter turn comes off in
-// integers; the rest, at most pi / 4, through the Taylor series up to x^9 and
-// x^8 (the terms left out are below 2 10^-9 and 3 10^-8).
-__device__ __forceinline__ void sin_cos(int turn, float& s, float& c) {
-  const int quarter = (int)((unsigned)turn + 0x20000000u) >> 30;
-  const float x = (float)(turn - (int)((unsigned)quarter << 30)) * 1.4629180792671596e-9f;   // 2 pi / 2^32
+// Sine and cosine of 2 pi turn / 2^64.  The nearest quarter turn comes off in
+// 64-bit integers, so what is left, at most pi / 4, is rounded to fp32 relative to
+// itself and small angles keep their precision; then the Taylor series up to x^9 and
+// x^8 (the terms left out are below 2 10^-9 and 3 10^-8).  In all under 3.2 roundings
+// of 2^-24: of the sine itself near 0, of 1 for the cosine.
+__device__ __forceinline__ void sin_cos(unsigned long long turn, float& s, float& c) {
+  const unsigned quarter = (unsigned)((turn + 0x2000000000000000ull) >> 62);
+  const float x = (float)(long long)(turn - ((unsigned long long)quarter << 62)) * 3.4061215800865545e-19f;   // 2 pi / 2^64
   const float z = x * x;
   float ps = fmaf(z, 1.f / 362880.f, -1.f / 5040.f);
   ps = fmaf(z, ps, 1.f / 120.f);
@@ -224,8 +225,8 @@ __device__ __forceinline__ void sin_cos(int turn, float& s, float& c) {
   pc = fmaf(z, pc, -0.5f);
   pc = fmaf(z, pc, 1.f);
   const float a = quarter & 1 ? pc : ps, b = quarter & 1 ? ps : pc;
-  s = __uint_as_float(__float_as_uint(a) ^ ((unsigned)(quarter & 2) << 30));
-  c = __uint_as_float(__float_as_uint(b) ^ ((unsigned)((quarter + 1) & 2) << 30));
+  s = __uint_as_float(__float_as_uint(a) ^ ((quarter & 2) << 30));
+  c = __uint_as_float(__float_as_uint(b) ^ (((quarter + 1) & 2) << 30));
 }
 
 // A lane's share of a token's angles: pairs `lane` and `lane + 32`.
@@ -259,7 +260,7 @@ struct Turner {
   }
   // sine and cosine of pair lane + 32 i at its fetched position
   __device__ __forceinline__ void turn(const Shared& sh, int lane, int i, float& s, float& c) const {
-    sin_cos((int)((sh.step[lane + 32 * i] * (unsigned long long)pos[i]) >> 32), s, c);
+    sin_cos(sh.step[lane + 32 * i] * (unsigned long long)pos[i], s, c);
   }
   // of all pairs, into the warp's shared rows
   __device__ __forceinline__ void make(const Shared& sh, int lane, float* cs, float* sn) const {

@@ -14,6 +14,7 @@ sum of magnitudes cover the longest chain of these shapes.
 from __future__ import annotations
 
 import math
+from fractions import Fraction
 
 import pytest
 import torch
@@ -546,3 +547,46 @@ def test_forward_mode_is_refused(rot):
             torch.autograd.grad(y, leaf, fwAD.make_dual(q, q))
     with pytest.raises(RuntimeError):
         torch.func.jvp(lambda x: rot.qk_norm_rope(x, k, f)[0], (q,), (q,))
+
+
+# 2 pi to 60 digits: turns of far positions are worked out in whole numbers
+_TWO_PI = 2 * Fraction(314159265358979323846264338327950288419716939937510582097494, 10 ** 59)
+
+
+def _sine_cosine(f, pos):
+    """sin, cos [positions, pairs] in 64 bits of position * f, reduced to half a turn exactly."""
+    s, c = [], []
+    for p in pos.tolist():
+        row = []
+        for x in f.tolist():
+            turn = Fraction(x) * p / _TWO_PI
+            row.append(float((turn - round(turn)) * _TWO_PI))
+        s.append([math.sin(a) for a in row])
+        c.append([math.cos(a) for a in row])
+    return (torch.tensor(t, dtype=torch.float64, device="cuda") for t in (s, c))
+
+
+def _one_hot_turns(rot, f, pos, inter):
+    """sin and cos that the kernels turn with, forward and backward: rows with a 1 as a
+    pair's first value, and no norm, hold the pair's cosine and sine."""
+    R, N = 2 * f.numel(), pos.numel()
+    first = torch.arange(R // 2, device="cuda") * (2 if inter else 1)
+    second = first + (1 if inter else R // 2)
+    q = torch.zeros((1, 1, N, R), device="cuda")
+    q[..., first] = 1
+    y, _ = rot.qk_norm_rope_forward(q, q, f, pos, interleaved=inter)
+    dq, _, _, _ = rot.qk_norm_rope_backward(q, None, q, q, f, pos, interleaved=inter)
+    return (y[0, 0][:, second], y[0, 0][:, first]), (-dq[0, 0][:, second], dq[0, 0][:, first])
+
+
+@pytest.mark.parametrize("inter", [False, True])
+def test_small_angles_keep_their_precision(rot, inter):
+    """Sines of small angles to 8 roundings of 2^-24 of themselves: the angle's
+    conversion, constant and product (3), the fixed-point fraction (2^-64 of a turn in 2^-23
+    of one), the series (2 and its last product's part)."""
+    f = rot.rotary_frequencies(128, theta=1e6)
+    pos = torch.tensor([1, 2, 3, 5, 8, 100, -1, -77], dtype=torch.int32, device="cuda")
+    s, c = _sine_cosine(f, pos)
+    for sine, cosine in _one_hot_turns(rot, f, pos, inter):
+        assert ((sine.double() - s).abs() <= 8 * U * s.abs()).all()
+        assert ((cosine.double() - c).abs() <= 8 * U).all()
