@@ -401,7 +401,7 @@ PU_API int pu_page_plan(const int32_t* page_table, int32_t* page_table_out,
  * for the pairs p < rotary_dim/2 of n: (p, p + rotary_dim/2), or with
  * `interleaved` (2p, 2p+1); values behind rotary_dim are normed only.
  * Computed in fp32 and rounded once.  An angle is a 64-bit fraction of a turn: off
- * by |position| 2^-54 of a turn, and sines of small angles keep fp32's precision.
+ * by |position| 2^-64 of a turn, and sines of small angles keep fp32's precision.
  *
  * The description's fields are all 8 bytes wide.  Strides are in elements;
  * the last dimension is dense.  Rows start on 16-byte boundaries.

@@ -14,9 +14,9 @@
 // are normed and not rotated.
 //
 // Everything is computed in fp32 from one read of each row and rounded once.
-// f_p / 2 pi is held as a 64-bit fixed-point fraction of a turn, so position * f_p
-// modulo one turn is one wrapping integer product; its error is position * 2^-54
-// turns, that of the double product it comes from (under 2^-23 up to 2^31).
+// f_p / 2 pi is held as a 64-bit fixed-point fraction of a turn, rounded from twice a
+// double's precision, so position * f_p modulo one turn is one wrapping integer
+// product, off by |position| 2^-64 of a turn (2^-33 at any int32 position).
 //
 // A row is spread over D/16 lanes (a group of 4 or 8): each lane holds two
 // vectors of 8 elements which are partners, 8p.. and R/2 + 8p.., so the rotation
@@ -200,9 +200,12 @@ __device__ __forceinline__ void fill_shared(const Params& p, Shared& sh) {
   }
   for (int i = threadIdx.x; i < p.R / 2; i += kThreads) {
     const double f = p.ang.freq64 ? static_cast<const double*>(p.ang.freq)[i] : (double)static_cast<const float*>(p.ang.freq)[i];
-    double turns = f * 0.15915494309189533577;               // per position: 1 / 2 pi
-    turns -= floor(turns);
-    sh.step[i] = (unsigned long long)(turns * 18446744073709551616.0);   // * 2^64, below it
+    // f / 2 pi as the sum of two doubles (1 / 2 pi is one, too), whole turns taken off,
+    // in 2^-64ths of a turn
+    const double inv = 0.15915494309189535, inv_lo = -9.839338337591243e-18;
+    const double turns = f * inv, rest = fma(f, inv, -turns) + f * inv_lo;
+    sh.step[i] = (unsigned long long)__double2ll_rn((turns - rint(turns)) * 18446744073709551616.0) +
+                 (unsigned long long)__double2ll_rn(rest * 18446744073709551616.0);
   }
   __syncthreads();
 }

@@ -14,7 +14,7 @@ For one row x of D values (one head of one token):
 Pair p is (p, p + R/2), or (2p, 2p + 1) with `interleaved`, where R = 2 *
 len(inv_freq); the values behind R are normed and not rotated.  Everything is
 fp32 inside and rounded once.  An angle is a 64-bit fraction of a turn: off by
-|position| 2^-54 of a turn, and sines of small angles keep fp32's precision.
+|position| 2^-64 of a turn, and sines of small angles keep fp32's precision.
 
 Differentiable by q, k and the weights (once, in reverse mode); the weights' gradients come
 from fixed-order sums, the same bits every time.  Into a CUDA graph, capture

@@ -590,3 +590,19 @@ def test_small_angles_keep_their_precision(rot, inter):
     for sine, cosine in _one_hot_turns(rot, f, pos, inter):
         assert ((sine.double() - s).abs() <= 8 * U * s.abs()).all()
         assert ((cosine.double() - c).abs() <= 8 * U).all()
+
+
+@pytest.mark.parametrize("inter", [False, True])
+def test_far_angles(rot, inter):
+    """Sines and cosines at any int32 position, and beyond: 8 roundings of 2^-24 (the
+    angle within its quarter turn, 3 of pi / 4; the series, 3), and what the fraction of
+    a turn per position, 2^-64, comes to at the position."""
+    f = rot.rotary_frequencies(64, theta=1e4)
+    far = torch.tensor([(1 << 31) - 1, (1 << 31) - 12345, -(1 << 31), (1 << 30) + 7, 1 << 27, -((1 << 24) + 1)],
+                       dtype=torch.int64, device="cuda")
+    further = torch.tensor([(1 << 40) + 3, -(1 << 36) - 5], dtype=torch.int64, device="cuda")
+    for pos in (far.int(), far, further):
+        s, c = _sine_cosine(f, pos)
+        tol = 8 * U + 2 * math.pi * pos.abs().double().view(-1, 1) * 2.0 ** -64
+        for sine, cosine in _one_hot_turns(rot, f, pos, inter):
+            assert ((sine.double() - s).abs() <= tol).all() and ((cosine.double() - c).abs() <= tol).all()
