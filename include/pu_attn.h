@@ -331,6 +331,8 @@ PU_API int pu_decode_paged(const void* q, int q_dtype,
  *   keys / values; D 64 or 128.  o bf16 [B,H,1,D]; lse fp32 [B,H] or NULL.
  *   A sequence of length 0 gives o = 0 and lse = -inf.
  * The work is shared evenly over the SMs whatever the lengths are.
+ * H <= 65535, and B * H <= 65535 or, on the tensor core (q and pools of one
+ * 16-bit type with H / H_kv >= 2, or e4m3 pools with D = 128), B <= 8192.
  *   workspace: pu_decode_paged_gqa_workspace_size() bytes, zeroed before its
  *   first use (left zeroed, as for pu_decode).
  */

@@ -657,7 +657,8 @@ int launch(const Params& prm, int q_dtype, int kv_dtype, int D, int BH, cudaStre
 }
 
 inline int check_args(const void* q, int q_dtype, const void* k, const void* v, int kv_dtype,
-                      long long B, long long H, long long n, long long D, bool allow_fp8 = false) {
+                      long long B, long long H, long long n, long long D, bool allow_fp8 = false,
+                      bool count_heads = true) {
   if (allow_fp8 && kv_dtype == PU_DTYPE_FP8_E4M3) kv_dtype = PU_DTYPE_F16;  // same checks otherwise
   if (!q || !k || !v) return set_error(PU_ERR_INVALID_ARGUMENT, "null q/k/v pointer");
   if (B <= 0 || H <= 0 || n <= 0) return set_error(PU_ERR_INVALID_ARGUMENT, "B, H and the cache length must be positive");
@@ -667,7 +668,7 @@ inline int check_args(const void* q, int q_dtype, const void* k, const void* v, 
     return set_error(PU_ERR_UNSUPPORTED, "decode dtypes must be f16 or bf16");
   if (!aligned16(q) || !aligned16(k) || !aligned16(v))
     return set_error(PU_ERR_INVALID_ARGUMENT, "q/k/v must be 16-byte aligned");
-  if (B * H > kMaxBH) return set_error(PU_ERR_UNSUPPORTED, "B*H = %lld exceeds %d", B * H, kMaxBH);
+  if (count_heads && B * H > kMaxBH) return set_error(PU_ERR_UNSUPPORTED, "B*H = %lld exceeds %d", B * H, kMaxBH);
   if (n > (1ll << 30)) return set_error(PU_ERR_UNSUPPORTED, "cache length too large");
   return PU_OK;
 }

@@ -80,6 +80,7 @@ constexpr int kCtaThreads = 512;
 // registers a thread: softmax 256 x 152, roles 128 x 80, ends 128 x 128 = the launch's 512 x 128 (with 160 / 72 / 120
 // the e4m3 kernels spilled: 24 sequences up to 32768 tokens 172 us instead of 166)
 constexpr int kSoftmaxRegs = 152, kRoleRegs = 80, kEndRegs = 128;
+constexpr int kMaxB = 8192;                // sequences, as many as a page plan takes (each CTA reads all lengths)
 constexpr int kHead = 4;                   // floats before o in a record: m, l, and two that keep o 16-byte aligned
 
 template <typename T, typename KVT, int D>
@@ -1042,6 +1043,7 @@ size_t pu_decode_paged_gqa_workspace_size(int64_t B, int64_t H, int64_t H_kv, in
                                           int64_t page_size, int64_t D) {
   using namespace pu::decode;
   if (B <= 0 || H <= 0 || H_kv <= 0 || H % H_kv || max_pages_per_seq <= 0 || page_size <= 0 || D <= 0) return 0;
+  if (B > kMaxBH / H) return ptc::workspace_bytes(D);      // the tensor-core kernel's alone
   return std::max(ptc::workspace_bytes(D), pu_decode_paged_workspace_size(B, H, max_pages_per_seq, page_size, D));
 }
 
@@ -1054,7 +1056,7 @@ int pu_decode_paged_gqa(const void* q, int q_dtype, const void* k_pool, const vo
   int rc = pu::paged::check_pages(page_table, max_pages_per_seq, num_pages, page_size, &shift);
   if (rc) return rc;
   const long long n_cap = max_pages_per_seq * page_size;
-  rc = check_args(q, q_dtype, k_pool, v_pool, kv_dtype, B, H, n_cap, D, true);
+  rc = check_args(q, q_dtype, k_pool, v_pool, kv_dtype, B, H, n_cap, D, true, false);
   if (rc) return rc;
   if (!o || !kv_lens) return pu::set_error(PU_ERR_INVALID_ARGUMENT, "null output or lengths");
   if (!pu::aligned16(o) || !pu::aligned16(workspace))
@@ -1065,7 +1067,13 @@ int pu_decode_paged_gqa(const void* q, int q_dtype, const void* k_pool, const vo
   if (!(k_scale > 0.f) || !(v_scale > 0.f) || !isfinite(k_scale) || !isfinite(v_scale))
     return pu::set_error(PU_ERR_INVALID_ARGUMENT, "k_scale and v_scale must be positive and finite");
   const bool tensor = ptc::eligible(H, H_kv, D, q_dtype, kv_dtype);
-  const Plan pl = make_plan(B * H, n_cap, D, pu::sm_count(), true, page_size);
+  // the query-head kernel has a counter and a grid row for each (b, h), the
+  // tensor-core kernel a counter for each CTA
+  if (H > kMaxBH || (B > kMaxBH / H && (!tensor || B > ptc::kMaxB)))
+    return pu::set_error(PU_ERR_UNSUPPORTED, "paged decode of %lld sequences with %lld heads (B * H up to %d, or on the tensor core B up to %d)",
+                         (long long)B, (long long)H, kMaxBH, ptc::kMaxB);
+  Plan pl{};
+  if (!tensor) pl = make_plan(B * H, n_cap, D, pu::sm_count(), true, page_size);
   const size_t need = tensor ? ptc::workspace_bytes(D) : pl.total_bytes;
   if (!workspace || workspace_bytes < need)
     return pu::set_error(PU_ERR_WORKSPACE, "paged decode workspace needs %zu bytes, got %zu", need, workspace_bytes);

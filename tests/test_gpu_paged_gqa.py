@@ -551,3 +551,18 @@ def test_serving_chain(mods, kvdt, captured):
         for got, w, mag, c in ((k, want, m, ks), (v, seqs[b][:, H + H_kv:].double(), None, vs)):
             mag = w.abs() if mag is None else mag
             assert ((got - w).abs() <= half * w.abs() + (2.0 ** -10 * c if kvdt == FP8 else 0) + 34 * 2.0 ** -24 * mag).all()
+
+
+@pytest.mark.parametrize("B,H,H_kv,D,kvdt", [(1024, 65, 1, 64, BF), (2100, 32, 8, 128, BF), (1100, 64, 4, 128, FP8)])
+def test_batches_of_many_heads(mods, B, H, H_kv, D, kvdt):
+    """More than 65535 (sequence, head) pairs: the tensor-core kernel counts per CTA."""
+    _lib, dec, paged = mods
+    assert B * H > 65535
+    lens = np.random.RandomState(B).randint(0, 40, B)
+    lens[[0, 17, B - 1]] = [300, 0, 129]
+    ks, vs = (0.02, 0.02) if kvdt == FP8 else (1.0, 1.0)
+    q, k, v, table, n = make(B, H, H_kv, D, 16, lens, BF, kvdt, 3, ks, vs)
+    o, lse = paged.paged_decode(q, k, v, table, n, return_lse=True, k_scale=ks, v_scale=vs)
+    torch.cuda.synchronize()
+    assert _lib.device_status() == (0, 0)
+    check(o, lse, q, k, v, table, lens, None, ks, vs, "many heads")

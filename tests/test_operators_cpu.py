@@ -365,3 +365,18 @@ def test_page_plan_in_place_counts(lib):
     a = [P, P, 4, P, P, Q, None, P, 8, P, P, 16, P, P, P, P, B, 3, None]
     for new in (P, P + 4, P - 4):
         assert so.pu_page_plan(*a[:5], new, *a[6:]) == _lib.PU_ERR_INVALID_ARGUMENT, new
+
+
+def test_batch_limits_of_grouped_paged_decode(lib):
+    """Up to 8192 sequences whatever their heads on the tensor core (what is refused
+    then is the workspace); the query-head kernel counts 65535 heads of sequences."""
+    _lib, so = lib
+    uns, ws = _lib.PU_ERR_UNSUPPORTED, _lib.PU_ERR_WORKSPACE
+    good = [P, 0, P, P, 0, P, 4, 8, 16, P, P, None, P, 1, 2, 8, 2, 128, 0.1, 1.0, 1.0, None]
+    for B, H, H_kv, kv, D, code in ((1024, 64, 8, 0, 128, ws), (8192, 64, 8, 0, 128, ws), (8192, 64, 8, 3, 128, ws), (8193, 64, 8, 0, 128, uns),
+                                    (16000, 4, 2, 0, 128, ws), (1024, 64, 8, 1, 128, uns), (1024, 64, 8, 3, 64, uns), (1, 1 << 20, 8, 0, 128, uns),
+                                    (8192, 1 << 20, 1 << 19, 0, 64, uns)):
+        a = list(good)
+        a[4], a[14], a[15], a[16], a[17] = kv, B, H, H_kv, D
+        assert so.pu_decode_paged_gqa(*a) == code, (B, H, H_kv, kv, D)
+    assert so.pu_decode_paged_gqa_workspace_size(8192, 64, 8, 4, 16, 128) >= so.pu_decode_paged_gqa_workspace_size(1, 64, 8, 4, 16, 128)
