@@ -65,18 +65,28 @@ class DecodeWorkspace:
     (device, stream).  The kernels leave it zeroed after each call, so one
     workspace must not be shared by decode calls that overlap on the GPU."""
 
-    _COUNTERS = 256 * 1024     # the part that must start zeroed
+    _COUNTERS = 256 * 1024     # the counters' part, in front of the records
     _cache: dict = {}
     _lock = threading.Lock()
 
+    @staticmethod
+    def _capturing(device: torch.device) -> bool:
+        """Whether `device`'s current stream, not the current device's, is being captured."""
+        if torch.cuda.current_device() == device.index:
+            return torch.cuda.is_current_stream_capturing()
+        with torch.cuda.device(device):
+            return torch.cuda.is_current_stream_capturing()
+
     @classmethod
-    def get(cls, device: torch.device, nbytes: int) -> torch.Tensor:
-        if torch.cuda.is_current_stream_capturing():
+    def get(cls, device: torch.device, nbytes: int, counters: int = _COUNTERS) -> torch.Tensor:
+        """Scratch of `nbytes`; the call counts in the first `counters` bytes at most."""
+        if cls._capturing(device):
             # a captured call owns its scratch: two graphs captured on one
             # stream may run at the same time, and a larger call may replace
-            # the cached buffer while a graph still points at it
+            # the cached buffer while a graph still points at it.  Every replay
+            # clears what the call counts in, and no more.
             buf = torch.empty(max(nbytes, cls._COUNTERS), dtype=torch.uint8, device=device)
-            buf[:cls._COUNTERS].zero_()
+            buf[:min(counters, cls._COUNTERS)].zero_()
             return buf
         key = (device.index, _lib._raw_stream(device.index))
         buf = cls._cache.get(key)
@@ -108,7 +118,7 @@ def decode_partial(q, k_cache, v_cache, *, kv_offset: int = 0, kv_lens=None,
         out = torch.empty((B * H, D + 2), dtype=torch.float32, device=q.device)
     lib = _lib.lib()
     need = int(lib.pu_decode_workspace_size(B, H, n_local, D))
-    ws = DecodeWorkspace.get(q.device, need)
+    ws = DecodeWorkspace.get(q.device, need, 4 * B * H)
     lens_ptr = kv_lens.data_ptr() if kv_lens is not None else None
     _lib.check(lib.pu_decode_partial(q.data_ptr(), _DT[q.dtype], k_cache.data_ptr(),
                                      v_cache.data_ptr(), _DT[k_cache.dtype], lens_ptr,
@@ -176,7 +186,7 @@ def pallas_flash_decoding(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
     if grouped:
         o = torch.empty((B, H, 1, D), dtype=torch.bfloat16, device=dev)
         lse = torch.empty((B, H), dtype=torch.float32, device=dev)
-        ws = DecodeWorkspace.get(dev, int(lib.pu_decode_gqa_workspace_size(B, H, H_kv, n_local, D)))
+        ws = DecodeWorkspace.get(dev, int(lib.pu_decode_gqa_workspace_size(B, H, H_kv, n_local, D)), 4 * B * H)
         _lib.check(lib.pu_decode_gqa(q_.data_ptr(), _DT[q_.dtype], k_.data_ptr(), v_.data_ptr(),
                                      _DT_KV[k_.dtype],
                                      lens.data_ptr() if lens is not None else None,
@@ -187,7 +197,7 @@ def pallas_flash_decoding(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
         o = torch.empty((B, H, 1, D), dtype=torch.bfloat16, device=dev)
         lse = torch.empty((B, H), dtype=torch.float32, device=dev)
         need = int(lib.pu_decode_workspace_size(B, H, n_local, D))
-        ws = DecodeWorkspace.get(dev, need)
+        ws = DecodeWorkspace.get(dev, need, 4 * B * H)
         _lib.check(lib.pu_decode(q_.data_ptr(), _DT[q_.dtype], k_.data_ptr(), v_.data_ptr(),
                                  _DT[k_.dtype], lens.data_ptr() if lens is not None else None,
                                  o.data_ptr(), lse.data_ptr(), ws.data_ptr(), ws.numel(), B, H,
@@ -207,7 +217,7 @@ def pallas_flash_decoding(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
         if transport == "peer":
             from ..distributed.peer import get_exchange
             ex = get_exchange(B, H, D, group)
-            ws = DecodeWorkspace.get(dev, int(lib.pu_decode_workspace_size(B, H, n_local, D)))
+            ws = DecodeWorkspace.get(dev, int(lib.pu_decode_workspace_size(B, H, n_local, D)), 4 * B * H)
             o, lse = ex.decode(q_, k_, v_, kv_offset=kv_offset, kv_lens=lens,
                                sm_scale=sm_scale, workspace=ws)
         elif transport in ("nccl", "lib"):

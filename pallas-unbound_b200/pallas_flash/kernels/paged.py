@@ -63,6 +63,11 @@ def _gqa_bytes(device: int, B: int, H: int, H_kv: int, max_pages: int, page_size
     return int(_lib.lib().pu_decode_paged_gqa_workspace_size(B, H, H_kv, max_pages, page_size, D))
 
 
+@functools.lru_cache(maxsize=64)
+def _cta_counters(device: int) -> int:
+    return 4 * torch.cuda.get_device_properties(device).multi_processor_count
+
+
 def paged_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
                  page_table: torch.Tensor, kv_lens: torch.Tensor, *,
                  sm_scale: Optional[float] = None, return_lse: bool = False,
@@ -91,14 +96,16 @@ def paged_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
             return (o, lse) if return_lse else o
         if H == H_kv and k_pool.dtype in _DT and k_scale == 1.0 and v_scale == 1.0:
             need = int(lib.pu_decode_paged_workspace_size(B, H, max_pages, page_size, D))
-            ws = DecodeWorkspace.get(q.device, need)
+            ws = DecodeWorkspace.get(q.device, need, 4 * B * H)
             _lib.check(lib.pu_decode_paged(q.data_ptr(), _DT[q.dtype], k_pool.data_ptr(),
                                            v_pool.data_ptr(), _DT[k_pool.dtype], page_table.data_ptr(),
                                            max_pages, P, page_size, kv_lens.data_ptr(), o.data_ptr(),
                                            lse.data_ptr(), ws.data_ptr(), ws.numel(), B, H, D,
                                            float(sm_scale), stream), "pu_decode_paged")
         else:
-            ws = DecodeWorkspace.get(q.device, _gqa_bytes(q.device.index, B, H, H_kv, max_pages, page_size, D))
+            # a counter for each CTA (one an SM), or in the query-head kernel for each head
+            ws = DecodeWorkspace.get(q.device, _gqa_bytes(q.device.index, B, H, H_kv, max_pages, page_size, D),
+                                     max(4 * B * H, _cta_counters(q.device.index)))
             _lib.check(lib.pu_decode_paged_gqa(q.data_ptr(), _DT[q.dtype], k_pool.data_ptr(),
                                                v_pool.data_ptr(), _DT_KV[k_pool.dtype],
                                                page_table.data_ptr(), max_pages, P, page_size,

@@ -566,3 +566,33 @@ def test_batches_of_many_heads(mods, B, H, H_kv, D, kvdt):
     torch.cuda.synchronize()
     assert _lib.device_status() == (0, 0)
     check(o, lse, q, k, v, table, lens, None, ks, vs, "many heads")
+
+
+def test_captured_decodes_clear_what_they_count_in(mods, monkeypatch):
+    """Captured decodes of every kernel on scratch full of garbage: each replay clears the
+    counters that it needs (4 bytes for a sequence's head or an SM) and no more, and is right."""
+    _lib, dec, paged = mods
+    q, k, v, table, n = make(3, 16, 4, 128, 64, [900, 5, 3000], BF, BF, 21)
+    k8, v8 = k.to(FP8), v.to(FP8)
+    dk, dv = _gen((3, 16, 500, 128), 1, BF), _gen((3, 16, 500, 128), 2, BF)
+    calls = [lambda: paged.paged_decode(q, k, v, table, n, return_lse=True),
+             lambda: paged.paged_decode(q, k8, v8, table, n, return_lse=True),
+             lambda: paged.paged_decode(q.half(), k, v, table, n, return_lse=True),       # the query-head kernel
+             lambda: paged.paged_decode(q[:, :4], k, v, table, n, return_lse=True),       # a K/V head each
+             lambda: dec.pallas_flash_decoding(q, dk, dv, return_lse=True),
+             lambda: dec.pallas_flash_decoding(q, dk[:, :4], dv[:, :4], return_lse=True)]
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    get, held = dec.DecodeWorkspace.get, []
+    monkeypatch.setattr(dec.DecodeWorkspace, "get", lambda *a: held.append(get(*a)) or held[-1])
+    for i, call in enumerate(calls):
+        want = [t.clone() for t in call()]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = call()
+        for _ in range(3):
+            held[-1].fill_(255)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), i
+            assert 0 < int((held[-1][:1 << 18] == 0).sum()) <= 4 * max(3 * 16, sms), i
+    assert _lib.device_status() == (0, 0)

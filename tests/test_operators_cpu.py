@@ -380,3 +380,18 @@ def test_batch_limits_of_grouped_paged_decode(lib):
         a[4], a[14], a[15], a[16], a[17] = kv, B, H, H_kv, D
         assert so.pu_decode_paged_gqa(*a) == code, (B, H, H_kv, kv, D)
     assert so.pu_decode_paged_gqa_workspace_size(8192, 64, 8, 4, 16, 128) >= so.pu_decode_paged_gqa_workspace_size(1, 64, 8, 4, 16, 128)
+
+
+def test_captured_scratch_clears_its_counters_only(monkeypatch):
+    """A captured call's own scratch: as many zeroed bytes as its kernels count in, and
+    the question whether a capture runs is asked of the device that was named."""
+    from pallas_flash.kernels.decoding import DecodeWorkspace
+    asked = []
+    monkeypatch.setattr(DecodeWorkspace, "_capturing", staticmethod(lambda device: asked.append(device) or True))
+    empty = torch.empty
+    monkeypatch.setattr(torch, "empty", lambda *a, **kw: empty(*a, **kw).fill_(255))
+    for counters in (4, 592, 8192, 1 << 18, 1 << 19):
+        buf = DecodeWorkspace.get(torch.device("cpu"), (1 << 18) + 4096, counters)
+        used = min(counters, 1 << 18)
+        assert buf.numel() >= (1 << 18) + 4096 and int((buf == 0).sum()) == used and not buf[:used].any()
+    assert asked == [torch.device("cpu")] * 5
