@@ -606,3 +606,86 @@ def test_far_angles(rot, inter):
         tol = 8 * U + 2 * math.pi * pos.abs().double().view(-1, 1) * 2.0 ** -64
         for sine, cosine in _one_hot_turns(rot, f, pos, inter):
             assert ((sine.double() - s).abs() <= tol).all() and ((cosine.double() - c).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("B,N,H,H_kv,D,R,dt,inter", [
+    (4, 700, 40, 8, 128, 128, torch.bfloat16, False), (2, 5000, 7, 3, 64, 32, torch.float16, True),
+    (1, 9001, 5, 2, 96, 96, torch.float32, False), (3, 2369, 4, 1, 128, 64, torch.bfloat16, True),
+    (7, 1016, 6, 2, 16, 16, torch.float32, False), (4, 4096, 32, 8, 128, 128, torch.bfloat16, False)])
+def test_weight_gradients_miss_no_row(rot, B, N, H, H_kv, D, R, dt, inter):
+    """Inputs and gradients of +-1 at position 0, without an epsilon: every row's norm
+    is 1 (looked at first), so the weight gradients are sums of +-1 over the rows, whole
+    numbers under 2^24 that fp32 adds without rounding in any order.  A row that is
+    missing or counted twice changes every one of them."""
+    rows = [B * N * h for h in (H, H_kv)]
+    assert max(rows) < 1 << 20
+    sign = lambda shape, s: (_gen(shape, s) > 0).to(dt) * 2 - 1     # noqa: E731
+    x, g = sign((B, N, (H + H_kv) * D), 1), sign((B, N, (H + H_kv) * D), 2)
+    heads = lambda t: [p.view(B, N, -1, D).transpose(1, 2) for p in t.split([H * D, H_kv * D], -1)]   # noqa: E731
+    q, k = heads(x)
+    gq, gk = heads(g)
+    w = torch.ones(D, device="cuda")
+    f = rot.rotary_frequencies(R)
+    pos = torch.zeros(N, dtype=torch.int32, device="cuda")
+    one = torch.ones((1, 1, 1, D), device="cuda")
+    assert (rot.qk_norm_rope_forward(one, one, f, q_weight=w, eps=0.0)[0] == 1).all()
+    _, _, dwq, dwk = rot.qk_norm_rope_backward(gq, gk, q, k, f, pos, q_weight=w, k_weight=w, eps=0.0, interleaved=inter)
+    for got, a, b in ((dwq, q, gq), (dwk, k, gk)):
+        want = (a.double() * b.double()).sum((0, 1, 2))
+        assert torch.equal(got.double(), want)
+
+
+def test_weight_gradient_behind_2_31_elements(rot):
+    """The weight gradient of a call whose offsets pass 2^31 elements: sums of +-1 as above,
+    whose partial sums stay far under 2^24 (18 million rows of random signs)."""
+    H, N, D = 20, 900_001, 128
+    q = torch.empty((1, H, N, D), dtype=torch.bfloat16, device="cuda")
+    g = torch.empty_like(q)
+    for i, t in enumerate((q, g)):
+        gen = torch.Generator(device="cuda")
+        gen.manual_seed(i)
+        t.random_(0, 2, generator=gen).mul_(2).sub_(1)
+    w, f = torch.ones(D, device="cuda"), rot.rotary_frequencies(D)
+    pos = torch.zeros(N, dtype=torch.int32, device="cuda")
+    dw = rot.qk_norm_rope_backward(g, None, q, q[:, :1], f, pos, q_weight=w, eps=0.0)[2]
+    want = torch.zeros(D, dtype=torch.int64, device="cuda")
+    for h in range(H):
+        want += (q[0, h] * g[0, h]).sum(0, dtype=torch.float32).long()      # +-1: exact in 32 bits under 2^24 rows
+    assert torch.equal(dw.double(), want.double())
+
+
+@pytest.mark.parametrize("B,N", [("7", "R/7"), ("7", "R/7+1"), ("2", "R-1"), ("3", "R"), ("2", "R+1"), ("3", "R+5"), ("4", "2*R-3"),
+                                 ("R+9", "2"), ("2*R+3", "1"), ("3*R//5", "5"), ("R//3+1", "9")])
+@pytest.mark.parametrize("H,H_kv,D", [(2, 1, 64), (6, 2, 128)])
+def test_batches_over_rounds_of_warps(rot, B, N, H, H_kv, D):
+    """Batches in which a warp takes a second and third whole token (R warps a round),
+    in sequences shorter than, equal to and longer than a round: every row equals, bit
+    for bit, the one of a call for its sequences alone, forward and backward, and those are
+    the formula's."""
+    R = torch.cuda.get_device_properties(0).multi_processor_count * 2 * 8
+    B, N = int(eval(B, {"R": R})), int(eval(N, {"R": R}))
+    assert B > 1 and B * N >= R - 7
+    f = rot.rotary_frequencies(D)
+    w = 1 + 0.2 * _gen((D,), 3)
+    q, k = _gen((B, H, N, D), 1, torch.bfloat16), _gen((B, H_kv, N, D), 2, torch.bfloat16)
+    gq, gk = _gen(q.shape, 4, torch.bfloat16), _gen(k.shape, 5, torch.bfloat16)
+    pos = torch.randint(0, 1 << 20, (B, N), device="cuda", dtype=torch.int32)
+    kw = dict(q_weight=w, k_weight=w)
+    y = rot.qk_norm_rope_forward(q, k, f, pos, **kw)
+    d = rot.qk_norm_rope_backward(gq, gk, q, k, f, pos, **kw)[:2]
+    # sequences in groups of less than a round of tokens, so that each is one unit or a part of one
+    step = max(1, (R // 2) // N)
+    for b in range(0, B, step):
+        s = slice(b, b + step)
+        for n in range(0, N, R // 2):
+            at = (s, slice(None), slice(n, n + R // 2))
+            a = [t[at].contiguous() for t in (q, k, gq, gk)]
+            p = pos[s, n:n + R // 2].contiguous()
+            assert all(torch.equal(u, v[at]) for u, v in zip(rot.qk_norm_rope_forward(a[0], a[1], f, p, **kw), y)), (b, n)
+            assert all(torch.equal(u, v[at]) for u, v in zip(rot.qk_norm_rope_backward(a[2], a[3], a[0], a[1], f, p, **kw)[:2], d)), (b, n)
+    cos, sin = _turns(f, pos, None, B, N)
+    for i, (x, g) in enumerate(((q, gq), (k, gk))):
+        want, mag = _oracle(x, w, cos, sin, False, 1e-6)
+        _close(y[i], want, mag, 32, f"output {i}")
+        dx, dxm, _, _ = _oracle_back(x, w, g, cos, sin, False, 1e-6)
+        _close(d[i], dx, dxm, 48, f"gradient {i}")
