@@ -394,7 +394,14 @@ class DevicePagedKVCache:
     o = cache.decode(q)                                        # one new token each
 
     Nothing here reads from the device, so a step can be captured into a CUDA
-    graph (new_lens, release, q, k and v in fixed buffers) and replayed."""
+    graph (new_lens, release, q, k and v in fixed buffers) and replayed.
+
+    This is one layer's cache.  A model of several layers plans once a step
+    (`plan_append`) and gives every layer the same slots, positions, table and
+    lengths with pools of its own (`qk_norm_rope_append`, `paged_decode`): L of these
+    caches would plan L times.  `decode` attends one token a sequence; a prompt's
+    own attention runs on dense tensors (`qk_norm_rope`, whose keys are those
+    that `append` stores, then `pallas_flash_attention`)."""
 
     def __init__(self, batch: int, kv_heads: int, head_dim: int, *, num_pages: int, page_size: int = 64,
                  max_seq_len: int, dtype=torch.bfloat16, k_scale: float = 1.0, v_scale: float = 1.0,

@@ -7,6 +7,10 @@ takes q, k, v as they are (src/pallas_flash/ops/interface.py:20-27).
     q, k = qk_norm_rope(q, k, inv_freq, positions, q_weight=wq, k_weight=wk)
     o = pallas_flash_attention(q, k, v, causal=True)
 
+With fewer key heads than query heads, k and v are repeated in between
+(`k.repeat_interleave(H // H_kv, 1)`): the attention takes a key head for each
+query head, while the norm and rotation need each key head once.
+
 For one row x of D values (one head of one token):
   n = x / sqrt(mean(x^2) + eps) * weight
   (a, b) = pair p of n  ->  (a cos t - b sin t, b cos t + a sin t),
@@ -282,10 +286,11 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, inv_freq: torch.Tensor,
                  sections: Optional[Sequence[int]] = None, interleaved: bool = False):
     """Norm and rotate every head of q [B,H,N,D] and k [B,H_kv,N,D].
 
-    Returns dense (q, k) of the same shapes and dtype (bf16, fp16 or fp32),
-    ready for `pallas_flash_attention`.  q and k may be strided views, such as
-    a projection's [B,N,H,D] transposed: rows that start on 16-byte boundaries
-    are read where they are, others through a copy.
+    Returns dense (q, k) of the same shapes and dtype (bf16, fp16 or fp32), what
+    `pallas_flash_attention` takes where H_kv == H (otherwise repeat k's heads
+    first).  q and k may be strided views, such as a projection's [B,N,H,D]
+    transposed: rows that start on 16-byte boundaries are read where they are,
+    others through a copy.
 
       inv_freq   [R/2] fp64 or fp32 radians per position; R/2 a multiple of 8.  There
                  is no gradient by them: one that requires_grad is refused

@@ -596,3 +596,59 @@ def test_captured_decodes_clear_what_they_count_in(mods, monkeypatch):
             assert all(torch.equal(a, b) for a, b in zip(got, want)), i
             assert 0 < int((held[-1][:1 << 18] == 0).sum()) <= 4 * max(3 * 16, sms), i
     assert _lib.device_status() == (0, 0)
+
+
+@pytest.mark.parametrize("kvdt", [BF, FP8])
+def test_layers_share_a_plan(mods, kvdt):
+    """A model of several layers plans a step once: every layer writes to the plan's slots
+    in pools of its own and decodes over the one table, all in one captured graph."""
+    from pallas_flash.ops.rotary import rotary_frequencies
+    _lib, dec, paged = mods
+    L, B, H, H_kv, D, page, P = 3, 3, 8, 2, 128, 16, 40
+    ks, vs = (0.05, 0.03) if kvdt == FP8 else (1.0, 1.0)
+    pools = [[torch.zeros((P, H_kv, page, D), device="cuda").to(kvdt) for _ in range(2)] for _ in range(L)]
+    table = torch.full((B, 12), -1, dtype=torch.int32, device="cuda")
+    lens = torch.zeros(B, dtype=torch.int32, device="cuda")
+    ring = torch.arange(P, dtype=torch.int32, device="cuda")
+    cursor = torch.tensor([0, P], dtype=torch.int64, device="cuda")
+    f = rotary_frequencies(D)
+    ws = [[1 + 0.1 * _gen((D,), 10 * i + s) for s in range(2)] for i in range(L)]
+
+    def step(new, xs, T):
+        plan = paged.plan_append(table, lens, new, ring, cursor, page_size=page, num_tokens=T, inplace=True)
+        qs = [paged.qk_norm_rope_append(x[:, :H], x[:, H:H + H_kv], x[:, H + H_kv:], f, plan.positions, plan.slots, *pools[i],
+                                        q_weight=ws[i][0], k_weight=ws[i][1], k_scale=ks, v_scale=vs) for i, x in enumerate(xs)]
+        return qs, plan
+
+    prompts = torch.tensor([33, 0, 100], dtype=torch.int32, device="cuda")
+    x0 = [_gen((140, H + 2 * H_kv, D), 30 + i, BF) for i in range(L)]
+    _, plan = step(prompts, x0, 140)
+    seqs = [[x[plan.seq_ids == b] for b in range(B)] for x in x0]
+    one = torch.ones(B, dtype=torch.int32, device="cuda")
+    xs = [torch.zeros((B, H + 2 * H_kv, D), dtype=BF, device="cuda") for _ in range(L)]
+    state = (table, lens, ring, cursor)
+    saved = [t.clone() for t in state]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        qs, _ = step(one, xs, B)
+        outs = [paged.paged_decode(q.unsqueeze(2), *pools[i], table, lens, return_lse=True, k_scale=ks, v_scale=vs)
+                for i, q in enumerate(qs)]
+    for t, s in zip(state, saved):
+        t.copy_(s)
+    held = [33, 0, 100]
+    for n in range(20):
+        for i in range(L):
+            xs[i].copy_(_gen(xs[i].shape, 1000 + 10 * n + i, BF))
+            seqs[i] = [torch.cat([s, xs[i][b:b + 1]]) for b, s in enumerate(seqs[i])]
+        graph.replay()
+        held = [m + 1 for m in held]
+        assert lens.tolist() == held
+        for i in range(L):
+            check(outs[i][0], outs[i][1], qs[i].unsqueeze(2), *pools[i], table, held, None, ks, vs, f"step {n} layer {i}")
+    assert _lib.device_status() == (0, 0)
+    half = 2.0 ** -4 if kvdt == FP8 else 2.0 ** -8
+    for i in range(L):
+        for b in range(B):
+            k = dense(pools[i][0], table, b, held[b], ks).transpose(0, 1)
+            want, m = _turned(seqs[i][b][:, H:H + H_kv], ws[i][1], f, torch.arange(held[b], device="cuda"))
+            assert ((k - want).abs() <= half * want.abs() + (2.0 ** -10 * ks if kvdt == FP8 else 0) + 34 * 2.0 ** -24 * m).all()

@@ -689,3 +689,38 @@ def test_batches_over_rounds_of_warps(rot, B, N, H, H_kv, D):
         _close(y[i], want, mag, 32, f"output {i}")
         dx, dxm, _, _ = _oracle_back(x, w, g, cos, sin, False, 1e-6)
         _close(d[i], dx, dxm, 48, f"gradient {i}")
+
+
+def test_training_chain_with_grouped_heads(rot):
+    """Fewer key heads than query heads: normed and rotated as they are, then repeated
+    for the attention, which takes one key head per query head; against the chain in 64 bits."""
+    from pallas_flash.ops.interface import pallas_flash_attention
+    B, N, H, H_kv, D = 2, 130, 6, 2, 128
+    G = H // H_kv
+    x = _gen((B, N, (H + 2 * H_kv) * D), 1, torch.bfloat16)
+    wq, wk = ((1 + 0.1 * _gen((D,), s)) for s in (2, 3))
+    f = rot.rotary_frequencies(D)
+    do = _gen((B, H, N, D), 4, torch.bfloat16)
+
+    def split(t):
+        return [p.view(B, N, -1, D).transpose(1, 2) for p in t.split([H * D, H_kv * D, H_kv * D], -1)]
+
+    leaf = x.clone().requires_grad_(True)
+    ws = [w.clone().requires_grad_(True) for w in (wq, wk)]
+    q, k, v = split(leaf)
+    q, k = rot.qk_norm_rope(q, k, f, q_weight=ws[0], k_weight=ws[1])
+    o = pallas_flash_attention(q, k.repeat_interleave(G, 1), v.repeat_interleave(G, 1), causal=True)
+    got = torch.autograd.grad(o, [leaf] + ws, do)
+
+    leaf64 = x.double().requires_grad_(True)
+    ws64 = [w.double().requires_grad_(True) for w in (wq, wk)]
+    q, k, v = split(leaf64)
+    cos, sin = _turns(f, None, None, B, N)
+    q, k = (_oracle(t, w, cos, sin, False, 1e-6)[0] for t, w in ((q, ws64[0]), (k, ws64[1])))
+    s = (q @ k.repeat_interleave(G, 1).transpose(2, 3)) / math.sqrt(D)
+    s = s.masked_fill(torch.ones(N, N, dtype=torch.bool, device="cuda").triu(1), -math.inf)
+    o64 = s.softmax(-1) @ v.repeat_interleave(G, 1)
+    want = torch.autograd.grad(o64, [leaf64] + ws64, do.double())
+    assert_close_o(to_np(o), to_np(o64), what="chain")
+    for n, a, b in zip(("x", "wq", "wk"), got, want):
+        assert_close_grad(to_np(a), to_np(b), what=n)
