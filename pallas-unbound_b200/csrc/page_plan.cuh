@@ -16,18 +16,19 @@
 // release is refused whole where the ring has no room for the pages (they would be
 // in neither table nor ring), and only entries that name a page go back.
 //
-// Every CTA scans all B sequences itself (three block-wide sums in 64 bits;
+// Every CTA scans all B sequences itself (block-wide sums in 64 bits;
 // a second kernel would cost more than the repeated reads of a few KB from
 // L2) and then takes its share of table rows and tokens.  Where the state is
 // advanced in place, the CTAs form one cluster of 8 and meet at its barrier
 // between the last read of the lengths and the first write; with separate
 // outputs nothing is shared and the grid grows with the work.
 //
-// Bound by latency: one read of the lengths, three scans, the dependent reads
-// of table and ring, one write.  256 sequences with 2048 table entries each
-// (2 MB of table written) and 61 prompts of up to 2500 tokens both take 9 us a
-// call back to back; the call's own host time is 20 us.
-// Released rows are read ahead of the scans, to count the pages that come back.
+// Bound by latency: one read of the lengths, two rounds of scans, the dependent reads
+// of table and ring, one write.  Measured back to back in a graph: 256 sequences with
+// 2048 table entries each (2 MB of table written) 9 us, 12.6 with 17 of them released
+// (their rows are read ahead of the scans, by every CTA, to count the pages that come
+// back; one released 9.6); 61 prompts of up to 2500 tokens 9.6; in place 64 sequences 5.9,
+// one of them released 7.3.  A call's own host time is 20 us.
 #pragma once
 
 #include "paged.cuh"
@@ -98,8 +99,10 @@ __global__ void __launch_bounds__(kThreads) page_plan_kernel(const Params p) {
                                          // -2 - place: the row has entries that are no pages
   __shared__ long long s_warp[2][32];
   __shared__ int s_used;                 // pages taken
+  __shared__ int s_released;             // rows that return pages
   const int tid = threadIdx.x;
-  if (tid == 0) s_used = 0;
+  if (tid == 0) s_used = s_released = 0;
+  __syncthreads();
   grid_dep_wait();
   grid_dep_launch_dependents();
 
@@ -116,29 +119,60 @@ __global__ void __launch_bounds__(kThreads) page_plan_kernel(const Params p) {
   auto held_of = [&](int b) { return (int)min((long long)max(p.lens[b], 0), cap); };
   auto gone = [&](int b) { return p.release != nullptr && p.release[b] != 0; };
   long long tokens = 0, freed = 0;
-  bool any = false;
-  for (int b = b0; b < b1; ++b) {
-    s_base[b] = gone(b) ? 0 : held_of(b);
-    s_freed[b] = gone(b) ? (held_of(b) + page - 1) >> p.page_shift : 0;
-    any |= s_freed[b] > 0;
-    tokens += max(p.add[b], 0);
-  }
   const int lane = tid & 31;
-  if (__syncthreads_or(any)) {
-    // how many of a released row's entries name a page (-1 - the count where some do
-    // not): a warp per row
-    for (int b = tid >> 5; b < p.B; b += kThreads / 32) {
-      const int old = s_freed[b];
-      if (old == 0) continue;
-      int good = 0;
-      for (int j = lane; j < old; j += 32) good += (unsigned)p.table[(size_t)b * p.max_pages + j] < (unsigned)p.num_pages;
+  for (int i = 0; i < per; ++i) {
+    const int b = b0 + i;
+    const bool mine = b < b1;
+    int back = 0;                        // pages that the row returns
+    if (mine) {
+      const int held = held_of(b);
+      if (gone(b)) back = (held + page - 1) >> p.page_shift;
+      s_base[b] = gone(b) ? 0 : held;
+      s_freed[b] = back;
+      tokens += max(p.add[b], 0);
+    }
+    // a list of the rows that return some, in s_new for now (an atomic for each of
+    // them, not each warp, took 2 us)
+    const unsigned some = __ballot_sync(0xffffffffu, back > 0);
+    if (some == 0) continue;
+    int at = 0;
+    if (lane == 0) at = atomicAdd(&s_released, __popc(some));
+    at = __shfl_sync(0xffffffffu, at, 0);
+    if (back > 0) {
+      s_new[at + __popc(some & ((1u << lane) - 1u))] = b;
+      s_last[b] = 0;                     // how many of its entries are pages
+    }
+  }
+  constexpr int kSeg = 512;              // entries a warp takes at once
+  const int segs = (p.max_pages + kSeg - 1) / kSeg;
+  constexpr int kPiece = 256;            // entries a warp counts at once
+  const int pieces = (p.max_pages + kPiece - 1) / kPiece;
+  __syncthreads();
+  if (s_released > 0) {
+    // How many of the released rows' entries name a page (s_freed: -1 - the count where
+    // some do not).  A warp has the loads of a piece in flight; with a row for a warp, 17
+    // rows of up to 1875 entries took 5 us, pieces of 256 take 3.2, of 512 and 128 3.6, 4.2.
+    const unsigned units = (unsigned)s_released * (unsigned)pieces;      // 2^13 * 2^18 at most
+    for (unsigned u = tid >> 5; u < units; u += kThreads / 32) {
+      const unsigned row = u / (unsigned)pieces;
+      const int b = s_new[row], lo = (int)(u - row * pieces) * kPiece, n = min(s_freed[b] - lo, kPiece);
+      if (n <= 0) continue;
+      const int32_t* in = p.table + (size_t)b * p.max_pages + lo;
+      int entry[kPiece / 32], good = 0;
 #pragma unroll
-      for (int off = 16; off > 0; off >>= 1) good += __shfl_xor_sync(0xffffffffu, good, off);
-      __syncwarp();                      // every lane has read the row's page count
-      if (lane == 0) s_freed[b] = good == old ? good : -1 - good;
+      for (int i = 0; i < kPiece / 32; ++i) entry[i] = i * 32 < n ? in[min(i * 32 + lane, n - 1)] : -1;
+#pragma unroll
+      for (int i = 0; i < kPiece / 32; ++i) good += i * 32 + lane < n && (unsigned)entry[i] < (unsigned)p.num_pages;
+      good = __reduce_add_sync(0xffffffffu, good);
+      if (lane == 0 && good > 0) atomicAdd(&s_last[b], good);
     }
     __syncthreads();
-    for (int b = b0; b < b1; ++b) freed += s_freed[b] < 0 ? -1 - s_freed[b] : s_freed[b];
+    for (int b = b0; b < b1; ++b) {
+      if (s_freed[b] == 0) continue;
+      const int good = s_last[b];
+      freed += good;
+      if (good != s_freed[b]) s_freed[b] = -1 - good;
+    }
   }
   long long sums[2] = {tokens, freed}, totals[2];
   block_scan(sums, s_warp, totals);
@@ -194,8 +228,6 @@ __global__ void __launch_bounds__(kThreads) page_plan_kernel(const Params p) {
   // rows: pages kept, pages taken, then none
   const int warps = (int)gridDim.x * (kThreads / 32), wid = (int)blockIdx.x * (kThreads / 32) + (tid >> 5);
   auto taken = [&](int i) { int r = head0 + i; return p.ring[r >= p.num_pages ? r - p.num_pages : r]; };
-  constexpr int kSeg = 512;              // entries a warp takes at once
-  const int segs = (p.max_pages + kSeg - 1) / kSeg;
   if constexpr (kInPlace) {
     // only the released rows still need their old lengths: put them where the
     // rows' owners find them before the lengths change
