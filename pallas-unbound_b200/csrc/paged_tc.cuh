@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
   const uint32_t tmem = *tmem_slot;
   const Start st = *s_start;
   // CTA c: units [c q + min(c, rem), ...), q or q + 1 of them
-  const long long ctas = st.ctas, q = st.q, rem = st.rem, first = st.first, end = st.end;
+  const long long q = st.q, rem = st.rem, first = st.first, end = st.end;
   auto part = [&](long long c) { return c * q + min(c, rem); };
   long long item0 = st.item0;
   Walk w0;

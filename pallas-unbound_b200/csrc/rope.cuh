@@ -49,8 +49,7 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kMaxDim = 128;
 constexpr int kMaxPairs = kMaxDim / 2;
 constexpr int kMaxAxes = 4;
-constexpr int kFwdCtasPerSm = 2;     // resident CTAs the grids ask for
-constexpr int kCtasPerSm = 2;
+constexpr int kCtasPerSm = 2;        // resident CTAs the grids ask for
 
 // Rows of one tensor: element (b, h, n, d) at b sB + h sH + n sN + d.
 struct Rows {
@@ -599,7 +598,7 @@ struct Feed {
 };
 
 template <typename T, int kLanes, bool kInter, bool kAppend>
-__global__ void __launch_bounds__(kThreads, kFwdCtasPerSm) fwd_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) fwd_kernel(const __grid_constant__ Params p) {
   constexpr int kRows = 32 / kLanes;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ __align__(16) Shared sh;
@@ -1007,7 +1006,7 @@ inline int share_out(Params& p, int kinds, int ctas_per_sm) {
 
 template <typename T, bool kAppend>
 int launch_fwd(Params& p, bool inter, cudaStream_t st) {
-  const int grid = share_out(p, kAppend ? 3 : 2, kFwdCtasPerSm);
+  const int grid = share_out(p, kAppend ? 3 : 2, kCtasPerSm);
   const bool wide = lanes_of(p.D) == 8;
   auto* k = wide ? (inter ? fwd_kernel<T, 8, true, kAppend> : fwd_kernel<T, 8, false, kAppend>)
                  : (inter ? fwd_kernel<T, 4, true, kAppend> : fwd_kernel<T, 4, false, kAppend>);
