@@ -240,18 +240,16 @@ def qk_norm_rope_backward(gq, gk, q, k, inv_freq, positions=None, *, q_weight=No
     return _backward(desc, gq, gk, q, k, weight_grads, weight_grads)
 
 
-def _plain(desc):
-    """What a description holds beside tensors and their strides."""
-    return desc[:8] + desc[11:13] + desc[15:]
-
-
 class _QkNormRope(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, inv_freq, positions, eps, sections, interleaved):
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(q, k, q_weight, k_weight, inv_freq, positions)
+        # positions and frequencies stay here, as they were described: a saved-tensor
+        # hook may give another tensor back, with other strides
+        ctx.save_for_backward(q, k, q_weight, k_weight)
         desc = _description(q, k, inv_freq, positions, q_weight, k_weight, eps, sections, interleaved)
-        ctx.plain, ctx.sections = _plain(desc), None if sections is None else desc[12][:desc[11]]
+        ctx.desc, ctx.angles = desc[:13] + (None, None) + desc[15:], (inv_freq, positions)
+        ctx.versions = [t._version for t in ctx.angles if t is not None]
         return _forward(desc, q, k)
 
     @staticmethod
@@ -262,18 +260,20 @@ class _QkNormRope(torch.autograd.Function):
 
     @staticmethod
     def _grads(ctx, gq, gk):
-        q, k, wq, wk, inv_freq, positions = ctx.saved_tensors
-        need, plain = ctx.needs_input_grad, ctx.plain
+        q, k, wq, wk = ctx.saved_tensors
+        need, desc, dev = ctx.needs_input_grad, ctx.desc, ctx.angles[0].device
+        B, N, H, H_kv, D, dtype = desc[:6]
+        if ctx.versions != [t._version for t in ctx.angles if t is not None]:
+            raise RuntimeError("positions or inv_freq were changed in place since the forward")
+        if q.shape != (B, H, N, D) or k.shape != (B, H_kv, N, D) or q.dtype != dtype or k.dtype != dtype \
+                or q.device != dev or k.device != dev:
+            raise ValueError("a saved tensor came back with another shape, type or device")
         if not (need[0] or need[2]):
             gq = None
         if not (need[1] or need[3]):
             gk = None
-        # described anew: saved-tensor hooks may give other tensors back (dense
-        # copies of strided views, say), so nothing of the forward's pointers,
-        # strides or types is carried over
-        desc = _description(q, k, inv_freq, positions, wq, wk, plain[-1], ctx.sections, plain[7])
-        if _plain(desc) != plain:
-            raise ValueError("a saved tensor came back with another shape or type")
+        wq, wk = _check_weight(wq, D, dev, "q_weight"), _check_weight(wk, D, dev, "k_weight")
+        desc = desc[:13] + (wq, wk) + desc[15:]
         dq, dk, dwq, dwk = _backward(desc, gq, gk, q, k, need[2], need[3])
         return (dq if need[0] else None, dk if need[1] else None, dwq, dwk, None, None, None, None, None)
 

@@ -4,6 +4,7 @@ decode entry points, without a GPU: the host checks come before any CUDA call
 from __future__ import annotations
 
 import ctypes
+import itertools
 import re
 from pathlib import Path
 
@@ -261,8 +262,8 @@ def _addressed(pointer, strides, shape, dtype):
 @pytest.mark.parametrize("sections", [None, (8, 12, 12)])
 @pytest.mark.parametrize("hooked", [False, True])
 def test_backward_addresses_the_saved_tensors(host_rotary, sections, hooked):
-    """What the backward is told to read lies inside the tensors that it was given, also
-    where saved-tensor hooks gave copies with other strides back."""
+    """What the backward is told to read lies inside tensors that are there, and holds
+    the positions, also where saved-tensor hooks gave copies with other strides back."""
     import contextlib
     rotary, so = host_rotary
     B, N, H, H_kv, D = 3, 4, 4, 2, 64
@@ -285,14 +286,16 @@ def test_backward_addresses_the_saved_tensors(host_rotary, sections, hooked):
         torch.autograd.grad(y, (q, k, w), tuple(torch.ones_like(t) for t in y))
     desc, pq, pk = so.calls["pu_qk_norm_rope_bwd"][:3]
     d = rotary._DESC.unpack(desc)
-    known = held if hooked else [t.detach() for t in (q, k, freq, pos, w)]
+    known = held + [t.detach() for t in (q, k, freq, pos, w)]
     inside = lambda lo, hi: any(t.data_ptr() <= lo and hi <= t.data_ptr() + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
                                 * t.element_size() for t in known)     # noqa: E731
     assert len(d) == 46 and d[10] != 0
     strides = d[12:15]
     shape = (3, B, N) if sections else (1, B, N)
-    assert strides == (((4 * B, 4, 1) if hooked else (100 * B, 100, 1)) if sections else ((0, 4, 1) if hooked else (0, 100, 1)))
     assert inside(*_addressed(d[10], strides, shape, torch.int32))
+    at = lambda i: ctypes.c_int32.from_address(d[10] + 4 * sum(a * b for a, b in zip(i, strides))).value     # noqa: E731
+    want = pos if sections else pos.expand(1, B, N)
+    assert all(at(i) == int(want[i]) for i in itertools.product(*map(range, shape if sections else (1, B, N))))
     for p, st, heads in ((pq, d[25:28], H), (pk, d[28:31], H_kv)):
         assert inside(*_addressed(p, tuple(st) + (1,), (B, heads, N, D), torch.bfloat16))
 
@@ -301,15 +304,28 @@ def test_hooks_that_give_other_tensors_back_are_refused(host_rotary):
     """A saved tensor of another type or shape is refused before the library is asked."""
     rotary, so = host_rotary
     q, k = (torch.randn(2, h, 5, 64, dtype=torch.bfloat16, requires_grad=True) for h in (4, 2))
+    w = torch.ones(64, requires_grad=True)
     f, pos = torch.ones(32, dtype=torch.float64), torch.zeros(2, 5, dtype=torch.int32)
-    for which, other in ((torch.int32, lambda t: t.float()), (torch.int32, lambda t: t[:, :3]), (torch.float64, lambda t: t[:8]),
-                         (torch.bfloat16, lambda t: t.float())):
+    for which, other in ((torch.float32, lambda t: t[:32]), (torch.float32, lambda t: t.double()), (torch.bfloat16, lambda t: t.float()),
+                         (torch.bfloat16, lambda t: t[:, :, 1:]), (torch.bfloat16, lambda t: t.to("meta"))):
         so.calls.clear()
         with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: other(t) if t.dtype == which else t):
-            y = rotary.qk_norm_rope(q, k, f, pos)
+            y = rotary.qk_norm_rope(q, k, f, pos, q_weight=w)
             with pytest.raises((ValueError, TypeError)):
-                torch.autograd.grad(y, (q, k), tuple(torch.ones_like(t) for t in y))
+                torch.autograd.grad(y, (q, k, w), tuple(torch.ones_like(t) for t in y))
         assert "pu_qk_norm_rope_bwd" not in so.calls
+
+
+@pytest.mark.parametrize("which", ["positions", "inv_freq", "q"])
+def test_inputs_changed_before_the_backward_are_refused(host_rotary, which):
+    rotary, so = host_rotary
+    x = {"q": torch.randn(2, 4, 5, 64), "inv_freq": torch.ones(32, dtype=torch.float64), "positions": torch.zeros(2, 5, dtype=torch.int32)}
+    k = torch.randn(2, 2, 5, 64, requires_grad=True)
+    y = rotary.qk_norm_rope(x["q"], k, x["inv_freq"], x["positions"])
+    x[which].add_(1)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(y[1], k, torch.ones_like(k))
+    assert "pu_qk_norm_rope_bwd" not in so.calls
 
 
 def test_forward_mode_is_refused(host_rotary):
