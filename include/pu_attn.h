@@ -330,6 +330,9 @@ PU_API int pu_decode_paged(const void* q, int q_dtype,
  *   PU_DTYPE_FP8_E4M3, whose stored values times k_scale / v_scale are the
  *   keys / values; D 64 or 128.  o bf16 [B,H,1,D]; lse fp32 [B,H] or NULL.
  *   A sequence of length 0 gives o = 0 and lse = -inf.
+ *   On the tensor core the softmax weights are rounded once to the pools'
+ *   16-bit type, or held in three e4m3 parts (12 bits); with e4m3 pools an
+ *   element of q is off by at most 2^-17 of its head's largest.
  * The work is shared evenly over the SMs whatever the lengths are.
  * H <= 65535, and B * H <= 65535 or, on the tensor core (q and pools of one
  * 16-bit type with H / H_kv >= 2, or e4m3 pools with D = 128), B <= 8192.

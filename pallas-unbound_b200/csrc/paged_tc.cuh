@@ -45,7 +45,10 @@
 //
 // e4m3: K and V tiles are operands as stored; q and P are split into e4m3
 // parts stacked along N: q into two parts if bf16 (8 significant bits are
-// two e4m3 parts exactly) and three if f16 (11 bits), P into three.
+// two e4m3 parts exactly) and three if f16 (11 bits), P into three.  The parts of
+// q share the scale of the head's largest element, so an element is off by at most
+// 2^-17 of that one.  With 16-bit pages P is rounded once to their type (the fp32
+// sums l are taken before): outputs differ from an fp32 P's inside bf16's last step.
 //
 // Pages.  Only pages that hold tokens of the sequence are read.  An entry
 // outside the pool is not followed: it is reported (detail 302) and its
@@ -55,8 +58,8 @@
 // Measured (calls back to back on pools that do not fit L2; the copy rate of
 // this GPU is 6.4 TB/s): 8 sequences of 4096 to 131072 tokens, 32 heads over 8
 // of 128, f16, 64-token pages: 2.51 GB in 357 us = 7.0 TB/s; 24 sequences of up
-// to 32768 tokens, 64 heads over 8, e4m3, 32-token pages: 0.98 GB in 166 us =
-// 5.9 TB/s (the splitting of P shares the issue slots with everything else); 256
+// to 32768 tokens, 64 heads over 8, e4m3, 32-token pages: 0.98 GB in 157 to 166 us =
+// 5.9 to 6.3 TB/s (the splitting of P shares the issue slots with everything else); 256
 // sequences of up to 2048 tokens, 16 heads over 2 of 64, 16-token pages: 135 MB
 // in 39 us, of which 28 us are the loads alone, the rest the start, the last
 // tile's chain and the joins; one sequence of 1000 tokens: 11 us.

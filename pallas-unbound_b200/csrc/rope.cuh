@@ -30,10 +30,14 @@
 // Both directions read and write each row once: forward 2, backward 3 passes
 // over the rows.  Measured (calls back to back; copy rate 6.4 TB/s): 4 x 4096
 // tokens, 32 + 8 heads of 128, bf16: forward 336 MB in 58 us (5.8 TB/s, 91 %),
-// backward 503 MB in 109 us (4.6 TB/s, 72 %: instructions share the time with
-// the copies).  128 registers and 16 warps an SM measured best: 24 warps forward
-// 65 us, 20 warps 64.  17 packed prompts of 15 thousand tokens into a cache,
-// 184 MB, 44 us.  64 tokens 4 us.
+// backward 503 MB in 109 us (4.6 TB/s, 72 %: neither issue slots, 56 %, nor DRAM
+// full, but the chains of a pass and its lane sums at 16 warps an SM); with
+// neighbouring pairs 83 to 87 and 176 (the exchange inside each packed pair); fp32
+// 671 MB in 165 us (4.1 TB/s) and 1.0 GB in 265 (3.8 TB/s: ring and sums leave one CTA
+// an SM, and the grid's other half runs behind the first).  128 registers and 16
+// warps an SM measured best in bf16: 24 warps forward 65 us, 20 warps 64.  17 packed
+// prompts of 15 thousand tokens into a cache, 184 MB, 44 us, into e4m3 pages 52 (a
+// division for each element).  64 tokens appended 5.2 us.
 #pragma once
 
 #include <cmath>
