@@ -353,6 +353,94 @@ PU_API int pu_decode_paged_gqa(const void* q, int q_dtype,
                                float sm_scale, float k_scale, float v_scale, void* stream);
 
 /*
+ * The same with page lists of their own for each K/V head: page_table
+ * [B][H_kv][max_pages_per_head], kv_lens [B][H_kv], as pu_select_pages makes
+ * them.  K/V head g's queries attend the first kv_lens[b][g] tokens of its list;
+ * no other page is read.  The workspace is that of pu_decode_paged_gqa (with
+ * max_pages_per_head).  B * H <= 65535 or, on the tensor core, B * H_kv <= 8192.
+ */
+PU_API int pu_decode_paged_heads(const void* q, int q_dtype,
+                                 const void* k_pool, const void* v_pool, int kv_dtype,
+                                 const int32_t* page_table, int64_t max_pages_per_head,
+                                 int64_t num_pages, int64_t page_size,
+                                 const int32_t* kv_lens, void* o, float* lse,
+                                 void* workspace, size_t workspace_bytes,
+                                 int64_t B, int64_t H, int64_t H_kv, int64_t D,
+                                 float sm_scale, float k_scale, float v_scale, void* stream);
+
+/*
+ * Paged decode of sequences that hold the same first pages: the pages shared by
+ * a group are read once for all of it.  No counterpart in the reference.
+ *   Arguments as for pu_decode_paged_gqa, and
+ *   group_starts int32 [groups + 1] (NULL with groups = 1: the whole batch):
+ *     group i is the sequences group_starts[i] <= b < group_starts[i + 1]
+ *     (starts are read as if clamped to [0, B] and raised to those before them;
+ *     sequences in no group share nothing);
+ *   shared_lens int32 [groups]: tokens that the group's sequences have in common,
+ *     in whole pages (rounded down).  They are read through the table row of the
+ *     group's first sequence that holds as many; the others' entries for them must
+ *     name the same pages.  A sequence that holds fewer attends those it holds.  A
+ *     group in which none holds as many shares nothing.
+ * q and pools of one 16-bit type, D 64 or 128, or e4m3 pools with D = 128; any
+ * H / H_kv; groups <= 64; B <= 8192; H <= 65535; H_kv * D <= 2^20 - 16.
+ *   workspace: pu_decode_paged_shared_workspace_size() bytes, zeroed before its
+ *   first use (left as pu_decode_paged_gqa needs it).
+ * The softmax weights of shared tokens are rounded once to the pools' 16-bit type,
+ * to f16 with e4m3 pools (bf16 queries are f16 times a power of two then: exact
+ * down to 2^-31 of a head's largest element).  A table entry of shared tokens
+ * outside the pool is reported (detail 311) and its tokens are left out.
+ */
+PU_API size_t pu_decode_paged_shared_workspace_size(int64_t B, int64_t H, int64_t H_kv,
+                                                    int64_t groups, int64_t D);
+
+PU_API int pu_decode_paged_shared(const void* q, int q_dtype,
+                                  const void* k_pool, const void* v_pool, int kv_dtype,
+                                  const int32_t* page_table, int64_t max_pages_per_seq,
+                                  int64_t num_pages, int64_t page_size,
+                                  const int32_t* kv_lens, const int32_t* shared_lens,
+                                  const int32_t* group_starts, int64_t groups,
+                                  void* o, float* lse, void* workspace, size_t workspace_bytes,
+                                  int64_t B, int64_t H, int64_t H_kv, int64_t D,
+                                  float sm_scale, float k_scale, float v_scale, void* stream);
+
+/*
+ * Bounds of the keys of each page: bounds [num_pages][H_kv][2][D], the
+ * elementwise minimum, then the maximum, in the pool's 16-bit type (f16 for an
+ * e4m3 pool, whose stored values it holds exactly).  No counterpart in the
+ * reference.
+ *   slots int32 [num_tokens]: places of keys that were written, as pu_page_plan
+ *     makes them (negative: none).  Rows of one page stand together and in order.
+ * For each page that a slot names the bounds become those of the rows named, and of
+ * what they were where the page's row 0 is not among the rows.  NaN stays NaN.  A
+ * slot past the pool is reported (PU_ERR_INVALID_ARGUMENT, detail 309) and left
+ * out.  D 64 or 128.
+ */
+PU_API int pu_page_bounds(const void* k_pool, int kv_dtype, const int32_t* slots, void* bounds,
+                          int64_t num_pages, int64_t page_size, int64_t H_kv, int64_t D,
+                          int64_t num_tokens, void* stream);
+
+/*
+ * Choose pages for each K/V head by an upper bound of their scores.  No
+ * counterpart in the reference.  For the queries h of a K/V head a page scores
+ *   sum_h sum_d max(q_hd lo_d, q_hd hi_d)   (sums in 64 bits).
+ * Chosen are the sequence's first `first` and last `last` pages and the best of
+ * the others (the lowest index among equals), `count` in all, or all pages where
+ * there are no more than that.
+ *   pages int32 [B][H_kv][count]: pool pages in the sequence's order, -1 behind;
+ *   lens int32 [B][H_kv]: tokens in them.
+ * Entries outside the pool are not chosen, and reported (detail 310).  Queries and
+ * bounds must be finite for the choice to be that of the formula.
+ * q [B,H,1,D] and bounds each f16 or bf16; D 64 or 128; max_pages_per_seq <= 24576;
+ * first + last <= count.
+ */
+PU_API int pu_select_pages(const void* q, int q_dtype, const void* bounds, int bounds_dtype,
+                           const int32_t* page_table, int64_t max_pages_per_seq,
+                           int64_t num_pages, int64_t page_size, const int32_t* kv_lens,
+                           int32_t* pages, int32_t* lens, int64_t count, int64_t first,
+                           int64_t last, int64_t B, int64_t H, int64_t H_kv, int64_t D,
+                           void* stream);
+
+/*
  * Plan a batch's next tokens on the device: page table rows, slots and
  * positions from lengths alone.  No counterpart in the reference.
  *   page_table [B][max_pages_per_seq], kv_lens [B]: the state before;

@@ -60,6 +60,7 @@ struct Params {
   int max_pages;
   int num_pages;
   int page_shift;        // log2(page_size)
+  int lists = 1;         // page lists (and lengths) of a sequence: 1, or one for each K/V head
   // push mode (sequence-sharded decode over peer memory): the shard's record
   // for (b, h) goes to slot [epoch & 1][rank][bh] of every rank's exchange
   // buffer as 64-bit words {value bits, epoch} (one store each, so a reader
@@ -326,9 +327,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) split_kv_kernel(const Pa
   grid_dep_wait();
   grid_dep_launch_dependents();
 
+  // K/V head of this query head (GQA / MQA: `group` query heads share one)
+  const int h = bh % p.H;
+  const int h_kv = h / p.group;
+  const int list = kPaged && p.lists > 1 ? b * p.lists + h_kv : b;
   int len = p.n_local;
   if (p.lens != nullptr) {
-    long long g = (long long)p.lens[b] - p.kv_offset;
+    long long g = (long long)p.lens[list] - p.kv_offset;
     len = g < 0 ? 0 : (g > p.n_local ? p.n_local : (int)g);
   }
   const int t_begin = split * p.chunk;
@@ -343,9 +348,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) split_kv_kernel(const Pa
     for (int i = 0; i < 8; ++i) qf[i] *= p.scale_log2;
   }
 
-  // K/V head of this query head (GQA / MQA: `group` query heads share one)
-  const int h = bh % p.H;
-  const int h_kv = h / p.group;
   const int H_kv = p.H / p.group;
   const size_t kv_head = (size_t)b * H_kv + h_kv;
   const KVT* kb = static_cast<const KVT*>(p.k) + kv_head * p.n_local * D + sub * 8;
@@ -363,7 +365,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) split_kv_kernel(const Pa
   if constexpr (kPaged) {
     kb = static_cast<const KVT*>(p.k) + sub * 8;
     vb = static_cast<const KVT*>(p.v) + sub * 8;
-    table_b = p.page_table + (size_t)b * p.max_pages;
+    table_b = p.page_table + (size_t)list * p.max_pages;
     one_page = (1 << p.page_shift) >= TW;
     const int base0 = t_begin + warp * TW;
     if (one_page && base0 < t_end) pg_next = __ldg(table_b + (base0 >> p.page_shift));

@@ -139,11 +139,16 @@ struct Params {
   const void* q;               // [B, H, D]
   const int32_t* table;        // [B][max_pages]
   const int32_t* lens;         // [B]
+  const int32_t* skip;         // [B] tokens at the front, whole pages, that another pass takes and lens leaves out; or nullptr
   __nv_bfloat16* o;            // [B, H, D]
+  float* o32;                  // the output in fp32 instead, or nullptr
   float* lse;                  // [B, H] or nullptr
   int* count;                  // [CTAs] zero between calls
   float* rec;                  // [CTAs][2][NP][D + kHead]
-  int B, H, H_kv, group, slices;
+  // Lists of pages: one for each sequence (lists = 1), or one for each K/V head of it (lists = pool_heads).
+  // In the second form B counts lists, H is the query heads of one, and an item's inner index is its slice.
+  int B, H, lists, pool_heads, group, slices;
+  int inner;                   // items of a list
   int max_pages, num_pages, page_shift;
   int box;                     // rows of one TMA box: min(page size, 128)
   float scale_log2, o_scale;
@@ -208,7 +213,7 @@ struct Start {
 template <int kItemCost>
 __device__ __forceinline__ void find_start(const Params& p, int lane, Start* out) {
   constexpr int kHold = 8;
-  const int inner = p.H_kv * p.slices, cap = p.max_pages << p.page_shift;
+  const int inner = p.inner, cap = p.max_pages << p.page_shift;
   int len[kHold];
   // lengths of sequences base + 8 lane + k, in a lane's registers
   auto load = [&](int base) {
@@ -428,7 +433,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
   long long item0 = st.item0;
   Walk w0;
   w0.p = &p;
-  w0.inner = p.H_kv * p.slices;
+  w0.inner = p.inner;
   w0.b = st.b;
   w0.r = st.r;
   w0.t = st.t;
@@ -449,9 +454,9 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
       const int lane_tile = lane / boxes, lane_row = (lane & (boxes - 1)) << box_shift, per_page = 1 << p.page_shift;
       Walk wl = w0;                          // the first tile of the next batch
       auto look_up = [&]() -> int {
-        const int cnt = min(min(wl.left, wl.tiles - wl.t), batch);
+        const int cnt = min(min(wl.left, wl.tiles - wl.t), batch), skipped = cnt > 0 && p.skip != nullptr ? p.skip[wl.b] : 0;
         const int row = (wl.t + lane_tile) * BT + lane_row;
-        const int32_t* at = p.table + (size_t)wl.b * p.max_pages + (row >> p.page_shift);
+        const int32_t* at = p.table + (size_t)wl.b * p.max_pages + ((row + skipped) >> p.page_shift);
         int pg = -1;
         asm volatile("{\n .reg .pred q;\n setp.ne.b32 q, %2, 0;\n @q ld.global.b32 %0, [%1];\n}"
                      : "+r"(pg) : "l"(at), "r"((int)(lane_tile < cnt && row < wl.len)));
@@ -470,14 +475,14 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
         }
         if (w.seg != seg) {
           seg = w.seg;
-          head = w.r / p.slices;
+          head = p.lists > 1 ? w.b % p.lists : w.r / p.slices;
         }
         const int pg = __shfl_sync(0xffffffffu, entries, (j * boxes + lane) & 31), row0 = w.t * BT;
         const bool mine = lane < boxes && row0 + lane_row < w.len;
         const bool good = mine && (unsigned)pg < (unsigned)p.num_pages;
         if (mine && !good) record_device_error(PU_ERR_INVALID_ARGUMENT, kSiteDecodePage);
         const unsigned loaded = __ballot_sync(0xffffffffu, good);
-        const int outer = pg * p.H_kv + head, in = p.box < BT ? 0 : row0 & (per_page - 1);
+        const int outer = pg * p.pool_heads + head, in = p.box < BT ? 0 : row0 & (per_page - 1);
         // one answer for the warp: a lane that gave up alone would leave the others at the next vote
         if (turn > 0 && !__all_sync(0xffffffffu, mbar_wait(bEmpty + s, (turn - 1) & 1, abort_flag, kSiteDecodeTc))) break;
         // box i's coordinates to the issuing thread (all of them ahead of it: a
@@ -880,13 +885,17 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
       // ---- result or record ----
       const size_t bh0 = (size_t)b * p.H + (size_t)(p.slices == 1 ? r : r / p.slices) * p.group + slice * NP;
       if (whole) {
-        __nv_bfloat16* o = p.o + bh0 * D + row;
+        const size_t at = bh0 * D + row;
 #pragma unroll
         for (int h0 = 0; h0 < NP; h0 += 4) {
           if (h0 >= G) break;
 #pragma unroll
-          for (int h = h0; h < h0 + 4; ++h)
-            if (row < D && h < G) o[h * D] = __float2bfloat16_rn(oa[h]);
+          for (int h = h0; h < h0 + 4; ++h) {
+            if (row < D && h < G) {
+              if (p.o32 != nullptr) p.o32[at + h * D] = oa[h];
+              else p.o[at + h * D] = __float2bfloat16_rn(oa[h]);
+            }
+          }
         }
         if (p.lse != nullptr && row < G) p.lse[bh0 + row] = L == 0.f ? -INFINITY : (M + lg2(L)) * kLn2;
       } else {
@@ -963,7 +972,9 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
               }
             }
             const float inv = Ls == 0.f ? 0.f : 1.f / Ls;
-            if (lane * 4 < D) {
+            if (lane * 4 < D && p.o32 != nullptr) {
+              reinterpret_cast<float4*>(p.o32 + (bh0 + h) * D)[lane] = make_float4(o4[0] * inv, o4[1] * inv, o4[2] * inv, o4[3] * inv);
+            } else if (lane * 4 < D) {
               uint2 out;
               out.x = pack_bf16x2(o4[0] * inv, o4[1] * inv);
               out.y = pack_bf16x2(o4[2] * inv, o4[3] * inv);
@@ -982,7 +993,8 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
     // sequences that hold nothing
     for (int b = blockIdx.x; b < p.B; b += (int)gridDim.x) {
       if (w0.len_of(b) > 0) continue;
-      for (int i = row; i < p.H * D / 2; i += 128)
+      // an fp32 output of no weight is not read
+      for (int i = row; p.o32 == nullptr && i < p.H * D / 2; i += 128)
         reinterpret_cast<uint32_t*>(p.o + (size_t)b * p.H * D)[i] = 0u;
       if (p.lse != nullptr)
         for (int i = row; i < p.H; i += 128) p.lse[(size_t)b * p.H + i] = -INFINITY;
@@ -1017,18 +1029,9 @@ int launch_as(const CUtensorMap& tk, const CUtensorMap& tv, const Params& prm, c
                     "paged grouped-head decode launch");
 }
 
-inline int launch(const Params& prm, const void* k, const void* v, int q_dtype, int kv_dtype, int D, cudaStream_t st) {
-  const bool f8 = kv_dtype == PU_DTYPE_FP8_E4M3;
-  const uint64_t rows = 1ull << prm.page_shift, outer = (uint64_t)prm.num_pages * prm.H_kv;
-  CUtensorMap tk, tv;
-  int rc = f8 ? make_tmap_u8_3d(&tk, k, D, rows, outer, 128, prm.box, true)
-              : make_tmap_bf16_3d(&tk, k, D, rows, outer, 64, prm.box, true);
-  if (!rc)
-    rc = f8 ? make_tmap_u8_3d(&tv, v, D, rows, outer, 128, prm.box, true)
-            : make_tmap_bf16_3d(&tv, v, D, rows, outer, 64, prm.box, true);
-  if (rc) return rc;
+inline int launch_with(const CUtensorMap& tk, const CUtensorMap& tv, const Params& prm, int q_dtype, int kv_dtype, int D, cudaStream_t st) {
   const bool h = q_dtype == PU_DTYPE_F16;
-  if (f8)
+  if (kv_dtype == PU_DTYPE_FP8_E4M3)
     return h ? launch_as<__half, __nv_fp8_e4m3, 128>(tk, tv, prm, st)
              : launch_as<__nv_bfloat16, __nv_fp8_e4m3, 128>(tk, tv, prm, st);
   if (D == 128)
@@ -1036,25 +1039,37 @@ inline int launch(const Params& prm, const void* k, const void* v, int q_dtype, 
   return h ? launch_as<__half, __half, 64>(tk, tv, prm, st) : launch_as<__nv_bfloat16, __nv_bfloat16, 64>(tk, tv, prm, st);
 }
 
+// Tensor maps of a pool of pages: boxes of `box` tokens, one swizzle block wide.
+inline int make_maps(CUtensorMap* tk, CUtensorMap* tv, const void* k, const void* v, int kv_dtype, long long num_pages, long long H_kv,
+                     int page_shift, int box, int D) {
+  const uint64_t rows = 1ull << page_shift, outer = (uint64_t)num_pages * H_kv;
+  if (kv_dtype == PU_DTYPE_FP8_E4M3) {
+    const int rc = make_tmap_u8_3d(tk, k, D, rows, outer, 128, box, true);
+    return rc ? rc : make_tmap_u8_3d(tv, v, D, rows, outer, 128, box, true);
+  }
+  const int rc = make_tmap_bf16_3d(tk, k, D, rows, outer, 64, box, true);
+  return rc ? rc : make_tmap_bf16_3d(tv, v, D, rows, outer, 64, box, true);
+}
+
+inline int launch(const Params& prm, const void* k, const void* v, int q_dtype, int kv_dtype, int D, cudaStream_t st) {
+  CUtensorMap tk, tv;
+  const int rc = make_maps(&tk, &tv, k, v, kv_dtype, prm.num_pages, prm.pool_heads, prm.page_shift, prm.box, D);
+  return rc ? rc : launch_with(tk, tv, prm, q_dtype, kv_dtype, D, st);
+}
+
 }  // namespace ptc
 }  // namespace decode
 }  // namespace pu
 
-extern "C" {
+namespace pu {
+namespace decode {
 
-size_t pu_decode_paged_gqa_workspace_size(int64_t B, int64_t H, int64_t H_kv, int64_t max_pages_per_seq,
-                                          int64_t page_size, int64_t D) {
-  using namespace pu::decode;
-  if (B <= 0 || H <= 0 || H_kv <= 0 || H % H_kv || max_pages_per_seq <= 0 || page_size <= 0 || D <= 0) return 0;
-  if (B > kMaxBH / H) return ptc::workspace_bytes(D);      // the tensor-core kernel's alone
-  return std::max(ptc::workspace_bytes(D), pu_decode_paged_workspace_size(B, H, max_pages_per_seq, page_size, D));
-}
-
-int pu_decode_paged_gqa(const void* q, int q_dtype, const void* k_pool, const void* v_pool, int kv_dtype,
-                        const int32_t* page_table, int64_t max_pages_per_seq, int64_t num_pages, int64_t page_size,
-                        const int32_t* kv_lens, void* o, float* lse, void* workspace, size_t workspace_bytes, int64_t B,
-                        int64_t H, int64_t H_kv, int64_t D, float sm_scale, float k_scale, float v_scale, void* stream) {
-  using namespace pu::decode;
+// Both forms of the paged grouped decode: one page list a sequence, or one for each K/V head (`by_head`:
+// page_table [B][H_kv][max_pages], kv_lens [B][H_kv]).
+inline int paged_gqa(const void* q, int q_dtype, const void* k_pool, const void* v_pool, int kv_dtype, const int32_t* page_table,
+                     int64_t max_pages_per_seq, int64_t num_pages, int64_t page_size, const int32_t* kv_lens, void* o, float* lse,
+                     void* workspace, size_t workspace_bytes, int64_t B, int64_t H, int64_t H_kv, int64_t D, float sm_scale, float k_scale,
+                     float v_scale, bool by_head, void* stream) {
   int shift = 0;
   int rc = pu::paged::check_pages(page_table, max_pages_per_seq, num_pages, page_size, &shift);
   if (rc) return rc;
@@ -1072,8 +1087,9 @@ int pu_decode_paged_gqa(const void* q, int q_dtype, const void* k_pool, const vo
   const bool tensor = ptc::eligible(H, H_kv, D, q_dtype, kv_dtype);
   // the query-head kernel has a counter and a grid row for each (b, h), the
   // tensor-core kernel a counter for each CTA
-  if (H > kMaxBH || (B > kMaxBH / H && (!tensor || B > ptc::kMaxB)))
-    return pu::set_error(PU_ERR_UNSUPPORTED, "paged decode of %lld sequences with %lld heads (B * H up to %d, or on the tensor core B up to %d)",
+  const long long lists = by_head ? H_kv : 1;
+  if (H > kMaxBH || (B > kMaxBH / H && (!tensor || B > ptc::kMaxB / lists)))
+    return pu::set_error(PU_ERR_UNSUPPORTED, "paged decode of %lld sequences with %lld heads (B * H up to %d, or on the tensor core %d page lists)",
                          (long long)B, (long long)H, kMaxBH, ptc::kMaxB);
   Plan pl{};
   if (!tensor) pl = make_plan(B * H, n_cap, D, pu::sm_count(), true, page_size);
@@ -1091,11 +1107,13 @@ int pu_decode_paged_gqa(const void* q, int q_dtype, const void* k_pool, const vo
     prm.lse = lse;
     prm.count = static_cast<int*>(workspace);
     prm.rec = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCountBytes);
-    prm.B = (int)B;
-    prm.H = (int)H;
-    prm.H_kv = (int)H_kv;
+    prm.B = (int)(B * lists);
+    prm.H = (int)(H / lists);
+    prm.lists = (int)lists;
+    prm.pool_heads = (int)H_kv;
     prm.group = (int)(H / H_kv);
     prm.slices = (prm.group + ptc::NP - 1) / ptc::NP;
+    prm.inner = (int)(H_kv / lists) * prm.slices;
     prm.max_pages = (int)max_pages_per_seq;
     prm.num_pages = (int)num_pages;
     prm.page_shift = shift;
@@ -1115,6 +1133,7 @@ int pu_decode_paged_gqa(const void* q, int q_dtype, const void* k_pool, const vo
   prm.n_local = (int)n_cap;
   prm.H = (int)H;
   prm.group = (int)(H / H_kv);
+  prm.lists = (int)lists;
   prm.o_scale = v_scale;
   prm.splits = pl.splits;
   prm.chunk = pl.chunk;
@@ -1128,6 +1147,35 @@ int pu_decode_paged_gqa(const void* q, int q_dtype, const void* k_pool, const vo
   prm.num_pages = (int)num_pages;
   prm.page_shift = shift;
   return launch<true, true>(prm, q_dtype, kv_dtype, (int)D, (int)(B * H), st);
+}
+
+}  // namespace decode
+}  // namespace pu
+
+extern "C" {
+
+size_t pu_decode_paged_gqa_workspace_size(int64_t B, int64_t H, int64_t H_kv, int64_t max_pages_per_seq,
+                                          int64_t page_size, int64_t D) {
+  using namespace pu::decode;
+  if (B <= 0 || H <= 0 || H_kv <= 0 || H % H_kv || max_pages_per_seq <= 0 || page_size <= 0 || D <= 0) return 0;
+  if (B > kMaxBH / H) return ptc::workspace_bytes(D);      // the tensor-core kernel's alone
+  return std::max(ptc::workspace_bytes(D), pu_decode_paged_workspace_size(B, H, max_pages_per_seq, page_size, D));
+}
+
+int pu_decode_paged_gqa(const void* q, int q_dtype, const void* k_pool, const void* v_pool, int kv_dtype,
+                        const int32_t* page_table, int64_t max_pages_per_seq, int64_t num_pages, int64_t page_size,
+                        const int32_t* kv_lens, void* o, float* lse, void* workspace, size_t workspace_bytes, int64_t B,
+                        int64_t H, int64_t H_kv, int64_t D, float sm_scale, float k_scale, float v_scale, void* stream) {
+  return pu::decode::paged_gqa(q, q_dtype, k_pool, v_pool, kv_dtype, page_table, max_pages_per_seq, num_pages, page_size, kv_lens, o, lse,
+                               workspace, workspace_bytes, B, H, H_kv, D, sm_scale, k_scale, v_scale, false, stream);
+}
+
+int pu_decode_paged_heads(const void* q, int q_dtype, const void* k_pool, const void* v_pool, int kv_dtype,
+                          const int32_t* page_table, int64_t max_pages_per_head, int64_t num_pages, int64_t page_size,
+                          const int32_t* kv_lens, void* o, float* lse, void* workspace, size_t workspace_bytes, int64_t B,
+                          int64_t H, int64_t H_kv, int64_t D, float sm_scale, float k_scale, float v_scale, void* stream) {
+  return pu::decode::paged_gqa(q, q_dtype, k_pool, v_pool, kv_dtype, page_table, max_pages_per_head, num_pages, page_size, kv_lens, o, lse,
+                               workspace, workspace_bytes, B, H, H_kv, D, sm_scale, k_scale, v_scale, true, stream);
 }
 
 }  // extern "C"

@@ -6,7 +6,9 @@
 #include "paged.cuh"
 #include "gqa_tc.cuh"
 #include "paged_tc.cuh"
+#include "paged_shared.cuh"
 #include "page_plan.cuh"
+#include "page_select.cuh"
 #include "rope.cuh"
 #include "peer.cuh"
 #include "outproj.cuh"

@@ -389,6 +389,11 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// The same barrier in two steps: nothing is ordered by it but that every CTA of
+// the cluster has begun.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
+
 // Arrive on an mbarrier given by its shared::cluster address (possibly the
 // peer CTA's).
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar_cluster_addr) {

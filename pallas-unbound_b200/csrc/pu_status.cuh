@@ -44,6 +44,9 @@ enum WaitSite : int {
   kSiteAppendSlot = 306,
   kSitePagePlan = 307,
   kSiteFreePages = 308,
+  kSitePageBounds = 309,
+  kSiteSelectPage = 310,
+  kSiteDecodeShared = 311,
   kSiteOutProj = 401,
   kSiteSelfTest = 901,
 };

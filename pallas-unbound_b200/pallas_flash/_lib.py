@@ -97,6 +97,19 @@ SIGNATURES = {
     "pu_decode_paged_gqa": (_int, [_c_void_p, _int, _c_void_p, _c_void_p, _int, _c_void_p, _i64,
                                    _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _size_t,
                                    _i64, _i64, _i64, _i64, _float, _float, _float, _c_void_p]),
+    "pu_decode_paged_heads": (_int, [_c_void_p, _int, _c_void_p, _c_void_p, _int, _c_void_p, _i64,
+                                     _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _size_t,
+                                     _i64, _i64, _i64, _i64, _float, _float, _float, _c_void_p]),
+    "pu_decode_paged_shared_workspace_size": (_size_t, [_i64, _i64, _i64, _i64, _i64]),
+    "pu_decode_paged_shared": (_int, [_c_void_p, _int, _c_void_p, _c_void_p, _int, _c_void_p, _i64,
+                                      _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p,
+                                      _c_void_p, _c_void_p, _size_t, _i64, _i64, _i64, _i64, _float,
+                                      _float, _float, _c_void_p]),
+    "pu_page_bounds": (_int, [_c_void_p, _int, _c_void_p, _c_void_p, _i64, _i64, _i64, _i64, _i64,
+                              _c_void_p]),
+    "pu_select_pages": (_int, [_c_void_p, _int, _c_void_p, _int, _c_void_p, _i64, _i64, _i64, _c_void_p,
+                               _c_void_p, _c_void_p, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                               _c_void_p]),
     "pu_page_plan": (_int, [_c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
                             _c_void_p, _i64, _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p,
                             _c_void_p, _c_void_p, _i64, _i64, _c_void_p]),

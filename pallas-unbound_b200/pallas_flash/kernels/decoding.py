@@ -38,7 +38,10 @@ Keyword-only additions:
   page_table  int32 [B, max_pages_per_seq]: the caches are then page pools
               [num_pages, H_kv, page_size, D] (see kernels/paged.py; H_kv
               divides H, fp16, bf16 or fp8 with k_scale / v_scale) and
-              kv_lens is required; single GPU only.
+              kv_lens is required; single GPU only.  [B, H_kv, pages] with
+              kv_lens [B, H_kv] are lists of each K/V head (select_pages).
+  shared_lens, shared_groups  with a page_table: sequences that hold the same
+              first pages, which are read once for all (see paged_decode)
 """
 from __future__ import annotations
 
@@ -147,7 +150,9 @@ def pallas_flash_decoding(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
                           sm_scale: Optional[float] = None, return_lse: bool = False,
                           group=None, transport: str = "nccl", sharding: str = "contiguous",
                           page_table: Optional[torch.Tensor] = None,
-                          k_scale: float = 1.0, v_scale: float = 1.0):
+                          k_scale: float = 1.0, v_scale: float = 1.0,
+                          shared_lens: Optional[torch.Tensor] = None,
+                          shared_groups: Optional[torch.Tensor] = None):
     """One decode step of attention for a query token per (b, h)."""
     if page_table is not None:
         global _paged_decode
@@ -156,7 +161,10 @@ def pallas_flash_decoding(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
         if group is not None or kv_lens is None:
             raise ValueError("a paged cache needs kv_lens and runs on one GPU (group=None)")
         return _paged_decode(q, k_cache, v_cache, page_table, kv_lens, sm_scale=sm_scale,
-                            return_lse=return_lse, k_scale=k_scale, v_scale=v_scale)
+                             return_lse=return_lse, k_scale=k_scale, v_scale=v_scale,
+                             shared_lens=shared_lens, shared_groups=shared_groups)
+    if shared_lens is not None or shared_groups is not None:
+        raise ValueError("a shared prefix needs a paged cache (page_table)")
     if q.dim() != 4 or q.shape[2] != 1:
         raise ValueError("q must be [B, H, 1, D]")
     if k_cache.shape != v_cache.shape or k_cache.shape[0] != q.shape[0] \

@@ -23,6 +23,15 @@ the next tokens from lengths alone, `qk_norm_rope_append`
 (pu_qk_norm_rope_append) norms and rotates q and k and writes keys and values
 to their slots, and `paged_decode` attends; the three calls can be captured
 into a CUDA graph and replayed.
+
+Long contexts are served with less reading:
+
+  - `page_bounds` (pu_page_bounds) keeps the elementwise minimum and maximum of
+    each page's keys, `select_pages` (pu_select_pages) lists for each K/V head
+    the pages whose bound of the scores is highest, and `paged_decode` over such
+    lists (pu_decode_paged_heads) reads those pages only.
+  - `paged_decode` with `shared_lens` (pu_decode_paged_shared) reads pages that
+    sequences have in common once for all of them.
 """
 from __future__ import annotations
 
@@ -37,8 +46,8 @@ from .. import _lib
 from ..ops.rotary import _DT as _DT_ROPE, _NONE, _check_angles, _check_weight, _pack, _refuse_tangents, _rows
 from .decoding import _DT, _DT_KV, DecodeWorkspace
 
-__all__ = ["PageAllocator", "PagedKVCache", "DevicePagedKVCache", "AppendPlan", "paged_decode", "kv_append",
-           "plan_append", "qk_norm_rope_append"]
+__all__ = ["PageAllocator", "PagedKVCache", "DevicePagedKVCache", "AppendPlan", "PageSelection", "paged_decode",
+           "kv_append", "plan_append", "qk_norm_rope_append", "empty_bounds", "page_bounds", "select_pages"]
 
 
 def _check_pool(k_pool: torch.Tensor, v_pool: torch.Tensor, page_table: torch.Tensor,
@@ -47,10 +56,16 @@ def _check_pool(k_pool: torch.Tensor, v_pool: torch.Tensor, page_table: torch.Te
         raise ValueError("k_pool and v_pool must both be [num_pages, H, page_size, D]")
     if k_pool.dtype != v_pool.dtype or k_pool.dtype not in kinds:
         raise ValueError("pools must share one dtype, fp16 or bf16" + (" or fp8 (e4m3)" if kinds is _DT_KV else ""))
-    if page_table.dtype != torch.int32 or page_table.dim() != 2:
-        raise ValueError("page_table must be int32 [B, max_pages_per_seq]")
-    if kv_lens.dtype != torch.int32 or kv_lens.numel() != page_table.shape[0]:
-        raise ValueError("kv_lens must be int32 [B]")
+    if page_table.dtype == torch.int32 and page_table.dim() == 3 and kinds is _DT_KV:
+        if page_table.shape[1] != k_pool.shape[1]:
+            raise ValueError(f"page lists of each K/V head must be int32 [B, {k_pool.shape[1]}, pages]")
+        if kv_lens.dtype != torch.int32 or kv_lens.shape != page_table.shape[:2]:
+            raise ValueError("kv_lens of page lists must be int32 [B, H_kv]")
+    else:
+        if page_table.dtype != torch.int32 or page_table.dim() != 2:
+            raise ValueError("page_table must be int32 [B, max_pages_per_seq]")
+        if kv_lens.dtype != torch.int32 or kv_lens.numel() != page_table.shape[0]:
+            raise ValueError("kv_lens must be int32 [B]")
     dev = k_pool.device
     if not (k_pool.is_cuda and v_pool.device == dev and page_table.device == dev and kv_lens.device == dev
             and k_pool.is_contiguous() and v_pool.is_contiguous() and page_table.is_contiguous()
@@ -68,21 +83,46 @@ def _cta_counters(device: int) -> int:
     return 4 * torch.cuda.get_device_properties(device).multi_processor_count
 
 
+@functools.lru_cache(maxsize=256)
+def _shared_bytes(device: int, B: int, H: int, H_kv: int, groups: int, D: int) -> int:
+    return int(_lib.lib().pu_decode_paged_shared_workspace_size(B, H, H_kv, groups, D))
+
+
 def paged_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
                  page_table: torch.Tensor, kv_lens: torch.Tensor, *,
                  sm_scale: Optional[float] = None, return_lse: bool = False,
-                 k_scale: float = 1.0, v_scale: float = 1.0):
+                 k_scale: float = 1.0, v_scale: float = 1.0,
+                 shared_lens: Optional[torch.Tensor] = None, shared_groups: Optional[torch.Tensor] = None):
     """One decode step over a paged cache -> o bf16 [B,H,1,D] (and lse fp32 [B,H]).
 
     q [B,H,1,D] fp16/bf16; the pools hold H_kv heads, H a multiple of H_kv,
     in fp16, bf16 or fp8 (e4m3; keys and values are the stored values times
-    k_scale and v_scale).  A sequence of length 0 gives o = 0, lse = -inf."""
+    k_scale and v_scale).  A sequence of length 0 gives o = 0, lse = -inf.
+
+    page_table [B,H_kv,pages] with kv_lens [B,H_kv] are lists of their own for
+    each K/V head, as `select_pages` makes them: the head's queries attend the
+    first kv_lens tokens of its list and read no other page.
+
+    shared_lens int32 [n] (n up to 64) says that sequences hold the same pages:
+    those of group i, sequences shared_groups[i] <= b < shared_groups[i + 1] (int32
+    [n + 1]; without it one group is the whole batch), have the same first
+    shared_lens[i] tokens, which are then read once for the group, through the
+    table row of one of its sequences.  Only whole pages are shared.  A sequence
+    that holds fewer tokens than that attends those it holds; a group in which
+    none holds as many shares nothing.  The result is that of the call without
+    it, up to the order of sums, and where q and the pools have different 16-bit
+    types, or e4m3 pools heads of 64, it is that call."""
     _check_pool(k_pool, v_pool, page_table, kv_lens, _DT_KV)
     P, H_kv, page_size, D = k_pool.shape
-    B, max_pages = page_table.shape
+    by_head = page_table.dim() == 3
+    B, max_pages = page_table.shape[0], page_table.shape[-1]
     H = q.shape[1] if q.dim() == 4 else 0
     if q.shape != (B, H, 1, D) or H == 0 or H_kv == 0 or H % H_kv or q.dtype not in _DT or q.device != k_pool.device:
         raise ValueError(f"q must be fp16/bf16 CUDA [{B}, multiple of {H_kv}, 1, {D}] on {k_pool.device}")
+    if shared_lens is not None:
+        _check_shared(shared_lens, shared_groups, by_head, q.device)
+    elif shared_groups is not None:
+        raise ValueError("shared_groups without shared_lens")
     q = q.contiguous()
     if q.data_ptr() % 16:
         q = q.clone()
@@ -94,7 +134,17 @@ def paged_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
         lse = torch.empty(B, H, dtype=torch.float32, device=q.device)
         if B == 0:
             return (o, lse) if return_lse else o
-        if H == H_kv and k_pool.dtype in _DT and k_scale == 1.0 and v_scale == 1.0:
+        if shared_lens is not None and (k_pool.dtype == q.dtype or (D == 128 and k_pool.dtype not in _DT)):
+            groups = shared_lens.numel()
+            ws = DecodeWorkspace.get(q.device, _shared_bytes(q.device.index, B, H, H_kv, groups, D),
+                                     _cta_counters(q.device.index))
+            _lib.check(lib.pu_decode_paged_shared(
+                q.data_ptr(), _DT[q.dtype], k_pool.data_ptr(), v_pool.data_ptr(), _DT_KV[k_pool.dtype],
+                page_table.data_ptr(), max_pages, P, page_size, kv_lens.data_ptr(), shared_lens.data_ptr(),
+                None if shared_groups is None else shared_groups.data_ptr(), groups, o.data_ptr(), lse.data_ptr(),
+                ws.data_ptr(), ws.numel(), B, H, H_kv, D, float(sm_scale), float(k_scale), float(v_scale),
+                stream), "pu_decode_paged_shared")
+        elif not by_head and H == H_kv and k_pool.dtype in _DT and k_scale == 1.0 and v_scale == 1.0:
             need = int(lib.pu_decode_paged_workspace_size(B, H, max_pages, page_size, D))
             ws = DecodeWorkspace.get(q.device, need, 4 * B * H)
             _lib.check(lib.pu_decode_paged(q.data_ptr(), _DT[q.dtype], k_pool.data_ptr(),
@@ -106,13 +156,123 @@ def paged_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
             # a counter for each CTA (one an SM), or in the query-head kernel for each head
             ws = DecodeWorkspace.get(q.device, _gqa_bytes(q.device.index, B, H, H_kv, max_pages, page_size, D),
                                      max(4 * B * H, _cta_counters(q.device.index)))
-            _lib.check(lib.pu_decode_paged_gqa(q.data_ptr(), _DT[q.dtype], k_pool.data_ptr(),
-                                               v_pool.data_ptr(), _DT_KV[k_pool.dtype],
-                                               page_table.data_ptr(), max_pages, P, page_size,
-                                               kv_lens.data_ptr(), o.data_ptr(), lse.data_ptr(),
-                                               ws.data_ptr(), ws.numel(), B, H, H_kv, D, float(sm_scale),
-                                               float(k_scale), float(v_scale), stream), "pu_decode_paged_gqa")
+            call = lib.pu_decode_paged_heads if by_head else lib.pu_decode_paged_gqa
+            _lib.check(call(q.data_ptr(), _DT[q.dtype], k_pool.data_ptr(), v_pool.data_ptr(), _DT_KV[k_pool.dtype],
+                            page_table.data_ptr(), max_pages, P, page_size, kv_lens.data_ptr(), o.data_ptr(),
+                            lse.data_ptr(), ws.data_ptr(), ws.numel(), B, H, H_kv, D, float(sm_scale),
+                            float(k_scale), float(v_scale), stream),
+                       "pu_decode_paged_heads" if by_head else "pu_decode_paged_gqa")
     return (o, lse) if return_lse else o
+
+
+def _check_shared(shared_lens: torch.Tensor, shared_groups: Optional[torch.Tensor], by_head: bool, dev: torch.device):
+    if by_head:
+        raise ValueError("page lists of each K/V head have no shared prefix")
+    n = shared_lens.numel()
+    if shared_lens.dtype != torch.int32 or shared_lens.dim() != 1 or not 1 <= n <= 64:
+        raise ValueError("shared_lens must be int32 [n], n from 1 to 64")
+    if shared_groups is None:
+        if n != 1:
+            raise ValueError("more than one shared prefix needs shared_groups")
+    elif shared_groups.dtype != torch.int32 or shared_groups.shape != (n + 1,):
+        raise ValueError(f"shared_groups must be int32 [{n + 1}]")
+    if shared_lens.device != dev or not shared_lens.is_contiguous() or \
+            (shared_groups is not None and (shared_groups.device != dev or not shared_groups.is_contiguous())):
+        raise ValueError(f"shared_lens and shared_groups must be contiguous on {dev}")
+
+
+class PageSelection(NamedTuple):
+    """Pages chosen for each K/V head (select_pages), as `paged_decode` takes them."""
+    pages: torch.Tensor        # int32 [B, H_kv, count]  pool pages in the sequence's order; -1 behind the last
+    lens: torch.Tensor         # int32 [B, H_kv]  tokens in them
+
+
+def empty_bounds(k_pool: torch.Tensor) -> torch.Tensor:
+    """Room for the bounds of a pool's pages: [num_pages, H_kv, 2, D] in the pool's
+    16-bit type, fp16 for an fp8 pool (which holds every e4m3 value).  [..., 0, :] is
+    the minimum and [..., 1, :] the maximum of a page's keys as stored."""
+    P, H_kv, _, D = k_pool.shape
+    return torch.zeros((P, H_kv, 2, D), dtype=k_pool.dtype if k_pool.dtype in _DT else torch.float16,
+                       device=k_pool.device)
+
+
+def _check_bounds(bounds: torch.Tensor):
+    if bounds.dim() != 4 or bounds.shape[2] != 2 or bounds.dtype not in _DT:
+        raise ValueError("bounds must be fp16/bf16 [num_pages, H_kv, 2, D]")
+    if not bounds.is_cuda or not bounds.is_contiguous():
+        raise ValueError("bounds must be a contiguous CUDA tensor")
+    if bounds.shape[3] not in (64, 128):
+        raise ValueError(f"page bounds of head size {bounds.shape[3]} (supported: 64, 128)")
+
+
+def page_bounds(k_pool: torch.Tensor, slots: torch.Tensor, bounds: torch.Tensor) -> None:
+    """Bring the pages' bounds up to date with keys that were written to `slots`.
+
+    slots int32 [T] as `plan_append` makes them (negative: no key): the rows of a
+    page stand together and in order, and a page begins with its row 0.  For each
+    page that a slot names, `bounds` (empty_bounds) becomes the elementwise minimum
+    and maximum of the keys in these rows, and of what it was where the page's row 0
+    is not among them.  A NaN makes its element's bounds NaN.  A slot past the pool is
+    reported (device_status detail 309) and left out."""
+    _check_bounds(bounds)
+    P, H_kv, _, D = bounds.shape
+    if k_pool.dim() != 4 or (k_pool.shape[0], k_pool.shape[1], k_pool.shape[3]) != (P, H_kv, D) or k_pool.dtype not in _DT_KV:
+        raise ValueError(f"k_pool must be fp16, bf16 or fp8 (e4m3) [{P}, {H_kv}, page_size, {D}]")
+    if bounds.dtype != (k_pool.dtype if k_pool.dtype in _DT else torch.float16):
+        raise ValueError("bounds must have the pool's 16-bit dtype, fp16 for an fp8 pool")
+    if slots.dtype != torch.int32 or slots.dim() != 1 or not slots.is_contiguous():
+        raise ValueError("slots must be a contiguous int32 [T]")
+    if k_pool.device != bounds.device or slots.device != bounds.device or not k_pool.is_contiguous():
+        raise ValueError("pool, slots and bounds must be contiguous CUDA tensors on one device")
+    if (k_pool.requires_grad or bounds.requires_grad) and torch.is_grad_enabled():
+        raise ValueError("page_bounds writes a cache's bounds and has no gradient")
+    with _lib.on_device(bounds.device) as stream:
+        _lib.check(_lib.lib().pu_page_bounds(k_pool.data_ptr(), _DT_KV[k_pool.dtype], slots.data_ptr(), bounds.data_ptr(),
+                                             P, k_pool.shape[2], H_kv, D, slots.numel(), stream), "pu_page_bounds")
+
+
+def select_pages(q: torch.Tensor, bounds: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor, count: int, *,
+                 page_size: int, first: int = 1, last: int = 1) -> PageSelection:
+    """The pages that each K/V head's queries attend, `count` of them at most.
+
+    A page's score is sum over the head's queries and their elements of
+    max(q_d lo_d, q_d hi_d): no key of the page scores higher, summed over the
+    queries.  The first `first` and the last `last` pages of a sequence are always
+    chosen, then those with the highest scores (the lowest index among equals), all
+    in the sequence's order; a sequence of no more than `count` pages keeps all of
+    them.  Scores are summed in 64 bits.  Table entries outside the pool are never
+    chosen and reported (device_status detail 310); queries and bounds are finite.
+
+    q [B,H,1,D] fp16/bf16, bounds of `page_bounds`, page_table int32
+    [B,max_pages_per_seq] (up to 24576), kv_lens int32 [B].  The scores' scale and
+    the scale of an fp8 pool change nothing.  The result goes into
+    `paged_decode(q, k_pool, v_pool, chosen.pages, chosen.lens)`."""
+    _check_bounds(bounds)
+    P, H_kv, _, D = bounds.shape
+    dev = bounds.device
+    if page_table.dtype != torch.int32 or page_table.dim() != 2:
+        raise ValueError("page_table must be int32 [B, max_pages_per_seq]")
+    B, max_pages = page_table.shape
+    if kv_lens.dtype != torch.int32 or kv_lens.shape != (B,):
+        raise ValueError(f"kv_lens must be int32 [{B}]")
+    H = q.shape[1] if q.dim() == 4 else 0
+    if q.shape != (B, H, 1, D) or H == 0 or H_kv == 0 or H % H_kv or q.dtype not in _DT or q.device != dev:
+        raise ValueError(f"q must be fp16/bf16 CUDA [{B}, multiple of {H_kv}, 1, {D}] on {dev}")
+    if page_table.device != dev or kv_lens.device != dev or not page_table.is_contiguous() or not kv_lens.is_contiguous():
+        raise ValueError("page table and lengths must be contiguous and on the bounds' device")
+    count, first, last = int(count), int(first), int(last)
+    if count < 1 or first < 0 or last < 0 or first + last > count:
+        raise ValueError(f"{first} first and {last} last of {count} pages")
+    q = q.contiguous()
+    with _lib.on_device(dev) as stream:
+        pages = torch.empty(B, H_kv, count, dtype=torch.int32, device=dev)
+        lens = torch.empty(B, H_kv, dtype=torch.int32, device=dev)
+        if B:
+            _lib.check(_lib.lib().pu_select_pages(
+                q.data_ptr(), _DT[q.dtype], bounds.data_ptr(), _DT[bounds.dtype], page_table.data_ptr(), max_pages, P,
+                int(page_size), kv_lens.data_ptr(), pages.data_ptr(), lens.data_ptr(), count, first, last, B, H, H_kv, D,
+                stream), "pu_select_pages")
+    return PageSelection(pages, lens)
 
 
 def kv_append(k_new: torch.Tensor, v_new: torch.Tensor, k_pool: torch.Tensor,
@@ -396,6 +556,14 @@ class DevicePagedKVCache:
     Nothing here reads from the device, so a step can be captured into a CUDA
     graph (new_lens, release, q, k and v in fixed buffers) and replayed.
 
+    With `bounds=True` the cache keeps its pages' bounds (every `append` brings them
+    up to date), and a step over a long context reads the pages that matter:
+
+    o = cache.decode(q, pages=cache.select(q, 64))
+
+    Sequences may begin with the pages of another one (`share`); `decode` reads them
+    once where `shared_lens` says so.
+
     This is one layer's cache.  A model of several layers plans once a step
     (`plan_append`) and gives every layer the same slots, positions, table and
     lengths with pools of its own (`qk_norm_rope_append`, `paged_decode`): L of these
@@ -405,7 +573,7 @@ class DevicePagedKVCache:
 
     def __init__(self, batch: int, kv_heads: int, head_dim: int, *, num_pages: int, page_size: int = 64,
                  max_seq_len: int, dtype=torch.bfloat16, k_scale: float = 1.0, v_scale: float = 1.0,
-                 device=None):
+                 bounds: bool = False, device=None):
         if dtype not in _DT_KV:
             raise ValueError("cache dtype must be fp16, bf16 or fp8 (e4m3)")
         if page_size < 16 or page_size > 4096 or page_size & (page_size - 1):
@@ -416,6 +584,7 @@ class DevicePagedKVCache:
         self.page_size, self.k_scale, self.v_scale = int(page_size), float(k_scale), float(v_scale)
         self.k_pool = torch.zeros((num_pages, kv_heads, page_size, head_dim), dtype=dtype, device=device)
         self.v_pool = torch.zeros_like(self.k_pool)
+        self.bounds = empty_bounds(self.k_pool) if bounds else None
         self.page_table = torch.full((batch, max_pages), -1, dtype=torch.int32, device=device)
         self.kv_lens = torch.zeros(batch, dtype=torch.int32, device=device)
         self.free_ring = torch.arange(num_pages, dtype=torch.int32, device=device)
@@ -431,12 +600,48 @@ class DevicePagedKVCache:
                positions: Optional[torch.Tensor] = None, **norm) -> torch.Tensor:
         """Norm and rotate the plan's tokens and write their keys and values
         (qk_norm_rope_append); positions [axes,T] replace the plan's where they have axes."""
-        return qk_norm_rope_append(q, k, v, inv_freq, plan.positions if positions is None else positions, plan.slots,
-                                   self.k_pool, self.v_pool, k_scale=self.k_scale, v_scale=self.v_scale, **norm)
+        q = qk_norm_rope_append(q, k, v, inv_freq, plan.positions if positions is None else positions, plan.slots,
+                                self.k_pool, self.v_pool, k_scale=self.k_scale, v_scale=self.v_scale, **norm)
+        if self.bounds is not None:
+            page_bounds(self.k_pool, plan.slots, self.bounds)
+        return q
 
-    def decode(self, q: torch.Tensor, *, sm_scale: Optional[float] = None, return_lse: bool = False):
-        """Attention of one token a sequence, q [B,H,1,D] or the appended [B,H,D], over all held tokens."""
+    def share(self, source: int, sequences: torch.Tensor, tokens: int) -> None:
+        """Let empty `sequences` (int64, on the cache's device) begin with the first `tokens`
+        of sequence `source`: whole pages of it, which they read and never write.  The pages stay
+        `source`'s: it is released after every sequence that shares them, and a sequence
+        gives them up with `unshare` before it is released."""
+        n = int(tokens) // self.page_size
+        if tokens % self.page_size or not 0 <= n <= self.page_table.shape[1]:
+            raise ValueError(f"{tokens} tokens are not whole pages of {self.page_size} that a table row holds")
+        self.page_table[sequences, :n] = self.page_table[source, :n]
+        self.kv_lens[sequences] = int(tokens)
+
+    def unshare(self, sequences: torch.Tensor, tokens: int) -> None:
+        """Take the first `tokens`, shared with another sequence, out of `sequences`: what is left of
+        them are their own pages, which can be released."""
+        n = int(tokens) // self.page_size
+        if tokens % self.page_size or not 0 <= n <= self.page_table.shape[1]:
+            raise ValueError(f"{tokens} tokens are not whole pages of {self.page_size} that a table row holds")
+        rows = self.page_table[sequences]
+        self.page_table[sequences] = torch.cat([rows[:, n:], torch.full_like(rows[:, :n], -1)], 1)
+        self.kv_lens[sequences] = (self.kv_lens[sequences] - int(tokens)).clamp(min=0)
+
+    def select(self, q: torch.Tensor, count: int, *, first: int = 1, last: int = 1) -> PageSelection:
+        """The pages that q [B,H,1,D] or [B,H,D] attends, for each K/V head (select_pages)."""
+        if self.bounds is None:
+            raise ValueError("this cache keeps no bounds of its pages (bounds=True)")
+        return select_pages(q.unsqueeze(2) if q.dim() == 3 else q, self.bounds, self.page_table, self.kv_lens, count,
+                            page_size=self.page_size, first=first, last=last)
+
+    def decode(self, q: torch.Tensor, *, sm_scale: Optional[float] = None, return_lse: bool = False,
+               pages: Optional[PageSelection] = None, shared_lens: Optional[torch.Tensor] = None,
+               shared_groups: Optional[torch.Tensor] = None):
+        """Attention of one token a sequence, q [B,H,1,D] or the appended [B,H,D], over all held tokens,
+        or over `pages` that `select` chose; `shared_lens` and `shared_groups` as in paged_decode."""
         if q.dim() == 3:
             q = q.unsqueeze(2)
-        return paged_decode(q, self.k_pool, self.v_pool, self.page_table, self.kv_lens, sm_scale=sm_scale,
-                            return_lse=return_lse, k_scale=self.k_scale, v_scale=self.v_scale)
+        table, lens = (self.page_table, self.kv_lens) if pages is None else pages
+        return paged_decode(q, self.k_pool, self.v_pool, table, lens, sm_scale=sm_scale,
+                            return_lse=return_lse, k_scale=self.k_scale, v_scale=self.v_scale,
+                            shared_lens=shared_lens, shared_groups=shared_groups)
