@@ -36,6 +36,7 @@ struct BoundParams {
   void* bounds;                // [num_pages][H_kv][2][D]
   int H_kv, num_pages, page_shift;
   int chunk;                   // rows of the packed batch a CTA looks at: 8 or 32
+  int heads;                   // K/V heads it takes
   long long T;
 };
 
@@ -66,11 +67,10 @@ __device__ __forceinline__ uint32_t pair_max(uint32_t a, uint32_t b) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// A CTA looks at 8 or 32 rows of the packed batch for one K/V head.  The rows of a
-// page stand together, in order: the first of such a run is its leader, and the
-// CTA that holds the leader takes the whole run, wherever it ends, so that one
-// CTA reads and writes the page's bounds.  Few leaders (prompts) share the
-// eight warps out, many (a step of single tokens) take one warp each.
+// A CTA looks at 8 or 32 rows of the packed batch and some of the K/V heads.  The rows of a page stand
+// together, in order: the first of such a run is its leader, and the CTA that holds the leader takes the
+// whole run, wherever it ends, so that one CTA reads and writes the page's bounds.  A warp takes a
+// (leader, head); where there are fewer of them than warps, warps share one.
 template <typename KVT, int D>
 __global__ void __launch_bounds__(kBoundThreads) bounds_kernel(const BoundParams p) {
   constexpr bool kF8 = sizeof(KVT) == 1;
@@ -78,29 +78,39 @@ __global__ void __launch_bounds__(kBoundThreads) bounds_kernel(const BoundParams
   constexpr int kLanes = D * (int)sizeof(KVT) / 16;                // lanes of a row, 16 bytes each
   constexpr int kRows = 32 / kLanes;                               // rows a warp reads at once
   constexpr int kWords = kF8 ? 8 : 4;                              // pairs a lane holds
-  constexpr int kAhead = 4;                                        // reads in flight
-  __shared__ int s_leader[kChunk], s_count;
+  constexpr int kVecs = kWords / 4;                                // 16-byte vectors of them
+  constexpr int kAhead = 8;                                        // reads in flight
+  __shared__ int s_slot[kChunk], s_at[kChunk], s_rows[kChunk], s_count;
   __shared__ uint4 s_part[kBoundThreads / 32][2][D / 8];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, head = blockIdx.y;
-  const int page = 1 << p.page_shift;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int page = 1 << p.page_shift, head0 = blockIdx.y * p.heads, heads = min(p.heads, p.H_kv - head0);
   const long long places = (long long)p.num_pages << p.page_shift;
   grid_dep_wait();
   grid_dep_launch_dependents();
   const long long t0 = (long long)blockIdx.x * p.chunk;
   if (warp == 0) {
     const long long t = t0 + lane;
-    const int slot = lane < p.chunk && t < p.T ? p.slots[t] : -1;
-    int before = __shfl_up_sync(0xffffffffu, slot, 1);
-    if (lane == 0) before = t0 > 0 ? p.slots[t0 - 1] : -1;
-    if (slot >= places && head == 0) record_device_error(PU_ERR_INVALID_ARGUMENT, kSitePageBounds);
-    const bool leads = slot >= 0 && slot < places && (before < 0 || before != slot - 1 || (slot & (page - 1)) == 0);
-    const unsigned all = __ballot_sync(0xffffffffu, leads);
-    if (leads) s_leader[__popc(all & ((1u << lane) - 1))] = lane;
-    if (lane == 0) s_count = __popc(all);
+    int slot = lane < p.chunk && t < p.T ? p.slots[t] : -1;
+    int before = lane == 0 && t0 > 0 ? p.slots[t0 - 1] : -1;
+    const int up = __shfl_up_sync(0xffffffffu, slot, 1);
+    if (lane > 0) before = up;
+    if (slot >= places) {
+      if (head0 == 0) record_device_error(PU_ERR_INVALID_ARGUMENT, kSitePageBounds);
+      slot = -1;
+    }
+    const bool follows = slot >= 0 && before == slot - 1 && (slot & (page - 1)) != 0, leads = slot >= 0 && !follows;
+    const unsigned first = __ballot_sync(0xffffffffu, leads), rest = __ballot_sync(0xffffffffu, follows);
+    if (leads) {
+      const int k = __popc(first & ((1u << lane) - 1)), n = __ffs(~((rest >> lane) >> 1));     // 1 and those that follow
+      s_slot[k] = slot;
+      s_at[k] = lane;
+      s_rows[k] = n;
+    }
+    if (lane == 0) s_count = __popc(first);
   }
   __syncthreads();
-  const int n = s_count;
-  // warps that share a leader: 8 where there is one, 1 from eight leaders on
+  const int n = s_count * heads;
+  // warps that share a unit: 8 where there is one, 1 from eight units on
   const int team = n <= 1 ? 8 : n <= 2 ? 4 : n <= 4 ? 2 : 1, teams = 8 / team;
   const int sub = lane / kLanes, vec = lane % kLanes;
   for (int i0 = 0; i0 < n; i0 += teams) {
@@ -111,48 +121,64 @@ __global__ void __launch_bounds__(kBoundThreads) bounds_kernel(const BoundParams
       lo[w] = Pair<B>::kInf;
       hi[w] = Pair<B>::kMinusInf;
     }
-    int slot = 0;
+    uint4* out = nullptr;
+    auto fold = [&](int w, const uint4& a, const uint4& b) {
+      const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        lo[w + j] = pair_min<B>(lo[w + j], x[j]);
+        hi[w + j] = pair_max<B>(hi[w + j], y[j]);
+      }
+    };
     if (i < n) {
-      const long long t = t0 + s_leader[i];
-      slot = p.slots[t];
-      // rows of the run: as long as the next slot is the next row of this page
-      const int most = (int)min((long long)(page - (slot & (page - 1))), p.T - t);
-      int rows = most;
-      for (int r = 0; r < most; r += 32) {
-        const bool more = r + lane < most && p.slots[t + r + lane] == slot + r + lane;
-        const unsigned gap = ~__ballot_sync(0xffffffffu, more);
-        if (gap) {
-          rows = min(most, r + __ffs(gap) - 1);
-          break;
+      const int k = i / heads, head = head0 + i % heads, slot = s_slot[k], row = slot & (page - 1);
+      const size_t at = (size_t)(slot >> p.page_shift) * p.H_kv + head;
+      out = reinterpret_cast<uint4*>(p.bounds) + at * (2 * D / 8) + vec * kVecs;
+      // what the page's bounds were, where rows of it were written before
+      const bool old = row != 0 && part == 0 && sub == 0;
+      uint4 old_lo[kVecs], old_hi[kVecs];
+#pragma unroll
+      for (int w = 0; w < kVecs; ++w) {
+        old_lo[w] = make_uint4(0u, 0u, 0u, 0u);
+        old_hi[w] = old_lo[w];
+        if (old) {
+          old_lo[w] = out[w];
+          old_hi[w] = out[D / 8 + w];
         }
       }
-      const uint4* at = reinterpret_cast<const uint4*>(p.k_pool) +
-                        (((((size_t)(slot >> p.page_shift) * p.H_kv + head) << p.page_shift) + (slot & (page - 1))) * kLanes + vec);
+      // a run that reaches the end of the CTA's rows may go on: as long as the next slot is the next row of the page
+      int rows = s_rows[k];
+      if (s_at[k] + rows == p.chunk) {
+        const long long t = t0 + s_at[k];
+        const int most = (int)min((long long)(page - row), p.T - t);
+        for (int r = rows; r < most; r += 32) {
+          const bool more = r + lane < most && p.slots[t + r + lane] == slot + r + lane;
+          const unsigned gap = ~__ballot_sync(0xffffffffu, more);
+          rows = gap ? r + __ffs(gap) - 1 : r + 32;
+          if (gap) break;
+        }
+      }
+      const uint4* src = reinterpret_cast<const uint4*>(p.k_pool) + ((at << p.page_shift) + row) * kLanes + vec;
       for (int r0 = part * kRows + sub; r0 < rows; r0 += kAhead * team * kRows) {
         uint4 x[kAhead];
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
           // past the end the first row again, which changes nothing
           const int r = r0 + u * team * kRows;
-          x[u] = decode::ld_stream(at + (size_t)(r < rows ? r : r0) * kLanes);
+          x[u] = decode::ld_stream(src + (size_t)(r < rows ? r : r0) * kLanes);
         }
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
           const uint32_t w4[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
-          if constexpr (kF8) {
 #pragma unroll
-            for (int w = 0; w < kWords; ++w) {
-              const __half2 h(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w4[w >> 1] >> (16 * (w & 1))), __NV_E4M3));
-              const uint32_t v = *reinterpret_cast<const uint32_t*>(&h);
-              lo[w] = pair_min<B>(lo[w], v);
-              hi[w] = pair_max<B>(hi[w], v);
+          for (int w = 0; w < kWords; ++w) {
+            uint32_t v = w4[w >> (kF8 ? 1 : 0)];
+            if constexpr (kF8) {
+              const __half2 h(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(v >> (16 * (w & 1))), __NV_E4M3));
+              v = *reinterpret_cast<const uint32_t*>(&h);
             }
-          } else {
-#pragma unroll
-            for (int w = 0; w < kWords; ++w) {
-              lo[w] = pair_min<B>(lo[w], w4[w]);
-              hi[w] = pair_max<B>(hi[w], w4[w]);
-            }
+            lo[w] = pair_min<B>(lo[w], v);
+            hi[w] = pair_max<B>(hi[w], v);
           }
         }
       }
@@ -165,33 +191,22 @@ __global__ void __launch_bounds__(kBoundThreads) bounds_kernel(const BoundParams
           hi[w] = pair_max<B>(hi[w], __shfl_xor_sync(0xffffffffu, hi[w], off));
         }
       }
-      if (team > 1 && sub == 0) {
 #pragma unroll
-        for (int w = 0; w < kWords; w += 4) {
-          s_part[warp][0][vec * (kWords / 4) + w / 4] = make_uint4(lo[w], lo[w + 1], lo[w + 2], lo[w + 3]);
-          s_part[warp][1][vec * (kWords / 4) + w / 4] = make_uint4(hi[w], hi[w + 1], hi[w + 2], hi[w + 3]);
+      for (int w = 0; w < kVecs; ++w) {
+        if (old) fold(4 * w, old_lo[w], old_hi[w]);
+        if (team > 1 && sub == 0) {
+          s_part[warp][0][vec * kVecs + w] = make_uint4(lo[4 * w], lo[4 * w + 1], lo[4 * w + 2], lo[4 * w + 3]);
+          s_part[warp][1][vec * kVecs + w] = make_uint4(hi[4 * w], hi[4 * w + 1], hi[4 * w + 2], hi[4 * w + 3]);
         }
       }
     }
     if (team > 1) __syncthreads();
     if (i < n && part == 0 && sub == 0) {
-      uint4* out = reinterpret_cast<uint4*>(p.bounds) + ((size_t)(slot >> p.page_shift) * p.H_kv + head) * (2 * D / 8);
-      const bool begun = (slot & (page - 1)) != 0;      // rows of the page were written before
 #pragma unroll
-      for (int w = 0; w < kWords; w += 4) {
-        const int c = vec * (kWords / 4) + w / 4;
-        auto fold = [&](const uint4& a, const uint4& b) {
-          const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            lo[w + j] = pair_min<B>(lo[w + j], x[j]);
-            hi[w + j] = pair_max<B>(hi[w + j], y[j]);
-          }
-        };
-        for (int o = 1; o < team; ++o) fold(s_part[warp + o][0][c], s_part[warp + o][1][c]);
-        if (begun) fold(out[c], out[D / 8 + c]);
-        out[c] = make_uint4(lo[w], lo[w + 1], lo[w + 2], lo[w + 3]);
-        out[D / 8 + c] = make_uint4(hi[w], hi[w + 1], hi[w + 2], hi[w + 3]);
+      for (int w = 0; w < kVecs; ++w) {
+        for (int o = 1; o < team; ++o) fold(4 * w, s_part[warp + o][0][vec * kVecs + w], s_part[warp + o][1][vec * kVecs + w]);
+        out[w] = make_uint4(lo[4 * w], lo[4 * w + 1], lo[4 * w + 2], lo[4 * w + 3]);
+        out[D / 8 + w] = make_uint4(hi[4 * w], hi[4 * w + 1], hi[4 * w + 2], hi[4 * w + 3]);
       }
     }
     if (team > 1) __syncthreads();       // before the parts are written again
@@ -205,7 +220,9 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 1024;
 constexpr int kRank = kThreads;          // as many candidates are ranked against each other
-constexpr int kMaxPages = 24576;         // scores of a sequence that one CTA's shared memory holds
+constexpr int kMaxPages = 18432;         // scores of a sequence that one CTA's shared memory holds
+constexpr int kMaxCtas = 8;              // of a cluster
+constexpr int kStages = 2;               // of a warp's copies, eight pages each
 
 struct Params {
   const void* q;               // [B][H][D]
@@ -218,12 +235,14 @@ struct Params {
   int max_pages, num_pages, page_shift;
   int count, first, last;
   int ctas;                    // of a cluster
+  int by_length;               // clusters take the longest sequences first
+  int ring;                    // first byte of the copies, behind the scores
+  int B;
 };
 
 // A 16-bit value as fp64 times a power of two (2^-896 for bf16, 2^-1008 for f16): its sign,
-// exponent and mantissa bits moved to their places, which is exact for subnormals as well, in two
-// or three integer instructions where the conversion unit takes 16 values a clock.  Infinities
-// and NaN become values beyond the largest.
+// exponent and mantissa bits moved to their places, which is exact for subnormals as well.
+// Infinities and NaN become values beyond the largest.
 template <typename T>
 __device__ __forceinline__ double wide(uint32_t high_half) {
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
@@ -232,53 +251,233 @@ __device__ __forceinline__ double wide(uint32_t high_half) {
 }
 
 template <typename T>
-__device__ __forceinline__ double to_double(T x);
+__device__ __forceinline__ float to_float(T x);
 template <>
-__device__ __forceinline__ double to_double<__half>(__half x) { return (double)__half2float(x); }
+__device__ __forceinline__ float to_float<__half>(__half x) { return __half2float(x); }
 template <>
-__device__ __forceinline__ double to_double<__nv_bfloat16>(__nv_bfloat16 x) { return (double)__bfloat162float(x); }
+__device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+// A pair of 16-bit values as packed fp32.
+template <typename T>
+__device__ __forceinline__ uint64_t pair_to_f2(uint32_t w);
+template <>
+__device__ __forceinline__ uint64_t pair_to_f2<__nv_bfloat16>(uint32_t w) {
+  return f2_pack(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ uint64_t pair_to_f2<__half>(uint32_t w) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  return f2_pack(f.x, f.y);
+}
+
+// The larger magnitude, element by element; a NaN stays one.
+template <typename T>
+__device__ __forceinline__ uint32_t pair_top(uint32_t top, uint32_t w) {
+  using V = typename Pair<T>::V;
+  const V r = __hmax2_nan(*reinterpret_cast<const V*>(&top), __habs2(*reinterpret_cast<const V*>(&w)));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// 16 bytes from global to shared memory, zeros unless `ok`.
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 __device__ __forceinline__ void st_cluster_f64(uint32_t addr, double v) {
   asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(addr), "d"(v) : "memory");
 }
+__device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
 
-// Sums over the block (every thread gets them); s: kWarps values of shared memory.
-__device__ __forceinline__ int block_sum(int x, int* s, int warp, int lane) {
+// Shared memory of the choice.
+struct Room {
+  double red[2][kWarps];
+  double cand[kRank];
+  double cut;
+  int bins[kBins];
+  int list[kRank];
+  int sum[kWarps], tie[kWarps], scan[kWarps];
+  int found[4];                // border bin, members above it, its members, members listed
+};
+
+// Sum over the block (every thread gets it).
+__device__ __forceinline__ int block_sum(int x, Room& s, int warp, int lane) {
   x = __reduce_add_sync(0xffffffffu, x);
-  if (lane == 0) s[warp] = x;
+  if (lane == 0) s.sum[warp] = x;
   __syncthreads();
   int all = 0;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) all += s[w];
+  for (int w = 0; w < kWarps; ++w) all += s.sum[w];
   __syncthreads();
   return all;
 }
 
-// One cluster a (sequence, K/V head): its CTAs score the pages between them
-// and leave the scores in the first one's shared memory, which chooses.
+// The want-th largest (want >= 1) of the finite scores in [from, to), of which there are more than
+// `want`, and how many that equal it are among the first `want`.
 //
-// The choice: scores lie in kBins bins of equal width between the smallest and
-// the largest candidate (a monotone map, so no rounding of it can order two
-// scores wrongly), bins are counted from the top until the one that holds the
-// border, and its members are ranked against each other; where they are more
-// than 256 the same is done again between their own smallest and largest.
+// The scores lie in kBins bins of equal width between the smallest and the largest (a monotone map, so no
+// rounding of it can order two scores wrongly), bins are counted from the top until the one that holds the
+// border, and its members are ranked against each other; where they are more than 256 the same is done
+// again between their own smallest and largest.
+__device__ __forceinline__ void border(const double* score, int from, int to, int want, Room& s, double* cut, int* ties) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  double lo = INFINITY, hi = -INFINITY;
+  for (int i = from + tid; i < to; i += kThreads) {
+    const double x = score[i];
+    if (isinf(x)) continue;
+    lo = fmin(lo, x);
+    hi = fmax(hi, x);
+  }
+  while (true) {
+    // smallest and largest candidate, of all threads
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) {
+      lo = fmin(lo, __shfl_xor_sync(0xffffffffu, lo, off));
+      hi = fmax(hi, __shfl_xor_sync(0xffffffffu, hi, off));
+    }
+    if (lane == 0) {
+      s.red[0][warp] = lo;
+      s.red[1][warp] = hi;
+    }
+    for (int i = tid; i < kBins; i += kThreads) s.bins[i] = 0;
+    if (tid < 4) s.found[tid] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      lo = fmin(lo, s.red[0][w]);
+      hi = fmax(hi, s.red[1][w]);
+    }
+    if (lo == hi) {                      // equal scores: the first of them
+      *cut = lo;
+      *ties = want;
+      break;
+    }
+    const double scale = (double)(kBins - 1) / (hi - lo);
+    auto bin_of = [&](double x) { return min(kBins - 1, (int)((x - lo) * scale)); };
+    for (int i = from + tid; i < to; i += kThreads) {
+      const double x = score[i];
+      if (x >= lo && x <= hi) atomicAdd(s.bins + bin_of(x), 1);
+    }
+    __syncthreads();
+    // a thread's four bins, counted from the top
+    constexpr int kPer = kBins / kThreads;
+    const int top = kBins - 1 - tid * kPer;
+    int mine = 0;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) mine += s.bins[top - k];
+    int before = mine;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, before, off);
+      if (lane >= off) before += y;
+    }
+    if (lane == 31) s.scan[warp] = before;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) before += s.scan[w];
+    before -= mine;                      // candidates in the bins above this thread's
+    if (before < want && before + mine >= want) {
+      int at = before;
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) {
+        const int c = s.bins[top - k];
+        if (at < want && at + c >= want) {
+          s.found[0] = top - k;
+          s.found[1] = at;
+          s.found[2] = c;
+        }
+        at += c;
+      }
+    }
+    __syncthreads();
+    const int at = s.found[0], members = s.found[2];
+    want -= s.found[1];
+    if (members <= kRank) {
+      for (int i = from + tid; i < to; i += kThreads) {
+        const double x = score[i];
+        if (x >= lo && x <= hi && bin_of(x) == at) s.cand[atomicAdd(s.found + 3, 1)] = x;
+      }
+      __syncthreads();
+      if (tid < members) {
+        // fewer than `want` above it, at least `want` with its equals
+        const double x = s.cand[tid];
+        int above = 0, same = 0;
+        for (int i = 0; i < members; ++i) {
+          above += s.cand[i] > x;
+          same += s.cand[i] == x;
+        }
+        if (above < want && above + same >= want) {
+          s.cut = x;
+          s.found[1] = want - above;     // equal threads write equal values
+        }
+      }
+      __syncthreads();
+      *cut = s.cut;
+      *ties = s.found[1];
+      break;
+    }
+    // again among the border's members
+    double lo2 = INFINITY, hi2 = -INFINITY;
+    for (int i = from + tid; i < to; i += kThreads) {
+      const double x = score[i];
+      if (x >= lo && x <= hi && bin_of(x) == at) {
+        lo2 = fmin(lo2, x);
+        hi2 = fmax(hi2, x);
+      }
+    }
+    lo = lo2;
+    hi = hi2;
+    __syncthreads();
+  }
+  __syncthreads();                       // the room is free again
+}
+
+// One cluster a (sequence, K/V head): its CTAs score the pages between them and leave the scores in
+// the first one's shared memory, which chooses.
+//
+// Scores are first summed in fp32, with a bound of what they are off by:
+//   e = 2^-19 max |x| sum_d |c_d|  (x the bounds, c the heads' sums; 16 + 4 roundings of 2^-24 each, and c's)
+// The k-th largest of the true scores then lies within e of the k-th largest v of these, so pages above
+// v + 2 e are chosen, pages below v - 2 e are not, and only pages between, if there are more than places
+// left, are summed again in fp64 from their bounds: nearly always none.
+//
+// A page's bounds of one head are 4 D bytes in one piece.  Eight lanes take a page, and each lane copies
+// the chunks that it will read itself into shared memory, eight pages a step and a step ahead: copies in
+// flight need no registers and no barrier.
 template <typename QT, typename BT, int D>
-__global__ void __launch_bounds__(kThreads) select_kernel(const Params p) {
-  constexpr int kChunks = 2 * D / 64;    // 16-byte chunks a lane reads of a page: eight lanes a page
+__global__ void __launch_bounds__(kThreads, 2) select_kernel(const Params p) {
+  constexpr int kChunks = 2 * D / 64;    // 16-byte chunks a lane reads of a page
   extern __shared__ __align__(16) uint8_t dyn[];
   double* s_score = reinterpret_cast<double*>(dyn);                     // [max_pages], in the first CTA
-  __shared__ double s_coef[2][D];        // sums of the heads' negative and positive parts
-  __shared__ double s_red[2][kWarps];
-  __shared__ int s_bins[kBins];
-  __shared__ int s_sum[kWarps], s_tie[kWarps], s_warp[kWarps];
-  __shared__ double s_cand[kRank];
-  __shared__ int s_found[4];             // border bin, members above it, its members, members listed
-  __shared__ double s_cut;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  __shared__ float s_coef[2][D];         // sums of the heads' negative and positive parts
+  __shared__ double s_wide[2][D];        // the same in fp64, times 2^800
+  __shared__ double s_abs[kWarps];       // parts of the sum of their magnitudes
+  __shared__ uint32_t s_top[kMaxCtas * kWarps];    // largest magnitude of a bound that a warp saw, as bits
+  __shared__ int s_b;
+  __shared__ Room s;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, l8 = lane & 7, sub = lane >> 3;
   const int ctas = p.ctas, rank = (int)(blockIdx.x % (unsigned)ctas), item = (int)(blockIdx.x / (unsigned)ctas);
-  const int b = item / p.H_kv, head = item % p.H_kv;
+  const int head = item % p.H_kv;
+  int b = item / p.H_kv;
   grid_dep_wait();
   grid_dep_launch_dependents();
+  if (p.by_length) {
+    // the longest sequences first: the last clusters to start are the short ones
+    int* lens = s.bins;
+    for (int i = tid; i < p.B; i += kThreads) lens[i] = p.lens[i];
+    __syncthreads();
+    for (int i = tid; i < p.B; i += kThreads) {
+      const int n = lens[i];
+      int before = 0;
+      for (int j = 0; j < p.B; ++j) before += lens[j] > n || (lens[j] == n && j < i);
+      if (before == b) s_b = i;
+    }
+    __syncthreads();
+    b = s_b;
+  }
   const int page = 1 << p.page_shift;
   const int len = max(0, min(p.lens[b], p.max_pages << p.page_shift));
   const int live = (len + page - 1) >> p.page_shift;
@@ -286,207 +485,199 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const Params p) {
   const bool all = live <= p.count;      // nothing to choose
   if (all && rank != 0) return;
   const int from = p.first, to = live - p.last;      // candidates between the pages that are always kept
+  const uint4* bounds = static_cast<const uint4*>(p.bounds);
+  uint32_t top = 0;
 
   if (!all) {
     cluster_arrive();                    // every CTA runs before another writes to its shared memory
-    // ---- the heads' parts ----
+    // ---- scores: a run of pages a warp ----
+    const int workers = ctas * kWarps, per = ((to - from + workers - 1) / workers + 7) & ~7;
+    const int begin = from + (rank * kWarps + warp) * per, end = min(to, begin + per);
+    const int steps = max(0, (end - begin + 7) >> 3);
+    uint8_t* ring = dyn + p.ring + (warp * kStages * 2 * kChunks * 32 + lane) * 16;
+    int pg = -1;                         // a table entry for each lane
+    uint32_t valid = 0;                  // pages of the newest step (bits 0, 1) and the one before (2, 3)
+    auto begin_step = [&](int k) {       // copies of pages begin + 8 k + 4 u + sub
+      if ((k & 3) == 0) {
+        const int i = begin + 8 * k + lane;
+        pg = i < end ? table[i] : -1;
+        if (i < end && (unsigned)pg >= (unsigned)p.num_pages) record_device_error(PU_ERR_INVALID_ARGUMENT, kSiteSelectPage);
+      }
+      const uint32_t dst = smem_u32(ring + (k & 1) * 2 * kChunks * 512);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int entry = __shfl_sync(0xffffffffu, pg, (8 * k + 4 * u + sub) & 31);
+        const bool ok = (unsigned)entry < (unsigned)p.num_pages;
+        valid = valid << 1 | (ok ? 1u : 0u);
+        const uint4* src = bounds + ((size_t)(ok ? entry : 0) * p.H_kv + head) * (2 * D / 8) + l8;
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) cp_async_16(dst + (u * kChunks + c) * 512, src + c * 8, ok);
+      }
+    };
+    if (steps > 0) begin_step(0);
+    cp_async_commit();
+    // ---- the heads' parts, while the first bounds arrive ----
+    double sum = 0.;
     for (int i = tid; i < D; i += kThreads) {
       const QT* q = static_cast<const QT*>(p.q) + ((size_t)b * p.H + (size_t)head * p.group) * D + i;
       double neg = 0., pos = 0.;
-      for (int h = 0; h < p.group; ++h) {
-        const double x = to_double(q[(size_t)h * D]);
-        neg += fmin(x, 0.);
-        pos += fmax(x, 0.);
+      for (int h0 = 0; h0 < p.group; h0 += 8) {
+        QT x[8];
+#pragma unroll
+        for (int h = 0; h < 8; ++h) x[h] = q[(size_t)min(h0 + h, p.group - 1) * D];
+#pragma unroll
+        for (int h = 0; h < 8; ++h) {
+          const float y = h0 + h < p.group ? to_float(x[h]) : 0.f;
+          neg += (double)fminf(y, 0.f);
+          pos += (double)fmaxf(y, 0.f);
+        }
       }
+      s_coef[0][i] = (float)neg;
+      s_coef[1][i] = (float)pos;
       // with the bounds as they are (wide) every product stays a normal number
-      s_coef[0][i] = neg * 0x1p800;
-      s_coef[1][i] = pos * 0x1p800;
+      s_wide[0][i] = neg * 0x1p800;
+      s_wide[1][i] = pos * 0x1p800;
+      sum += pos - neg;
     }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    if (lane == 0) s_abs[warp] = sum;
     __syncthreads();
-    const int l8 = lane & 7, sub = lane >> 3;
-    double coef[kChunks][8];             // of this lane's chunks
+    uint64_t coef[kChunks][4];           // of this lane's chunks
 #pragma unroll
     for (int c = 0; c < kChunks; ++c)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int at = (c * 8 + l8) * 8 + e;             // element of the page's 2 D
-        coef[c][e] = s_coef[at / D][at % D];
+      for (int e = 0; e < 4; ++e) {
+        const int i = (c * 8 + l8) * 8 + 2 * e;          // element of the page's 2 D
+        coef[c][e] = *reinterpret_cast<const uint64_t*>(&s_coef[i / D][i % D]);
       }
-    // ---- scores: a run of pages a warp, 32 table entries at a time, four pages a read ----
-    const int workers = ctas * kWarps, per = ((to - from + workers - 1) / workers + 3) & ~3;
-    const int begin = from + (rank * kWarps + warp) * per, end = min(to, begin + per);
-    const uint4* bounds = static_cast<const uint4*>(p.bounds);
     const uint32_t dst = mapa_shared(s_score, 0);
     cluster_wait();
-    for (int base = begin; base < end; base += 32) {
-      const int pg = base + lane < end ? table[base + lane] : -1;
-      const bool bad = base + lane < end && (unsigned)pg >= (unsigned)p.num_pages;
-      if (bad) record_device_error(PU_ERR_INVALID_ARGUMENT, kSiteSelectPage);
-      const int n = min(32, end - base);
-      for (int j = 0; j < n; j += 8) {
-        uint4 x[2][kChunks];
-        bool ok[2];
+    for (int k = 0; k < steps; ++k) {
+      if (k + 1 < steps) begin_step(k + 1);
+      else valid <<= 2;
+      cp_async_commit();
+      cp_async_wait<1>();
+      const uint8_t* src = ring + (k & 1) * 2 * kChunks * 512;
+      float x[2];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int k = j + u * 4 + sub, entry = __shfl_sync(0xffffffffu, pg, k & 31);
-          ok[u] = k < n && (unsigned)entry < (unsigned)p.num_pages;
-          const uint4* at = bounds + ((size_t)(ok[u] ? entry : 0) * p.H_kv + head) * (2 * D / 8) + l8;
+      for (int u = 0; u < 2; ++u) {
+        uint64_t s2 = 0ull;
 #pragma unroll
-          for (int c = 0; c < kChunks; ++c) x[u][c] = decode::ld_stream_if(at + c * 8, ok[u]);
-        }
+        for (int c = 0; c < kChunks; ++c) {
+          const uint4 v = *reinterpret_cast<const uint4*>(src + (u * kChunks + c) * 512);
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          double s0 = 0., s1 = 0.;
-#pragma unroll
-          for (int c = 0; c < kChunks; ++c) {
-            const uint32_t w[4] = {x[u][c].x, x[u][c].y, x[u][c].z, x[u][c].w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              s0 = fma(wide<BT>(w[e] << 16), coef[c][2 * e], s0);
-              s1 = fma(wide<BT>(w[e]), coef[c][2 * e + 1], s1);
-            }
+          for (int e = 0; e < 4; ++e) {
+            s2 = f2_fma(pair_to_f2<BT>(w[e]), coef[c][e], s2);
+            top = pair_top<BT>(top, w[e]);
           }
-          double s = s0 + s1;
-#pragma unroll
-          for (int off = 4; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-          // finite for what follows (queries that are not finite); -inf marks an entry outside the pool
-          s = s != s ? 0x1p1000 : fmin(fmax(s, -0x1p1000), 0x1p1000);
-          if (l8 == 0 && j + u * 4 + sub < n) st_cluster_f64(dst + 8u * (uint32_t)(base + j + u * 4 + sub), ok[u] ? s : -INFINITY);
         }
+        float y;
+        f2_unpack(s2, x[u], y);
+        x[u] += y;
       }
+      // over the eight lanes: the upper four go on with the second page
+      const bool up = l8 & 4;
+      float y = up ? x[1] : x[0];
+      y += __shfl_xor_sync(0xffffffffu, up ? x[0] : x[1], 4);
+      y += __shfl_xor_sync(0xffffffffu, y, 2);
+      y += __shfl_xor_sync(0xffffffffu, y, 1);
+      // -inf marks an entry outside the pool; a sum that is not finite is summed again below
+      const int i = begin + 8 * k + (up ? 4 : 0) + sub;
+      const bool ok = (valid >> (up ? 2 : 3)) & 1u;
+      if (!isfinite(y)) top = 0x7fff7fffu;
+      if ((l8 & 3) == 0 && i < end) st_cluster_f64(dst + 8u * (uint32_t)i, !ok ? -INFINITY : isfinite(y) ? (double)y : 0x1p1000);
     }
+    top = max(top >> 16, top & 0xffffu);
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0) st_cluster_u32(mapa_shared(s_top + rank * kWarps + warp, 0), top);
     cluster_sync();
     if (rank != 0) return;
+    top = lane < workers ? s_top[lane] : 0u;
+    if (lane + 32 < workers) top = max(top, s_top[lane + 32]);
+    top = __reduce_max_sync(0xffffffffu, top);
   }
 
-  // ---- pages that are always kept, and all of them where nothing is chosen ----
-  int kept = 0;
+  // ---- pages that are always kept (all of them where nothing is chosen), and candidates ----
+  int counts = 0;                        // kept, and candidates times 2^16
   for (int i = tid; i < live; i += kThreads) {
-    if (!all && i >= from && i < to) continue;
-    const bool good = (unsigned)table[i] < (unsigned)p.num_pages;
-    if (!good) record_device_error(PU_ERR_INVALID_ARGUMENT, kSiteSelectPage);
-    s_score[i] = good ? INFINITY : -INFINITY;
-    kept += good;
+    if (!all && i >= from && i < to) {
+      counts += s_score[i] != -INFINITY ? 1 << 16 : 0;
+    } else {
+      const bool good = (unsigned)table[i] < (unsigned)p.num_pages;
+      if (!good) record_device_error(PU_ERR_INVALID_ARGUMENT, kSiteSelectPage);
+      s_score[i] = good ? INFINITY : -INFINITY;
+      counts += good;
+    }
   }
-  kept = block_sum(kept, s_sum, warp, lane);       // and the scores are visible to all
+  counts = block_sum(counts, s, warp, lane);         // and the scores are visible to all
 
   // ---- the border: every score above `cut` is kept, and the first `ties` equal to it ----
   double cut = -INFINITY;
   int ties = 0;
   if (!all) {
-    int want = p.count - kept;           // of the candidates
-    double lo = INFINITY, hi = -INFINITY;
-    int cands = 0;
-    for (int i = from + tid; i < to; i += kThreads) {
-      const double s = s_score[i];
-      if (s == -INFINITY) continue;
-      ++cands;
-      lo = fmin(lo, s);
-      hi = fmax(hi, s);
-    }
-    cands = block_sum(cands, s_sum, warp, lane);
+    int want = p.count - (counts & 0xffff);          // of the candidates
     if (want <= 0) {
       cut = 0x1p1010;                    // none but those always kept
-    } else if (cands > want) {
-      while (true) {
-        // smallest and largest candidate, of all threads
+    } else if (counts >> 16 > want) {
+      border(s_score, from, to, want, s, &cut, &ties);
+      // what the fp32 sums are off by; 2^-140: sums of subnormals
+      double e = 0.;
 #pragma unroll
-        for (int off = 16; off > 0; off >>= 1) {
-          lo = fmin(lo, __shfl_xor_sync(0xffffffffu, lo, off));
-          hi = fmax(hi, __shfl_xor_sync(0xffffffffu, hi, off));
+      for (int w = 0; w < kWarps; ++w) e += s_abs[w];
+      const float big = to_float(*reinterpret_cast<const BT*>(&top));
+      e = isfinite(big) && e < 0x1p1000 ? fma(e * (double)big, 0x1p-19, 0x1p-140) : INFINITY;
+      const double sure = cut + 2. * e, none = cut - 2. * e;
+      if (tid == 0) s.found[3] = 0;
+      __syncthreads();
+      counts = 0;                        // above, and near times 2^16
+      for (int i = from + tid; i < to; i += kThreads) {
+        const double x = s_score[i];
+        if (x == -INFINITY) continue;
+        if (x > sure) {
+          ++counts;
+          s_score[i] = INFINITY;
+        } else if (x < none) {
+          s_score[i] = -INFINITY;
+        } else {
+          counts += 1 << 16;
+          const int k = atomicAdd(s.found + 3, 1);
+          if (k < kRank) s.list[k] = i;
         }
-        if (lane == 0) {
-          s_red[0][warp] = lo;
-          s_red[1][warp] = hi;
-        }
-        for (int i = tid; i < kBins; i += kThreads) s_bins[i] = 0;
-        if (tid < 4) s_found[tid] = 0;
-        __syncthreads();
+      }
+      counts = block_sum(counts, s, warp, lane);
+      const int near = counts >> 16;
+      want -= counts & 0xffff;
+      cut = -INFINITY;                   // as many as places: all of them
+      ties = 0;
+      if (near > want) {
+        // ---- summed again in fp64, a warp a page ----
+        const bool listed = near <= kRank;
+        for (int k = listed ? warp : from + warp; k < (listed ? near : to); k += kWarps) {
+          const int i = listed ? s.list[k] : k;
+          if (isinf(s_score[i])) continue;
+          const uint4* src = bounds + ((size_t)table[i] * p.H_kv + head) * (2 * D / 8);
+          double x = 0.;
+          for (int c = lane; c < 2 * D / 8; c += 32) {
+            const uint4 v = src[c];
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+            const double* f = &s_wide[0][0] + c * 8;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          lo = fmin(lo, s_red[0][w]);
-          hi = fmax(hi, s_red[1][w]);
-        }
-        if (lo == hi) {                  // equal scores: the first of them
-          cut = lo;
-          ties = want;
-          break;
-        }
-        const double scale = (double)(kBins - 1) / (hi - lo);
-        auto bin_of = [&](double s) { return min(kBins - 1, (int)((s - lo) * scale)); };
-        for (int i = from + tid; i < to; i += kThreads) {
-          const double s = s_score[i];
-          if (s >= lo && s <= hi) atomicAdd(s_bins + bin_of(s), 1);
-        }
-        __syncthreads();
-        // a thread's four bins, counted from the top
-        constexpr int kPer = kBins / kThreads;
-        const int top = kBins - 1 - tid * kPer;
-        int mine = 0;
-#pragma unroll
-        for (int k = 0; k < kPer; ++k) mine += s_bins[top - k];
-        int before = mine;
-#pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-          const int y = __shfl_up_sync(0xffffffffu, before, off);
-          if (lane >= off) before += y;
-        }
-        if (lane == 31) s_warp[warp] = before;
-        __syncthreads();
-        for (int w = 0; w < warp; ++w) before += s_warp[w];
-        before -= mine;                  // candidates in the bins above this thread's
-        if (before < want && before + mine >= want) {
-          int at = before;
-#pragma unroll
-          for (int k = 0; k < kPer; ++k) {
-            const int c = s_bins[top - k];
-            if (at < want && at + c >= want) {
-              s_found[0] = top - k;
-              s_found[1] = at;
-              s_found[2] = c;
-            }
-            at += c;
-          }
-        }
-        __syncthreads();
-        const int border = s_found[0], members = s_found[2];
-        want -= s_found[1];
-        if (members <= kRank) {
-          for (int i = from + tid; i < to; i += kThreads) {
-            const double s = s_score[i];
-            if (s >= lo && s <= hi && bin_of(s) == border) s_cand[atomicAdd(s_found + 3, 1)] = s;
-          }
-          __syncthreads();
-          if (tid < members) {
-            // the want-th largest: fewer than `want` above it, at least `want` with its equals
-            const double s = s_cand[tid];
-            int above = 0, same = 0;
-            for (int i = 0; i < members; ++i) {
-              above += s_cand[i] > s;
-              same += s_cand[i] == s;
-            }
-            if (above < want && above + same >= want) {
-              s_cut = s;
-              s_found[1] = want - above; // equal threads write equal values
+            for (int j = 0; j < 4; ++j) {
+              x = fma(wide<BT>(w[j] << 16), f[2 * j], x);
+              x = fma(wide<BT>(w[j]), f[2 * j + 1], x);
             }
           }
-          __syncthreads();
-          cut = s_cut;
-          ties = s_found[1];
-          break;
+#pragma unroll
+          for (int off = 16; off > 0; off >>= 1) x += __shfl_xor_sync(0xffffffffu, x, off);
+          // finite, also for queries that are not
+          if (lane == 0) s_score[i] = x != x ? 0x1p1000 : fmin(fmax(x, -0x1p1000), 0x1p1000);
+          __syncwarp();
         }
-        // again among the border's members
-        double lo2 = INFINITY, hi2 = -INFINITY;
-        for (int i = from + tid; i < to; i += kThreads) {
-          const double s = s_score[i];
-          if (s >= lo && s <= hi && bin_of(s) == border) {
-            lo2 = fmin(lo2, s);
-            hi2 = fmax(hi2, s);
-          }
-        }
-        lo = lo2;
-        hi = hi2;
         __syncthreads();
+        if (want > 0) border(s_score, from, to, want, s, &cut, &ties);
+        else cut = 0x1p1010;
       }
     }
   }
@@ -495,30 +686,30 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const Params p) {
   const int run = ((live + kWarps - 1) / kWarps + 31) & ~31, begin = warp * run, end = min(live, begin + run);
   int above = 0, same = 0;
   for (int i = begin; i < end; i += 32) {
-    const double s = i + lane < end ? s_score[i + lane] : -INFINITY;
-    above += __popc(__ballot_sync(0xffffffffu, s > cut));
-    same += __popc(__ballot_sync(0xffffffffu, s == cut && s != -INFINITY));
+    const double x = i + lane < end ? s_score[i + lane] : -INFINITY;
+    above += __popc(__ballot_sync(0xffffffffu, x > cut));
+    same += __popc(__ballot_sync(0xffffffffu, x == cut && x != -INFINITY));
   }
   if (lane == 0) {
-    s_sum[warp] = above;
-    s_tie[warp] = same;
+    s.sum[warp] = above;
+    s.tie[warp] = same;
   }
   __syncthreads();
   int a0 = 0, t0 = 0, a1 = 0, t1 = 0;    // before this warp, and in all
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {
     if (w < warp) {
-      a0 += s_sum[w];
-      t0 += s_tie[w];
+      a0 += s.sum[w];
+      t0 += s.tie[w];
     }
-    a1 += s_sum[w];
-    t1 += s_tie[w];
+    a1 += s.sum[w];
+    t1 += s.tie[w];
   }
   const int chosen = min(p.count, a1 + min(ties, t1));
-  int32_t* out = p.pages + (size_t)item * p.count;
+  int32_t* out = p.pages + ((size_t)b * p.H_kv + head) * p.count;
   for (int i = begin; i < end; i += 32) {
-    const double s = i + lane < end ? s_score[i + lane] : -INFINITY;
-    const unsigned up = __ballot_sync(0xffffffffu, s > cut), eq = __ballot_sync(0xffffffffu, s == cut && s != -INFINITY);
+    const double x = i + lane < end ? s_score[i + lane] : -INFINITY;
+    const unsigned up = __ballot_sync(0xffffffffu, x > cut), eq = __ballot_sync(0xffffffffu, x == cut && x != -INFINITY);
     const unsigned below = (1u << lane) - 1;
     const int nth = t0 + __popc(eq & below);             // ties before this page
     const int place = a0 + __popc(up & below) + min(ties, nth);
@@ -531,30 +722,33 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const Params p) {
     // only the sequence's last page may hold fewer tokens than a page; it is last in the list
     int tokens = chosen << p.page_shift;
     if (live > 0) {
-      const double s = s_score[live - 1];
-      const bool in = s > cut || (s == cut && s != -INFINITY && t1 - 1 < ties);
+      const double x = s_score[live - 1];
+      const bool in = x > cut || (x == cut && x != -INFINITY && t1 - 1 < ties);
       if (in) tokens -= (live << p.page_shift) - len;
     }
-    p.out_lens[item] = tokens;
+    p.out_lens[(size_t)b * p.H_kv + head] = tokens;
   }
 }
 
-// CTAs of a cluster: one for 64 pages of a full table row, up to the portable eight
-inline int cluster_size(long long max_pages) {
+// CTAs of a cluster: what brings the grid to about three CTAs an SM, but no more than one for 64 pages of a
+// full table row.
+inline int cluster_size(long long max_pages, long long items) {
   int c = 1;
-  while (c < 8 && max_pages > 64ll * c) c *= 2;
+  while (c < kMaxCtas && max_pages > 64ll * c && 2 * c * items <= 4ll * sm_count()) c *= 2;
   return c;
 }
 
 template <typename QT, typename BT, int D>
-int launch_select(const Params& p, long long items, cudaStream_t st) {
+int launch_select(Params p, long long items, cudaStream_t st) {
   const auto f = select_kernel<QT, BT, D>;
-  int rc = set_max_dynamic_smem(reinterpret_cast<const void*>(f), kMaxPages * (int)sizeof(double), "page choice shared memory");
+  constexpr int kRing = kStages * kWarps * 32 * D;   // eight pages of 4 D bytes a warp and stage
+  p.ring = (p.max_pages * (int)sizeof(double) + 15) / 16 * 16;
+  int rc = set_max_dynamic_smem(reinterpret_cast<const void*>(f), kMaxPages * (int)sizeof(double) + kRing, "page choice shared memory");
   if (rc) return rc;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(items * p.ctas));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = (size_t)p.max_pages * sizeof(double);
+  cfg.dynamicSmemBytes = (size_t)(p.ring + kRing);
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -564,12 +758,12 @@ int launch_select(const Params& p, long long items, cudaStream_t st) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return check_cuda(cudaLaunchKernelEx(&cfg, f, p), "page choice launch");
+  return check_cuda(cudaLaunchKernelEx(&cfg, f, static_cast<const Params>(p)), "page choice launch");
 }
 
 template <typename KVT, int D>
 int launch_bounds(const BoundParams& p, cudaStream_t st) {
-  const dim3 grid((unsigned)((p.T + p.chunk - 1) / p.chunk), (unsigned)p.H_kv);
+  const dim3 grid((unsigned)((p.T + p.chunk - 1) / p.chunk), (unsigned)((p.H_kv + p.heads - 1) / p.heads));
   return check_cuda(decode::launch_pdl(bounds_kernel<KVT, D>, grid, dim3(kBoundThreads), 0, st, p), "page bounds launch");
 }
 
@@ -599,7 +793,12 @@ extern "C" int pu_page_bounds(const void* k_pool, int kv_dtype, const int32_t* s
   p.num_pages = (int)num_pages;
   p.page_shift = shift;
   p.T = num_tokens;
-  p.chunk = 32;
+  // Small batches are spread out: eight single tokens and one head a CTA are a warp's row each.
+  // Larger ones share the reads of the slots over as many heads as leave four CTAs an SM.
+  const long long room = 4ll * pu::sm_count();
+  p.chunk = (num_tokens + 7) / 8 * H_kv <= room ? 8 : 32;
+  p.heads = (int)std::min<long long>(H_kv, std::max<long long>(1, (num_tokens + p.chunk - 1) / p.chunk * H_kv / room));
+  p.heads = (int)((H_kv + (H_kv + p.heads - 1) / p.heads - 1) / ((H_kv + p.heads - 1) / p.heads));   // as evenly
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (kv_dtype == PU_DTYPE_FP8_E4M3)
     return D == 128 ? launch_bounds<__nv_fp8_e4m3, 128>(p, st) : launch_bounds<__nv_fp8_e4m3, 64>(p, st);
@@ -629,7 +828,7 @@ extern "C" int pu_select_pages(const void* q, int q_dtype, const void* bounds, i
     return pu::set_error(PU_ERR_UNSUPPORTED, "page choice: %lld pages per sequence (up to %d)", (long long)max_pages_per_seq, kMaxPages);
   if (count > (1ll << 30) / page_size) return pu::set_error(PU_ERR_UNSUPPORTED, "page choice: %lld pages chosen", (long long)count);
   Params p{};
-  p.ctas = cluster_size(max_pages_per_seq);
+  p.ctas = cluster_size(max_pages_per_seq, B * H_kv);
   if (H > 2147483647ll || B > 2147483647ll / p.ctas / H) return pu::set_error(PU_ERR_UNSUPPORTED, "page choice: batch too large");
   p.q = q;
   p.bounds = bounds;
@@ -643,6 +842,9 @@ extern "C" int pu_select_pages(const void* q, int q_dtype, const void* bounds, i
   p.max_pages = (int)max_pages_per_seq;
   p.num_pages = (int)num_pages;
   p.page_shift = shift;
+  p.B = (int)B;
+  // where the clusters do not all start at once; 256 lengths took 5 us to rank
+  p.by_length = B > 1 && B <= 64 && B * H_kv * p.ctas > 2ll * pu::sm_count();
   p.count = (int)count;
   p.first = (int)first;
   p.last = (int)last;

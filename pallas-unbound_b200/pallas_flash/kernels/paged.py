@@ -244,7 +244,7 @@ def select_pages(q: torch.Tensor, bounds: torch.Tensor, page_table: torch.Tensor
     chosen and reported (device_status detail 310); queries and bounds are finite.
 
     q [B,H,1,D] fp16/bf16, bounds of `page_bounds`, page_table int32
-    [B,max_pages_per_seq] (up to 24576), kv_lens int32 [B].  The scores' scale and
+    [B,max_pages_per_seq] (up to 18432), kv_lens int32 [B].  The scores' scale and
     the scale of an fp8 pool change nothing.  The result goes into
     `paged_decode(q, k_pool, v_pool, chosen.pages, chosen.lens)`."""
     _check_bounds(bounds)
