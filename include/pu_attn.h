@@ -379,10 +379,10 @@ PU_API int pu_decode_paged_heads(const void* q, int q_dtype,
  *   shared_lens int32 [groups]: tokens that the group's sequences have in common,
  *     in whole pages (rounded down).  They are read through the table row of the
  *     group's first sequence that holds as many; the others' entries for them must
- *     name the same pages.  A sequence that holds fewer attends those it holds.  A
+ *     name the same pages.  A sequence that holds fewer attends them by itself.  A
  *     group in which none holds as many shares nothing.
  * q and pools of one 16-bit type, D 64 or 128, or e4m3 pools with D = 128; any
- * H / H_kv; groups <= 64; B <= 8192; H <= 65535; H_kv * D <= 2^20 - 16.
+ * H / H_kv; groups <= 64; B <= 8192; H <= 65535; H_kv * D <= 2^21 - 32.
  *   workspace: pu_decode_paged_shared_workspace_size() bytes, zeroed before its
  *   first use (left as pu_decode_paged_gqa needs it).
  * The softmax weights of shared tokens are rounded once to the pools' 16-bit type,

@@ -44,7 +44,7 @@ namespace shared {
 constexpr int BT = 128;                  // tokens of a tile
 constexpr int kRows = 256;               // rows of an item
 constexpr int kMaxGroups = 64;
-constexpr int kItemCost = 1;             // what starting and ending an item costs, in tiles
+constexpr int kItemCost = 2;             // what starting and ending an item costs, in tiles
 constexpr int kBadRing = 8;
 
 template <typename T, typename KVT, int D>
@@ -128,6 +128,16 @@ struct Line {
 };
 
 __device__ __forceinline__ int tiles_of(const Group& g) { return (g.tokens + BT - 1) / BT; }
+
+// Items of the groups before g.
+__device__ __forceinline__ int items_before(const Group* gs, int g) {
+  int n = 0;
+  for (int i = 0; i < g; ++i) {
+    const int tiles = tiles_of(gs[i]);
+    if (tiles > 0) n += (gs[i + 1].unit - gs[i].unit) / (tiles + kItemCost);
+  }
+  return n;
+}
 
 // A CTA's runs of tiles, one item after the other.
 struct Walk {
@@ -328,7 +338,8 @@ __global__ void __launch_bounds__(Cfg<T, KVT, D>::kThreads, 1)
     for (int i = tid; i <= p.groups; i += C::kThreads) p.desc[i] = s_groups[i];
     for (int b = tid; b < p.B; b += C::kThreads) {
       const int g = group_of(s_groups, p.groups, b);
-      const int skip = g >= 0 ? s_groups[g].tokens : 0;
+      // a sequence that holds fewer tokens than its group shares attends them by itself
+      const int skip = g >= 0 && p.lens[b] >= s_groups[g].tokens ? s_groups[g].tokens : 0;
       p.skip[b] = skip;
       p.own_lens[b] = max(0, min(p.lens[b], p.max_pages << p.page_shift) - skip);
     }
@@ -528,7 +539,7 @@ __global__ void __launch_bounds__(Cfg<T, KVT, D>::kThreads, 1)
     int j0 = 0;                          // tiles of the CTA so far
     while (w.next()) {
       const Group& g = s_groups[w.g];
-      const int head = w.head(), row0 = w.row0(), tokens = g.tokens;
+      const int head = w.head(), row0 = w.row0();
       // ---- this slot's part of the queries ----
       if (w.seg > 0) mbar_wait(bQe, (w.seg - 1) & 1, abort_flag, kSiteDecodeTc);
       {
@@ -581,9 +592,6 @@ __global__ void __launch_bounds__(Cfg<T, KVT, D>::kThreads, 1)
       }
       const int item_row = w.split ? row : t * 128 + row;
       const bool active = (item_row & ~31) < w.rows;     // a warp without rows only takes part in the barriers
-      // tokens that this row sees: its sequence may hold fewer than the group
-      int lim = tokens;
-      if (item_row < w.rows) lim = min(lim, p.lens[g.start + (row0 + item_row) / p.group]);
       float scale = p.scale_log2;
       if constexpr (kF8) {
         mbar_wait(bQ, w.seg & 1, abort_flag, kSiteDecodeTc);
@@ -592,7 +600,7 @@ __global__ void __launch_bounds__(Cfg<T, KVT, D>::kThreads, 1)
       float m = -INFINITY, l = 0.f;
       const int jobs = w.jobs(), step = w.split ? 0 : 1;
       for (int k = t; k < jobs; k += 2, ++js) {
-        const int tile = w.t0 + (k >> step), j = j0 + (k >> step), kv0 = tile * BT;
+        const int j = j0 + (k >> step);
         mbar_wait(bS + t, js & 1, abort_flag, kSiteDecodeTc);
         __syncwarp();
         tc_fence_after();
@@ -626,11 +634,6 @@ __global__ void __launch_bounds__(Cfg<T, KVT, D>::kThreads, 1)
 #pragma unroll
           for (int c = 0; c < BT; ++c)
             if ((bad >> (c >> 4)) & 1u) s[c] = __float_as_uint(-INFINITY);
-        }
-        if (__any_sync(0xffffffffu, kv0 + BT > lim)) {
-#pragma unroll
-          for (int c = 0; c < BT; ++c)
-            if (kv0 + c >= lim) s[c] = __float_as_uint(-INFINITY);
         }
         float mx8[8];
 #pragma unroll
@@ -689,18 +692,10 @@ __global__ void __launch_bounds__(Cfg<T, KVT, D>::kThreads, 1)
       __syncwarp();
       tc_fence_after();
       const bool whole = w.n == w.tiles;
-      // items before this one's group: units say how many
-      int item = w.r;
-      if (whole) {
-        for (int i = 0; i < w.g; ++i) {
-          const int tl = tiles_of(s_groups[i]);
-          if (tl > 0) item += (s_groups[i + 1].unit - s_groups[i].unit) / (tl + kItemCost);
-        }
-      }
-      float* slab = p.slabs + (size_t)(whole ? 2 * (int)gridDim.x + item : 2 * cta + (w.seg > 0)) * kSlab<D>;
+      float* slab = p.slabs + (size_t)(whole ? 2 * (int)gridDim.x + items_before(s_groups, w.g) + w.r : 2 * cta + (w.seg > 0)) * kSlab<D>;
       const int place = t * 128 + row;
       reinterpret_cast<float2*>(slab)[place] = make_float2(m, l);
-      if (t < jobs && active) {          // the slot has had a job
+      if (active) {
         float4* o = reinterpret_cast<float4*>(slab + 2 * kRows) + place;
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
@@ -708,6 +703,10 @@ __global__ void __launch_bounds__(Cfg<T, KVT, D>::kThreads, 1)
           tmem_ld32(tO + c * 32, ov);
           tmem_wait_ld();
           reg_fence(ov);
+          if (t >= jobs) {               // no tile for this slot
+#pragma unroll
+            for (int i = 0; i < 32; ++i) ov[i] = 0u;
+          }
 #pragma unroll
           for (int i = 0; i < 8; ++i)
             o[(c * 8 + i) * kRows] = make_float4(__uint_as_float(ov[4 * i]), __uint_as_float(ov[4 * i + 1]), __uint_as_float(ov[4 * i + 2]),
@@ -727,10 +726,11 @@ __global__ void __launch_bounds__(Cfg<T, KVT, D>::kThreads, 1)
 }
 
 // ---------------------------------------------------------------------------
-// the join: a thread a row and a few columns
+// the join: a thread a row and four columns, a warp 32 rows of one K/V head
 // ---------------------------------------------------------------------------
 struct JoinParams {
   const Group* desc;
+  const int32_t* skip;         // [B]
   const float* slabs;
   const float* own_o;          // [B * H][D] fp32, the own tokens' output
   const float* own_lse;        // [B * H]
@@ -740,70 +740,53 @@ struct JoinParams {
   float o_scale;
 };
 
-constexpr int kJoinThreads = 128;
-constexpr int kJoinCols = 16;            // columns of a thread
+constexpr int kJoinWarps = 8;
 
+// Up to eight records are asked for at once, weights and columns together (first weights, then columns
+// where they count, with four records at once and 16 columns a thread: 64 sequences, 19 records a row, 18 us).
 template <int D>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const JoinParams p) {
+__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const JoinParams p) {
   grid_dep_wait();
   grid_dep_launch_dependents();
-  constexpr int kVec = kJoinCols / 4;
-  const long long rows = (long long)p.B * p.group;
-  const long long x = (long long)blockIdx.x * kJoinThreads + threadIdx.x;  // row of the head, sequences first
-  const int head = (int)(blockIdx.y % (unsigned)p.H_kv), part = (int)(blockIdx.y / (unsigned)p.H_kv);
+  constexpr int kParts = D / 4 / kJoinWarps;
+  const int rows = p.B * p.group, x = (int)blockIdx.x * 32 + (int)(threadIdx.x & 31);       // row of the head, sequences first
+  const int head = (int)(blockIdx.y / kParts), col = (int)(blockIdx.y % kParts) * kJoinWarps + (int)(threadIdx.x >> 5);
   if (x >= rows) return;
-  const int b = (int)(x / p.group);
-  const size_t out = (size_t)b * p.H + (size_t)head * p.group + (int)(x % p.group);
-  // the sequence's own tokens
-  float M = p.own_lse[out] * kLog2e, L = M == -INFINITY ? 0.f : 1.f;
-  float4 acc[kVec];
-#pragma unroll
-  for (int v = 0; v < kVec; ++v) {
-    acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (L > 0.f) acc[v] = reinterpret_cast<const float4*>(p.own_o + out * D + part * kJoinCols)[v];
+  const int b = x / p.group;
+  const size_t out = (size_t)b * p.H + (size_t)head * p.group + (x - b * p.group);
+  // the sequence's own tokens; an output of no weight is not there
+  float M = p.own_lse[out] * kLog2e, L = 1.f;
+  float4 acc = reinterpret_cast<const float4*>(p.own_o + out * D)[col];
+  const int skip = p.skip[b];
+  if (M == -INFINITY) {
+    L = 0.f;
+    acc = make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  const int g = group_of(p.desc, p.groups, b);
-  if (g >= 0 && p.desc[g].tokens > 0) {
+  if (skip > 0) {
+    const int g = group_of(p.desc, p.groups, b);
     const Group a = p.desc[g];
     const Line line(p.desc[p.groups].unit, p.grid);
     const int all = (p.desc[g + 1].start - a.start) * p.group, pairs = (all + kRows - 1) / kRows, tiles = tiles_of(a);
-    const int at = (int)(x - (long long)a.start * p.group), pair = at / kRows, in = at % kRows;
+    const int at = x - a.start * p.group, pair = at / kRows;
     const int r = head * pairs + pair, item0 = a.unit + r * (tiles + kItemCost), first = item0 + kItemCost;
     const int c0 = line.holder(first), c1 = line.holder(first + tiles - 1);
-    const bool split = min(kRows, all - pair * kRows) <= kRows / 2;
-    const int many = (c1 - c0 + 1) << (split ? 1 : 0);
-    int item = r;
-    if (c0 == c1) {
-      for (int i = 0; i < g; ++i) {
-        const int tl = tiles_of(p.desc[i]);
-        if (tl > 0) item += (p.desc[i + 1].unit - p.desc[i].unit) / (tl + kItemCost);
-      }
-    }
+    // both slots of a CTA leave a record where they shared the rows
+    const int shift = min(kRows, all - pair * kRows) <= kRows / 2 ? 1 : 0, many = (c1 - c0 + 1) << shift;
     const bool second = line.part(c0) < item0;     // the item is not the first run of its first CTA
-    auto slab_of = [&](int i) -> const float* {    // record i: its slab, moved to this row's place
-      const int c = c0 + (split ? i >> 1 : i);
-      const size_t id = c0 == c1 ? (size_t)2 * p.grid + item : (size_t)2 * c + (c == c0 && second);
-      return p.slabs + id * kSlab<D>;
-    };
-    constexpr int kAhead = 4;
+    const size_t only = c0 == c1 ? (size_t)(2 * p.grid + items_before(p.desc, g) + r) : 0;
+    constexpr int kAhead = 8;
     for (int i0 = 0; i0 < many; i0 += kAhead) {
       float2 ml[kAhead];
-      float4 v[kAhead][kVec];
+      float4 v[kAhead];
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
         ml[u] = make_float2(-INFINITY, 0.f);
-        const int i = i0 + u, place = split ? (i & 1) * 128 + in : in;
-        if (i < many) ml[u] = __ldcg(reinterpret_cast<const float2*>(slab_of(i)) + place);
-      }
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const int i = i0 + u, place = split ? (i & 1) * 128 + in : in;
-#pragma unroll
-        for (int c = 0; c < kVec; ++c) {
-          v[u][c] = make_float4(0.f, 0.f, 0.f, 0.f);
-          // a record without weight may hold anything
-          if (ml[u].x != -INFINITY)
-            v[u][c] = __ldcg(reinterpret_cast<const float4*>(slab_of(i) + 2 * kRows) + (part * kVec + c) * kRows + place);
+        v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        const int i = i0 + u, c = c0 + (i >> shift), place = at % kRows + (shift ? (i & 1) * (kRows / 2) : 0);
+        if (i < many) {
+          const float* slab = p.slabs + (only ? only : (size_t)(2 * c + (c == c0 && second))) * kSlab<D>;
+          ml[u] = __ldcg(reinterpret_cast<const float2*>(slab) + place);
+          v[u] = __ldcg(reinterpret_cast<const float4*>(slab + 2 * kRows) + col * kRows + place);
         }
       }
       float top = M;
@@ -811,39 +794,28 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const JoinParams p) 
       for (int u = 0; u < kAhead; ++u) top = fmaxf(top, ml[u].x);
       const float keep = M == -INFINITY ? 0.f : ex2(M - top);
       L *= keep;
-#pragma unroll
-      for (int c = 0; c < kVec; ++c) {
-        acc[c].x *= keep;
-        acc[c].y *= keep;
-        acc[c].z *= keep;
-        acc[c].w *= keep;
-      }
+      acc.x *= keep;
+      acc.y *= keep;
+      acc.z *= keep;
+      acc.w *= keep;
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
         const float wt = ml[u].x == -INFINITY ? 0.f : ex2(ml[u].x - top), wo = wt * p.o_scale;
         L = fmaf(wt, ml[u].y, L);
-#pragma unroll
-        for (int c = 0; c < kVec; ++c) {
-          acc[c].x = fmaf(wo, v[u][c].x, acc[c].x);
-          acc[c].y = fmaf(wo, v[u][c].y, acc[c].y);
-          acc[c].z = fmaf(wo, v[u][c].z, acc[c].z);
-          acc[c].w = fmaf(wo, v[u][c].w, acc[c].w);
-        }
+        acc.x = fmaf(wo, v[u].x, acc.x);
+        acc.y = fmaf(wo, v[u].y, acc.y);
+        acc.z = fmaf(wo, v[u].z, acc.z);
+        acc.w = fmaf(wo, v[u].w, acc.w);
       }
       M = top;
     }
   }
   const float inv = L == 0.f ? 0.f : 1.f / L;
-  uint32_t y[2 * kVec];
-#pragma unroll
-  for (int c = 0; c < kVec; ++c) {
-    y[2 * c] = pack_bf16x2(acc[c].x * inv, acc[c].y * inv);
-    y[2 * c + 1] = pack_bf16x2(acc[c].z * inv, acc[c].w * inv);
-  }
-  uint4* dst = reinterpret_cast<uint4*>(p.o + out * D + part * kJoinCols);
-#pragma unroll
-  for (int c = 0; c < kVec / 2; ++c) dst[c] = make_uint4(y[4 * c], y[4 * c + 1], y[4 * c + 2], y[4 * c + 3]);
-  if (part == 0 && p.lse != nullptr) p.lse[out] = L == 0.f ? -INFINITY : (M + lg2(L)) * kLn2;
+  uint2 y;
+  y.x = pack_bf16x2(acc.x * inv, acc.y * inv);
+  y.y = pack_bf16x2(acc.z * inv, acc.w * inv);
+  reinterpret_cast<uint2*>(p.o + out * D)[col] = y;
+  if (col == 0 && p.lse != nullptr) p.lse[out] = L == 0.f ? -INFINITY : (M + lg2(L)) * kLn2;
 }
 
 // ---------------------------------------------------------------------------
@@ -919,7 +891,7 @@ int pu_decode_paged_shared(const void* q, int q_dtype, const void* k_pool, const
   // units of the line are 32-bit: items times (tiles + cost)
   const long long tiles = (max_pages_per_seq * page_size + shared::BT - 1) / shared::BT + shared::kItemCost;
   const long long items = H_kv * (B * (H / H_kv) / shared::kRows + groups);
-  if (B > ptc::kMaxB || H > kMaxBH || H_kv * (D / shared::kJoinCols) > 65535 || items > 2147483647ll / tiles)
+  if (B > ptc::kMaxB || H > kMaxBH || H_kv * (D / 4 / shared::kJoinWarps) > 65535 || items > 2147483647ll / tiles)
     return pu::set_error(PU_ERR_UNSUPPORTED, "shared prefix of %lld sequences with %lld heads over %lld tokens", (long long)B, (long long)H,
                          (long long)(max_pages_per_seq * page_size));
   const shared::Layout l = shared::layout(B, H, H_kv, D, groups);
@@ -989,6 +961,7 @@ int pu_decode_paged_shared(const void* q, int q_dtype, const void* k_pool, const
 
   shared::JoinParams jp{};
   jp.desc = prm.desc;
+  jp.skip = prm.skip;
   jp.slabs = prm.slabs;
   jp.own_o = own.o32;
   jp.own_lse = own.lse;
@@ -1001,9 +974,9 @@ int pu_decode_paged_shared(const void* q, int q_dtype, const void* k_pool, const
   jp.groups = prm.groups;
   jp.grid = pu::sm_count();
   jp.o_scale = v_scale;
-  const dim3 grid((unsigned)((B * prm.group + shared::kJoinThreads - 1) / shared::kJoinThreads), (unsigned)(H_kv * (D / shared::kJoinCols)));
-  return pu::check_cuda(D == 128 ? launch_pdl(shared::join_kernel<128>, grid, dim3(shared::kJoinThreads), 0, st, jp)
-                                 : launch_pdl(shared::join_kernel<64>, grid, dim3(shared::kJoinThreads), 0, st, jp),
+  const dim3 grid((unsigned)((B * prm.group + 31) / 32), (unsigned)(H_kv * (D / 4 / shared::kJoinWarps))), block(shared::kJoinWarps * 32);
+  return pu::check_cuda(D == 128 ? launch_pdl(shared::join_kernel<128>, grid, block, 0, st, jp)
+                                 : launch_pdl(shared::join_kernel<64>, grid, block, 0, st, jp),
                         "shared prefix join launch");
 }
 

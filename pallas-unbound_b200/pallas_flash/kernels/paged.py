@@ -108,7 +108,7 @@ def paged_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     [n + 1]; without it one group is the whole batch), have the same first
     shared_lens[i] tokens, which are then read once for the group, through the
     table row of one of its sequences.  Only whole pages are shared.  A sequence
-    that holds fewer tokens than that attends those it holds; a group in which
+    that holds fewer tokens than that attends them by itself; a group in which
     none holds as many shares nothing.  The result is that of the call without
     it, up to the order of sums, and where q and the pools have different 16-bit
     types, or e4m3 pools heads of 64, it is that call."""
