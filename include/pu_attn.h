@@ -430,7 +430,7 @@ PU_API int pu_page_bounds(const void* k_pool, int kv_dtype, const int32_t* slots
  *   lens int32 [B][H_kv]: tokens in them.
  * Entries outside the pool are not chosen, and reported (detail 310).  Queries and
  * bounds must be finite for the choice to be that of the formula.
- * q [B,H,1,D] and bounds each f16 or bf16; D 64 or 128; max_pages_per_seq <= 18432;
+ * q [B,H,1,D] and bounds each f16 or bf16; D 64 or 128; max_pages_per_seq <= 24576;
  * first + last <= count.
  */
 PU_API int pu_select_pages(const void* q, int q_dtype, const void* bounds, int bounds_dtype,

@@ -72,7 +72,7 @@ __device__ __forceinline__ uint32_t pair_max(uint32_t a, uint32_t b) {
 // whole run, wherever it ends, so that one CTA reads and writes the page's bounds.  A warp takes a
 // (leader, head); where there are fewer of them than warps, warps share one.
 template <typename KVT, int D>
-__global__ void __launch_bounds__(kBoundThreads) bounds_kernel(const BoundParams p) {
+__global__ void __launch_bounds__(kBoundThreads, 3) bounds_kernel(const BoundParams p) {
   constexpr bool kF8 = sizeof(KVT) == 1;
   using B = typename std::conditional<kF8, __half, KVT>::type;     // type of the bounds
   constexpr int kLanes = D * (int)sizeof(KVT) / 16;                // lanes of a row, 16 bytes each
@@ -220,9 +220,10 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 1024;
 constexpr int kRank = kThreads;          // as many candidates are ranked against each other
-constexpr int kMaxPages = 18432;         // scores of a sequence that one CTA's shared memory holds
+constexpr int kMaxPages = 24576;         // scores of a sequence that one CTA's shared memory holds
 constexpr int kMaxCtas = 8;              // of a cluster
-constexpr int kStages = 2;               // of a warp's copies, eight pages each
+constexpr int kStages = 3;               // of a warp's copies, eight pages each
+constexpr float kBig = 0x1p125f;         // fp32 sums from here on are not used
 
 struct Params {
   const void* q;               // [B][H][D]
@@ -286,8 +287,8 @@ __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commi
 template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-__device__ __forceinline__ void st_cluster_f64(uint32_t addr, double v) {
-  asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(addr), "d"(v) : "memory");
+__device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
 __device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t v) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
@@ -296,7 +297,7 @@ __device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t v) {
 // Shared memory of the choice.
 struct Room {
   double red[2][kWarps];
-  double cand[kRank];
+  double cand[kRank];          // or floats; scores summed again
   double cut;
   int bins[kBins];
   int list[kRank];
@@ -317,49 +318,53 @@ __device__ __forceinline__ int block_sum(int x, Room& s, int warp, int lane) {
 }
 
 // The want-th largest (want >= 1) of the finite scores in [from, to), of which there are more than
-// `want`, and how many that equal it are among the first `want`.
+// `want`, and how many that equal it are among the first `want`.  Differences of scores are finite.
 //
 // The scores lie in kBins bins of equal width between the smallest and the largest (a monotone map, so no
 // rounding of it can order two scores wrongly), bins are counted from the top until the one that holds the
 // border, and its members are ranked against each other; where they are more than 256 the same is done
 // again between their own smallest and largest.
-__device__ __forceinline__ void border(const double* score, int from, int to, int want, Room& s, double* cut, int* ties) {
+template <typename S>
+__device__ __forceinline__ void border(const S* score, int from, int to, int want, Room& s, S* cut, int* ties) {
+  S(&red)[2][kWarps] = reinterpret_cast<S(&)[2][kWarps]>(s.red);
+  S* cand = reinterpret_cast<S*>(s.cand);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  double lo = INFINITY, hi = -INFINITY;
+  S lo = INFINITY, hi = -INFINITY;
   for (int i = from + tid; i < to; i += kThreads) {
-    const double x = score[i];
+    const S x = score[i];
     if (isinf(x)) continue;
-    lo = fmin(lo, x);
-    hi = fmax(hi, x);
+    lo = min(lo, x);
+    hi = max(hi, x);
   }
   while (true) {
     // smallest and largest candidate, of all threads
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) {
-      lo = fmin(lo, __shfl_xor_sync(0xffffffffu, lo, off));
-      hi = fmax(hi, __shfl_xor_sync(0xffffffffu, hi, off));
+      lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, off));
+      hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, off));
     }
     if (lane == 0) {
-      s.red[0][warp] = lo;
-      s.red[1][warp] = hi;
+      red[0][warp] = lo;
+      red[1][warp] = hi;
     }
     for (int i = tid; i < kBins; i += kThreads) s.bins[i] = 0;
     if (tid < 4) s.found[tid] = 0;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      lo = fmin(lo, s.red[0][w]);
-      hi = fmax(hi, s.red[1][w]);
+      lo = min(lo, red[0][w]);
+      hi = max(hi, red[1][w]);
     }
     if (lo == hi) {                      // equal scores: the first of them
       *cut = lo;
       *ties = want;
       break;
     }
-    const double scale = (double)(kBins - 1) / (hi - lo);
-    auto bin_of = [&](double x) { return min(kBins - 1, (int)((x - lo) * scale)); };
+    // (hi - lo is neither 0 nor infinite, so hi is never in lo's bin)
+    const S scale = (S)(kBins - 1) / (hi - lo);
+    auto bin_of = [&](S x) { return min(kBins - 1, (int)((x - lo) * scale)); };
     for (int i = from + tid; i < to; i += kThreads) {
-      const double x = score[i];
+      const S x = score[i];
       if (x >= lo && x <= hi) atomicAdd(s.bins + bin_of(x), 1);
     }
     __syncthreads();
@@ -397,17 +402,17 @@ __device__ __forceinline__ void border(const double* score, int from, int to, in
     want -= s.found[1];
     if (members <= kRank) {
       for (int i = from + tid; i < to; i += kThreads) {
-        const double x = score[i];
-        if (x >= lo && x <= hi && bin_of(x) == at) s.cand[atomicAdd(s.found + 3, 1)] = x;
+        const S x = score[i];
+        if (x >= lo && x <= hi && bin_of(x) == at) cand[atomicAdd(s.found + 3, 1)] = x;
       }
       __syncthreads();
       if (tid < members) {
         // fewer than `want` above it, at least `want` with its equals
-        const double x = s.cand[tid];
+        const S x = cand[tid];
         int above = 0, same = 0;
         for (int i = 0; i < members; ++i) {
-          above += s.cand[i] > x;
-          same += s.cand[i] == x;
+          above += cand[i] > x;
+          same += cand[i] == x;
         }
         if (above < want && above + same >= want) {
           s.cut = x;
@@ -415,17 +420,17 @@ __device__ __forceinline__ void border(const double* score, int from, int to, in
         }
       }
       __syncthreads();
-      *cut = s.cut;
+      *cut = (S)s.cut;
       *ties = s.found[1];
       break;
     }
     // again among the border's members
-    double lo2 = INFINITY, hi2 = -INFINITY;
+    S lo2 = INFINITY, hi2 = -INFINITY;
     for (int i = from + tid; i < to; i += kThreads) {
-      const double x = score[i];
+      const S x = score[i];
       if (x >= lo && x <= hi && bin_of(x) == at) {
-        lo2 = fmin(lo2, x);
-        hi2 = fmax(hi2, x);
+        lo2 = min(lo2, x);
+        hi2 = max(hi2, x);
       }
     }
     lo = lo2;
@@ -433,6 +438,58 @@ __device__ __forceinline__ void border(const double* score, int from, int to, in
     __syncthreads();
   }
   __syncthreads();                       // the room is free again
+}
+
+// The list, in the sequence's order: a run of pages a warp, counted and then written.
+template <typename S>
+__device__ __forceinline__ void write_list(const Params& p, const int32_t* table, const S* score, S cut, int ties, int live, int len, size_t row,
+                                           Room& s) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int run = ((live + kWarps - 1) / kWarps + 31) & ~31, begin = warp * run, end = min(live, begin + run);
+  int above = 0, same = 0;
+  for (int i = begin; i < end; i += 32) {
+    const S x = i + lane < end ? score[i + lane] : -INFINITY;
+    above += __popc(__ballot_sync(0xffffffffu, x > cut));
+    same += __popc(__ballot_sync(0xffffffffu, x == cut && x != -INFINITY));
+  }
+  if (lane == 0) {
+    s.sum[warp] = above;
+    s.tie[warp] = same;
+  }
+  __syncthreads();
+  int a0 = 0, t0 = 0, a1 = 0, t1 = 0;    // before this warp, and in all
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) {
+      a0 += s.sum[w];
+      t0 += s.tie[w];
+    }
+    a1 += s.sum[w];
+    t1 += s.tie[w];
+  }
+  const int chosen = min(p.count, a1 + min(ties, t1));
+  int32_t* out = p.pages + row * p.count;
+  for (int i = begin; i < end; i += 32) {
+    const S x = i + lane < end ? score[i + lane] : -INFINITY;
+    const unsigned up = __ballot_sync(0xffffffffu, x > cut), eq = __ballot_sync(0xffffffffu, x == cut && x != -INFINITY);
+    const unsigned below = (1u << lane) - 1;
+    const int nth = t0 + __popc(eq & below);             // ties before this page
+    const int place = a0 + __popc(up & below) + min(ties, nth);
+    if ((((up >> lane) & 1u) || (((eq >> lane) & 1u) && nth < ties)) && place < p.count) out[place] = table[i + lane];
+    a0 += __popc(up);
+    t0 += __popc(eq);
+  }
+  for (int i = chosen + tid; i < p.count; i += kThreads) out[i] = -1;
+  if (tid == 0) {
+    // only the sequence's last page may hold fewer tokens than a page; it is last in the list
+    int tokens = chosen << p.page_shift;
+    if (live > 0) {
+      const S x = score[live - 1];
+      const bool in = x > cut || (x == cut && x != -INFINITY && t1 - 1 < ties);
+      if (in) tokens -= (live << p.page_shift) - len;
+    }
+    p.out_lens[row] = tokens;
+  }
 }
 
 // One cluster a (sequence, K/V head): its CTAs score the pages between them and leave the scores in
@@ -445,13 +502,13 @@ __device__ __forceinline__ void border(const double* score, int from, int to, in
 // left, are summed again in fp64 from their bounds: nearly always none.
 //
 // A page's bounds of one head are 4 D bytes in one piece.  Eight lanes take a page, and each lane copies
-// the chunks that it will read itself into shared memory, eight pages a step and a step ahead: copies in
-// flight need no registers and no barrier.
+// the chunks that it will read itself into shared memory, eight pages a step and two steps ahead: copies
+// in flight need no registers and no barrier.
 template <typename QT, typename BT, int D>
 __global__ void __launch_bounds__(kThreads, 2) select_kernel(const Params p) {
   constexpr int kChunks = 2 * D / 64;    // 16-byte chunks a lane reads of a page
   extern __shared__ __align__(16) uint8_t dyn[];
-  double* s_score = reinterpret_cast<double*>(dyn);                     // [max_pages], in the first CTA
+  float* s_score = reinterpret_cast<float*>(dyn);        // [max_pages], in the first CTA
   __shared__ float s_coef[2][D];         // sums of the heads' negative and positive parts
   __shared__ double s_wide[2][D];        // the same in fp64, times 2^800
   __shared__ double s_abs[kWarps];       // parts of the sum of their magnitudes
@@ -496,14 +553,16 @@ __global__ void __launch_bounds__(kThreads, 2) select_kernel(const Params p) {
     const int steps = max(0, (end - begin + 7) >> 3);
     uint8_t* ring = dyn + p.ring + (warp * kStages * 2 * kChunks * 32 + lane) * 16;
     int pg = -1;                         // a table entry for each lane
-    uint32_t valid = 0;                  // pages of the newest step (bits 0, 1) and the one before (2, 3)
+    uint32_t valid = 0;                  // pages of the steps begun, two bits each, the newest in bits 0 and 1
+    int to_stage = 0, from_stage = 0;
     auto begin_step = [&](int k) {       // copies of pages begin + 8 k + 4 u + sub
       if ((k & 3) == 0) {
         const int i = begin + 8 * k + lane;
         pg = i < end ? table[i] : -1;
         if (i < end && (unsigned)pg >= (unsigned)p.num_pages) record_device_error(PU_ERR_INVALID_ARGUMENT, kSiteSelectPage);
       }
-      const uint32_t dst = smem_u32(ring + (k & 1) * 2 * kChunks * 512);
+      const uint32_t dst = smem_u32(ring + to_stage * 2 * kChunks * 512);
+      to_stage = to_stage + 1 == kStages ? 0 : to_stage + 1;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int entry = __shfl_sync(0xffffffffu, pg, (8 * k + 4 * u + sub) & 31);
@@ -514,8 +573,11 @@ __global__ void __launch_bounds__(kThreads, 2) select_kernel(const Params p) {
         for (int c = 0; c < kChunks; ++c) cp_async_16(dst + (u * kChunks + c) * 512, src + c * 8, ok);
       }
     };
-    if (steps > 0) begin_step(0);
-    cp_async_commit();
+    for (int k = 0; k < kStages - 1; ++k) {
+      if (k < steps) begin_step(k);
+      else valid <<= 2;
+      cp_async_commit();
+    }
     // ---- the heads' parts, while the first bounds arrive ----
     double sum = 0.;
     for (int i = tid; i < D; i += kThreads) {
@@ -554,11 +616,12 @@ __global__ void __launch_bounds__(kThreads, 2) select_kernel(const Params p) {
     const uint32_t dst = mapa_shared(s_score, 0);
     cluster_wait();
     for (int k = 0; k < steps; ++k) {
-      if (k + 1 < steps) begin_step(k + 1);
+      if (k + kStages - 1 < steps) begin_step(k + kStages - 1);
       else valid <<= 2;
       cp_async_commit();
-      cp_async_wait<1>();
-      const uint8_t* src = ring + (k & 1) * 2 * kChunks * 512;
+      cp_async_wait<kStages - 1>();
+      const uint8_t* src = ring + from_stage * 2 * kChunks * 512;
+      from_stage = from_stage + 1 == kStages ? 0 : from_stage + 1;
       float x[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -583,11 +646,11 @@ __global__ void __launch_bounds__(kThreads, 2) select_kernel(const Params p) {
       y += __shfl_xor_sync(0xffffffffu, up ? x[0] : x[1], 4);
       y += __shfl_xor_sync(0xffffffffu, y, 2);
       y += __shfl_xor_sync(0xffffffffu, y, 1);
-      // -inf marks an entry outside the pool; a sum that is not finite is summed again below
+      // -inf marks an entry outside the pool; a sum that is too large, or NaN, is summed again below
       const int i = begin + 8 * k + (up ? 4 : 0) + sub;
-      const bool ok = (valid >> (up ? 2 : 3)) & 1u;
-      if (!isfinite(y)) top = 0x7fff7fffu;
-      if ((l8 & 3) == 0 && i < end) st_cluster_f64(dst + 8u * (uint32_t)i, !ok ? -INFINITY : isfinite(y) ? (double)y : 0x1p1000);
+      const bool ok = (valid >> (2 * kStages - (up ? 2 : 1))) & 1u, usable = fabsf(y) < kBig;
+      if (!usable) top = 0x7fff7fffu;
+      if ((l8 & 3) == 0 && i < end) st_cluster_f32(dst + 4u * (uint32_t)i, !ok ? -INFINITY : usable ? y : kBig);
     }
     top = max(top >> 16, top & 0xffffu);
     top = __reduce_max_sync(0xffffffffu, top);
@@ -613,13 +676,13 @@ __global__ void __launch_bounds__(kThreads, 2) select_kernel(const Params p) {
   }
   counts = block_sum(counts, s, warp, lane);         // and the scores are visible to all
 
-  // ---- the border: every score above `cut` is kept, and the first `ties` equal to it ----
-  double cut = -INFINITY;
+  // ---- the border: every score above it is kept, and the first `ties` equal to it ----
+  float cut = -INFINITY;
   int ties = 0;
   if (!all) {
     int want = p.count - (counts & 0xffff);          // of the candidates
     if (want <= 0) {
-      cut = 0x1p1010;                    // none but those always kept
+      cut = 0x1p126f;                    // none but those always kept
     } else if (counts >> 16 > want) {
       border(s_score, from, to, want, s, &cut, &ties);
       // what the fp32 sums are off by; 2^-140: sums of subnormals
@@ -628,17 +691,17 @@ __global__ void __launch_bounds__(kThreads, 2) select_kernel(const Params p) {
       for (int w = 0; w < kWarps; ++w) e += s_abs[w];
       const float big = to_float(*reinterpret_cast<const BT*>(&top));
       e = isfinite(big) && e < 0x1p1000 ? fma(e * (double)big, 0x1p-19, 0x1p-140) : INFINITY;
-      const double sure = cut + 2. * e, none = cut - 2. * e;
+      const double sure = (double)cut + 2. * e, none = (double)cut - 2. * e;
       if (tid == 0) s.found[3] = 0;
       __syncthreads();
       counts = 0;                        // above, and near times 2^16
       for (int i = from + tid; i < to; i += kThreads) {
-        const double x = s_score[i];
+        const float x = s_score[i];
         if (x == -INFINITY) continue;
-        if (x > sure) {
+        if ((double)x > sure) {
           ++counts;
           s_score[i] = INFINITY;
-        } else if (x < none) {
+        } else if ((double)x < none) {
           s_score[i] = -INFINITY;
         } else {
           counts += 1 << 16;
@@ -653,10 +716,7 @@ __global__ void __launch_bounds__(kThreads, 2) select_kernel(const Params p) {
       ties = 0;
       if (near > want) {
         // ---- summed again in fp64, a warp a page ----
-        const bool listed = near <= kRank;
-        for (int k = listed ? warp : from + warp; k < (listed ? near : to); k += kWarps) {
-          const int i = listed ? s.list[k] : k;
-          if (isinf(s_score[i])) continue;
+        auto again = [&](int i) -> double {
           const uint4* src = bounds + ((size_t)table[i] * p.H_kv + head) * (2 * D / 8);
           double x = 0.;
           for (int c = lane; c < 2 * D / 8; c += 32) {
@@ -672,62 +732,48 @@ __global__ void __launch_bounds__(kThreads, 2) select_kernel(const Params p) {
 #pragma unroll
           for (int off = 16; off > 0; off >>= 1) x += __shfl_xor_sync(0xffffffffu, x, off);
           // finite, also for queries that are not
-          if (lane == 0) s_score[i] = x != x ? 0x1p1000 : fmin(fmax(x, -0x1p1000), 0x1p1000);
-          __syncwarp();
+          return x != x ? 0x1p1000 : fmin(fmax(x, -0x1p1000), 0x1p1000);
+        };
+        if (near <= kRank) {
+          for (int k = warp; k < near; k += kWarps) {
+            const double x = again(s.list[k]);
+            if (lane == 0) s.cand[k] = x;
+          }
+          __syncthreads();
+          if (tid < near) {
+            const double x = s.cand[tid];
+            const int i = s.list[tid];
+            int before = 0;
+            for (int j = 0; j < near; ++j) before += s.cand[j] > x || (s.cand[j] == x && s.list[j] < i);
+            s_score[i] = before < want ? INFINITY : -INFINITY;
+          }
+          __syncthreads();
+        } else {
+          // more than can be ranked against each other (equal pages, say): all scores as fp64 in the same
+          // place, which has room for them once the copies are over, and the border among those
+          double* fine = reinterpret_cast<double*>(dyn);
+          for (int base = (live - 1) / kThreads * kThreads; base >= 0; base -= kThreads) {
+            const int i = base + tid;
+            const float x = i < live ? s_score[i] : 0.f;
+            __syncthreads();
+            if (i < live) fine[i] = x;
+            __syncthreads();
+          }
+          for (int i = from + warp; i < to; i += kWarps) {
+            if (isinf(fine[i])) continue;
+            const double x = again(i);
+            if (lane == 0) fine[i] = x;
+          }
+          __syncthreads();
+          double at = 0x1p1010;
+          if (want > 0) border(fine, from, to, want, s, &at, &ties);
+          write_list<double>(p, table, fine, at, ties, live, len, (size_t)b * p.H_kv + head, s);
+          return;
         }
-        __syncthreads();
-        if (want > 0) border(s_score, from, to, want, s, &cut, &ties);
-        else cut = 0x1p1010;
       }
     }
   }
-
-  // ---- the list, in the sequence's order: a run of pages a warp, counted and then written ----
-  const int run = ((live + kWarps - 1) / kWarps + 31) & ~31, begin = warp * run, end = min(live, begin + run);
-  int above = 0, same = 0;
-  for (int i = begin; i < end; i += 32) {
-    const double x = i + lane < end ? s_score[i + lane] : -INFINITY;
-    above += __popc(__ballot_sync(0xffffffffu, x > cut));
-    same += __popc(__ballot_sync(0xffffffffu, x == cut && x != -INFINITY));
-  }
-  if (lane == 0) {
-    s.sum[warp] = above;
-    s.tie[warp] = same;
-  }
-  __syncthreads();
-  int a0 = 0, t0 = 0, a1 = 0, t1 = 0;    // before this warp, and in all
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) {
-      a0 += s.sum[w];
-      t0 += s.tie[w];
-    }
-    a1 += s.sum[w];
-    t1 += s.tie[w];
-  }
-  const int chosen = min(p.count, a1 + min(ties, t1));
-  int32_t* out = p.pages + ((size_t)b * p.H_kv + head) * p.count;
-  for (int i = begin; i < end; i += 32) {
-    const double x = i + lane < end ? s_score[i + lane] : -INFINITY;
-    const unsigned up = __ballot_sync(0xffffffffu, x > cut), eq = __ballot_sync(0xffffffffu, x == cut && x != -INFINITY);
-    const unsigned below = (1u << lane) - 1;
-    const int nth = t0 + __popc(eq & below);             // ties before this page
-    const int place = a0 + __popc(up & below) + min(ties, nth);
-    if ((((up >> lane) & 1u) || (((eq >> lane) & 1u) && nth < ties)) && place < p.count) out[place] = table[i + lane];
-    a0 += __popc(up);
-    t0 += __popc(eq);
-  }
-  for (int i = chosen + tid; i < p.count; i += kThreads) out[i] = -1;
-  if (tid == 0) {
-    // only the sequence's last page may hold fewer tokens than a page; it is last in the list
-    int tokens = chosen << p.page_shift;
-    if (live > 0) {
-      const double x = s_score[live - 1];
-      const bool in = x > cut || (x == cut && x != -INFINITY && t1 - 1 < ties);
-      if (in) tokens -= (live << p.page_shift) - len;
-    }
-    p.out_lens[(size_t)b * p.H_kv + head] = tokens;
-  }
+  write_list<float>(p, table, s_score, cut, ties, live, len, (size_t)b * p.H_kv + head, s);
 }
 
 // CTAs of a cluster: what brings the grid to about three CTAs an SM, but no more than one for 64 pages of a
@@ -741,14 +787,16 @@ inline int cluster_size(long long max_pages, long long items) {
 template <typename QT, typename BT, int D>
 int launch_select(Params p, long long items, cudaStream_t st) {
   const auto f = select_kernel<QT, BT, D>;
-  constexpr int kRing = kStages * kWarps * 32 * D;   // eight pages of 4 D bytes a warp and stage
-  p.ring = (p.max_pages * (int)sizeof(double) + 15) / 16 * 16;
-  int rc = set_max_dynamic_smem(reinterpret_cast<const void*>(f), kMaxPages * (int)sizeof(double) + kRing, "page choice shared memory");
+  // scores, and behind them the copies: eight pages of 4 D bytes a warp and stage, or as much as lets the
+  // scores be held in fp64
+  constexpr int kRing = kStages * kWarps * 32 * D;
+  p.ring = (p.max_pages * (int)sizeof(float) + 15) / 16 * 16;
+  const int rc = set_max_dynamic_smem(reinterpret_cast<const void*>(f), 2 * kMaxPages * (int)sizeof(float) + 16, "page choice shared memory");
   if (rc) return rc;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(items * p.ctas));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = (size_t)(p.ring + kRing);
+  cfg.dynamicSmemBytes = (size_t)(p.ring + std::max(kRing, p.ring));
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -794,8 +842,8 @@ extern "C" int pu_page_bounds(const void* k_pool, int kv_dtype, const int32_t* s
   p.page_shift = shift;
   p.T = num_tokens;
   // Small batches are spread out: eight single tokens and one head a CTA are a warp's row each.
-  // Larger ones share the reads of the slots over as many heads as leave four CTAs an SM.
-  const long long room = 4ll * pu::sm_count();
+  // Larger ones share the reads of the slots over as many heads as leave three CTAs an SM, all of them resident.
+  const long long room = 3ll * pu::sm_count();
   p.chunk = (num_tokens + 7) / 8 * H_kv <= room ? 8 : 32;
   p.heads = (int)std::min<long long>(H_kv, std::max<long long>(1, (num_tokens + p.chunk - 1) / p.chunk * H_kv / room));
   p.heads = (int)((H_kv + (H_kv + p.heads - 1) / p.heads - 1) / ((H_kv + p.heads - 1) / p.heads));   // as evenly

@@ -171,6 +171,10 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
     (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+# the current device's index, without the public call's checks
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 class on_device:
     """Makes `device` current where it is not and gives the handle of its
     current stream: `with on_device(t.device) as stream`."""
@@ -181,7 +185,7 @@ class on_device:
         self.index = device.index
 
     def __enter__(self) -> int:
-        now = torch.cuda.current_device()
+        now = _current_device()
         if now == self.index:
             self.before = None
         else:

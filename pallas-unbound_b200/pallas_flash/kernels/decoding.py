@@ -60,6 +60,8 @@ _FP8 = getattr(torch, "float8_e4m3fn", None)
 _DT_KV = {**_DT, **({_FP8: _lib.PU_DTYPE_FP8_E4M3} if _FP8 is not None else {})}
 
 
+_is_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", None) or torch.cuda.is_current_stream_capturing
+
 _paged_decode = None     # kernels.paged.paged_decode, which imports this module
 
 
@@ -75,8 +77,8 @@ class DecodeWorkspace:
     @staticmethod
     def _capturing(device: torch.device) -> bool:
         """Whether `device`'s current stream, not the current device's, is being captured."""
-        if torch.cuda.current_device() == device.index:
-            return torch.cuda.is_current_stream_capturing()
+        if _lib._current_device() == device.index:
+            return _is_capturing()
         with torch.cuda.device(device):
             return torch.cuda.is_current_stream_capturing()
 

@@ -52,22 +52,23 @@ __all__ = ["PageAllocator", "PagedKVCache", "DevicePagedKVCache", "AppendPlan", 
 
 def _check_pool(k_pool: torch.Tensor, v_pool: torch.Tensor, page_table: torch.Tensor,
                 kv_lens: torch.Tensor, kinds=_DT):
-    if k_pool.shape != v_pool.shape or k_pool.dim() != 4:
+    shape, kind, rows = k_pool.shape, k_pool.dtype, page_table.shape
+    if shape != v_pool.shape or len(shape) != 4:
         raise ValueError("k_pool and v_pool must both be [num_pages, H, page_size, D]")
-    if k_pool.dtype != v_pool.dtype or k_pool.dtype not in kinds:
+    if kind != v_pool.dtype or kind not in kinds:
         raise ValueError("pools must share one dtype, fp16 or bf16" + (" or fp8 (e4m3)" if kinds is _DT_KV else ""))
-    if page_table.dtype == torch.int32 and page_table.dim() == 3 and kinds is _DT_KV:
-        if page_table.shape[1] != k_pool.shape[1]:
-            raise ValueError(f"page lists of each K/V head must be int32 [B, {k_pool.shape[1]}, pages]")
-        if kv_lens.dtype != torch.int32 or kv_lens.shape != page_table.shape[:2]:
+    if len(rows) == 3 and kinds is _DT_KV and page_table.dtype == torch.int32:
+        if rows[1] != shape[1]:
+            raise ValueError(f"page lists of each K/V head must be int32 [B, {shape[1]}, pages]")
+        if kv_lens.dtype != torch.int32 or kv_lens.shape != rows[:2]:
             raise ValueError("kv_lens of page lists must be int32 [B, H_kv]")
     else:
-        if page_table.dtype != torch.int32 or page_table.dim() != 2:
+        if page_table.dtype != torch.int32 or len(rows) != 2:
             raise ValueError("page_table must be int32 [B, max_pages_per_seq]")
-        if kv_lens.dtype != torch.int32 or kv_lens.numel() != page_table.shape[0]:
+        if kv_lens.dtype != torch.int32 or kv_lens.numel() != rows[0]:
             raise ValueError("kv_lens must be int32 [B]")
-    dev = k_pool.device
-    if not (k_pool.is_cuda and v_pool.device == dev and page_table.device == dev and kv_lens.device == dev
+    at = k_pool.get_device()             # -1 on the host
+    if not (at >= 0 and v_pool.get_device() == at and page_table.get_device() == at and kv_lens.get_device() == at
             and k_pool.is_contiguous() and v_pool.is_contiguous() and page_table.is_contiguous()
             and kv_lens.is_contiguous()):
         raise ValueError("pools, page table and lengths must be contiguous CUDA tensors on one device")
@@ -114,30 +115,32 @@ def paged_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     types, or e4m3 pools heads of 64, it is that call."""
     _check_pool(k_pool, v_pool, page_table, kv_lens, _DT_KV)
     P, H_kv, page_size, D = k_pool.shape
-    by_head = page_table.dim() == 3
-    B, max_pages = page_table.shape[0], page_table.shape[-1]
-    H = q.shape[1] if q.dim() == 4 else 0
-    if q.shape != (B, H, 1, D) or H == 0 or H_kv == 0 or H % H_kv or q.dtype not in _DT or q.device != k_pool.device:
-        raise ValueError(f"q must be fp16/bf16 CUDA [{B}, multiple of {H_kv}, 1, {D}] on {k_pool.device}")
+    rows = page_table.shape
+    by_head = len(rows) == 3
+    B, max_pages = rows[0], rows[-1]
+    qs, dev = q.shape, k_pool.device
+    H = qs[1] if len(qs) == 4 else 0
+    if qs != (B, H, 1, D) or H == 0 or H_kv == 0 or H % H_kv or q.dtype not in _DT or q.device != dev:
+        raise ValueError(f"q must be fp16/bf16 CUDA [{B}, multiple of {H_kv}, 1, {D}] on {dev}")
     if shared_lens is not None:
-        _check_shared(shared_lens, shared_groups, by_head, q.device)
+        _check_shared(shared_lens, shared_groups, by_head, dev)
     elif shared_groups is not None:
         raise ValueError("shared_groups without shared_lens")
-    q = q.contiguous()
+    if not q.is_contiguous():
+        q = q.contiguous()
     if q.data_ptr() % 16:
         q = q.clone()
     if sm_scale is None:
         sm_scale = 1.0 / math.sqrt(D)
     lib = _lib.lib()
-    with _lib.on_device(q.device) as stream:
+    with _lib.on_device(dev) as stream:
         o = torch.empty_like(q, dtype=torch.bfloat16)
-        lse = torch.empty(B, H, dtype=torch.float32, device=q.device)
+        lse = torch.empty((B, H), dtype=torch.float32, device=dev)
         if B == 0:
             return (o, lse) if return_lse else o
         if shared_lens is not None and (k_pool.dtype == q.dtype or (D == 128 and k_pool.dtype not in _DT)):
             groups = shared_lens.numel()
-            ws = DecodeWorkspace.get(q.device, _shared_bytes(q.device.index, B, H, H_kv, groups, D),
-                                     _cta_counters(q.device.index))
+            ws = DecodeWorkspace.get(dev, _shared_bytes(dev.index, B, H, H_kv, groups, D), _cta_counters(dev.index))
             _lib.check(lib.pu_decode_paged_shared(
                 q.data_ptr(), _DT[q.dtype], k_pool.data_ptr(), v_pool.data_ptr(), _DT_KV[k_pool.dtype],
                 page_table.data_ptr(), max_pages, P, page_size, kv_lens.data_ptr(), shared_lens.data_ptr(),
@@ -146,7 +149,7 @@ def paged_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
                 stream), "pu_decode_paged_shared")
         elif not by_head and H == H_kv and k_pool.dtype in _DT and k_scale == 1.0 and v_scale == 1.0:
             need = int(lib.pu_decode_paged_workspace_size(B, H, max_pages, page_size, D))
-            ws = DecodeWorkspace.get(q.device, need, 4 * B * H)
+            ws = DecodeWorkspace.get(dev, need, 4 * B * H)
             _lib.check(lib.pu_decode_paged(q.data_ptr(), _DT[q.dtype], k_pool.data_ptr(),
                                            v_pool.data_ptr(), _DT[k_pool.dtype], page_table.data_ptr(),
                                            max_pages, P, page_size, kv_lens.data_ptr(), o.data_ptr(),
@@ -154,8 +157,8 @@ def paged_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
                                            float(sm_scale), stream), "pu_decode_paged")
         else:
             # a counter for each CTA (one an SM), or in the query-head kernel for each head
-            ws = DecodeWorkspace.get(q.device, _gqa_bytes(q.device.index, B, H, H_kv, max_pages, page_size, D),
-                                     max(4 * B * H, _cta_counters(q.device.index)))
+            ws = DecodeWorkspace.get(dev, _gqa_bytes(dev.index, B, H, H_kv, max_pages, page_size, D),
+                                     max(4 * B * H, _cta_counters(dev.index)))
             call = lib.pu_decode_paged_heads if by_head else lib.pu_decode_paged_gqa
             _lib.check(call(q.data_ptr(), _DT[q.dtype], k_pool.data_ptr(), v_pool.data_ptr(), _DT_KV[k_pool.dtype],
                             page_table.data_ptr(), max_pages, P, page_size, kv_lens.data_ptr(), o.data_ptr(),
@@ -196,13 +199,13 @@ def empty_bounds(k_pool: torch.Tensor) -> torch.Tensor:
                        device=k_pool.device)
 
 
-def _check_bounds(bounds: torch.Tensor):
-    if bounds.dim() != 4 or bounds.shape[2] != 2 or bounds.dtype not in _DT:
+def _check_bounds(bounds: torch.Tensor, shape):
+    if len(shape) != 4 or shape[2] != 2 or bounds.dtype not in _DT:
         raise ValueError("bounds must be fp16/bf16 [num_pages, H_kv, 2, D]")
-    if not bounds.is_cuda or not bounds.is_contiguous():
+    if shape[3] != 128 and shape[3] != 64:
+        raise ValueError(f"page bounds of head size {shape[3]} (supported: 64, 128)")
+    if bounds.get_device() < 0 or not bounds.is_contiguous():
         raise ValueError("bounds must be a contiguous CUDA tensor")
-    if bounds.shape[3] not in (64, 128):
-        raise ValueError(f"page bounds of head size {bounds.shape[3]} (supported: 64, 128)")
 
 
 def page_bounds(k_pool: torch.Tensor, slots: torch.Tensor, bounds: torch.Tensor) -> None:
@@ -214,21 +217,23 @@ def page_bounds(k_pool: torch.Tensor, slots: torch.Tensor, bounds: torch.Tensor)
     and maximum of the keys in these rows, and of what it was where the page's row 0
     is not among them.  A NaN makes its element's bounds NaN.  A slot past the pool is
     reported (device_status detail 309) and left out."""
-    _check_bounds(bounds)
-    P, H_kv, _, D = bounds.shape
-    if k_pool.dim() != 4 or (k_pool.shape[0], k_pool.shape[1], k_pool.shape[3]) != (P, H_kv, D) or k_pool.dtype not in _DT_KV:
+    shape, pool, kind = bounds.shape, k_pool.shape, k_pool.dtype
+    _check_bounds(bounds, shape)
+    P, H_kv, _, D = shape
+    if len(pool) != 4 or pool[0] != P or pool[1] != H_kv or pool[3] != D or kind not in _DT_KV:
         raise ValueError(f"k_pool must be fp16, bf16 or fp8 (e4m3) [{P}, {H_kv}, page_size, {D}]")
-    if bounds.dtype != (k_pool.dtype if k_pool.dtype in _DT else torch.float16):
+    if bounds.dtype != (kind if kind in _DT else torch.float16):
         raise ValueError("bounds must have the pool's 16-bit dtype, fp16 for an fp8 pool")
     if slots.dtype != torch.int32 or slots.dim() != 1 or not slots.is_contiguous():
         raise ValueError("slots must be a contiguous int32 [T]")
-    if k_pool.device != bounds.device or slots.device != bounds.device or not k_pool.is_contiguous():
+    at = bounds.get_device()
+    if k_pool.get_device() != at or slots.get_device() != at or not k_pool.is_contiguous():
         raise ValueError("pool, slots and bounds must be contiguous CUDA tensors on one device")
     if (k_pool.requires_grad or bounds.requires_grad) and torch.is_grad_enabled():
         raise ValueError("page_bounds writes a cache's bounds and has no gradient")
     with _lib.on_device(bounds.device) as stream:
-        _lib.check(_lib.lib().pu_page_bounds(k_pool.data_ptr(), _DT_KV[k_pool.dtype], slots.data_ptr(), bounds.data_ptr(),
-                                             P, k_pool.shape[2], H_kv, D, slots.numel(), stream), "pu_page_bounds")
+        _lib.check(_lib.lib().pu_page_bounds(k_pool.data_ptr(), _DT_KV[kind], slots.data_ptr(), bounds.data_ptr(),
+                                             P, pool[2], H_kv, D, slots.numel(), stream), "pu_page_bounds")
 
 
 def select_pages(q: torch.Tensor, bounds: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor, count: int, *,
@@ -244,33 +249,35 @@ def select_pages(q: torch.Tensor, bounds: torch.Tensor, page_table: torch.Tensor
     chosen and reported (device_status detail 310); queries and bounds are finite.
 
     q [B,H,1,D] fp16/bf16, bounds of `page_bounds`, page_table int32
-    [B,max_pages_per_seq] (up to 18432), kv_lens int32 [B].  The scores' scale and
+    [B,max_pages_per_seq] (up to 24576), kv_lens int32 [B].  The scores' scale and
     the scale of an fp8 pool change nothing.  The result goes into
     `paged_decode(q, k_pool, v_pool, chosen.pages, chosen.lens)`."""
-    _check_bounds(bounds)
-    P, H_kv, _, D = bounds.shape
-    dev = bounds.device
-    if page_table.dtype != torch.int32 or page_table.dim() != 2:
+    shape, rows, qs, kind = bounds.shape, page_table.shape, q.shape, q.dtype
+    _check_bounds(bounds, shape)
+    P, H_kv, _, D = shape
+    if page_table.dtype != torch.int32 or len(rows) != 2:
         raise ValueError("page_table must be int32 [B, max_pages_per_seq]")
-    B, max_pages = page_table.shape
+    B, max_pages = rows
     if kv_lens.dtype != torch.int32 or kv_lens.shape != (B,):
         raise ValueError(f"kv_lens must be int32 [{B}]")
-    H = q.shape[1] if q.dim() == 4 else 0
-    if q.shape != (B, H, 1, D) or H == 0 or H_kv == 0 or H % H_kv or q.dtype not in _DT or q.device != dev:
+    dev, at = bounds.device, bounds.get_device()
+    H = qs[1] if len(qs) == 4 else 0
+    if qs != (B, H, 1, D) or H == 0 or H_kv == 0 or H % H_kv or kind not in _DT or q.get_device() != at:
         raise ValueError(f"q must be fp16/bf16 CUDA [{B}, multiple of {H_kv}, 1, {D}] on {dev}")
-    if page_table.device != dev or kv_lens.device != dev or not page_table.is_contiguous() or not kv_lens.is_contiguous():
+    if page_table.get_device() != at or kv_lens.get_device() != at or not page_table.is_contiguous() \
+            or not kv_lens.is_contiguous():
         raise ValueError("page table and lengths must be contiguous and on the bounds' device")
-    count, first, last = int(count), int(first), int(last)
     if count < 1 or first < 0 or last < 0 or first + last > count:
         raise ValueError(f"{first} first and {last} last of {count} pages")
-    q = q.contiguous()
+    if not q.is_contiguous():
+        q = q.contiguous()
     with _lib.on_device(dev) as stream:
-        pages = torch.empty(B, H_kv, count, dtype=torch.int32, device=dev)
-        lens = torch.empty(B, H_kv, dtype=torch.int32, device=dev)
+        pages = torch.empty((B, H_kv, count), dtype=torch.int32, device=dev)
+        lens = torch.empty((B, H_kv), dtype=torch.int32, device=dev)
         if B:
             _lib.check(_lib.lib().pu_select_pages(
-                q.data_ptr(), _DT[q.dtype], bounds.data_ptr(), _DT[bounds.dtype], page_table.data_ptr(), max_pages, P,
-                int(page_size), kv_lens.data_ptr(), pages.data_ptr(), lens.data_ptr(), count, first, last, B, H, H_kv, D,
+                q.data_ptr(), _DT[kind], bounds.data_ptr(), _DT[bounds.dtype], page_table.data_ptr(), max_pages, P,
+                page_size, kv_lens.data_ptr(), pages.data_ptr(), lens.data_ptr(), count, first, last, B, H, H_kv, D,
                 stream), "pu_select_pages")
     return PageSelection(pages, lens)
 

@@ -175,7 +175,7 @@ def test_choice(mods, H, H_kv, D, page, qdt, bdt, count, first, last):
     assert _lib.device_status() == (0, 0)
 
 
-@pytest.mark.parametrize("pages,width", [(1, 1), (63, 64), (65, 65), (129, 200), (700, 700), (5000, 6000), (18432, 18432)])
+@pytest.mark.parametrize("pages,width", [(1, 1), (63, 64), (65, 65), (129, 200), (700, 700), (5000, 6000), (24576, 24576)])
 def test_choice_widths(mods, pages, width):
     """One CTA to a full cluster, few pages to as many as a call takes."""
     _lib, dec, paged = mods
@@ -426,7 +426,7 @@ def test_refusals(mods):
         with pytest.raises(_lib.PuError):
             paged.select_pages(q, bounds, table, n, **kw)
     with pytest.raises(_lib.PuError):
-        paged.select_pages(q, bounds, torch.zeros((2, 18433), dtype=torch.int32, device="cuda"), n, 2, page_size=16)
+        paged.select_pages(q, bounds, torch.zeros((2, 24577), dtype=torch.int32, device="cuda"), n, 2, page_size=16)
     slots = ints([0, 1])
     for a in [(k, slots.long(), bounds), (k, slots, bounds.half()), (k[:4], slots, bounds), (k.float(), slots, bounds), (k.transpose(0, 1), slots, bounds),
               (k, slots.cpu(), bounds), (k, ints([0, 1, 2, 3])[::2], bounds), (k.to(FP8), slots, bounds)]:
