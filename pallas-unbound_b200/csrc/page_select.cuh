@@ -222,8 +222,9 @@ constexpr int kBins = 1024;
 constexpr int kRank = kThreads;          // as many candidates are ranked against each other
 constexpr int kMaxPages = 24576;         // scores of a sequence that one CTA's shared memory holds
 constexpr int kMaxCtas = 8;              // of a cluster
-constexpr int kStages = 3;               // of a warp's copies, eight pages each
+constexpr int kFew = 3, kMany = 6;       // stages of a warp's copies, eight pages each
 constexpr float kBig = 0x1p125f;         // fp32 sums from here on are not used
+constexpr uint32_t kOutside = 0x10000u;  // a warp has seen a table entry outside the pool
 
 struct Params {
   const void* q;               // [B][H][D]
@@ -237,7 +238,7 @@ struct Params {
   int count, first, last;
   int ctas;                    // of a cluster
   int by_length;               // clusters take the longest sequences first
-  int ring;                    // first byte of the copies, behind the scores
+  int ring, stages;            // first byte of the copies, behind the scores; kFew or kMany
   int B;
 };
 
@@ -271,14 +272,6 @@ __device__ __forceinline__ uint64_t pair_to_f2<__half>(uint32_t w) {
   return f2_pack(f.x, f.y);
 }
 
-// The larger magnitude, element by element; a NaN stays one.
-template <typename T>
-__device__ __forceinline__ uint32_t pair_top(uint32_t top, uint32_t w) {
-  using V = typename Pair<T>::V;
-  const V r = __hmax2_nan(*reinterpret_cast<const V*>(&top), __habs2(*reinterpret_cast<const V*>(&w)));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-
 // 16 bytes from global to shared memory, zeros unless `ok`.
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool ok) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
@@ -296,13 +289,15 @@ __device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t v) {
 
 // Shared memory of the choice.
 struct Room {
+  double cand[kRank];          // scores summed again
   double red[2][kWarps];
-  double cand[kRank];          // or floats; scores summed again
   double cut;
   int bins[kBins];
   int list[kRank];
+  float near[kRank];           // their fp32 sums
   int sum[kWarps], tie[kWarps], scan[kWarps];
   int found[4];                // border bin, members above it, its members, members listed
+  float edge;
 };
 
 // Sum over the block (every thread gets it).
@@ -317,102 +312,136 @@ __device__ __forceinline__ int block_sum(int x, Room& s, int warp, int lane) {
   return all;
 }
 
-// The want-th largest (want >= 1) of the finite scores in [from, to), of which there are more than
-// `want`, and how many that equal it are among the first `want`.  Differences of scores are finite.
-//
-// The scores lie in kBins bins of equal width between the smallest and the largest (a monotone map, so no
-// rounding of it can order two scores wrongly), bins are counted from the top until the one that holds the
-// border, and its members are ranked against each other; where they are more than 256 the same is done
-// again between their own smallest and largest.
-template <typename S>
-__device__ __forceinline__ void border(const S* score, int from, int to, int want, Room& s, S* cut, int* ties) {
-  S(&red)[2][kWarps] = reinterpret_cast<S(&)[2][kWarps]>(s.red);
-  S* cand = reinterpret_cast<S*>(s.cand);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  S lo = INFINITY, hi = -INFINITY;
-  for (int i = from + tid; i < to; i += kThreads) {
-    const S x = score[i];
-    if (isinf(x)) continue;
-    lo = min(lo, x);
-    hi = max(hi, x);
+// Calls f(i, score[i]) for this thread's part of [from, to): four reads at a time, which a loop with
+// atomics or stores between its reads would take one after the other.
+template <typename S, typename F>
+__device__ __forceinline__ void each(const S* score, int from, int to, F f) {
+  constexpr int kAhead = 4;
+  int i = from + (int)threadIdx.x;
+  for (; i + (kAhead - 1) * kThreads < to; i += kAhead * kThreads) {
+    S x[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) x[u] = score[i + u * kThreads];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) f(i + u * kThreads, x[u]);
   }
+#pragma unroll 1
+  for (; i < to; i += kThreads) f(i, score[i]);
+}
+
+// Smallest and largest of all threads' lo and hi.
+template <typename S>
+__device__ __forceinline__ void block_range(S& lo, S& hi, Room& s, int warp, int lane) {
+  S(&red)[2][kWarps] = reinterpret_cast<S(&)[2][kWarps]>(s.red);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, off));
+    hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, off));
+  }
+  if (lane == 0) {
+    red[0][warp] = lo;
+    red[1][warp] = hi;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    lo = min(lo, red[0][w]);
+    hi = max(hi, red[1][w]);
+  }
+}
+
+// Counts the scores in [lo, hi] (lo < hi) in kBins bins of equal width and finds the one that holds the
+// want-th largest: s.found = {bin, members of the bins above, its members, 0}.  The map to bins is
+// monotone, so no rounding of it orders two scores wrongly.
+template <typename S>
+struct Bins {
+  S lo, scale;
+  // (hi - lo is neither 0 nor infinite, so hi is never in lo's bin)
+  __device__ __forceinline__ Bins(S lo_, S hi) : lo(lo_), scale((S)(kBins - 1) / (hi - lo_)) {}
+  __device__ __forceinline__ int of(S x) const { return min(kBins - 1, (int)((x - lo) * scale)); }
+};
+
+template <typename S>
+__device__ __forceinline__ void find_bin(const S* score, int from, int to, S lo, S hi, const Bins<S>& bins, int want, Room& s) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  for (int i = tid; i < kBins; i += kThreads) s.bins[i] = 0;
+  __syncthreads();
+  each(score, from, to, [&](int, S x) {
+    if (x >= lo && x <= hi) atomicAdd(s.bins + bins.of(x), 1);
+  });
+  __syncthreads();
+  // a thread's four bins, counted from the top
+  constexpr int kPer = kBins / kThreads;
+  const int top = kBins - 1 - tid * kPer;
+  int c[kPer], mine = 0;
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    c[k] = s.bins[top - k];
+    mine += c[k];
+  }
+  int before = mine;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, before, off);
+    if (lane >= off) before += y;
+  }
+  if (lane == 31) s.scan[warp] = before;
+  if (tid == 0) s.found[3] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) before += w < warp ? s.scan[w] : 0;
+  before -= mine;                        // candidates in the bins above this thread's
+  if (before < want && before + mine >= want) {
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      if (before < want && before + c[k] >= want) {
+        s.found[0] = top - k;
+        s.found[1] = before;
+        s.found[2] = c[k];
+      }
+      before += c[k];
+    }
+  }
+  __syncthreads();
+}
+
+// The want-th largest (want >= 1) of the finite scores in [from, to), of which there are more than `want`,
+// and how many that equal it are among the first `want`.  Bins, then the border bin's members are ranked
+// against each other; where they are more than 256 the same is done again between their own smallest and
+// largest.
+__device__ __forceinline__ void border(const double* score, int from, int to, int want, Room& s, double* cut, int* ties) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  double lo = INFINITY, hi = -INFINITY;
+  each(score, from, to, [&](int, double x) {
+    if (!isinf(x)) {
+      lo = min(lo, x);
+      hi = max(hi, x);
+    }
+  });
   while (true) {
-    // smallest and largest candidate, of all threads
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-      lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, off));
-      hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, off));
-    }
-    if (lane == 0) {
-      red[0][warp] = lo;
-      red[1][warp] = hi;
-    }
-    for (int i = tid; i < kBins; i += kThreads) s.bins[i] = 0;
-    if (tid < 4) s.found[tid] = 0;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      lo = min(lo, red[0][w]);
-      hi = max(hi, red[1][w]);
-    }
+    block_range(lo, hi, s, warp, lane);
     if (lo == hi) {                      // equal scores: the first of them
       *cut = lo;
       *ties = want;
       break;
     }
-    // (hi - lo is neither 0 nor infinite, so hi is never in lo's bin)
-    const S scale = (S)(kBins - 1) / (hi - lo);
-    auto bin_of = [&](S x) { return min(kBins - 1, (int)((x - lo) * scale)); };
-    for (int i = from + tid; i < to; i += kThreads) {
-      const S x = score[i];
-      if (x >= lo && x <= hi) atomicAdd(s.bins + bin_of(x), 1);
-    }
-    __syncthreads();
-    // a thread's four bins, counted from the top
-    constexpr int kPer = kBins / kThreads;
-    const int top = kBins - 1 - tid * kPer;
-    int mine = 0;
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) mine += s.bins[top - k];
-    int before = mine;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, before, off);
-      if (lane >= off) before += y;
-    }
-    if (lane == 31) s.scan[warp] = before;
-    __syncthreads();
-    for (int w = 0; w < warp; ++w) before += s.scan[w];
-    before -= mine;                      // candidates in the bins above this thread's
-    if (before < want && before + mine >= want) {
-      int at = before;
-#pragma unroll
-      for (int k = 0; k < kPer; ++k) {
-        const int c = s.bins[top - k];
-        if (at < want && at + c >= want) {
-          s.found[0] = top - k;
-          s.found[1] = at;
-          s.found[2] = c;
-        }
-        at += c;
-      }
-    }
-    __syncthreads();
+    const Bins<double> bins(lo, hi);
+    find_bin(score, from, to, lo, hi, bins, want, s);
     const int at = s.found[0], members = s.found[2];
     want -= s.found[1];
+    __syncthreads();
     if (members <= kRank) {
-      for (int i = from + tid; i < to; i += kThreads) {
-        const S x = score[i];
-        if (x >= lo && x <= hi && bin_of(x) == at) cand[atomicAdd(s.found + 3, 1)] = x;
-      }
+      each(score, from, to, [&](int, double x) {
+        if (x >= lo && x <= hi && bins.of(x) == at) s.cand[atomicAdd(s.found + 3, 1)] = x;
+      });
       __syncthreads();
       if (tid < members) {
         // fewer than `want` above it, at least `want` with its equals
-        const S x = cand[tid];
+        const double x = s.cand[tid];
         int above = 0, same = 0;
         for (int i = 0; i < members; ++i) {
-          above += cand[i] > x;
-          same += cand[i] == x;
+          above += s.cand[i] > x;
+          same += s.cand[i] == x;
         }
         if (above < want && above + same >= want) {
           s.cut = x;
@@ -420,19 +449,18 @@ __device__ __forceinline__ void border(const S* score, int from, int to, int wan
         }
       }
       __syncthreads();
-      *cut = (S)s.cut;
+      *cut = s.cut;
       *ties = s.found[1];
       break;
     }
     // again among the border's members
-    S lo2 = INFINITY, hi2 = -INFINITY;
-    for (int i = from + tid; i < to; i += kThreads) {
-      const S x = score[i];
-      if (x >= lo && x <= hi && bin_of(x) == at) {
+    double lo2 = INFINITY, hi2 = -INFINITY;
+    each(score, from, to, [&](int, double x) {
+      if (x >= lo && x <= hi && bins.of(x) == at) {
         lo2 = min(lo2, x);
         hi2 = max(hi2, x);
       }
-    }
+    });
     lo = lo2;
     hi = hi2;
     __syncthreads();
@@ -440,17 +468,27 @@ __device__ __forceinline__ void border(const S* score, int from, int to, int wan
   __syncthreads();                       // the room is free again
 }
 
-// The list, in the sequence's order: a run of pages a warp, counted and then written.
+// The list, in the sequence's order: pages above `cut`, and the first `ties` equal to it (a cut of -inf has
+// none).  A run of pages a warp, counted and then written.
 template <typename S>
 __device__ __forceinline__ void write_list(const Params& p, const int32_t* table, const S* score, S cut, int ties, int live, int len, size_t row,
                                            Room& s) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int run = ((live + kWarps - 1) / kWarps + 31) & ~31, begin = warp * run, end = min(live, begin + run);
+  constexpr int kAhead = 4;              // reads of 32 scores at a time
+  S x[kAhead];
+  auto load = [&](int base) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) x[u] = base + u * 32 + lane < end ? score[base + u * 32 + lane] : (S)-INFINITY;
+  };
   int above = 0, same = 0;
-  for (int i = begin; i < end; i += 32) {
-    const S x = i + lane < end ? score[i + lane] : -INFINITY;
-    above += __popc(__ballot_sync(0xffffffffu, x > cut));
-    same += __popc(__ballot_sync(0xffffffffu, x == cut && x != -INFINITY));
+  for (int base = begin; base < end; base += kAhead * 32) {
+    load(base);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      above += __popc(__ballot_sync(0xffffffffu, x[u] > cut));
+      if (ties > 0) same += __popc(__ballot_sync(0xffffffffu, x[u] == cut));
+    }
   }
   if (lane == 0) {
     s.sum[warp] = above;
@@ -469,24 +507,32 @@ __device__ __forceinline__ void write_list(const Params& p, const int32_t* table
   }
   const int chosen = min(p.count, a1 + min(ties, t1));
   int32_t* out = p.pages + row * p.count;
-  for (int i = begin; i < end; i += 32) {
-    const S x = i + lane < end ? score[i + lane] : -INFINITY;
-    const unsigned up = __ballot_sync(0xffffffffu, x > cut), eq = __ballot_sync(0xffffffffu, x == cut && x != -INFINITY);
-    const unsigned below = (1u << lane) - 1;
-    const int nth = t0 + __popc(eq & below);             // ties before this page
-    const int place = a0 + __popc(up & below) + min(ties, nth);
-    if ((((up >> lane) & 1u) || (((eq >> lane) & 1u) && nth < ties)) && place < p.count) out[place] = table[i + lane];
-    a0 += __popc(up);
-    t0 += __popc(eq);
+  for (int base = begin; base < end; base += kAhead * 32) {
+    if (run > kAhead * 32) load(base);   // otherwise they are still there
+    int32_t entry[kAhead];
+    int place[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const unsigned up = __ballot_sync(0xffffffffu, x[u] > cut), eq = ties > 0 ? __ballot_sync(0xffffffffu, x[u] == cut) : 0u;
+      const unsigned below = (1u << lane) - 1;
+      const int nth = t0 + __popc(eq & below);           // ties before this page
+      const bool in = ((up >> lane) & 1u) || (((eq >> lane) & 1u) && nth < ties);
+      place[u] = in ? a0 + __popc(up & below) + min(ties, nth) : p.count;
+      entry[u] = place[u] < p.count ? table[base + u * 32 + lane] : 0;
+      a0 += __popc(up);
+      t0 += __popc(eq);
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (place[u] < p.count) out[place[u]] = entry[u];
   }
   for (int i = chosen + tid; i < p.count; i += kThreads) out[i] = -1;
   if (tid == 0) {
     // only the sequence's last page may hold fewer tokens than a page; it is last in the list
     int tokens = chosen << p.page_shift;
     if (live > 0) {
-      const S x = score[live - 1];
-      const bool in = x > cut || (x == cut && x != -INFINITY && t1 - 1 < ties);
-      if (in) tokens -= (live << p.page_shift) - len;
+      const S y = score[live - 1];
+      if (y > cut || (y == cut && t1 - 1 < ties)) tokens -= (live << p.page_shift) - len;
     }
     p.out_lens[row] = tokens;
   }
@@ -551,31 +597,32 @@ __global__ void __launch_bounds__(kThreads, 2) select_kernel(const Params p) {
     const int workers = ctas * kWarps, per = ((to - from + workers - 1) / workers + 7) & ~7;
     const int begin = from + (rank * kWarps + warp) * per, end = min(to, begin + per);
     const int steps = max(0, (end - begin + 7) >> 3);
-    uint8_t* ring = dyn + p.ring + (warp * kStages * 2 * kChunks * 32 + lane) * 16;
-    int pg = -1;                         // a table entry for each lane
-    uint32_t valid = 0;                  // pages of the steps begun, two bits each, the newest in bits 0 and 1
+    uint8_t* ring = dyn + p.ring + (warp * p.stages * 2 * kChunks * 32 + lane) * 16;
+    int row = -1;                        // of a table entry for each lane: its bounds' place; negative: not in the pool
+    bool outside = false;                // the warp has seen such an entry
     int to_stage = 0, from_stage = 0;
     auto begin_step = [&](int k) {       // copies of pages begin + 8 k + 4 u + sub
       if ((k & 3) == 0) {
-        const int i = begin + 8 * k + lane;
-        pg = i < end ? table[i] : -1;
-        if (i < end && (unsigned)pg >= (unsigned)p.num_pages) record_device_error(PU_ERR_INVALID_ARGUMENT, kSiteSelectPage);
+        const int i = begin + 8 * k + lane, pg = i < end ? table[i] : 0;
+        const bool bad = i < end && (unsigned)pg >= (unsigned)p.num_pages;
+        row = bad || i >= end ? -1 : pg * p.H_kv + head;
+        if (__any_sync(0xffffffffu, bad)) {
+          if (bad) record_device_error(PU_ERR_INVALID_ARGUMENT, kSiteSelectPage);
+          outside = true;
+        }
       }
       const uint32_t dst = smem_u32(ring + to_stage * 2 * kChunks * 512);
-      to_stage = to_stage + 1 == kStages ? 0 : to_stage + 1;
+      to_stage = to_stage + 1 == p.stages ? 0 : to_stage + 1;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const int entry = __shfl_sync(0xffffffffu, pg, (8 * k + 4 * u + sub) & 31);
-        const bool ok = (unsigned)entry < (unsigned)p.num_pages;
-        valid = valid << 1 | (ok ? 1u : 0u);
-        const uint4* src = bounds + ((size_t)(ok ? entry : 0) * p.H_kv + head) * (2 * D / 8) + l8;
+        const int at = __shfl_sync(0xffffffffu, row, (8 * k + 4 * u + sub) & 31);
+        const uint4* src = bounds + (size_t)max(at, 0) * (2 * D / 8) + l8;
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c) cp_async_16(dst + (u * kChunks + c) * 512, src + c * 8, ok);
+        for (int c = 0; c < kChunks; ++c) cp_async_16(dst + (u * kChunks + c) * 512, src + c * 8, at >= 0);
       }
     };
-    for (int k = 0; k < kStages - 1; ++k) {
+    for (int k = 0; k < p.stages - 1; ++k) {
       if (k < steps) begin_step(k);
-      else valid <<= 2;
       cp_async_commit();
     }
     // ---- the heads' parts, while the first bounds arrive ----
@@ -615,13 +662,15 @@ __global__ void __launch_bounds__(kThreads, 2) select_kernel(const Params p) {
       }
     const uint32_t dst = mapa_shared(s_score, 0);
     cluster_wait();
+    uint32_t least = 0u, most = 0u;      // of the minima and the maxima, pair by pair
+    bool usable = true;
     for (int k = 0; k < steps; ++k) {
-      if (k + kStages - 1 < steps) begin_step(k + kStages - 1);
-      else valid <<= 2;
+      if (k + p.stages - 1 < steps) begin_step(k + p.stages - 1);
       cp_async_commit();
-      cp_async_wait<kStages - 1>();
+      if (p.stages == kMany) cp_async_wait<kMany - 1>();
+      else cp_async_wait<kFew - 1>();
       const uint8_t* src = ring + from_stage * 2 * kChunks * 512;
-      from_stage = from_stage + 1 == kStages ? 0 : from_stage + 1;
+      from_stage = from_stage + 1 == p.stages ? 0 : from_stage + 1;
       float x[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -633,7 +682,9 @@ __global__ void __launch_bounds__(kThreads, 2) select_kernel(const Params p) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             s2 = f2_fma(pair_to_f2<BT>(w[e]), coef[c][e], s2);
-            top = pair_top<BT>(top, w[e]);
+            // chunks of minima, then of maxima: no bound is larger than the largest of these two
+            if (c < kChunks / 2) least = pair_min<BT>(least, w[e]);
+            else most = pair_max<BT>(most, w[e]);
           }
         }
         float y;
@@ -646,157 +697,230 @@ __global__ void __launch_bounds__(kThreads, 2) select_kernel(const Params p) {
       y += __shfl_xor_sync(0xffffffffu, up ? x[0] : x[1], 4);
       y += __shfl_xor_sync(0xffffffffu, y, 2);
       y += __shfl_xor_sync(0xffffffffu, y, 1);
-      // -inf marks an entry outside the pool; a sum that is too large, or NaN, is summed again below
+      // a sum that is too large, or NaN, is summed again below
       const int i = begin + 8 * k + (up ? 4 : 0) + sub;
-      const bool ok = (valid >> (2 * kStages - (up ? 2 : 1))) & 1u, usable = fabsf(y) < kBig;
-      if (!usable) top = 0x7fff7fffu;
-      if ((l8 & 3) == 0 && i < end) st_cluster_f32(dst + 4u * (uint32_t)i, !ok ? -INFINITY : usable ? y : kBig);
+      const bool fits = fabsf(y) < kBig;
+      usable = usable && fits;
+      if ((l8 & 3) == 0 && i < end) st_cluster_f32(dst + 4u * (uint32_t)i, fits ? y : kBig);
     }
-    top = max(top >> 16, top & 0xffffu);
-    top = __reduce_max_sync(0xffffffffu, top);
+    // as bits of a 16-bit magnitude, which order like it; a NaN is the largest
+    least &= 0x7fff7fffu;
+    most &= 0x7fff7fffu;
+    top = usable ? max(max(least >> 16, least & 0xffffu), max(most >> 16, most & 0xffffu)) : 0x7fffu;
+    top = __reduce_max_sync(0xffffffffu, top & 0x7fffu) | (outside ? kOutside : 0u);
     if (lane == 0) st_cluster_u32(mapa_shared(s_top + rank * kWarps + warp, 0), top);
     cluster_sync();
     if (rank != 0) return;
     top = lane < workers ? s_top[lane] : 0u;
-    if (lane + 32 < workers) top = max(top, s_top[lane + 32]);
-    top = __reduce_max_sync(0xffffffffu, top);
+    const uint32_t more = lane + 32 < workers ? s_top[lane + 32] : 0u;
+    if (__any_sync(0xffffffffu, (top | more) & kOutside)) {
+      // -inf marks an entry outside the pool
+      for (int i = from + tid; i < to; i += kThreads)
+        if ((unsigned)table[i] >= (unsigned)p.num_pages) s_score[i] = -INFINITY;
+      __syncthreads();
+    }
+    top = __reduce_max_sync(0xffffffffu, max(top & 0x7fffu, more & 0x7fffu));
   }
 
   // ---- pages that are always kept (all of them where nothing is chosen), and candidates ----
   int counts = 0;                        // kept, and candidates times 2^16
-  for (int i = tid; i < live; i += kThreads) {
-    if (!all && i >= from && i < to) {
-      counts += s_score[i] != -INFINITY ? 1 << 16 : 0;
-    } else {
-      const bool good = (unsigned)table[i] < (unsigned)p.num_pages;
-      if (!good) record_device_error(PU_ERR_INVALID_ARGUMENT, kSiteSelectPage);
-      s_score[i] = good ? INFINITY : -INFINITY;
-      counts += good;
-    }
+  float lo = INFINITY, hi = -INFINITY;   // of the candidates
+  for (int i = tid; i < live - (all ? 0 : to - from); i += kThreads) {
+    const int at = all || i < from ? i : i + (to - from);
+    const bool good = (unsigned)table[at] < (unsigned)p.num_pages;
+    if (!good) record_device_error(PU_ERR_INVALID_ARGUMENT, kSiteSelectPage);
+    s_score[at] = good ? INFINITY : -INFINITY;
+    counts += good;
   }
-  counts = block_sum(counts, s, warp, lane);         // and the scores are visible to all
-
-  // ---- the border: every score above it is kept, and the first `ties` equal to it ----
-  float cut = -INFINITY;
-  int ties = 0;
   if (!all) {
-    int want = p.count - (counts & 0xffff);          // of the candidates
-    if (want <= 0) {
-      cut = 0x1p126f;                    // none but those always kept
-    } else if (counts >> 16 > want) {
-      border(s_score, from, to, want, s, &cut, &ties);
-      // what the fp32 sums are off by; 2^-140: sums of subnormals
-      double e = 0.;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) e += s_abs[w];
-      const float big = to_float(*reinterpret_cast<const BT*>(&top));
-      e = isfinite(big) && e < 0x1p1000 ? fma(e * (double)big, 0x1p-19, 0x1p-140) : INFINITY;
-      const double sure = (double)cut + 2. * e, none = (double)cut - 2. * e;
-      if (tid == 0) s.found[3] = 0;
-      __syncthreads();
-      counts = 0;                        // above, and near times 2^16
-      for (int i = from + tid; i < to; i += kThreads) {
-        const float x = s_score[i];
-        if (x == -INFINITY) continue;
-        if ((double)x > sure) {
-          ++counts;
-          s_score[i] = INFINITY;
-        } else if ((double)x < none) {
-          s_score[i] = -INFINITY;
-        } else {
-          counts += 1 << 16;
-          const int k = atomicAdd(s.found + 3, 1);
-          if (k < kRank) s.list[k] = i;
-        }
+    each(s_score, from, to, [&](int, float x) {
+      if (x != -INFINITY) {
+        counts += 1 << 16;
+        lo = min(lo, x);
+        hi = max(hi, x);
       }
-      counts = block_sum(counts, s, warp, lane);
-      const int near = counts >> 16;
-      want -= counts & 0xffff;
-      cut = -INFINITY;                   // as many as places: all of them
-      ties = 0;
-      if (near > want) {
-        // ---- summed again in fp64, a warp a page ----
-        auto again = [&](int i) -> double {
-          const uint4* src = bounds + ((size_t)table[i] * p.H_kv + head) * (2 * D / 8);
-          double x = 0.;
-          for (int c = lane; c < 2 * D / 8; c += 32) {
-            const uint4 v = src[c];
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-            const double* f = &s_wide[0][0] + c * 8;
+    });
+  }
+  counts = __reduce_add_sync(0xffffffffu, counts);
+  if (lane == 0) s.sum[warp] = counts;
+  block_range(lo, hi, s, warp, lane);    // and the scores are visible to all
+  counts = 0;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              x = fma(wide<BT>(w[j] << 16), f[2 * j], x);
-              x = fma(wide<BT>(w[j]), f[2 * j + 1], x);
-            }
-          }
+  for (int w = 0; w < kWarps; ++w) counts += s.sum[w];
+
+  const size_t out_row = (size_t)b * p.H_kv + head;
+  int want = p.count - (counts & 0xffff);            // of the candidates
+  if (all || counts >> 16 <= want) {
+    __syncthreads();                     // s.sum has been read
+    write_list<float>(p, table, s_score, -INFINITY, 0, live, len, out_row, s);
+    return;
+  }
+  if (want <= 0) {
+    __syncthreads();
+    write_list<float>(p, table, s_score, 0x1p126f, 0, live, len, out_row, s);    // none but those always kept
+    return;
+  }
+  // what the fp32 sums are off by; 2^-140: sums of subnormals
+  double sum_abs = 0.;
 #pragma unroll
-          for (int off = 16; off > 0; off >>= 1) x += __shfl_xor_sync(0xffffffffu, x, off);
-          // finite, also for queries that are not
-          return x != x ? 0x1p1000 : fmin(fmax(x, -0x1p1000), 0x1p1000);
-        };
-        if (near <= kRank) {
-          for (int k = warp; k < near; k += kWarps) {
-            const double x = again(s.list[k]);
-            if (lane == 0) s.cand[k] = x;
-          }
-          __syncthreads();
-          if (tid < near) {
-            const double x = s.cand[tid];
-            const int i = s.list[tid];
-            int before = 0;
-            for (int j = 0; j < near; ++j) before += s.cand[j] > x || (s.cand[j] == x && s.list[j] < i);
-            s_score[i] = before < want ? INFINITY : -INFINITY;
-          }
-          __syncthreads();
-        } else {
-          // more than can be ranked against each other (equal pages, say): all scores as fp64 in the same
-          // place, which has room for them once the copies are over, and the border among those
-          double* fine = reinterpret_cast<double*>(dyn);
-          for (int base = (live - 1) / kThreads * kThreads; base >= 0; base -= kThreads) {
-            const int i = base + tid;
-            const float x = i < live ? s_score[i] : 0.f;
-            __syncthreads();
-            if (i < live) fine[i] = x;
-            __syncthreads();
-          }
-          for (int i = from + warp; i < to; i += kWarps) {
-            if (isinf(fine[i])) continue;
-            const double x = again(i);
-            if (lane == 0) fine[i] = x;
-          }
-          __syncthreads();
-          double at = 0x1p1010;
-          if (want > 0) border(fine, from, to, want, s, &at, &ties);
-          write_list<double>(p, table, fine, at, ties, live, len, (size_t)b * p.H_kv + head, s);
-          return;
-        }
+  for (int w = 0; w < kWarps; ++w) sum_abs += s_abs[w];
+  const float big = to_float(*reinterpret_cast<const BT*>(&top));
+  const double e = isfinite(big) && sum_abs < 0x1p1000 ? fma(sum_abs * (double)big, 0x1p-19, 0x1p-140) : INFINITY;
+  // a page in fp64, by a warp
+  auto again = [&](int i) -> double {
+    const uint4* src = bounds + ((size_t)table[i] * p.H_kv + head) * (2 * D / 8);
+    double x = 0.;
+    for (int c = lane; c < 2 * D / 8; c += 32) {
+      const uint4 v = src[c];
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+      const double* f = &s_wide[0][0] + c * 8;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x = fma(wide<BT>(w[j] << 16), f[2 * j], x);
+        x = fma(wide<BT>(w[j]), f[2 * j + 1], x);
       }
     }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) x += __shfl_xor_sync(0xffffffffu, x, off);
+    // finite, also for queries that are not
+    return x != x ? 0x1p1000 : fmin(fmax(x, -0x1p1000), 0x1p1000);
+  };
+
+  // ---- the border: bins, until those within 2 e of the border's are few enough to be ranked ----
+  while (lo < hi) {
+    const Bins<float> bins(lo, hi);
+    find_bin(s_score, from, to, lo, hi, bins, want, s);
+    const int at = s.found[0], reach = (int)fmin(2. * e * (double)bins.scale, 64.) + 1;
+    if (reach > 32) break;
+    const int first = max(0, at - reach), last = min(kBins - 1, at + reach);
+    int above = s.found[1], members = s.found[2];
+    for (int i = at + 1; i <= last; ++i) above -= s.bins[i];
+    for (int i = first; i <= last; ++i) members += i == at ? 0 : s.bins[i];
+    want -= above;
+    if (members <= kRank) {
+      // ---- ranked, the near ones of the border by fp64 sums ----
+      each(s_score, from, to, [&](int i, float x) {
+        const int c = bins.of(x);
+        if (x >= lo && x <= hi && c >= first && c <= last) {
+          const int k = atomicAdd(s.found + 3, 1);
+          s.list[k] = i;
+          s.near[k] = x;
+        }
+      });
+      __syncthreads();
+      const float x = tid < members ? s.near[tid] : 0.f;
+      const int mine = tid < members ? s.list[tid] : 0;
+      int before = 0;
+      if (tid < members) {
+        for (int j = 0; j < members; ++j) before += s.near[j] > x || (s.near[j] == x && s.list[j] < mine);
+        if (before == want - 1) s.edge = x;
+      }
+      __syncthreads();
+      const float edge = s.edge;
+      const bool near = tid < members && fabs((double)x - (double)edge) <= 2. * e;
+      bool in = before < want;
+      if (__syncthreads_count(near) > 1) {
+        const int sure = __syncthreads_count(tid < members && !near && x > edge);
+        for (int k = warp; k < members; k += kWarps) {
+          if (!(fabs((double)s.near[k] - (double)edge) <= 2. * e)) continue;
+          const double y = again(s.list[k]);
+          if (lane == 0) s.cand[k] = y;
+        }
+        __syncthreads();
+        if (near) {
+          const double y = s.cand[tid];
+          int ahead = sure;
+          for (int j = 0; j < members; ++j) {
+            if (!(fabs((double)s.near[j] - (double)edge) <= 2. * e)) continue;
+            ahead += s.cand[j] > y || (s.cand[j] == y && s.list[j] < mine);
+          }
+          in = ahead < want;
+        } else {
+          in = x > edge;
+        }
+      }
+      if (tid < members) s_score[mine] = in ? INFINITY : -INFINITY;
+      __syncthreads();
+      write_list<float>(p, table, s_score, edge, 0, live, len, out_row, s);
+      return;
+    }
+    // again between the smallest and the largest of them
+    float lo2 = INFINITY, hi2 = -INFINITY;
+    each(s_score, from, to, [&](int, float x) {
+      const int c = bins.of(x);
+      if (x >= lo && x <= hi && c >= first && c <= last) {
+        lo2 = min(lo2, x);
+        hi2 = max(hi2, x);
+      }
+    });
+    block_range(lo2, hi2, s, warp, lane);
+    __syncthreads();
+    if (lo2 == lo && hi2 == hi) break;
+    lo = lo2;
+    hi = hi2;
   }
-  write_list<float>(p, table, s_score, cut, ties, live, len, (size_t)b * p.H_kv + head, s);
+
+  // ---- more pages than can be ranked are as close as the fp32 sums tell (equal pages, say): those in [lo, hi]
+  // and within 2 e of it in fp64, all scores as fp64 in the same place, which has room for them once the copies
+  // are over ----
+  const double least = (double)lo - 2. * e, most = (double)hi + 2. * e;
+  double* fine = reinterpret_cast<double*>(dyn);
+  for (int base = (live - 1) / kThreads * kThreads; base >= 0; base -= kThreads) {
+    const int i = base + tid;
+    const float x = i < live ? s_score[i] : 0.f;
+    __syncthreads();
+    if (i < live) fine[i] = x;
+    __syncthreads();
+  }
+  want = p.count;                        // less those that are sure
+  counts = 0;
+  for (int i = tid; i < live; i += kThreads) {
+    const double x = fine[i];
+    if (x > most || x == INFINITY) {
+      ++counts;
+      fine[i] = INFINITY;
+    } else if (x < least) {
+      fine[i] = -INFINITY;
+    }
+  }
+  want -= block_sum(counts, s, warp, lane);
+  for (int i = from + warp; i < to; i += kWarps) {
+    if (isinf(fine[i])) continue;
+    const double x = again(i);
+    if (lane == 0) fine[i] = x;
+  }
+  __syncthreads();
+  double cut = 0x1p1010;
+  int ties = 0;
+  if (want > 0) border(fine, from, to, want, s, &cut, &ties);
+  write_list<double>(p, table, fine, cut, ties, live, len, out_row, s);
 }
 
-// CTAs of a cluster: what brings the grid to about three CTAs an SM, but no more than one for 64 pages of a
-// full table row.
+// CTAs of a cluster: as many as leave the grid at two CTAs an SM, but no more than one for 64 pages of a full
+// table row.  Each CTA pays about 3 us before its first score, and the first one as much for the choice.
 inline int cluster_size(long long max_pages, long long items) {
   int c = 1;
-  while (c < kMaxCtas && max_pages > 64ll * c && 2 * c * items <= 4ll * sm_count()) c *= 2;
+  while (c < kMaxCtas && max_pages > 64ll * c && 2 * c * items <= 2ll * sm_count()) c *= 2;
   return c;
 }
 
 template <typename QT, typename BT, int D>
 int launch_select(Params p, long long items, cudaStream_t st) {
   const auto f = select_kernel<QT, BT, D>;
-  // scores, and behind them the copies: eight pages of 4 D bytes a warp and stage, or as much as lets the
-  // scores be held in fp64
-  constexpr int kRing = kStages * kWarps * 32 * D;
+  // scores, and behind them the copies (eight pages of 4 D bytes a warp and stage) or as much as lets the scores
+  // be held in fp64
+  constexpr int kStage = kWarps * 32 * D;
   p.ring = (p.max_pages * (int)sizeof(float) + 15) / 16 * 16;
+  // twice the copies in flight where a warp has many steps, and about one CTA an SM (it then has all of the
+  // SM's shared memory, and the next call's CTAs do not start beside it)
+  p.stages = p.max_pages > 512 * p.ctas && 2 * items * p.ctas <= 3ll * sm_count() && p.ring + kMany * kStage <= 2 * kMaxPages * (int)sizeof(float) ? kMany : kFew;
+  const int ring = std::max(p.stages * kStage, p.ring);
   const int rc = set_max_dynamic_smem(reinterpret_cast<const void*>(f), 2 * kMaxPages * (int)sizeof(float) + 16, "page choice shared memory");
   if (rc) return rc;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(items * p.ctas));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = (size_t)(p.ring + std::max(kRing, p.ring));
+  cfg.dynamicSmemBytes = (size_t)(p.ring + ring);
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -892,7 +1016,7 @@ extern "C" int pu_select_pages(const void* q, int q_dtype, const void* bounds, i
   p.page_shift = shift;
   p.B = (int)B;
   // where the clusters do not all start at once; 256 lengths took 5 us to rank
-  p.by_length = B > 1 && B <= 64 && B * H_kv * p.ctas > 2ll * pu::sm_count();
+  p.by_length = B > 1 && B <= 64 && B * H_kv * p.ctas > pu::sm_count();
   p.count = (int)count;
   p.first = (int)first;
   p.last = (int)last;
