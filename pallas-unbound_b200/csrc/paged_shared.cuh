@@ -543,49 +543,51 @@ __global__ void __launch_bounds__(Cfg<T, KVT, D>::kThreads, 1)
       // ---- this slot's part of the queries ----
       if (w.seg > 0) mbar_wait(bQe, (w.seg - 1) & 1, abort_flag, kSiteDecodeTc);
       {
-        constexpr int kVecs = D / 8, kStep = 128 / kVecs;      // lanes of a row, rows at once
-        const int c = row % kVecs;
-        const int lo = w.split ? t * 64 : t * 128, many = w.split ? 64 : 128;
-#pragma unroll 1
-        for (int i0 = 0; i0 < many; i0 += 4 * kStep) {
-          uint4 v[4];
+        constexpr int kVecs = D / 8, kStep = 128 / kVecs, kLoads = 128 / kStep;    // lanes of a row, rows at once
+        const int c = row % kVecs, lo = (w.split ? t * 64 : t * 128) + row / kVecs;
+        // sequence and query head of the first row; kStep rows on, without a division
+        const int first = row0 + lo, dseq = kStep / p.group, dhead = kStep - dseq * p.group;
+        int seq = first / p.group, at = first - seq * p.group;
+        const T* q = static_cast<const T*>(p.q) + ((size_t)g.start * p.H + (size_t)head * p.group) * D + c * 8;
+        uint4 v[kLoads];
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const int r = lo + i0 + u * kStep + row / kVecs;   // row of the item
-            v[u] = make_uint4(0u, 0u, 0u, 0u);
-            if (r < w.rows) {
-              const int at = row0 + r;
-              const size_t qrow = (size_t)(g.start + at / p.group) * p.H + head * p.group + at % p.group;
-              v[u] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + qrow * D + c * 8);
-            }
+        for (int u = 0; u < kLoads; ++u) {
+          v[u] = make_uint4(0u, 0u, 0u, 0u);
+          if ((!w.split || u < kLoads / 2) && lo + u * kStep < w.rows) v[u] = *reinterpret_cast<const uint4*>(q + ((size_t)seq * p.H + at) * D);
+          seq += dseq;
+          at += dhead;
+          if (at >= p.group) {
+            at -= p.group;
+            ++seq;
           }
+        }
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const int r = lo + i0 + u * kStep + row / kVecs;
-            if constexpr (kF8) {
-              float x[8];
-              unpack8<T>(v[u], x);
-              float down = 1.f;
-              if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-                // by a power of two that puts the row's largest |q| into [2^14, 2^15): bf16's 8 bits
-                // are f16 values down to 2^-31 of it
-                float mx = 0.f;
+        for (int u = 0; u < kLoads; ++u) {
+          if (w.split && u >= kLoads / 2) break;
+          const int r = lo + u * kStep;
+          if constexpr (kF8) {
+            float x[8];
+            unpack8<T>(v[u], x);
+            float down = 1.f;
+            if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+              // by a power of two that puts the row's largest |q| into [2^14, 2^15): bf16's 8 bits
+              // are f16 values down to 2^-31 of it
+              float mx = 0.f;
 #pragma unroll
-                for (int k = 0; k < 8; ++k) mx = fmaxf(mx, fabsf(x[k]));
+              for (int k = 0; k < 8; ++k) mx = fmaxf(mx, fabsf(x[k]));
 #pragma unroll
-                for (int off = kVecs / 2; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-                const int e = (mx > 0.f && isfinite(mx)) ? ((__float_as_int(mx) >> 23) & 0xff) - 127 : 14;
-                const int sh = min(126, 14 - e);
-                const float up = __int_as_float((127 + sh) << 23);
-                down = __int_as_float((127 - sh) << 23);
+              for (int off = kVecs / 2; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+              const int e = (mx > 0.f && isfinite(mx)) ? ((__float_as_int(mx) >> 23) & 0xff) - 127 : 14;
+              const int sh = min(126, 14 - e);
+              const float up = __int_as_float((127 + sh) << 23);
+              down = __int_as_float((127 - sh) << 23);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) x[k] *= up;
-              }
-              if (c == 0) s_scale[r] = down;
-              v[u] = make_uint4(pack16<__half>(x[0], x[1]), pack16<__half>(x[2], x[3]), pack16<__half>(x[4], x[5]), pack16<__half>(x[6], x[7]));
+              for (int k = 0; k < 8; ++k) x[k] *= up;
             }
-            *reinterpret_cast<uint4*>(sQ + (r >> 7) * kTile + (c >> 3) * (BT * 128) + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[u];
+            if (c == 0) s_scale[r] = down;
+            v[u] = make_uint4(pack16<__half>(x[0], x[1]), pack16<__half>(x[2], x[3]), pack16<__half>(x[4], x[5]), pack16<__half>(x[6], x[7]));
           }
+          *reinterpret_cast<uint4*>(sQ + (r >> 7) * kTile + (c >> 3) * (BT * 128) + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[u];
         }
         fence_proxy_async_smem();
         mbar_arrive(bQ);
