@@ -380,7 +380,8 @@ PU_API int pu_decode_paged_heads(const void* q, int q_dtype,
  *     in whole pages (rounded down).  They are read through the table row of the
  *     group's first sequence that holds as many; the others' entries for them must
  *     name the same pages.  A sequence that holds fewer attends them by itself.  A
- *     group in which none holds as many shares nothing.
+ *     group in which none holds as many shares nothing, nor does a call where that
+ *     would save little (a thousand tiles of 128 tokens of one K/V head).
  * q and pools of one 16-bit type, D 64 or 128, or e4m3 pools with D = 128; any
  * H / H_kv; groups <= 64; B <= 8192; H <= 65535; H_kv * D <= 2^21 - 32.
  *   workspace: pu_decode_paged_shared_workspace_size() bytes, zeroed before its
@@ -388,7 +389,7 @@ PU_API int pu_decode_paged_heads(const void* q, int q_dtype,
  * The softmax weights of shared tokens are rounded once to the pools' 16-bit type,
  * to f16 with e4m3 pools (bf16 queries are f16 times a power of two then: exact
  * down to 2^-31 of a head's largest element).  A table entry of shared tokens
- * outside the pool is reported (detail 311) and its tokens are left out.
+ * outside the pool is reported (detail 302) and its tokens are left out for all.
  */
 PU_API size_t pu_decode_paged_shared_workspace_size(int64_t B, int64_t H, int64_t H_kv,
                                                     int64_t groups, int64_t D);

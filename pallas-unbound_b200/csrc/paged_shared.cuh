@@ -45,6 +45,10 @@ constexpr int BT = 128;                  // tokens of a tile
 constexpr int kRows = 256;               // rows of an item
 constexpr int kMaxGroups = 64;
 constexpr int kItemCost = 2;             // what starting and ending an item costs, in tiles
+// A pass over shared tokens and its join cost about 16 us before their first tile; the tiles that the
+// sequences would read by themselves instead are spread over all CTAs and come from L2 (four sequences of 8
+// K/V heads with 1024 shared tokens, 256 tiles: 28 us shared, 20 us not).  Below this many nothing is shared.
+constexpr int kWorth = 1024;
 constexpr int kBadRing = 8;
 
 template <typename T, typename KVT, int D>
@@ -100,7 +104,7 @@ struct Params {
   int32_t* own_lens;           // [B] and those that are left
   Group* desc;                 // [kMaxGroups + 1]
   float* slabs;                // records
-  int B, H, H_kv, group, groups;
+  int B, H, H_kv, group, slices, groups;
   int max_pages, num_pages, page_shift, box;
   float scale_log2;
 };
@@ -223,12 +227,22 @@ __device__ __forceinline__ void make_groups(const Params& p, Group* gs, int tid,
   }
   __syncthreads();
   if (tid < 32) {
+    // tiles that sharing saves; one sequence alone shares with nobody
+    long long saved = 0;
+    for (int i = lane; i < p.groups; i += 32) {
+      const int n = gs[i + 1].start - gs[i].start;
+      if (gs[i].rep == 0x7fffffff || n < 2) gs[i].tokens = 0;
+      saved += (long long)n * p.slices * tiles_of(gs[i]);
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) saved += __shfl_xor_sync(0xffffffffu, saved, off);
+    const bool worth = saved * p.H_kv >= kWorth;
     int before = 0;
     for (int base = 0; base <= p.groups; base += 32) {
       const int i = base + lane;
       int units = 0;
       if (i < p.groups) {
-        if (gs[i].rep == 0x7fffffff) gs[i].tokens = 0;
+        if (!worth) gs[i].tokens = 0;
         const int all = (gs[i + 1].start - gs[i].start) * p.group;
         if (gs[i].tokens > 0) units = (all + kRows - 1) / kRows * p.H_kv * (tiles_of(gs[i]) + kItemCost);
       }
@@ -378,7 +392,7 @@ __global__ void __launch_bounds__(Cfg<T, KVT, D>::kThreads, 1)
           }
           const int pg = __shfl_sync(0xffffffffu, entries, (k * boxes + lane) & 31), row0 = t * BT;
           const bool mine = lane < boxes && row0 + lane_row < g.tokens, good = mine && (unsigned)pg < (unsigned)p.num_pages;
-          if (mine && !good) record_device_error(PU_ERR_INVALID_ARGUMENT, kSiteDecodeShared);
+          if (mine && !good) record_device_error(PU_ERR_INVALID_ARGUMENT, kSiteDecodePage);
           const unsigned loaded = __ballot_sync(0xffffffffu, good);
           const unsigned bad = __ballot_sync(0xffffffffu, lane < BT / 16 && !((loaded >> ((lane * 16) >> box_shift)) & 1u));
           const int outer = pg * p.H_kv + head, in = p.box < BT ? 0 : row0 & ((1 << p.page_shift) - 1);
@@ -917,6 +931,7 @@ int pu_decode_paged_shared(const void* q, int q_dtype, const void* k_pool, const
   prm.H = (int)H;
   prm.H_kv = (int)H_kv;
   prm.group = (int)(H / H_kv);
+  prm.slices = (prm.group + ptc::NP - 1) / ptc::NP;
   prm.groups = (int)groups;
   prm.max_pages = (int)max_pages_per_seq;
   prm.num_pages = (int)num_pages;
@@ -938,7 +953,7 @@ int pu_decode_paged_shared(const void* q, int q_dtype, const void* k_pool, const
   own.pool_heads = prm.H_kv;
   own.lists = 1;
   own.group = prm.group;
-  own.slices = (prm.group + ptc::NP - 1) / ptc::NP;
+  own.slices = prm.slices;
   own.inner = prm.H_kv * own.slices;
   own.max_pages = prm.max_pages;
   own.num_pages = prm.num_pages;

@@ -46,7 +46,6 @@ enum WaitSite : int {
   kSiteFreePages = 308,
   kSitePageBounds = 309,
   kSiteSelectPage = 310,
-  kSiteDecodeShared = 311,
   kSiteOutProj = 401,
   kSiteSelfTest = 901,
 };

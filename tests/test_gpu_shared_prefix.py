@@ -35,7 +35,12 @@ def ints(a):
     return torch.from_numpy(np.ascontiguousarray(a)).int().cuda()
 
 
-def check(o, lse, q, k_pool, v_pool, table, lens, k_scale=1.0, v_scale=1.0, scale=None, what=""):
+def enough(tokens, H, H_kv):
+    """Sequences from which on a prefix of `tokens` tokens is shared."""
+    return -(-1024 // (-(-tokens // 128) * H_kv * -(-(H // H_kv) // 16)))
+
+
+def check(o, lse, q, k_pool, v_pool, table, lens, k_scale=1.0, v_scale=1.0, scale=None, what="", sample=60):
     B, H, _, D = q.shape
     H_kv = k_pool.shape[1]
     G = H // H_kv
@@ -44,7 +49,10 @@ def check(o, lse, q, k_pool, v_pool, table, lens, k_scale=1.0, v_scale=1.0, scal
     rnd = 2.0 ** -8 if k_pool.dtype == BF else 2.0 ** -11
     lost = 0.0 if k_pool.dtype == BF else 2.0 ** -25
     assert o.dtype == BF and o.shape == q.shape and lse.shape == (B, H)
+    some = np.random.RandomState(B).permutation(B)[:sample].tolist() + [0, B - 1]
     for b, n in enumerate(np.asarray(lens).tolist()):
+        if b not in some:
+            continue
         if n == 0:
             assert (o[b] == 0).all() and (lse[b] == -math.inf).all(), f"{what}: empty sequence {b}"
             continue
@@ -111,11 +119,33 @@ def test_prefixes(mods, H, H_kv, D, qdt, kvdt, page):
 
 
 @pytest.mark.parametrize("H,H_kv,D,qdt,kvdt", KINDS)
+@pytest.mark.parametrize("page,tokens", [(16, 16), (16, 144), (64, 128), (64, 960), (256, 2048)])
+def test_shared(mods, H, H_kv, D, qdt, kvdt, page, tokens):
+    """As few sequences as share, and one fewer: one page, tiles and a rest, several items of 256 rows;
+    the sequences' own tokens from none on, one sequence shorter than the prefix."""
+    _lib, dec, paged = mods
+    r = np.random.RandomState(page + tokens)
+    ks, vs = (0.05, 0.03) if kvdt == FP8 else (1.0, 1.0)
+    n = enough(tokens, H, H_kv)
+    own = [0, 1, page, 129] + r.randint(0, 40, max(0, n - 4)).tolist()
+    table, P, lens, shared, _ = batch([(tokens, own[:n])], page, 7)
+    lens[n // 2] = max(0, tokens - 1)
+    q, k, v = make(P, n, H, H_kv, D, page, qdt, kvdt, 3, ks, vs)
+    for m in (n, max(1, n - 1)):
+        args = q[:m], k, v, table[:m].contiguous(), ints(lens[:m])
+        o, lse = paged.paged_decode(*args, shared_lens=shared, k_scale=ks, v_scale=vs, return_lse=True)
+        assert _lib.device_status() == (0, 0)
+        check(o, lse, args[0], k, v, args[3], lens[:m], ks, vs, what=f"{tokens} shared by {m}")
+        assert torch.equal(o, paged.paged_decode(*args, shared_lens=shared, k_scale=ks, v_scale=vs))
+
+
+@pytest.mark.parametrize("H,H_kv,D,qdt,kvdt", KINDS)
 def test_groups(mods, H, H_kv, D, qdt, kvdt):
     """Several prefixes, groups without one, empty groups, sequences in no group."""
     _lib, dec, paged = mods
     page = 32
-    groups = [(96, [5, 0, 70]), (0, [3, 200]), (1024, list(range(50))), (64, []), (320, [1] * 9), (512, [0])]
+    # 7680 tokens shared by 160 sequences: 9600 tiles of a K/V head
+    groups = [(96, [5, 0, 70]), (0, [3, 200]), (7680, list(range(160))), (64, []), (320, [1] * 9), (512, [0])]
     table, P, lens, shared, starts = batch(groups, page, 3)
     q, k, v = make(P, len(lens), H, H_kv, D, page, qdt, kvdt, 5)
     o, lse = paged.paged_decode(q, k, v, table, ints(lens), shared_lens=shared, shared_groups=starts, return_lse=True)
@@ -133,7 +163,7 @@ def test_groups(mods, H, H_kv, D, qdt, kvdt):
 def test_many_groups(mods, groups):
     _lib, dec, paged = mods
     page = 16
-    table, P, lens, shared, starts = batch([(16 * (1 + i % 20), [i, 3 * i, 0][:1 + i % 3]) for i in range(groups)], page, 3)
+    table, P, lens, shared, starts = batch([(16 * (1 + i % 60), [i, 3 * i, 0, 5, 1, 17][:1 + i % 6]) for i in range(groups)], page, 3)
     q, k, v = make(P, len(lens), 8, 2, 128, page, BF, BF, 5)
     o, lse = paged.paged_decode(q, k, v, table, ints(lens), shared_lens=shared, shared_groups=starts, return_lse=True)
     assert _lib.device_status() == (0, 0)
@@ -147,18 +177,25 @@ def test_lengths_that_do_not_fit(mods, kvdt):
     plain decode."""
     _lib, dec, paged = mods
     page = 64
-    table, P, lens, shared, _ = batch([(640, [10, 0, 100, 33, 5])], page, 3)
-    q, k, v = make(P, 5, 8, 2, 128, page, BF, kvdt, 5)
+    more = [7] * 140                     # so that 640 tokens are shared
+    table, P, lens, shared, _ = batch([(640, [10, 0, 100, 33, 5] + more)], page, 3)
+    B = len(lens)
+    assert B >= enough(640, 8, 2)
+    q, k, v = make(P, B, 8, 2, 128, page, BF, kvdt, 5)
     for s in (639, 641, 65, 63, 0, -5):
         o, lse = paged.paged_decode(q, k, v, table, ints(lens), shared_lens=ints([s]), return_lse=True)
         check(o, lse, q, k, v, table, lens, what=f"shared {s}")
     for short in ([0, 640, 740, 673, 645], [0, 0, 740, 1, 645], [300, 639, 0, 128, 640], [0, 0, 0, 0, 0], [5, 639, 70, 64, 1]):
+        short = np.array(short + [647] * (B - 5))
         o, lse = paged.paged_decode(q, k, v, table, ints(short), shared_lens=shared, return_lse=True)
         check(o, lse, q, k, v, table, short, what=f"lengths {short}")
+    low = np.minimum(lens, 639)           # none holds the prefix
+    o, lse = paged.paged_decode(q, k, v, table, ints(low), shared_lens=shared, return_lse=True)
+    check(o, lse, q, k, v, table, low, what="none holds it")
     # longer than any sequence: nothing is shared
     o, lse = paged.paged_decode(q, k, v, table, ints(lens), shared_lens=ints([2 ** 31 - 1]), return_lse=True)
     check(o, lse, q, k, v, table, lens, what="too long")
-    for starts in ([0, 5, 3], [-7, 2, 900], [4, 1, 5], [5, 5, 5]):
+    for starts in ([0, B, 3], [-7, 2, 900], [4, 1, B], [5, 5, 5], [1, 140, B + 1]):
         o, lse = paged.paged_decode(q, k, v, table, ints(lens), shared_lens=ints([640, 640]), shared_groups=ints(starts), return_lse=True)
         check(o, lse, q, k, v, table, lens, what=f"starts {starts}")
     # an empty slot whose row names no page
@@ -173,7 +210,8 @@ def test_stale_and_missing_pages(mods, D, page, kvdt):
     """NaN in pages of nobody never counts; table entries outside the pool are reported and their
     tokens left out for all."""
     _lib, dec, paged = mods
-    table, P, lens, shared, _ = batch([(384 + page, [5, 0, 100] + [7] * 60)], page, 3, spare=9)
+    table, P, lens, shared, _ = batch([(384 + page, [5, 0, 100] + [7] * 180)], page, 3, spare=9)
+    assert len(lens) >= enough(384 + page, 8, 2)
     q, k, v = make(P, len(lens), 8, 2, D, page, HF if kvdt == HF else BF, kvdt, 5)
     used = torch.zeros(P, dtype=torch.bool, device="cuda")
     used[table[table >= 0].long()] = True
@@ -188,7 +226,7 @@ def test_stale_and_missing_pages(mods, D, page, kvdt):
     gone = [1, 3]
     bad[:, 1], bad[:, 3] = P, -1
     o, lse = paged.paged_decode(q, k, v, bad, ints(lens), shared_lens=shared, return_lse=True)
-    assert _lib.device_status() == (_lib.PU_ERR_INVALID_ARGUMENT, 311)
+    assert _lib.device_status() == (_lib.PU_ERR_INVALID_ARGUMENT, 302)
     rest = [i for i in range(table.shape[1]) if i not in gone]
     check(o, lse, q, k, v, table[:, rest].contiguous(), lens - 2 * page, what="missing")
 
@@ -273,7 +311,7 @@ def test_a_shared_document(mods):
 def test_streams_and_graphs(mods):
     """Two captured calls replayed at once on two streams: each has a workspace of its own."""
     _lib, dec, paged = mods
-    table, P, lens, shared, _ = batch([(1024, [40, 0, 700] + [9] * 30)], 32, 3)
+    table, P, lens, shared, _ = batch([(1024, [40, 0, 700] + [9] * 70)], 32, 3)
     n, sets = ints(lens), []
     for i in range(2):
         q, k, v = make(P, len(lens), 8, 2, 128, 32, BF, BF, 5 + 10 * i)
