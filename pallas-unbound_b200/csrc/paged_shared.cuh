@@ -101,6 +101,7 @@ struct Params {
   const int32_t* shared_lens;  // [groups]
   const int32_t* starts;       // [groups + 1] or nullptr: one group of all
   int32_t* skip;               // [B] tokens of each sequence that the prefix pass takes
+  int32_t* in_group;           // [B] and its group
   int32_t* own_lens;           // [B] and those that are left
   Group* desc;                 // [kMaxGroups + 1]
   float* slabs;                // records
@@ -116,18 +117,17 @@ constexpr size_t kSlab = (size_t)kRows * (D + 2);
 
 // The line of units and its parts.
 struct Line {
-  long long q, rem;
-  int ctas;
+  int q, rem, ctas;
   __device__ __forceinline__ Line(int units, int grid) {
     ctas = min(units, grid);
     q = ctas > 0 ? units / ctas : 0;
     rem = units - q * ctas;
   }
-  __device__ __forceinline__ int part(int c) const { return (int)(c * q + min((long long)c, rem)); }
+  __device__ __forceinline__ int part(int c) const { return c * q + min(c, rem); }
   // the part that holds unit x
   __device__ __forceinline__ int holder(int x) const {
-    const int big = (int)(rem * (q + 1));
-    return x < big ? x / (int)(q + 1) : (int)rem + (x - big) / (int)q;
+    const int big = rem * (q + 1);
+    return x < big ? x / (q + 1) : rem + (x - big) / q;
   }
 };
 
@@ -355,6 +355,7 @@ __global__ void __launch_bounds__(Cfg<T, KVT, D>::kThreads, 1)
       // a sequence that holds fewer tokens than its group shares attends them by itself
       const int skip = g >= 0 && p.lens[b] >= s_groups[g].tokens ? s_groups[g].tokens : 0;
       p.skip[b] = skip;
+      p.in_group[b] = g;
       p.own_lens[b] = max(0, min(p.lens[b], p.max_pages << p.page_shift) - skip);
     }
   }
@@ -747,6 +748,7 @@ __global__ void __launch_bounds__(Cfg<T, KVT, D>::kThreads, 1)
 struct JoinParams {
   const Group* desc;
   const int32_t* skip;         // [B]
+  const int32_t* in_group;     // [B]
   const float* slabs;
   const float* own_o;          // [B * H][D] fp32, the own tokens' output
   const float* own_lse;        // [B * H]
@@ -758,8 +760,8 @@ struct JoinParams {
 
 constexpr int kJoinWarps = 8;
 
-// Up to eight records are asked for at once, weights and columns together (first weights, then columns
-// where they count, with four records at once and 16 columns a thread: 64 sequences, 19 records a row, 18 us).
+// Many records are asked for at once, weights and columns together (first weights, then columns where they
+// count, with four records at once and 16 columns a thread: 64 sequences, 19 records a row, 18 us).
 template <int D>
 __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const JoinParams p) {
   grid_dep_wait();
@@ -773,15 +775,14 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const JoinParams 
   // the sequence's own tokens; an output of no weight is not there
   float M = p.own_lse[out] * kLog2e, L = 1.f;
   float4 acc = reinterpret_cast<const float4*>(p.own_o + out * D)[col];
-  const int skip = p.skip[b];
+  const int skip = p.skip[b], g = p.in_group[b], units = p.desc[p.groups].unit;
   if (M == -INFINITY) {
     L = 0.f;
     acc = make_float4(0.f, 0.f, 0.f, 0.f);
   }
   if (skip > 0) {
-    const int g = group_of(p.desc, p.groups, b);
     const Group a = p.desc[g];
-    const Line line(p.desc[p.groups].unit, p.grid);
+    const Line line(units, p.grid);
     const int all = (p.desc[g + 1].start - a.start) * p.group, pairs = (all + kRows - 1) / kRows, tiles = tiles_of(a);
     const int at = x - a.start * p.group, pair = at / kRows;
     const int r = head * pairs + pair, item0 = a.unit + r * (tiles + kItemCost), first = item0 + kItemCost;
@@ -790,7 +791,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const JoinParams 
     const int shift = min(kRows, all - pair * kRows) <= kRows / 2 ? 1 : 0, many = (c1 - c0 + 1) << shift;
     const bool second = line.part(c0) < item0;     // the item is not the first run of its first CTA
     const size_t only = c0 == c1 ? (size_t)(2 * p.grid + items_before(p.desc, g) + r) : 0;
-    constexpr int kAhead = 8;
+    constexpr int kAhead = 16;
     for (int i0 = 0; i0 < many; i0 += kAhead) {
       float2 ml[kAhead];
       float4 v[kAhead];
@@ -838,7 +839,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const JoinParams 
 // host side
 // ---------------------------------------------------------------------------
 struct Layout {
-  size_t own, own_lse, skip, own_lens, desc, slabs, total;   // byte offsets behind the own tokens' decode
+  size_t own, own_lse, skip, in_group, own_lens, desc, slabs, total;   // byte offsets behind the own tokens' decode
 };
 
 inline Layout layout(long long B, long long H, long long H_kv, long long D, long long groups) {
@@ -847,7 +848,8 @@ inline Layout layout(long long B, long long H, long long H_kv, long long D, long
   l.own = round_up(ptc::workspace_bytes(D), 256);
   l.own_lse = l.own + round_up(rows * D * sizeof(float), 256);
   l.skip = l.own_lse + round_up(rows * sizeof(float), 256);
-  l.own_lens = l.skip + round_up((size_t)B * sizeof(int32_t), 256);
+  l.in_group = l.skip + round_up((size_t)B * sizeof(int32_t), 256);
+  l.own_lens = l.in_group + round_up((size_t)B * sizeof(int32_t), 256);
   l.desc = l.own_lens + round_up((size_t)B * sizeof(int32_t), 256);
   l.slabs = l.desc + round_up((kMaxGroups + 1) * sizeof(Group), 256);
   const size_t items = (size_t)H_kv * ((size_t)(B * (H / H_kv)) / kRows + (size_t)groups);
@@ -924,6 +926,7 @@ int pu_decode_paged_shared(const void* q, int q_dtype, const void* k_pool, const
   prm.shared_lens = shared_lens;
   prm.starts = group_starts;
   prm.skip = reinterpret_cast<int32_t*>(ws + l.skip);
+  prm.in_group = reinterpret_cast<int32_t*>(ws + l.in_group);
   prm.own_lens = reinterpret_cast<int32_t*>(ws + l.own_lens);
   prm.desc = reinterpret_cast<shared::Group*>(ws + l.desc);
   prm.slabs = reinterpret_cast<float*>(ws + l.slabs);
@@ -979,6 +982,7 @@ int pu_decode_paged_shared(const void* q, int q_dtype, const void* k_pool, const
   shared::JoinParams jp{};
   jp.desc = prm.desc;
   jp.skip = prm.skip;
+  jp.in_group = prm.in_group;
   jp.slabs = prm.slabs;
   jp.own_o = own.o32;
   jp.own_lse = own.lse;
