@@ -998,6 +998,7 @@ extern "C" int pu_select_pages(const void* q, int q_dtype, const void* bounds, i
   if (rc) return rc;
   if (max_pages_per_seq > kMaxPages)
     return pu::set_error(PU_ERR_UNSUPPORTED, "page choice: %lld pages per sequence (up to %d)", (long long)max_pages_per_seq, kMaxPages);
+  if (num_pages > 2147483647ll / H_kv) return pu::set_error(PU_ERR_UNSUPPORTED, "page pool too large");
   if (count > (1ll << 30) / page_size) return pu::set_error(PU_ERR_UNSUPPORTED, "page choice: %lld pages chosen", (long long)count);
   Params p{};
   p.ctas = cluster_size(max_pages_per_seq, B * H_kv);
