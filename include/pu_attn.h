@@ -442,6 +442,20 @@ PU_API int pu_select_pages(const void* q, int q_dtype, const void* bounds, int b
                            void* stream);
 
 /*
+ * The entry points named below with their arguments as 8-byte words, in their
+ * order: pointers and whole numbers as they are, scales as doubles.  For bindings
+ * whose foreign calls pay for each argument (about 0.08 us in ctypes).  `words` is
+ * host memory.  An unknown entry is PU_ERR_INVALID_ARGUMENT.
+ */
+#define PU_CALL_DECODE_PAGED_GQA 0
+#define PU_CALL_DECODE_PAGED_HEADS 1
+#define PU_CALL_DECODE_PAGED_SHARED 2
+#define PU_CALL_PAGE_BOUNDS 3
+#define PU_CALL_SELECT_PAGES 4
+
+PU_API int pu_call_packed(int entry, const int64_t* words);
+
+/*
  * Plan a batch's next tokens on the device: page table rows, slots and
  * positions from lengths alone.  No counterpart in the reference.
  *   page_table [B][max_pages_per_seq], kv_lens [B]: the state before;

@@ -160,6 +160,35 @@ int pu_device_status(int* detail) {
   return PU_OK;
 }
 
+int pu_call_packed(int entry, const int64_t* w) {
+  if (!w) return pu::set_error(PU_ERR_INVALID_ARGUMENT, "packed call: null words");
+  auto ptr = [&](int i) { return reinterpret_cast<void*>(w[i]); };
+  auto i32 = [&](int i) { return reinterpret_cast<const int32_t*>(w[i]); };
+  auto f32 = [&](int i) {
+    double d;
+    memcpy(&d, w + i, sizeof(d));
+    return static_cast<float>(d);
+  };
+  switch (entry) {
+    case PU_CALL_DECODE_PAGED_GQA:
+    case PU_CALL_DECODE_PAGED_HEADS:
+      return (entry == PU_CALL_DECODE_PAGED_GQA ? pu_decode_paged_gqa : pu_decode_paged_heads)(
+          ptr(0), (int)w[1], ptr(2), ptr(3), (int)w[4], i32(5), w[6], w[7], w[8], i32(9), ptr(10), static_cast<float*>(ptr(11)), ptr(12),
+          (size_t)w[13], w[14], w[15], w[16], w[17], f32(18), f32(19), f32(20), ptr(21));
+    case PU_CALL_DECODE_PAGED_SHARED:
+      return pu_decode_paged_shared(ptr(0), (int)w[1], ptr(2), ptr(3), (int)w[4], i32(5), w[6], w[7], w[8], i32(9), i32(10), i32(11), w[12],
+                                    ptr(13), static_cast<float*>(ptr(14)), ptr(15), (size_t)w[16], w[17], w[18], w[19], w[20], f32(21), f32(22),
+                                    f32(23), ptr(24));
+    case PU_CALL_PAGE_BOUNDS:
+      return pu_page_bounds(ptr(0), (int)w[1], i32(2), ptr(3), w[4], w[5], w[6], w[7], w[8], ptr(9));
+    case PU_CALL_SELECT_PAGES:
+      return pu_select_pages(ptr(0), (int)w[1], ptr(2), (int)w[3], i32(4), w[5], w[6], w[7], i32(8), static_cast<int32_t*>(ptr(9)),
+                             static_cast<int32_t*>(ptr(10)), w[11], w[12], w[13], w[14], w[15], w[16], w[17], ptr(18));
+    default:
+      return pu::set_error(PU_ERR_INVALID_ARGUMENT, "packed call: no entry %d", entry);
+  }
+}
+
 }  // extern "C"
 
 // ---------------------------------------------------------------------------

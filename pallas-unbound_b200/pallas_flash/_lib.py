@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 from pathlib import Path
 
@@ -110,6 +111,8 @@ SIGNATURES = {
     "pu_select_pages": (_int, [_c_void_p, _int, _c_void_p, _int, _c_void_p, _i64, _i64, _i64, _c_void_p,
                                _c_void_p, _c_void_p, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
                                _c_void_p]),
+    # arguments as packed 8-byte words (PAGED_GQA and the like below)
+    "pu_call_packed": (_int, [_int, _c_void_p]),
     "pu_page_plan": (_int, [_c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
                             _c_void_p, _i64, _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p,
                             _c_void_p, _c_void_p, _i64, _i64, _c_void_p]),
@@ -121,6 +124,13 @@ SIGNATURES = {
     "pu_kv_append": (_int, [_c_void_p, _c_void_p, _int, _c_void_p, _c_void_p, _c_void_p, _i64,
                             _i64, _i64, _c_void_p, _i64, _i64, _i64, _c_void_p]),
 }
+
+# entries of pu_call_packed, and their words: whole numbers and pointers, scales as doubles
+DECODE_PAGED_GQA, DECODE_PAGED_HEADS, DECODE_PAGED_SHARED, PAGE_BOUNDS, SELECT_PAGES = range(5)
+pack_decode = struct.Struct("<18q3dq").pack
+pack_shared = struct.Struct("<21q3dq").pack
+pack_bounds = struct.Struct("<10q").pack
+pack_select = struct.Struct("<19q").pack
 
 _lock = threading.Lock()
 _lib = None
@@ -169,6 +179,16 @@ def check(code: int, where: str) -> None:
 # first, which costs more than a small kernel's launch)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
     (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+_empty_strided = getattr(getattr(getattr(torch._C, "_dynamo", None), "guards", None), "_empty_strided_cuda", None)
+
+
+def empty(shape, strides, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    """A new tensor on `device`, which is current: a third of torch.empty's time for the outputs of a small call."""
+    if _empty_strided is not None:
+        return _empty_strided(shape, strides, dtype)
+    return torch.empty_strided(shape, strides, dtype=dtype, device=device)
 
 
 # the current device's index, without the public call's checks

@@ -135,19 +135,19 @@ def paged_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
         sm_scale = 1.0 / math.sqrt(D)
     lib = _lib.lib()
     with _lib.on_device(dev) as stream:
-        o = torch.empty_like(q, dtype=torch.bfloat16)
-        lse = torch.empty((B, H), dtype=torch.float32, device=dev)
+        o = _lib.empty((B, H, 1, D), (H * D, D, D, 1), torch.bfloat16, dev)
+        lse = _lib.empty((B, H), (H, 1), torch.float32, dev)
         if B == 0:
             return (o, lse) if return_lse else o
         if shared_lens is not None and (k_pool.dtype == q.dtype or (D == 128 and k_pool.dtype not in _DT)):
             groups = shared_lens.numel()
             ws = DecodeWorkspace.get(dev, _shared_bytes(dev.index, B, H, H_kv, groups, D), _cta_counters(dev.index))
-            _lib.check(lib.pu_decode_paged_shared(
+            _lib.check(lib.pu_call_packed(_lib.DECODE_PAGED_SHARED, _lib.pack_shared(
                 q.data_ptr(), _DT[q.dtype], k_pool.data_ptr(), v_pool.data_ptr(), _DT_KV[k_pool.dtype],
                 page_table.data_ptr(), max_pages, P, page_size, kv_lens.data_ptr(), shared_lens.data_ptr(),
-                None if shared_groups is None else shared_groups.data_ptr(), groups, o.data_ptr(), lse.data_ptr(),
-                ws.data_ptr(), ws.numel(), B, H, H_kv, D, float(sm_scale), float(k_scale), float(v_scale),
-                stream), "pu_decode_paged_shared")
+                0 if shared_groups is None else shared_groups.data_ptr(), groups, o.data_ptr(), lse.data_ptr(),
+                ws.data_ptr(), ws.numel(), B, H, H_kv, D, sm_scale, k_scale, v_scale, stream)),
+                "pu_decode_paged_shared")
         elif not by_head and H == H_kv and k_pool.dtype in _DT and k_scale == 1.0 and v_scale == 1.0:
             need = int(lib.pu_decode_paged_workspace_size(B, H, max_pages, page_size, D))
             ws = DecodeWorkspace.get(dev, need, 4 * B * H)
@@ -160,12 +160,12 @@ def paged_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
             # a counter for each CTA (one an SM), or in the query-head kernel for each head
             ws = DecodeWorkspace.get(dev, _gqa_bytes(dev.index, B, H, H_kv, max_pages, page_size, D),
                                      max(4 * B * H, _cta_counters(dev.index)))
-            call = lib.pu_decode_paged_heads if by_head else lib.pu_decode_paged_gqa
-            _lib.check(call(q.data_ptr(), _DT[q.dtype], k_pool.data_ptr(), v_pool.data_ptr(), _DT_KV[k_pool.dtype],
-                            page_table.data_ptr(), max_pages, P, page_size, kv_lens.data_ptr(), o.data_ptr(),
-                            lse.data_ptr(), ws.data_ptr(), ws.numel(), B, H, H_kv, D, float(sm_scale),
-                            float(k_scale), float(v_scale), stream),
-                       "pu_decode_paged_heads" if by_head else "pu_decode_paged_gqa")
+            _lib.check(lib.pu_call_packed(
+                _lib.DECODE_PAGED_HEADS if by_head else _lib.DECODE_PAGED_GQA, _lib.pack_decode(
+                    q.data_ptr(), _DT[q.dtype], k_pool.data_ptr(), v_pool.data_ptr(), _DT_KV[k_pool.dtype],
+                    page_table.data_ptr(), max_pages, P, page_size, kv_lens.data_ptr(), o.data_ptr(), lse.data_ptr(),
+                    ws.data_ptr(), ws.numel(), B, H, H_kv, D, sm_scale, k_scale, v_scale, stream)),
+                "pu_decode_paged_heads" if by_head else "pu_decode_paged_gqa")
     return (o, lse) if return_lse else o
 
 
@@ -233,8 +233,9 @@ def page_bounds(k_pool: torch.Tensor, slots: torch.Tensor, bounds: torch.Tensor)
     if (k_pool.requires_grad or bounds.requires_grad) and torch.is_grad_enabled():
         raise ValueError("page_bounds writes a cache's bounds and has no gradient")
     with _lib.on_device(bounds.device) as stream:
-        _lib.check(_lib.lib().pu_page_bounds(k_pool.data_ptr(), _DT_KV[kind], slots.data_ptr(), bounds.data_ptr(),
-                                             P, pool[2], H_kv, D, slots.numel(), stream), "pu_page_bounds")
+        _lib.check(_lib.lib().pu_call_packed(_lib.PAGE_BOUNDS, _lib.pack_bounds(
+            k_pool.data_ptr(), _DT_KV[kind], slots.data_ptr(), bounds.data_ptr(), P, pool[2], H_kv, D, slots.numel(),
+            stream)), "pu_page_bounds")
 
 
 def select_pages(q: torch.Tensor, bounds: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor, count: int, *,
@@ -273,13 +274,13 @@ def select_pages(q: torch.Tensor, bounds: torch.Tensor, page_table: torch.Tensor
     if not q.is_contiguous():
         q = q.contiguous()
     with _lib.on_device(dev) as stream:
-        pages = torch.empty((B, H_kv, count), dtype=torch.int32, device=dev)
-        lens = torch.empty((B, H_kv), dtype=torch.int32, device=dev)
+        pages = _lib.empty((B, H_kv, count), (H_kv * count, count, 1), torch.int32, dev)
+        lens = _lib.empty((B, H_kv), (H_kv, 1), torch.int32, dev)
         if B:
-            _lib.check(_lib.lib().pu_select_pages(
+            _lib.check(_lib.lib().pu_call_packed(_lib.SELECT_PAGES, _lib.pack_select(
                 q.data_ptr(), _DT[kind], bounds.data_ptr(), _DT[bounds.dtype], page_table.data_ptr(), max_pages, P,
                 page_size, kv_lens.data_ptr(), pages.data_ptr(), lens.data_ptr(), count, first, last, B, H, H_kv, D,
-                stream), "pu_select_pages")
+                stream)), "pu_select_pages")
     return PageSelection(pages, lens)
 
 

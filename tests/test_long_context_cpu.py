@@ -120,3 +120,35 @@ def test_sharing_arguments():
                                   (ints(5, 6, 7)[::2], ints(0, 1, 2), False)]:
         with pytest.raises(ValueError):
             _check_shared(shared, groups, lists, cpu)
+
+
+def test_packed_calls_are_the_entry_points(lib):
+    """pu_call_packed takes the same arguments in the same order: every refusal comes back alike, for each
+    argument changed in turn."""
+    import struct
+    _lib, so = lib
+    scale = [0.1, 1.0, 1.0]
+    cases = [(_lib.DECODE_PAGED_GQA, so.pu_decode_paged_gqa, _lib.pack_decode, [P, BF, P, P, BF, P, 4, 8, 16, P, P, 0, P, 1, 2, 8, 2, 128] + scale + [0]),
+             (_lib.DECODE_PAGED_HEADS, so.pu_decode_paged_heads, _lib.pack_decode, [P, BF, P, P, BF, P, 4, 8, 16, P, P, 0, P, 1, 2, 8, 2, 128] + scale + [0]),
+             (_lib.DECODE_PAGED_SHARED, so.pu_decode_paged_shared, _lib.pack_shared,
+              [P, BF, P, P, BF, P, 4, 8, 16, P, P, P, 2, P, 0, P, 1, 2, 8, 2, 128] + scale + [0]),
+             (_lib.PAGE_BOUNDS, so.pu_page_bounds, _lib.pack_bounds, [P, BF, P, P, 8, 16, 2, 96, 5, 0]),
+             (_lib.SELECT_PAGES, so.pu_select_pages, _lib.pack_select, [P, BF, P, F16, P, 4, 8, 16, P, P, P, 3, 1, 1, 2, 8, 2, 96, 0])]
+    for entry, call, pack, good in cases:
+        seen = set()
+        for i in range(len(good)):
+            for v in ((0.0, -1.0) if isinstance(good[i], float) else (0, -1, 3, P + 8, 1 << 40)):
+                a = list(good)
+                a[i] = v
+                if i in (1, 3, 4) and abs(v) >= 1 << 31:
+                    continue                  # 32-bit arguments
+                if good[i] == 1 and pack is not _lib.pack_bounds and pack is not _lib.pack_select:
+                    continue                  # the workspace's bytes: as they are, every call is refused
+                want = call(*a)
+                text = so.pu_last_error()
+                assert want in (_lib.PU_ERR_INVALID_ARGUMENT, _lib.PU_ERR_UNSUPPORTED, _lib.PU_ERR_WORKSPACE), (entry, i, v)
+                assert so.pu_call_packed(entry, pack(*a)) == want and so.pu_last_error() == text, (entry, i, v)
+                seen.add(text)
+        assert len(seen) > 4
+    assert so.pu_call_packed(5, struct.pack("<q", 0)) == _lib.PU_ERR_INVALID_ARGUMENT
+    assert so.pu_call_packed(0, None) == _lib.PU_ERR_INVALID_ARGUMENT
