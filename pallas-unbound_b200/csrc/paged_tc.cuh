@@ -59,8 +59,9 @@
 // this GPU is 6.4 TB/s): 8 sequences of 4096 to 131072 tokens, 32 heads over 8
 // of 128, f16, 64-token pages: 2.51 GB in 357 us = 7.0 TB/s; 24 sequences of up
 // to 32768 tokens, 64 heads over 8, e4m3, 32-token pages: 0.98 GB in 157 to 166 us =
-// 5.9 to 6.3 TB/s (the splitting of P shares the issue slots with everything else); 256
-// sequences of up to 2048 tokens, 16 heads over 2 of 64, 16-token pages: 135 MB
+// 5.9 to 6.3 TB/s (the splitting of P shares the issue slots with everything
+// else), and 93 of up to 2500 tokens, 0.26 GB in 83 us (their starts and ends);
+// 256 sequences of up to 2048 tokens, 16 heads over 2 of 64, 16-token pages: 135 MB
 // in 39 us, of which 28 us are the loads alone, the rest the start, the last
 // tile's chain and the joins; one sequence of 1000 tokens: 11 us.
 #pragma once
@@ -155,11 +156,11 @@ struct Params {
 };
 
 // x as N e4m3 parts, x ~ sum_i part_i / kPartScale^i: each part is the e4m3
-// rounding of what the ones before left, times kPartScale when `scaled` (a
-// remainder of a value up to 256 is at most 8, so 32 keeps it below 256).
+// rounding of what the ones before left, times kPartScale (a remainder of a
+// value up to 256 is at most 8, so 32 keeps it below 256).
 constexpr float kPartScale = 32.f;
 
-template <bool scaled, int N>
+template <int N>
 __device__ __forceinline__ void split_e4m3(float a, float b, uint16_t (&part)[N]) {
 #pragma unroll
   for (int i = 0; i < N; ++i) {
@@ -167,10 +168,18 @@ __device__ __forceinline__ void split_e4m3(float a, float b, uint16_t (&part)[N]
     part[i] = (uint16_t)h2;
     if (i + 1 < N) {
       const float2 hf = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(h2, __NV_E4M3)));
-      a = (a - hf.x) * (scaled ? kPartScale : 1.f);
-      b = (b - hf.y) * (scaled ? kPartScale : 1.f);
+      a = (a - hf.x) * kPartScale;
+      b = (b - hf.y) * kPartScale;
     }
   }
+}
+
+// The larger magnitudes of two pairs (a NaN counts as nothing).
+template <typename T>
+__device__ __forceinline__ uint32_t pair_abs_max(uint32_t a, uint32_t b) {
+  using V = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+  const V r = __hmax2(*reinterpret_cast<const V*>(&a), __habs2(*reinterpret_cast<const V*>(&b)));
+  return *reinterpret_cast<const uint32_t*>(&r);
 }
 
 // The tiles of this CTA in order.  An item is (sequence b, inner index r =
@@ -519,66 +528,113 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
       for (int i = max(0, n - NS); i < n; ++i) mbar_wait(bFull + i % NS, (i / NS) & 1, &no_abort, kSiteDecodeTc);
     } else if (warp == kQueryWarp) {
       // ---------------- queries -> shared memory ----------------
-      int done = -1;                         // last segment staged
-      for (Walk w = w0; w.left > 0; w.next()) {
-        if (w.seg == done) continue;
-        done = w.seg;
-        const int slot = w.seg % kQSlots;
-        if (w.seg >= kQSlots &&
-            !__all_sync(0xffffffffu, mbar_wait(bQfree + slot, (w.seg / kQSlots - 1) & 1, abort_flag, kSiteDecodeTc)))
-          break;
-        const int slice = w.r % p.slices, heads = min(NP, p.group - slice * NP);
-        const T* q = static_cast<const T*>(p.q) + ((size_t)w.b * p.H + (w.r / p.slices) * p.group + slice * NP) * D;
-        uint8_t* dst = sQ + slot * C::kQBytes;
-        constexpr int kVecs = D / 8;         // 16-byte vectors of a row
-        constexpr int kHold = NP * kVecs / 64;   // vectors a lane holds, in two rounds
+      constexpr int kVecs = D / 8, kRows = 32 / kVecs;       // 16-byte vectors of a row, rows at once
+      const int c = lane % kVecs;
+      auto rows_of = [&](const Walk& w, int* heads) {
+        const int slice = w.r % p.slices;
+        *heads = min(NP, p.group - slice * NP);
+        return static_cast<const T*>(p.q) + ((size_t)w.b * p.H + (w.r / p.slices) * p.group + slice * NP) * D + lane * 8;
+      };
+      if constexpr (!kF8) {
+        int done = -1;                       // last segment staged
+        for (Walk w = w0; w.left > 0; w.next()) {
+          if (w.seg == done) continue;
+          done = w.seg;
+          const int slot = w.seg % kQSlots;
+          if (w.seg >= kQSlots &&
+              !__all_sync(0xffffffffu, mbar_wait(bQfree + slot, (w.seg / kQSlots - 1) & 1, abort_flag, kSiteDecodeTc)))
+            break;
+          int heads;
+          const T* q = rows_of(w, &heads);
+          uint8_t* dst = sQ + slot * C::kQBytes;
+          constexpr int kHold = NP / kRows / 2;              // vectors a lane holds, in two rounds
 #pragma unroll
-        for (int i0 = 0; i0 < 2 * kHold; i0 += kHold) {
-          uint4 v[kHold];
+          for (int i0 = 0; i0 < 2 * kHold; i0 += kHold) {
+            uint4 v[kHold];
 #pragma unroll
-          for (int i = 0; i < kHold; ++i) {
-            const int h = ((i0 + i) * 32 + lane) / kVecs, c = ((i0 + i) * 32 + lane) % kVecs;
-            v[i] = make_uint4(0u, 0u, 0u, 0u);
-            if (h < heads) v[i] = *reinterpret_cast<const uint4*>(q + (size_t)h * D + c * 8);
-          }
+            for (int i = 0; i < kHold; ++i) {
+              v[i] = make_uint4(0u, 0u, 0u, 0u);
+              if ((i0 + i) * kRows + lane / kVecs < heads) v[i] = *reinterpret_cast<const uint4*>(q + (i0 + i) * 256);
+            }
 #pragma unroll
-          for (int i = 0; i < kHold; ++i) {
-            const int h = ((i0 + i) * 32 + lane) / kVecs, c = ((i0 + i) * 32 + lane) % kVecs;
-            if constexpr (!kF8) {
+            for (int i = 0; i < kHold; ++i) {
+              const int h = (i0 + i) * kRows + lane / kVecs;
               *reinterpret_cast<uint4*>(dst + (c >> 3) * C::kQBlock + h * 128 + (((c & 7) ^ (h & 7)) << 4)) = v[i];
+            }
+          }
+          fence_proxy_async_smem();
+          mbar_arrive(bQfull + slot);
+        }
+      } else {
+        // A segment's rows are asked for ahead, and the loop that splits them is not
+        // unrolled: under a saturated memory both the loads and the fetch of code that runs
+        // once a segment take 2 us and more (7 us a segment, which bounded CTAs of short
+        // sequences: 93 of up to 2500 tokens took 92 us, now 83)
+        int heads = 0;
+        const T* next = nullptr;
+        auto ask = [&](const Walk& w) {
+          next = rows_of(w, &heads);
+          if (lane * 64 < heads * D) asm volatile("prefetch.global.L1 [%0];" ::"l"(next + lane * 56));
+        };
+        if (w0.left > 0) ask(w0);
+        for (Walk w = w0; w.left > 0;) {
+          const int seg = w.seg, slot = seg % kQSlots, rows = heads;
+          const T* q = next;
+          w.next(min(w.left, w.tiles - w.t));
+          if (w.left > 0) ask(w);
+          if (seg >= kQSlots &&
+              !__all_sync(0xffffffffu, mbar_wait(bQfree + slot, (seg / kQSlots - 1) & 1, abort_flag, kSiteDecodeTc)))
+            break;
+          uint8_t* dst = sQ + slot * C::kQBytes;
+#pragma unroll 1
+          for (int i = 0; i < NP / kRows; ++i) {
+            const int h = i * kRows + lane / kVecs;
+            uint4 x4 = make_uint4(0u, 0u, 0u, 0u);
+            if (h < rows) x4 = *reinterpret_cast<const uint4*>(q + i * 256);
+            // scaled by a power of two so that the head's largest |q| lies in
+            // [128, 256), then split; 16 lanes hold a head.  Rows that hold no
+            // head are zeros.  The parts are worked out in f16 pairs, which hold
+            // a scaled q exactly as far as e4m3 parts reach.
+            uint32_t wd[kQParts][2];
+            if (i * kRows >= rows) {
+#pragma unroll
+              for (int j = 0; j < kQParts; ++j) wd[j][0] = wd[j][1] = 0u;
+              if (c == 0) s_qinv[slot * NP + h] = 1.f;
             } else {
-              // scaled by a power of two so that the head's largest |q| lies in
-              // [128, 256), then split; 16 lanes hold a head
+              const uint32_t in[4] = {x4.x, x4.y, x4.z, x4.w};
+              uint32_t top = 0u;
+#pragma unroll
+              for (int k = 0; k < 4; ++k) top = pair_abs_max<T>(top, in[k]);
+#pragma unroll
+              for (int off = 8; off > 0; off >>= 1) top = pair_abs_max<T>(top, __shfl_xor_sync(0xffffffffu, top, off));
               float x[8];
-              unpack8<T>(v[i], x);
-              float mx = 0.f;
-#pragma unroll
-              for (int k = 0; k < 8; ++k) mx = fmaxf(mx, fabsf(x[k]));
-#pragma unroll
-              for (int off = 8; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+              unpack8<T>(make_uint4(top, 0u, 0u, 0u), x);
+              const float mx = fmaxf(x[0], x[1]);
               const int e = (mx > 0.f && isfinite(mx)) ? ((__float_as_int(mx) >> 23) & 0xff) - 127 : 7;
               const int sh = min(126, 7 - e);      // -120 at least: 2^sh and 2^-sh are both normal numbers
               const float up = __int_as_float((127 + sh) << 23), down = __int_as_float((127 - sh) << 23);
-              uint32_t wd[kQParts][2];
+              unpack8<T>(x4, x);
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
-                uint16_t pr[kQParts];
-                split_e4m3<false>(x[2 * k] * up, x[2 * k + 1] * up, pr);
+                __half2 y = __floats2half2_rn(x[2 * k] * up, x[2 * k + 1] * up);
 #pragma unroll
-                for (int j = 0; j < kQParts; ++j)
-                  wd[j][k >> 1] = (k & 1) ? (wd[j][k >> 1] | ((uint32_t)pr[j] << 16)) : (uint32_t)pr[j];
+                for (int j = 0; j < kQParts; ++j) {
+                  const __nv_fp8x2_storage_t h2 = __nv_cvt_halfraw2_to_fp8x2(__half2_raw(y), __NV_SATFINITE, __NV_E4M3);
+                  wd[j][k >> 1] = (k & 1) ? (wd[j][k >> 1] | ((uint32_t)h2 << 16)) : (uint32_t)h2;
+                  if (j + 1 < kQParts) y = __hsub2(y, __half2(__nv_cvt_fp8x2_to_halfraw2(h2, __NV_E4M3)));
+                }
               }
-              const int at = h * 128 + (((c >> 1) ^ (h & 7)) << 4) + (c & 1) * 8;
-#pragma unroll
-              for (int j = 0; j < kQParts; ++j)
-                *reinterpret_cast<uint2*>(dst + j * C::kQBlock + at) = make_uint2(wd[j][0], wd[j][1]);
               // a head that is not finite makes its scores NaN, as it would in 16 bits
               if (c == 0) s_qinv[slot * NP + h] = isfinite(mx) ? down : mx - mx;
             }
+            const int at = h * 128 + (((c >> 1) ^ (h & 7)) << 4) + (c & 1) * 8;
+#pragma unroll
+            for (int j = 0; j < kQParts; ++j)
+              *reinterpret_cast<uint2*>(dst + j * C::kQBlock + at) = make_uint2(wd[j][0], wd[j][1]);
           }
+          fence_proxy_async_smem();
+          mbar_arrive(bQfull + slot);
         }
-        fence_proxy_async_smem();
-        mbar_arrive(bQfull + slot);
       }
     } else if (warp == kScoreWarp) {
       // ---------------- tcgen05: S products ----------------
@@ -748,7 +804,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
             mbar_wait(bPv + grp, (mine - 1) & 1, abort_flag, kSiteDecodeTc);
             __syncwarp();
             tc_fence_after();
-#pragma unroll
+#pragma unroll 1
             for (int k = 0; k < kPParts; ++k) {
               uint32_t ov[NP];
               const uint32_t at = tmem + lane_base + C::kColO + (par * kGroups + grp) * C::kOCols + k * NP;
@@ -790,7 +846,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
 #pragma unroll
             for (int h = h0; h < h0 + 4; h += 2) {
               uint16_t part[kPParts];
-              split_e4m3<true>(pr[h], pr[h + 1], part);
+              split_e4m3(pr[h], pr[h + 1], part);
               const int o0 = h * 128 + ((chunk ^ (h & 7)) << 4), o1 = (h + 1) * 128 + ((chunk ^ ((h + 1) & 7)) << 4);
 #pragma unroll
               for (int k = 0; k < kPParts; ++k) {
@@ -857,12 +913,13 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
       float oa[NP];                        // thread `row`: column row of o
 #pragma unroll
       for (int h = 0; h < NP; ++h) oa[h] = 0.f;
-#pragma unroll
+      // (e4m3: not unrolled, six times the code that runs once a segment would be fetched)
+#pragma unroll (kF8 ? 1 : kGroups)
       for (int g = 0; g < kGroups; ++g) {
         // a group has an accumulator iff it took a tile
         if (!(n > 1 || (t & 1) == g)) continue;
         float wk = 1.f;
-#pragma unroll
+#pragma unroll 1
         for (int k = 0; k < kPParts; ++k, wk *= 1.f / kPartScale) {
           uint32_t ov[NP];
           tmem_ld16(tmem + lane_base + C::kColO + (par * kGroups + g) * C::kOCols + k * NP, ov);
