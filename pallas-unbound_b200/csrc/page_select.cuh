@@ -598,14 +598,19 @@ __global__ void __launch_bounds__(kThreads, 2) select_kernel(const Params p) {
     const int begin = from + (rank * kWarps + warp) * per, end = min(to, begin + per);
     const int steps = max(0, (end - begin + 7) >> 3);
     uint8_t* ring = dyn + p.ring + (warp * p.stages * 2 * kChunks * 32 + lane) * 16;
-    int row = -1;                        // of a table entry for each lane: its bounds' place; negative: not in the pool
+    // table entries of 32 pages at a time, the next 32 on their way
+    auto look_up = [&](int i) { return i + lane < end ? table[i + lane] : 0; };
+    int entry = look_up(begin), ahead = look_up(begin + 32);
+    int row = -1;                        // of an entry for each lane: its bounds' place; negative: not in the pool
     bool outside = false;                // the warp has seen such an entry
     int to_stage = 0, from_stage = 0;
     auto begin_step = [&](int k) {       // copies of pages begin + 8 k + 4 u + sub
       if ((k & 3) == 0) {
-        const int i = begin + 8 * k + lane, pg = i < end ? table[i] : 0;
-        const bool bad = i < end && (unsigned)pg >= (unsigned)p.num_pages;
-        row = bad || i >= end ? -1 : pg * p.H_kv + head;
+        const int i = begin + 8 * k + lane;
+        const bool bad = i < end && (unsigned)entry >= (unsigned)p.num_pages;
+        row = bad || i >= end ? -1 : entry * p.H_kv + head;
+        entry = ahead;
+        ahead = look_up(begin + 8 * k + 64);
         if (__any_sync(0xffffffffu, bad)) {
           if (bad) record_device_error(PU_ERR_INVALID_ARGUMENT, kSiteSelectPage);
           outside = true;
