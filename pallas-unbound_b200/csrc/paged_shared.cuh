@@ -75,8 +75,8 @@ struct Cfg {
   static constexpr int kBars = 2 * NK + 2 * NV + 4 * NS + 8 + 3;
   static constexpr int kOffMisc = kOffBar + kBars * 8;                 // tmem base, abort flag
   static constexpr int kOffBad = kOffMisc + 8;                         // [kBadRing] which 16 tokens of a tile were not loaded
-  static constexpr int kOffScale = kOffBad + kBadRing * 4;             // [kRows] what undoes a row's scale (e4m3)
-  static constexpr int kOffGroups = (kOffScale + (kF8 ? kRows * 4 : 0) + 7) / 8 * 8;
+  static constexpr int kOffScale = kOffBad + kBadRing * 4;             // [2 runs][kRows] exponent of what undoes a row's scale (e4m3)
+  static constexpr int kOffGroups = (kOffScale + (kF8 ? 2 * kRows : 0) + 7) / 8 * 8;
   static constexpr int kSmem = kOffGroups + 16 * (kMaxGroups + 1);
   static_assert(kSmem <= 232448, "shared memory of one CTA");
 };
@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(Cfg<T, KVT, D>::kThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kOffMisc + 4);
   volatile uint32_t* s_bad = reinterpret_cast<volatile uint32_t*>(smem + C::kOffBad);
-  float* s_scale = reinterpret_cast<float*>(smem + C::kOffScale);
+  uint8_t* s_scale = smem + C::kOffScale;
   Group* s_groups = reinterpret_cast<Group*>(smem + C::kOffGroups);
 
   if (tid == 0) {
@@ -583,7 +583,7 @@ __global__ void __launch_bounds__(Cfg<T, KVT, D>::kThreads, 1)
           if constexpr (kF8) {
             float x[8];
             unpack8<T>(v[u], x);
-            float down = 1.f;
+            int down = 127;              // of 2^0
             if constexpr (std::is_same<T, __nv_bfloat16>::value) {
               // by a power of two that puts the row's largest |q| into [2^14, 2^15): bf16's 8 bits
               // are f16 values down to 2^-31 of it
@@ -595,11 +595,14 @@ __global__ void __launch_bounds__(Cfg<T, KVT, D>::kThreads, 1)
               const int e = (mx > 0.f && isfinite(mx)) ? ((__float_as_int(mx) >> 23) & 0xff) - 127 : 14;
               const int sh = min(126, 14 - e);
               const float up = __int_as_float((127 + sh) << 23);
-              down = __int_as_float((127 - sh) << 23);
+              down = 127 - sh;
 #pragma unroll
               for (int k = 0; k < 8; ++k) x[k] *= up;
             }
-            if (c == 0) s_scale[r] = down;
+            // Two buffers: both slots' threads stage rows that both slots read, and where a run has two
+            // jobs a slot can end it, and stage the next, before a warp of the other has read its scale.
+            // The run after that has products only once every thread has staged its part of the next.
+            if (c == 0) s_scale[(w.seg & 1) * kRows + r] = (uint8_t)down;
             v[u] = make_uint4(pack16<__half>(x[0], x[1]), pack16<__half>(x[2], x[3]), pack16<__half>(x[4], x[5]), pack16<__half>(x[6], x[7]));
           }
           *reinterpret_cast<uint4*>(sQ + (r >> 7) * kTile + (c >> 3) * (BT * 128) + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[u];
@@ -612,7 +615,7 @@ __global__ void __launch_bounds__(Cfg<T, KVT, D>::kThreads, 1)
       float scale = p.scale_log2;
       if constexpr (kF8) {
         mbar_wait(bQ, w.seg & 1, abort_flag, kSiteDecodeTc);
-        scale *= s_scale[item_row];
+        scale *= __uint_as_float((uint32_t)s_scale[(w.seg & 1) * kRows + item_row] << 23);
       }
       float m = -INFINITY, l = 0.f;
       const int jobs = w.jobs(), step = w.split ? 0 : 1;
