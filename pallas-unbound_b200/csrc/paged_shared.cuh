@@ -35,6 +35,8 @@
 // once to the operands' type; sums and maxima are fp32.
 #pragma once
 
+#include <cfloat>
+
 #include "paged_tc.cuh"
 
 namespace pu {
@@ -971,6 +973,16 @@ int pu_decode_paged_shared(const void* q, int q_dtype, const void* k_pool, const
   CUtensorMap tk, tv;
   rc = ptc::make_maps(&tk, &tv, k_pool, v_pool, kv_dtype, num_pages, H_kv, shift, prm.box, (int)D);
   if (rc) return rc;
+  // The prefix pass masks scores and takes their maximum before it scales them, which saves a product a score and
+  // is the same only for a positive factor.  With any other (NaN too) all tokens are each sequence's own.
+  if (!(prm.scale_log2 >= FLT_MIN && prm.scale_log2 <= FLT_MAX)) {
+    own.lens = kv_lens;
+    own.skip = nullptr;
+    own.o32 = nullptr;
+    own.o = static_cast<__nv_bfloat16*>(o);
+    own.lse = lse;
+    return ptc::launch_with(tk, tv, own, q_dtype, kv_dtype, (int)D, st);
+  }
   if (f8)
     rc = h ? shared::launch_as<__half, __nv_fp8_e4m3, 128>(tk, tv, prm, st)
            : shared::launch_as<__nv_bfloat16, __nv_fp8_e4m3, 128>(tk, tv, prm, st);

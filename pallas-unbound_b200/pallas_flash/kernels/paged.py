@@ -110,7 +110,8 @@ def paged_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     shared_lens[i] tokens, which are then read once for the group, through the
     table row of one of its sequences.  Only whole pages are shared.  A sequence
     that holds fewer tokens than that attends them by itself; a group in which
-    none holds as many shares nothing, nor does a call where that would save little.
+    none holds as many shares nothing, nor does a call where that would save little or
+    whose scale is not positive.
     The result is that of the call without
     it, up to the order of sums, and where q and the pools have different 16-bit
     types, or e4m3 pools heads of 64, it is that call."""
