@@ -501,6 +501,38 @@ PU_API int pu_page_plan(const int32_t* page_table, int32_t* page_table_out,
                         int64_t B, int64_t num_tokens, void* stream);
 
 /*
+ * Sequences that begin with pages of another one.  No counterpart in the reference.
+ *   shared_lens int32 [B]: tokens at the front of each sequence, whole pages, that are
+ *     another one's; sources int32 [B]: whose (any value where shared_lens is 0).
+ * Both begin as zeros and belong to the state of the cache, like its lengths.
+ *
+ * pu_page_share puts the first `tokens` (whole pages) of sequence `source` in front of
+ * the listed sequences (int64 [n], negative: from the batch's end), which must be
+ * empty; pages that the source has itself from another sequence count as that one's
+ * where they are all.  With source = -1 it takes the first `tokens` out of sequences
+ * that share as many, which leaves their own.  A sequence for which that cannot be
+ * done stays as it is and is reported (PU_ERR_INVALID_ARGUMENT, detail 311): it is out of range, not
+ * empty or the source itself, the source holds fewer tokens, it shares fewer than are
+ * to be taken out, or others hold its pages.  A sequence listed twice counts once.
+ *
+ * pu_page_plan_shared is pu_page_plan in place, and a release returns only a
+ * sequence's own pages; shared_lens becomes 0 and sources -1 there.  A release of a sequence whose
+ * pages others hold that are not released in the call is refused: it keeps its pages
+ * and length, its rows get slot -1, and it is reported (detail 311).
+ */
+PU_API int pu_page_share(int32_t* page_table, int64_t max_pages_per_seq, int64_t page_size,
+                         int32_t* kv_lens, int32_t* shared_lens, int32_t* sources,
+                         const int64_t* sequences, int64_t n, int64_t source, int64_t tokens,
+                         int64_t B, void* stream);
+
+PU_API int pu_page_plan_shared(int32_t* page_table, int64_t max_pages_per_seq, int32_t* kv_lens,
+                               const int32_t* new_lens, const uint8_t* release,
+                               int32_t* free_ring, int64_t num_pages, int64_t* cursor,
+                               int64_t page_size, int32_t* slots, int32_t* positions,
+                               int32_t* seq_ids, int32_t* cu_new, int32_t* shared_lens,
+                               int32_t* sources, int64_t B, int64_t num_tokens, void* stream);
+
+/*
  * Norms of queries and keys for each head with the position rotation in the
  * same pass.  No counterpart in the reference (its attention takes q, k, v as
  * they are, src/pallas_flash/ops/interface.py:20-27).  For a row x of D values

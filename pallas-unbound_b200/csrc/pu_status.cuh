@@ -46,6 +46,7 @@ enum WaitSite : int {
   kSiteFreePages = 308,
   kSitePageBounds = 309,
   kSiteSelectPage = 310,
+  kSitePageShare = 311,
   kSiteOutProj = 401,
   kSiteSelfTest = 901,
 };

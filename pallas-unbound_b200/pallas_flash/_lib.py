@@ -116,6 +116,11 @@ SIGNATURES = {
     "pu_page_plan": (_int, [_c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
                             _c_void_p, _i64, _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p,
                             _c_void_p, _c_void_p, _i64, _i64, _c_void_p]),
+    "pu_page_share": (_int, [_c_void_p, _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64,
+                             _i64, _i64, _c_void_p]),
+    "pu_page_plan_shared": (_int, [_c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p,
+                                   _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64,
+                                   _i64, _c_void_p]),
     # the description (pu_qk_rope_desc) is passed as packed bytes
     "pu_qk_norm_rope_fwd": (_int, [_c_void_p] * 6),
     "pu_qk_norm_rope_bwd_workspace_size": (_size_t, [_i64]),

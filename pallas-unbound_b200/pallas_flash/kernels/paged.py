@@ -316,7 +316,8 @@ class AppendPlan(NamedTuple):
 
 def plan_append(page_table: torch.Tensor, kv_lens: torch.Tensor, new_lens: torch.Tensor,
                 free_ring: torch.Tensor, cursor: torch.Tensor, *, page_size: int, num_tokens: int,
-                release: Optional[torch.Tensor] = None, inplace: bool = False) -> AppendPlan:
+                release: Optional[torch.Tensor] = None, inplace: bool = False,
+                shared_lens: Optional[torch.Tensor] = None, sources: Optional[torch.Tensor] = None) -> AppendPlan:
     """Table rows, slots and positions of a batch's next tokens, on the device.
 
     kv_lens, new_lens int32 [B]: tokens held, and tokens that each sequence
@@ -338,7 +339,13 @@ def plan_append(page_table: torch.Tensor, kv_lens: torch.Tensor, new_lens: torch
 
     With `inplace` the table, lengths and cursor are advanced where they are
     (the same tensors come back); otherwise new ones are returned and only the
-    ring's places behind its tail are written."""
+    ring's places behind its tail are written.
+
+    shared_lens and sources int32 [B] (with `inplace`) say which sequences begin with
+    pages of another one: sequence b's first shared_lens[b] tokens are sources[b]'s
+    (DevicePagedKVCache.share).  A release then returns only a sequence's own pages and
+    clears its entries; a sequence whose pages others hold that are not
+    released with it is not released, its rows get slot -1, and it is reported (detail 311)."""
     if page_table.dim() != 2 or page_table.dtype != torch.int32:
         raise ValueError("page_table must be int32 [B, max_pages_per_seq]")
     B, max_pages = page_table.shape
@@ -356,6 +363,12 @@ def plan_append(page_table: torch.Tensor, kv_lens: torch.Tensor, new_lens: torch
     if release is not None and (release.dtype not in (torch.bool, torch.uint8) or release.shape != (B,)
                                 or release.device != dev or not release.is_contiguous()):
         raise ValueError(f"release must be a contiguous bool [{B}] on {dev}")
+    if shared_lens is not None or sources is not None:
+        if not inplace or shared_lens is None or sources is None:
+            raise ValueError("shared_lens and sources come together, with inplace")
+        for t in (shared_lens, sources):
+            if t.dtype != torch.int32 or t.shape != (B,) or t.device != dev or not t.is_contiguous():
+                raise ValueError(f"shared_lens and sources must be contiguous int32 [{B}] on {dev}")
     if inplace and abs(new_lens.data_ptr() - kv_lens.data_ptr()) < 4 * B:
         raise ValueError("new_lens must not overlap kv_lens when they are advanced in place")
     T = int(num_tokens)
@@ -368,6 +381,13 @@ def plan_append(page_table: torch.Tensor, kv_lens: torch.Tensor, new_lens: torch
             table_out, lens_out, cursor_out = page_table, kv_lens, cursor
         else:
             table_out, cursor_out = torch.empty_like(page_table), torch.empty_like(cursor)
+        if shared_lens is not None and release is not None:
+            _lib.check(_lib.lib().pu_page_plan_shared(
+                page_table.data_ptr(), max_pages, kv_lens.data_ptr(), new_lens.data_ptr(), release.data_ptr(),
+                free_ring.data_ptr(), free_ring.numel(), cursor.data_ptr(), int(page_size), slots.data_ptr(),
+                positions.data_ptr(), seq_ids.data_ptr(), cu.data_ptr(), shared_lens.data_ptr(), sources.data_ptr(),
+                B, T, stream), "pu_page_plan_shared")
+            return AppendPlan(slots, positions, seq_ids, cu, lens_out, cursor_out, table_out)
         _lib.check(_lib.lib().pu_page_plan(
             page_table.data_ptr(), table_out.data_ptr(), max_pages, kv_lens.data_ptr(), lens_out.data_ptr(),
             new_lens.data_ptr(), None if release is None else release.data_ptr(), free_ring.data_ptr(),
@@ -599,12 +619,17 @@ class DevicePagedKVCache:
         self.kv_lens = torch.zeros(batch, dtype=torch.int32, device=device)
         self.free_ring = torch.arange(num_pages, dtype=torch.int32, device=device)
         self.cursor = torch.tensor([0, num_pages], dtype=torch.int64, device=device)
+        # tokens at the front of each sequence that are another one's, and whose (share)
+        self.shared_lens, self.sources = torch.zeros_like(self.kv_lens), torch.full_like(self.kv_lens, -1)
 
     def plan(self, new_lens: torch.Tensor, *, num_tokens: int,
              release: Optional[torch.Tensor] = None) -> AppendPlan:
-        """Map pages for new_lens [B] more tokens and advance the lengths (plan_append in place)."""
+        """Map pages for new_lens [B] more tokens and advance the lengths (plan_append in place).
+        A released sequence that shares pages gives them up; one whose pages others share stays
+        until they are released or `unshare` (or are in the same call), and is reported (detail 311)."""
         return plan_append(self.page_table, self.kv_lens, new_lens, self.free_ring, self.cursor,
-                           page_size=self.page_size, num_tokens=num_tokens, release=release, inplace=True)
+                           page_size=self.page_size, num_tokens=num_tokens, release=release, inplace=True,
+                           shared_lens=self.shared_lens, sources=self.sources)
 
     def append(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: AppendPlan, inv_freq: torch.Tensor, *,
                positions: Optional[torch.Tensor] = None, **norm) -> torch.Tensor:
@@ -619,23 +644,39 @@ class DevicePagedKVCache:
     def share(self, source: int, sequences: torch.Tensor, tokens: int) -> None:
         """Let empty `sequences` (int64, on the cache's device) begin with the first `tokens`
         of sequence `source`: whole pages of it, which they read and never write.  The pages stay
-        `source`'s: it is released after every sequence that shares them, and a sequence
-        gives them up with `unshare` before it is released."""
-        n = int(tokens) // self.page_size
-        if tokens % self.page_size or not 0 <= n <= self.page_table.shape[1]:
-            raise ValueError(f"{tokens} tokens are not whole pages of {self.page_size} that a table row holds")
-        self.page_table[sequences, :n] = self.page_table[source, :n]
-        self.kv_lens[sequences] = int(tokens)
+        `source`'s, which is not released before the sequences that share them.  A sequence
+        that holds something, or for which `source` does not hold that many tokens, stays
+        as it is and is reported (device_status detail 311)."""
+        B = self.kv_lens.shape[0]
+        if not -B <= int(source) < B:
+            raise ValueError(f"sequence {source} of {B}")
+        self._share(int(source) % B, sequences, tokens)
 
     def unshare(self, sequences: torch.Tensor, tokens: int) -> None:
         """Take the first `tokens`, shared with another sequence, out of `sequences`: what is left of
-        them are their own pages, which can be released."""
-        n = int(tokens) // self.page_size
-        if tokens % self.page_size or not 0 <= n <= self.page_table.shape[1]:
+        them are their own pages (and what else they share).  A release does the same.  A sequence
+        that shares fewer tokens, or whose pages others share, stays as it is and
+        is reported (device_status detail 311)."""
+        self._share(-1, sequences, tokens)
+
+    def _share(self, source: int, sequences: torch.Tensor, tokens: int) -> None:
+        B, max_pages = self.page_table.shape
+        dev = self.page_table.device
+        if tokens % self.page_size or not 0 <= tokens <= max_pages * self.page_size:
             raise ValueError(f"{tokens} tokens are not whole pages of {self.page_size} that a table row holds")
-        rows = self.page_table[sequences]
-        self.page_table[sequences] = torch.cat([rows[:, n:], torch.full_like(rows[:, :n], -1)], 1)
-        self.kv_lens[sequences] = (self.kv_lens[sequences] - int(tokens)).clamp(min=0)
+        at = torch.as_tensor(sequences, device=dev)
+        if at.dtype == torch.bool:
+            at = at.nonzero()
+        elif at.is_floating_point() or at.is_complex():
+            raise ValueError("sequences must be whole numbers")
+        at = at.to(torch.int64).reshape(-1).contiguous()
+        if not at.is_cuda:
+            raise ValueError("the cache must be on a CUDA device")
+        with _lib.on_device(dev) as stream:
+            _lib.check(_lib.lib().pu_page_share(
+                self.page_table.data_ptr(), max_pages, self.page_size, self.kv_lens.data_ptr(),
+                self.shared_lens.data_ptr(), self.sources.data_ptr(), at.data_ptr(), at.numel(), source, int(tokens), B,
+                stream), "pu_page_share")
 
     def select(self, q: torch.Tensor, count: int, *, first: int = 1, last: int = 1) -> PageSelection:
         """The pages that q [B,H,1,D] or [B,H,D] attends, for each K/V head (select_pages)."""
