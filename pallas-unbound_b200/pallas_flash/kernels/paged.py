@@ -192,11 +192,17 @@ class PageSelection(NamedTuple):
     lens: torch.Tensor         # int32 [B, H_kv]  tokens in them
 
 
+def _check_bounds_size(D: int):
+    if D != 128 and D != 64:
+        raise ValueError(f"page bounds of head size {D} (supported: 64, 128)")
+
+
 def empty_bounds(k_pool: torch.Tensor) -> torch.Tensor:
     """Room for the bounds of a pool's pages: [num_pages, H_kv, 2, D] in the pool's
     16-bit type, fp16 for an fp8 pool (which holds every e4m3 value).  [..., 0, :] is
-    the minimum and [..., 1, :] the maximum of a page's keys as stored."""
+    the minimum and [..., 1, :] the maximum of a page's keys as stored.  D is 64 or 128."""
     P, H_kv, _, D = k_pool.shape
+    _check_bounds_size(D)
     return torch.zeros((P, H_kv, 2, D), dtype=k_pool.dtype if k_pool.dtype in _DT else torch.float16,
                        device=k_pool.device)
 
@@ -204,8 +210,7 @@ def empty_bounds(k_pool: torch.Tensor) -> torch.Tensor:
 def _check_bounds(bounds: torch.Tensor, shape):
     if len(shape) != 4 or shape[2] != 2 or bounds.dtype not in _DT:
         raise ValueError("bounds must be fp16/bf16 [num_pages, H_kv, 2, D]")
-    if shape[3] != 128 and shape[3] != 64:
-        raise ValueError(f"page bounds of head size {shape[3]} (supported: 64, 128)")
+    _check_bounds_size(shape[3])
     if bounds.get_device() < 0 or not bounds.is_contiguous():
         raise ValueError("bounds must be a contiguous CUDA tensor")
 
