@@ -188,10 +188,15 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
 
 _empty_strided = getattr(getattr(getattr(torch._C, "_dynamo", None), "guards", None), "_empty_strided_cuda", None)
 
+# dispatch modes in force
+_modes = getattr(torch._C, "_len_torch_dispatch_stack", None) or (lambda: 1)
+
 
 def empty(shape, strides, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
-    """A new tensor on `device`, which is current: a third of torch.empty's time for the outputs of a small call."""
-    if _empty_strided is not None:
+    """A new tensor on `device`, which is current: a third of torch.empty's time for the outputs of a small call.
+    That function goes past the dispatcher, so dispatch modes and the deterministic fill of new memory, which
+    act there, get torch.empty_strided."""
+    if _empty_strided is not None and not _modes() and not torch._C._get_deterministic_algorithms():
         return _empty_strided(shape, strides, dtype)
     return torch.empty_strided(shape, strides, dtype=dtype, device=device)
 
