@@ -222,7 +222,10 @@ constexpr int kBins = 1024;
 constexpr int kRank = kThreads;          // as many candidates are ranked against each other
 constexpr int kMaxPages = 24576;         // scores of a sequence that one CTA's shared memory holds
 constexpr int kMaxCtas = 8;              // of a cluster
-constexpr int kFew = 3, kMany = 6;       // stages of a warp's copies, eight pages each
+// Stages of a warp's copies, eight pages each.  Six, where a warp has many steps, leave one CTA an SM: 24 sequences
+// of 131072 tokens, heads of 64, pages of 16 take 131 us instead of 84, three of them 22 instead of 18 (lengths
+// from 0 to 131072: 67 instead of 73).  With heads of 128 they make no difference (52.5 to 53, 98.6 to 99.7).
+constexpr int kStages = 3;
 constexpr float kBig = 0x1p125f;         // fp32 sums from here on are not used
 constexpr uint32_t kOutside = 0x10000u;  // a warp has seen a table entry outside the pool
 
@@ -237,8 +240,10 @@ struct Params {
   int max_pages, num_pages, page_shift;
   int count, first, last;
   int ctas;                    // of a cluster
-  int by_length;               // clusters take the longest sequences first
-  int ring, stages;            // first byte of the copies, behind the scores; kFew or kMany
+  int by_length;               // the longest sequences are placed first
+  int ring;                    // first byte of the copies, behind the scores
+  int stages;                  // kStages, as an argument: known to the compiler, its order of the scoring loop takes 104.5 us
+                               // instead of 98.8 (24 sequences of 131072 tokens, heads of 128), 88 instead of 84 (64)
   int B;
 };
 
@@ -568,7 +573,7 @@ __global__ void __launch_bounds__(kThreads, 2) select_kernel(const Params p) {
   grid_dep_wait();
   grid_dep_launch_dependents();
   if (p.by_length) {
-    // the longest sequences first: the last clusters to start are the short ones
+    // the longest sequences first: they get an SM each while there are any, the short ones the rest
     int* lens = s.bins;
     for (int i = tid; i < p.B; i += kThreads) lens[i] = p.lens[i];
     __syncthreads();
@@ -672,8 +677,7 @@ __global__ void __launch_bounds__(kThreads, 2) select_kernel(const Params p) {
     for (int k = 0; k < steps; ++k) {
       if (k + p.stages - 1 < steps) begin_step(k + p.stages - 1);
       cp_async_commit();
-      if (p.stages == kMany) cp_async_wait<kMany - 1>();
-      else cp_async_wait<kFew - 1>();
+      cp_async_wait<kStages - 1>();
       const uint8_t* src = ring + from_stage * 2 * kChunks * 512;
       from_stage = from_stage + 1 == p.stages ? 0 : from_stage + 1;
       float x[2];
@@ -916,10 +920,8 @@ int launch_select(Params p, long long items, cudaStream_t st) {
   // be held in fp64
   constexpr int kStage = kWarps * 32 * D;
   p.ring = (p.max_pages * (int)sizeof(float) + 15) / 16 * 16;
-  // twice the copies in flight where a warp has many steps, and about one CTA an SM (it then has all of the
-  // SM's shared memory, and the next call's CTAs do not start beside it)
-  p.stages = p.max_pages > 512 * p.ctas && 2 * items * p.ctas <= 3ll * sm_count() && p.ring + kMany * kStage <= 2 * kMaxPages * (int)sizeof(float) ? kMany : kFew;
-  const int ring = std::max(p.stages * kStage, p.ring);
+  p.stages = kStages;
+  const int ring = std::max(kStages * kStage, p.ring);
   const int rc = set_max_dynamic_smem(reinterpret_cast<const void*>(f), 2 * kMaxPages * (int)sizeof(float) + 16, "page choice shared memory");
   if (rc) return rc;
   cudaLaunchConfig_t cfg{};
@@ -1021,7 +1023,10 @@ extern "C" int pu_select_pages(const void* q, int q_dtype, const void* bounds, i
   p.num_pages = (int)num_pages;
   p.page_shift = shift;
   p.B = (int)B;
-  // where the clusters do not all start at once; 256 lengths took 5 us to rank
+  // Where SMs take two CTAs, and while ranking the lengths, which every CTA does, costs less than it gives: 24
+  // sequences of up to 131072 tokens, 8 K/V heads of 128: 52 us with it, 63 without; 40 of them 74.5, 85; 64 of up to
+  // 32768, heads of 64: 22, 25; but 64 of up to 65536, heads of 128: 74, 68; 64 of up to 4000, 4 K/V heads: 11.4, 10.3.
+  // From 65 on it is left out: 65 of up to 32768: 22.7, 26; 128: 34.8, 35; of up to 4000 20, 17.5; 256: 72, 59.
   p.by_length = B > 1 && B <= 64 && B * H_kv * p.ctas > pu::sm_count();
   p.count = (int)count;
   p.first = (int)first;
