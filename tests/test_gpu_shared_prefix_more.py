@@ -1,5 +1,5 @@
 """Shared prefixes where test_gpu_shared_prefix does not reach: many short runs over
-e4m3 pools, scales that are not positive.
+e4m3 pools, scales that are not positive, and that shared pages are read once at all.
 
 Tolerances are those of test_gpu_shared_prefix (its `check`).
 """
@@ -70,3 +70,39 @@ def test_scales_whose_product_vanishes(mods):
     o, lse = paged.paged_decode(q, k, v, table, ints(lens), shared_lens=shared, sm_scale=1e-30, k_scale=1e-30, return_lse=True)
     assert _lib.device_status() == (0, 0)
     check(o, lse, q, k, v, table, lens, scale=0.0, what="product")
+
+
+# --------------------------------------------------------------------------
+# what is shared is read through one row
+# --------------------------------------------------------------------------
+@pytest.mark.parametrize("H,H_kv,D,qdt,kvdt", KINDS)
+@pytest.mark.parametrize("page,tokens", [(16, 144), (64, 960), (256, 2048)])
+def test_others_rows_are_not_read(mods, H, H_kv, D, qdt, kvdt, page, tokens):
+    """Where sequences share, only one row names the shared pages: the others' entries may be anything.
+    With one sequence fewer nothing is shared, and the missing entries are reported."""
+    _lib, dec, paged = mods
+    n = enough(tokens, H, H_kv)
+    own = ([0, 1, 90, 130] + [9] * n)[:n]
+    table, P, lens, shared, _ = batch([(tokens, own)], page, 7)
+    q, k, v = make(P, n, H, H_kv, D, page, qdt, kvdt, 3)
+    lens[0] = tokens - 1                 # the first sequence is too short to be the one that is read
+    bare = table.clone()
+    bare[2:, :tokens // page] = -1
+    o, lse = paged.paged_decode(q, k, v, bare, ints(lens), shared_lens=shared, return_lse=True)
+    assert _lib.device_status() == (0, 0)
+    check(o, lse, q, k, v, table, lens, what="one row")
+    paged.paged_decode(q[:-1], k, v, bare[:-1].contiguous(), ints(lens[:-1]), shared_lens=shared)
+    assert _lib.device_status() == (_lib.PU_ERR_INVALID_ARGUMENT, 302)
+
+
+def test_others_rows_of_several_groups_are_not_read(mods):
+    _lib, dec, paged = mods
+    page, groups = 32, [(960, [5, 0, 70] * 20), (320, [1] * 40), (64, []), (512, [33] * 50)]
+    table, P, lens, shared, starts = batch(groups, page, 3)
+    q, k, v = make(P, len(lens), 8, 2, 128, page, BF, BF, 5)
+    bare, at = table.clone(), starts.tolist()
+    for i, (tokens, _) in enumerate(groups):
+        bare[at[i] + 1:at[i + 1], :tokens // page] = -1
+    o, lse = paged.paged_decode(q, k, v, bare, ints(lens), shared_lens=shared, shared_groups=starts, return_lse=True)
+    assert _lib.device_status() == (0, 0)
+    check(o, lse, q, k, v, table, lens, what="groups")
