@@ -380,8 +380,8 @@ PU_API int pu_decode_paged_heads(const void* q, int q_dtype,
  *     in whole pages (rounded down).  They are read through the table row of the
  *     group's first sequence that holds as many; the others' entries for them must
  *     name the same pages.  A sequence that holds fewer attends them by itself.  A
- *     group in which none holds as many shares nothing, nor does a call where that
- *     would save little (a thousand tiles of 128 tokens of one K/V head), or whose
+ *     group in which too few hold as many shares nothing, nor does a call that saves
+ *     little (about 2048 tiles of 128 tokens of one K/V head), or whose
  *     sm_scale * k_scale is not a positive, finite, normal number.
  * q and pools of one 16-bit type, D 64 or 128, or e4m3 pools with D = 128; any
  * H / H_kv; groups <= 64; B <= 8192; H <= 65535; H_kv * D <= 2^21 - 32.

@@ -47,10 +47,15 @@ constexpr int BT = 128;                  // tokens of a tile
 constexpr int kRows = 256;               // rows of an item
 constexpr int kMaxGroups = 64;
 constexpr int kItemCost = 2;             // what starting and ending an item costs, in tiles
-// A pass over shared tokens and its join cost about 16 us before their first tile; the tiles that the
-// sequences would read by themselves instead are spread over all CTAs and come from L2 (four sequences of 8
-// K/V heads with 1024 shared tokens, 256 tiles: 28 us shared, 20 us not).  Below this many nothing is shared.
-constexpr int kWorth = 1024;
+// Whether sharing pays.  A pass over shared tokens and its join cost 8 to 12 us before their first tile, and each
+// tile of 128 rows as much as 2 tiles that a sequence reads by itself (64 KB of keys and values, spread over all CTAs, from
+// L2 where they fit), or 4 of 32 KB (heads of 64, e4m3).  A group for which that is more than its sequences' own
+// tiles shares nothing, nor does a call that saves fewer than kWorth tiles.  Measured, shared against not, tiles saved:
+//   64 KB: 4 sequences behind 8192 tokens 36.3 us, 30.7 (1024), 24 behind 1024 33.2, 31.4 (1408), 32: 34.6, 35.2 (1920),
+//     40: 36.4, 39.0 (2304), 64: 44.2, 53.2 (3840), 256 behind 128 72.5, 78.3 (1920), 2 behind 40960 65.6, 62.0 (0)
+//   32 KB: e4m3, 16 behind 2048 34.3, 31.4 (1536), 20: 36.5, 34.4 (2048), 24: 37.0, 37.8 (2560), 4 behind 16384 48.5, 37.4 (0);
+//     heads of 64, 80 behind 2048 33.0, 31.5 (1920), 96: 32.1, 34.3 (2304)
+constexpr int kWorth = 2048;
 constexpr int kBadRing = 8;
 
 template <typename T, typename KVT, int D>
@@ -109,6 +114,7 @@ struct Params {
   float* slabs;                // records
   int B, H, H_kv, group, slices, groups;
   int max_pages, num_pages, page_shift, box;
+  int pass_cost;               // a tile of 128 rows of the prefix pass, in tiles that a sequence reads by itself
   float scale_log2;
 };
 
@@ -218,6 +224,7 @@ __device__ __forceinline__ void make_groups(const Params& p, Group* gs, int tid,
       if (i <= p.groups) {
         gs[i].start = s;
         gs[i].rep = 0x7fffffff;
+        gs[i].unit = 0;                  // for now: sequences that hold the shared tokens
         gs[i].tokens = i < p.groups ? max(0, min(p.shared_lens[i], p.max_pages << p.page_shift)) >> p.page_shift << p.page_shift : 0;
       }
     }
@@ -225,16 +232,20 @@ __device__ __forceinline__ void make_groups(const Params& p, Group* gs, int tid,
   __syncthreads();
   for (int b = tid; b < p.B; b += threads) {
     const int g = group_of(gs, p.groups, b);
-    if (g >= 0 && p.lens[b] >= gs[g].tokens) atomicMin(&gs[g].rep, b);
+    if (g >= 0 && p.lens[b] >= gs[g].tokens) {
+      atomicMin(&gs[g].rep, b);
+      atomicAdd(&gs[g].unit, 1);
+    }
   }
   __syncthreads();
   if (tid < 32) {
     // tiles that sharing saves; one sequence alone shares with nobody
     long long saved = 0;
     for (int i = lane; i < p.groups; i += 32) {
-      const int n = gs[i + 1].start - gs[i].start;
-      if (gs[i].rep == 0x7fffffff || n < 2) gs[i].tokens = 0;
-      saved += (long long)n * p.slices * tiles_of(gs[i]);
+      const int rows = (gs[i + 1].start - gs[i].start) * p.group, holders = gs[i].unit;
+      const long long less = (long long)holders * p.slices - (long long)((rows + kRows / 2 - 1) / (kRows / 2)) * p.pass_cost;
+      if (holders < 2 || less <= 0) gs[i].tokens = 0;
+      saved += less * tiles_of(gs[i]);
     }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) saved += __shfl_xor_sync(0xffffffffu, saved, off);
@@ -945,6 +956,7 @@ int pu_decode_paged_shared(const void* q, int q_dtype, const void* k_pool, const
   prm.num_pages = (int)num_pages;
   prm.page_shift = shift;
   prm.box = (int)std::min<long long>(page_size, shared::BT);
+  prm.pass_cost = D == 128 && !f8 ? 2 : 4;
   prm.scale_log2 = sm_scale * k_scale * kLog2e;
 
   ptc::Params own{};

@@ -109,8 +109,8 @@ def paged_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     [n + 1]; without it one group is the whole batch), have the same first
     shared_lens[i] tokens, which are then read once for the group, through the
     table row of one of its sequences.  Only whole pages are shared.  A sequence
-    that holds fewer tokens than that attends them by itself; a group in which
-    none holds as many shares nothing, nor does a call where that would save little or
+    that holds fewer tokens than that attends them by itself; a group in which too few
+    hold as many shares nothing, nor does a call where that would save little or
     whose scale is not positive.
     The result is that of the call without
     it, up to the order of sums, and where q and the pools have different 16-bit

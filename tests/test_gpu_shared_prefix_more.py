@@ -7,18 +7,28 @@ from __future__ import annotations
 
 import math
 
+import numpy as np
 import pytest
 import torch
-from test_gpu_paged_gqa import BF, FP8
-from test_gpu_shared_prefix import KINDS, batch, check, enough, ints, make, mods  # noqa: F401  (a fixture)
+from test_gpu_paged_gqa import BF, FP8, HF
+from test_gpu_shared_prefix import KINDS, batch, check, ints, make, mods  # noqa: F401  (a fixture)
 
 pytestmark = pytest.mark.gpu
+
+
+def enough(tokens, H, H_kv, D, kvdt, short=0):
+    """Sequences from which on a prefix of `tokens` tokens is shared: 2048 tiles saved, where a pass
+    of 128 rows, those of `short` sequences that do not hold it among them, costs as much as 2 of a
+    sequence's own tiles of 64 KB, or 4 of 32."""
+    G, cost = H // H_kv, 2 if D == 128 and kvdt != FP8 else 4
+    saved = lambda n: (n * -(-G // 16) - -(-(n + short) * G // 128) * cost) * -(-tokens // 128) * H_kv      # noqa: E731
+    return next(n for n in range(2, 10000) if saved(n) >= 2048)
 
 
 # --------------------------------------------------------------------------
 # short runs
 # --------------------------------------------------------------------------
-@pytest.mark.parametrize("tokens,each", [(256, 3), (128, 5), (256, 15), (384, 3)])
+@pytest.mark.parametrize("tokens,each", [(256, 6), (128, 8), (256, 15), (384, 6)])
 def test_short_runs_of_scaled_queries(mods, tokens, each):
     """Many prefixes of one to three tiles with no more than 128 rows, e4m3 pools and bf16 queries
     of very different magnitudes: a CTA takes several of them one after the other, and each
@@ -46,7 +56,7 @@ def test_any_scale(mods, H, H_kv, D, qdt, kvdt, sm_scale):
     has masked tokens, whose weight is nothing whatever the scale."""
     _lib, dec, paged = mods
     page, tokens = 16, 144
-    n = enough(tokens, H, H_kv)
+    n = enough(tokens, H, H_kv, D, kvdt)
     table, P, lens, shared, _ = batch([(tokens, ([0, 1, 90] + [9] * n)[:n])], page, 7)
     q, k, v = make(P, n, H, H_kv, D, page, qdt, kvdt, 3)
     o, lse = paged.paged_decode(q, k, v, table, ints(lens), shared_lens=shared, sm_scale=sm_scale, return_lse=True)
@@ -65,8 +75,8 @@ def test_any_scale(mods, H, H_kv, D, qdt, kvdt, sm_scale):
 def test_scales_whose_product_vanishes(mods):
     """sm_scale and k_scale are positive, their product is not."""
     _lib, dec, paged = mods
-    table, P, lens, shared, _ = batch([(144, [9] * 140)], 16, 7)
-    q, k, v = make(P, 140, 12, 4, 128, 16, BF, FP8, 3)
+    table, P, lens, shared, _ = batch([(144, [9] * 400)], 16, 7)
+    q, k, v = make(P, 400, 12, 4, 128, 16, BF, FP8, 3)
     o, lse = paged.paged_decode(q, k, v, table, ints(lens), shared_lens=shared, sm_scale=1e-30, k_scale=1e-30, return_lse=True)
     assert _lib.device_status() == (0, 0)
     check(o, lse, q, k, v, table, lens, scale=0.0, what="product")
@@ -79,25 +89,31 @@ def test_scales_whose_product_vanishes(mods):
 @pytest.mark.parametrize("page,tokens", [(16, 144), (64, 960), (256, 2048)])
 def test_others_rows_are_not_read(mods, H, H_kv, D, qdt, kvdt, page, tokens):
     """Where sequences share, only one row names the shared pages: the others' entries may be anything.
-    With one sequence fewer nothing is shared, and the missing entries are reported."""
+    With one sequence fewer nothing is shared, and the missing entries are reported; so with one
+    more that is too short to share."""
     _lib, dec, paged = mods
-    n = enough(tokens, H, H_kv)
-    own = ([0, 1, 90, 130] + [9] * n)[:n]
+    n = enough(tokens, H, H_kv, D, kvdt)
+    own = ([1, 0, 90, 130] + [9] * n)[:n]
     table, P, lens, shared, _ = batch([(tokens, own)], page, 7)
     q, k, v = make(P, n, H, H_kv, D, page, qdt, kvdt, 3)
-    lens[0] = tokens - 1                 # the first sequence is too short to be the one that is read
     bare = table.clone()
-    bare[2:, :tokens // page] = -1
+    bare[1:, :tokens // page] = -1
     o, lse = paged.paged_decode(q, k, v, bare, ints(lens), shared_lens=shared, return_lse=True)
     assert _lib.device_status() == (0, 0)
     check(o, lse, q, k, v, table, lens, what="one row")
     paged.paged_decode(q[:-1], k, v, bare[:-1].contiguous(), ints(lens[:-1]), shared_lens=shared)
     assert _lib.device_status() == (_lib.PU_ERR_INVALID_ARGUMENT, 302)
+    lens[2] = tokens - 1
+    o, lse = paged.paged_decode(q, k, v, table, ints(lens), shared_lens=shared, return_lse=True)
+    check(o, lse, q, k, v, table, lens, what="one too short")
+    assert _lib.device_status() == (0, 0)
+    paged.paged_decode(q, k, v, bare, ints(lens), shared_lens=shared)
+    assert _lib.device_status() == (_lib.PU_ERR_INVALID_ARGUMENT, 302)
 
 
 def test_others_rows_of_several_groups_are_not_read(mods):
     _lib, dec, paged = mods
-    page, groups = 32, [(960, [5, 0, 70] * 20), (320, [1] * 40), (64, []), (512, [33] * 50)]
+    page, groups = 32, [(960, [5, 0, 70] * 40), (320, [1] * 80), (64, []), (512, [33] * 90)]
     table, P, lens, shared, starts = batch(groups, page, 3)
     q, k, v = make(P, len(lens), 8, 2, 128, page, BF, BF, 5)
     bare, at = table.clone(), starts.tolist()
@@ -106,3 +122,105 @@ def test_others_rows_of_several_groups_are_not_read(mods):
     o, lse = paged.paged_decode(q, k, v, bare, ints(lens), shared_lens=shared, shared_groups=starts, return_lse=True)
     assert _lib.device_status() == (0, 0)
     check(o, lse, q, k, v, table, lens, what="groups")
+
+
+# --------------------------------------------------------------------------
+# enough sequences that the device shares
+# --------------------------------------------------------------------------
+@pytest.mark.parametrize("H,H_kv,D,qdt,kvdt", KINDS)
+@pytest.mark.parametrize("page,tokens", [(16, 16), (16, 144), (64, 128), (64, 960), (256, 2048)])
+def test_just_enough(mods, H, H_kv, D, qdt, kvdt, page, tokens):
+    """As few sequences as share: one page, tiles and a rest, several items of 256 rows; the sequences'
+    own tokens from none on, some shorter than the prefix, the first among them."""
+    _lib, dec, paged = mods
+    r = np.random.RandomState(page + tokens)
+    ks, vs = (0.05, 0.03) if kvdt == FP8 else (1.0, 1.0)
+    n = enough(tokens, H, H_kv, D, kvdt, short=3) + 3
+    own = [0, 1, page, 129] + r.randint(0, 40, n).tolist()
+    table, P, lens, shared, _ = batch([(tokens, own[:n])], page, 7)
+    lens[0], lens[n // 2], lens[n - 1] = 0, tokens - 1, tokens // 2
+    q, k, v = make(P, n, H, H_kv, D, page, qdt, kvdt, 3)
+    bare = table.clone()                 # the second sequence's row is the one that is read
+    bare[2:, :tokens // page] = torch.where(ints(lens[2:] >= tokens).bool().unsqueeze(1), -1, table[2:, :tokens // page])
+    o, lse = paged.paged_decode(q, k, v, bare, ints(lens), shared_lens=shared, k_scale=ks, v_scale=vs, return_lse=True)
+    assert _lib.device_status() == (0, 0)
+    check(o, lse, q, k, v, table, lens, ks, vs, what=f"{tokens} shared by {n}")
+    assert torch.equal(o, paged.paged_decode(q, k, v, table, ints(lens), shared_lens=shared, k_scale=ks, v_scale=vs))
+
+
+@pytest.mark.parametrize("kvdt", [BF, FP8])
+def test_lengths_that_do_not_fit_a_large_batch(mods, kvdt):
+    """Shared lengths inside a page, longer than the table or negative, sequences shorter than the
+    prefix, starts in disorder, where what is left is still shared."""
+    _lib, dec, paged = mods
+    page, B = 64, 420
+    table, P, lens, shared, _ = batch([(640, [10, 0, 100, 33, 5] + [7] * (B - 5))], page, 3)
+    assert B - 20 >= enough(640, 8, 2, 128, kvdt, short=20)
+    q, k, v = make(P, B, 8, 2, 128, page, BF, kvdt, 5)
+    bare = table.clone()
+    bare[7:, :10] = -1                   # the first seven hold it in what follows, or do not
+    for s in (640, 641, 703):
+        o, lse = paged.paged_decode(q, k, v, bare, ints(lens), shared_lens=ints([s]), return_lse=True)
+        assert _lib.device_status() == (0, 0)
+        check(o, lse, q, k, v, table, lens, what=f"shared {s}")
+    for s in (2 ** 31 - 1, 639, 65, 0, -5):
+        o, lse = paged.paged_decode(q, k, v, table, ints(lens), shared_lens=ints([s]), return_lse=True)
+        check(o, lse, q, k, v, table, lens, what=f"shared {s}")
+    for short in ([0, 640, 740, 673, 645], [0, 0, 740, 1, 645], [300, 639, 0, 128, 640], [0, 0, 0, 0, 0], [5, 639, 70, 64, 1]):
+        short = np.array(short + [647] * (B - 5))
+        o, lse = paged.paged_decode(q, k, v, bare, ints(short), shared_lens=shared, return_lse=True)
+        assert _lib.device_status() == (0, 0)
+        check(o, lse, q, k, v, table, short, what=f"lengths {short}")
+    for starts in ([0, B, 3], [-7, 2, 900], [4, 9, B], [5, 5, 5], [1, 410, B + 1]):
+        o, lse = paged.paged_decode(q, k, v, table, ints(lens), shared_lens=ints([640, 640]), shared_groups=ints(starts), return_lse=True)
+        check(o, lse, q, k, v, table, lens, what=f"starts {starts}")
+    assert _lib.device_status() == (0, 0)
+
+
+@pytest.mark.parametrize("D,page,kvdt", [(128, 16, BF), (64, 32, HF), (128, 64, FP8), (128, 256, BF)])
+def test_stale_and_missing_pages_of_a_large_batch(mods, D, page, kvdt):
+    """NaN in pages of nobody never counts; shared entries outside the pool are reported and their tokens
+    left out for all, in every tile of the prefix and in its last, partial one."""
+    _lib, dec, paged = mods
+    pages = 4 if page == 256 else 384 // page + 3
+    tokens = pages * page
+    table, P, lens, shared, _ = batch([(tokens, [5, 0, 100] + [7] * 500)], page, 3, spare=9)
+    assert len(lens) >= enough(tokens, 8, 2, D, kvdt)
+    q, k, v = make(P, len(lens), 8, 2, D, page, HF if kvdt == HF else BF, kvdt, 5)
+    used = torch.zeros(P, dtype=torch.bool, device="cuda")
+    used[table[table >= 0].long()] = True
+    nan = torch.full((1,), math.nan, device="cuda").to(kvdt)
+    for pool in (k, v):
+        raw = pool.view(torch.uint8) if kvdt == FP8 else pool
+        raw[~used] = nan.view(torch.uint8) if kvdt == FP8 else nan
+    bare = table.clone()
+    bare[1:, :pages] = -1
+    o, lse = paged.paged_decode(q, k, v, bare, ints(lens), shared_lens=shared, return_lse=True)
+    assert _lib.device_status() == (0, 0)
+    check(o, lse, q, k, v, table, lens, what="stale")
+    for gone in ([1, pages - 1], list(range(pages))):
+        if gone == list(range(pages)):
+            lens = np.maximum(lens, tokens + 1)          # something is left of each
+        bare[0] = table[0]
+        bare[0, gone] = torch.tensor([P, -1] * len(gone), dtype=torch.int32, device="cuda")[:len(gone)]
+        o, lse = paged.paged_decode(q, k, v, bare, ints(lens), shared_lens=shared, return_lse=True)
+        assert _lib.device_status() == (_lib.PU_ERR_INVALID_ARGUMENT, 302)
+        rest = [i for i in range(table.shape[1]) if i not in gone]
+        check(o, lse, q, k, v, table[:, rest].contiguous(), lens - len(gone) * page, what="missing")
+
+
+def test_large_scores_of_a_large_batch(mods):
+    """Scores of far more than exp's range: the maxima move and nothing overflows."""
+    _lib, dec, paged = mods
+    page, B = 32, 120
+    table, P, lens, shared, _ = batch([(2048, [40] * B)], page, 3)
+    for kvdt, qdt in ((BF, BF), (HF, HF), (FP8, BF), (FP8, HF)):
+        assert B >= enough(2048, 8, 2, 128, kvdt)
+        q, k, v = make(P, B, 8, 2, 128, page, qdt, kvdt, 5)
+        q = (q.float() * torch.linspace(0.01, 40, B, device="cuda").view(-1, 1, 1, 1)).to(qdt)
+        k[table[0, :64].long()] = (k[table[0, :64].long()].float() * torch.linspace(0.1, 2, 64, device="cuda").view(-1, 1, 1, 1)).to(kvdt)
+        bare = table.clone()
+        bare[1:, :64] = -1
+        o, lse = paged.paged_decode(q, k, v, bare, ints(lens), shared_lens=shared, return_lse=True)
+        assert _lib.device_status() == (0, 0)
+        check(o, lse, q, k, v, table, lens, what=f"{kvdt}")
