@@ -973,11 +973,13 @@ extern "C" int pu_page_bounds(const void* k_pool, int kv_dtype, const int32_t* s
   p.page_shift = shift;
   p.T = num_tokens;
   // Small batches are spread out: eight single tokens and one head a CTA are a warp's row each.
-  // Larger ones share the reads of the slots over as many heads as leave three CTAs an SM, all of them resident.
+  // Larger ones share the reads of the slots over as many heads as leave three CTAs an SM, which start at once (10000
+  // tokens, 2 heads: 3.5 us, with one CTA more for each chunk 5.7; 14100 e4m3 tokens, 4 heads: 5.0, 8.5).  From
+  // three chunks an SM on, 14208 tokens, the rest wait for a place: 14800 tokens 6.8 us, 64000 18.8.
   const long long room = 3ll * pu::sm_count();
   p.chunk = (num_tokens + 7) / 8 * H_kv <= room ? 8 : 32;
-  p.heads = (int)std::min<long long>(H_kv, std::max<long long>(1, (num_tokens + p.chunk - 1) / p.chunk * H_kv / room));
-  p.heads = (int)((H_kv + (H_kv + p.heads - 1) / p.heads - 1) / ((H_kv + p.heads - 1) / p.heads));   // as evenly
+  const long long chunks = (num_tokens + p.chunk - 1) / p.chunk, parts = std::min<long long>(H_kv, std::max<long long>(1, room / chunks));
+  p.heads = (int)((H_kv + parts - 1) / parts);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (kv_dtype == PU_DTYPE_FP8_E4M3)
     return D == 128 ? launch_bounds<__nv_fp8_e4m3, 128>(p, st) : launch_bounds<__nv_fp8_e4m3, 64>(p, st);

@@ -66,3 +66,19 @@ def test_equal_lists_are_the_table(mods, H, H_kv, D, qdt, kvdt):
     b = paged.paged_decode(q, k, v, table.unsqueeze(1).repeat(1, H_kv, 1), n.unsqueeze(1).repeat(1, H_kv), k_scale=0.5, v_scale=2.0, return_lse=True)
     assert _lib.device_status() == (0, 0)
     assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("T,H_kv,D,dt", [(700, 4, 128, FP8), (4000, 4, 128, FP8), (3000, 8, 128, BF), (10000, 2, 64, HF), (14100, 3, 64, FP8), (14300, 5, 128, BF), (9000, 7, 64, BF)])
+def test_bounds_of_prompts(mods, T, H_kv, D, dt):
+    """Packed prompts of every cut of rows and heads over the CTAs, pages begun before among them."""
+    from test_gpu_page_select import bounds_after, packed
+    _lib, dec, paged = mods
+    r = np.random.RandomState(T)
+    new = r.multinomial(T - 40, [1 / 20] * 20)
+    slots, P = packed(r.randint(0, 90, 20), new, 32, T, pad=40)
+    k = _gen((P, H_kv, 32, D), 1).to(dt)
+    bounds = _gen((P, H_kv, 2, D), 2).to(HF if dt == FP8 else dt)
+    want = bounds_after(k, slots, bounds)
+    paged.page_bounds(k, ints(slots), bounds)
+    assert torch.equal(bounds.double(), want)
+    assert _lib.device_status() == (0, 0)
