@@ -224,3 +224,32 @@ def test_large_scores_of_a_large_batch(mods):
         o, lse = paged.paged_decode(q, k, v, bare, ints(lens), shared_lens=shared, return_lse=True)
         assert _lib.device_status() == (0, 0)
         check(o, lse, q, k, v, table, lens, what=f"{kvdt}")
+
+
+@pytest.mark.parametrize("H,H_kv,D,qdt,kvdt", [(8, 2, 128, BF, BF), (40, 2, 64, BF, BF), (12, 4, 128, BF, FP8), (64, 1, 128, HF, HF)])
+def test_too_little_for_any_lengths(mods, H, H_kv, D, qdt, kvdt):
+    """Tables in which too little can be shared: the decode without a prefix, bit for bit; and one sequence
+    alone however long."""
+    _lib, dec, paged = mods
+    for tokens, own, page in ((512, [30, 0, 300, 7], 64), (40000, [9], 64)):
+        table, P, lens, shared, _ = batch([(tokens, own)], page, 5)
+        q, k, v = make(P, len(lens), H, H_kv, D, page, qdt, kvdt, 3)
+        a = paged.paged_decode(q, k, v, table, ints(lens), shared_lens=shared, return_lse=True)
+        b = paged.paged_decode(q, k, v, table, ints(lens), return_lse=True)
+        assert _lib.device_status() == (0, 0)
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_the_bound_on_what_can_be_saved(mods):
+    """As narrow a table as shares, and as few sequences: what the host may skip is never shared."""
+    _lib, dec, paged = mods
+    for kvdt, H, H_kv, page, tokens in ((BF, 8, 2, 128, 1024), (FP8, 8, 2, 128, 1024), (BF, 64, 1, 128, 4096)):
+        n = enough(tokens, H, H_kv, 128, kvdt)
+        table, P, lens, shared, _ = batch([(tokens, [0] * n)], page, 5)
+        table = table[:, :tokens // page].contiguous()
+        q, k, v = make(P, n, H, H_kv, 128, page, BF, kvdt, 3)
+        bare = table.clone()
+        bare[1:] = -1
+        o, lse = paged.paged_decode(q, k, v, bare, ints(lens), shared_lens=shared, return_lse=True)
+        assert _lib.device_status() == (0, 0)
+        check(o, lse, q, k, v, table, lens, what="narrow")
