@@ -386,7 +386,9 @@ PU_API int pu_decode_paged_heads(const void* q, int q_dtype,
  * q and pools of one 16-bit type, D 64 or 128, or e4m3 pools with D = 128; any
  * H / H_kv; groups <= 64; B <= 8192; H <= 65535; H_kv * D <= 2^21 - 32.
  *   workspace: pu_decode_paged_shared_workspace_size() bytes, zeroed before its
- *   first use (left as pu_decode_paged_gqa needs it).
+ *   first use (left as pu_decode_paged_gqa needs it).  That is 1024 (D + 2) bytes for
+ *   two records of each SM and one of each 256 rows of a K/V head (39 MB and more at
+ *   D = 128), and 4 D bytes a query head.
  * The softmax weights of shared tokens are rounded once to the pools' 16-bit type,
  * to f16 with e4m3 pools (bf16 queries are f16 times a power of two then: exact
  * down to 2^-31 of a head's largest element).  A table entry of shared tokens

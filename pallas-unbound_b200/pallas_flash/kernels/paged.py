@@ -112,9 +112,13 @@ def paged_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     that holds fewer tokens than that attends them by itself; a group in which too few
     hold as many shares nothing, nor does a call where that would save little or
     whose scale is not positive.
-    The result is that of the call without
-    it, up to the order of sums, and where q and the pools have different 16-bit
-    types, or e4m3 pools heads of 64, it is that call."""
+    The result is that of the call without it, up to the order of sums and the rounding of the
+    softmax weights: those of shared tokens are rounded once to the pools' 16-bit type, to
+    f16 over fp8 pools (which keep three e4m3 parts without it), and so are all tokens' of 16-bit
+    pools, as in the grouped decode (with a query head to each K/V head the call
+    without it keeps them in fp32).  Where q and the pools have different 16-bit
+    types, or e4m3 pools heads of 64, it is that call.  Up to 8192 sequences; the scratch, kept for
+    the stream, is 39 MB at D = 128 and more for larger batches (pu_decode_paged_shared)."""
     _check_pool(k_pool, v_pool, page_table, kv_lens, _DT_KV)
     P, H_kv, page_size, D = k_pool.shape
     rows = page_table.shape
