@@ -676,7 +676,7 @@ class DevicePagedKVCache:
         at = torch.as_tensor(sequences, device=dev)
         if at.dtype == torch.bool:
             at = at.nonzero()
-        elif at.is_floating_point() or at.is_complex():
+        elif at.numel() and (at.is_floating_point() or at.is_complex()):
             raise ValueError("sequences must be whole numbers")
         at = at.to(torch.int64).reshape(-1).contiguous()
         if not at.is_cuda:

@@ -108,6 +108,7 @@ def test_share_of_what_cannot_be(mods):
     assert rows(cache)[3] == rows(cache)[5] == rows(cache)[0][:3]
     cache.share(0, torch.tensor([4], device="cuda"), 0)              # nothing
     cache.share(0, torch.tensor([], dtype=torch.int64, device="cuda"), 16)
+    cache.share(0, [], 16)
     cache.share(-6, torch.tensor([False, True, False, False, False, False], device="cuda"), 64)
     assert _lib.device_status() == (0, 0) and cache.kv_lens.tolist() == [70, 64, 3, 48, 0, 48]
     for bad in (lambda: cache.share(6, [1], 16), lambda: cache.share(-7, [1], 16), lambda: cache.share(0, [1.0], 16), lambda: cache.share(0, [1], 17),
