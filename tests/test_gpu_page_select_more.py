@@ -82,3 +82,27 @@ def test_bounds_of_prompts(mods, T, H_kv, D, dt):
     paged.page_bounds(k, ints(slots), bounds)
     assert torch.equal(bounds.double(), want)
     assert _lib.device_status() == (0, 0)
+
+
+@pytest.mark.parametrize("kvdt,D,H_kv,page", [(BF, 128, 2, 4096), (FP8, 64, 1, 4096), (HF, 64, 3, 1024)])
+def test_large_pages(mods, kvdt, D, H_kv, page):
+    """Bounds of runs far longer than a CTA's rows, choice and decode of the largest pages."""
+    from test_gpu_page_select import bounds_after, check_lists, packed
+    _lib, dec, paged = mods
+    held, new = [0, page - 1, 5, page], [2 * page + 3, 2, page, 1]
+    slots, P = packed(held, new, page, 3, pad=3)
+    k, v = (_gen((P, H_kv, page, D), 1 + i).to(kvdt) for i in range(2))
+    bounds = _gen((P, H_kv, 2, D), 50).to(HF if kvdt == FP8 else kvdt)
+    want = bounds_after(k, slots, bounds)
+    paged.page_bounds(k, ints(slots), bounds)
+    assert torch.equal(bounds.double(), want)
+    lens = (np.array(held) + new).tolist()
+    table, _ = pages_of(lens, page, 3)
+    bounds, q = spread(P, H_kv, D, BF, 7), _gen((4, 4 * H_kv, 1, D), 9, HF if kvdt == HF else BF)
+    strided = q.transpose(0, 1).contiguous().transpose(0, 1)
+    chosen = paged.select_pages(strided, bounds, table, ints(lens), 2, page_size=page)
+    want = choose(q, bounds, table, lens, page, 2, 1, 1)
+    assert torch.equal(chosen.pages, want[0]) and torch.equal(chosen.lens, want[1])
+    o, lse = paged.paged_decode(q, k, v, chosen.pages, chosen.lens, return_lse=True)
+    check_lists(o, lse, q, k, v, chosen.pages, chosen.lens.cpu().numpy(), what="large pages")
+    assert _lib.device_status() == (0, 0)

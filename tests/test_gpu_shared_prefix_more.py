@@ -253,3 +253,37 @@ def test_the_bound_on_what_can_be_saved(mods):
         o, lse = paged.paged_decode(q, k, v, bare, ints(lens), shared_lens=shared, return_lse=True)
         assert _lib.device_status() == (0, 0)
         check(o, lse, q, k, v, table, lens, what="narrow")
+
+
+@pytest.mark.parametrize("H,H_kv,D,page,qdt,kvdt,tokens,n", [
+    # more query heads of a K/V head than an item has rows; as many as that; the largest pages; one head
+    (300, 1, 128, 64, BF, BF, 1024, 21), (300, 1, 128, 32, BF, FP8, 2048, 30), (512, 2, 64, 16, HF, HF, 1040, 16), (8, 2, 128, 4096, BF, BF, 8192, 30),
+    (8, 4, 128, 4096, HF, FP8, 4096, 40), (2, 2, 64, 1024, HF, HF, 4096, 200), (1, 1, 128, 128, BF, BF, 2048, 140)])
+def test_heads_and_pages(mods, H, H_kv, D, page, qdt, kvdt, tokens, n):
+    _lib, dec, paged = mods
+    ks, vs = (0.05, 0.03) if kvdt == FP8 else (1.0, 1.0)
+    assert n >= enough(tokens, H, H_kv, D, kvdt)
+    table, P, lens, shared, _ = batch([(tokens, [(37 * i) % 200 for i in range(n)])], page, n)
+    q, k, v = make(P, n, H, H_kv, D, page, qdt, kvdt, 3, ks, vs)
+    bare = table.clone()
+    bare[1:, :tokens // page] = -1
+    o, lse = paged.paged_decode(q, k, v, bare, ints(lens), shared_lens=shared, k_scale=ks, v_scale=vs, return_lse=True)
+    assert _lib.device_status() == (0, 0)
+    check(o, lse, q, k, v, table, lens, ks, vs, what="heads and pages", sample=12)
+
+
+def test_the_largest_batch(mods):
+    """8192 sequences in 64 groups, queries that are a view of other strides."""
+    _lib, dec, paged = mods
+    page, B = 16, 8192
+    table, P, lens, shared, starts = batch([(16 * (1 + i % 20), [(5 * i + j) % 40 for j in range(128)]) for i in range(64)], page, 1)
+    q, k, v = make(P, B, 4, 1, 128, page, BF, BF, 3)
+    bare, at = table.clone(), starts.tolist()
+    for i in range(64):
+        bare[at[i] + 1:at[i + 1], :1 + i % 20] = -1
+    strided = q.transpose(0, 1).contiguous().transpose(0, 1)
+    o, lse = paged.paged_decode(strided, k, v, bare, ints(lens), shared_lens=shared, shared_groups=starts, return_lse=True)
+    assert _lib.device_status() == (0, 0)
+    check(o, lse, q, k, v, table, lens, what="largest batch", sample=100)
+    odd = torch.empty(q.numel() + 1, dtype=BF, device="cuda")[1:].view(q.shape).copy_(q)     # 2 bytes off
+    assert torch.equal(o, paged.paged_decode(odd, k, v, bare, ints(lens), shared_lens=shared, shared_groups=starts))
