@@ -409,7 +409,7 @@ __global__ void __launch_bounds__(kThreads) share_kernel(const ShareParams p) {
     do {
       more = false;
       for (int b = tid; b < p.B; b += kThreads) {
-        const int held = p.shared[b], from = p.owner[b];
+        const int held = min(p.shared[b], p.lens[b]), from = p.owner[b];      // as a plan counts it
         if (held <= 0 || (unsigned)from >= (unsigned)p.B || (held == p.tokens && (s_mark[b] & 3) == 1)) continue;
         more |= s_mark[from] != 0 && !(atomicOr(&s_mark[from], 2) & 2);
       }

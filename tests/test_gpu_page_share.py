@@ -143,6 +143,21 @@ def test_unshare_of_what_is_not_shared(mods):
     assert cache.kv_lens.tolist() == [100, 0, 40, 0, 32]
 
 
+def test_a_sequence_that_was_emptied_by_hand_holds_nothing(mods):
+    _lib, paged = mods
+    cache = make(paged, 4)
+    plan(cache, [50, 0, 0, 0])
+    cache.share(0, [1], 32)
+    plan(cache, [0, 20, 0, 0])
+    cache.share(1, [2], 48)
+    cache.kv_lens[2] = 0
+    cache.unshare([1], 32)
+    assert _lib.device_status() == (0, 0) and cache.kv_lens.tolist() == [50, 20, 0, 0]
+    cache.share(0, [2], 16)              # and may begin anew
+    plan(cache, [0] * 4, release=[1])
+    assert _lib.device_status() == (0, 0) and cache.kv_lens.tolist() == [50, 0, 16, 0]
+
+
 def test_chains(mods):
     """Pages shared on: a release waits for all that hold them, through others too."""
     _lib, paged = mods
